@@ -483,6 +483,64 @@ tq_status tq_attention_launch(tq_dtype dtype,
                               void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
+/* Attention with a window, sinks and shared key heads; a paged cache in 8 bits                  */
+/* No counterpart in the reference, which has no cache and no attention kernel.                  */
+
+/* out[b,h,i,:] = sum_j softmax_j(scale * q[b,h,i,:] . k[b,h',j,:]) v[b,h',j,:] with h' = h / (heads / kv_heads), over the keys
+ * that query i sees: it stands at position p = k_tokens - q_tokens + i (the last query at the last key) and sees j <= p with
+ * j > p - window or j < sinks. window 0: no window (every j <= p). A query before the first key (p < 0) sees nothing and
+ * its result is zeros; what lies in keys that a query does not see, NaN included, does not reach its result. Types, head_dim,
+ * strides and scale as for tq_attention_launch; heads is a multiple of kv_heads; k_tokens may be 0. `workspace` must hold
+ * tq_window_attention_workspace_bytes bytes that no other launch in flight uses; null where that is 0. */
+tq_status tq_window_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim,
+                                              int64_t window, int64_t sinks, int32_t device, size_t* bytes);
+tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, const void* k, const void* v, void* out, int64_t batch, int64_t heads,
+                                     int64_t kv_heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim, const int64_t* q_strides,
+                                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides, double scale, int64_t window,
+                                     int64_t sinks, void* workspace, size_t workspace_bytes, int32_t device, void* stream);
+
+/* A paged cache: packed [pages, kv_heads, page_tokens, head_dim] codes (e4m3: 4 exponent and 3 fraction bits, no infinities)
+ * for the keys and as many for the values, and a packed [pages, kv_heads] f32 scale for each; an element is code times scale.
+ * page_tokens is a power of two from 16 to 1024, head_dim a multiple of 16 up to 128. `table` is int32 [batch, blocks] with
+ * `table_stride` elements between rows: the page that holds tokens page_tokens * n to page_tokens * (n + 1) - 1 of sequence b is
+ * table[b][n]. Entries behind a sequence's end are not read. A page outside the pool, or a position behind the table's end, is left out
+ * and reported through tq_status_poll (0x50414745 "PAGE", 0x4c454e47 "LENG").
+ *
+ * tq_cache_attention_launch: as tq_window_attention_launch over the first lengths[b] (int32, device memory) tokens of each sequence:
+ * query i of q_tokens stands at position lengths[b] - q_tokens + i. bf16 or f16 q and out; k_tokens is lengths[b]; 0 is a
+ * sequence without keys (zeros). */
+tq_status tq_cache_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens,
+                                             int64_t blocks, int64_t window, int64_t sinks, int32_t device, size_t* bytes);
+tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                                    const int32_t* table, const int32_t* lengths, void* out, int64_t batch, int64_t heads, int64_t kv_heads,
+                                    int64_t q_tokens, int64_t head_dim, int64_t pages, int64_t page_tokens, int64_t blocks, int64_t table_stride,
+                                    const int64_t* q_strides, const int64_t* out_strides, double scale, int64_t window, int64_t sinks, void* workspace,
+                                    size_t workspace_bytes, int32_t device, void* stream);
+
+/* Writes new tokens into the cache: token i < counts[b] of sequence b (k and v are [batch, kv_heads, tokens, head_dim], bf16 or f16,
+ * with element strides {batch, head, token}, multiples of 8, 16-byte aligned) goes to position starts[b] + i. `starts` and `counts` are
+ * int32 [batch] in device memory; counts null: all tokens; starts[b] < 0: the sequence is left as it is. The scale of each page and head
+ * that is written becomes the smallest power of two s, at least 2^-126, with every new |x| <= 448 s, and at least the scale that
+ * was there if the page held tokens before starts[b]; codes are x / s rounded to nearest even; where s has grown, the page's earlier
+ * tokens are encoded again. NaN and infinities become NaN and do not count for the scale. What lies behind the new tokens in a page stays. A page
+ * that is written must belong to one sequence alone. */
+tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const void* v, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                                const int32_t* table, const int32_t* starts, const int32_t* counts, int64_t batch, int64_t kv_heads, int64_t tokens,
+                                int64_t head_dim, int64_t pages, int64_t page_tokens, int64_t blocks, int64_t table_stride, const int64_t* k_strides,
+                                const int64_t* v_strides, int32_t device, void* stream);
+
+/* One tensor of a cache: `layers` times `pages` pages of `page_bytes` contiguous bytes, at base + layer * layer_stride + page * page_stride (bytes). */
+typedef struct tq_paged_tensor {
+  void* base;
+  int64_t layers, layer_stride, page_stride, page_bytes;
+} tq_paged_tensor;
+
+/* Copies page sources[i] to page targets[i], i < pairs, in every layer of every tensor. All arrays are HOST memory, read before the call returns. Pages are
+ * numbers below `pages`; the targets are distinct and none of them is a source (TQ_INVALID_ARGUMENT otherwise), so the order of the copies does not show. */
+tq_status tq_copy_pages_launch(const tq_paged_tensor* tensors, int32_t count, int64_t pages, const int64_t* sources, const int64_t* targets,
+                               int64_t pairs, int32_t device, void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
 /* Recipes: a compiled graph's launches, replayed by native code                                */
 /* Replaces the per-call Python interpreter loop of RecipeExecutor                              */
 /* (python/tessiq/executor.py:146-239), to which the reference attributes 42 % + 34 % of a call   */

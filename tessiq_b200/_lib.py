@@ -29,6 +29,10 @@ class tq_layout(ctypes.Structure):
     _fields_ = [("rank", c_int32), ("sizes", c_int64 * 8), ("strides", c_int64 * 8)]
 
 
+class tq_paged_tensor(ctypes.Structure):
+    _fields_ = [("base", c_void_p), ("layers", c_int64), ("layer_stride", c_int64), ("page_stride", c_int64), ("page_bytes", c_int64)]
+
+
 class Declined(TypeError):
     """TQ_UNSUPPORTED: well-formed arguments this library has no kernel for (the reference's
     `unsupported`, which its callers answer by running their own fallback)."""
@@ -93,6 +97,14 @@ SIGNATURES = {
     "tq_attention_launch": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
                                        POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_double, c_int32,
                                        c_int32, c_void_p]),
+    "tq_window_attention_workspace_bytes": (c_int32, [c_int64] * 8 + [c_int32, POINTER(c_size_t)]),
+    "tq_window_attention_launch": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int64] * 6 + [POINTER(c_int64)] * 4
+                                   + [c_double, c_int64, c_int64, c_void_p, c_size_t, c_int32, c_void_p]),
+    "tq_cache_attention_workspace_bytes": (c_int32, [c_int64] * 9 + [c_int32, POINTER(c_size_t)]),
+    "tq_cache_attention_launch": (c_int32, [c_int32] + [c_void_p] * 8 + [c_int64] * 9 + [POINTER(c_int64)] * 2
+                                  + [c_double, c_int64, c_int64, c_void_p, c_size_t, c_int32, c_void_p]),
+    "tq_cache_store_launch": (c_int32, [c_int32] + [c_void_p] * 9 + [c_int64] * 8 + [POINTER(c_int64)] * 2 + [c_int32, c_void_p]),
+    "tq_copy_pages_launch": (c_int32, [POINTER(tq_paged_tensor), c_int32, c_int64, POINTER(c_int64), POINTER(c_int64), c_int64, c_int32, c_void_p]),
     "tq_recipe_create": (c_int32, [POINTER(c_void_p)]),
     "tq_recipe_destroy": (c_int32, [c_void_p]),
     "tq_recipe_begin_recording": (c_int32, [c_void_p]),

@@ -62,6 +62,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "keyed.h"
 #include "tcgen05.h"
 
 namespace tq {
@@ -708,4 +709,67 @@ extern "C" tq_status tq_attention_launch(tq_dtype dtype, const void* q, const vo
     return form.keys == 128 ? with_width(std::integral_constant<int, 128>{}, few) : with_width(std::integral_constant<int, 64>{}, few);
   };
   return form.few ? with_keys(std::true_type{}) : with_keys(std::false_type{});
+}
+
+extern "C" tq_status tq_window_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t k_tokens,
+                                                         int64_t head_dim, int64_t window, int64_t sinks, int32_t device, size_t* bytes) {
+  TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
+  *bytes = 0;
+  return TQ_OK;
+}
+
+extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, const void* k, const void* v, void* out, int64_t batch, int64_t heads,
+                                                int64_t kv_heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim, const int64_t* q_strides,
+                                                const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides, double scale,
+                                                int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, int32_t device, void* stream) {
+  TQ_REQUIRE(q_strides != nullptr && k_strides != nullptr && v_strides != nullptr && out_strides != nullptr, TQ_INVALID_ARGUMENT,
+             "null strides");
+  if (tq::recording()) {
+    struct Kept { int64_t q[3], k[3], v[3], out[3]; } kept;
+    for (int i = 0; i < 3; ++i) {
+      kept.q[i] = q_strides[i];
+      kept.k[i] = k_strides[i];
+      kept.v[i] = v_strides[i];
+      kept.out[i] = out_strides[i];
+    }
+    return tq::record([=](int32_t d, void* s) {
+      return tq_window_attention_launch(dtype, q, k, v, out, batch, heads, kv_heads, q_tokens, k_tokens, head_dim, kept.q, kept.k, kept.v, kept.out, scale,
+                                        window, sinks, workspace, workspace_bytes, d, s);
+    });
+  }
+  TQ_REQUIRE(dtype == TQ_BF16 || dtype == TQ_F16, TQ_UNSUPPORTED, "window attention takes bf16 or f16 operands, not %s", tq::dtype_name(dtype));
+  TQ_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 0 && q_tokens >= 0 && k_tokens >= 0 && window >= 0 && sinks >= 0, TQ_INVALID_ARGUMENT,
+             "negative extent in batch=%lld heads=%lld kv_heads=%lld q_tokens=%lld k_tokens=%lld window=%lld sinks=%lld", (long long)batch,
+             (long long)heads, (long long)kv_heads, (long long)q_tokens, (long long)k_tokens, (long long)window, (long long)sinks);
+  TQ_REQUIRE(head_dim >= 8 && head_dim <= 2 * tq::kHeadDim && head_dim % 8 == 0, TQ_UNSUPPORTED,
+             "window attention has a kernel for heads of 8, 16, ... %d elements, not %lld", 2 * tq::kHeadDim, (long long)head_dim);
+  if (batch == 0 || heads == 0 || q_tokens == 0) return TQ_OK;
+  TQ_REQUIRE(kv_heads > 0 && heads % kv_heads == 0, TQ_INVALID_ARGUMENT, "%lld heads do not share %lld key heads evenly", (long long)heads, (long long)kv_heads);
+  TQ_REQUIRE(std::isfinite(scale) && scale > 0.0, TQ_UNSUPPORTED, "the score scale must be positive and finite, not %g", scale);
+  TQ_REQUIRE(q != nullptr && out != nullptr && (k_tokens == 0 || (k != nullptr && v != nullptr)), TQ_INVALID_ARGUMENT, "null operand or result");
+  TQ_REQUIRE(q_tokens < (1LL << 24) && k_tokens < (1LL << 30) && heads < 65536 && batch * heads < (1LL << 24) && heads / kv_heads * q_tokens < (1LL << 24),
+             TQ_UNSUPPORTED, "extents beyond the kernel's index range");
+  TQ_REQUIRE(tq::legal_strides(q, q_strides, head_dim, q_tokens, heads, batch) && tq::legal_strides(k, k_strides, head_dim, k_tokens, kv_heads, batch) &&
+                 tq::legal_strides(v, v_strides, head_dim, k_tokens, kv_heads, batch),
+             TQ_UNSUPPORTED, "Q, K and V must be 16-byte aligned with positive strides that are multiples of 8 elements (TMA's rules)");
+  TQ_REQUIRE(tq::keyed_query_fits(q, q_strides, out, out_strides, batch, heads, q_tokens), TQ_INVALID_ARGUMENT,
+             "misaligned result or negative result stride");
+  tq::DeviceScope device_scope(device);
+  if (tq_status s = device_scope.status()) return s;
+  tq::KeyedParams p = {};
+  p.status = tq::wait_status_for(device);
+  TQ_REQUIRE(p.status.abort != nullptr, TQ_RESOURCE_EXHAUSTED, "no device memory for the status word");
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  for (int i = 0; i < 3; ++i) {
+    p.q_strides[i] = q_strides[i];
+    p.k_strides[i] = k_strides[i];
+    p.v_strides[i] = v_strides[i];
+    p.out_strides[i] = out_strides[i];
+  }
+  p.k_tokens = static_cast<int>(k_tokens);
+  tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
+  return tq::keyed_attention(dtype, false, p, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,64 @@
+// What the entry points of window and cache attention (cache.cu, attention.cu) hand to the kernels of keyed.cu.
+#pragma once
+
+#include "common.h"
+
+namespace tq {
+
+// Codes of the status word for a cache whose table or lengths a kernel could not follow: it leaves out the keys that are not there.
+enum KeyedFault { kKeyedPage = 0x50414745, kKeyedLength = 0x4c454e47 };      // "PAGE", "LENG"
+
+struct KeyedParams {
+  const void *q, *k, *v;
+  void* out;
+  long long q_strides[3], k_strides[3], v_strides[3], out_strides[3];      // batch, head, token, in elements; k and v: dense keys only
+  const float *k_scales, *v_scales;                                        // paged keys: [pages, kv_heads]
+  const int32_t *table, *lengths;
+  long long table_stride;
+  int blocks, page_shift, pages;
+  int batch, heads, kv_heads, group, q_tokens, k_tokens, head_dim;
+  int window, sinks;
+  int row_tiles;
+  float scale_log2;
+  WaitStatus status;
+};
+
+// What queries and results have to be: read 16 bytes at a time, written through any strides.
+inline bool keyed_query_fits(const void* q, const int64_t* q_strides, const void* out, const int64_t* out_strides, int64_t batch, int64_t heads,
+                             int64_t q_tokens) {
+  const bool whole = (batch == 1 || q_strides[0] % 8 == 0) && (heads == 1 || q_strides[1] % 8 == 0) && (q_tokens == 1 || q_strides[2] % 8 == 0);
+  return whole && aligned_to(q, 16) && aligned_to(out, 2) && out_strides[0] >= 0 && out_strides[1] >= 0 && out_strides[2] >= 0;
+}
+
+// `window` 0: none. Positions stay below 2^30, so this one reaches them all and position - window does not wrap.
+constexpr int64_t kKeyedEverything = 1LL << 30;
+inline void keyed_extents(KeyedParams& p, int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, double scale,
+                          int64_t window, int64_t sinks) {
+  p.batch = static_cast<int>(batch);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = static_cast<int>(heads / kv_heads);
+  p.q_tokens = static_cast<int>(q_tokens);
+  p.head_dim = static_cast<int>(head_dim);
+  p.window = static_cast<int>(window == 0 || window > kKeyedEverything ? kKeyedEverything : window);
+  p.sinks = static_cast<int>(sinks > kKeyedEverything ? kKeyedEverything : sinks);
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+}
+
+// Few rows a key head against many keys; `p` is complete but for row_tiles.
+tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, cudaStream_t stream);
+
+#ifdef __CUDACC__
+// The first fault since the last poll is kept, with where it was.
+__device__ __forceinline__ void report(const WaitStatus& status, int code, int sequence, int what) {
+  int* words = status.sticky();
+  if (atomicCAS(words, 0, code) == 0) {
+    words[1] = static_cast<int>(blockIdx.x);
+    words[2] = static_cast<int>(threadIdx.x);
+    words[3] = sequence;
+    words[4] = what;
+  }
+}
+#endif
+
+}  // namespace tq

@@ -11,6 +11,7 @@ is where the reference would call its host fallback.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from functools import lru_cache
 from typing import Sequence
@@ -20,6 +21,7 @@ import torch
 from .kernel import (DTYPE_NAMES, REDUCE_OPS, AttentionKernel, FusedKernel, GemmKernel, LayerNormKernel, PackKernel, SoftmaxKernel, _device_of,
                      _pointer, _stream, broadcast_shape, check_status, classify_read, dtype_code, launch_reduce, launch_transposed,
                      prefers_transposed, reduce_workspace_bytes, transposed_workspace_bytes, workspace)
+from . import _lib
 from ._lib import LIBRARY_PATH, Declined, check, lib, load_launcher
 
 UNARY = {"abs", "neg", "relu", "sigmoid", "sqrt", "tanh", "exp", "expm1", "log", "log1p", "log2", "log10", "rsqrt",
@@ -557,6 +559,172 @@ def attention(q, k, v, scale=None, causal=False, token_major=True):
         _keep_plan(False, _CODES["attention"], operands, _ATTENTION, (out,),
                    (dtype, *extents[:5], *[n for strides in extents[5:] for n in strides], int(bool(causal))), (float(scale),), b"", None)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Serving: attention with a window, and the paged cache in 8 bits (tessiq_b200/cache.py hands out its pages)
+
+
+def _three_strides(t: torch.Tensor, what: str):
+    if t.dim() != 4:
+        raise Declined(f"{what} must be [batch, heads, tokens, width]")
+    if t.shape[-1] != 1 and t.stride(-1) != 1:
+        raise Declined(f"the last axis of {what} must be contiguous")
+    return (ctypes.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _attention_result(q: torch.Tensor, token_major: bool) -> torch.Tensor:
+    batch, heads, tokens, width = q.shape
+    if token_major:
+        return torch.empty([batch, tokens, heads, width], dtype=q.dtype, device=q.device).transpose(1, 2)
+    return torch.empty([batch, heads, tokens, width], dtype=q.dtype, device=q.device)
+
+
+def _window(window, sinks) -> tuple[int, int]:
+    """(window, sinks) as the C interface has them: 0 for no window."""
+    if window is not None and int(window) < 1:
+        raise ValueError(f"a window has at least one key, not {window}; None is no window")
+    if int(sinks) < 0:
+        raise ValueError(f"sinks are a number of first keys, not {sinks}")
+    return 0 if window is None else int(window), int(sinks)
+
+
+def _own_scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Scratch of one call: from torch's allocator, so that calls on different streams, and captured graphs, never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True):
+    """Causal attention with a sliding window and sinks: softmax(scale * q @ k.T) @ v over the keys that a query sees. q is
+    [batch, heads, q_tokens, width], k and v are [batch, kv_heads, k_tokens, width] with heads a multiple of kv_heads (head h
+    reads key head h // (heads // kv_heads)). Query i stands at position p = k_tokens - q_tokens + i, so one query against a cache is
+    its last token, and sees the keys j <= p with j > p - window or j < sinks; `window` None: all of j <= p. A query before the
+    first key gives zeros. What lies in keys a query does not see (NaN too) does not reach its result. Types, widths, strides and
+    `token_major` as for `attention`."""
+    operands = (q, k, v)
+    for t, what in zip(operands, ("the queries", "the keys", "the values")):
+        if t.dim() != 4:
+            raise Declined(f"{what} must be [batch, heads, tokens, width]")
+    if not q.dtype == k.dtype == v.dtype:
+        raise Declined("attention operands must share one element type")
+    batch, heads, q_tokens, width = q.shape
+    if tuple(k.shape) != tuple(v.shape) or k.shape[0] != batch or k.shape[3] != width or (k.shape[1] == 0) != (heads == 0) or (heads and heads % k.shape[1]):
+        raise ValueError(f"attention shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    window, sinks = _window(window, sinks)
+    scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
+    device = _device_of(operands)
+    out = _attention_result(q, token_major)
+    extents = (batch, heads, k.shape[1], q_tokens, k.shape[2], width)
+    nbytes = ctypes.c_size_t()
+    check(lib.tq_window_attention_workspace_bytes(*extents, window, sinks, device, ctypes.byref(nbytes)))
+    scratch = _own_scratch(nbytes.value, q.device)
+    check(lib.tq_window_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k), _pointer(v), _pointer(out), *extents, _three_strides(q, "the queries"),
+                                         _three_strides(k, "the keys"), _three_strides(v, "the values"), _three_strides(out, "the result"), scale, window,
+                                         sinks, _pointer(scratch), nbytes.value, device, _stream(None, device)))
+    return out
+
+
+def _cache_extents(k_pages, v_pages, k_scales, v_scales, table, batch: int, kv_heads: int, width: int) -> tuple[int, int, int, int]:
+    """(pages, page_tokens, blocks, table_stride) of a cache, checked."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"the cache's pages are float8_e4m3fn [pages, kv_heads, page_tokens, width], twice, not {k_pages.dtype} {tuple(k_pages.shape)} "
+                         f"and {v_pages.dtype} {tuple(v_pages.shape)}")
+    pages, heads, page_tokens, columns = k_pages.shape
+    if heads != kv_heads or columns != width:
+        raise ValueError(f"the cache holds {heads} heads of {columns}, not {kv_heads} of {width}")
+    for t in (k_scales, v_scales):
+        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads):
+            raise ValueError(f"the cache's scales are float32 [pages, kv_heads], not {t.dtype} {tuple(t.shape)}")
+    if not all(t.is_contiguous() for t in (k_pages, v_pages, k_scales, v_scales)):
+        raise ValueError("the cache's pages and scales must be packed")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"the table is int32 [batch, blocks] with contiguous rows, not {table.dtype} {tuple(table.shape)} with strides {table.stride()}")
+    return pages, page_tokens, table.shape[1], table.stride(0)
+
+
+def _per_sequence(t, batch: int, what: str):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous()):
+        raise ValueError(f"{what} are packed int32 [batch], not {t.dtype} {tuple(t.shape)}")
+
+
+def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, window=None, sinks=0, scale=None, token_major=True):
+    """`window_attention` over a paged cache in 8 bits. The pages are float8_e4m3fn [pages, kv_heads, page_tokens, width] (page_tokens
+    a power of two from 16 to 1024, width a multiple of 16 up to 128), the scales float32 [pages, kv_heads]; an element is
+    code * scale. Row b of `table` (int32 [batch, blocks]) names the pages of sequence b in order, lengths[b] (int32, on the
+    device) says how many tokens it has, the queries' own among them: query i of q [batch, heads, q_tokens, width] stands at
+    position lengths[b] - q_tokens + i. Page numbers and lengths stay on the device; one that leads out of the pool or the table is left
+    out, and `kernel.check_status` then raises."""
+    if q.dim() != 4:
+        raise Declined("the queries must be [batch, heads, tokens, width]")
+    batch, heads, q_tokens, width = q.shape
+    kv_heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    pages, page_tokens, blocks, table_stride = _cache_extents(k_pages, v_pages, k_scales, v_scales, table, batch, kv_heads, width)
+    if (kv_heads == 0) != (heads == 0) or (heads and heads % kv_heads):
+        raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
+    _per_sequence(lengths, batch, "lengths")
+    window, sinks = _window(window, sinks)
+    scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
+    device = _device_of((q, k_pages, v_pages, k_scales, v_scales, table, lengths))
+    out = _attention_result(q, token_major)
+    nbytes = ctypes.c_size_t()
+    check(lib.tq_cache_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page_tokens, blocks, window, sinks, device, ctypes.byref(nbytes)))
+    scratch = _own_scratch(nbytes.value, q.device)
+    check(lib.tq_cache_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),
+                                        _pointer(table), _pointer(lengths), _pointer(out), batch, heads, kv_heads, q_tokens, width, pages, page_tokens, blocks,
+                                        table_stride, _three_strides(q, "the queries"), _three_strides(out, "the result"), scale, window, sinks,
+                                        _pointer(scratch), nbytes.value, device, _stream(None, device)))
+    return out
+
+
+def cache_store(k, v, k_pages, v_pages, k_scales, v_scales, table, starts, counts=None) -> None:
+    """Writes new keys and values [batch, kv_heads, tokens, width] (bf16 or f16) into the cache that `cache_attention` reads: token i
+    of sequence b goes to position starts[b] + i, for i < counts[b] (None: all of them); starts[b] < 0 leaves a sequence as it is.
+    A page and head's scale is the smallest power of two s with every |x| <= 448 s among its tokens since it was begun (position 0 of the
+    page begins it anew); where a new token raises it, the page's earlier ones are encoded again. Each page that is written must belong
+    to one sequence alone. `starts` and `counts` are int32 on the device."""
+    for t in (k, v):
+        if t.dim() != 4:
+            raise Declined("new keys and values must be [batch, kv_heads, tokens, width]")
+    if k.dtype != v.dtype or tuple(k.shape) != tuple(v.shape):
+        raise ValueError(f"new keys and values differ: {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+    batch, kv_heads, tokens, width = k.shape
+    pages, page_tokens, blocks, table_stride = _cache_extents(k_pages, v_pages, k_scales, v_scales, table, batch, kv_heads, width)
+    _per_sequence(starts, batch, "starts")
+    _per_sequence(counts, batch, "counts")
+    device = _device_of([t for t in (k, v, k_pages, v_pages, k_scales, v_scales, table, starts, counts) if t is not None])
+    check(lib.tq_cache_store_launch(dtype_code(k.dtype), _pointer(k), _pointer(v), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),
+                                    _pointer(table), _pointer(starts), _pointer(counts), batch, kv_heads, tokens, width, pages, page_tokens, blocks, table_stride,
+                                    _three_strides(k, "new keys"), _three_strides(v, "new values"), device, _stream(None, device)))
+
+
+def copy_pages(tensors, sources, targets, page_axis=0) -> None:
+    """Copies page sources[i] to page targets[i] in every one of `tensors` (pages of a cache, their scales, of any type), whose axis
+    `page_axis` (0, or 1 behind an axis of layers) counts the pages; a page's own elements are contiguous. `sources` and `targets` are numbers on
+    the host; the targets are distinct and none is a source, so the order of the copies does not show."""
+    if page_axis not in (0, 1):
+        raise Declined(f"pages are counted by axis 0 or 1, not {page_axis}")
+    tensors = list(tensors)
+    if len(sources) != len(targets):
+        raise ValueError(f"{len(sources)} sources and {len(targets)} targets")
+    if not tensors:
+        return
+    pages = None
+    described = (_lib.tq_paged_tensor * len(tensors))()
+    for one, t in zip(described, tensors):
+        if t.dim() <= page_axis or (pages is not None and t.shape[page_axis] != pages):
+            raise ValueError("the tensors of one call have the same number of pages along the page axis")
+        pages = t.shape[page_axis]
+        inner = t[0] if page_axis and t.shape[0] else t
+        if t.numel() and not inner[0].is_contiguous():
+            raise Declined("the elements of a page must be contiguous")
+        size = t.element_size()
+        one.base, one.layers = t.data_ptr(), t.shape[0] if page_axis else 1
+        one.layer_stride = t.stride(0) * size if page_axis else 0
+        one.page_bytes = math.prod(t.shape[page_axis + 1 :]) * size
+        one.page_stride = max(t.stride(page_axis) * size, one.page_bytes if pages == 1 else 0)
+    device = _device_of(tensors)
+    numbers = ctypes.c_int64 * len(sources)
+    check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*sources), numbers(*targets), len(sources), device, _stream(None, device)))
 
 
 # ---------------------------------------------------------------------------------------------

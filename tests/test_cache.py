@@ -1,0 +1,155 @@
+"""Window attention and the paged cache without a GPU: what their entry points refuse."""
+
+import ctypes
+
+import pytest
+import torch
+
+THREE = ctypes.c_int64 * 3
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from tessiq_b200 import _lib
+
+    return _lib
+
+
+AT = ctypes.c_void_p(1 << 20)      # aligned, never followed: every call here is refused or has nothing to do
+OFF = ctypes.c_void_p((1 << 20) + 2)
+
+
+def window(lib, **changed):
+    a = dict(dtype=lib.BF16, q=AT, k=AT, v=AT, out=AT, batch=2, heads=4, kv_heads=2, q_tokens=3, k_tokens=50, width=64, scale=0.125, window=8, sinks=2,
+             q_strides=THREE(4 * 3 * 64, 3 * 64, 64), k_strides=THREE(2 * 50 * 64, 50 * 64, 64), out_strides=THREE(4 * 3 * 64, 3 * 64, 64))
+    a.update(changed)
+    return lib.lib.tq_window_attention_launch(a["dtype"], a["q"], a["k"], a["v"], a["out"], a["batch"], a["heads"], a["kv_heads"], a["q_tokens"], a["k_tokens"],
+                                              a["width"], a["q_strides"], a["k_strides"], a["k_strides"], a["out_strides"], a["scale"], a["window"], a["sinks"],
+                                              None, 0, 0, None)
+
+
+@pytest.mark.parametrize("changed, code", [
+    ({"dtype": 0}, "TQ_UNSUPPORTED"), ({"width": 63}, "TQ_UNSUPPORTED"), ({"width": 136}, "TQ_UNSUPPORTED"), ({"heads": 3}, "TQ_INVALID_ARGUMENT"),
+    ({"kv_heads": 0}, "TQ_INVALID_ARGUMENT"), ({"batch": -1}, "TQ_INVALID_ARGUMENT"), ({"window": -1}, "TQ_INVALID_ARGUMENT"), ({"sinks": -2}, "TQ_INVALID_ARGUMENT"),
+    ({"scale": 0.0}, "TQ_UNSUPPORTED"), ({"scale": float("nan")}, "TQ_UNSUPPORTED"), ({"q": None}, "TQ_INVALID_ARGUMENT"), ({"out": None}, "TQ_INVALID_ARGUMENT"),
+    ({"v": None}, "TQ_INVALID_ARGUMENT"), ({"q": OFF}, "TQ_UNSUPPORTED"), ({"k": OFF}, "TQ_UNSUPPORTED"), ({"k_strides": THREE(6400, 3200, 60)}, "TQ_UNSUPPORTED"),
+    ({"k_strides": THREE(6400, 0, 64)}, "TQ_UNSUPPORTED"), ({"q_strides": THREE(768, 196, 64)}, "TQ_UNSUPPORTED"), ({"out_strides": THREE(768, -192, 64)}, "TQ_INVALID_ARGUMENT"),
+    ({"k_tokens": 1 << 31}, "TQ_UNSUPPORTED"), ({"q_tokens": 1 << 31}, "TQ_UNSUPPORTED"), ({"k_strides": None}, "TQ_INVALID_ARGUMENT"),
+    ({"batch": 0}, "TQ_OK"), ({"heads": 0, "kv_heads": 0}, "TQ_OK"), ({"q_tokens": 0}, "TQ_OK"),
+], ids=str)
+def test_window_attention_refuses(lib, changed, code):
+    assert window(lib, **changed) == getattr(lib, code), lib.last_error()
+
+
+def attend(lib, **changed):
+    a = dict(dtype=lib.F16, q=AT, k=AT, v=AT, ks=AT, vs=AT, table=AT, lengths=AT, out=AT, batch=2, heads=4, kv_heads=2, q_tokens=1, width=64, pages=9, page=16, blocks=4,
+             table_stride=4, q_strides=THREE(256, 64, 64), out_strides=THREE(256, 64, 64), scale=0.1, window=0, sinks=0)
+    a.update(changed)
+    return lib.lib.tq_cache_attention_launch(a["dtype"], a["q"], a["k"], a["v"], a["ks"], a["vs"], a["table"], a["lengths"], a["out"], a["batch"], a["heads"], a["kv_heads"],
+                                             a["q_tokens"], a["width"], a["pages"], a["page"], a["blocks"], a["table_stride"], a["q_strides"], a["out_strides"],
+                                             a["scale"], a["window"], a["sinks"], None, 0, 0, None)
+
+
+@pytest.mark.parametrize("changed, code", [
+    ({"dtype": 1}, "TQ_UNSUPPORTED"), ({"width": 72}, "TQ_UNSUPPORTED"), ({"width": 144}, "TQ_UNSUPPORTED"), ({"page": 8}, "TQ_UNSUPPORTED"), ({"page": 48}, "TQ_UNSUPPORTED"),
+    ({"page": 2048}, "TQ_UNSUPPORTED"), ({"pages": -1}, "TQ_INVALID_ARGUMENT"), ({"heads": 5}, "TQ_INVALID_ARGUMENT"), ({"kv_heads": 0}, "TQ_INVALID_ARGUMENT"),
+    ({"window": -4}, "TQ_INVALID_ARGUMENT"), ({"lengths": None}, "TQ_INVALID_ARGUMENT"), ({"table": None}, "TQ_INVALID_ARGUMENT"), ({"ks": None}, "TQ_INVALID_ARGUMENT"),
+    ({"q": OFF}, "TQ_UNSUPPORTED"), ({"v": OFF}, "TQ_UNSUPPORTED"), ({"table": OFF}, "TQ_UNSUPPORTED"), ({"blocks": 1 << 27}, "TQ_UNSUPPORTED"),
+    ({"scale": -1.0}, "TQ_UNSUPPORTED"), ({"batch": 0}, "TQ_OK"), ({"q_tokens": 0}, "TQ_OK"),
+], ids=str)
+def test_cache_attention_refuses(lib, changed, code):
+    assert attend(lib, **changed) == getattr(lib, code), lib.last_error()
+
+
+def store(lib, **changed):
+    a = dict(dtype=lib.F16, k=AT, v=AT, kp=AT, vp=AT, ks=AT, vs=AT, table=AT, starts=AT, counts=None, batch=2, kv_heads=2, tokens=3, width=64, pages=9, page=16, blocks=4,
+             table_stride=4, strides=THREE(384, 192, 64))
+    a.update(changed)
+    return lib.lib.tq_cache_store_launch(a["dtype"], a["k"], a["v"], a["kp"], a["vp"], a["ks"], a["vs"], a["table"], a["starts"], a["counts"], a["batch"], a["kv_heads"],
+                                         a["tokens"], a["width"], a["pages"], a["page"], a["blocks"], a["table_stride"], a["strides"], a["strides"], 0, None)
+
+
+@pytest.mark.parametrize("changed, code", [
+    ({"dtype": 0}, "TQ_UNSUPPORTED"), ({"width": 8}, "TQ_UNSUPPORTED"), ({"page": 17}, "TQ_UNSUPPORTED"), ({"tokens": -1}, "TQ_INVALID_ARGUMENT"), ({"k": None}, "TQ_INVALID_ARGUMENT"),
+    ({"starts": None}, "TQ_INVALID_ARGUMENT"), ({"vp": None}, "TQ_INVALID_ARGUMENT"), ({"strides": THREE(384, 190, 64)}, "TQ_UNSUPPORTED"), ({"v": OFF}, "TQ_UNSUPPORTED"),
+    ({"counts": OFF}, "TQ_UNSUPPORTED"), ({"tokens": 0}, "TQ_OK"), ({"batch": 0}, "TQ_OK"),
+], ids=str)
+def test_cache_store_refuses(lib, changed, code):
+    assert store(lib, **changed) == getattr(lib, code), lib.last_error()
+
+
+def copy(lib, sources, targets, pages=10, **changed):
+    one = dict(base=1 << 20, layers=1, layer_stride=0, page_stride=64, page_bytes=64)
+    one.update(changed)
+    tensors = (lib.tq_paged_tensor * 1)(lib.tq_paged_tensor(**one))
+    return lib.lib.tq_copy_pages_launch(tensors, 1, pages, (ctypes.c_int64 * len(sources))(*sources), (ctypes.c_int64 * len(targets))(*targets), len(sources), 0, None)
+
+
+@pytest.mark.parametrize("sources, targets, changed", [
+    ([0], [10], {}), ([10], [0], {}), ([-1], [0], {}), ([0], [-1], {}), ([0, 1], [2, 2], {}), ([0, 1], [1, 2], {}), ([3], [3], {}), ([0, 1, 2], [5, 6, 0], {}),
+    ([0], [1], {"page_stride": 60}), ([0], [1], {"layers": -1}), ([0], [1], {"base": None}),
+], ids=str)
+def test_copy_pages_refuses(lib, sources, targets, changed):
+    assert copy(lib, sources, targets, **changed) == lib.TQ_INVALID_ARGUMENT, lib.last_error()
+
+
+def test_copy_pages_with_nothing_to_do(lib):
+    assert copy(lib, [], []) == lib.TQ_OK
+    assert lib.lib.tq_copy_pages_launch(None, 0, 4, None, None, 3, 0, None) == lib.TQ_OK
+
+
+def test_python_refuses_before_the_library():
+    from tessiq_b200 import ops
+    from tessiq_b200._lib import Declined
+
+    q, k = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 9, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.window_attention(q, k, k, 4)
+    with pytest.raises(ValueError, match="at least one key"):
+        ops.window_attention(q, k, k, 0)
+    with pytest.raises(ValueError, match="first keys"):
+        ops.window_attention(q, k, k, 4, -1)
+    with pytest.raises(ValueError, match="do not agree"):
+        ops.window_attention(q, k, k[:, :, :5])
+    with pytest.raises(ValueError, match="do not agree"):
+        ops.window_attention(q[:, :3], k, k)
+    with pytest.raises(Declined, match="element type"):
+        ops.window_attention(q, k.half(), k)
+    with pytest.raises(Declined, match="batch, heads"):
+        ops.window_attention(q[0], k, k)
+    pages = torch.zeros(7, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scales, table, lengths = torch.ones(7, 2), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    good = (pages, pages, scales, scales, table)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.cache_attention(q, *good, lengths)
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        ops.cache_attention(q, pages.view(torch.uint8), pages, scales, scales, table, lengths)
+    with pytest.raises(ValueError, match="scales"):
+        ops.cache_attention(q, pages, pages, scales[:6], scales, table, lengths)
+    with pytest.raises(ValueError, match="scales"):
+        ops.cache_attention(q, pages, pages, scales, scales.double(), table, lengths)
+    with pytest.raises(ValueError, match="table"):
+        ops.cache_attention(q, pages, pages, scales, scales, table.long(), lengths)
+    with pytest.raises(ValueError, match="table"):
+        ops.cache_attention(q, pages, pages, scales, scales, table[:1], lengths)
+    with pytest.raises(ValueError, match="lengths"):
+        ops.cache_attention(q, *good, lengths.long())
+    with pytest.raises(ValueError, match="holds"):
+        ops.cache_attention(q[..., :32], *good, lengths)
+    with pytest.raises(ValueError, match="packed"):
+        ops.cache_attention(q, pages.transpose(0, 0)[::2], pages[::2], scales[:4], scales[:4], table, lengths)
+    with pytest.raises(ValueError, match="evenly"):
+        ops.cache_attention(q[:, :3], *good, lengths)
+    with pytest.raises(ValueError, match="differ"):
+        ops.cache_store(k, k[:, :, :4], *good, lengths)
+    with pytest.raises(ValueError, match="counts"):
+        ops.cache_store(k, k, *good, lengths, lengths[:1])
+    with pytest.raises(ValueError, match="same number of pages"):
+        ops.copy_pages([pages.view(torch.uint8), scales[:3]], [0], [1])
+    with pytest.raises(ValueError, match="sources"):
+        ops.copy_pages([scales], [0, 1], [2])
+    with pytest.raises(Declined, match="contiguous"):
+        ops.copy_pages([torch.zeros(7, 4, 4).transpose(1, 2)], [0], [1])
+    with pytest.raises(Declined, match="axis"):
+        ops.copy_pages([scales], [0], [1], page_axis=2)
+    ops.copy_pages([], [0], [1])

@@ -1,0 +1,485 @@
+"""Attention with a window and sinks, the paged cache in 8 bits, its writer and the copies of its pages, against plain 64-bit forms.
+
+How far a result may be off (`bound`): half a step of its type, relative (bf16 2^-8, f16 2^-11); half a step of the probabilities' rounding
+relative to sum_j p_j |v_j| (f16 2^-11, below its normal range 2^-25 a key absolutely; bf16 2^-8 in the tensor-core tiles, the
+coarser of the forms); an error d of a score is a relative error of 2 d in the probabilities, and f32 sums of `width` products give
+d = (width + 4) 2^-24 sum |q| |k| scale, ex2.approx another 2^-21; f32 sums over n keys (n + 8) 2^-24. Codes, scales and copies are exact."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def tq():
+    if not torch.cuda.is_available():
+        pytest.fail("the gpu tests need a CUDA device")
+    from tessiq_b200 import ops
+
+    return ops
+
+
+def status(device=0):
+    from tessiq_b200 import _lib
+
+    code = ctypes.c_int32(-1)
+    _lib.check(_lib.lib.tq_status_poll(device, None, ctypes.byref(code)))
+    return code.value
+
+
+def reference(q, k, v, lengths, window, sinks, scale):
+    """(result, bound) in f64 on the CPU: q [batch, heads, queries, width], k and v [batch, kv_heads, keys, width]; only visible keys are touched."""
+    q, k, v = (t.detach().cpu() for t in (q, k, v))
+    dtype = q.dtype
+    u_out = torch.finfo(dtype).eps / 2
+    batch, heads, queries, width = q.shape
+    group = heads // k.shape[1]
+    out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.full(q.shape, 1e-30, dtype=torch.float64)
+    for b in range(batch):
+        for i in range(queries):
+            p = lengths[b] - queries + i
+            if p < 0:
+                continue
+            j = torch.arange(p + 1)
+            j = j[(j > p - window) | (j < sinks)] if window is not None else j
+            for h in range(heads):
+                qq, kk, vv = q[b, h, i].double(), k[b, h // group, j].double(), v[b, h // group, j].double()
+                weight = torch.softmax(kk @ qq * scale, 0)
+                out[b, h, i] = weight @ vv
+                spread = weight @ vv.abs()
+                d = (width + 4) * 2.0**-24 * (kk.abs() @ qq.abs()).max().item() * scale + 2.0**-21
+                bound[b, h, i] += u_out * out[b, h, i].abs() + (u_out + 2 * d + (len(j) + 8) * 2.0**-24) * spread
+                bound[b, h, i] += 2.0**-25 * vv.abs().sum(0)
+    return out, bound
+
+
+def held(got, expected):
+    exact, bound = expected
+    got = got.detach().cpu().double()
+    assert torch.equal(got.isnan(), exact.isnan())
+    error = (got - exact).abs()
+    over = (error / bound).nan_to_num(0.0).max().item()
+    assert over <= 1.0, f"{over:.2f} times what roundings explain"
+
+
+def drawn(shape, dtype, seed, spread=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * spread).to(dtype).cuda()
+
+
+def by_token(shape, dtype, seed):
+    """[batch, heads, tokens, width] as a projection's [batch, tokens, heads, width] is seen."""
+    batch, heads, tokens, width = shape
+    return drawn((batch, tokens, heads, width), dtype, seed).transpose(1, 2)
+
+
+# ---- dense keys ----------------------------------------------------------------------------------
+
+WINDOWS = [  # batch, heads, kv_heads, queries, keys, width, window, sinks
+    (1, 1, 1, 1, 1, 64, None, 0), (1, 1, 1, 1, 1, 64, 1, 0), (2, 3, 3, 1, 77, 64, 10, 4), (1, 4, 2, 3, 130, 128, 40, 0), (1, 8, 1, 1, 300, 64, 64, 1),
+    (2, 16, 2, 2, 333, 128, 100, 33), (1, 2, 2, 5, 3, 64, None, 0), (1, 2, 1, 9, 4, 64, 2, 1), (1, 2, 2, 100, 100, 64, 7, 3), (1, 6, 2, 130, 130, 96, 64, 64),
+    (2, 2, 1, 129, 200, 128, 128, 5), (1, 1, 1, 257, 257, 64, 1, 0), (1, 2, 2, 300, 300, 64, 1000, 2), (1, 1, 1, 70, 600, 40, 200, 500), (1, 2, 1, 260, 90, 64, 30, 10),
+    (1, 3, 3, 17, 1100, 8, 129, 4), (1, 12, 12, 4, 2049, 64, 2048, 4), (1, 2, 2, 384, 384, 128, 65, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", WINDOWS, ids=lambda c: "-".join(map(str, c)))
+def test_window_attention(tq, case, dtype):
+    batch, heads, kv_heads, queries, keys, width, window, sinks = case
+    q, k, v = by_token((batch, heads, queries, width), dtype, 1), by_token((batch, kv_heads, keys, width), dtype, 2), by_token((batch, kv_heads, keys, width), dtype, 3)
+    got = tq.window_attention(q, k, v, window, sinks)
+    assert got.shape == q.shape and got.dtype == dtype
+    held(got, reference(q, k, v, [keys] * batch, window, sinks, 1 / math.sqrt(width)))
+    assert status() == 0
+
+
+def test_without_a_window_it_is_causal_attention(tq):
+    q, k, v = (drawn((2, 4, 200, 64), torch.bfloat16, s) for s in (1, 2, 3))
+    expected = reference(q, k, v, [200, 200], None, 0, 0.2)
+    held(tq.window_attention(q, k, v, scale=0.2), expected)
+    held(tq.attention(q, k, v, 0.2, causal=True), expected)
+
+
+@pytest.mark.parametrize("token_major", [True, False])
+def test_window_attention_writes_either_order(tq, token_major):
+    q, k, v = (drawn((2, 4, 5, 64), torch.float16, s) for s in (1, 2, 3))
+    got = tq.window_attention(q, k, v, 3, 1, token_major=token_major)
+    assert got.is_contiguous() != token_major
+    held(got, reference(q, k, v, [5, 5], 3, 1, 0.125))
+
+
+def test_window_attention_over_no_keys_and_no_queries(tq):
+    q = drawn((2, 4, 3, 64), torch.bfloat16, 1)
+    none = torch.empty(2, 2, 0, 64, dtype=torch.bfloat16, device="cuda")
+    assert tq.window_attention(q, none, none, 4, 1).count_nonzero().item() == 0
+    assert tq.window_attention(q[:, :, :0], none, none).shape == (2, 4, 0, 64)
+    assert tq.window_attention(q[:0], none[:0], none[:0]).shape == (0, 4, 3, 64)
+
+
+@pytest.mark.parametrize("queries", [1, 3, 70, 200], ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_no_query_sees_does_not_reach_a_result(tq, queries, bad):
+    """Keys 20 to 39 lie between the sinks and the first query's window, and the last keys are the last queries' own."""
+    keys, window = queries + 100, 50
+    q, k, v = drawn((1, 4, queries, 64), torch.bfloat16, 1), drawn((1, 2, keys, 64), torch.bfloat16, 2), drawn((1, 2, keys, 64), torch.bfloat16, 3)
+    k[:, :, 20:40], v[:, :, 20:40] = bad, bad
+    expected = reference(q, k, v, [keys], window, 20, 0.125)
+    assert not expected[0].isnan().any()
+    held(tq.window_attention(q, k, v, window, 20), expected)
+
+
+@pytest.mark.parametrize("queries", [4, 150], ids=str)
+def test_a_value_that_is_not_a_number_reaches_the_queries_that_see_it(tq, queries):
+    """Key `at` is seen from the query at `at` for a window's length, and by those alone; sinks by all of them."""
+    keys, window, at = queries + 30, 20, 29 + queries // 2
+    q, k, v = (drawn((1, 2, n, 64), torch.float16, s) for n, s in ((queries, 1), (keys, 2), (keys, 3)))
+    v[0, 1, at, 5] = math.nan
+    v[0, 0, keys - 1, 7] = math.inf
+    expected = reference(q, k, v, [keys], window, 3, 0.125)
+    got = tq.window_attention(q, k, v, window, 3).cpu().double()
+    assert expected[0].isnan().any() and torch.equal(got.isnan(), expected[0].isnan()) and torch.equal(got.isinf(), expected[0].isinf())
+    fine = expected[0].isfinite()
+    assert ((got - expected[0]).abs()[fine] <= expected[1][fine]).all()
+
+
+def test_scores_that_are_all_minus_infinity_are_not_a_number(tq):
+    """As softmax over them is; a query that sees nothing is zeros instead."""
+    q, k, v = (drawn((1, 1, 2, 64), torch.bfloat16, s).abs() + 0.5 for s in (1, 2, 3))
+    k[:, :, 0] = -math.inf
+    got = tq.window_attention(q, k, v, 1, 0)
+    assert got[0, 0, 0].isnan().all() and got[0, 0, 1].isfinite().all()
+    got = tq.window_attention(q, k[:, :, :1], v[:, :, :1])
+    assert got[0, 0, 0].count_nonzero().item() == 0 and got[0, 0, 1].isnan().all()
+
+
+# ---- the cache -----------------------------------------------------------------------------------
+
+
+class Cache:
+    """A pool with a table of scattered pages; what no sequence owns is NaN."""
+
+    def __init__(self, batch, kv_heads, width, page, blocks, seed=0):
+        self.page, pages = page, batch * blocks + 2
+        g = torch.Generator().manual_seed(seed)
+        shape = (pages, kv_heads, page, width)
+        self.codes = [torch.full(shape, 0x7F, dtype=torch.uint8).view(E4M3).cuda() for _ in range(2)]
+        self.scales = [torch.full(shape[:2], math.nan).cuda() for _ in range(2)]
+        order = torch.randperm(pages, generator=g)
+        self.table = order[: batch * blocks].to(torch.int32).reshape(batch, blocks).cuda()
+        self.generator = g
+
+    @property
+    def tensors(self):
+        return (*self.codes, *self.scales)
+
+    def fill(self, lengths):
+        """Random tokens at each sequence's first positions; the rest stays NaN."""
+        for codes, scales in zip(self.codes, self.scales):
+            for b, length in enumerate(lengths):
+                for n in range(-(-length // self.page)):
+                    page, tokens = int(self.table[b, n]), min(self.page, length - n * self.page)
+                    part = (torch.randn(codes.shape[1], tokens, codes.shape[3], generator=self.generator) * 60).clamp(-448, 448).to(E4M3)
+                    codes.view(torch.uint8)[page, :, :tokens] = part.view(torch.uint8).cuda()
+                    scales[page] = torch.exp2(torch.randn(codes.shape[1], generator=self.generator) * 2 - 6).cuda()
+        return self
+
+    def decoded(self, which):
+        """[batch, kv_heads, tokens, width] in f32 on the CPU."""
+        pages = self.table.long().cpu()
+        codes, scales = self.codes[which].view(torch.uint8).cpu()[pages].view(E4M3).float(), self.scales[which].cpu()[pages]
+        values = codes * scales[..., None, None]
+        return values.permute(0, 2, 1, 3, 4).flatten(2, 3)
+
+
+CACHES = [  # heads, kv_heads, queries, width, page, window, sinks, lengths
+    (1, 1, 1, 64, 16, None, 0, [1]), (2, 2, 1, 64, 16, None, 0, [0, 1, 15, 16, 17]), (12, 12, 1, 64, 64, None, 0, [100, 3, 64, 65]), (8, 1, 1, 128, 32, None, 0, [31, 33, 257]),
+    (16, 2, 1, 128, 64, 100, 4, [1, 99, 104, 105, 640]), (6, 3, 4, 64, 16, 20, 5, [0, 1, 3, 4, 5, 200]), (16, 2, 4, 128, 64, None, 0, [2, 300]), (4, 4, 3, 16, 128, 30, 0, [500, 7]),
+    (64, 8, 1, 80, 64, 64, 64, [63, 700]), (3, 1, 11, 96, 32, 33, 1, [5, 90]), (2, 1, 40, 32, 16, 17, 2, [39, 41, 130]), (5, 1, 2, 112, 1024, None, 0, [1500]), (14, 2, 1, 64, 32, 1, 0, [1, 50]),
+    (8, 8, 1, 128, 64, None, 0, [5000, 1]), (32, 8, 2, 128, 16, 3000, 16, [4097]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", CACHES, ids=lambda c: "-".join(map(str, c[:7])) + f"-{len(c[7])}")
+def test_cache_attention(tq, case, dtype):
+    heads, kv_heads, queries, width, page, window, sinks, lengths = case
+    batch = len(lengths)
+    cache = Cache(batch, kv_heads, width, page, max(1, -(-max(lengths) // page))).fill(lengths)
+    q = by_token((batch, heads, queries, width), dtype, 1)
+    got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor(lengths, dtype=torch.int32).cuda(), window, sinks)
+    # (codes times scales in f64: the keys as they stand)
+    expected = reference(q, cache.decoded(0).double(), cache.decoded(1).double(), lengths, window, sinks, 1 / math.sqrt(width))
+    held(got, expected)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("spread", [2.0**-60, 2.0**-20, 2.0**20, 2.0**60])
+def test_queries_of_any_size(tq, spread):
+    """bf16 queries far outside the range of f16, with scores that stay moderate."""
+    cache = Cache(1, 2, 64, 16, 4).fill([50])
+    q = drawn((1, 4, 2, 64), torch.bfloat16, 1, spread)
+    q[0, 1, 0] = 0.0
+    scale = 0.125 / spread
+    got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor([50], dtype=torch.int32).cuda(), scale=scale)
+    held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [50], None, 0, scale))
+
+
+def test_scales_far_apart_between_pages(tq):
+    cache = Cache(1, 1, 64, 16, 6).fill([96])
+    cache.scales[1][cache.table[0].long(), 0] = torch.tensor([1e-12, 1e12, 3.0, 1e-30, 1e20, 0.7]).cuda()
+    cache.scales[0][cache.table[0].long(), 0] = torch.tensor([0.01, 0.03, 1e-8, 0.02, 0.004, 0.01]).cuda()
+    q = drawn((1, 1, 1, 64), torch.bfloat16, 1)
+    for window in (None, 16, 40):
+        got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor([96], dtype=torch.int32).cuda(), window)
+        held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [96], window, 0, 0.125))
+
+
+def test_pages_that_are_not_there_are_left_out_and_reported(tq):
+    from tessiq_b200.kernel import DeviceWaitError, check_status
+
+    assert status() == 0
+    lengths = [64, 64]
+    cache = Cache(2, 1, 64, 16, 4).fill(lengths)
+    q, at = drawn((2, 1, 1, 64), torch.bfloat16, 1), torch.tensor(lengths, dtype=torch.int32).cuda()
+    keys, values = cache.decoded(0).double(), cache.decoded(1).double()
+    table = cache.table.clone()
+    table[1, 3] = 1 << 30
+    table[1, 2] = -1
+    got = tq.cache_attention(q, *cache.tensors, table, at)
+    with pytest.raises(DeviceWaitError, match="outside the pool"):
+        check_status()
+    held(got[:1], reference(q[:1], keys[:1], values[:1], [64], None, 0, 0.125))
+    weights = torch.softmax(keys[1, 0, :32] @ q[1, 0, 0].cpu().double() * 0.125, 0)
+    torch.testing.assert_close(got[1, 0, 0].cpu().double(), weights @ values[1, 0, :32], rtol=2e-2, atol=2e-2)
+    tq.cache_attention(q, *cache.tensors, cache.table, at + 1)
+    with pytest.raises(DeviceWaitError, match="longer than its table"):
+        check_status()
+    starts = torch.tensor([0, 64], dtype=torch.int32).cuda()
+    before = [t.clone().view(torch.uint8) if t.dtype == E4M3 else t.clone() for t in cache.tensors]
+    k = drawn((2, 1, 1, 64), torch.bfloat16, 4)
+    table[0, 0] = 99
+    tq.cache_store(k, k, *cache.tensors, table, starts)
+    with pytest.raises(DeviceWaitError):
+        check_status()
+    for was, now in zip(before, cache.tensors):
+        assert torch.equal(was.nan_to_num() if was.dtype == torch.float32 else was, now.view(torch.uint8) if now.dtype == E4M3 else now.nan_to_num())
+    assert status() == 0
+
+
+# ---- writing -------------------------------------------------------------------------------------
+
+
+def nearest_code(x):
+    """e4m3 of f64 values of at most 448, to nearest even, as f64; NaN where x is not finite."""
+    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0**-40))).clamp(min=-6) - 3)
+    return torch.where(x.isfinite(), torch.round(x / step) * step, math.nan)
+
+
+def stored(cache_codes, cache_scales, table, x, starts, counts, page):
+    """What the pool holds after a write, by the definition, in f64 on the CPU: (codes, scales)."""
+    codes, scales = cache_codes.cpu().float().double(), cache_scales.cpu().double()
+    x, table = x.cpu().double(), table.cpu()
+    for b in range(x.shape[0]):
+        n = 0
+        while starts[b] >= 0 and n < counts[b]:
+            block, offset = divmod(starts[b] + n, page)
+            take = min(page - offset, counts[b] - n)
+            where, part = int(table[b, block]), x[b, :, n : n + take]
+            for h in range(x.shape[1]):
+                largest = torch.where(part[h].isfinite(), part[h].abs(), 0.0).max().item()
+                s = 2.0**-126
+                old = scales[where, h].item() if offset else 0.0
+                while largest > 448 * s or s < old:      # (a power of two, whatever the scale that was there)
+                    s *= 2
+                if offset:
+                    codes[where, h, :offset] = nearest_code(codes[where, h, :offset] * (old / s))
+                codes[where, h, offset : offset + take] = nearest_code(part[h] / s)
+                scales[where, h] = s
+            n += take
+    return codes, scales
+
+
+def same(got, expected):
+    return torch.equal(got.isnan(), expected.isnan()) and torch.equal(got.nan_to_num(), expected.nan_to_num())
+
+
+STORES = [  # kv_heads, tokens, width, page, starts, counts
+    (1, 1, 64, 16, [0], None), (2, 1, 64, 16, [0, 1, 15, 16, 31, -1], None), (12, 1, 64, 64, [999, 0, 63], None), (3, 5, 16, 16, [14, 0, 16, 30], [5, 0, 3, 2]),
+    (2, 100, 128, 64, [0, 1, 63, 64], [100, 99, 1, 64]), (1, 300, 128, 128, [0, 100], None), (2, 40, 80, 16, [7, -5, 0], [40, 40, 17]), (1, 1100, 96, 1024, [3], None),
+    (8, 2, 128, 32, [31, 30], None), (1, 17, 128, 16, [15], None),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", STORES, ids=lambda c: "-".join(map(str, c[:4])) + f"-{len(c[4])}")
+def test_cache_store(tq, case, dtype):
+    kv_heads, tokens, width, page, starts, counts = case
+    batch = len(starts)
+    cache = Cache(batch, kv_heads, width, page, -(-(max(starts) + tokens) // page)).fill([max(s, 0) for s in starts])
+    # from far smaller to far larger than what is there
+    size = torch.exp2(torch.randn(batch, kv_heads, 1, 1, generator=cache.generator) * 4).cuda()
+    k, v = (by_token((batch, kv_heads, tokens, width), torch.float32, s).mul(size).to(dtype) for s in (5, 6))
+    given = [tokens] * batch if counts is None else counts
+    expected = [stored(cache.codes[i], cache.scales[i], cache.table, x, starts, given, page) for i, x in ((0, k), (1, v))]
+    tq.cache_store(k, v, *cache.tensors, cache.table, torch.tensor(starts, dtype=torch.int32).cuda(),
+                   None if counts is None else torch.tensor(counts, dtype=torch.int32).cuda())
+    for i in range(2):
+        assert same(cache.scales[i].cpu().double(), expected[i][1])
+        assert same(cache.codes[i].cpu().float().double(), expected[i][0])
+    assert status() == 0
+
+
+def test_a_scale_is_the_smallest_power_of_two(tq):
+    """Around the border 448 * 2^n, at zeros, at the smallest and the largest numbers."""
+    values = [0.0, 448.0, 450.0, 446.0, 1.75, 1.7578125, 2.0**-126, 2.0**-133, 3.0e38, 1.0]
+    cache = Cache(len(values), 1, 16, 16, 1)
+    k = torch.zeros(len(values), 1, 1, 16)
+    k[:, 0, 0, 3] = torch.tensor(values)
+    k = k.bfloat16().cuda()
+    starts = torch.zeros(len(values), dtype=torch.int32).cuda()
+    tq.cache_store(k, -k, *cache.tensors, cache.table, starts)
+    for i, x in ((0, k), (1, -k)):
+        codes, scales = stored(cache.codes[i], cache.scales[i], cache.table, x, [0] * len(values), [1] * len(values), 16)
+        assert same(cache.scales[i].cpu().double(), scales) and same(cache.codes[i].cpu().float().double(), codes)
+    pages = cache.table[:, 0].long()
+    back = cache.codes[0][pages][:, 0, 0, 3].float() * cache.scales[0][pages, 0]
+    assert ((back - k[:, 0, 0, 3].float()).abs() <= 2.0**-4 * k[:, 0, 0, 3].float().abs()).all()
+
+
+def test_what_is_not_finite_is_stored_as_nan_and_has_no_say_in_the_scale(tq):
+    cache = Cache(1, 1, 16, 16, 1)
+    k = torch.ones(1, 1, 4, 16).half().cuda()
+    k[0, 0, 1, 2], k[0, 0, 2, 5], k[0, 0, 3, 7] = math.inf, -math.inf, math.nan
+    tq.cache_store(k, k, *cache.tensors, cache.table, torch.zeros(1, dtype=torch.int32).cuda())
+    page = int(cache.table[0, 0])
+    assert cache.scales[0][page, 0].item() == 2.0**-8
+    codes = cache.codes[0][page, 0, :4].float()
+    assert torch.equal(codes.isnan(), ~k[0, 0].isfinite()) and (codes[~codes.isnan()] == 256.0).all()
+
+
+def test_token_by_token_is_the_prompt_at_once(tq):
+    """A cache filled a token at a time holds what a prompt written in one call holds, where codes have not gone below their normal range."""
+    kv_heads, width, tokens = 2, 64, 70
+    one, other = Cache(2, kv_heads, width, 32, 3, seed=3), Cache(2, kv_heads, width, 32, 3, seed=3)
+    k, v = ((drawn((2, kv_heads, tokens, width), torch.float32, s).sign() * (1 + drawn((2, kv_heads, tokens, width), torch.float32, s + 9).abs())).bfloat16() for s in (1, 2))
+    zero = torch.zeros(2, dtype=torch.int32).cuda()
+    tq.cache_store(k, v, *one.tensors, one.table, zero)
+    for t in range(tokens):
+        tq.cache_store(k[:, :, t : t + 1], v[:, :, t : t + 1], *other.tensors, other.table, zero + t)
+    for a, b in zip(one.tensors, other.tensors):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) if a.dtype == E4M3 else same(a, b)
+
+
+# ---- copying -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.float16, torch.float32, torch.float64, E4M3], ids=str)
+@pytest.mark.parametrize("inner", [(1,), (3,), (12,), (2, 16, 64), (5, 7)], ids=str)
+def test_copy_pages(tq, dtype, inner):
+    pages = 40
+    t = torch.randint(0, 100, (pages, *inner), generator=torch.Generator().manual_seed(1)).to(torch.float32).to(dtype).cuda()
+    before = t.float().cpu()
+    tq.copy_pages([t], [3, 0, 39, 3], [5, 38, 1, 7])
+    expected = before.clone()
+    expected[[5, 38, 1, 7]] = before[[3, 0, 39, 3]]
+    assert torch.equal(t.float().cpu(), expected)
+
+
+def test_copy_pages_of_layers_views_and_many_pairs(tq):
+    g = torch.Generator().manual_seed(1)
+    pages = 1000
+    tensors = [torch.randn(3, pages, 2, 8, generator=g).cuda(), torch.randn(3, pages, 5, generator=g).cuda()[:, :, :],
+               torch.randn(4, 2 * pages, 3, generator=g).cuda()[1:3, ::2, :2], torch.randint(0, 255, (5, pages, 20000 // 8), dtype=torch.uint8, generator=g).cuda()]
+    tensors += [torch.randn(1, pages, 4, generator=g).cuda() for _ in range(20)]
+    order = torch.randperm(pages, generator=g).tolist()
+    sources, targets = order[:450], order[500:950]
+    expected = [t.clone() for t in tensors]
+    for t in expected:
+        t[:, targets] = t[:, sources]
+    beside = [t._base.clone() if t._base is not None else None for t in tensors]
+    tq.copy_pages(tensors, sources, targets, page_axis=1)
+    for t, e in zip(tensors, expected):
+        assert torch.equal(t, e)
+    untouched = tensors[2]._base
+    assert torch.equal(untouched[:, 1::2], beside[2][:, 1::2]) and torch.equal(untouched[0], beside[2][0]) and torch.equal(untouched[..., 2], beside[2][..., 2])
+
+
+def test_copy_pages_of_a_page_longer_than_a_share(tq):
+    t = torch.randint(0, 255, (4, 100003), dtype=torch.uint8, generator=torch.Generator().manual_seed(2)).cuda()
+    before = t.clone()
+    tq.copy_pages([t], [0], [3])
+    assert torch.equal(t[3], before[0]) and torch.equal(t[:3], before[:3])
+
+
+# ---- together ------------------------------------------------------------------------------------
+
+
+def test_a_conversation_a_fork_and_its_two_ends(tq):
+    """Prompts, a step, a fork that copies the last page, and a step of both: attention over the cache is attention over what was stored."""
+    heads, kv_heads, width, page = 8, 2, 64, 16
+    cache = Cache(3, kv_heads, width, page, 5)
+    prompts = [37, 20]
+    k, v = (by_token((3, kv_heads, 60, width), torch.bfloat16, s) for s in (1, 2))
+    counts = torch.tensor([*prompts, 0], dtype=torch.int32).cuda()
+    zero = torch.zeros(3, dtype=torch.int32).cuda()
+    tq.cache_store(k[:, :, :37], v[:, :, :37], *cache.tensors, cache.table, zero, counts)
+    # the third sequence is the first one's fork: its full pages are shared, its last one is a copy
+    cache.table[2, :2] = cache.table[0, :2]
+    tq.copy_pages(cache.tensors, [int(cache.table[0, 2])], [int(cache.table[2, 2])])
+    lengths = [38, 21, 38]
+    step = torch.tensor([n - 1 for n in lengths], dtype=torch.int32).cuda()
+    tq.cache_store(k[:, :, 40:41], v[:, :, 40:41], *cache.tensors, cache.table, step)
+    q = by_token((3, heads, 1, width), torch.bfloat16, 7)
+    for window, sinks in ((None, 0), (16, 4)):
+        got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor(lengths, dtype=torch.int32).cuda(), window, sinks)
+        held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), lengths, window, sinks, 0.125))
+    # what the cache holds is what went in, to half a step of e4m3 (2^-4) of it or, below the normal range, 2^-10 of the scale
+    for which, x in ((0, k), (1, v)):
+        values = cache.decoded(which)
+        for b, n in ((0, 37), (1, 20)):
+            error = (values[b, :, :n] - x[b, :, :n].float().cpu()).abs()
+            pages = cache.table[b].long().cpu()
+            step_of = cache.scales[which].cpu()[pages].T.repeat_interleave(page, 1)[:, :n, None] * 2.0**-10
+            assert (error <= torch.maximum(2.0**-4 * x[b, :, :n].float().cpu().abs(), step_of)).all()
+        assert torch.equal(values[0, :, :37].view(torch.uint8), values[2, :, :37].view(torch.uint8))
+    assert status() == 0
+
+
+def test_a_step_replayed_from_a_graph(tq):
+    """Lengths, starts and tables are read on the device: a captured step goes on as they change. Two graphs share nothing."""
+    heads, kv_heads, width, page = 4, 2, 64, 16
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    caches = [Cache(2, kv_heads, width, page, 40, seed=i).fill([600, 5]) for i in range(2)]
+    k, q = by_token((2, kv_heads, 1, width), torch.bfloat16, 1), by_token((2, heads, 1, width), torch.bfloat16, 2)
+    starts = [torch.tensor([600, 5], dtype=torch.int32).cuda() for _ in range(2)]
+    lengths = [s + 1 for s in starts]
+    graphs, results = [], []
+    for cache, start, length in zip(caches, starts, lengths):
+        tq.cache_store(k, k, *cache.tensors, cache.table, start)
+        tq.cache_attention(q, *cache.tensors, cache.table, length)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            tq.cache_store(k, k, *cache.tensors, cache.table, start)
+            start.add_(1)
+            results.append(tq.cache_attention(q, *cache.tensors, cache.table, length))
+            length.add_(1)
+        graphs.append(graph)
+    for start, length in zip(starts, lengths):
+        start.copy_(torch.tensor([600, 5]))
+        length.copy_(torch.tensor([601, 6]))
+    torch.cuda.synchronize()
+    for step in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for cache, got in zip(caches, results):
+        held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [620, 25], None, 0, 0.125))
+    assert status() == 0
