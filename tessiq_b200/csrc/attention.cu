@@ -715,6 +715,10 @@ extern "C" tq_status tq_window_attention_workspace_bytes(int64_t batch, int64_t 
                                                          int64_t head_dim, int64_t window, int64_t sinks, int32_t device, size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   *bytes = 0;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || k_tokens <= 0) return TQ_OK;      // the launch has nothing to do, or refuses
+  tq::KeyedParams p = {};
+  tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
+  *bytes = tq::keyed_workspace(false, p, k_tokens, device);
   return TQ_OK;
 }
 
@@ -771,5 +775,5 @@ extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, c
   }
   p.k_tokens = static_cast<int>(k_tokens);
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
-  return tq::keyed_attention(dtype, false, p, static_cast<cudaStream_t>(stream));
+  return tq::keyed_attention(dtype, false, p, k_tokens, workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }

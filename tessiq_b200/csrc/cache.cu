@@ -285,6 +285,10 @@ extern "C" tq_status tq_cache_attention_workspace_bytes(int64_t batch, int64_t h
                                                         size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   *bytes = 0;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || blocks <= 0) return TQ_OK;      // the launch has nothing to do, or refuses
+  tq::KeyedParams p = {};
+  tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
+  *bytes = tq::keyed_workspace(true, p, blocks * page_tokens, device);
   return TQ_OK;
 }
 
@@ -342,7 +346,7 @@ extern "C" tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, co
     p.out_strides[i] = out_strides[i];
   }
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
-  return tq::keyed_attention(dtype, true, p, static_cast<cudaStream_t>(stream));
+  return tq::keyed_attention(dtype, true, p, blocks * page_tokens, workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const void* v, void* k_pages, void* v_pages, float* k_scales, float* v_scales,

@@ -21,7 +21,10 @@
 // A masked key must not reach a result through 0 * NaN: its score is replaced, and where the rows of a tile see a chunk's keys
 // alike its value is replaced by zeros. Where they do not (several queries, at an end of the window) the chunk's product is
 // taken once a query with that query's keys alone, and each row keeps its own.
+#include <cuda.h>
+
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #include "common.h"
@@ -34,26 +37,59 @@ namespace {
 constexpr int kKeyedWarps = 4;
 constexpr int kKeyedThreads = 32 * kKeyedWarps;
 
+#ifndef KSTAGES
+#define KSTAGES 2
+#define KCTAS 3
+#endif
+constexpr int kKeyedStages = KSTAGES;      // chunks of a warp in flight or in use
+constexpr uint32_t kStageBytes = 8192;
+constexpr uint32_t kWarpRing = kKeyedStages * kStageBytes;
+constexpr int kWaitKeyed = 0x4b455931;      // "KEY1"
+constexpr float kSlack = 8.f;
+
 // BITS of a key element, W: the head's elements, rounded up to 64 or 128.
 template <int BITS, int W>
 struct KeyedShape {
-  static constexpr int kKeys = BITS == 16 && W == 128 ? 16 : 32;      // a chunk: what a warp takes at a time
+  static constexpr int kKeys = static_cast<int>(kStageBytes) * 4 / (W * BITS);      // a chunk: what a warp takes at a time, keys and then values in a stage
   static constexpr int kTiles = kKeys / 16;
-  static constexpr int kPieces = W * BITS / 512;                      // 16-byte pieces of a key a lane holds (four lanes a key)
+  static constexpr int kPieces = W * BITS / 512;                      // 16-byte pieces of a key a lane takes (four lanes a key)
   static constexpr int kPieceWidth = 128 / BITS;                      // head elements in one
-  static constexpr int kValueWords = W * BITS / 256;                  // 32-bit words of a value a lane holds (eight lanes a value)
+  static constexpr int kValueWords = W * BITS / 256;                  // 32-bit words of a value a lane takes (eight lanes a value)
   static constexpr int kSlices = W / 16;                              // 16 head elements of the result
+  static constexpr int kLine = W * BITS / 8 < 128 ? W * BITS / 8 : 128;      // bytes of a key in a box: 64 or 128, swizzled as many
+  static constexpr int kLines = W * BITS / 8 / kLine;                 // boxes side by side (two for 16-bit heads over 64)
+  static constexpr uint32_t kBoxBytes = kKeys * kLine;                // a chunk's keys (or values), one of the boxes side by side
+  // Where byte `column` of key `key` of a chunk lies: TMA exchanges 16-byte units within a line by the line's place in 8.
+  static __device__ __forceinline__ uint32_t at(int key, int column) {
+    const uint32_t box = kLines == 1 ? 0u : static_cast<uint32_t>(column / kLine) * kBoxBytes;
+    const int unit = (column % kLine) / 16;
+    const int turned = kLine == 128 ? unit ^ (key & 7) : unit ^ ((key >> 1) & 3);
+    return box + key * kLine + turned * 16 + column % 16;
+  }
 };
+constexpr size_t kKeyedSmem = 1024 + kKeyedWarps * kWarpRing;
 
-__device__ __forceinline__ uint4 load_piece(const void* pointer) {
+__device__ __forceinline__ uint4 load_shared_16(uint32_t address) {
   uint4 word;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(word.x), "=r"(word.y), "=r"(word.z), "=r"(word.w) : "l"(pointer));
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(word.x), "=r"(word.y), "=r"(word.z), "=r"(word.w) : "r"(address));
   return word;
 }
-__device__ __forceinline__ uint2 load_half_piece(const void* pointer) {
+__device__ __forceinline__ uint2 load_shared_8(uint32_t address) {
   uint2 word;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(word.x), "=r"(word.y) : "l"(pointer));
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(word.x), "=r"(word.y) : "r"(address));
   return word;
+}
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(column), "r"(row)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_tokens(uint32_t dst, const CUtensorMap* map, uint32_t bar, int column, int token, int head, int batch) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(column), "r"(token), "r"(head), "r"(batch)
+      : "memory");
 }
 
 // Two e4m3 codes (the low or the high half of a word) as f16.
@@ -126,50 +162,236 @@ __device__ __forceinline__ ChunkList chunks_of(int low, int high, int window, in
   return list;
 }
 
-// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile.
-template <typename T, int BITS, int W, int NT>
-__global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __grid_constant__ KeyedParams p) {
+// Eight elements of a result row: the gathered values over their sum, zeros for a query before the first key.
+template <typename T>
+__device__ __forceinline__ void write_result(const KeyedParams& p, int batch, int kv_head, int row, int column, int length, float total, const float (&value)[8]) {
+  const int token = row / p.group, head = kv_head * p.group + row % p.group;
+  const bool sees_some = length - p.q_tokens + token >= 0;
+  T* to = static_cast<T*>(p.out) + batch * p.out_strides[0] + head * p.out_strides[1] + token * p.out_strides[2] + column;
+  const float inverse = sees_some ? 1.f / total : 0.f;
+  uint32_t word[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) word[c] = sees_some ? round_pair<T>(value[2 * c] * inverse, value[2 * c + 1] * inverse) : 0u;
+  if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) to[c] = reinterpret_cast<const T*>(word)[c];
+  }
+}
+
+// A sequence's chunks, by every query of it.
+template <int BITS, int CHUNK>
+__device__ __forceinline__ int length_of(const KeyedParams& p, int sequence) {
+  if constexpr (BITS == 16) return p.k_tokens;
+  return min(max(p.lengths[sequence], 0), p.blocks << p.page_shift);
+}
+template <int BITS, int CHUNK>
+__device__ __forceinline__ ChunkList sequence_chunks(const KeyedParams& p, int length) {
+  return chunks_of(length - p.q_tokens, max(length - 1, -1), p.window, p.sinks, CHUNK);
+}
+
+// Where the chunks of all units (sequence, key head, tile of rows) are dealt out as one range of equal shares, a CTA each: a place in that range.
+struct Place {
+  int sequence;
+  int before;      // places of the sequences before it
+};
+
+// The chunks that a head of sequence `sequence` counts for: one at least, so that each has somebody to write its result.
+template <int BITS, int CHUNK>
+__device__ __forceinline__ int counted(const KeyedParams& p, int sequence) {
+  return max(sequence_chunks<BITS, CHUNK>(p, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
+}
+
+// What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another.
+constexpr int kUnitCost = 2;
+constexpr int kLeastShare = 4;       // of the same
+
+// The range has less than 2^31 places (plan_shape sees to it). The first `longer` shares have one place more than the others.
+struct Dealt {
+  int total, shares, each, longer;
+  __device__ int start(int share) const { return share * each + min(share, longer); }
+  // the share that has place `at` of the range
+  __device__ int holder(int at) const {
+    const int border = longer * (each + 1);
+    return at < border ? at / (each + 1) : longer + (at - border) / each;
+  }
+};
+
+// All threads: the range, and where in it the share of each warp, first_share + warp, starts. Each thread adds up a run of sequences.
+template <int BITS, int CHUNK>
+__device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Place& place) {
+  __shared__ int warp_sum_of[kKeyedWarps];
+  __shared__ Place found[kKeyedWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int units = p.kv_heads * p.row_tiles;
+  const int run = (p.batch + kKeyedThreads - 1) / kKeyedThreads;
+  const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
+  int mine = 0;
+  for (int b = first; b < last; ++b) mine += kUnitCost + counted<BITS, CHUNK>(p, b);
+  mine *= units;
+  int upto = mine;
+#pragma unroll
+  for (int offset = 1; offset < 32; offset *= 2) {
+    const int other = __shfl_up_sync(0xffffffffu, upto, offset);
+    if (lane >= offset) upto += other;
+  }
+  if (lane == 31) warp_sum_of[warp] = upto;
+  __syncthreads();
+  Dealt dealt;
+  dealt.total = 0;
+#pragma unroll
+  for (int w = 0; w < kKeyedWarps; ++w) {
+    if (w < warp) upto += warp_sum_of[w];
+    dealt.total += warp_sum_of[w];
+  }
+  dealt.shares = min(p.shares, (dealt.total + kLeastShare - 1) / kLeastShare);
+  dealt.each = dealt.total / dealt.shares;
+  dealt.longer = dealt.total % dealt.shares;
+#pragma unroll
+  for (int w = 0; w < kKeyedWarps; ++w) {
+    if (first_share + w >= dealt.shares) break;
+    const int at = dealt.start(first_share + w);
+    int before = upto - mine;
+    if (before <= at && at < upto) {
+      int b = first;
+      for (; b < last; ++b) {
+        const int here = (kUnitCost + counted<BITS, CHUNK>(p, b)) * units;
+        if (at < before + here) break;
+        before += here;
+      }
+      found[w] = {b, before};
+    }
+  }
+  __syncthreads();
+  place = found[warp];
+  return dealt;
+}
+
+// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. SHARED: the chunks of all units are dealt out in equal shares, one a warp (then
+// keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory.
+template <typename T, int BITS, int W, int NT, bool SHARED>
+__global__ void __launch_bounds__(kKeyedThreads, NT == 1 ? KCTAS : 2)
+keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
   using M = std::conditional_t<BITS == 8, __half, T>;      // what the matrix instructions take
   constexpr bool kTwoOperands = std::is_same_v<M, __nv_bfloat16>;
   constexpr int kRows = 8 * NT, kTiles = S::kTiles, kSlices = S::kSlices;
+  static_assert(kRows * W * sizeof(float) <= kWarpRing, "a warp leaves its part where its stages were");
+  extern __shared__ unsigned char raw_smem[];
   __shared__ float part_top[kKeyedWarps][kRows], part_sum[kKeyedWarps][kRows];
-  __shared__ __align__(16) float part_out[kKeyedWarps][kRows][W];
+  __shared__ __align__(8) uint64_t full[kKeyedWarps][kKeyedStages];
+  __shared__ int staged_page[kKeyedWarps][kKeyedStages][4];      // of each box of a stage; -1: not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = lane >> 2, corner = lane & 3;       // the instruction's row (or column) of eight, and the lane's place in it
-
-  const long long unit = blockIdx.x;
-  const int tile = static_cast<int>(unit % p.row_tiles);
-  const long long head_index = unit / p.row_tiles;
-  const int kv_head = static_cast<int>(head_index % p.kv_heads), batch = static_cast<int>(head_index / p.kv_heads);
-  const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group
-  const int row0 = tile * kRows;
-
-  int length = p.k_tokens;
-  if constexpr (BITS == 8) {
-    length = max(p.lengths[batch], 0);
-    if (length > p.blocks << p.page_shift) {           // the table does not go that far
-      length = p.blocks << p.page_shift;
-      if (threadIdx.x == 0) report(p.status, kKeyedLength, batch, p.lengths[batch]);
-    }
+  const uint32_t ring_all = (smem_address(raw_smem) + 1023u) & ~1023u, ring = ring_all + warp * kWarpRing;
+  unsigned char* const parts_at = raw_smem + (ring_all - smem_address(raw_smem));      // [warp][row][column] f32, a ring apart
+  const uint32_t barrier0 = smem_address(&full[warp][0]);
+  if (lane == 0) {
+    for (int st = 0; st < kKeyedStages; ++st) barrier_init(barrier0 + 8 * st, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    if (blockIdx.x == 0 && warp == 0) p.status.begin();
   }
-  const int first_token = row0 / p.group, last_token = min(row0 + kRows, rows) - 1 < 0 ? 0 : (min(row0 + kRows, rows) - 1) / p.group;
-  const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
-  const ChunkList list = chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys);
+  __syncwarp();
+  uint32_t turn = 0;                                   // chunks this warp has waited for: the stage and the phase of the next
+  const int quad = lane >> 2, corner = lane & 3;       // the instruction's row (or column) of eight, and the lane's place in it
+  const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group
 
+  // SHARED: this warp's share of the range, [at, until)
+  constexpr int kStep = SHARED ? 1 : kKeyedWarps;      // a warp takes every chunk of its share, or every fourth of the unit
+  const int share = static_cast<int>(blockIdx.x) * kKeyedWarps + warp;
+  Place place = {0, 0};
+  int at = 0, until = 1;
+  Dealt dealt = {};
+  if constexpr (SHARED) {
+    dealt = deal<BITS, S::kKeys>(p, blockIdx.x * kKeyedWarps, place);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel may start: it waits for this one's end itself
+    if (lane == 0) p.borders[share] = make_int4(0, 0, 0, 0);               // (the border behind this share; see below)
+    if (share >= dealt.shares) return;
+    at = dealt.start(share);
+    until = dealt.start(share + 1);
+  }
+  while (at < until) {
+  // ---- one unit, or what of it is in the share: chunks [first_chunk, last_chunk) ----
+  int batch, kv_head, tile, first_chunk = 0, last_chunk;
+  bool whole = true, begins = true;
+  int counted_length;
+  ChunkList list;
+  if constexpr (SHARED) {
+    batch = place.sequence;
+    counted_length = length_of<BITS, S::kKeys>(p, batch);
+    list = sequence_chunks<BITS, S::kKeys>(p, counted_length);
+    const int cost = kUnitCost + max(list.count(), 1), units = p.kv_heads * p.row_tiles;
+    const int inside = at - place.before;
+    const int unit = inside / cost;
+    tile = unit % p.row_tiles;
+    kv_head = unit / p.row_tiles;
+    const int from = inside - unit * cost, to = min(cost, from + (until - at));
+    first_chunk = max(from - kUnitCost, 0);
+    last_chunk = max(to - kUnitCost, 0);
+    begins = first_chunk == 0;
+    whole = begins && to == cost;
+    const int unit_start = at - from;
+    at += to - from;
+    if (last_chunk > 0 && to < cost && lane == 0) {      // the border behind this share cuts the unit: which shares have parts of it
+      const int first = dealt.holder(unit_start + kUnitCost), last = dealt.holder(unit_start + cost - 1);
+      p.borders[share] = make_int4(batch, unit, first, last);
+    }
+    if (at - place.before >= units * cost) place = {batch + 1, place.before + units * cost};
+    if (last_chunk == 0) continue;                     // a border just before its first chunk: it is the next share's
+    last_chunk = min(last_chunk, list.count());
+  } else {
+    const long long unit = blockIdx.x;
+    tile = static_cast<int>(unit % p.row_tiles);
+    const long long head_index = unit / p.row_tiles;
+    kv_head = static_cast<int>(head_index % p.kv_heads);
+    batch = static_cast<int>(head_index / p.kv_heads);
+    counted_length = length_of<BITS, S::kKeys>(p, batch);
+    at = until;
+  }
+  const int length = counted_length;
+  const int row0 = tile * kRows;
+  if constexpr (BITS == 8) {
+    if ((SHARED ? lane : threadIdx.x) == 0 && p.lengths[batch] > length) report(p.status, kKeyedLength, batch, p.lengths[batch]);      // the table does not go that far
+  }
+  const int first_token = row0 / p.group, last_token = (min(row0 + kRows, rows) - 1) / p.group;
+  const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
+  if constexpr (!SHARED) {
+    list = chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys);
+    last_chunk = list.count();
+  }
+
+  // ---- the warp's chunks ----
+  if constexpr (!SHARED) first_chunk = warp;
+  const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
+  auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
+  // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks.
+  const int boxes = BITS == 8 ? p.boxes : 1, box_shift = BITS == 8 ? p.box_shift : 31;
+  const int ahead = 32 / boxes;
+  auto look_up = [&](int n) {
+    if constexpr (BITS == 8) {
+      n += lane / boxes;
+      if (n >= mine) return -1;
+      const int key = chunk_at(n) * S::kKeys + ((lane % boxes) << box_shift);
+      if (key >= length) return -1;
+      const int at_block = key >> p.page_shift;
+      const int page = p.table[batch * p.table_stride + at_block];
+      if (page >= 0 && page < p.pages) return page;
+      report(p.status, kKeyedPage, batch, at_block);
+    }
+    return -1;
+  };
+  int page_now = look_up(0), page_next = look_up(ahead);
   // The query: row `quad` of each eight, the elements that the lane's pieces of a key hold.
-  uint32_t query[NT][S::kPieces][32 / BITS][2];      // [piece][step of 16 elements][operand word]
-  float row_scale[NT][2];                                        // of the lane's two columns: rows 2 corner and 2 corner + 1
-  int position[NT][2];
+  constexpr int kWords = S::kPieceWidth / 2;                     // of a piece's query elements: 8 or 4
+  uint32_t word[NT][S::kPieces][kWords];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = row0 + n * 8 + quad;
     const int token = row / p.group, head = kv_head * p.group + row % p.group;
     const T* from = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
-    constexpr int kWords = S::kPieceWidth / 2;                   // of a piece's query elements: 8 or 4
-    uint32_t word[S::kPieces][kWords];
-    float largest = 0.f;
 #pragma unroll
     for (int j = 0; j < S::kPieces; ++j) {
       const int column = (4 * j + corner) * S::kPieceWidth;
@@ -177,21 +399,80 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
       for (int w = 0; w < kWords; w += 4) {
         uint4 four = make_uint4(0, 0, 0, 0);
         if (row < rows && column + 2 * w < p.head_dim) four = *reinterpret_cast<const uint4*>(from + column + 2 * w);
-        word[j][w] = four.x;
-        word[j][w + 1] = four.y;
-        word[j][w + 2] = four.z;
-        word[j][w + 3] = four.w;
+        word[n][j][w] = four.x;
+        word[n][j][w + 1] = four.y;
+        word[n][j][w + 2] = four.z;
+        word[n][j][w + 3] = four.w;
       }
-      if constexpr (BITS == 8) {
+    }
+  }
+  auto fill = [&](int n, int stage) {                  // chunk n of the warp into a stage that nobody reads any more
+    const int key0 = chunk_at(n) * S::kKeys;
+    const uint32_t to = ring + stage * kStageBytes, bar = barrier0 + 8 * stage;
+    if constexpr (BITS == 8) {
+      if (n > 0 && n % ahead == 0) {
+        page_now = page_next;
+        page_next = look_up(n + ahead);
+      }
+      const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
+      const bool loads = lane < boxes && page >= 0;
+      const uint32_t box_bytes = static_cast<uint32_t>(S::kLine) << box_shift;
+      const uint32_t bytes = 2u * box_bytes * __popc(__ballot_sync(0xffffffffu, loads));
+      if (lane < boxes) staged_page[warp][stage][lane] = page;
+      if (lane == 0) barrier_expect_tx(bar, bytes);
+      __syncwarp();
+      if (loads) {
+        const int row = static_cast<int>(((static_cast<long long>(page) * p.kv_heads + kv_head) << p.page_shift) +
+                                         ((key0 + (lane << box_shift)) & ((1 << p.page_shift) - 1)));
+        tma_load_rows(to + lane * box_bytes, &map_k, bar, 0, row);
+        tma_load_rows(to + kStageBytes / 2 + lane * box_bytes, &map_v, bar, 0, row);
+      }
+    } else {
+      if (lane == 0) {
+        barrier_expect_tx(bar, kStageBytes);
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-          const float2 pair = widen_pair<T>(word[j][w]);
-          largest = fmaxf(largest, fmaxf(fabsf(pair.x), fabsf(pair.y)));
+        for (int l = 0; l < S::kLines; ++l) {
+          tma_load_tokens(to + l * S::kBoxBytes, &map_k, bar, l * 64, key0, kv_head, batch);
+          tma_load_tokens(to + kStageBytes / 2 + l * S::kBoxBytes, &map_v, bar, l * 64, key0, kv_head, batch);
         }
       }
     }
+  };
+  // Lane t holds the scales of tile t of the next chunk: they are asked for a step before they are used.
+  float k_scale_next = 0.f, v_scale_next = 0.f;
+  auto ask_scales = [&](int stage) {
+    if constexpr (BITS == 8) {
+      if (lane < kTiles) {
+        const int page = staged_page[warp][stage][(lane * 16) >> box_shift];
+        if (page >= 0) {
+          const long long block = static_cast<long long>(page) * p.kv_heads + kv_head;
+          k_scale_next = p.k_scales[block];
+          v_scale_next = p.v_scales[block];
+        }
+      }
+    }
+  };
+  for (int first = 0; first < min(mine, kKeyedStages); ++first) fill(first, (turn + first) % kKeyedStages);
+  __syncwarp();
+  if (mine > 0) ask_scales(turn % kKeyedStages);
+
+  // ... as the matrix instructions take it: [piece][step of 16 elements][operand word]
+  uint32_t query[NT][S::kPieces][32 / BITS][2];
+  float row_scale[NT][2];                                        // of the lane's two columns: rows 2 corner and 2 corner + 1
+  int position[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     float back = p.scale_log2;
     if constexpr (BITS == 8) {
+      float largest = 0.f;
+#pragma unroll
+      for (int j = 0; j < S::kPieces; ++j) {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          const float2 pair = widen_pair<T>(word[n][j][w]);
+          largest = fmaxf(largest, fmaxf(fabsf(pair.x), fabsf(pair.y)));
+        }
+      }
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
       // a power of two that brings the row's largest element to [2^14, 2^15); none for zeros and infinities
@@ -203,21 +484,21 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
       for (int j = 0; j < S::kPieces; ++j) {
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-          const float2 pair = widen_pair<T>(word[j][w]);
-          word[j][w] = round_pair<__half>(pair.x * up, pair.y * up);
+          const float2 pair = widen_pair<T>(word[n][j][w]);
+          word[n][j][w] = round_pair<__half>(pair.x * up, pair.y * up);
         }
       }
     }
 #pragma unroll
     for (int j = 0; j < S::kPieces; ++j) {
 #pragma unroll
-      for (int w = 0; w < kWords; ++w) query[n][j][w / 2][w % 2] = word[j][w];
+      for (int w = 0; w < kWords; ++w) query[n][j][w / 2][w % 2] = word[n][j][w];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * corner + e) * 4);
-      const int mine = row0 + n * 8 + 2 * corner + e;
-      position[n][e] = mine < rows ? length - p.q_tokens + mine / p.group : high;
+      const int here = row0 + n * 8 + 2 * corner + e;
+      position[n][e] = here < rows ? length - p.q_tokens + here / p.group : high;
     }
   }
 
@@ -236,86 +517,28 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
     }
   }
 
-  const int chunks = list.count();
-  for (int i = warp; i < chunks; i += kKeyedWarps) {
-    const int key0 = list.at(i) * S::kKeys;
-    // where the chunk's tiles of 16 keys lie
-    const char *k_base[kTiles], *v_base[kTiles];
-    float k_scale[kTiles], v_scale[kTiles];
-    long long k_step, v_step;                          // bytes from a key to the next
+  for (int step = 0; step < mine; ++step, ++turn) {
+    const int key0 = chunk_at(step) * S::kKeys;
+    const int stage = turn % kKeyedStages;
+    if (!barrier_wait(barrier0 + 8 * stage, (turn / kKeyedStages) & 1, p.status, kWaitKeyed)) {
+      // the result is lost (the status says so); the copies that are under way still have to land before the stages are used otherwise
+      for (int m = step; m < min(step + kKeyedStages, mine); ++m, ++turn) {
+        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(barrier0 + 8 * (turn % kKeyedStages), (turn / kKeyedStages) & 1); ++spin) {
+        }
+      }
+      break;
+    }
+    const uint32_t k_at = ring + stage * kStageBytes, v_at = k_at + kStageBytes / 2;
     int stop = length;                                 // keys from here on are not there
+    float k_scale[kTiles], v_scale[kTiles];
     if constexpr (BITS == 8) {
-      k_step = v_step = p.head_dim;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const int key = key0 + t * 16;
-        k_base[t] = v_base[t] = nullptr;
-        k_scale[t] = v_scale[t] = 0.f;
-        if (key < stop) {
-          const int page = p.table[batch * p.table_stride + (key >> p.page_shift)];
-          if (page < 0 || page >= p.pages) {
-            if (lane == 0) report(p.status, kKeyedPage, batch, key >> p.page_shift);
-            stop = key;
-          } else {
-            const long long block = static_cast<long long>(page) * p.kv_heads + kv_head;
-            const long long offset = ((block << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * p.head_dim;
-            k_base[t] = static_cast<const char*>(p.k) + offset;
-            v_base[t] = static_cast<const char*>(p.v) + offset;
-            k_scale[t] = p.k_scales[block];
-            v_scale[t] = p.v_scales[block];
-          }
-        }
+      for (int t = kTiles - 1; t >= 0; --t) {
+        k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
+        v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
+        if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
       }
-    } else {
-      k_step = p.k_strides[2] * 2;
-      v_step = p.v_strides[2] * 2;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const long long key = key0 + t * 16;
-        k_base[t] = static_cast<const char*>(p.k) + (batch * p.k_strides[0] + kv_head * p.k_strides[1] + key * p.k_strides[2]) * 2;
-        v_base[t] = static_cast<const char*>(p.v) + (batch * p.v_strides[0] + kv_head * p.v_strides[1] + key * p.v_strides[2]) * 2;
-      }
-    }
-    uint4 key_piece[kTiles][2][S::kPieces];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int inside = quad + 8 * h;
-#pragma unroll
-        for (int j = 0; j < S::kPieces; ++j) {
-          const int column = (4 * j + corner) * S::kPieceWidth;
-          key_piece[t][h][j] = make_uint4(0, 0, 0, 0);
-          if (column < p.head_dim && key0 + t * 16 + inside < stop) key_piece[t][h][j] = load_piece(k_base[t] + inside * k_step + column * BITS / 8);
-        }
-      }
-    }
-    uint32_t value[kTiles][4][S::kValueWords];         // keys 2 corner, 2 corner + 1, and those 8 further on
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int inside = 2 * corner + (r & 1) + 8 * (r >> 1);
-        const bool there = key0 + t * 16 + inside < stop;
-        const char* from = v_base[t] + inside * v_step;
-        if constexpr (S::kValueWords == 2) {
-          uint2 word = make_uint2(0, 0);
-          if (there && quad * 8 < p.head_dim) word = load_half_piece(from + quad * 8);
-          value[t][r][0] = word.x;
-          value[t][r][1] = word.y;
-        } else {
-#pragma unroll
-          for (int w = 0; w < S::kValueWords; w += 4) {
-            const int column = (w / 4) * 64 + quad * S::kPieceWidth;
-            uint4 word = make_uint4(0, 0, 0, 0);
-            if (there && column < p.head_dim) word = load_piece(from + column * BITS / 8);
-            value[t][r][w] = word.x;
-            value[t][r][w + 1] = word.y;
-            value[t][r][w + 2] = word.z;
-            value[t][r][w + 3] = word.w;
-          }
-        }
-      }
+      if (step + 1 < mine) ask_scales((turn + 1) % kKeyedStages);
     }
 
     // S^T: keys quad and quad + 8 of each tile by rows 2 corner and 2 corner + 1
@@ -326,8 +549,9 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
       for (int n = 0; n < NT; ++n) score[t][n][0] = score[t][n][1] = score[t][n][2] = score[t][n][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < S::kPieces; ++j) {
-        const uint32_t a[4] = {key_piece[t][0][j].x, key_piece[t][0][j].y, key_piece[t][0][j].z, key_piece[t][0][j].w};
-        const uint32_t b[4] = {key_piece[t][1][j].x, key_piece[t][1][j].y, key_piece[t][1][j].z, key_piece[t][1][j].w};
+        const uint4 near = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
+        const uint4 far = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
+        const uint32_t a[4] = {near.x, near.y, near.z, near.w}, b[4] = {far.x, far.y, far.z, far.w};
         if constexpr (BITS == 8) {
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
@@ -350,13 +574,14 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
     const int last = key0 + S::kKeys - 1;
     const bool open = last <= low && last < stop && (key0 > high - p.window || last < p.sinks);
     auto sees = [&](int at, int key) { return key <= at && key < stop && (key > at - p.window || key < p.sinks); };
-    float factor[NT][2];
-    bool moved = false;
+    // Any reference point gives the same softmax: a row's moves only when a score lies more than 2^kSlack above it, which one vote tells.
+    float most[NT][2];
+    bool rises = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float most = -INFINITY;
+        most[n][e] = -INFINITY;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           const float by = BITS == 8 ? row_scale[n][e] * k_scale[t] : row_scale[n][e];
@@ -365,37 +590,46 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
             float& s = score[t][n][2 * h + e];
             s *= by;
             if (!open && !sees(position[n][e], key0 + t * 16 + quad + 8 * h)) s = -INFINITY;
-            most = fmaxf(most, s);
+            most[n][e] = fmaxf(most[n][e], s);
           }
         }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-        most = fmaxf(most, top[n][e]);
-        factor[n][e] = rescale(top[n][e], most);
-        moved |= factor[n][e] != 1.f;
-        top[n][e] = most;
-        const float reference = most == -INFINITY ? 0.f : most;
-        float gained = 0.f;
+        rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
+      }
+    }
+    if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float now = most[n][e];
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+          now = fmaxf(now, top[n][e]);
+          const float factor = rescale(top[n][e], now);
+          top[n][e] = now;
+          sum[n][e] *= factor;
+#pragma unroll
+          for (int s = 0; s < kSlices; ++s) {
+            result[n][s][e] *= factor;
+            result[n][s][2 + e] *= factor;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float reference = top[n][e] == -INFINITY ? 0.f : top[n][e];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float& s = score[t][n][2 * h + e];
             s = exp2_ftz(s - reference);
-            gained += s;
+            sum[n][e] += s;
           }
-        }
-        sum[n][e] = sum[n][e] * factor[n][e] + gained;
-      }
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int s = 0; s < kSlices; ++s) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) result[n][s][e] *= factor[n][e & 1];
         }
       }
     }
@@ -419,13 +653,56 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
       }
     }
 
+    // (of the lane's part of a tile: no NaN, and no infinity in 16 bits)
+    auto values_are_numbers = [&](int t) {
+      bool fine = true;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+        for (int w = 0; w < S::kValueWords; w += 2) {
+          const uint2 two = load_shared_8(v_at + S::at(key, S::kValueWords == 2 ? quad * 8 : ((w / 4) * 8 + quad) * 16 + (w % 4) * 4));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t word = h == 0 ? two.x : two.y;
+            if constexpr (BITS == 8) {
+              fine &= (((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0;
+            } else {
+              constexpr uint32_t kExponent = std::is_same_v<M, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+              fine &= (word & kExponent) != kExponent && (word >> 16 & kExponent) != kExponent;
+            }
+          }
+        }
+      }
+      return fine;
+    };
     // O^T += V^T P^T of one tile of keys, for the rows of token `only` (all rows: -1) and the keys that `kept` has (a bit for each of the lane's four)
-    auto add_product = [&](int t, uint32_t kept, int only) {
+    auto add_product = [&](int t, uint32_t kept, int only, auto direct) {
+      constexpr bool kDirect = decltype(direct)::value;      // every row adds, and nothing scales what it adds
+      uint32_t value[4][S::kValueWords];               // keys 2 corner, 2 corner + 1, and those 8 further on
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1);
+        if constexpr (S::kValueWords == 2) {
+          const uint2 word = load_shared_8(v_at + S::at(key, quad * 8));
+          value[r][0] = word.x;
+          value[r][1] = word.y;
+        } else {
+#pragma unroll
+          for (int w = 0; w < S::kValueWords; w += 4) {
+            const uint4 word = load_shared_16(v_at + S::at(key, ((w / 4) * 8 + quad) * 16));
+            value[r][w] = word.x;
+            value[r][w + 1] = word.y;
+            value[r][w + 2] = word.z;
+            value[r][w + 3] = word.w;
+          }
+        }
+      }
 #pragma unroll
       for (int w = 0; w < S::kValueWords; ++w) {
         uint32_t v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = value[t][r][w] & (kept >> r & 1 ? 0xffffffffu : 0u);
+        for (int r = 0; r < 4; ++r) v[r] = value[r][w] & (kept >> r & 1 ? 0xffffffffu : 0u);
 #pragma unroll
         for (int half = 0; half < (BITS == 8 ? 2 : 1); ++half) {
           uint32_t a0, a1, a2, a3;
@@ -444,7 +721,7 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
           const int slice = BITS == 8 ? 2 * w + half : w;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            if (BITS == 16 && only < 0) {
+            if (BITS == 16 && kDirect) {
               multiply<M>(result[n][slice], a0, a1, a2, a3, weight[t][n][0], weight[t][n][1]);
               if constexpr (kTwoOperands) multiply<M>(result[n][slice], a0, a1, a2, a3, rest[t][n][0], rest[t][n][1]);
             } else {
@@ -463,94 +740,321 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_attention_kernel(const __
     };
     if (open) {
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) add_product(t, 15u, -1);
+      for (int t = 0; t < kTiles; ++t) add_product(t, 15u, -1, std::true_type{});
     } else {
-#pragma unroll 1
-      for (int at = low; at <= high; ++at) {
+      // Where several queries see different keys: if all of the tile's values are numbers, a probability of zero is all a mask needs.
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+      for (int t = 0; t < kTiles; ++t) {
+        auto kept_of = [&](int at) {
           uint32_t kept = 0;
 #pragma unroll
           for (int r = 0; r < 4; ++r) kept |= (sees(at, key0 + t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1)) ? 1u : 0u) << r;
-          if (__any_sync(0xffffffffu, kept != 0)) add_product(t, kept, at);
+          return kept;
+        };
+        uint32_t some = 0;
+#pragma unroll 1
+        for (int at = low; at <= high; ++at) some |= kept_of(at);
+        if (!__any_sync(0xffffffffu, some != 0)) continue;
+        const bool once = low == high || __all_sync(0xffffffffu, values_are_numbers(t));
+#pragma unroll 1
+        for (int at = low; at <= high; ++at) {
+          add_product(t, low == high ? some : once ? 15u : kept_of(at), once ? -1 : at, std::false_type{});
+          if (once) break;
         }
       }
     }
+    __syncwarp();                                      // the stage has been read
+    if (step + kKeyedStages < mine) fill(step + kKeyedStages, stage);
   }
 
-  // The warps meet in shared memory.
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int offset = 4; offset < 32; offset *= 2) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], offset);
-      const int row = n * 8 + 2 * corner + e;
-      if (quad == 0) {
-        part_top[warp][row] = top[n][e];
-        part_sum[warp][row] = sum[n][e];
-      }
-#pragma unroll
-      for (int s = 0; s < kSlices; ++s) {
-        const int column = BITS == 8 ? quad * (W / 8) + 2 * s : (s / 4) * 64 + quad * 8 + 2 * (s % 4);
-        *reinterpret_cast<float2*>(&part_out[warp][row][column]) = make_float2(result[n][s][e], result[n][s][2 + e]);
-      }
     }
   }
-  __syncthreads();
-  for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
+  // A lane has, of its rows, runs of eight neighbouring elements.
+  constexpr int kRuns = kSlices / 4;
+  auto column_of = [&](int run) { return BITS == 8 ? quad * (W / 8) + 8 * run : run * 64 + quad * 8; };
+  auto run_of = [&](int n, int e, int run, float (&value)[8]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      value[2 * c] = result[n][4 * run + c][e];
+      value[2 * c + 1] = result[n][4 * run + c][2 + e];
+    }
+  };
+  if constexpr (SHARED) {
+    const long long slot0 = (2LL * share + (begins ? 1 : 0)) * kRows;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = n * 8 + 2 * corner + e;
+        if (row0 + row >= rows) continue;
+        if (!whole && quad == 0) p.part_stats[slot0 + row] = make_float2(top[n][e], sum[n][e]);
+#pragma unroll
+        for (int run = 0; run < kRuns; ++run) {
+          float value[8];
+          run_of(n, e, run, value);
+          const int column = column_of(run);
+          if (column >= p.head_dim) continue;
+          if (whole) {
+            write_result<T>(p, batch, kv_head, row0 + row, column, length, sum[n][e], value);
+          } else {
+            float4* to = reinterpret_cast<float4*>(p.parts + (slot0 + row) * W + column);
+            to[0] = make_float4(value[0], value[1], value[2], value[3]);
+            to[1] = make_float4(value[4], value[5], value[6], value[7]);
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = n * 8 + 2 * corner + e;
+        if (quad == 0) {
+          part_top[warp][row] = top[n][e];
+          part_sum[warp][row] = sum[n][e];
+        }
+#pragma unroll
+        for (int run = 0; run < kRuns; ++run) {
+          float value[8];
+          run_of(n, e, run, value);
+          float4* to = reinterpret_cast<float4*>(parts_at + warp * kWarpRing + (row * W + column_of(run)) * 4);
+          to[0] = make_float4(value[0], value[1], value[2], value[3]);
+          to[1] = make_float4(value[4], value[5], value[6], value[7]);
+        }
+      }
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
+      const int row = item / (W / 8), column = item % (W / 8) * 8;
+      if (row0 + row >= rows || column >= p.head_dim) continue;
+      float most = part_top[0][row];
+#pragma unroll
+      for (int w = 1; w < kKeyedWarps; ++w) most = fmaxf(most, part_top[w][row]);
+      float total = 0.f, value[8] = {};
+#pragma unroll
+      for (int w = 0; w < kKeyedWarps; ++w) {
+        const float by = rescale(part_top[w][row], most);
+        total += part_sum[w][row] * by;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
+      }
+      write_result<T>(p, batch, kv_head, row0 + row, column, length, total, value);
+    }
+  }
+  }
+}
+
+// SHARED: joins the parts of the units that a border between two shares cut. A CTA for each border; the CTAs of a unit's borders split its result.
+template <typename T, int W, int NT>
+__global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_constant__ KeyedParams p) {
+  constexpr int kRows = 8 * NT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // by every CTA: whoever comes after this kernel comes after the one before it too
+  const int share = static_cast<int>(blockIdx.x);         // the border lies behind it
+  const int4 border = p.borders[share];
+  const int batch = border.x, unit = border.y, first = border.z, last = border.w;
+  if (first == last) return;                              // it lies between two units
+  const int tile = unit % p.row_tiles, kv_head = unit / p.row_tiles;
+  const int rows = min(kRows, p.group * p.q_tokens - tile * kRows);
+  for (int item = (share - first) * kKeyedThreads + threadIdx.x; item < rows * (W / 8); item += (last - first) * kKeyedThreads) {
     const int row = item / (W / 8), column = item % (W / 8) * 8;
-    const int mine = row0 + row;
-    if (mine >= rows || column >= p.head_dim) continue;
-    float most = part_top[0][row];
+    if (column >= p.head_dim) continue;
+    float most = -INFINITY, total = 0.f, value[8] = {};
+    for (int from = first; from <= last; from += 4) {
+      float2 stats[4];
+      float4 part[4][2];
 #pragma unroll
-    for (int w = 1; w < kKeyedWarps; ++w) most = fmaxf(most, part_top[w][row]);
-    float total = 0.f, value[8] = {};
+      for (int u = 0; u < 4; ++u) {
+        const long long slot = (2LL * (from + u) + (from + u == first ? 1 : 0)) * kRows + row;
+        stats[u] = make_float2(-INFINITY, 0.f);
+        part[u][0] = part[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (from + u <= last) {
+          stats[u] = p.part_stats[slot];
+          const float4* at = reinterpret_cast<const float4*>(p.parts + slot * W + column);
+          part[u][0] = at[0];
+          part[u][1] = at[1];
+        }
+      }
+      const float before = most;
 #pragma unroll
-    for (int w = 0; w < kKeyedWarps; ++w) {
-      const float by = rescale(part_top[w][row], most);
-      total += part_sum[w][row] * by;
+      for (int u = 0; u < 4; ++u) most = fmaxf(most, stats[u].x);
+      const float kept = rescale(before, most);
+      total *= kept;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) value[c] += part_out[w][row][column + c] * by;
+      for (int c = 0; c < 8; ++c) value[c] *= kept;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float by = rescale(stats[u].x, most);
+        const float x[8] = {part[u][0].x, part[u][0].y, part[u][0].z, part[u][0].w, part[u][1].x, part[u][1].y, part[u][1].z, part[u][1].w};
+        total += stats[u].y * by;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) value[c] = fmaf(x[c], by, value[c]);
+      }
     }
-    const int token = mine / p.group, head = kv_head * p.group + mine % p.group;
-    const bool sees_some = length - p.q_tokens + token >= 0;
-    T* to = static_cast<T*>(p.out) + batch * p.out_strides[0] + head * p.out_strides[1] + token * p.out_strides[2] + column;
-    const float inverse = sees_some ? 1.f / total : 0.f;
-    uint32_t word[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) word[c] = sees_some ? round_pair<T>(value[2 * c] * inverse, value[2 * c + 1] * inverse) : 0u;
-    if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-      *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
+    const int length = p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
+    write_result<T>(p, batch, kv_head, tile * kRows + row, column, length, total, value);
+  }
+}
+
+// How many CTAs of a kernel run at once on `device`, asked once for each.
+template <auto kKernel>
+int resident(int32_t device) {
+  static std::mutex mutex;
+  static int known[64] = {};
+  if (device < 0 || device >= 64) return 2 * 148;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (known[device] == 0) {
+    int per_sm = 0;
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, kKeyedThreads, kKeyedSmem) != cudaSuccess || per_sm <= 0) {
+      cudaGetLastError();
+      per_sm = 2;
+    }
+    known[device] = per_sm * sm_count(device);
+  }
+  return known[device];
+}
+
+// The most chunks a unit can have: all its keys, or what a window and the sinks leave.
+long long most_chunks(const KeyedParams& p, long long keys, int chunk) {
+  const long long all = (keys + chunk - 1) / chunk;
+  const long long seen = (p.sinks + chunk - 1LL) / chunk + (p.window + p.q_tokens + chunk - 2LL) / chunk + 1;
+  return all < seen ? all : seen;
+}
+
+// A unit of so few chunks is a CTA's (two steps of its warps); of more, chunks are dealt out.
+constexpr int kWholeChunks = 2 * kKeyedWarps;
+
+struct KeyedPlan {
+  int nt, row_tiles, shares;      // shares 0: a CTA a unit
+  size_t bytes;
+};
+
+template <int BITS, int W>
+KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
+  KeyedPlan plan = {};
+  const int rows = p.group * p.q_tokens;
+  plan.nt = rows <= 8 ? 1 : 2;
+  plan.row_tiles = (rows + 8 * plan.nt - 1) / (8 * plan.nt);
+  const long long chunks = most_chunks(p, keys, KeyedShape<BITS, W>::kKeys);
+  const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
+  if (chunks > kWholeChunks && (chunks + kUnitCost) * units < (1LL << 31)) {
+    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, true>>(device)
+                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, true>>(device);
+    plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
+    plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
+  }
+  return plan;
+}
+
+KeyedPlan plan_keyed(bool paged, const KeyedParams& p, long long keys, int32_t device) {
+  if (paged) return p.head_dim <= 64 ? plan_shape<8, 64>(p, keys, device) : plan_shape<8, 128>(p, keys, device);
+  return p.head_dim <= 64 ? plan_shape<16, 64>(p, keys, device) : plan_shape<16, 128>(p, keys, device);
+}
+
+tq_status keyed_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* pointer, const cuuint64_t* dims, const cuuint64_t* byte_strides,
+                    const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  EncodeTiled encode = encode_tiled();
+  TQ_REQUIRE(encode != nullptr, TQ_EXTERNAL, "the CUDA driver does not provide cuTensorMapEncodeTiled");
+  const cuuint32_t element_strides[4] = {1, 1, 1, 1};
+  const CUresult result = encode(map, type, rank, const_cast<void*>(pointer), dims, byte_strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TQ_REQUIRE(result == CUDA_SUCCESS, TQ_UNSUPPORTED, "this operand layout cannot be described to TMA (driver code %d)", static_cast<int>(result));
+  return TQ_OK;
+}
+
+// Maps of the keys and of the values: rows of a page and head, or [batch, head, token] through the caller's strides. What a row has less than W
+// elements, and rows behind the last token, arrive as zeros.
+template <typename T, int BITS, int W>
+tq_status keyed_maps(CUtensorMap* maps, KeyedParams& p) {
+  using S = KeyedShape<BITS, W>;
+  const CUtensorMapSwizzle swizzle = S::kLine == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const void* operands[2] = {p.k, p.v};
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (BITS == 8) {
+      const int box_rows = 1 << p.page_shift < S::kKeys ? 1 << p.page_shift : S::kKeys;
+      p.boxes = S::kKeys / box_rows;
+      p.box_shift = 31 - __builtin_clz(static_cast<unsigned>(box_rows));
+      if (p.pages == 0) continue;
+      const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.head_dim), (static_cast<cuuint64_t>(p.pages) * p.kv_heads) << p.page_shift};
+      const cuuint64_t byte_strides[1] = {static_cast<cuuint64_t>(p.head_dim)};
+      const cuuint32_t box[2] = {static_cast<cuuint32_t>(W), static_cast<cuuint32_t>(box_rows)};
+      TQ_REQUIRE(dims[1] < (1ull << 31), TQ_UNSUPPORTED, "a pool of more than 2^31 tokens and heads");
+      if (tq_status s = keyed_map(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, operands[i], dims, byte_strides, box, swizzle)) return s;
     } else {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) to[c] = reinterpret_cast<const T*>(word)[c];
+      if (p.k_tokens == 0) continue;
+      const long long* strides = i == 0 ? p.k_strides : p.v_strides;
+      const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(p.k_tokens), static_cast<cuuint64_t>(p.kv_heads),
+                                  static_cast<cuuint64_t>(p.batch)};
+      // an axis of extent 1 never moves, so its stride only has to be legal
+      const cuuint64_t byte_strides[3] = {static_cast<cuuint64_t>(p.k_tokens > 1 ? strides[2] : p.head_dim) * 2,
+                                          static_cast<cuuint64_t>(p.kv_heads > 1 ? strides[1] : p.head_dim) * 2,
+                                          static_cast<cuuint64_t>(p.batch > 1 ? strides[0] : p.head_dim) * 2};
+      const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(S::kKeys), 1, 1};
+      const CUtensorMapDataType type = std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      if (tq_status s = keyed_map(&maps[i], type, 4, operands[i], dims, byte_strides, box, swizzle)) return s;
     }
   }
+  return TQ_OK;
 }
 
 template <typename T, int BITS, int W, int NT>
-tq_status launch_keyed(const KeyedParams& p, cudaStream_t stream) {
-  const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles;
-  TQ_REQUIRE(units < (1LL << 31), TQ_UNSUPPORTED, "too many heads and rows for one launch");
-  keyed_attention_kernel<T, BITS, W, NT><<<static_cast<unsigned>(units), kKeyedThreads, 0, stream>>>(p);
-  return check_launch("keyed_attention_kernel");
+tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
+  CUtensorMap maps[2] = {};
+  if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
+  TQ_CUDA(cudaFuncSetAttribute(p.shares == 0 ? keyed_attention_kernel<T, BITS, W, NT, false> : keyed_attention_kernel<T, BITS, W, NT, true>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)));
+  if (p.shares == 0) {
+    const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles;
+    TQ_REQUIRE(units < (1LL << 31), TQ_UNSUPPORTED, "too many heads and rows for one launch");
+    keyed_attention_kernel<T, BITS, W, NT, false><<<static_cast<unsigned>(units), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
+    return check_launch("keyed_attention_kernel");
+  }
+  keyed_attention_kernel<T, BITS, W, NT, true><<<static_cast<unsigned>(p.shares / kKeyedWarps), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
+  if (tq_status s = check_launch("keyed_attention_kernel")) return s;
+  // The second kernel's start passes under the first one's end (it waits for all of it before it reads the parts).
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(p.shares - 1));
+  config.blockDim = dim3(kKeyedThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  TQ_CUDA(cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT>, p));
+  return check_launch("keyed_join_kernel");
 }
 
 template <typename T, int BITS>
-tq_status launch_keyed_width(KeyedParams& p, cudaStream_t stream) {
-  const int rows = p.group * p.q_tokens;
-  const int nt = rows <= 8 ? 1 : 2;
-  p.row_tiles = (rows + 8 * nt - 1) / (8 * nt);
+tq_status launch_keyed_width(KeyedParams& p, int nt, cudaStream_t stream) {
   if (p.head_dim <= 64) return nt == 1 ? launch_keyed<T, BITS, 64, 1>(p, stream) : launch_keyed<T, BITS, 64, 2>(p, stream);
   return nt == 1 ? launch_keyed<T, BITS, 128, 1>(p, stream) : launch_keyed<T, BITS, 128, 2>(p, stream);
 }
 
 }  // namespace
 
-tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, cudaStream_t stream) {
-  if (dtype == TQ_BF16) return paged ? launch_keyed_width<__nv_bfloat16, 8>(p, stream) : launch_keyed_width<__nv_bfloat16, 16>(p, stream);
-  return paged ? launch_keyed_width<__half, 8>(p, stream) : launch_keyed_width<__half, 16>(p, stream);
+size_t keyed_workspace(bool paged, const KeyedParams& p, long long keys, int32_t device) { return plan_keyed(paged, p, keys, device).bytes; }
+
+tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long keys, void* workspace, size_t workspace_bytes, int32_t device,
+                          cudaStream_t stream) {
+  const KeyedPlan plan = plan_keyed(paged, p, keys, device);
+  TQ_REQUIRE(plan.bytes == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes && aligned_to(workspace, 16)), TQ_INVALID_ARGUMENT,
+             "this attention needs %zu bytes of workspace, 16-byte aligned, and was given %zu", plan.bytes, workspace_bytes);
+  p.row_tiles = plan.row_tiles;
+  p.shares = plan.shares;
+  const size_t slots = 2ull * plan.shares * 8 * plan.nt;
+  p.borders = static_cast<int4*>(workspace);
+  p.part_stats = reinterpret_cast<float2*>(p.borders + plan.shares);
+  p.parts = reinterpret_cast<float*>(p.part_stats + slots);
+  if (dtype == TQ_BF16) return paged ? launch_keyed_width<__nv_bfloat16, 8>(p, plan.nt, stream) : launch_keyed_width<__nv_bfloat16, 16>(p, plan.nt, stream);
+  return paged ? launch_keyed_width<__half, 8>(p, plan.nt, stream) : launch_keyed_width<__half, 16>(p, plan.nt, stream);
 }
 
 }  // namespace tq

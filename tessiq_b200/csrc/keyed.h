@@ -16,9 +16,13 @@ struct KeyedParams {
   const int32_t *table, *lengths;
   long long table_stride;
   int blocks, page_shift, pages;
+  int boxes, box_shift;                                                    // of a chunk: its pieces of a page, and log2 of their tokens
   int batch, heads, kv_heads, group, q_tokens, k_tokens, head_dim;
   int window, sinks;
-  int row_tiles;
+  int row_tiles, shares;
+  float* parts;                                                            // of units that a border between two shares cuts
+  int4* borders;                                                           // the border behind each share: {sequence, unit, first and last share with parts of it}, none where these are equal
+  float2* part_stats;                                                      // ... their maximum and sum
   float scale_log2;
   WaitStatus status;
 };
@@ -45,8 +49,10 @@ inline void keyed_extents(KeyedParams& p, int64_t batch, int64_t heads, int64_t 
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
 }
 
-// Few rows a key head against many keys; `p` is complete but for row_tiles.
-tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, cudaStream_t stream);
+// Few rows a key head against many keys: `p` is complete but for what follows from the plan; no sequence has more than `keys` keys.
+size_t keyed_workspace(bool paged, const KeyedParams& p, long long keys, int32_t device);
+tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long keys, void* workspace, size_t workspace_bytes, int32_t device,
+                          cudaStream_t stream);
 
 #ifdef __CUDACC__
 // The first fault since the last poll is kept, with where it was.
