@@ -36,7 +36,7 @@
 
 namespace {
 
-enum Family { kFused, kReduce, kPack, kSoftmax, kLayerNorm, kTransposed, kBatchNorm, kGemm, kAttention };
+enum Family { kFused, kReduce, kPack, kSoftmax, kLayerNorm, kTransposed, kBatchNorm, kGemm, kAttention, kWindow, kCacheAttention, kCacheStore, kFamilies };
 
 // The library's entry points.
 struct Library {
@@ -50,6 +50,10 @@ struct Library {
   decltype(&tq_batch_norm_eval_launch) batch_norm_eval_launch = nullptr;
   decltype(&tq_gemm_bias_act_residual_launch) gemm_bias_act_residual_launch = nullptr;
   decltype(&tq_attention_launch) attention_launch = nullptr;
+  decltype(&tq_window_attention_launch) window_attention_launch = nullptr;
+  decltype(&tq_cache_attention_launch) cache_attention_launch = nullptr;
+  decltype(&tq_cache_store_launch) cache_store_launch = nullptr;
+  decltype(&tq_copy_pages_launch) copy_pages_launch = nullptr;
 } library;
 
 template <typename Function>
@@ -263,6 +267,23 @@ tq_status launch(const Plan& p, const Call& call, const std::vector<at::Tensor>&
     case kAttention:
       return library.attention_launch(small(0), pointer(0), pointer(1), pointer(2), result(0), n[1], n[2], n[3], n[4], n[5], n + 6, n + 9, n + 12, n + 15,
                                  p.doubles[0], small(18), device, stream);
+    case kWindow:
+      return library.window_attention_launch(small(0), pointer(0), pointer(1), pointer(2), result(0), n[1], n[2], n[3], n[4], n[5], n[6], n + 7, n + 10, n + 13,
+                                        n + 16, p.doubles[0], n[19], n[20], scratch, scratch_bytes, device, stream);
+    case kCacheAttention:
+      return library.cache_attention_launch(small(0), pointer(0), pointer(1), pointer(2), static_cast<const float*>(pointer(3)),
+                                       static_cast<const float*>(pointer(4)), static_cast<const int32_t*>(pointer(5)), static_cast<const int32_t*>(pointer(6)),
+                                       result(0), n[1], n[2], n[3], n[4], n[5], n[6], n[7], n[8], n[9], n + 10, n + 13, p.doubles[0], n[16], n[17], scratch,
+                                       scratch_bytes, device, stream);
+    case kCacheStore: {
+      // (the cache's tensors are written: what they hold is theirs whatever the key says)
+      auto written = [&](int i) { return const_cast<void*>(pointer(i)); };
+      return library.cache_store_launch(small(0), pointer(0), pointer(1), written(2), written(3), static_cast<float*>(written(4)), static_cast<float*>(written(5)),
+                                   static_cast<const int32_t*>(pointer(6)), static_cast<const int32_t*>(pointer(7)), static_cast<const int32_t*>(pointer(8)), n[1],
+                                   n[2], n[3], n[4], n[5], n[6], n[7], n[8], n + 9, n + 12, device, stream);
+    }
+    case kFamilies:
+      break;
   }
   return TQ_INTERNAL;
 }
@@ -298,12 +319,21 @@ PyObject* run(PyObject* const* values, Py_ssize_t count, bool by_type) {
     pybind11::gil_scoped_release unlocked;
     const c10::Device device(c10::kCUDA, static_cast<c10::DeviceIndex>(call.device));
     out.reserve(plan->outputs.size());
+    // scratch of the call's own, so that calls on other streams and captured graphs never share it; torch's allocator orders its reuse
+    const int64_t own = plan->family == kWindow ? plan->ints[21] : plan->family == kCacheAttention ? plan->ints[18] : 0;
+    at::Tensor own_scratch;
+    if (own > 0) {
+      own_scratch = at::detail::empty_cuda({own}, at::kByte, device, std::nullopt);
+      scratch = own_scratch.mutable_data_ptr();
+      scratch_bytes = static_cast<size_t>(own);
+    }
     for (const Output& o : plan->outputs)
       out.push_back(o.packed ? at::detail::empty_cuda(o.sizes, o.dtype, device, std::nullopt)
                              : at::detail::empty_strided_cuda(o.sizes, o.strides, o.dtype, device));
     status = launch(*plan, call, out, scratch, scratch_bytes, stream);
   }
   if (status != TQ_OK) Py_RETURN_NONE;
+  if (out.empty()) Py_RETURN_TRUE;
   if (out.size() == 1) return THPVariable_Wrap(std::move(out[0]));
   PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(out.size()));
   if (tuple == nullptr) return nullptr;
@@ -355,19 +385,20 @@ PyObject* keep(PyObject*, PyObject* args) {
   PyBuffer_Release(&layouts);
   Call call;
   call.key.push_back(code);
-  if (family < 0 || family > kAttention || !read(call, PySequence_Fast_ITEMS(operands), PyTuple_GET_SIZE(operands), by_type != 0)) Py_RETURN_FALSE;
+  if (family < 0 || family >= kFamilies || !read(call, PySequence_Fast_ITEMS(operands), PyTuple_GET_SIZE(operands), by_type != 0)) Py_RETURN_FALSE;
   plan->family = static_cast<Family>(family);
   if (!int_list(ints, plan->ints)) return nullptr;
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(doubles); ++i) plan->doubles.push_back(PyFloat_AsDouble(PyTuple_GET_ITEM(doubles, i)));
   if (PyErr_Occurred()) return nullptr;
   // Behind the operands that `launch` reads come numbers, whose values the key holds, unless a number came as a tensor: the long way
   // read its value, of which the key has nothing.
-  const Py_ssize_t operands_of[] = {kMostOperands, 1, 1, 1, 3, plan->ints.size() > 0 && plan->ints[0] == 0 ? 1 : 3, 5, 4, 3};
+  const Py_ssize_t operands_of[] = {kMostOperands, 1, 1, 1, 3, plan->ints.size() > 0 && plan->ints[0] == 0 ? 1 : 3, 5, 4, 3, 3, 7, 9};
   for (Py_ssize_t i = operands_of[family]; i < PyTuple_GET_SIZE(operands); ++i)
     if (THPVariable_Check(PyTuple_GET_ITEM(operands, i))) Py_RETURN_FALSE;
   // what `launch` reads of each family
-  const size_t least[] = {2, 6, 2, 5, 4, 6, 5, 12, 19};
-  const bool has_double = family == kLayerNorm || family == kTransposed || family == kBatchNorm || family == kAttention;
+  const size_t least[] = {2, 6, 2, 5, 4, 6, 5, 12, 19, 22, 19, 15};
+  const bool has_double = family == kLayerNorm || family == kTransposed || family == kBatchNorm || family == kAttention || family == kWindow ||
+                          family == kCacheAttention;
   if (plan->ints.size() < least[family] || (has_double && plan->doubles.empty()) ||
       (family == kPack && plan->ints.size() < 2 + 2 * static_cast<size_t>(plan->ints[1])))
     Py_RETURN_FALSE;
@@ -381,7 +412,7 @@ PyObject* keep(PyObject*, PyObject* args) {
     output.packed = c10::IntArrayRef(output.strides) == c10::IntArrayRef(c10::contiguous_strides(t.sizes()));
     plan->outputs.push_back(std::move(output));
   }
-  if (plan->outputs.empty()) Py_RETURN_FALSE;
+  if (plan->outputs.empty() != (family == kCacheStore)) Py_RETURN_FALSE;
   if (family == kFused) plan->ints.push_back(1);      // (never without a divisor to point at)
   if (family == kFused && plan->layouts.empty()) plan->layouts.resize(1);
   plan->key = std::move(call.key);
@@ -411,7 +442,11 @@ PyObject* setup(PyObject*, PyObject* args) {
         find_entry(handle, "tq_layer_norm_transposed_launch", library.layer_norm_transposed_launch) &&
         find_entry(handle, "tq_batch_norm_eval_launch", library.batch_norm_eval_launch) &&
         find_entry(handle, "tq_gemm_bias_act_residual_launch", library.gemm_bias_act_residual_launch) &&
-        find_entry(handle, "tq_attention_launch", library.attention_launch))) {
+        find_entry(handle, "tq_attention_launch", library.attention_launch) &&
+        find_entry(handle, "tq_window_attention_launch", library.window_attention_launch) &&
+        find_entry(handle, "tq_cache_attention_launch", library.cache_attention_launch) &&
+        find_entry(handle, "tq_cache_store_launch", library.cache_store_launch) &&
+        find_entry(handle, "tq_copy_pages_launch", library.copy_pages_launch))) {
     PyErr_Format(PyExc_ImportError, "%s: %s", path, dlerror());
     return nullptr;
   }
@@ -422,11 +457,70 @@ PyObject* setup(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// copy_pages(tensors, sources, targets, page_axis): ops.copy_pages, whose pages are given anew each time, from plain lists and tensors. None: the long
+// way, which says what is wrong.
+PyObject* copy_pages(PyObject*, PyObject* const* values, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 4 || !PyList_CheckExact(values[0]) || !PyList_CheckExact(values[1]) || !PyList_CheckExact(values[2]) || !PyLong_CheckExact(values[3]) ||
+      c10::impl::TorchDispatchModeTLS::any_modes_set())
+    Py_RETURN_NONE;
+  const long axis = PyLong_AsLong(values[3]);
+  if (axis == -1 && PyErr_Occurred()) PyErr_Clear();
+  const Py_ssize_t tensors = PyList_GET_SIZE(values[0]), pairs = PyList_GET_SIZE(values[1]);
+  if ((axis != 0 && axis != 1) || tensors == 0 || tensors > 4096 || PyList_GET_SIZE(values[2]) != pairs) Py_RETURN_NONE;
+  std::vector<tq_paged_tensor> described;
+  int device = -1;
+  int64_t pages = 0;
+  for (Py_ssize_t i = 0; i < tensors; ++i) {
+    PyObject* value = PyList_GET_ITEM(values[0], i);
+    if (!THPVariable_CheckExact(value)) Py_RETURN_NONE;
+    const at::Tensor& t = THPVariable_Unpack(value);
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->is_python_dispatch() || !t.unsafeGetTensorImpl()->has_storage() || t.dim() <= axis ||
+        t.unsafeGetTensorImpl()->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                                                        c10::DispatchKey::Functionalize, c10::DispatchKey::Batched})))
+      Py_RETURN_NONE;
+    if (device < 0) device = t.get_device();
+    if (i == 0) pages = t.size(axis);
+    if (t.get_device() != device || t.size(axis) != pages || pages < 2) Py_RETURN_NONE;
+    int64_t inner = 1;
+    for (int64_t d = t.dim() - 1; d > axis; --d) {
+      if (t.size(d) != 1 && t.stride(d) != inner) Py_RETURN_NONE;
+      inner *= t.size(d);
+    }
+    const int64_t size = static_cast<int64_t>(t.element_size());
+    described.push_back({t.mutable_data_ptr(), axis == 1 ? t.size(0) : 1, axis == 1 ? t.stride(0) * size : 0, t.stride(axis) * size, inner * size});
+  }
+  std::vector<int64_t> numbers[2];
+  for (int k = 0; k < 2; ++k) {
+    numbers[k].reserve(pairs);
+    for (Py_ssize_t i = 0; i < pairs; ++i) {
+      PyObject* value = PyList_GET_ITEM(values[1 + k], i);
+      if (!PyLong_CheckExact(value)) Py_RETURN_NONE;
+      const int64_t number = PyLong_AsLongLong(value);
+      if (number == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+      numbers[k].push_back(number);
+    }
+  }
+  void* const stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
+  tq_status status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    status = library.copy_pages_launch(described.data(), static_cast<int32_t>(described.size()), pages, numbers[0].data(), numbers[1].data(), pairs, device, stream);
+  }
+  if (status != TQ_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* size(PyObject*, PyObject*) { return PyLong_FromSize_t(plans().young.size() + plans().old.size()); }
 
 PyMethodDef methods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_planned)), METH_FASTCALL, nullptr},
     {"elementwise", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_elementwise)), METH_FASTCALL, nullptr},
+    {"copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(copy_pages)), METH_FASTCALL, nullptr},
     {"keep", keep, METH_VARARGS, nullptr},
     {"setup", setup, METH_VARARGS, nullptr},
     {"size", size, METH_NOARGS, nullptr},

@@ -46,10 +46,11 @@ _gemm_kernel, _attention_kernel = lru_cache(maxsize=64)(GemmKernel), lru_cache(m
 # plan for; the long way below it leaves one when a call was a single launch over the operands as they came.
 _launcher = load_launcher()
 _launcher.setup(torch.nn.Parameter, workspace, str(LIBRARY_PATH))
-_FUSED, _REDUCE, _PACK, _SOFTMAX, _LAYER_NORM, _TRANSPOSED, _BATCH_NORM, _GEMM, _ATTENTION = range(9)      # launcher.cpp: Family
+_FUSED, _REDUCE, _PACK, _SOFTMAX, _LAYER_NORM, _TRANSPOSED, _BATCH_NORM, _GEMM, _ATTENTION, _WINDOW, _CACHE_ATTENTION, _CACHE_STORE = range(12)      # launcher.cpp: Family
 _call, _keep_plan = _launcher.call, _launcher.keep
 _CODES = {name: 1 + i for i, name in enumerate(("pack", "softmax", "layer_norm", "native_layer_norm", "batch_norm", "attention", "sum", "mean", "amax",
-                                                "amin", "argmax", "gemm none", "gemm gelu", "gemm gelu_erf", "gemm gelu_tanh"))}
+                                                "amin", "argmax", "gemm none", "gemm gelu", "gemm gelu_erf", "gemm gelu_tanh", "window attention",
+                                                "cache attention", "cache store"))}
 
 
 def _fused_ints(kernel: FusedKernel, elements: int, divisors) -> tuple:
@@ -601,6 +602,10 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True
     its last token, and sees the keys j <= p with j > p - window or j < sinks; `window` None: all of j <= p. A query before the
     first key gives zeros. What lies in keys a query does not see (NaN too) does not reach its result. Types, widths, strides and
     `token_major` as for `attention`."""
+    given = (q, k, v, window, sinks, scale, token_major)
+    out = _call(_CODES["window attention"], *given)
+    if out is not None:
+        return out
     operands = (q, k, v)
     for t, what in zip(operands, ("the queries", "the keys", "the values")):
         if t.dim() != 4:
@@ -618,9 +623,12 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True
     nbytes = ctypes.c_size_t()
     check(lib.tq_window_attention_workspace_bytes(*extents, window, sinks, device, ctypes.byref(nbytes)))
     scratch = _own_scratch(nbytes.value, q.device)
-    check(lib.tq_window_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k), _pointer(v), _pointer(out), *extents, _three_strides(q, "the queries"),
-                                         _three_strides(k, "the keys"), _three_strides(v, "the values"), _three_strides(out, "the result"), scale, window,
-                                         sinks, _pointer(scratch), nbytes.value, device, _stream(None, device)))
+    strides = (_three_strides(q, "the queries"), _three_strides(k, "the keys"), _three_strides(v, "the values"), _three_strides(out, "the result"))
+    check(lib.tq_window_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k), _pointer(v), _pointer(out), *extents, *strides, scale, window, sinks,
+                                         _pointer(scratch), nbytes.value, device, _stream(None, device)))
+    if out.numel():
+        _keep_plan(False, _CODES["window attention"], given, _WINDOW, (out,),
+                   (dtype_code(q.dtype), *extents, *[n for three in strides for n in three], window, sinks, nbytes.value), (scale,), b"", None)
     return out
 
 
@@ -654,6 +662,10 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, win
     device) says how many tokens it has, the queries' own among them: query i of q [batch, heads, q_tokens, width] stands at
     position lengths[b] - q_tokens + i. Page numbers and lengths stay on the device; one that leads out of the pool or the table is left
     out, and `kernel.check_status` then raises."""
+    given = (q, k_pages, v_pages, k_scales, v_scales, table, lengths, window, sinks, scale, token_major)
+    out = _call(_CODES["cache attention"], *given)
+    if out is not None:
+        return out
     if q.dim() != 4:
         raise Declined("the queries must be [batch, heads, tokens, width]")
     batch, heads, q_tokens, width = q.shape
@@ -669,10 +681,14 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, win
     nbytes = ctypes.c_size_t()
     check(lib.tq_cache_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page_tokens, blocks, window, sinks, device, ctypes.byref(nbytes)))
     scratch = _own_scratch(nbytes.value, q.device)
+    strides = (_three_strides(q, "the queries"), _three_strides(out, "the result"))
+    extents = (batch, heads, kv_heads, q_tokens, width, pages, page_tokens, blocks, table_stride)
     check(lib.tq_cache_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),
-                                        _pointer(table), _pointer(lengths), _pointer(out), batch, heads, kv_heads, q_tokens, width, pages, page_tokens, blocks,
-                                        table_stride, _three_strides(q, "the queries"), _three_strides(out, "the result"), scale, window, sinks,
-                                        _pointer(scratch), nbytes.value, device, _stream(None, device)))
+                                        _pointer(table), _pointer(lengths), _pointer(out), *extents, *strides, scale, window, sinks, _pointer(scratch),
+                                        nbytes.value, device, _stream(None, device)))
+    if out.numel():
+        _keep_plan(False, _CODES["cache attention"], given, _CACHE_ATTENTION, (out,),
+                   (dtype_code(q.dtype), *extents, *[n for three in strides for n in three], window, sinks, nbytes.value), (scale,), b"", None)
     return out
 
 
@@ -682,6 +698,9 @@ def cache_store(k, v, k_pages, v_pages, k_scales, v_scales, table, starts, count
     A page and head's scale is the smallest power of two s with every |x| <= 448 s among its tokens since it was begun (position 0 of the
     page begins it anew); where a new token raises it, the page's earlier ones are encoded again. Each page that is written must belong
     to one sequence alone. `starts` and `counts` are int32 on the device."""
+    given = (k, v, k_pages, v_pages, k_scales, v_scales, table, starts, counts)
+    if _call(_CODES["cache store"], *given) is not None:
+        return
     for t in (k, v):
         if t.dim() != 4:
             raise Declined("new keys and values must be [batch, kv_heads, tokens, width]")
@@ -691,16 +710,20 @@ def cache_store(k, v, k_pages, v_pages, k_scales, v_scales, table, starts, count
     pages, page_tokens, blocks, table_stride = _cache_extents(k_pages, v_pages, k_scales, v_scales, table, batch, kv_heads, width)
     _per_sequence(starts, batch, "starts")
     _per_sequence(counts, batch, "counts")
-    device = _device_of([t for t in (k, v, k_pages, v_pages, k_scales, v_scales, table, starts, counts) if t is not None])
-    check(lib.tq_cache_store_launch(dtype_code(k.dtype), _pointer(k), _pointer(v), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),
-                                    _pointer(table), _pointer(starts), _pointer(counts), batch, kv_heads, tokens, width, pages, page_tokens, blocks, table_stride,
-                                    _three_strides(k, "new keys"), _three_strides(v, "new values"), device, _stream(None, device)))
+    device = _device_of([t for t in given if t is not None])
+    extents = (batch, kv_heads, tokens, width, pages, page_tokens, blocks, table_stride)
+    strides = (_three_strides(k, "new keys"), _three_strides(v, "new values"))
+    check(lib.tq_cache_store_launch(dtype_code(k.dtype), *[_pointer(t) for t in given], *extents, *strides, device, _stream(None, device)))
+    if k.numel():
+        _keep_plan(False, _CODES["cache store"], given, _CACHE_STORE, (), (dtype_code(k.dtype), *extents, *[n for three in strides for n in three]), (), b"", None)
 
 
 def copy_pages(tensors, sources, targets, page_axis=0) -> None:
     """Copies page sources[i] to page targets[i] in every one of `tensors` (pages of a cache, their scales, of any type), whose axis
     `page_axis` (0, or 1 behind an axis of layers) counts the pages; a page's own elements are contiguous. `sources` and `targets` are numbers on
     the host; the targets are distinct and none is a source, so the order of the copies does not show."""
+    if _launcher.copy_pages(tensors, sources, targets, page_axis):
+        return
     if page_axis not in (0, 1):
         raise Declined(f"pages are counted by axis 0 or 1, not {page_axis}")
     tensors = list(tensors)
