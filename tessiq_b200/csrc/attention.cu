@@ -68,6 +68,9 @@
 namespace tq {
 namespace {
 
+#ifndef WKEYS
+#define WKEYS 64
+#endif
 constexpr int kHeadDim = 64;
 constexpr int kRows = 128;            // query rows per CTA
 constexpr int kAttnThreads = 256;     // four softmax warps; producer and issuer in a second group of four
@@ -120,6 +123,14 @@ struct AttnParams {
   WaitStatus status;
 };
 
+// With a window: what a query sees (keyed.h), which key head it shares, and, for rows whose result has to be taken again, where the operands lie.
+struct WindowAttnParams : AttnParams {
+  int group, offset;               // heads a key head serves; k_tokens - q_tokens
+  int window, sinks;
+  const void *q, *k, *v;
+  long long q_strides[3], k_strides[3], v_strides[3];
+};
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
@@ -163,10 +174,64 @@ __device__ __forceinline__ uint32_t pack_rest(uint32_t rounded, float2 exact) {
   }
 }
 
-template <typename T, int D, int KEYS, bool FEW>
+// One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a lane for the result.
+template <typename T, int D>
+__device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int batch, int head, int key_head, int row) {
+  const int lane = threadIdx.x & 31, position = row + p.offset;
+  const T* q = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + row * p.q_strides[2];
+  const T* k = static_cast<const T*>(p.k) + batch * p.k_strides[0] + key_head * p.k_strides[1];
+  const T* v = static_cast<const T*>(p.v) + batch * p.v_strides[0] + key_head * p.v_strides[1];
+  constexpr int kMine = D / 32;
+  float most = -INFINITY, total = 0.f, result[kMine];
+#pragma unroll
+  for (int c = 0; c < kMine; ++c) result[c] = 0.f;
+  const int start = max(position - p.window + 1, 0), sinks = min(min(p.sinks, position + 1), start);
+  const int count = sinks + position + 1 - start;
+#pragma unroll 1
+  for (int first = 0; first < count; first += 32) {
+    const int nth = first + lane, key = nth < sinks ? nth : nth - sinks + start;
+    float score = -INFINITY;
+    if (nth < count) {
+      const T* from = k + key * p.k_strides[2];
+      score = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < p.head_dim; ++c) score = fmaf(to_compute(q[c]), to_compute(from[c]), score);
+      score *= p.scale_log2;
+    }
+    float top = score;
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+    top = fmaxf(top, most);
+    const float factor = most == top ? 1.f : exp2_ftz(most - top);
+    most = top;
+    const float weight = nth < count ? exp2_ftz(score - (top == -INFINITY ? 0.f : top)) : 0.f;
+    total = total * factor + warp_sum(weight);
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) result[c] *= factor;
+#pragma unroll 1
+    for (int i = 0; i < min(32, count - first); ++i) {
+      const float w = __shfl_sync(0xffffffffu, weight, i);
+      const T* from = v + __shfl_sync(0xffffffffu, key, i) * p.v_strides[2];
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) {
+        const int column = c * 32 + lane;
+        if (column < p.head_dim) result[c] = fmaf(w, to_compute(from[column]), result[c]);
+      }
+    }
+  }
+  T* out = static_cast<T*>(p.out) + batch * p.out_batch + head * p.out_head + row * p.out_token;
+#pragma unroll
+  for (int c = 0; c < kMine; ++c) {
+    const int column = c * 32 + lane;
+    if (column < p.head_dim) out[column] = from_compute<T, float>(result[c] / total);
+  }
+  __syncwarp();
+}
+
+template <typename T, int D, int KEYS, bool FEW, bool WINDOW = false>
 __global__ void __launch_bounds__(kAttnThreads, AttnLayout<D, KEYS, FEW>::kCtasPerSm)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
+                 const __grid_constant__ CUtensorMap map_v, const std::conditional_t<WINDOW, WindowAttnParams, AttnParams> p) {
   using L = AttnLayout<D, KEYS, FEW>;
   constexpr int kKeys = KEYS;
   constexpr bool kAhead = KEYS < 128;      // the reference point takes the second tile's scores too
@@ -202,12 +267,24 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int q0 = q_block * kRows;
   const int key_tiles = (p.k_tokens + kKeys - 1) / kKeys;
   // under a causal mask only the key tiles that hold a key <= the CTA's last row; at least one step
-  const int steps = p.causal ? min(key_tiles, (min(q0 + kRows, p.q_tokens) - 1) / kKeys + 1) : key_tiles;
+  int steps = p.causal ? min(key_tiles, (min(q0 + kRows, p.q_tokens) - 1) / kKeys + 1) : key_tiles;
+  // Under a window: the tiles that hold a key some row of the CTA sees, those of the sinks and then those from the first row's window to the last
+  // row; at least one.
+  int sink_tiles = 0, gap = 0, key_head = head;      // the tiles left out behind the sinks'
+  if constexpr (WINDOW) {
+    const int low = q0 + p.offset, high = min(q0 + kRows, p.q_tokens) - 1 + p.offset;       // positions
+    const int stop = (max(high, -1) + kKeys) / kKeys, start = min(max(low - p.window + 1, 0) / kKeys, stop);
+    sink_tiles = min((min(p.sinks, max(high, -1) + 1) + kKeys - 1) / kKeys, start);
+    gap = start - sink_tiles;
+    steps = max(stop - gap, 1);
+    key_head = head / p.group;
+  }
+  auto first_key = [&](int j) { return (WINDOW && j >= sink_tiles ? j + gap : j) * kKeys; };      // of step j's tile
 
   auto load_tile = [&](const CUtensorMap* map, uint32_t ring, uint32_t full, int j) {
     barrier_expect_tx(full, kTileBytes);
     for (int h = 0; h < kSubTiles; ++h)
-      tma_load_4d(base + ring + (j % kRing) * kTileBytes + h * kSubTileBytes, map, full, h * kHeadDim, j * kKeys, head, batch);
+      tma_load_4d(base + ring + (j % kRing) * kTileBytes + h * kSubTileBytes, map, full, h * kHeadDim, first_key(j), key_head, batch);
   };
 
   // The producer lane sets the barriers up and fills the rings for the first time before the CTA meets: the
@@ -367,6 +444,32 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_load_wait();
     };
     auto mask = [&](Scores& r, int key0) {
+      if constexpr (WINDOW) {
+        const int low = q0 + p.offset, position = query + p.offset;
+        if (key0 + kKeys - 1 > low) {                 // (all three uniform in the CTA)
+          const int limit = position - key0;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) {
+            if (i > limit) r[i] = 0xff800000u;
+          }
+        }
+        if (key0 <= low + kRows - 1 - p.window) {
+          const int from = position - p.window + 1 - key0;
+          if (key0 >= p.sinks) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+              if (i < from) r[i] = 0xff800000u;
+            }
+          } else if (key0 + kKeys > p.sinks) {
+            const int sinks = p.sinks - key0;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+              if (i < from && i >= sinks) r[i] = 0xff800000u;
+            }
+          }
+        }
+        return;
+      }
       if (key0 + kKeys - 1 > open_until) {            // uniform in the CTA
         const int limit = last_allowed - key0;        // columns > limit are masked for this row
 #pragma unroll
@@ -397,7 +500,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         Scores r;
         tcgen05_fence_after();
         load_scores(r, tmem_o);
-        mask(r, kKeys);
+        mask(r, first_key(1));
         second_max = maximum(r);
       }
     }
@@ -410,7 +513,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) barrier_arrive(s_free);
-      mask(r, j * kKeys);
+      mask(r, first_key(j));
       const float tile_max = maximum(r);
       // The reference point: the first two tiles' maximum, moved only when a tile rises more than
       // 2^kSlack above it (from -inf, any finite maximum does). `factor` rescales what the row has
@@ -478,7 +581,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       // the result row leaves tensor memory 32 columns at a time (the loads are warp-wide: every lane takes
       // part, rows beyond the queries only skip the stores)
       const bool stores = query < p.q_tokens;
-      const float inverse = 1.0f / row_sum;
+      const bool sees_some = !WINDOW || query + (p.k_tokens - p.q_tokens) >= 0;      // else: zeros
+      const float inverse = sees_some ? 1.0f / row_sum : 0.f;
+      bool odd = false;                                  // something in the row is no finite number
       T* out_row = static_cast<T*>(p.out) + batch * p.out_batch + head * p.out_head + static_cast<long long>(query) * p.out_token;
       const bool vector_ok = (reinterpret_cast<uintptr_t>(out_row) & 15) == 0;
       const int width = p.head_dim;       // a multiple of 8: whole 16-byte vectors
@@ -488,6 +593,13 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         uint32_t o[32];
         tmem_load_32(tmem_o + c * 32, o);
         tmem_load_wait();
+        if constexpr (WINDOW) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!sees_some) o[i] = 0;
+            odd |= !(fabsf(__uint_as_float(o[i]) * inverse) < INFINITY);
+          }
+        }
         if (stores && vector_ok) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -507,6 +619,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
         __syncwarp();
+      }
+      // The products above take every key of a tile, at a probability of zero where a row does not see it, and zero times an infinity or a NaN is
+      // a NaN. So a row that came out with one is taken again from its own keys alone, by the warp, in plain f32: slow, and rare on real data.
+      if constexpr (WINDOW) {
+        uint32_t again = __ballot_sync(0xffffffffu, odd && stores);
+        while (again != 0) {
+          const int row = q0 + warp * 32 + __ffs(again) - 1;
+          again &= again - 1;
+          take_row_again<T, D>(p, batch, head, key_head, row);
+        }
       }
     }
   }
@@ -602,6 +724,64 @@ AttentionForm choose_attention_form(long long heads, long long q_tokens, long lo
   const bool thirds = !causal && ctas > 2 * sms && ctas <= 3 * sms;
   const bool half_step = !causal && k_tokens < 1280 && (k_tokens + 63) / 64 % 2 == 1;
   return {false, ctas <= 2 * sms || (k_tokens >= 512 && !thirds && !half_step) ? 128 : 64, false};
+}
+
+// Keys a step of the tensor-core tiles for window attention, or 0: few rows, whose keys are streamed (keyed.cu).
+int window_tile_keys(const KeyedParams& p) {
+  if (p.k_tokens == 0 || p.group * p.q_tokens <= 16) return 0;
+  return p.head_dim > kHeadDim ? 64 : WKEYS;
+}
+
+tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, cudaStream_t stream) {
+  CUtensorMap map_q, map_k, map_v;
+  const int64_t q_strides[3] = {from.q_strides[0], from.q_strides[1], from.q_strides[2]}, k_strides[3] = {from.k_strides[0], from.k_strides[1], from.k_strides[2]},
+                v_strides[3] = {from.v_strides[0], from.v_strides[1], from.v_strides[2]};
+  if (tq_status s = attention_map(&map_q, dtype, from.q, from.head_dim, from.q_tokens, from.heads, from.batch, q_strides, kRows)) return s;
+  if (tq_status s = attention_map(&map_k, dtype, from.k, from.head_dim, from.k_tokens, from.kv_heads, from.batch, k_strides, keys)) return s;
+  if (tq_status s = attention_map(&map_v, dtype, from.v, from.head_dim, from.k_tokens, from.kv_heads, from.batch, v_strides, keys)) return s;
+  WindowAttnParams p = {};
+  p.batch = from.batch;
+  p.heads = from.heads;
+  p.q_tokens = from.q_tokens;
+  p.k_tokens = from.k_tokens;
+  p.head_dim = from.head_dim;
+  p.q_blocks = (from.q_tokens + kRows - 1) / kRows;
+  p.causal = 1;
+  p.scale_log2 = from.scale_log2;
+  p.out = from.out;
+  p.out_batch = from.out_strides[0];
+  p.out_head = from.out_strides[1];
+  p.out_token = from.out_strides[2];
+  p.status = from.status;
+  p.group = from.group;
+  p.offset = from.k_tokens - from.q_tokens;
+  p.window = from.window;
+  p.sinks = from.sinks;
+  p.q = from.q;
+  p.k = from.k;
+  p.v = from.v;
+  for (int i = 0; i < 3; ++i) {
+    p.q_strides[i] = from.q_strides[i];
+    p.k_strides[i] = from.k_strides[i];
+    p.v_strides[i] = from.v_strides[i];
+  }
+  const long long ctas = static_cast<long long>(p.q_blocks) * p.heads * p.batch;
+  TQ_REQUIRE(ctas < (1LL << 31), TQ_UNSUPPORTED, "too many query blocks for one launch");
+  auto go = [&](auto width, auto step) -> tq_status {
+    constexpr int kWidth = decltype(width)::value, kKeys = decltype(step)::value;
+    constexpr size_t smem = AttnLayout<kWidth, kKeys, false>::kSmemBytes;
+    auto start = [&](auto kernel) -> tq_status {
+      TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+      kernel<<<static_cast<unsigned>(ctas), kAttnThreads, smem, stream>>>(map_q, map_k, map_v, p);
+      return check_launch("attention_kernel (window)");
+    };
+    if (dtype == TQ_BF16) return start(attention_kernel<__nv_bfloat16, kWidth, kKeys, false, true>);
+    return start(attention_kernel<__half, kWidth, kKeys, false, true>);
+  };
+  auto with_keys = [&](auto width) {
+    return keys == 128 ? go(width, std::integral_constant<int, 128>{}) : go(width, std::integral_constant<int, 64>{});
+  };
+  return from.head_dim > kHeadDim ? with_keys(std::integral_constant<int, 2 * kHeadDim>{}) : with_keys(std::integral_constant<int, kHeadDim>{});
 }
 
 }  // namespace tq
@@ -718,7 +898,8 @@ extern "C" tq_status tq_window_attention_workspace_bytes(int64_t batch, int64_t 
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || k_tokens <= 0) return TQ_OK;      // the launch has nothing to do, or refuses
   tq::KeyedParams p = {};
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
-  *bytes = tq::keyed_workspace(false, p, k_tokens, device);
+  p.k_tokens = static_cast<int>(k_tokens);
+  if (tq::window_tile_keys(p) == 0) *bytes = tq::keyed_workspace(false, p, k_tokens, device);
   return TQ_OK;
 }
 
@@ -775,5 +956,7 @@ extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, c
   }
   p.k_tokens = static_cast<int>(k_tokens);
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
+  const int tile_keys = tq::window_tile_keys(p);
+  if (tile_keys != 0) return tq::window_tiles(dtype, p, tile_keys, static_cast<cudaStream_t>(stream));
   return tq::keyed_attention(dtype, false, p, k_tokens, workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }

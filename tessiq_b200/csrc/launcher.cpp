@@ -276,8 +276,7 @@ tq_status launch(const Plan& p, const Call& call, const std::vector<at::Tensor>&
                                        result(0), n[1], n[2], n[3], n[4], n[5], n[6], n[7], n[8], n[9], n + 10, n + 13, p.doubles[0], n[16], n[17], scratch,
                                        scratch_bytes, device, stream);
     case kCacheStore: {
-      // (the cache's tensors are written: what they hold is theirs whatever the key says)
-      auto written = [&](int i) { return const_cast<void*>(pointer(i)); };
+      auto written = [&](int i) -> void* { return i < call.tensor_count && call.tensors[i] != nullptr ? call.tensors[i]->mutable_data_ptr() : nullptr; };
       return library.cache_store_launch(small(0), pointer(0), pointer(1), written(2), written(3), static_cast<float*>(written(4)), static_cast<float*>(written(5)),
                                    static_cast<const int32_t*>(pointer(6)), static_cast<const int32_t*>(pointer(7)), static_cast<const int32_t*>(pointer(8)), n[1],
                                    n[2], n[3], n[4], n[5], n[6], n[7], n[8], n + 9, n + 12, device, stream);
