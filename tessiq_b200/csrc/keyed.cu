@@ -39,7 +39,7 @@ constexpr int kKeyedThreads = 32 * kKeyedWarps;
 
 #ifndef KSTAGES
 #define KSTAGES 2
-#define KCTAS 3
+#define KCTAS 2
 #endif
 constexpr int kKeyedStages = KSTAGES;      // chunks of a warp in flight or in use
 constexpr uint32_t kStageBytes = 8192;
@@ -104,17 +104,23 @@ __device__ __forceinline__ uint32_t decode_high(uint32_t codes) {
   return pair;
 }
 
+// D = A B + C, 16 x 8 x 16. (C apart from D: the first product of a sum has zeros there, which cost no register.)
 template <typename M>
-__device__ __forceinline__ void multiply(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void multiply(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
   if constexpr (std::is_same_v<M, __half>) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
+}
+template <typename M>
+__device__ __forceinline__ void multiply(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  if (first) multiply<M>(d, a, b0, b1, 0.f, 0.f, 0.f, 0.f);
+  else multiply<M>(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
 
 // An 8 x 8 tile of 16-bit elements, transposed across the warp.
@@ -269,8 +275,8 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 }
 
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. SHARED: the chunks of all units are dealt out in equal shares, one a warp (then
-// keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory.
-template <typename T, int BITS, int W, int NT, bool SHARED>
+// keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory. ONE: a chunk lies in one page (or in none: dense keys).
+template <typename T, int BITS, int W, int NT, bool SHARED, bool ONE>
 __global__ void __launch_bounds__(kKeyedThreads, NT == 1 ? KCTAS : 2)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
@@ -368,13 +374,13 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
   auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
   // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks.
-  const int boxes = BITS == 8 ? p.boxes : 1, box_shift = BITS == 8 ? p.box_shift : 31;
-  const int ahead = 32 / boxes;
+  const int boxes = ONE ? 1 : p.boxes, box_shift = ONE ? 31 : p.box_shift;
+  const int ahead = ONE ? 32 : 32 / boxes;
   auto look_up = [&](int n) {
     if constexpr (BITS == 8) {
-      n += lane / boxes;
+      n += ONE ? lane : lane / boxes;
       if (n >= mine) return -1;
-      const int key = chunk_at(n) * S::kKeys + ((lane % boxes) << box_shift);
+      const int key = chunk_at(n) * S::kKeys + (ONE ? 0 : (lane % boxes) << box_shift);
       if (key >= length) return -1;
       const int at_block = key >> p.page_shift;
       const int page = p.table[batch * p.table_stride + at_block];
@@ -414,18 +420,31 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         page_now = page_next;
         page_next = look_up(n + ahead);
       }
-      const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
-      const bool loads = lane < boxes && page >= 0;
-      const uint32_t box_bytes = static_cast<uint32_t>(S::kLine) << box_shift;
-      const uint32_t bytes = 2u * box_bytes * __popc(__ballot_sync(0xffffffffu, loads));
-      if (lane < boxes) staged_page[warp][stage][lane] = page;
-      if (lane == 0) barrier_expect_tx(bar, bytes);
-      __syncwarp();
-      if (loads) {
-        const int row = static_cast<int>(((static_cast<long long>(page) * p.kv_heads + kv_head) << p.page_shift) +
-                                         ((key0 + (lane << box_shift)) & ((1 << p.page_shift) - 1)));
-        tma_load_rows(to + lane * box_bytes, &map_k, bar, 0, row);
-        tma_load_rows(to + kStageBytes / 2 + lane * box_bytes, &map_v, bar, 0, row);
+      const int inside = key0 & ((1 << p.page_shift) - 1);
+      if constexpr (ONE) {
+        const int page = __shfl_sync(0xffffffffu, page_now, n & 31);
+        if (lane == 0) {
+          staged_page[warp][stage][0] = page;
+          barrier_expect_tx(bar, page >= 0 ? kStageBytes : 0);
+          if (page >= 0) {
+            const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + inside;      // (below 2^31: keyed_maps)
+            tma_load_rows(to, &map_k, bar, 0, row);
+            tma_load_rows(to + kStageBytes / 2, &map_v, bar, 0, row);
+          }
+        }
+      } else {
+        const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
+        const bool loads = lane < boxes && page >= 0;
+        const uint32_t box_bytes = static_cast<uint32_t>(S::kLine) << box_shift;
+        const uint32_t bytes = 2u * box_bytes * __popc(__ballot_sync(0xffffffffu, loads));
+        if (lane < boxes) staged_page[warp][stage][lane] = page;
+        if (lane == 0) barrier_expect_tx(bar, bytes);
+        __syncwarp();
+        if (loads) {
+          const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + ((key0 + (lane << box_shift)) & ((1 << p.page_shift) - 1));
+          tma_load_rows(to + lane * box_bytes, &map_k, bar, 0, row);
+          tma_load_rows(to + kStageBytes / 2 + lane * box_bytes, &map_v, bar, 0, row);
+        }
       }
     } else {
       if (lane == 0) {
@@ -438,14 +457,15 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
   };
-  // Lane t holds the scales of tile t of the next chunk: they are asked for a step before they are used.
+  // The scales of the next chunk's pages (of its tile t in lane t, unless they are one page's) are asked for a step before they are used; 0: no page.
   float k_scale_next = 0.f, v_scale_next = 0.f;
   auto ask_scales = [&](int stage) {
     if constexpr (BITS == 8) {
-      if (lane < kTiles) {
-        const int page = staged_page[warp][stage][(lane * 16) >> box_shift];
+      if (ONE || lane < kTiles) {
+        const int page = staged_page[warp][stage][ONE ? 0 : (lane * 16) >> box_shift];
+        k_scale_next = v_scale_next = 0.f;
         if (page >= 0) {
-          const long long block = static_cast<long long>(page) * p.kv_heads + kv_head;
+          const int block = page * p.kv_heads + kv_head;
           k_scale_next = p.k_scales[block];
           v_scale_next = p.v_scales[block];
         }
@@ -530,42 +550,54 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     const uint32_t k_at = ring + stage * kStageBytes, v_at = k_at + kStageBytes / 2;
     int stop = length;                                 // keys from here on are not there
-    float k_scale[kTiles], v_scale[kTiles];
+    constexpr int kScales = BITS == 8 && !ONE ? kTiles : 1;
+    float k_scale[kScales], v_scale[kScales], v_scale_now = 0.f;
+    k_scale[0] = k_scale_next;
+    v_scale[0] = v_scale_next;
     if constexpr (BITS == 8) {
+      if constexpr (ONE) {
+        if (staged_page[warp][stage][0] < 0) stop = key0;
+      } else {
 #pragma unroll
-      for (int t = kTiles - 1; t >= 0; --t) {
-        k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
-        v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
-        if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
+        for (int t = kTiles - 1; t >= 0; --t) {
+          k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
+          v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
+          if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
+        }
       }
+      v_scale_now = v_scale_next;
       if (step + 1 < mine) ask_scales((turn + 1) % kKeyedStages);
     }
 
     // S^T: keys quad and quad + 8 of each tile by rows 2 corner and 2 corner + 1
     float score[kTiles][NT][4];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
+    for (int j = 0; j < S::kPieces; ++j) {
+      uint4 near[kTiles], far[kTiles];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) score[t][n][0] = score[t][n][1] = score[t][n][2] = score[t][n][3] = 0.f;
+      for (int t = 0; t < kTiles; ++t) {
+        near[t] = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
+        far[t] = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
+      }
 #pragma unroll
-      for (int j = 0; j < S::kPieces; ++j) {
-        const uint4 near = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
-        const uint4 far = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
-        const uint32_t a[4] = {near.x, near.y, near.z, near.w}, b[4] = {far.x, far.y, far.z, far.w};
-        if constexpr (BITS == 8) {
+      for (int w = 0; w < 32 / BITS; ++w) {
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t a0 = decode_low(a[s]), a1 = decode_low(b[s]), a2 = decode_high(a[s]), a3 = decode_high(b[s]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) multiply<M>(score[t][n], a0, a1, a2, a3, query[n][j][s][0], query[n][j][s][1]);
+        for (int t = 0; t < kTiles; ++t) {
+          const uint32_t x[4] = {near[t].x, near[t].y, near[t].z, near[t].w}, y[4] = {far[t].x, far[t].y, far[t].z, far[t].w};
+          uint32_t a[4];
+          if constexpr (BITS == 8) {
+            a[0] = decode_low(x[w]);
+            a[1] = decode_low(y[w]);
+            a[2] = decode_high(x[w]);
+            a[3] = decode_high(y[w]);
+          } else {
+            a[0] = x[2 * w];
+            a[1] = y[2 * w];
+            a[2] = x[2 * w + 1];
+            a[3] = y[2 * w + 1];
           }
-        } else {
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              multiply<M>(score[t][n], a[2 * s], b[2 * s], a[2 * s + 1], b[2 * s + 1], query[n][j][s][0], query[n][j][s][1]);
-          }
+          for (int n = 0; n < NT; ++n) multiply<M>(score[t][n], a, query[n][j][w][0], query[n][j][w][1], j == 0 && w == 0);
         }
       }
     }
@@ -579,22 +611,27 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     bool rises = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      most[n][0] = most[n][1] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        most[n][e] = -INFINITY;
+      for (int t = 0; t < kTiles; ++t) {
+        float2 by = make_float2(row_scale[n][0], row_scale[n][1]);
+        if constexpr (BITS == 8) by = __fmul2_rn(by, make_float2(k_scale[t % kScales], k_scale[t % kScales]));
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const float by = BITS == 8 ? row_scale[n][e] * k_scale[t] : row_scale[n][e];
+        for (int h = 0; h < 2; ++h) {
+          const float2 scaled = __fmul2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), by);
+          score[t][n][2 * h] = scaled.x;
+          score[t][n][2 * h + 1] = scaled.y;
+          if (!open) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& s = score[t][n][2 * h + e];
-            s *= by;
-            if (!open && !sees(position[n][e], key0 + t * 16 + quad + 8 * h)) s = -INFINITY;
-            most[n][e] = fmaxf(most[n][e], s);
+            for (int e = 0; e < 2; ++e)
+              if (!sees(position[n][e], key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
           }
         }
-        rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) most[n][e] = fmaxf(most[n][e], fmaxf(score[t][n][e], score[t][n][2 + e]));
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
     }
     if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
@@ -619,19 +656,20 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : -top[n][0], top[n][1] == -INFINITY ? 0.f : -top[n][1]);
+      float2 gained = make_float2(sum[n][0], sum[n][1]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float reference = top[n][e] == -INFINITY ? 0.f : top[n][e];
+      for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& s = score[t][n][2 * h + e];
-            s = exp2_ftz(s - reference);
-            sum[n][e] += s;
-          }
+        for (int h = 0; h < 2; ++h) {
+          const float2 moved = __fadd2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), shift);
+          score[t][n][2 * h] = exp2_ftz(moved.x);
+          score[t][n][2 * h + 1] = exp2_ftz(moved.y);
+          gained = __fadd2_rn(gained, make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]));
         }
       }
+      sum[n][0] = gained.x;
+      sum[n][1] = gained.y;
     }
 
     // P^T in the layout of the second product: keys 2 corner ... of row quad
@@ -653,115 +691,167 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
 
-    // (of the lane's part of a tile: no NaN, and no infinity in 16 bits)
-    auto values_are_numbers = [&](int t) {
-      bool fine = true;
+    bool apart = false;                                // the rows' products have to be taken one query at a time
+    if (!open) {
+      // Values of keys that no row sees become zeros; where several queries see different keys, a probability of zero is mask enough if
+      // all the values are numbers.
+      constexpr int kUnits = W * BITS / 128;           // 16-byte units of a value
+#pragma unroll 1
+      for (int i = lane; i < S::kKeys * kUnits; i += 32) {
+        const int inside = i / kUnits, key = key0 + inside;
+        const uint32_t unit_at = v_at + S::at(inside, i % kUnits * 16);
+        if (!(key <= high && key < stop && (key > low - p.window || key < p.sinks))) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(unit_at), "r"(0) : "memory");
+        } else if (low != high) {
+          const uint4 unit = load_shared_16(unit_at);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-        for (int w = 0; w < S::kValueWords; w += 2) {
-          const uint2 two = load_shared_8(v_at + S::at(key, S::kValueWords == 2 ? quad * 8 : ((w / 4) * 8 + quad) * 16 + (w % 4) * 4));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t word = h == 0 ? two.x : two.y;
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t four = c == 0 ? unit.x : c == 1 ? unit.y : c == 2 ? unit.z : unit.w;
             if constexpr (BITS == 8) {
-              fine &= (((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0;
+              apart |= (((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
             } else {
               constexpr uint32_t kExponent = std::is_same_v<M, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
-              fine &= (word & kExponent) != kExponent && (word >> 16 & kExponent) != kExponent;
+              apart |= (four & kExponent) == kExponent || (four >> 16 & kExponent) == kExponent;
             }
           }
         }
       }
-      return fine;
+      apart = __any_sync(0xffffffffu, apart);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA fills the stage again
+      __syncwarp();
+    }
+
+    // One slice of V^T (16 head elements) for one tile of keys, as the instruction takes it, from the words of the lane's four keys.
+    auto operand = [&](const uint32_t (&v)[4], int half, uint32_t (&a)[4]) {
+      if constexpr (BITS == 8) {
+        const uint32_t near = __byte_perm(v[0], v[1], half ? 0x7362 : 0x5140), far = __byte_perm(v[2], v[3], half ? 0x7362 : 0x5140);
+        a[0] = decode_low(near);
+        a[1] = decode_high(near);
+        a[2] = decode_low(far);
+        a[3] = decode_high(far);
+      } else {
+        a[0] = __byte_perm(v[0], v[1], 0x5410);
+        a[1] = __byte_perm(v[0], v[1], 0x7632);
+        a[2] = __byte_perm(v[2], v[3], 0x5410);
+        a[3] = __byte_perm(v[2], v[3], 0x7632);
+      }
     };
-    // O^T += V^T P^T of one tile of keys, for the rows of token `only` (all rows: -1) and the keys that `kept` has (a bit for each of the lane's four)
-    auto add_product = [&](int t, uint32_t kept, int only, auto direct) {
-      constexpr bool kDirect = decltype(direct)::value;      // every row adds, and nothing scales what it adds
-      uint32_t value[4][S::kValueWords];               // keys 2 corner, 2 corner + 1, and those 8 further on
+    auto key_of = [&](int t, int r) { return t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1); };
+    constexpr int kHalves = BITS == 8 ? 2 : 1;
+    if (!apart) {
+      // O^T += V^T P^T
+      uint32_t value[kTiles][4][S::kValueWords];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1);
-        if constexpr (S::kValueWords == 2) {
-          const uint2 word = load_shared_8(v_at + S::at(key, quad * 8));
-          value[r][0] = word.x;
-          value[r][1] = word.y;
-        } else {
+      for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
-          for (int w = 0; w < S::kValueWords; w += 4) {
-            const uint4 word = load_shared_16(v_at + S::at(key, ((w / 4) * 8 + quad) * 16));
-            value[r][w] = word.x;
-            value[r][w + 1] = word.y;
-            value[r][w + 2] = word.z;
-            value[r][w + 3] = word.w;
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (S::kValueWords == 2) {
+            const uint2 two = load_shared_8(v_at + S::at(key_of(t, r), quad * 8));
+            value[t][r][0] = two.x;
+            value[t][r][1] = two.y;
+          } else {
+#pragma unroll
+            for (int w = 0; w < S::kValueWords; w += 4) {
+              const uint4 four = load_shared_16(v_at + S::at(key_of(t, r), ((w / 4) * 8 + quad) * 16));
+              value[t][r][w] = four.x;
+              value[t][r][w + 1] = four.y;
+              value[t][r][w + 2] = four.z;
+              value[t][r][w + 3] = four.w;
+            }
           }
         }
       }
 #pragma unroll
       for (int w = 0; w < S::kValueWords; ++w) {
-        uint32_t v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = value[r][w] & (kept >> r & 1 ? 0xffffffffu : 0u);
+        for (int half = 0; half < kHalves; ++half) {
+          const int slice = kHalves * w + half;
+          float d[NT][4];
 #pragma unroll
-        for (int half = 0; half < (BITS == 8 ? 2 : 1); ++half) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (BITS == 8) {
-            const uint32_t near = __byte_perm(v[0], v[1], half ? 0x7362 : 0x5140), far = __byte_perm(v[2], v[3], half ? 0x7362 : 0x5140);
-            a0 = decode_low(near);
-            a1 = decode_high(near);
-            a2 = decode_low(far);
-            a3 = decode_high(far);
-          } else {
-            a0 = __byte_perm(v[0], v[1], 0x5410);
-            a1 = __byte_perm(v[0], v[1], 0x7632);
-            a2 = __byte_perm(v[2], v[3], 0x5410);
-            a3 = __byte_perm(v[2], v[3], 0x7632);
+          for (int t = 0; t < kTiles; ++t) {
+            uint32_t a[4];
+            const uint32_t v[4] = {value[t][0][w], value[t][1][w], value[t][2][w], value[t][3][w]};
+            operand(v, half, a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (BITS == 16) {
+                multiply<M>(result[n][slice], a, weight[t][n][0], weight[t][n][1], false);
+                if constexpr (kTwoOperands) multiply<M>(result[n][slice], a, rest[t][n][0], rest[t][n][1], false);
+              } else {
+                multiply<M>(d[n], a, weight[t][n][0], weight[t][n][1], kScales > 1 || t == 0);
+              }
+              if constexpr (kScales > 1) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) result[n][slice][e] = fmaf(d[n][e], v_scale[t], result[n][slice][e]);
+              }
+            }
           }
-          const int slice = BITS == 8 ? 2 * w + half : w;
+          if constexpr (BITS == 8 && kScales == 1) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (BITS == 16 && kDirect) {
-              multiply<M>(result[n][slice], a0, a1, a2, a3, weight[t][n][0], weight[t][n][1]);
-              if constexpr (kTwoOperands) multiply<M>(result[n][slice], a0, a1, a2, a3, rest[t][n][0], rest[t][n][1]);
-            } else {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              multiply<M>(d, a0, a1, a2, a3, weight[t][n][0], weight[t][n][1]);
-              if constexpr (kTwoOperands) multiply<M>(d, a0, a1, a2, a3, rest[t][n][0], rest[t][n][1]);
-              const float by = BITS == 8 ? v_scale[t] : 1.f;
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (only < 0 || position[n][e & 1] == only) result[n][slice][e] = fmaf(d[e], by, result[n][slice][e]);
+              for (int e = 0; e < 4; e += 2) {
+                const float2 sum2 = __ffma2_rn(make_float2(d[n][e], d[n][e + 1]), make_float2(v_scale[0], v_scale[0]), make_float2(result[n][slice][e], result[n][slice][e + 1]));
+                result[n][slice][e] = sum2.x;
+                result[n][slice][e + 1] = sum2.y;
               }
             }
           }
         }
       }
-    };
-    if (open) {
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) add_product(t, 15u, -1, std::true_type{});
     } else {
-      // Where several queries see different keys: if all of the tile's values are numbers, a probability of zero is all a mask needs.
+      // (Rare, and written to be small.) The probabilities go where the chunk's keys were, and each query has a pass of its own over the tiles, with the
+      // values it does not see as zeros; each row keeps what its own query's pass gives.
+      uint32_t* const kept = reinterpret_cast<uint32_t*>(parts_at + warp * kWarpRing + stage * kStageBytes);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        auto kept_of = [&](int at) {
-          uint32_t kept = 0;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) kept |= (sees(at, key0 + t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1)) ? 1u : 0u) << r;
-          return kept;
-        };
-        uint32_t some = 0;
-#pragma unroll 1
-        for (int at = low; at <= high; ++at) some |= kept_of(at);
-        if (!__any_sync(0xffffffffu, some != 0)) continue;
-        const bool once = low == high || __all_sync(0xffffffffu, values_are_numbers(t));
-#pragma unroll 1
-        for (int at = low; at <= high; ++at) {
-          add_product(t, low == high ? some : once ? 15u : kept_of(at), once ? -1 : at, std::false_type{});
-          if (once) break;
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kept[((t * NT + n) * 4 + h) * 32 + lane] = weight[t][n][h];
+            if constexpr (kTwoOperands) kept[((t * NT + n) * 4 + 2 + h) * 32 + lane] = rest[t][n][h];
+          }
         }
       }
+#pragma unroll 1
+      for (int at = low; at <= high; ++at) {
+#pragma unroll 1
+        for (int t = 0; t < kTiles; ++t) {
+          float scale = v_scale[0];
+          if constexpr (kScales > 1) scale = __shfl_sync(0xffffffffu, v_scale_now, t);
+#pragma unroll
+          for (int w = 0; w < S::kValueWords; ++w) {
+            uint32_t v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int column = S::kValueWords == 2 ? quad * 8 + w * 4 : ((w / 4) * 8 + quad) * 16 + w % 4 * 4;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(v_at + S::at(key_of(t, r), column)));
+              if (!sees(at, key0 + key_of(t, r))) v[r] = 0;
+            }
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              uint32_t a[4];
+              operand(v, half, a);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const uint32_t* b = kept + (t * NT + n) * 4 * 32 + lane;
+                float d[4];
+                multiply<M>(d, a, b[0], b[32], true);
+                if constexpr (kTwoOperands) multiply<M>(d, a, b[64], b[96], false);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (position[n][e & 1] == at) {
+                    float& into = result[n][kHalves * w + half][e];
+                    into = BITS == 8 ? fmaf(d[e], scale, into) : into + d[e];
+                  }
+                }
+              }
+            }
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();                                      // the stage has been read
     if (step + kKeyedStages < mine) fill(step + kKeyedStages, stage);
@@ -862,43 +952,65 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
   if (first == last) return;                              // it lies between two units
   const int tile = unit % p.row_tiles, kv_head = unit / p.row_tiles;
   const int rows = min(kRows, p.group * p.q_tokens - tile * kRows);
-  for (int item = (share - first) * kKeyedThreads + threadIdx.x; item < rows * (W / 8); item += (last - first) * kKeyedThreads) {
-    const int row = item / (W / 8), column = item % (W / 8) * 8;
-    if (column >= p.head_dim) continue;
-    float most = -INFINITY, total = 0.f, value[8] = {};
-    for (int from = first; from <= last; from += 4) {
-      float2 stats[4];
-      float4 part[4][2];
+  const int length = p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
+  // A warp takes 64 elements of a row at a time, eight lanes of eight elements by four groups, each of every fourth part; and so of several rows at once, so
+  // that its loads are under way together.
+  constexpr int kAtOnce = NT == 1 ? 2 : 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane >> 3;
+  const int items = rows * (W / 64), stride = (last - first) * kKeyedWarps;
+  for (int item0 = (share - first) * kKeyedWarps + warp; item0 < items; item0 += kAtOnce * stride) {
+    float most[kAtOnce], total[kAtOnce], value[kAtOnce][8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const long long slot = (2LL * (from + u) + (from + u == first ? 1 : 0)) * kRows + row;
-        stats[u] = make_float2(-INFINITY, 0.f);
-        part[u][0] = part[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (from + u <= last) {
-          stats[u] = p.part_stats[slot];
-          const float4* at = reinterpret_cast<const float4*>(p.parts + slot * W + column);
-          part[u][0] = at[0];
-          part[u][1] = at[1];
+    for (int i = 0; i < kAtOnce; ++i) {
+      most[i] = -INFINITY;
+      total[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) value[i][c] = 0.f;
+    }
+    for (int from = first + group; from <= last; from += 4) {
+      float2 stats[kAtOnce];
+      float4 part[kAtOnce][2];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int item = item0 + i * stride, column = item % (W / 64) * 64 + lane % 8 * 8;
+        stats[i] = make_float2(-INFINITY, 0.f);
+        part[i][0] = part[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (item < items) {
+          const long long slot = (2LL * from + (from == first ? 1 : 0)) * kRows + item / (W / 64);
+          stats[i] = p.part_stats[slot];
+          if (column < p.head_dim) {
+            const float4* at = reinterpret_cast<const float4*>(p.parts + slot * W + column);
+            part[i][0] = at[0];
+            part[i][1] = at[1];
+          }
         }
       }
-      const float before = most;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) most = fmaxf(most, stats[u].x);
-      const float kept = rescale(before, most);
-      total *= kept;
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float both = fmaxf(most[i], stats[i].x);
+        const float mine = rescale(most[i], both), theirs = rescale(stats[i].x, both);
+        const float x[8] = {part[i][0].x, part[i][0].y, part[i][0].z, part[i][0].w, part[i][1].x, part[i][1].y, part[i][1].z, part[i][1].w};
+        most[i] = both;
+        total[i] = total[i] * mine + stats[i].y * theirs;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) value[c] *= kept;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float by = rescale(stats[u].x, most);
-        const float x[8] = {part[u][0].x, part[u][0].y, part[u][0].z, part[u][0].w, part[u][1].x, part[u][1].y, part[u][1].z, part[u][1].w};
-        total += stats[u].y * by;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) value[c] = fmaf(x[c], by, value[c]);
+        for (int c = 0; c < 8; ++c) value[i][c] = value[i][c] * mine + x[c] * theirs;
       }
     }
-    const int length = p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
-    write_result<T>(p, batch, kv_head, tile * kRows + row, column, length, total, value);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int item = item0 + i * stride, column = item % (W / 64) * 64 + lane % 8 * 8;
+#pragma unroll
+      for (int offset = 8; offset < 32; offset *= 2) {
+        const float other = __shfl_xor_sync(0xffffffffu, most[i], offset), both = fmaxf(most[i], other);
+        const float mine = rescale(most[i], both), theirs = rescale(other, both);
+        most[i] = both;
+        total[i] = total[i] * mine + __shfl_xor_sync(0xffffffffu, total[i], offset) * theirs;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) value[i][c] = value[i][c] * mine + __shfl_xor_sync(0xffffffffu, value[i][c], offset) * theirs;
+      }
+      if (item < items && group == 0 && column < p.head_dim)
+        write_result<T>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, total[i], value[i]);
+    }
   }
 }
 
@@ -945,8 +1057,8 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const long long chunks = most_chunks(p, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
   if (chunks > kWholeChunks && (chunks + kUnitCost) * units < (1LL << 31)) {
-    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, true>>(device)
-                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, true>>(device);
+    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, true, true>>(device)
+                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, true, true>>(device);
     plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
     plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
   }
@@ -1008,16 +1120,24 @@ template <typename T, int BITS, int W, int NT>
 tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
   CUtensorMap maps[2] = {};
   if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
-  TQ_CUDA(cudaFuncSetAttribute(p.shares == 0 ? keyed_attention_kernel<T, BITS, W, NT, false> : keyed_attention_kernel<T, BITS, W, NT, true>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)));
+  auto start = [&](auto kernel, long long ctas) -> tq_status {
+    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)));
+    kernel<<<static_cast<unsigned>(ctas), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
+    return check_launch("keyed_attention_kernel");
+  };
+  auto start_boxes = [&](auto shared, long long ctas) {
+    constexpr bool kShared = decltype(shared)::value;
+    if constexpr (BITS == 8) {
+      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kShared, false>, ctas);
+    }
+    return start(keyed_attention_kernel<T, BITS, W, NT, kShared, true>, ctas);
+  };
   if (p.shares == 0) {
     const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles;
     TQ_REQUIRE(units < (1LL << 31), TQ_UNSUPPORTED, "too many heads and rows for one launch");
-    keyed_attention_kernel<T, BITS, W, NT, false><<<static_cast<unsigned>(units), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
-    return check_launch("keyed_attention_kernel");
+    return start_boxes(std::false_type{}, units);
   }
-  keyed_attention_kernel<T, BITS, W, NT, true><<<static_cast<unsigned>(p.shares / kKeyedWarps), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
-  if (tq_status s = check_launch("keyed_attention_kernel")) return s;
+  if (tq_status s = start_boxes(std::true_type{}, p.shares / kKeyedWarps)) return s;
   // The second kernel's start passes under the first one's end (it waits for all of it before it reads the parts).
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(p.shares - 1));
