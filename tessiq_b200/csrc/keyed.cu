@@ -67,7 +67,8 @@ struct KeyedShape {
     return box + key * kLine + turned * 16 + column % 16;
   }
 };
-constexpr size_t kKeyedSmem = 1024 + kKeyedWarps * kWarpRing;
+// The rings and, where a CTA's warps join their parts of a unit first, room for each warp's first part (its last one goes where its ring was).
+constexpr size_t keyed_smem(bool gather, int w, int nt) { return 1024 + kKeyedWarps * (kWarpRing + (gather ? 8 * nt * w * sizeof(float) : 0)); }
 
 __device__ __forceinline__ uint4 load_shared_16(uint32_t address) {
   uint4 word;
@@ -274,18 +275,19 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   return dealt;
 }
 
-// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. SHARED: the chunks of all units are dealt out in equal shares, one a warp (then
+// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal shares, one a warp (then
 // keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory. ONE: a chunk lies in one page (or in none: dense keys).
-template <typename T, int BITS, int W, int NT, bool SHARED, bool ONE>
+template <typename T, int BITS, int W, int NT, int JOINS, bool ONE>
 __global__ void __launch_bounds__(kKeyedThreads, NT == 1 ? KCTAS : 2)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
   using M = std::conditional_t<BITS == 8, __half, T>;      // what the matrix instructions take
+  constexpr bool SHARED = JOINS > 0;
   constexpr bool kTwoOperands = std::is_same_v<M, __nv_bfloat16>;
   constexpr int kRows = 8 * NT, kTiles = S::kTiles, kSlices = S::kSlices;
   static_assert(kRows * W * sizeof(float) <= kWarpRing, "a warp leaves its part where its stages were");
   extern __shared__ unsigned char raw_smem[];
-  __shared__ float part_top[kKeyedWarps][kRows], part_sum[kKeyedWarps][kRows];
+  __shared__ float part_top[SHARED ? 1 : kKeyedWarps][kRows], part_sum[SHARED ? 1 : kKeyedWarps][kRows];
   __shared__ __align__(8) uint64_t full[kKeyedWarps][kKeyedStages];
   __shared__ int staged_page[kKeyedWarps][kKeyedStages][4];      // of each box of a stage; -1: not there
 
@@ -301,6 +303,16 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (blockIdx.x == 0 && warp == 0) p.status.begin();
   }
   __syncwarp();
+  // JOINS > 1: what a warp has of units that others have parts of too: of one that began before its share (0), of one that goes on behind it (1)
+  struct Piece {
+    int sequence, unit, first, last;                   // shares with parts of the unit
+    bool there, begins, ends;
+  };
+  __shared__ Piece pieces[JOINS > 1 ? kKeyedWarps : 1][2];
+  __shared__ float2 piece_stats[JOINS > 1 ? kKeyedWarps : 1][2][JOINS > 1 ? kRows : 1];
+  unsigned char* const heads_at = parts_at + kKeyedWarps * kWarpRing;      // [warp][row][column] f32
+  auto piece_at = [&](int of, int which) { return reinterpret_cast<float*>(which ? parts_at + of * kWarpRing : heads_at + of * (kRows * W * 4)); };
+  if (JOINS > 1 && lane < 2) pieces[JOINS > 1 ? warp : 0][lane].there = false;
   uint32_t turn = 0;                                   // chunks this warp has waited for: the stage and the phase of the next
   const int quad = lane >> 2, corner = lane & 3;       // the instruction's row (or column) of eight, and the lane's place in it
   const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group
@@ -315,9 +327,12 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     dealt = deal<BITS, S::kKeys>(p, blockIdx.x * kKeyedWarps, place);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel may start: it waits for this one's end itself
     if (lane == 0) p.borders[share] = make_int4(0, 0, 0, 0);               // (the border behind this share; see below)
-    if (share >= dealt.shares) return;
-    at = dealt.start(share);
-    until = dealt.start(share + 1);
+    if (share < dealt.shares) {
+      at = dealt.start(share);
+      until = dealt.start(share + 1);
+    } else {
+      until = 0;
+    }
   }
   while (at < until) {
   // ---- one unit, or what of it is in the share: chunks [first_chunk, last_chunk) ----
@@ -341,9 +356,10 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     whole = begins && to == cost;
     const int unit_start = at - from;
     at += to - from;
-    if (last_chunk > 0 && to < cost && lane == 0) {      // the border behind this share cuts the unit: which shares have parts of it
+    if (last_chunk > 0 && !whole && lane == 0) {         // which shares have parts of the unit
       const int first = dealt.holder(unit_start + kUnitCost), last = dealt.holder(unit_start + cost - 1);
-      p.borders[share] = make_int4(batch, unit, first, last);
+      if constexpr (JOINS > 1) pieces[warp][begins ? 1 : 0] = {batch, unit, first, last, true, begins, to == cost};
+      else if (to < cost) p.borders[share] = make_int4(batch, unit, first, last);      // the border behind this share cuts it
     }
     if (at - place.before >= units * cost) place = {batch + 1, place.before + units * cost};
     if (last_chunk == 0) continue;                     // a border just before its first chunk: it is the next share's
@@ -883,7 +899,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       for (int e = 0; e < 2; ++e) {
         const int row = n * 8 + 2 * corner + e;
         if (row0 + row >= rows) continue;
-        if (!whole && quad == 0) p.part_stats[slot0 + row] = make_float2(top[n][e], sum[n][e]);
+        if (!whole && quad == 0) *(JOINS > 1 ? &piece_stats[JOINS > 1 ? warp : 0][begins ? 1 : 0][JOINS > 1 ? row : 0] : p.part_stats + slot0 + row) = make_float2(top[n][e], sum[n][e]);
 #pragma unroll
         for (int run = 0; run < kRuns; ++run) {
           float value[8];
@@ -893,7 +909,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           if (whole) {
             write_result<T>(p, batch, kv_head, row0 + row, column, length, sum[n][e], value);
           } else {
-            float4* to = reinterpret_cast<float4*>(p.parts + (slot0 + row) * W + column);
+            float4* to = reinterpret_cast<float4*>((JOINS > 1 ? piece_at(warp, begins ? 1 : 0) + row * W : p.parts + (slot0 + row) * W) + column);
             to[0] = make_float4(value[0], value[1], value[2], value[3]);
             to[1] = make_float4(value[4], value[5], value[6], value[7]);
           }
@@ -939,26 +955,83 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
   }
   }
+  if constexpr (JOINS > 1) {
+    // The pieces of a unit meet, in the order of the warps; what other CTAs have parts of too goes to memory, as the part of the first of its warps.
+    __syncthreads();
+    for (int i = 0; i < 2 * kKeyedWarps;) {
+      if (!pieces[i / 2][i % 2].there) {
+        ++i;
+        continue;
+      }
+      const Piece head = pieces[i / 2][i % 2];
+      const int share0 = static_cast<int>(blockIdx.x) * kKeyedWarps + i / 2;
+      int last = i;
+      bool ends = head.ends;
+      for (int next = i + 1; next < 2 * kKeyedWarps && !ends; ++next) {
+        if (!pieces[next / 2][next % 2].there) continue;
+        last = next;
+        ends = pieces[next / 2][next % 2].ends;
+      }
+      if (!ends && threadIdx.x == 0)
+        p.borders[blockIdx.x * kKeyedWarps + kKeyedWarps - 1] = make_int4(head.sequence, head.unit, head.first, head.last);
+      const int tile = head.unit % p.row_tiles, kv_head = head.unit / p.row_tiles;
+      const bool whole = head.begins && ends;
+      const long long slot0 = (2LL * share0 + (head.begins ? 1 : 0)) * kRows;
+#pragma unroll 1
+      for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
+        const int row = item / (W / 8), column = item % (W / 8) * 8;
+        if (tile * kRows + row >= rows || column >= p.head_dim) continue;
+        float most = -INFINITY, total = 0.f, value[8] = {};
+#pragma unroll 1
+        for (int j = i; j <= last; ++j) {
+          if (!pieces[j / 2][j % 2].there) continue;
+          const float2 stats = piece_stats[j / 2][j % 2][row];
+          const float4* from = reinterpret_cast<const float4*>(piece_at(j / 2, j % 2) + row * W + column);
+          const float4 near = from[0], far = from[1];
+          const float both = fmaxf(most, stats.x), mine = rescale(most, both), theirs = rescale(stats.x, both);
+          const float x[8] = {near.x, near.y, near.z, near.w, far.x, far.y, far.z, far.w};
+          most = both;
+          total = total * mine + stats.y * theirs;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) value[c] = value[c] * mine + x[c] * theirs;
+        }
+        if (whole) {
+          write_result<T>(p, head.sequence, kv_head, tile * kRows + row, column, length_of<BITS, S::kKeys>(p, head.sequence), total, value);
+        } else {
+          float4* to = reinterpret_cast<float4*>(p.parts + (slot0 + row) * W + column);
+          to[0] = make_float4(value[0], value[1], value[2], value[3]);
+          to[1] = make_float4(value[4], value[5], value[6], value[7]);
+          if (column == 0) p.part_stats[slot0 + row] = make_float2(most, total);
+        }
+      }
+      i = last + 1;
+    }
+  }
 }
 
-// SHARED: joins the parts of the units that a border between two shares cut. A CTA for each border; the CTAs of a unit's borders split its result.
-template <typename T, int W, int NT>
+// SHARED: joins the parts of the units that a border between two shares (or two CTAs' shares: JOINS of them) cut. A CTA for each border; the CTAs of a
+// unit's borders split its result, 64 elements of a row at a time: eight lanes of eight elements, by as many groups as there are
+// parts, four groups in a warp or, of many parts, sixteen in the CTA.
+template <typename T, int W, int NT, int JOINS>
 __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_constant__ KeyedParams p) {
   constexpr int kRows = 8 * NT;
+  __shared__ float2 warp_stats[kKeyedWarps][8];
+  __shared__ float4 warp_value[kKeyedWarps][8][2];
   asm volatile("griddepcontrol.wait;" ::: "memory");      // by every CTA: whoever comes after this kernel comes after the one before it too
-  const int share = static_cast<int>(blockIdx.x);         // the border lies behind it
+  const int share = static_cast<int>(blockIdx.x) * JOINS + JOINS - 1;         // the border lies behind it
   const int4 border = p.borders[share];
   const int batch = border.x, unit = border.y, first = border.z, last = border.w;
-  if (first == last) return;                              // it lies between two units
+  const int borders = last / JOINS - first / JOINS, nth = share / JOINS - first / JOINS, parts = borders + 1;
+  if (first == last || borders == 0) return;              // it lies between two units
   const int tile = unit % p.row_tiles, kv_head = unit / p.row_tiles;
   const int rows = min(kRows, p.group * p.q_tokens - tile * kRows);
   const int length = p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
-  // A warp takes 64 elements of a row at a time, eight lanes of eight elements by four groups, each of every fourth part; and so of several rows at once, so
-  // that its loads are under way together.
-  constexpr int kAtOnce = NT == 1 ? 2 : 4;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane >> 3;
-  const int items = rows * (W / 64), stride = (last - first) * kKeyedWarps;
-  for (int item0 = (share - first) * kKeyedWarps + warp; item0 < items; item0 += kAtOnce * stride) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool many = JOINS > 1 && parts > 16;              // (uniform in the CTA)
+  constexpr int kAtOnce = NT == 1 ? 2 : 4;                // rows whose loads are under way together
+  const int groups = many ? 16 : 4, group = many ? threadIdx.x >> 3 : lane >> 3;
+  const int items = rows * (W / 64), mine0 = many ? nth : nth * kKeyedWarps + warp, stride = many ? borders : borders * kKeyedWarps;
+  for (int item0 = mine0; item0 < items; item0 += kAtOnce * stride) {
     float most[kAtOnce], total[kAtOnce], value[kAtOnce][8];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
@@ -967,7 +1040,9 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
 #pragma unroll
       for (int c = 0; c < 8; ++c) value[i][c] = 0.f;
     }
-    for (int from = first + group; from <= last; from += 4) {
+#pragma unroll 2
+    for (int of = group; of < parts; of += groups) {
+      const int from = of == 0 ? first : (first / JOINS + of) * JOINS;
       float2 stats[kAtOnce];
       float4 part[kAtOnce][2];
 #pragma unroll
@@ -976,7 +1051,7 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
         stats[i] = make_float2(-INFINITY, 0.f);
         part[i][0] = part[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (item < items) {
-          const long long slot = (2LL * from + (from == first ? 1 : 0)) * kRows + item / (W / 64);
+          const long long slot = (2LL * from + (of == 0 ? 1 : 0)) * kRows + item / (W / 64);
           stats[i] = p.part_stats[slot];
           if (column < p.head_dim) {
             const float4* at = reinterpret_cast<const float4*>(p.parts + slot * W + column);
@@ -1008,7 +1083,29 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
 #pragma unroll
         for (int c = 0; c < 8; ++c) value[i][c] = value[i][c] * mine + __shfl_xor_sync(0xffffffffu, value[i][c], offset) * theirs;
       }
-      if (item < items && group == 0 && column < p.head_dim)
+      if (many) {
+        __syncthreads();
+        if (lane < 8) {
+          warp_stats[warp][lane] = make_float2(most[i], total[i]);
+          warp_value[warp][lane][0] = make_float4(value[i][0], value[i][1], value[i][2], value[i][3]);
+          warp_value[warp][lane][1] = make_float4(value[i][4], value[i][5], value[i][6], value[i][7]);
+        }
+        __syncthreads();
+        if (warp == 0 && lane < 8) {
+#pragma unroll
+          for (int w = 1; w < kKeyedWarps; ++w) {
+            const float2 stats = warp_stats[w][lane];
+            const float4 near = warp_value[w][lane][0], far = warp_value[w][lane][1];
+            const float both = fmaxf(most[i], stats.x), mine = rescale(most[i], both), theirs = rescale(stats.x, both);
+            const float x[8] = {near.x, near.y, near.z, near.w, far.x, far.y, far.z, far.w};
+            most[i] = both;
+            total[i] = total[i] * mine + stats.y * theirs;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) value[i][c] = value[i][c] * mine + x[c] * theirs;
+          }
+        }
+      }
+      if (item < items && lane < 8 && (!many || warp == 0) && column < p.head_dim)
         write_result<T>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, total[i], value[i]);
     }
   }
@@ -1016,15 +1113,15 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
 
 // How many CTAs of a kernel run at once on `device`, asked once for each.
 template <auto kKernel>
-int resident(int32_t device) {
+int resident(int32_t device, size_t smem) {
   static std::mutex mutex;
   static int known[64] = {};
   if (device < 0 || device >= 64) return 2 * 148;
   std::lock_guard<std::mutex> lock(mutex);
   if (known[device] == 0) {
     int per_sm = 0;
-    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, kKeyedThreads, kKeyedSmem) != cudaSuccess || per_sm <= 0) {
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, kKeyedThreads, smem) != cudaSuccess || per_sm <= 0) {
       cudaGetLastError();
       per_sm = 2;
     }
@@ -1043,8 +1140,11 @@ long long most_chunks(const KeyedParams& p, long long keys, int chunk) {
 // A unit of so few chunks is a CTA's (two steps of its warps); of more, chunks are dealt out.
 constexpr int kWholeChunks = 2 * kKeyedWarps;
 
+// From as many parts a unit on, the warps of a CTA join theirs before they go to memory.
+constexpr int kManyParts = 8;
+
 struct KeyedPlan {
-  int nt, row_tiles, shares;      // shares 0: a CTA a unit
+  int nt, row_tiles, shares, joins;      // shares 0: a CTA a unit
   size_t bytes;
 };
 
@@ -1057,9 +1157,10 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const long long chunks = most_chunks(p, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
   if (chunks > kWholeChunks && (chunks + kUnitCost) * units < (1LL << 31)) {
-    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, true, true>>(device)
-                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, true, true>>(device);
+    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, 1, true>>(device, keyed_smem(false, W, 1))
+                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, 1, true>>(device, keyed_smem(false, W, 2));
     plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
+    plan.joins = plan.shares >= kManyParts * units ? kKeyedWarps : 1;
     plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
   }
   return plan;
@@ -1121,26 +1222,29 @@ tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
   CUtensorMap maps[2] = {};
   if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
   auto start = [&](auto kernel, long long ctas) -> tq_status {
-    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kKeyedSmem)));
-    kernel<<<static_cast<unsigned>(ctas), kKeyedThreads, kKeyedSmem, stream>>>(maps[0], maps[1], p);
+    const size_t smem = keyed_smem(p.joins > 1, W, NT);
+    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(keyed_smem(true, W, NT))));
+    kernel<<<static_cast<unsigned>(ctas), kKeyedThreads, smem, stream>>>(maps[0], maps[1], p);
     return check_launch("keyed_attention_kernel");
   };
-  auto start_boxes = [&](auto shared, long long ctas) {
-    constexpr bool kShared = decltype(shared)::value;
+  auto start_boxes = [&](auto joins, long long ctas) {
+    constexpr int kJoins = decltype(joins)::value;
     if constexpr (BITS == 8) {
-      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kShared, false>, ctas);
+      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false>, ctas);
     }
-    return start(keyed_attention_kernel<T, BITS, W, NT, kShared, true>, ctas);
+    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true>, ctas);
   };
   if (p.shares == 0) {
     const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles;
     TQ_REQUIRE(units < (1LL << 31), TQ_UNSUPPORTED, "too many heads and rows for one launch");
-    return start_boxes(std::false_type{}, units);
+    return start_boxes(std::integral_constant<int, 0>{}, units);
   }
-  if (tq_status s = start_boxes(std::true_type{}, p.shares / kKeyedWarps)) return s;
+  const bool gathers = p.joins > 1;
+  if (tq_status s = gathers ? start_boxes(std::integral_constant<int, kKeyedWarps>{}, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, p.shares / kKeyedWarps))
+    return s;
   // The second kernel's start passes under the first one's end (it waits for all of it before it reads the parts).
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(p.shares - 1));
+  config.gridDim = dim3(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
   config.blockDim = dim3(kKeyedThreads);
   config.stream = stream;
   cudaLaunchAttribute attribute[1];
@@ -1148,7 +1252,7 @@ tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  TQ_CUDA(cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT>, p));
+  TQ_CUDA(gathers ? cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT, kKeyedWarps>, p) : cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT, 1>, p));
   return check_launch("keyed_join_kernel");
 }
 
@@ -1169,6 +1273,7 @@ tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long 
              "this attention needs %zu bytes of workspace, 16-byte aligned, and was given %zu", plan.bytes, workspace_bytes);
   p.row_tiles = plan.row_tiles;
   p.shares = plan.shares;
+  p.joins = plan.joins;
   const size_t slots = 2ull * plan.shares * 8 * plan.nt;
   p.borders = static_cast<int4*>(workspace);
   p.part_stats = reinterpret_cast<float2*>(p.borders + plan.shares);

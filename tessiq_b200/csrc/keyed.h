@@ -19,7 +19,7 @@ struct KeyedParams {
   int boxes, box_shift;                                                    // of a chunk: its pieces of a page, and log2 of their tokens
   int batch, heads, kv_heads, group, q_tokens, k_tokens, head_dim;
   int window, sinks;
-  int row_tiles, shares;
+  int row_tiles, shares, joins;                                            // joins: shares whose parts of a unit are joined before they go to memory
   float* parts;                                                            // of units that a border between two shares cuts
   int4* borders;                                                           // the border behind each share: {sequence, unit, first and last share with parts of it}, none where these are equal
   float2* part_stats;                                                      // ... their maximum and sum
