@@ -5,11 +5,13 @@
 //   code = e4m3(x / s), to nearest even
 // e4m3 is a floating format, so a power of two costs it no precision, x / s is exact, and an earlier code brought to
 // a larger scale only steps down in exponent: exact again, except for what falls under its smallest normal. The tokens are read once, kept in
-// registers between the maximum and the encoding. Bound: HBM (2 bytes read and 1 written an element); for one new
-// token a sequence, the latency of start, table entry, scale and token, one after another.
+// registers between the maximum and the encoding. Bound: HBM (2 bytes read and 1 written an element: 402 MB in 66 us, 6.1 TB/s); for one new
+// token a sequence, the latency of start, table entry, scale and token, one after another (5 us with the launch). Divisions by the vectors
+// of a token in the addresses had it at 94 us and bound by instructions; the next head's tokens loaded ahead took the registers of half the CTAs and gained nothing.
 //
 // Copying. Source and target pages are given by the host, which is where a cache's pages are handed out; they travel to the kernel as
-// its argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once).
+// its argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 87 us, 6.3 TB/s). Small pages of several layers are
+// one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -33,6 +35,7 @@ struct StoreParams {
   int blocks, page_shift, pages;
   int batch, kv_heads, tokens, head_dim;
   int touched;                     // pages that `tokens` tokens touch at most
+  int each, runs;                  // of the 2 * kv_heads a page has, how many a team takes, and how many teams that makes
   WaitStatus status;
 };
 
@@ -67,12 +70,27 @@ __device__ __forceinline__ uint32_t encode(float a, float b, float c, float d) {
   return word;
 }
 
+// The larger magnitudes of two pairs; a NaN is passed over.
+template <typename T>
+__device__ __forceinline__ uint32_t larger_pair(uint32_t most, uint32_t word) {
+  word &= 0x7fff7fffu;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.bf16x2 %0, %0, %1;" : "+r"(most) : "r"(word));
+  else asm("max.f16x2 %0, %0, %1;" : "+r"(most) : "r"(word));
+  return most;
+}
+
 // x / s for a power of two s, NaN where x is not finite.
 __device__ __forceinline__ float scaled(float x, float inverse) { return fmaf(x, inverse, x - x); }
 
-template <typename T>
+// Eight elements over s. FINITE: there is no infinity among them.
+template <typename T, bool FINITE>
 __device__ __forceinline__ uint2 encode_vector(uint4 word, float inverse) {
   const float2 a = pair_of<T>(word.x), b = pair_of<T>(word.y), c = pair_of<T>(word.z), d = pair_of<T>(word.w);
+  if constexpr (FINITE) {
+    const float2 by = make_float2(inverse, inverse);
+    const float2 e = __fmul2_rn(a, by), f = __fmul2_rn(b, by), g = __fmul2_rn(c, by), h = __fmul2_rn(d, by);
+    return make_uint2(encode(e.x, e.y, f.x, f.y), encode(g.x, g.y, h.x, h.y));
+  }
   return make_uint2(encode(scaled(a.x, inverse), scaled(a.y, inverse), scaled(b.x, inverse), scaled(b.y, inverse)),
                     encode(scaled(c.x, inverse), scaled(c.y, inverse), scaled(d.x, inverse), scaled(d.y, inverse)));
 }
@@ -88,19 +106,16 @@ __device__ __forceinline__ uint32_t encode_again(uint32_t codes, float ratio) {
   return encode(scaled(pair[0].x, ratio), scaled(pair[0].y, ratio), scaled(pair[1].x, ratio), scaled(pair[1].y, ratio));
 }
 
-// TEAM threads (a warp, or all) take one page and head of the keys or of the values.
+// TEAM threads (a warp, or all) take some heads of the keys and values of one page, one after another.
 template <typename T, int TEAM>
-__global__ void __launch_bounds__(kStoreThreads) cache_store_kernel(const __grid_constant__ StoreParams p) {
+__global__ void __launch_bounds__(kStoreThreads, 8) cache_store_kernel(const __grid_constant__ StoreParams p) {
   constexpr int kHeld = 8;                 // vectors of 8 elements a thread keeps: a page of 64 tokens of 128 for 128 threads
-  __shared__ uint32_t warp_most[kStoreThreads / 32];
+  __shared__ uint32_t warp_most[3][kStoreThreads / 32];
   const int thread = threadIdx.x % TEAM;
   long long item = static_cast<long long>(blockIdx.x) * (kStoreThreads / TEAM) + threadIdx.x / TEAM;
-  const bool none = item >= static_cast<long long>(p.batch) * p.touched * p.kv_heads * 2;
-  if (none) return;                        // whole warps, and whole CTAs where a team is one
-  const int which = static_cast<int>(item & 1);
-  item >>= 1;
-  const int head = static_cast<int>(item % p.kv_heads);
-  item /= p.kv_heads;
+  if (item >= static_cast<long long>(p.batch) * p.touched * p.runs) return;      // whole warps, and whole CTAs where a team is one
+  const int run = static_cast<int>(item % p.runs);
+  item /= p.runs;
   const int nth = static_cast<int>(item % p.touched), sequence = static_cast<int>(item / p.touched);
 
   const int start = p.starts[sequence];
@@ -115,79 +130,120 @@ __global__ void __launch_bounds__(kStoreThreads) cache_store_kernel(const __grid
     return;
   }
   const int page = p.table[sequence * p.table_stride + block];
+  const int held_tokens = static_cast<int>(first_position - (block << p.page_shift));      // earlier ones, in this page
+  const int vectors = p.head_dim / 8;
+  const int work = static_cast<int>(last_position - first_position) * vectors;
+  const int first = run * p.each, last = min(first + p.each, 2 * p.kv_heads);       // the keys' heads, then the values'
+
+  auto source_of = [&](int n) {
+    const int which = n >= p.kv_heads ? 1 : 0, head = n - which * p.kv_heads;
+    return static_cast<const T*>(p.x[which]) + sequence * p.strides[which][0] + head * p.strides[which][1] + (first_position - start) * p.strides[which][2];
+  };
+  // A thread's vectors are every TEAM-th of the page's: from the place of one to the next without a division.
+  const int token0 = thread / vectors, column0 = thread % vectors, token_step = TEAM / vectors, column_step = TEAM % vectors;
+  auto each_vector = [&](const T* from, long long token_stride, auto visit) {      // visit(number, whether it is there, where)
+    const T* at = from + token0 * token_stride + column0 * 8;
+    int column = column0, i = thread;
+    const long long step = token_step * token_stride + column_step * 8, wrap = token_stride - vectors * 8;
+    auto go_on = [&] {
+      column += column_step;
+      at += step;
+      if (column >= vectors) {
+        column -= vectors;
+        at += wrap;
+      }
+      i += TEAM;
+    };
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      visit(h, i, at);
+      go_on();
+    }
+#pragma unroll 1
+    for (; i < work; go_on()) visit(kHeld, i, at);
+  };
   if (page < 0 || page >= p.pages) {
     if (thread == 0) report(p.status, kKeyedPage, sequence, static_cast<int>(block));
     return;
   }
-  const long long slot = static_cast<long long>(page) * p.kv_heads + head;
-  const int held_tokens = static_cast<int>(first_position - (block << p.page_shift));      // earlier ones, in this page
-  const int vectors = p.head_dim / 8;
-  const int work = static_cast<int>(last_position - first_position) * vectors;
-  const T* from = static_cast<const T*>(p.x[which]) + sequence * p.strides[which][0] + head * p.strides[which][1] + (first_position - start) * p.strides[which][2];
-  uint8_t* to = p.codes[which] + ((slot << p.page_shift) + held_tokens) * p.head_dim;
-  float* const scale_at = p.scales[which] + slot;
-  float old = 0.f;
-  if (held_tokens > 0) old = *scale_at;      // (every thread reads it before the team meets, and one writes it after)
-
-  auto vector_at = [&](int i) { return *reinterpret_cast<const uint4*>(from + static_cast<long long>(i / vectors) * p.strides[which][2] + (i % vectors) * 8); };
-  uint4 kept[kHeld];
-  uint32_t most = 0;
+  for (int n = first; n < last; ++n) {
+    const int which = n >= p.kv_heads ? 1 : 0;
+    const long long slot = static_cast<long long>(page) * p.kv_heads + (n - which * p.kv_heads);
+    uint8_t* const page_at = p.codes[which] + (slot << p.page_shift) * p.head_dim;
+    uint2* const to = reinterpret_cast<uint2*>(page_at + held_tokens * p.head_dim);
+    float* const scale_at = p.scales[which] + slot;
+    float old = 0.f;
+    if (held_tokens > 0) old = *scale_at;  // (every thread reads it before the team meets, and one writes it after)
+    const T* const from = source_of(n);
+    const long long token_stride = p.strides[which][2];
+    uint4 kept[kHeld];
+    // The team's maximum by `step`, which takes a pair of elements into a pair of maxima; `loads`: the first vectors are not in registers yet.
+    auto team_most = [&](auto step, int turn, auto loads) {
+      uint32_t pair = 0;
+      auto take = [&](uint4 word) { pair = step(step(step(step(pair, word.x), word.y), word.z), word.w); };
+      each_vector(from, token_stride, [&](int h, int i, const T* at) {
+        if (h == kHeld) take(*reinterpret_cast<const uint4*>(at));
+        else if (decltype(loads)::value) kept[h] = i < work ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+      });
 #pragma unroll
-  for (int n = 0; n < kHeld; ++n) {
-    const int i = thread + n * TEAM;
-    kept[n] = make_uint4(0, 0, 0, 0);
-    if (i < work) kept[n] = vector_at(i);
-  }
+      for (int h = 0; h < kHeld; ++h) take(kept[h]);
+      uint32_t most = __reduce_max_sync(0xffffffffu, max(pair & 0xffffu, pair >> 16));      // (magnitudes order like integers)
+      if constexpr (TEAM > 32) {           // (places in turn: the next maxima do not overtake these)
+        if (threadIdx.x % 32 == 0) warp_most[turn][threadIdx.x / 32] = most;
+        __syncthreads();
 #pragma unroll
-  for (int n = 0; n < kHeld; ++n) most = larger<T>(larger<T>(larger<T>(larger<T>(most, kept[n].x), kept[n].y), kept[n].z), kept[n].w);
-  for (int i = thread + kHeld * TEAM; i < work; i += TEAM) {
-    const uint4 word = vector_at(i);
-    most = larger<T>(larger<T>(larger<T>(larger<T>(most, word.x), word.y), word.z), word.w);
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  if constexpr (TEAM > 32) {
-    if (threadIdx.x % 32 == 0) warp_most[threadIdx.x / 32] = most;
-    __syncthreads();
+        for (int w = 0; w < TEAM / 32; ++w) most = max(most, warp_most[turn][w]);
+      }
+      return most;
+    };
+    constexpr uint32_t kInfinity = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+    uint32_t most = team_most([](uint32_t m, uint32_t w) { return larger_pair<T>(m, w); }, n & 1, std::true_type{});
+    const bool finite = most < kInfinity;  // (the same for the team)
+    if (!finite) most = team_most([](uint32_t m, uint32_t w) { return larger<T>(m, w); }, 2, std::false_type{});
+    // the power of two: amax = m 2^e needs 2^(e - 8) where m <= 1.75 = 448 / 2^8, else twice that
+    const float largest = pair_of<T>(most).x;
+    const uint32_t bits = __float_as_uint(largest);
+    int exponent = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const uint32_t old_bits = __float_as_uint(old) & 0x7fffffffu;
+    if (old_bits < 0x7f000000u) exponent = max(exponent, static_cast<int>(old_bits >> 23) + ((old_bits & 0x7fffffu) != 0 ? 1 : 0));
+    exponent = max(exponent, 1);
+    const float scale = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
+    const float inverse = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
+    if (held_tokens > 0 && scale != old) {
+      const float ratio = old * inverse;
+      uint2* const earlier = reinterpret_cast<uint2*>(page_at);
+      for (int i = thread; i < held_tokens * vectors; i += TEAM) {
+        const uint2 word = earlier[i];
+        earlier[i] = make_uint2(encode_again(word.x, ratio), encode_again(word.y, ratio));
+      }
+    }
+    __syncwarp();
+    if (thread == 0) *scale_at = scale;
 #pragma unroll
-    for (int w = 0; w < TEAM / 32; ++w) most = max(most, warp_most[w]);
-  }
-  // the power of two: amax = m 2^e needs 2^(e - 8) where m <= 1.75 = 448 / 2^8, else twice that
-  const float largest = pair_of<T>(most).x;
-  const uint32_t bits = __float_as_uint(largest);
-  int exponent = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  const uint32_t old_bits = __float_as_uint(old) & 0x7fffffffu;
-  if (old_bits < 0x7f000000u) exponent = max(exponent, static_cast<int>(old_bits >> 23) + ((old_bits & 0x7fffffu) != 0 ? 1 : 0));
-  exponent = max(exponent, 1);
-  const float scale = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
-  const float inverse = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
-  if (held_tokens > 0 && scale != old) {
-    const float ratio = old * inverse;
-    uint2* const earlier = reinterpret_cast<uint2*>(p.codes[which] + (slot << p.page_shift) * p.head_dim);
-    for (int i = thread; i < held_tokens * vectors; i += TEAM) {
-      const uint2 word = earlier[i];
-      earlier[i] = make_uint2(encode_again(word.x, ratio), encode_again(word.y, ratio));
+    for (int h = 0; h < kHeld; ++h) {
+      const int i = thread + h * TEAM;
+      if (i < work) to[i] = finite ? encode_vector<T, true>(kept[h], inverse) : encode_vector<T, false>(kept[h], inverse);
+    }
+    if (work > kHeld * TEAM) {
+      each_vector(from, token_stride, [&](int h, int i, const T* at) {
+        if (h == kHeld) to[i] = encode_vector<T, false>(*reinterpret_cast<const uint4*>(at), inverse);
+      });
     }
   }
-  __syncwarp();
-  if (thread == 0) *scale_at = scale;
-#pragma unroll
-  for (int n = 0; n < kHeld; ++n) {
-    const int i = thread + n * TEAM;
-    if (i < work) reinterpret_cast<uint2*>(to)[i] = encode_vector<T>(kept[n], inverse);
-  }
-  for (int i = thread + kHeld * TEAM; i < work; i += TEAM) reinterpret_cast<uint2*>(to)[i] = encode_vector<T>(vector_at(i), inverse);
 }
 
 // ---------------------------------------------------------------------------------------------
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyBytes = 16 * 1024;      // a CTA's share of a page
-constexpr int kCopyTensors = 16, kCopyPairs = 384;
+constexpr int kCopyBytes = 16 * 1024;      // a CTA's piece: of one layer's page, or of several layers' small ones
+constexpr int kCopyTensors = 16, kCopyPairs = 1024;
 
 struct CopyTensor {
   char* base;
-  long long layer_stride, page_stride, page_bytes;
+  long long layer_stride, page_stride;
+  long long page_bytes;
   int layers, width;                       // bytes a load moves: 16, 4 or 1
+  int layer_pieces, piece_layers;          // pieces of a layer's page (1 where a piece has several layers), layers of a piece
 };
 struct CopyParams {
   CopyTensor tensors[kCopyTensors];
@@ -195,37 +251,39 @@ struct CopyParams {
   int count, pairs;
 };
 
+// `layers` runs of `bytes` bytes, `stride` apart.
 template <typename V>
-__device__ __forceinline__ void copy_share(char* to, const char* from, int bytes) {
-  const int n = bytes / static_cast<int>(sizeof(V));
-  V* target = reinterpret_cast<V*>(to);
-  const V* source = reinterpret_cast<const V*>(from);
+__device__ __forceinline__ void copy_piece(char* to, const char* from, int bytes, int layers, long long stride) {
+  const int each = bytes / static_cast<int>(sizeof(V)), n = each * layers;
   constexpr int kUnroll = 4;
+  auto place = [&](int i) { return layers == 1 ? static_cast<long long>(i) * sizeof(V) : i / each * stride + static_cast<long long>(i % each) * sizeof(V); };
   for (int i = threadIdx.x; i < n; i += kUnroll * kCopyThreads) {
     V kept[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i + u * kCopyThreads < n) kept[u] = source[i + u * kCopyThreads];
+      if (i + u * kCopyThreads < n) kept[u] = *reinterpret_cast<const V*>(from + place(i + u * kCopyThreads));
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i + u * kCopyThreads < n) target[i + u * kCopyThreads] = kept[u];
+      if (i + u * kCopyThreads < n) *reinterpret_cast<V*>(to + place(i + u * kCopyThreads)) = kept[u];
   }
 }
 
-// grid: (shares of the largest page, pairs, layers of all tensors)
+// grid: (pieces of all tensors, pairs)
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
-  int layer = static_cast<int>(blockIdx.z), t = 0;
-  while (t + 1 < p.count && layer >= p.tensors[t].layers) layer -= p.tensors[t++].layers;
+  int piece = static_cast<int>(blockIdx.x), t = 0;
+  auto pieces_of = [&](const CopyTensor& tensor) { return (tensor.layers + tensor.piece_layers - 1) / tensor.piece_layers * tensor.layer_pieces; };
+  while (t + 1 < p.count && piece >= pieces_of(p.tensors[t])) piece -= pieces_of(p.tensors[t++]);
   const CopyTensor& tensor = p.tensors[t];
-  const long long first = static_cast<long long>(blockIdx.x) * kCopyBytes;
-  if (first >= tensor.page_bytes) return;
+  const int layer = piece / tensor.layer_pieces * tensor.piece_layers;
+  const long long first = static_cast<long long>(piece % tensor.layer_pieces) * kCopyBytes;
   const int bytes = static_cast<int>(min(tensor.page_bytes - first, static_cast<long long>(kCopyBytes)));
+  const int layers = min(tensor.piece_layers, tensor.layers - layer);
   char* const base = tensor.base + layer * tensor.layer_stride + first;
   const char* from = base + p.sources[blockIdx.y] * tensor.page_stride;
   char* to = base + p.targets[blockIdx.y] * tensor.page_stride;
-  if (tensor.width == 16) copy_share<uint4>(to, from, bytes);
-  else if (tensor.width == 4) copy_share<uint32_t>(to, from, bytes);
-  else copy_share<uint8_t>(to, from, bytes);
+  if (tensor.width == 16) copy_piece<uint4>(to, from, bytes, layers, tensor.layer_stride);
+  else if (tensor.width == 4) copy_piece<uint32_t>(to, from, bytes, layers, tensor.layer_stride);
+  else copy_piece<uint8_t>(to, from, bytes, layers, tensor.layer_stride);
 }
 
 tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vector<int64_t>& sources, const std::vector<int64_t>& targets, int32_t device,
@@ -234,16 +292,18 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
   if (tq_status s = device_scope.status()) return s;
   for (size_t t0 = 0; t0 < tensors.size();) {
     CopyParams p = {};
-    long long layers = 0, largest = 0;
+    long long pieces = 0;
     for (; t0 < tensors.size() && p.count < kCopyTensors; ++t0) {
       const tq_paged_tensor& from = tensors[t0];
-      if (layers > 0 && layers + from.layers > 65535) break;
       const bool sixteen = aligned_to(from.base, 16) && from.layer_stride % 16 == 0 && from.page_stride % 16 == 0 && from.page_bytes % 16 == 0;
       const bool four = aligned_to(from.base, 4) && from.layer_stride % 4 == 0 && from.page_stride % 4 == 0 && from.page_bytes % 4 == 0;
-      p.tensors[p.count++] = {static_cast<char*>(from.base), from.layer_stride, from.page_stride, from.page_bytes, static_cast<int>(from.layers),
-                              sixteen ? 16 : four ? 4 : 1};
-      layers += from.layers;
-      largest = from.page_bytes > largest ? from.page_bytes : largest;
+      CopyTensor& to = p.tensors[p.count];
+      to = {static_cast<char*>(from.base), from.layer_stride, from.page_stride, from.page_bytes, static_cast<int>(from.layers), sixteen ? 16 : four ? 4 : 1,
+            static_cast<int>((from.page_bytes + kCopyBytes - 1) / kCopyBytes), static_cast<int>(from.page_bytes < kCopyBytes ? kCopyBytes / from.page_bytes : 1)};
+      const long long more = (from.layers + to.piece_layers - 1) / to.piece_layers * to.layer_pieces;
+      if (p.count > 0 && pieces + more >= (1LL << 31)) break;
+      pieces += more;
+      ++p.count;
     }
     for (size_t i = 0; i < sources.size(); i += kCopyPairs) {
       p.pairs = static_cast<int>(sources.size() - i < kCopyPairs ? sources.size() - i : kCopyPairs);
@@ -251,7 +311,7 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
         p.sources[n] = static_cast<int>(sources[i + n]);
         p.targets[n] = static_cast<int>(targets[i + n]);
       }
-      const dim3 grid(static_cast<unsigned>((largest + kCopyBytes - 1) / kCopyBytes), static_cast<unsigned>(p.pairs), static_cast<unsigned>(layers));
+      const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(p.pairs));
       copy_pages_kernel<<<grid, kCopyThreads, 0, stream>>>(p);
       if (tq_status s = check_launch("copy_pages_kernel")) return s;
     }
@@ -406,9 +466,15 @@ extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const 
   p.tokens = static_cast<int>(tokens);
   p.head_dim = static_cast<int>(head_dim);
   p.touched = static_cast<int>((tokens + page_tokens - 2) / page_tokens + 1);
-  const long long items = static_cast<long long>(p.batch) * p.touched * p.kv_heads * 2;
-  const bool warps = tokens * head_dim <= 8 * 32 * 8;      // what a warp keeps in registers
-  const long long ctas = warps ? (items + 3) / 4 : items;
+  // A warp where it keeps a page's new tokens in registers, else a CTA; and each several heads where there would be more than four times as many teams as run at
+  // once (128 warps, 32 CTAs an SM). us, with as many as run at once, four times as many and one for every head: 32 x 8 heads of 2047 tokens of 128, pages of 64 68.4, 65.8,
+  // 65.7, pages of 16 77.7, 71.5, 71.6; 32 x 12 of 64, pages of 16 82.4, 74.8, 85.9.
+  const bool warps = (tokens < page_tokens ? tokens : page_tokens) * head_dim <= 8 * 32 * 8;
+  const long long pairs = static_cast<long long>(p.batch) * p.touched, teams_at_once = static_cast<long long>(tq::sm_count(device)) * (warps ? 128 : 32);
+  const long long runs = teams_at_once / pairs < 1 ? 1 : teams_at_once / pairs < 2 * kv_heads ? teams_at_once / pairs : 2 * kv_heads;
+  p.each = static_cast<int>((2 * kv_heads + runs - 1) / runs);
+  p.runs = (2 * p.kv_heads + p.each - 1) / p.each;
+  const long long items = pairs * p.runs, ctas = warps ? (items + 3) / 4 : items;
   TQ_REQUIRE(ctas < (1LL << 31), TQ_UNSUPPORTED, "too many pages and heads for one launch");
   cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel) {

@@ -37,11 +37,9 @@ namespace {
 constexpr int kKeyedWarps = 4;
 constexpr int kKeyedThreads = 32 * kKeyedWarps;
 
-#ifndef KSTAGES
-#define KSTAGES 2
-#define KCTAS 2
-#endif
-constexpr int kKeyedStages = KSTAGES;      // chunks of a warp in flight or in use
+// Chunks of a warp in flight or in use. Measured, 16 x 8 key heads of 128 of 20001 to 40000 keys: two stages and two CTAs an SM 165 us, three stages 164, two stages and three CTAs 181 (registers spill); four
+// queries under a window 45.2, 49.2, 44.8.
+constexpr int kKeyedStages = 2;
 constexpr uint32_t kStageBytes = 8192;
 constexpr uint32_t kWarpRing = kKeyedStages * kStageBytes;
 constexpr int kWaitKeyed = 0x4b455931;      // "KEY1"
@@ -210,8 +208,9 @@ __device__ __forceinline__ int counted(const KeyedParams& p, int sequence) {
   return max(sequence_chunks<BITS, CHUNK>(p, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
 }
 
-// What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another.
-constexpr int kUnitCost = 2;
+// What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another, and its masked ends. Measured with 2, 4 and 6 of them, us: heads of
+// 128, 48 x 8 of four queries under a window 41.2, 39.3, 40.4, 30 x 4 of 96 55.7, 51.4, 52.8; heads of 64 (chunks of twice the keys) 100 x 12 34.3, 36.9, 39.0.
+constexpr int unit_cost(int chunk) { return chunk > 32 ? 2 : 4; }
 constexpr int kLeastShare = 4;       // of the same
 
 // The range has less than 2^31 places (plan_shape sees to it). The first `longer` shares have one place more than the others.
@@ -235,7 +234,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   const int run = (p.batch + kKeyedThreads - 1) / kKeyedThreads;
   const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
   int mine = 0;
-  for (int b = first; b < last; ++b) mine += kUnitCost + counted<BITS, CHUNK>(p, b);
+  for (int b = first; b < last; ++b) mine += unit_cost(CHUNK) + counted<BITS, CHUNK>(p, b);
   mine *= units;
   int upto = mine;
 #pragma unroll
@@ -263,7 +262,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
     if (before <= at && at < upto) {
       int b = first;
       for (; b < last; ++b) {
-        const int here = (kUnitCost + counted<BITS, CHUNK>(p, b)) * units;
+        const int here = (unit_cost(CHUNK) + counted<BITS, CHUNK>(p, b)) * units;
         if (at < before + here) break;
         before += here;
       }
@@ -278,11 +277,12 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal shares, one a warp (then
 // keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory. ONE: a chunk lies in one page (or in none: dense keys).
 template <typename T, int BITS, int W, int NT, int JOINS, bool ONE>
-__global__ void __launch_bounds__(kKeyedThreads, NT == 1 ? KCTAS : 2)
+__global__ void __launch_bounds__(kKeyedThreads, 2)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
   using M = std::conditional_t<BITS == 8, __half, T>;      // what the matrix instructions take
   constexpr bool SHARED = JOINS > 0;
+  constexpr int kUnitCost = unit_cost(S::kKeys);
   constexpr bool kTwoOperands = std::is_same_v<M, __nv_bfloat16>;
   constexpr int kRows = 8 * NT, kTiles = S::kTiles, kSlices = S::kSlices;
   static_assert(kRows * W * sizeof(float) <= kWarpRing, "a warp leaves its part where its stages were");
@@ -1137,8 +1137,10 @@ long long most_chunks(const KeyedParams& p, long long keys, int chunk) {
   return all < seen ? all : seen;
 }
 
-// A unit of so few chunks is a CTA's (two steps of its warps); of more, chunks are dealt out.
-constexpr int kWholeChunks = 2 * kKeyedWarps;
+// A unit of few chunks is a CTA's; of more, chunks are dealt out, which costs the finding of places at the start and the join at the end: from 14 us on, whatever there is to do.
+// A CTA a unit takes 6 and about 1 for each step of its warps, and where CTAs come in several waves about 5 more for each. In us, CTA a unit and dealt out, 16-bit queries: 12 heads of 64
+// 1000 tokens 9.3 / 14.5, 64 x 12 heads 25.1 / 29.0, 64 x 12 x 1500 32.9 / 37.4, 8 x 8 key heads of 128 1000 tokens 12.4 / 16.5, 128 x 8 x 300 30.8 / 26.8, x 600 40.8 / 39.0.
+constexpr int kFewChunks = 2 * kKeyedWarps, kSomeChunks = 8 * kKeyedWarps;
 
 // From as many parts a unit on, the warps of a CTA join theirs before they go to memory.
 constexpr int kManyParts = 8;
@@ -1156,9 +1158,10 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   plan.row_tiles = (rows + 8 * plan.nt - 1) / (8 * plan.nt);
   const long long chunks = most_chunks(p, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
-  if (chunks > kWholeChunks && (chunks + kUnitCost) * units < (1LL << 31)) {
+  if (chunks > kFewChunks && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
     const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, 1, true>>(device, keyed_smem(false, W, 1))
                                   : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, 1, true>>(device, keyed_smem(false, W, 2));
+    if (chunks <= kSomeChunks && units <= 2LL * most) return plan;
     plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
     plan.joins = plan.shares >= kManyParts * units ? kKeyedWarps : 1;
     plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
