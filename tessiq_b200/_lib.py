@@ -97,6 +97,7 @@ SIGNATURES = {
     "tq_attention_launch": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
                                        POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_double, c_int32,
                                        c_int32, c_void_p]),
+    "tq_window_attention_form": (c_int32, [c_int64] * 8 + [c_int32, POINTER(c_int32), POINTER(c_int32)]),
     "tq_window_attention_workspace_bytes": (c_int32, [c_int64] * 8 + [c_int32, POINTER(c_size_t)]),
     "tq_window_attention_launch": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int64] * 6 + [POINTER(c_int64)] * 4
                                    + [c_double, c_int64, c_int64, c_void_p, c_size_t, c_int32, c_void_p]),

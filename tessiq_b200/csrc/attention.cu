@@ -68,9 +68,6 @@
 namespace tq {
 namespace {
 
-#ifndef WKEYS
-#define WKEYS 64
-#endif
 constexpr int kHeadDim = 64;
 constexpr int kRows = 128;            // query rows per CTA
 constexpr int kAttnThreads = 256;     // four softmax warps; producer and issuer in a second group of four
@@ -726,10 +723,29 @@ AttentionForm choose_attention_form(long long heads, long long q_tokens, long lo
   return {false, ctas <= 2 * sms || (k_tokens >= 512 && !thirds && !half_step) ? 128 : 64, false};
 }
 
-// Keys a step of the tensor-core tiles for window attention, or 0: few rows, whose keys are streamed (keyed.cu).
-int window_tile_keys(const KeyedParams& p) {
-  if (p.k_tokens == 0 || p.group * p.q_tokens <= 16) return 0;
-  return p.head_dim > kHeadDim ? 64 : WKEYS;
+// Keys a step of the tensor-core tiles for window attention, or 0: the keys are streamed (keyed.cu), which shares a head's keys among all SMs but takes 16 rows of a key head at
+// a time where a tile has 128 and walks its keys in one CTA. The smaller of two expected times (us; B200, bf16; measured: tiles / streamed). 12 heads of 64, 8000 keys, 8 queries 80 / 14.5,
+// 128 queries 80 / 36, 300 queries 82 / 70; 8 x 12 heads 40 queries 84 / 88, 100 queries 85 / 190; 8 key heads of 128 for 32, 100 queries, 300 keys 10.3 / 12.4, 2000 keys 24.7 / 41, 8000 keys
+// 83 / 107, 5 queries 82 / 29.
+// Tiles: 128 keys a step where few CTAs leave the steps' latency bare (up to two an SM, one of heads above 64), and for heads up to 64 where there are many steps: 8 x 12 x 4096 tokens under a
+// window of 64 110.9 with 128 and 86.6 with 64, of 1024 196.4 and 195.9, of 4096 334 and 356; 2 x 32 x 2501 of 128 under 333 104 and 76.
+int window_tile_keys(const KeyedParams& p, long long sms) {
+  const bool wide = p.head_dim > kHeadDim;
+  const long long rows = static_cast<long long>(p.group) * p.q_tokens;
+  if (p.k_tokens == 0 || rows <= 16) return 0;      // (of one tile of rows streaming was the quicker in every case)
+  const long long keys = p.window < p.k_tokens ? p.window : p.k_tokens;
+  auto steps_of = [&](long long queries, long long step) {      // that some row of a block sees
+    const long long all = (p.k_tokens + step - 1) / step, seen = (p.sinks + step - 1) / step + (keys + queries + step - 2) / step + 1;
+    return all < seen ? all : seen;
+  };
+  const long long blocks = (p.q_tokens + kRows - 1) / kRows, ctas = blocks * p.heads * p.batch, at_once = wide ? sms : 2 * sms;
+  const double tiles = 5.5 + 1.2 * steps_of(p.q_tokens < kRows ? p.q_tokens : kRows, 128) * (ctas > at_once ? static_cast<double>(ctas) / at_once : 1.0);
+  const long long tile_rows = rows <= 8 ? 8 : 16, units = (rows + tile_rows - 1) / tile_rows * p.kv_heads * p.batch;
+  const long long chunks = steps_of((tile_rows + p.group - 1) / p.group, wide ? 16 : 32);
+  const bool whole = chunks <= 8 || (chunks <= 32 && units <= 4 * sms);      // keyed.cu: a CTA a unit
+  const double streamed = whole ? 6.0 + (chunks + 3) / 4 * (units > 2 * sms ? units / (2.0 * sms) : 1.0) : 13.0 + units * chunks * 1.2 / (8.0 * sms);
+  if (streamed <= tiles) return 0;
+  return ctas <= at_once || (!wide && keys >= 2048) ? 128 : 64;
 }
 
 tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, cudaStream_t stream) {
@@ -891,15 +907,32 @@ extern "C" tq_status tq_attention_launch(tq_dtype dtype, const void* q, const vo
   return form.few ? with_keys(std::true_type{}) : with_keys(std::false_type{});
 }
 
+extern "C" tq_status tq_window_attention_form(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim, int64_t window,
+                                              int64_t sinks, int32_t device, int32_t* form, int32_t* keys) {
+  TQ_REQUIRE(form != nullptr && keys != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
+  TQ_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && q_tokens > 0 && k_tokens > 0 && window >= 0 && sinks >= 0 && k_tokens < (1LL << 30) &&
+                 q_tokens < (1LL << 24) && batch * heads < (1LL << 24),
+             TQ_INVALID_ARGUMENT, "no such launch");
+  tq::KeyedParams p = {};
+  tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
+  p.k_tokens = static_cast<int>(k_tokens);
+  *keys = tq::window_tile_keys(p, device < 0 ? 148 : tq::sm_count(device));
+  *form = *keys == 0 ? TQ_ATTENTION_STREAMED : TQ_ATTENTION_TILES;
+  return TQ_OK;
+}
+
 extern "C" tq_status tq_window_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t k_tokens,
                                                          int64_t head_dim, int64_t window, int64_t sinks, int32_t device, size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   *bytes = 0;
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || k_tokens <= 0) return TQ_OK;      // the launch has nothing to do, or refuses
+  // (of what the launch has nothing to do for, or refuses: nothing)
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || k_tokens <= 0 || k_tokens >= (1LL << 30) || q_tokens >= (1LL << 24) ||
+      batch * heads >= (1LL << 24) || window < 0 || sinks < 0 || head_dim <= 0 || head_dim > 2 * tq::kHeadDim)
+    return TQ_OK;
   tq::KeyedParams p = {};
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
   p.k_tokens = static_cast<int>(k_tokens);
-  if (tq::window_tile_keys(p) == 0) *bytes = tq::keyed_workspace(false, p, k_tokens, device);
+  if (tq::window_tile_keys(p, tq::sm_count(device)) == 0) *bytes = tq::keyed_workspace(false, p, k_tokens, device);
   return TQ_OK;
 }
 
@@ -956,7 +989,7 @@ extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, c
   }
   p.k_tokens = static_cast<int>(k_tokens);
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
-  const int tile_keys = tq::window_tile_keys(p);
+  const int tile_keys = tq::window_tile_keys(p, tq::sm_count(device));
   if (tile_keys != 0) return tq::window_tiles(dtype, p, tile_keys, static_cast<cudaStream_t>(stream));
   return tq::keyed_attention(dtype, false, p, k_tokens, workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }

@@ -345,7 +345,11 @@ extern "C" tq_status tq_cache_attention_workspace_bytes(int64_t batch, int64_t h
                                                         size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   *bytes = 0;
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || blocks <= 0) return TQ_OK;      // the launch has nothing to do, or refuses
+  // (of what the launch has nothing to do for, or refuses: nothing)
+  const int page_shift = tq::page_shift_of(page_tokens);
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || q_tokens <= 0 || blocks <= 0 || page_shift < 0 || blocks >= (1LL << 30) >> page_shift ||
+      batch >= (1LL << 24) || kv_heads >= 65536 || heads / kv_heads * q_tokens >= (1LL << 24) || window < 0 || sinks < 0 || head_dim <= 0 || head_dim > 128)
+    return TQ_OK;
   tq::KeyedParams p = {};
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, 1.0, window, sinks);
   *bytes = tq::keyed_workspace(true, p, blocks * page_tokens, device);

@@ -99,6 +99,31 @@ def test_window_attention(tq, case, dtype):
     assert status() == 0
 
 
+def form(*extents):
+    from tessiq_b200 import _lib
+
+    kind, keys = ctypes.c_int32(), ctypes.c_int32()
+    _lib.check(_lib.lib.tq_window_attention_form(*extents, 0, ctypes.byref(kind), ctypes.byref(keys)))
+    return keys.value
+
+
+FORMS = [  # batch, heads, kv_heads, queries, keys, width, window, sinks: every form, at its edges
+    ((1, 2, 2, 20, 3000, 64, 2500, 4), 0), ((1, 4, 1, 40, 1500, 128, 0, 0), 0), ((2, 12, 12, 200, 260, 64, 0, 0), 128), ((1, 8, 8, 300, 2000, 128, 0, 8), 128),
+    ((40, 12, 6, 130, 130, 64, 50, 2), 64), ((12, 16, 8, 150, 200, 96, 90, 70), 64),
+]
+
+
+@pytest.mark.parametrize("case, keys", FORMS, ids=str)
+def test_every_form_of_window_attention(tq, case, keys):
+    batch, heads, kv_heads, queries, k_tokens, width, window, sinks = case
+    assert form(*case) == keys
+    q, k, v = by_token((batch, heads, queries, width), torch.bfloat16, 1), by_token((batch, kv_heads, k_tokens, width), torch.bfloat16, 2), by_token((batch, kv_heads, k_tokens, width), torch.bfloat16, 3)
+    got = tq.window_attention(q, k, v, window or None, sinks)
+    some = [0, batch - 1] if batch > 1 else [0]
+    held(got[some, :2], reference(q[some, :2], k[some, : max(1, 2 * kv_heads // heads)], v[some, : max(1, 2 * kv_heads // heads)], [k_tokens] * len(some), window or None, sinks, 1 / math.sqrt(width)))
+    assert status() == 0
+
+
 def test_without_a_window_it_is_causal_attention(tq):
     q, k, v = (drawn((2, 4, 200, 64), torch.bfloat16, s) for s in (1, 2, 3))
     expected = reference(q, k, v, [200, 200], None, 0, 0.2)
@@ -122,27 +147,33 @@ def test_window_attention_over_no_keys_and_no_queries(tq):
     assert tq.window_attention(q[:0], none[:0], none[:0]).shape == (0, 4, 3, 64)
 
 
-@pytest.mark.parametrize("queries", [1, 3, 70, 200], ids=str)
+@pytest.mark.parametrize("batch, queries", [(1, 1), (1, 3), (1, 70), (40, 70), (40, 200)], ids=str)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_what_no_query_sees_does_not_reach_a_result(tq, queries, bad):
-    """Keys 20 to 39 lie between the sinks and the first query's window, and the last keys are the last queries' own."""
+def test_what_no_query_sees_does_not_reach_a_result(tq, batch, queries, bad):
+    """Keys 20 to 39 lie between the sinks and the first query's window, and the last keys are the last queries' own. The large batches run on tiles."""
     keys, window = queries + 100, 50
-    q, k, v = drawn((1, 4, queries, 64), torch.bfloat16, 1), drawn((1, 2, keys, 64), torch.bfloat16, 2), drawn((1, 2, keys, 64), torch.bfloat16, 3)
+    assert (form(batch, 4, 2, queries, keys, 64, window, 20) > 0) == (batch > 1)
+    q, k, v = drawn((batch, 4, queries, 64), torch.bfloat16, 1), drawn((batch, 2, keys, 64), torch.bfloat16, 2), drawn((batch, 2, keys, 64), torch.bfloat16, 3)
     k[:, :, 20:40], v[:, :, 20:40] = bad, bad
-    expected = reference(q, k, v, [keys], window, 20, 0.125)
+    expected = reference(q[-1:], k[-1:], v[-1:], [keys], window, 20, 0.125)
     assert not expected[0].isnan().any()
-    held(tq.window_attention(q, k, v, window, 20), expected)
+    got = tq.window_attention(q, k, v, window, 20)
+    held(got[-1:], expected)
+    assert got.isfinite().all()
 
 
-@pytest.mark.parametrize("queries", [4, 150], ids=str)
-def test_a_value_that_is_not_a_number_reaches_the_queries_that_see_it(tq, queries):
-    """Key `at` is seen from the query at `at` for a window's length, and by those alone; sinks by all of them."""
+@pytest.mark.parametrize("batch, queries", [(1, 4), (1, 150), (40, 150)], ids=str)
+def test_a_value_that_is_not_a_number_reaches_the_queries_that_see_it(tq, batch, queries):
+    """Key `at` is seen from the query at `at` for a window's length, and by those alone; sinks by all of them. The large batch runs on tiles."""
     keys, window, at = queries + 30, 20, 29 + queries // 2
-    q, k, v = (drawn((1, 2, n, 64), torch.float16, s) for n, s in ((queries, 1), (keys, 2), (keys, 3)))
+    assert (form(batch, 2, 2, queries, keys, 64, window, 3) > 0) == (batch > 1)
+    q, k, v = (drawn((batch, 2, n, 64), torch.float16, s) for n, s in ((queries, 1), (keys, 2), (keys, 3)))
     v[0, 1, at, 5] = math.nan
     v[0, 0, keys - 1, 7] = math.inf
-    expected = reference(q, k, v, [keys], window, 3, 0.125)
-    got = tq.window_attention(q, k, v, window, 3).cpu().double()
+    expected = reference(q[:1], k[:1], v[:1], [keys], window, 3, 0.125)
+    got = tq.window_attention(q, k, v, window, 3)
+    assert got[1:].isfinite().all()
+    got = got[:1].cpu().double()
     assert expected[0].isnan().any() and torch.equal(got.isnan(), expected[0].isnan()) and torch.equal(got.isinf(), expected[0].isinf())
     fine = expected[0].isfinite()
     assert ((got - expected[0]).abs()[fine] <= expected[1][fine]).all()
