@@ -743,7 +743,8 @@ int window_tile_keys(const KeyedParams& p, long long sms) {
   const long long tile_rows = rows <= 8 ? 8 : 16, units = (rows + tile_rows - 1) / tile_rows * p.kv_heads * p.batch;
   const long long chunks = steps_of((tile_rows + p.group - 1) / p.group, wide ? 16 : 32);
   const bool whole = chunks <= 8 || (chunks <= 32 && units <= 4 * sms);      // keyed.cu: a CTA a unit
-  const double streamed = whole ? 6.0 + (chunks + 3) / 4 * (units > 2 * sms ? units / (2.0 * sms) : 1.0) : 13.0 + units * chunks * 1.2 / (8.0 * sms);
+  const double steps = static_cast<double>((chunks + 3) / 4), waves = units > 2 * sms ? units / (2.0 * sms) : 1.0;
+  const double streamed = whole ? 1.0 + waves * (5.0 + steps) : 13.0 + units * chunks * 1.2 / (8.0 * sms);
   if (streamed <= tiles) return 0;
   return ctas <= at_once || (!wide && keys >= 2048) ? 128 : 64;
 }

@@ -1130,10 +1130,10 @@ int resident(int32_t device, size_t smem) {
   return known[device];
 }
 
-// The most chunks a unit can have: all its keys, or what a window and the sinks leave.
-long long most_chunks(const KeyedParams& p, long long keys, int chunk) {
+// The most chunks that some of `tokens` neighbouring queries can see: all keys, or what a window and the sinks leave.
+long long most_chunks(const KeyedParams& p, long long tokens, long long keys, int chunk) {
   const long long all = (keys + chunk - 1) / chunk;
-  const long long seen = (p.sinks + chunk - 1LL) / chunk + (p.window + p.q_tokens + chunk - 2LL) / chunk + 1;
+  const long long seen = (p.sinks + chunk - 1LL) / chunk + (p.window + tokens + chunk - 2LL) / chunk + 1;
   return all < seen ? all : seen;
 }
 
@@ -1156,12 +1156,15 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const int rows = p.group * p.q_tokens;
   plan.nt = rows <= 8 ? 1 : 2;
   plan.row_tiles = (rows + 8 * plan.nt - 1) / (8 * plan.nt);
-  const long long chunks = most_chunks(p, keys, KeyedShape<BITS, W>::kKeys);
+  // a tile's own, and of all the sequence's queries together, which is what every tile walks where chunks are dealt out
+  const long long tokens = (8 * plan.nt + p.group - 2) / p.group + 1;
+  const long long own = most_chunks(p, tokens < p.q_tokens ? tokens : p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
+  const long long chunks = most_chunks(p, p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
-  if (chunks > kFewChunks && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
+  if (own > kFewChunks && chunks <= 2 * own && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
     const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, 1, true>>(device, keyed_smem(false, W, 1))
                                   : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, 1, true>>(device, keyed_smem(false, W, 2));
-    if (chunks <= kSomeChunks && units <= 2LL * most) return plan;
+    if (own <= kSomeChunks && units <= 2LL * most) return plan;
     plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
     plan.joins = plan.shares >= kManyParts * units ? kKeyedWarps : 1;
     plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
