@@ -2,6 +2,7 @@
 
     tessiq_b200.kernel   the `Kernel` launch interface (FusedKernel, ReductionKernel, PackKernel, …)
     tessiq_b200.ops      eager entry points and the `torch.ops.tessiq.<name>` custom operations
+    tessiq_b200.cache    the paged cache of a serving loop: pages, forks, the calls of a step
     tessiq_b200.build    builds libtessiq_b200.so in tree (`python -m tessiq_b200.build`)
 
 Submodules load on first use so that `python -m tessiq_b200.build` works before the library
@@ -12,7 +13,7 @@ raises ImportError.
 from importlib import import_module
 
 __version__ = "0.1.0"
-_SUBMODULES = ("kernel", "ops", "build", "backend", "executor", "sharding")
+_SUBMODULES = ("kernel", "ops", "build", "backend", "executor", "sharding", "cache")
 
 
 def __getattr__(name):

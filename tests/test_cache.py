@@ -153,3 +153,124 @@ def test_python_refuses_before_the_library():
     with pytest.raises(Declined, match="axis"):
         ops.copy_pages([scales], [0], [1], page_axis=2)
     ops.copy_pages([], [0], [1])
+
+
+# ---- the books -----------------------------------------------------------------------------------
+
+
+def test_pages_are_handed_out_lowest_first_and_taken_back():
+    from tessiq_b200.cache import Pages
+
+    books = Pages(6, 16)
+    a, b = books.start(), books.start()
+    assert books.extend([a, b], [17, 16]) == ([], [])
+    assert books.pages_of(a) == [0, 1] and books.pages_of(b) == [2] and books.free_pages == 3
+    books.extend([b], [0])
+    assert books.pages_of(b) == [2]
+    books.extend([b], [1])
+    assert books.pages_of(b) == [2, 3] and books.length(b) == 17
+    books.free(a)
+    assert books.free_pages == 4 and books.sequences == [b]
+    with pytest.raises(KeyError):
+        books.length(a)
+    c = books.start()
+    books.extend([c], [3])
+    assert books.pages_of(c) == [0]
+
+
+def test_a_call_that_cannot_be_met_changes_nothing():
+    from tessiq_b200.cache import Pages
+
+    books = Pages(4, 16)
+    a = books.start()
+    books.extend([a], [20])
+    b = books.fork(a)
+    with pytest.raises(MemoryError):
+        books.extend([a, b], [13, 17])      # a page of its own for a, one more for each
+    assert books.free_pages == 2 and books.length(a) == books.length(b) == 20 and books.pages_of(a) == books.pages_of(b) == [0, 1]
+    with pytest.raises(ValueError):
+        books.extend([a, a], [1, 1])
+    with pytest.raises(ValueError):
+        books.extend([a], [-1])
+    with pytest.raises(ValueError):
+        books.truncate(a, 21)
+    assert books.extend([a, b], [1, 1]) == ([1], [2])      # the second one has the shared page to itself by then
+    assert books.pages_of(a) == [0, 2] and books.pages_of(b) == [0, 1] and books.references[:3] == [2, 1, 1]
+
+
+def test_the_books_against_copies_of_every_sequence():
+    """Random calls: each sequence's tokens, followed through writes, page copies and moves, stay its own."""
+    import random
+
+    from tessiq_b200.cache import Pages
+
+    rng, page = random.Random(3), 4
+    books, memory, tokens, serial = Pages(30, page), {}, {}, 0
+    for _ in range(3000):
+        kind = rng.choice(["start", "fork", "extend", "extend", "extend", "truncate", "free", "compact"])
+        known = list(tokens)
+        if kind == "start" and len(known) < 8:
+            tokens[books.start()] = []
+        elif kind == "fork" and known and len(known) < 8:
+            old = rng.choice(known)
+            tokens[books.fork(old)] = list(tokens[old])
+        elif kind == "extend" and known:
+            some = rng.sample(known, rng.randint(1, len(known)))
+            counts = [rng.randint(0, 9) for _ in some]
+            try:
+                sources, targets = books.extend(some, counts)
+            except MemoryError:
+                continue
+            assert not set(sources) & set(targets) and len(set(targets)) == len(targets)
+            for s, t in zip(sources, targets):
+                memory.update({(t, i): memory.get((s, i)) for i in range(page)})
+            for sequence, count in zip(some, counts):
+                for _ in range(count):
+                    at, serial = len(tokens[sequence]), serial + 1
+                    where = books.pages_of(sequence)[at // page]
+                    assert books.references[where] == 1
+                    memory[where, at % page] = serial
+                    tokens[sequence].append(serial)
+        elif kind == "truncate" and known:
+            sequence = rng.choice(known)
+            length = rng.randint(0, len(tokens[sequence]))
+            books.truncate(sequence, length)
+            del tokens[sequence][length:]
+        elif kind == "free" and known:
+            sequence = rng.choice(known)
+            books.free(sequence)
+            del tokens[sequence]
+        elif kind == "compact":
+            sources, targets = books.compact()
+            assert not set(sources) & set(targets)
+            for s, t in zip(sources, targets):
+                memory.update({(t, i): memory.get((s, i)) for i in range(page)})
+            used = len(books.references) - books.free_pages
+            assert all(books.references[:used]) and not any(books.references[used:])
+        for sequence, held in tokens.items():
+            pages = books.pages_of(sequence)
+            assert books.length(sequence) == len(held) and len(pages) == -(-len(held) // page)
+            assert [memory[pages[i // page], i % page] for i in range(len(held))] == held
+        counted = [0] * len(books.references)
+        for sequence in tokens:
+            for where in books.pages_of(sequence):
+                counted[where] += 1
+        assert counted == books.references and books.free_pages == counted.count(0)
+
+
+def test_a_step_names_pages_starts_and_lengths():
+    from tessiq_b200.cache import PagedCache
+
+    cache = PagedCache(2, 3, 32, pages=9, page_tokens=16, device="cpu")
+    a, b = cache.start(), cache.start()
+    step = cache.extend([a, b], [17, 5])
+    assert step.table.tolist() == [[0, 1], [2, 0]] and step.starts.tolist() == [0, 0] and step.counts.tolist() == [17, 5] and step.lengths.tolist() == [17, 5]
+    step = cache.extend([b, a], 2)
+    assert step.starts.tolist() == [5, 17] and step.lengths.tolist() == [7, 19] and step.tokens == 2
+    assert step.table.dtype == torch.int32 and step.table.tolist() == [[2, 0], [0, 1]]
+    assert cache.extend([], 1).table.shape == (0, 0)
+    with pytest.raises(ValueError, match="nobody wrote"):
+        cache.store(step, 0, torch.zeros(2, 3, 1, 32).half(), torch.zeros(2, 3, 1, 32).half())
+    for bad in (dict(page_tokens=48), dict(width=24), dict(layers=0), dict(pages=0)):
+        with pytest.raises(ValueError):
+            PagedCache(**{**dict(layers=1, kv_heads=2, width=64, pages=4, device="cpu"), **bad})

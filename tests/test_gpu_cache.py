@@ -514,3 +514,60 @@ def test_a_step_replayed_from_a_graph(tq):
     for cache, got in zip(caches, results):
         held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [620, 25], None, 0, 0.125))
     assert status() == 0
+
+
+def test_a_paged_cache_through_forks_drafts_and_moves(tq):
+    """Two layers, three conversations: what each one's attention gives is attention over the tokens it was given, as the cache holds them."""
+    from tessiq_b200.cache import PagedCache
+
+    layers, heads, kv_heads, width = 2, 4, 2, 32
+    cache = PagedCache(layers, kv_heads, width, pages=24, page_tokens=16)
+    for t in cache.tensors:      # whatever memory held before
+        (t.view(torch.uint8) if t.dtype == E4M3 else t).fill_(0x7F if t.dtype == E4M3 else math.nan)
+    given = {}                   # sequence -> what was stored, [layers, 2, kv_heads, tokens, width]
+    seeds = iter(range(1000))
+
+    def write(sequences, tokens):
+        counts = [tokens] * len(sequences) if isinstance(tokens, int) else tokens
+        step = cache.extend(sequences, tokens)
+        new = [[drawn((len(sequences), kv_heads, max(counts), width), torch.bfloat16, next(seeds)) for _ in range(2)] for _ in range(layers)]
+        for layer, (k, v) in enumerate(new):
+            cache.store(step, layer, k, v)
+        for i, sequence in enumerate(sequences):
+            more = torch.stack([torch.stack([x[i, :, : counts[i]] for x in pair]) for pair in new])
+            given[sequence] = torch.cat([given[sequence], more], 3) if sequence in given else more
+        return step
+
+    def agrees(sequences, step, window=None, sinks=0):
+        q = by_token((len(sequences), heads, 1, width), torch.bfloat16, next(seeds))
+        for layer in range(layers):
+            got = cache.attention(step, layer, q, window, sinks)
+            for i, sequence in enumerate(sequences):
+                pages = cache.books.pages_of(sequence)
+                length = cache.length(sequence)
+                k, v = ((codes[layer].view(torch.uint8)[pages].view(E4M3).float() * scales[layer][pages][..., None, None]).permute(1, 0, 2, 3).flatten(1, 2)[None, :, :length]
+                        for codes, scales in ((cache.k_pages, cache.k_scales), (cache.v_pages, cache.v_scales)))
+                for held_values, was in ((k, given[sequence][layer, 0]), (v, given[sequence][layer, 1])):
+                    # (half a step of e4m3, or of its smallest numbers at a scale of at most max / 224)
+                    assert was.shape[1] == length
+                    assert ((held_values[0] - was.float()).abs() <= 2.0**-4 * was.float().abs() + 2.0**-10 * was.float().abs().max() / 224).all()
+                held(got[i : i + 1], reference(q[i : i + 1], k.double(), v.double(), [length], window, sinks, width**-0.5))
+
+    a, b = cache.start(), cache.start()
+    agrees([a, b], write([a, b], [37, 5]))
+    c = cache.fork(a)
+    given[c] = given[a]
+    agrees([c, a, b], write([c, a, b], 1))
+    d = cache.fork(b)
+    given[d] = given[b]
+    agrees([d, b], write([d, b], [4, 20]), 7, 2)
+    cache.truncate(d, 8)
+    given[d] = given[d][:, :, :, :8]
+    cache.free(a)
+    del given[a]
+    assert cache.compact() > 0
+    live = [b, c, d]
+    agrees(live, write(live, [1, 16, 3]))
+    agrees(live, write(live, 1), 20, 3)
+    used = {page for sequence in live for page in cache.books.pages_of(sequence)}
+    assert len(used) + cache.books.free_pages == 24 and status() == 0
