@@ -120,14 +120,6 @@ struct AttnParams {
   WaitStatus status;
 };
 
-// With a window: what a query sees (keyed.h), which key head it shares, and, for rows whose result has to be taken again, where the operands lie.
-struct WindowAttnParams : AttnParams {
-  int group, offset;               // heads a key head serves; k_tokens - q_tokens
-  int window, sinks;
-  const void *q, *k, *v;
-  long long q_strides[3], k_strides[3], v_strides[3];
-};
-
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
@@ -171,64 +163,10 @@ __device__ __forceinline__ uint32_t pack_rest(uint32_t rounded, float2 exact) {
   }
 }
 
-// One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a lane for the result.
-template <typename T, int D>
-__device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int batch, int head, int key_head, int row) {
-  const int lane = threadIdx.x & 31, position = row + p.offset;
-  const T* q = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + row * p.q_strides[2];
-  const T* k = static_cast<const T*>(p.k) + batch * p.k_strides[0] + key_head * p.k_strides[1];
-  const T* v = static_cast<const T*>(p.v) + batch * p.v_strides[0] + key_head * p.v_strides[1];
-  constexpr int kMine = D / 32;
-  float most = -INFINITY, total = 0.f, result[kMine];
-#pragma unroll
-  for (int c = 0; c < kMine; ++c) result[c] = 0.f;
-  const int start = max(position - p.window + 1, 0), sinks = min(min(p.sinks, position + 1), start);
-  const int count = sinks + position + 1 - start;
-#pragma unroll 1
-  for (int first = 0; first < count; first += 32) {
-    const int nth = first + lane, key = nth < sinks ? nth : nth - sinks + start;
-    float score = -INFINITY;
-    if (nth < count) {
-      const T* from = k + key * p.k_strides[2];
-      score = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < p.head_dim; ++c) score = fmaf(to_compute(q[c]), to_compute(from[c]), score);
-      score *= p.scale_log2;
-    }
-    float top = score;
-#pragma unroll
-    for (int offset = 16; offset > 0; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-    top = fmaxf(top, most);
-    const float factor = most == top ? 1.f : exp2_ftz(most - top);
-    most = top;
-    const float weight = nth < count ? exp2_ftz(score - (top == -INFINITY ? 0.f : top)) : 0.f;
-    total = total * factor + warp_sum(weight);
-#pragma unroll
-    for (int c = 0; c < kMine; ++c) result[c] *= factor;
-#pragma unroll 1
-    for (int i = 0; i < min(32, count - first); ++i) {
-      const float w = __shfl_sync(0xffffffffu, weight, i);
-      const T* from = v + __shfl_sync(0xffffffffu, key, i) * p.v_strides[2];
-#pragma unroll
-      for (int c = 0; c < kMine; ++c) {
-        const int column = c * 32 + lane;
-        if (column < p.head_dim) result[c] = fmaf(w, to_compute(from[column]), result[c]);
-      }
-    }
-  }
-  T* out = static_cast<T*>(p.out) + batch * p.out_batch + head * p.out_head + row * p.out_token;
-#pragma unroll
-  for (int c = 0; c < kMine; ++c) {
-    const int column = c * 32 + lane;
-    if (column < p.head_dim) out[column] = from_compute<T, float>(result[c] / total);
-  }
-  __syncwarp();
-}
-
-template <typename T, int D, int KEYS, bool FEW, bool WINDOW = false>
+template <typename T, int D, int KEYS, bool FEW>
 __global__ void __launch_bounds__(kAttnThreads, AttnLayout<D, KEYS, FEW>::kCtasPerSm)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const std::conditional_t<WINDOW, WindowAttnParams, AttnParams> p) {
+                 const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
   using L = AttnLayout<D, KEYS, FEW>;
   constexpr int kKeys = KEYS;
   constexpr bool kAhead = KEYS < 128;      // the reference point takes the second tile's scores too
@@ -264,24 +202,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int q0 = q_block * kRows;
   const int key_tiles = (p.k_tokens + kKeys - 1) / kKeys;
   // under a causal mask only the key tiles that hold a key <= the CTA's last row; at least one step
-  int steps = p.causal ? min(key_tiles, (min(q0 + kRows, p.q_tokens) - 1) / kKeys + 1) : key_tiles;
-  // Under a window: the tiles that hold a key some row of the CTA sees, those of the sinks and then those from the first row's window to the last
-  // row; at least one.
-  int sink_tiles = 0, gap = 0, key_head = head;      // the tiles left out behind the sinks'
-  if constexpr (WINDOW) {
-    const int low = q0 + p.offset, high = min(q0 + kRows, p.q_tokens) - 1 + p.offset;       // positions
-    const int stop = (max(high, -1) + kKeys) / kKeys, start = min(max(low - p.window + 1, 0) / kKeys, stop);
-    sink_tiles = min((min(p.sinks, max(high, -1) + 1) + kKeys - 1) / kKeys, start);
-    gap = start - sink_tiles;
-    steps = max(stop - gap, 1);
-    key_head = head / p.group;
-  }
-  auto first_key = [&](int j) { return (WINDOW && j >= sink_tiles ? j + gap : j) * kKeys; };      // of step j's tile
+  const int steps = p.causal ? min(key_tiles, (min(q0 + kRows, p.q_tokens) - 1) / kKeys + 1) : key_tiles;
 
   auto load_tile = [&](const CUtensorMap* map, uint32_t ring, uint32_t full, int j) {
     barrier_expect_tx(full, kTileBytes);
     for (int h = 0; h < kSubTiles; ++h)
-      tma_load_4d(base + ring + (j % kRing) * kTileBytes + h * kSubTileBytes, map, full, h * kHeadDim, first_key(j), key_head, batch);
+      tma_load_4d(base + ring + (j % kRing) * kTileBytes + h * kSubTileBytes, map, full, h * kHeadDim, j * kKeys, head, batch);
   };
 
   // The producer lane sets the barriers up and fills the rings for the first time before the CTA meets: the
@@ -441,32 +367,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_load_wait();
     };
     auto mask = [&](Scores& r, int key0) {
-      if constexpr (WINDOW) {
-        const int low = q0 + p.offset, position = query + p.offset;
-        if (key0 + kKeys - 1 > low) {                 // (all three uniform in the CTA)
-          const int limit = position - key0;
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i) {
-            if (i > limit) r[i] = 0xff800000u;
-          }
-        }
-        if (key0 <= low + kRows - 1 - p.window) {
-          const int from = position - p.window + 1 - key0;
-          if (key0 >= p.sinks) {
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-              if (i < from) r[i] = 0xff800000u;
-            }
-          } else if (key0 + kKeys > p.sinks) {
-            const int sinks = p.sinks - key0;
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-              if (i < from && i >= sinks) r[i] = 0xff800000u;
-            }
-          }
-        }
-        return;
-      }
       if (key0 + kKeys - 1 > open_until) {            // uniform in the CTA
         const int limit = last_allowed - key0;        // columns > limit are masked for this row
 #pragma unroll
@@ -497,7 +397,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         Scores r;
         tcgen05_fence_after();
         load_scores(r, tmem_o);
-        mask(r, first_key(1));
+        mask(r, kKeys);
         second_max = maximum(r);
       }
     }
@@ -510,7 +410,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) barrier_arrive(s_free);
-      mask(r, first_key(j));
+      mask(r, j * kKeys);
       const float tile_max = maximum(r);
       // The reference point: the first two tiles' maximum, moved only when a tile rises more than
       // 2^kSlack above it (from -inf, any finite maximum does). `factor` rescales what the row has
@@ -578,9 +478,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       // the result row leaves tensor memory 32 columns at a time (the loads are warp-wide: every lane takes
       // part, rows beyond the queries only skip the stores)
       const bool stores = query < p.q_tokens;
-      const bool sees_some = !WINDOW || query + (p.k_tokens - p.q_tokens) >= 0;      // else: zeros
-      const float inverse = sees_some ? 1.0f / row_sum : 0.f;
-      bool odd = false;                                  // something in the row is no finite number
+      const float inverse = 1.0f / row_sum;
       T* out_row = static_cast<T*>(p.out) + batch * p.out_batch + head * p.out_head + static_cast<long long>(query) * p.out_token;
       const bool vector_ok = (reinterpret_cast<uintptr_t>(out_row) & 15) == 0;
       const int width = p.head_dim;       // a multiple of 8: whole 16-byte vectors
@@ -590,13 +488,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         uint32_t o[32];
         tmem_load_32(tmem_o + c * 32, o);
         tmem_load_wait();
-        if constexpr (WINDOW) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!sees_some) o[i] = 0;
-            odd |= !(fabsf(__uint_as_float(o[i]) * inverse) < INFINITY);
-          }
-        }
         if (stores && vector_ok) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -617,15 +508,439 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         __syncwarp();
       }
-      // The products above take every key of a tile, at a probability of zero where a row does not see it, and zero times an infinity or a NaN is
-      // a NaN. So a row that came out with one is taken again from its own keys alone, by the warp, in plain f32: slow, and rare on real data.
-      if constexpr (WINDOW) {
-        uint32_t again = __ballot_sync(0xffffffffu, odd && stores);
-        while (again != 0) {
-          const int row = q0 + warp * 32 + __ffs(again) - 1;
-          again &= again - 1;
-          take_row_again<T, D>(p, batch, head, key_head, row);
+    }
+  }
+
+  // ---- teardown: every thread arrives here, also after a wait that gave up -------------------
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tcgen05_fence_after();
+    if constexpr (L::kTwoAllocations) tmem_dealloc(tmem_p, kTmemColumnsP);
+    tmem_dealloc(tmem_base, L::kTmemColumns);
+  }
+}
+
+// ---- With a window, sinks and shared key heads ------------------------------------------------------
+//
+// The same products, softmax and hand-overs as above, for rows that see the keys j <= p with j > p - window or j < sinks (p = row + k_tokens -
+// q_tokens): a block of rows walks the tiles of the sinks and then those from its first row's window to its last row. Under a short
+// window such a walk is a few steps, and a CTA's start (barriers, tensor memory, first loads: about 8 us of latency beside 0.9 a step) would be most of
+// it; so CTAs stay, as many as fit, and take blocks one after another. Counted through all blocks, step g of a CTA has ring stage g % kRing and the phases
+// that g gives, and the first loads and scores of the next block run under the last step and the result of the one before: its query tile is loaded
+// once the last scores of that block are out (q_empty), and its first product writes the result columns only after p_full, which the
+// softmax warps signal when they have read the result before it.
+//
+// Blocks are dealt out by length, the longest of all heads first, so that CTAs get sums of about the same length.
+// With a window: what a query sees (keyed.h), which key head it shares, and, for rows whose result has to be taken again, where the operands lie.
+struct WindowAttnParams : AttnParams {
+  int group, offset;               // heads a key head serves; k_tokens - q_tokens
+  int window, sinks;
+  const void *q, *k, *v;
+  long long q_strides[3], k_strides[3], v_strides[3];
+};
+
+struct WindowBlock {
+  int q0, head, batch, key_head;
+  int sink_tiles, gap, steps;        // tiles of the sinks; tiles left out behind them; at least one step
+};
+template <int KEYS>
+__device__ __forceinline__ WindowBlock window_block(const WindowAttnParams& p, int item) {
+  WindowBlock b;
+  const int heads = p.batch * p.heads, head_index = item % heads;
+  b.q0 = (p.q_blocks - 1 - item / heads) * kRows;
+  b.head = head_index % p.heads;
+  b.batch = head_index / p.heads;
+  b.key_head = b.head / p.group;
+  const int low = b.q0 + p.offset, high = min(b.q0 + kRows, p.q_tokens) - 1 + p.offset;       // positions
+  const int stop = (max(high, -1) + KEYS) / KEYS, start = min(max(low - p.window + 1, 0) / KEYS, stop);
+  b.sink_tiles = min((min(p.sinks, max(high, -1) + 1) + KEYS - 1) / KEYS, start);
+  b.gap = start - b.sink_tiles;
+  b.steps = max(stop - b.gap, 1);
+  return b;
+}
+
+// One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a lane for the result.
+template <typename T, int D>
+__device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int batch, int head, int key_head, int row) {
+  const int lane = threadIdx.x & 31, position = row + p.offset;
+  const T* q = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + row * p.q_strides[2];
+  const T* k = static_cast<const T*>(p.k) + batch * p.k_strides[0] + key_head * p.k_strides[1];
+  const T* v = static_cast<const T*>(p.v) + batch * p.v_strides[0] + key_head * p.v_strides[1];
+  constexpr int kMine = D / 32;
+  float most = -INFINITY, total = 0.f, result[kMine];
+#pragma unroll
+  for (int c = 0; c < kMine; ++c) result[c] = 0.f;
+  const int start = max(position - p.window + 1, 0), sinks = min(min(p.sinks, position + 1), start);
+  const int count = sinks + position + 1 - start;
+#pragma unroll 1
+  for (int first = 0; first < count; first += 32) {
+    const int nth = first + lane, key = nth < sinks ? nth : nth - sinks + start;
+    float score = -INFINITY;
+    if (nth < count) {
+      const T* from = k + key * p.k_strides[2];
+      score = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < p.head_dim; ++c) score = fmaf(to_compute(q[c]), to_compute(from[c]), score);
+      score *= p.scale_log2;
+    }
+    float top = score;
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+    top = fmaxf(top, most);
+    const float factor = most == top ? 1.f : exp2_ftz(most - top);
+    most = top;
+    const float weight = nth < count ? exp2_ftz(score - (top == -INFINITY ? 0.f : top)) : 0.f;
+    total = total * factor + warp_sum(weight);
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) result[c] *= factor;
+#pragma unroll 1
+    for (int i = 0; i < min(32, count - first); ++i) {
+      const float w = __shfl_sync(0xffffffffu, weight, i);
+      const T* from = v + __shfl_sync(0xffffffffu, key, i) * p.v_strides[2];
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) {
+        const int column = c * 32 + lane;
+        if (column < p.head_dim) result[c] = fmaf(w, to_compute(from[column]), result[c]);
+      }
+    }
+  }
+  T* out = static_cast<T*>(p.out) + batch * p.out_batch + head * p.out_head + row * p.out_token;
+#pragma unroll
+  for (int c = 0; c < kMine; ++c) {
+    const int column = c * 32 + lane;
+    if (column < p.head_dim) out[column] = from_compute<T, float>(result[c] / total);
+  }
+  __syncwarp();
+}
+
+template <typename T, int D, int KEYS>
+__global__ void __launch_bounds__(kAttnThreads, AttnLayout<D, KEYS, false>::kCtasPerSm)
+window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, const WindowAttnParams p) {
+  using L = AttnLayout<D, KEYS, false>;
+  constexpr int kKeys = KEYS, kRing = L::kRing, kSubTiles = L::kSubTiles;
+  constexpr uint32_t kSubTileBytes = L::kSubTileBytes, kTileBytes = L::kTileBytes, kOffsetK = L::kOffsetK, kOffsetV = L::kOffsetV;
+  constexpr uint32_t kOffsetBarriers = L::kOffsetBarriers, kColumnO = L::kColumnO;
+  extern __shared__ unsigned char raw_smem[];
+  const uint32_t base = (smem_address(raw_smem) + 1023u) & ~1023u;
+  unsigned char* aligned = raw_smem + (base - smem_address(raw_smem));
+  const uint32_t barriers = base + kOffsetBarriers;
+  const uint32_t q_full = barriers;
+  auto k_full = [&](uint32_t s) { return barriers + 8u * (1 + s); };
+  auto k_empty = [&](uint32_t s) { return barriers + 8u * (1 + kRing + s); };
+  auto v_full = [&](uint32_t s) { return barriers + 8u * (1 + 2 * kRing + s); };
+  auto v_empty = [&](uint32_t s) { return barriers + 8u * (1 + 3 * kRing + s); };
+  const uint32_t s_full = barriers + 8u * (1 + 4 * kRing), s_free = s_full + 8, p_full = s_full + 16, pv_done = s_full + 24;
+  const uint32_t q_empty = s_full + 32;                         // all scores of a block are out: its queries are spent
+  constexpr int kBarrierCount = 1 + 4 * kRing + 5;
+  const uint32_t tmem_slot = barriers + 8u * kBarrierCount;
+  volatile uint32_t* tmem_slot_pointer = reinterpret_cast<volatile uint32_t*>(aligned + kOffsetBarriers + 8 * kBarrierCount);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int items = p.q_blocks * p.batch * p.heads;
+
+  auto load_queries = [&](const WindowBlock& b) {
+    barrier_expect_tx(q_full, kSubTiles * kQueryBytes);
+    for (int h = 0; h < kSubTiles; ++h) tma_load_4d(base + h * kQueryBytes, &map_q, q_full, h * kHeadDim, b.q0, b.head, b.batch);
+  };
+  // step j of a block, the CTA's step g
+  auto load_tile = [&](const CUtensorMap* map, uint32_t ring, uint32_t full, const WindowBlock& b, int j, uint32_t g) {
+    barrier_expect_tx(full, kTileBytes);
+    const int key = (j < b.sink_tiles ? j : j + b.gap) * kKeys;
+    for (int h = 0; h < kSubTiles; ++h)
+      tma_load_4d(base + ring + (g % kRing) * kTileBytes + h * kSubTileBytes, map, full, h * kHeadDim, key, b.key_head, b.batch);
+  };
+
+  const int early = min(window_block<KEYS>(p, blockIdx.x).steps, kRing);      // steps of the first block whose tiles are loaded before the CTA meets
+  if (warp == 4 && elect_one()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    if (blockIdx.x == 0) p.status.begin();
+    barrier_init(q_full, 1);
+    for (int s = 0; s < kRing; ++s) {
+      barrier_init(k_full(s), 1);
+      barrier_init(k_empty(s), 1);
+      barrier_init(v_full(s), 1);
+      barrier_init(v_empty(s), 1);
+    }
+    barrier_init(s_full, 1);
+    barrier_init(pv_done, 1);
+    barrier_init(p_full, kRows / 32);
+    barrier_init(s_free, kRows / 32);
+    barrier_init(q_empty, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    const WindowBlock b = window_block<KEYS>(p, blockIdx.x);
+    load_queries(b);
+    for (int j = 0; j < early; ++j) load_tile(&map_k, kOffsetK, k_full(j), b, j, j);
+    for (int j = 0; j < early; ++j) load_tile(&map_v, kOffsetV, v_full(j), b, j, j);
+  }
+  if (warp == 5) {
+    if constexpr (L::kTwoAllocations) {
+      tmem_alloc_more(tmem_slot, L::kTmemColumns);
+      tmem_alloc(tmem_slot + 4, kTmemColumnsP);
+    } else {
+      tmem_alloc(tmem_slot, L::kTmemColumns);
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_slot_pointer[0];
+  const uint32_t tmem_p = L::kTwoAllocations ? tmem_slot_pointer[1] : tmem_base + L::kColumnP;
+
+  if (L::kMovesRegisters && warp >= 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegisters));
+  if (warp == 4) {
+    // ---- producer --------------------------------------------------------------------------------
+    if (elect_one()) {
+      uint32_t g = 0, block = 0, keys_loaded = early, values_loaded = early, queries_of = 0;      // steps and blocks before this one, what was asked for
+      bool alive = true;
+      for (int item = blockIdx.x; alive && item < items; item += gridDim.x, ++block) {
+        const WindowBlock b = window_block<KEYS>(p, item);
+        for (int j = block == 0 ? early : 0; alive && j < b.steps; ++j) {
+          const uint32_t n = g + j, phase = (n / kRing) & 1;
+          alive = barrier_wait(k_empty(n % kRing), phase ^ 1, p.status, kWaitKeyEmpty);
+          if (!alive) break;
+          load_tile(&map_k, kOffsetK, k_full(n % kRing), b, j, n);
+          keys_loaded = n + 1;
+          if (j == 0) {      // (of a later block)
+            alive = barrier_wait(q_empty, (block - 1) & 1, p.status, kWaitQ);
+            if (!alive) break;
+            load_queries(b);
+            queries_of = block;
+          }
+          alive = barrier_wait(v_empty(n % kRing), phase ^ 1, p.status, kWaitValueEmpty);
+          if (!alive) break;
+          load_tile(&map_v, kOffsetV, v_full(n % kRing), b, j, n);
+          values_loaded = n + 1;
         }
+        g += b.steps;
+      }
+      if (!alive) {      // what is under way has to land before the CTA leaves
+        auto landed = [&](uint32_t bar, uint32_t parity) {
+          for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(bar, parity); ++spin) {
+          }
+        };
+        landed(q_full, queries_of & 1);
+        for (uint32_t n = keys_loaded > kRing ? keys_loaded - kRing : 0; n < keys_loaded; ++n) landed(k_full(n % kRing), (n / kRing) & 1);
+        for (uint32_t n = values_loaded > kRing ? values_loaded - kRing : 0; n < values_loaded; ++n) landed(v_full(n % kRing), (n / kRing) & 1);
+      }
+    }
+  } else if (warp == 5) {
+    // ---- issuer ----------------------------------------------------------------------------------
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = attn_instruction_descriptor<T>(kKeys, false);
+      constexpr uint32_t idesc_o = attn_instruction_descriptor<T>(kHeadDim, true);
+      constexpr uint32_t kHighWord = kDescriptorHigh;
+      const uint32_t low_q = descriptor_low(base, 0), low_k = descriptor_low(base + kOffsetK, 0);
+      const uint32_t low_v = descriptor_low(base + kOffsetV, kSubTileBytes);
+      // the scores of step g, once its keys (and a block's queries) are there and the softmax warps hold the scores before in registers
+      auto scores = [&](uint32_t g, bool ends) {
+        if (!barrier_wait(k_full(g % kRing), (g / kRing) & 1, p.status, kWaitKeyFull)) return false;
+        if (g > 0 && !barrier_wait(s_free, (g - 1) & 1, p.status, kWaitBufferFree)) return false;
+        tcgen05_fence_after();
+        const uint32_t k = low_k + (g % kRing) * (kTileBytes >> 4);
+#pragma unroll
+        for (int h = 0; h < kSubTiles; ++h) {
+#pragma unroll
+          for (int kk = 0; kk < kHeadDim / 16; ++kk)
+            mma_f16_split(tmem_base, low_q + h * (kQueryBytes >> 4) + kk * 2, kHighWord, k + h * (kSubTileBytes >> 4) + kk * 2, kHighWord, idesc_s,
+                          (h != 0 || kk != 0) ? 1u : 0u);
+        }
+        mma_commit(s_full);
+        if (ends) mma_commit(q_empty);
+        return true;
+      };
+      auto partial = [&](uint32_t g, bool first) {
+        if (!barrier_wait(v_full(g % kRing), (g / kRing) & 1, p.status, kWaitValueFull)) return false;
+        if (!barrier_wait(p_full, g & 1, p.status, kWaitProbabilities)) return false;
+        tcgen05_fence_after();
+        const uint32_t v = low_v + (g % kRing) * (kTileBytes >> 4);
+#pragma unroll
+        for (int h = 0; h < kSubTiles; ++h) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_f16_tmem_a(tmem_base + kColumnO + h * kHeadDim, tmem_p + kk * 8, v + h * (kSubTileBytes >> 4) + kk * (2048 >> 4), kHighWord, idesc_o,
+                           (!first || kk != 0) ? 1u : 0u);
+        }
+        mma_commit(pv_done);
+        return true;
+      };
+      uint32_t g = 0, block = 0;
+      int item = blockIdx.x, left = window_block<KEYS>(p, item).steps;      // of the block of step g, g among them
+      bool first = true;                                                     // step g is the first of its block
+      bool alive = barrier_wait(q_full, 0, p.status, kWaitQ) && scores(0, left == 1);
+      while (alive) {
+        if (left > 1) {      // the scores of the block's next step, then the product of this one
+          alive = scores(g + 1, left == 2) && partial(g, first);
+          first = false;
+          --left;
+        } else {             // the block's last product first: its result is what the softmax warps wait for
+          alive = partial(g, first);
+          item += gridDim.x;
+          if (!alive || item >= items) break;
+          left = window_block<KEYS>(p, item).steps;
+          first = true;
+          alive = barrier_wait(q_full, ++block & 1, p.status, kWaitQ) && scores(g + 1, left == 1);
+        }
+        ++g;
+      }
+    }
+  } else if (warp < 4) {
+    // ---- softmax ---------------------------------------------------------------------------------
+    if constexpr (L::kMovesRegisters) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegisters));
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t tmem_s = tmem_base + lanes, tmem_o = tmem_base + kColumnO + lanes, tmem_mine = tmem_p + lanes;
+    uint32_t g = 0;
+    bool alive = true;
+    auto wait_product = [&](uint32_t n) {
+      if (!barrier_wait(pv_done, n & 1, p.status, kWaitPartial)) return false;
+      tcgen05_fence_after();
+      if (threadIdx.x == 0) barrier_arrive(v_empty(n % kRing));
+      return true;
+    };
+    for (int item = blockIdx.x; alive && item < items; item += gridDim.x) {
+      const WindowBlock b = window_block<KEYS>(p, item);
+      const int query = b.q0 + static_cast<int>(threadIdx.x), position = query + p.offset, low = b.q0 + p.offset;
+      float reference = -INFINITY, row_sum = 0.f;
+      for (int j = 0; j < b.steps; ++j, ++g) {
+        alive = barrier_wait(s_full, g & 1, p.status, kWaitScores);
+        if (!alive) break;
+        tcgen05_fence_after();
+        if (threadIdx.x == 0) barrier_arrive(k_empty(g % kRing));
+        uint32_t r[kKeys];
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 32) tmem_load_32(tmem_s + i, *reinterpret_cast<uint32_t(*)[32]>(&r[i]));
+        tmem_load_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(s_free);
+        // masks (the conditions are uniform in the CTA)
+        const int key0 = (j < b.sink_tiles ? j : j + b.gap) * kKeys;
+        if (key0 + kKeys - 1 > low) {
+          const int limit = position - key0;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) {
+            if (i > limit) r[i] = 0xff800000u;
+          }
+        }
+        if (key0 <= low + kRows - 1 - p.window) {
+          const int from = position - p.window + 1 - key0;
+          if (key0 >= p.sinks) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+              if (i < from) r[i] = 0xff800000u;
+            }
+          } else if (key0 + kKeys > p.sinks) {
+            const int sinks = p.sinks - key0;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+              if (i < from && i >= sinks) r[i] = 0xff800000u;
+            }
+          }
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 8) {
+          m0 = max3(m0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          m1 = max3(m1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+          m2 = max3(m2, __uint_as_float(r[i + 4]), __uint_as_float(r[i + 5]));
+          m3 = max3(m3, __uint_as_float(r[i + 6]), __uint_as_float(r[i + 7]));
+        }
+        const float tile_max = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        float factor = 1.f;
+        const bool moves = j == 0 || (tile_max - reference) * p.scale_log2 > kSlack;       // false for NaN
+        if (moves) {
+          if (j != 0) factor = exp2_ftz((reference - tile_max) * p.scale_log2);             // from -inf: 0, and nothing was gathered
+          reference = tile_max;
+        }
+        const bool rescale = j != 0 && __any_sync(0xffffffffu, moves);
+        const float shift = reference == -INFINITY ? 0.f : -reference * p.scale_log2;
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+        uint32_t packed[kKeys / 2];
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
+#pragma unroll
+        for (int chunk = 0; chunk < kKeys / 4; ++chunk) {
+          const float2 t0 = __ffma2_rn(make_float2(__uint_as_float(r[chunk * 4 + 0]), __uint_as_float(r[chunk * 4 + 1])), scale2, shift2);
+          const float2 t1 = __ffma2_rn(make_float2(__uint_as_float(r[chunk * 4 + 2]), __uint_as_float(r[chunk * 4 + 3])), scale2, shift2);
+          const float2 e0 = make_float2(exp2_ftz(t0.x), exp2_ftz(t0.y));
+          const float2 e1 = make_float2(exp2_ftz(t1.x), exp2_ftz(t1.y));
+          sum0 = __fadd2_rn(sum0, e0);
+          sum1 = __fadd2_rn(sum1, e1);
+          packed[chunk * 2 + 0] = pack_pair<T>(e0.x, e0.y);
+          packed[chunk * 2 + 1] = pack_pair<T>(e1.x, e1.y);
+        }
+        const float2 sum01 = __fadd2_rn(sum0, sum1);
+        row_sum = row_sum * factor + (sum01.x + sum01.y);
+        if (j > 0) {
+          alive = wait_product(g - 1);
+          if (!alive) break;
+          if (rescale) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_load_16(tmem_o + c * 16, o);
+              tmem_load_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_store_16(tmem_o + c * 16, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; i += 32) tmem_store_32(tmem_mine + i, *reinterpret_cast<uint32_t(*)[32]>(&packed[i]));
+        tmem_store_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(p_full);
+      }
+      if (!alive || !wait_product(g - 1)) {
+        alive = false;
+        break;
+      }
+      // the result row leaves tensor memory 32 columns at a time (every lane takes part; rows beyond the queries only skip the stores)
+      const bool stores = query < p.q_tokens, sees_some = position >= 0;      // a query before the first key: zeros
+      const float inverse = sees_some ? 1.0f / row_sum : 0.f;
+      T* out_row = static_cast<T*>(p.out) + b.batch * p.out_batch + b.head * p.out_head + static_cast<long long>(query) * p.out_token;
+      const bool vector_ok = (reinterpret_cast<uintptr_t>(out_row) & 15) == 0;
+      bool odd = false;                                  // something in the row is no finite number
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        if (c * 32 >= p.head_dim) break;
+        uint32_t o[32];
+        tmem_load_32(tmem_o + c * 32, o);
+        tmem_load_wait();
+        float value[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          value[i] = sees_some ? __uint_as_float(o[i]) * inverse : 0.f;
+          odd |= !(fabsf(value[i]) < INFINITY);
+        }
+        if (stores && vector_ok) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (c * 32 + v * 8 < p.head_dim) {
+              *reinterpret_cast<uint4*>(out_row + c * 32 + v * 8) =
+                  make_uint4(pack_pair<T>(value[v * 8], value[v * 8 + 1]), pack_pair<T>(value[v * 8 + 2], value[v * 8 + 3]),
+                             pack_pair<T>(value[v * 8 + 4], value[v * 8 + 5]), pack_pair<T>(value[v * 8 + 6], value[v * 8 + 7]));
+            }
+          }
+        } else if (stores) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (c * 32 + i < p.head_dim) out_row[c * 32 + i] = from_compute<T, float>(value[i]);
+          }
+        }
+        __syncwarp();
+      }
+      tcgen05_fence_before();
+      // The products take every key of a tile, at a probability of zero where a row does not see it, and zero times an infinity or a NaN is a
+      // NaN. So a row that came out with one is taken again from its own keys alone, by the warp, in plain f32: slow, and rare on real data.
+      uint32_t again = __ballot_sync(0xffffffffu, odd && stores);
+      while (again != 0) {
+        const int row = b.q0 + warp * 32 + __ffs(again) - 1;
+        again &= again - 1;
+        take_row_again<T, D>(p, b.batch, b.head, b.key_head, row);
       }
     }
   }
@@ -749,7 +1064,7 @@ int window_tile_keys(const KeyedParams& p, long long sms) {
   return ctas <= at_once || (!wide && keys >= 2048) ? 128 : 64;
 }
 
-tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, cudaStream_t stream) {
+tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, int sms, cudaStream_t stream) {
   CUtensorMap map_q, map_k, map_v;
   const int64_t q_strides[3] = {from.q_strides[0], from.q_strides[1], from.q_strides[2]}, k_strides[3] = {from.k_strides[0], from.k_strides[1], from.k_strides[2]},
                 v_strides[3] = {from.v_strides[0], from.v_strides[1], from.v_strides[2]};
@@ -782,18 +1097,19 @@ tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, cudaSt
     p.k_strides[i] = from.k_strides[i];
     p.v_strides[i] = from.v_strides[i];
   }
-  const long long ctas = static_cast<long long>(p.q_blocks) * p.heads * p.batch;
-  TQ_REQUIRE(ctas < (1LL << 31), TQ_UNSUPPORTED, "too many query blocks for one launch");
+  const long long blocks = static_cast<long long>(p.q_blocks) * p.heads * p.batch;
+  TQ_REQUIRE(blocks < (1LL << 30), TQ_UNSUPPORTED, "too many query blocks for one launch");
   auto go = [&](auto width, auto step) -> tq_status {
     constexpr int kWidth = decltype(width)::value, kKeys = decltype(step)::value;
     constexpr size_t smem = AttnLayout<kWidth, kKeys, false>::kSmemBytes;
     auto start = [&](auto kernel) -> tq_status {
       TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-      kernel<<<static_cast<unsigned>(ctas), kAttnThreads, smem, stream>>>(map_q, map_k, map_v, p);
-      return check_launch("attention_kernel (window)");
+      const long long fit = static_cast<long long>(sms) * AttnLayout<kWidth, kKeys, false>::kCtasPerSm;
+      kernel<<<static_cast<unsigned>(blocks < fit ? blocks : fit), kAttnThreads, smem, stream>>>(map_q, map_k, map_v, p);
+      return check_launch("window_attention_kernel");
     };
-    if (dtype == TQ_BF16) return start(attention_kernel<__nv_bfloat16, kWidth, kKeys, false, true>);
-    return start(attention_kernel<__half, kWidth, kKeys, false, true>);
+    if (dtype == TQ_BF16) return start(window_attention_kernel<__nv_bfloat16, kWidth, kKeys>);
+    return start(window_attention_kernel<__half, kWidth, kKeys>);
   };
   auto with_keys = [&](auto width) {
     return keys == 128 ? go(width, std::integral_constant<int, 128>{}) : go(width, std::integral_constant<int, 64>{});
@@ -991,6 +1307,6 @@ extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, c
   p.k_tokens = static_cast<int>(k_tokens);
   tq::keyed_extents(p, batch, heads, kv_heads, q_tokens, head_dim, scale, window, sinks);
   const int tile_keys = tq::window_tile_keys(p, tq::sm_count(device));
-  if (tile_keys != 0) return tq::window_tiles(dtype, p, tile_keys, static_cast<cudaStream_t>(stream));
+  if (tile_keys != 0) return tq::window_tiles(dtype, p, tile_keys, tq::sm_count(device), static_cast<cudaStream_t>(stream));
   return tq::keyed_attention(dtype, false, p, k_tokens, workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }
