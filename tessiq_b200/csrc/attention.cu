@@ -540,6 +540,13 @@ struct WindowAttnParams : AttnParams {
   long long q_strides[3], k_strides[3], v_strides[3];
 };
 
+// The first n of 32 bits; none for n <= 0, all for n >= 32.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+  uint32_t bits;
+  asm("shl.b32 %0, 1, %1;" : "=r"(bits) : "r"(min(max(n, 0), 32)));      // (shifted by 32: 0)
+  return bits - 1;
+}
+
 struct WindowBlock {
   int q0, head, batch, key_head;
   int sink_tiles, gap, steps;        // tiles of the sinks; tiles left out behind them; at least one step
@@ -815,27 +822,17 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) barrier_arrive(s_free);
-        // masks (the conditions are uniform in the CTA)
+        // Masks, where the tile has a key that some row does not see (uniform in the CTA): what the row sees as bits, 32 keys a word, which the compiler turns into
+        // predicates eight at a time; two comparisons and selections for each key were half of all instructions under a window of 64.
         const int key0 = (j < b.sink_tiles ? j : j + b.gap) * kKeys;
-        if (key0 + kKeys - 1 > low) {
-          const int limit = position - key0;
+        if (key0 + kKeys - 1 > low || (key0 <= low + kRows - 1 - p.window && key0 + kKeys > p.sinks)) {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) {
-            if (i > limit) r[i] = 0xff800000u;
-          }
-        }
-        if (key0 <= low + kRows - 1 - p.window) {
-          const int from = position - p.window + 1 - key0;
-          if (key0 >= p.sinks) {
+          for (int i0 = 0; i0 < kKeys; i0 += 32) {
+            const int at = key0 + i0;
+            const uint32_t sees = first_bits(position + 1 - at) & (~first_bits(position - p.window + 1 - at) | first_bits(p.sinks - at));
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-              if (i < from) r[i] = 0xff800000u;
-            }
-          } else if (key0 + kKeys > p.sinks) {
-            const int sinks = p.sinks - key0;
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-              if (i < from && i >= sinks) r[i] = 0xff800000u;
+            for (int i = 0; i < 32; ++i) {
+              if (!(sees >> i & 1)) r[i0 + i] = 0xff800000u;
             }
           }
         }
