@@ -298,8 +298,10 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   if (lane == 0) {
     for (int st = 0; st < kKeyedStages; ++st) barrier_init(barrier0 + 8 * st, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    if ((BITS == 8 ? p.pages : p.k_tokens) > 0) {      // (else there is no map)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
     if (blockIdx.x == 0 && warp == 0) p.status.begin();
   }
   __syncwarp();
@@ -1120,6 +1122,8 @@ int resident(int32_t device, size_t smem) {
   std::lock_guard<std::mutex> lock(mutex);
   if (known[device] == 0) {
     int per_sm = 0;
+    DeviceScope device_scope(device);
+    if (device_scope.status() != TQ_OK) return 2 * 148;      // (a plan without a GPU)
     if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, kKeyedThreads, smem) != cudaSuccess || per_sm <= 0) {
       cudaGetLastError();

@@ -360,7 +360,7 @@ def release_workspaces() -> None:
 
 
 class DeviceWaitError(RuntimeError):
-    """A bounded wait inside one of the library's kernels gave up (tq_status_poll)."""
+    """A bounded wait inside one of the library's kernels gave up, or one could not follow a cache's table (tq_status_poll)."""
 
 
 _WAIT_CODES = {0x53454c46: "the bounded-wait self test", 0x504e4c31: "panel normalisation: a panel's flag never went up",
@@ -382,6 +382,9 @@ def check_status(device: int = 0, stream: int | None = None) -> None:
     check(lib.tq_status_poll(device, ctypes.c_void_p(stream or 0), ctypes.byref(code)))
     if code.value != 0:
         what = _WAIT_CODES.get(code.value, "a tensor-core kernel's pipeline wait")
+        if code.value in (0x50414745, 0x4c454e47):
+            raise DeviceWaitError(f"a cache launch on device {device} left out what it could not follow: {what}; sequence {words[3]}, "
+                                  f"{'block' if code.value == 0x50414745 else 'length or start'} {words[4]}")
         raise DeviceWaitError(f"a bounded wait on device {device} gave up: code {code.value:#x} ({what}); "
                               f"CTA {words[1]}, thread {words[2]}, detail {list(words[3:7])}")
 

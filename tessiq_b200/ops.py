@@ -601,7 +601,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True
     reads key head h // (heads // kv_heads)). Query i stands at position p = k_tokens - q_tokens + i, so one query against a cache is
     its last token, and sees the keys j <= p with j > p - window or j < sinks; `window` None: all of j <= p. A query before the
     first key gives zeros. What lies in keys a query does not see (NaN too) does not reach its result. Types, widths, strides and
-    `token_major` as for `attention`."""
+    `token_major` as for `attention`; as everywhere here, no gradient is recorded."""
     given = (q, k, v, window, sinks, scale, token_major)
     out = _call(_CODES["window attention"], *given)
     if out is not None:
@@ -747,7 +747,8 @@ def copy_pages(tensors, sources, targets, page_axis=0) -> None:
         one.page_stride = max(t.stride(page_axis) * size, one.page_bytes if pages == 1 else 0)
     device = _device_of(tensors)
     numbers = ctypes.c_int64 * len(sources)
-    check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*sources), numbers(*targets), len(sources), device, _stream(None, device)))
+    check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*map(int, sources)), numbers(*map(int, targets)), len(sources), device,
+                                   _stream(None, device)))
 
 
 # ---------------------------------------------------------------------------------------------

@@ -250,6 +250,29 @@ def test_cache_attention(tq, case, dtype):
     assert status() == 0
 
 
+@pytest.mark.parametrize("case", [(24, 16, 4, 1, 64, 64, None, 0, 2500), (40, 16, 8, 2, 128, 32, 700, 4, 1500), (1, 8, 1, 1, 128, 64, None, 0, 20000),
+                                  (2, 6, 2, 3, 80, 16, 9000, 40, 12000), (300, 2, 1, 1, 64, 16, None, 0, 1600)], ids=lambda c: "-".join(map(str, c)))
+def test_chunks_dealt_out_over_the_gpu(tq, case):
+    """Sequences of all lengths in one batch, some empty: every form of the split, checked at some of them."""
+    batch, heads, kv_heads, queries, width, page, window, sinks, longest = case
+    lengths = [longest * (b * 7 % batch + 1) // batch if b % 5 else b % 3 for b in range(batch)]
+    lengths[-1] = longest
+    blocks = -(-longest // page)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = batch * blocks
+    codes = [(torch.randn(pages, kv_heads, page, width, device="cuda", generator=g) * 60).clamp_(-448, 448).to(E4M3) for _ in range(2)]
+    scales = [torch.exp2(torch.randn(pages, kv_heads, device="cuda", generator=g) - 6) for _ in range(2)]
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32).reshape(batch, blocks)
+    q = by_token((batch, heads, queries, width), torch.bfloat16, 1)
+    got = tq.cache_attention(q, *codes, *scales, table, torch.tensor(lengths, dtype=torch.int32).cuda(), window, sinks)
+    assert got.isfinite().all()
+    for b in sorted({0, min(1, batch - 1), batch // 2, batch - 1}):
+        at = table[b].long()
+        k, v = ((c.view(torch.uint8)[at].view(E4M3).float() * s[at][..., None, None]).permute(1, 0, 2, 3).flatten(1, 2)[None] for c, s in zip(codes, scales))
+        held(got[b : b + 1], reference(q[b : b + 1], k.double(), v.double(), [lengths[b]], window, sinks, width**-0.5))
+    assert status() == 0
+
+
 @pytest.mark.parametrize("spread", [2.0**-60, 2.0**-20, 2.0**20, 2.0**60])
 def test_queries_of_any_size(tq, spread):
     """bf16 queries far outside the range of f16, with scores that stay moderate."""
@@ -482,13 +505,14 @@ def test_a_conversation_a_fork_and_its_two_ends(tq):
     assert status() == 0
 
 
-def test_a_step_replayed_from_a_graph(tq):
-    """Lengths, starts and tables are read on the device: a captured step goes on as they change. Two graphs share nothing."""
+@pytest.mark.parametrize("blocks, long", [(40, 600), (300, 4500)], ids=["whole units", "shares"])
+def test_a_step_replayed_from_a_graph(tq, blocks, long):
+    """Lengths, starts and tables are read on the device: a captured step goes on as they change. Two graphs share nothing, on two streams at once."""
     heads, kv_heads, width, page = 4, 2, 64, 16
     streams = [torch.cuda.Stream() for _ in range(2)]
-    caches = [Cache(2, kv_heads, width, page, 40, seed=i).fill([600, 5]) for i in range(2)]
+    caches = [Cache(2, kv_heads, width, page, blocks, seed=i).fill([long, 5]) for i in range(2)]
     k, q = by_token((2, kv_heads, 1, width), torch.bfloat16, 1), by_token((2, heads, 1, width), torch.bfloat16, 2)
-    starts = [torch.tensor([600, 5], dtype=torch.int32).cuda() for _ in range(2)]
+    starts = [torch.tensor([long, 5], dtype=torch.int32).cuda() for _ in range(2)]
     lengths = [s + 1 for s in starts]
     graphs, results = [], []
     for cache, start, length in zip(caches, starts, lengths):
@@ -503,8 +527,8 @@ def test_a_step_replayed_from_a_graph(tq):
             length.add_(1)
         graphs.append(graph)
     for start, length in zip(starts, lengths):
-        start.copy_(torch.tensor([600, 5]))
-        length.copy_(torch.tensor([601, 6]))
+        start.copy_(torch.tensor([long, 5]))
+        length.copy_(torch.tensor([long + 1, 6]))
     torch.cuda.synchronize()
     for step in range(20):
         for graph, stream in zip(graphs, streams):
@@ -512,8 +536,62 @@ def test_a_step_replayed_from_a_graph(tq):
                 graph.replay()
     torch.cuda.synchronize()
     for cache, got in zip(caches, results):
-        held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [620, 25], None, 0, 0.125))
+        held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [long + 20, 25], None, 0, 0.125))
     assert status() == 0
+
+
+def test_repeated_calls_give_the_same_bits_on_any_stream_and_from_threads(tq):
+    import threading
+
+    cache = Cache(3, 2, 64, 16, 200).fill([3100, 40, 1])
+    q, lengths = by_token((3, 8, 2, 64), torch.bfloat16, 1), torch.tensor([3100, 40, 1], dtype=torch.int32).cuda()
+    first = tq.cache_attention(q, *cache.tensors, cache.table, lengths, 2500, 4)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def many():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                again = tq.cache_attention(q, *cache.tensors, cache.table, lengths, 2500, 4)
+                if not torch.equal(again, first):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=many) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and status() == 0
+
+
+def test_a_pool_beyond_four_gigabytes(tq):
+    kv_heads, width, page, pages = 8, 128, 64, 72000      # 4.7 GB of codes each
+    shape = (pages, kv_heads, page, width)
+    codes = [torch.empty(shape, dtype=E4M3, device="cuda") for _ in range(2)]
+    scales = [torch.empty(shape[:2], device="cuda") for _ in range(2)]
+    table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32).cuda()
+    k, v = (by_token((1, kv_heads, 150, width), torch.bfloat16, s) for s in (1, 2))
+    tq.cache_store(k, v, *codes, *scales, table, torch.zeros(1, dtype=torch.int32).cuda())
+    tq.copy_pages([*codes, *scales], [pages - 1], [40000])
+    for t in (*codes, *scales):
+        raw = t.view(torch.uint8) if t.dtype == E4M3 else t
+        assert torch.equal(raw[40000], raw[pages - 1])
+    table[0, 0] = 40000
+    q = by_token((1, 16, 1, width), torch.bfloat16, 3)
+    got = tq.cache_attention(q, *codes, *scales, table, torch.tensor([150], dtype=torch.int32).cuda())
+    at = table[0].long()
+    values = [(c.view(torch.uint8)[at].view(E4M3).float() * s[at][..., None, None]).permute(1, 0, 2, 3).flatten(1, 2)[None] for c, s in zip(codes, scales)]
+    held(got, reference(q, values[0].double(), values[1].double(), [150], None, 0, width**-0.5))
+    assert status() == 0
+
+
+def test_on_another_device_than_the_current_one(tq):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    q, k = drawn((2, 4, 3, 64), torch.float16, 1).to("cuda:1"), drawn((2, 2, 2000, 64), torch.float16, 2).to("cuda:1")
+    got = tq.window_attention(q, k, k, 1500, 4)
+    assert got.device.index == 1 and torch.cuda.current_device() == 0
+    held(got, reference(q, k, k, [2000, 2000], 1500, 4, 0.125))
 
 
 def test_a_paged_cache_through_forks_drafts_and_moves(tq):
