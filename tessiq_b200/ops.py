@@ -757,6 +757,17 @@ def copy_pages(tensors, sources, targets, page_axis=0) -> None:
 _library = None
 
 
+def _window_attention_by_aten(q, k, v, window, sinks, scale):
+    """`window_attention` in ATen, for what the kernels decline (f32, heads over 128 elements)."""
+    group, difference = q.shape[1] // max(k.shape[1], 1), k.shape[2] - q.shape[2]
+    k, v = (t.repeat_interleave(group, 1) for t in (k, v))
+    scores = (q @ k.transpose(-1, -2)) * (q.shape[-1] ** -0.5 if scale is None else scale)
+    at, key = torch.arange(q.shape[2], device=q.device)[:, None] + difference, torch.arange(k.shape[2], device=q.device)
+    sees = (key <= at) & ((key > at - (k.shape[2] + 1 if window is None else window)) | (key < sinks))
+    weights = torch.softmax(scores.float().masked_fill(~sees, -math.inf), -1).masked_fill(~sees, 0.0)
+    return (weights.to(q.dtype) @ v).contiguous()
+
+
 def register_custom_ops() -> None:
     """Defines the `tessiq` operator namespace with the reference's schemas and registers the
     kernels above for the CUDA dispatch key. Calling an operation with CPU tensors fails in
@@ -796,6 +807,13 @@ def register_custom_ops() -> None:
                                                                  lambda gate, up: functional.silu(gate) * up),
         "attention(Tensor q, Tensor k, Tensor v, float scale, bool causal) -> Tensor": or_reference(
             attention, lambda q, k, v, scale, causal: functional.scaled_dot_product_attention(q, k, v, is_causal=causal, scale=scale)),
+        "window_attention(Tensor q, Tensor k, Tensor v, int? window, int sinks, float? scale) -> Tensor": or_reference(window_attention, _window_attention_by_aten),
+        # (over the cache, and into it, there is no ATen definition to fall back to: a decline is raised)
+        "cache_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor table, Tensor lengths, int? window, int sinks, "
+        "float? scale) -> Tensor": cache_attention,
+        "cache_store(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor table, Tensor starts, "
+        "Tensor? counts) -> ()": cache_store,
+        "copy_pages(Tensor(a!)[] tensors, int[] sources, int[] targets, int page_axis) -> ()": copy_pages,
     }
     for schema, implementation in schemas.items():
         library.define(schema)

@@ -72,3 +72,26 @@ def test_a_declined_call_runs_the_aten_definition_on_the_gpu(tessiq):
 def test_host_tensors_have_no_implementation(tessiq):
     with pytest.raises((NotImplementedError, RuntimeError)):
         tessiq.fast_gelu(torch.randn(8))
+
+
+def test_window_attention_and_the_cache_are_operations_too(tessiq):
+    from tessiq_b200 import ops
+
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(2, n, t, 64, generator=g).bfloat16().cuda() for n, t in ((4, 5), (2, 40), (2, 40)))
+    assert torch.equal(tessiq.window_attention(q, k, v, 16, 2, None), ops.window_attention(q, k, v, 16, 2))
+    # f32 has no kernel: the ATen definition, queries before the first key included
+    wide = tessiq.window_attention(q.float(), k.float()[:, :, :3], v.float()[:, :, :3], None, 0, 0.1)
+    assert wide.dtype == torch.float32 and wide[:, :, :2].count_nonzero().item() == 0
+    narrow = ops.window_attention(q, k[:, :, :3].contiguous(), v[:, :, :3].contiguous(), scale=0.1)
+    # (bf16 against f32: half a step of the result, 2^-8, and at most as much of the weights)
+    torch.testing.assert_close(narrow.float(), wide, rtol=2.0**-7, atol=2.0**-7 * v.float().abs().max().item())
+    pages = [torch.zeros(6, 2, 16, 64, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.zeros(6, 2, device="cuda") for _ in range(2)]
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32).cuda()
+    starts, lengths = torch.zeros(2, dtype=torch.int32).cuda(), torch.tensor([40, 30], dtype=torch.int32).cuda()
+    tessiq.cache_store(k, v, *pages, *scales, table, starts, lengths)
+    got = tessiq.cache_attention(q, *pages, *scales, table, lengths, 16, 2, None)
+    assert torch.equal(got, ops.cache_attention(q, *pages, *scales, table, lengths, 16, 2)) and got.isfinite().all()
+    tessiq.copy_pages([*(p.view(torch.uint8) for p in pages), *scales], [0], [5], 0)
+    assert torch.equal(scales[0][5], scales[0][0]) and torch.equal(pages[1].view(torch.uint8)[5], pages[1].view(torch.uint8)[0])
