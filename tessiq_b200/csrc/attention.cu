@@ -524,11 +524,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 // ---- With a window, sinks and shared key heads ------------------------------------------------------
 //
 // The same products, softmax and hand-overs as above, for rows that see the keys j <= p with j > p - window or j < sinks (p = row + k_tokens -
-// q_tokens): a block of rows walks the tiles of the sinks and then those from its first row's window to its last row. Under a short
-// window such a walk is a few steps, and a CTA's start (barriers, tensor memory, first loads: about 8 us of latency beside 0.9 a step) would be most of
-// it; so CTAs stay, as many as fit, and take blocks one after another. Counted through all blocks, step g of a CTA has ring stage g % kRing and the phases
-// that g gives, and the first loads and scores of the next block run under the last step and the result of the one before: its query tile is loaded
-// once the last scores of that block are out (q_empty), and its first product writes the result columns only after p_full, which the
+// q_tokens): a block of rows walks the tiles of the sinks and then those from its first row's window to its last row. Under a short window such a
+// walk is a few steps, and a CTA's start (barriers, tensor memory, first loads: about 8 us of latency beside 0.9 a step) would be most of it; so
+// CTAs stay, as many as fit, and take blocks one after another. Counted through all blocks, step g of a CTA has ring stage g % kRing and the
+// phases that g gives, and the first loads and scores of the next block run under the last step and the result of the one before: its query tile
+// is loaded once the last scores of that block are out (q_empty), and its first product writes the result columns only after p_full, which the
 // softmax warps signal when they have read the result before it.
 //
 // Blocks are dealt out by length, the longest of all heads first, so that CTAs get sums of about the same length.
@@ -567,7 +567,8 @@ __device__ __forceinline__ WindowBlock window_block(const WindowAttnParams& p, i
   return b;
 }
 
-// One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a lane for the result.
+// One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a
+// lane for the result.
 template <typename T, int D>
 __device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int batch, int head, int key_head, int row) {
   const int lane = threadIdx.x & 31, position = row + p.offset;
@@ -822,8 +823,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) barrier_arrive(s_free);
-        // Masks, where the tile has a key that some row does not see (uniform in the CTA): what the row sees as bits, 32 keys a word, which the compiler turns into
-        // predicates eight at a time; two comparisons and selections for each key were half of all instructions under a window of 64.
+        // Masks, where the tile has a key that some row does not see (uniform in the CTA): what the row sees as bits, 32 keys a word, which the
+        // compiler turns into predicates eight at a time; two comparisons and selections for each key were half of all instructions under a
+        // window of 64.
         const int key0 = (j < b.sink_tiles ? j : j + b.gap) * kKeys;
         if (key0 + kKeys - 1 > low || (key0 <= low + kRows - 1 - p.window && key0 + kKeys > p.sinks)) {
 #pragma unroll
@@ -1035,12 +1037,13 @@ AttentionForm choose_attention_form(long long heads, long long q_tokens, long lo
   return {false, ctas <= 2 * sms || (k_tokens >= 512 && !thirds && !half_step) ? 128 : 64, false};
 }
 
-// Keys a step of the tensor-core tiles for window attention, or 0: the keys are streamed (keyed.cu), which shares a head's keys among all SMs but takes 16 rows of a key head at
-// a time where a tile has 128 and walks its keys in one CTA. The smaller of two expected times (us; B200, bf16; measured: tiles / streamed). 12 heads of 64, 8000 keys, 8 queries 80 / 14.5,
-// 128 queries 80 / 36, 300 queries 82 / 70; 8 x 12 heads 40 queries 84 / 88, 100 queries 85 / 190; 8 key heads of 128 for 32, 100 queries, 300 keys 10.3 / 12.4, 2000 keys 24.7 / 41, 8000 keys
-// 83 / 107, 5 queries 82 / 29.
-// Tiles: 128 keys a step where few CTAs leave the steps' latency bare (up to two an SM, one of heads above 64), and for heads up to 64 where there are many steps: 8 x 12 x 4096 tokens under a
-// window of 64 110.9 with 128 and 86.6 with 64, of 1024 196.4 and 195.9, of 4096 334 and 356; 2 x 32 x 2501 of 128 under 333 104 and 76.
+// Keys a step of the tensor-core tiles for window attention, or 0: the keys are streamed (keyed.cu), which shares a head's keys among all SMs but
+// takes 16 rows of a key head at a time where a tile has 128 and walks its keys in one CTA. The smaller of two expected times (us; B200, bf16;
+// measured: tiles / streamed). 12 heads of 64, 8000 keys, 8 queries 80 / 14.5, 128 queries 80 / 36, 300 queries 82 / 70; 8 x 12 heads 40 queries
+// 84 / 88, 100 queries 85 / 190; 8 key heads of 128 for 32, 100 queries, 300 keys 10.3 / 12.4, 2000 keys 24.7 / 41, 8000 keys 83 / 107, 5 queries
+// 82 / 29. Tiles: 128 keys a step where few CTAs leave the steps' latency bare (up to two an SM, one of heads above 64), and for heads up to 64
+// where there are many steps: 8 x 12 x 4096 tokens under a window of 64 110.9 with 128 and 86.6 with 64, of 1024 196.4 and 195.9, of 4096 334 and
+// 356; 2 x 32 x 2501 of 128 under 333 104 and 76.
 int window_tile_keys(const KeyedParams& p, long long sms) {
   const bool wide = p.head_dim > kHeadDim;
   const long long rows = static_cast<long long>(p.group) * p.q_tokens;

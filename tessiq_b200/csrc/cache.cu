@@ -3,15 +3,15 @@
 // Writing. A team of threads takes what one page and head gets of a sequence's new tokens:
 //   s = the smallest power of two >= max |x| / 448, at least 2^-126 and at least what the page's earlier tokens need
 //   code = e4m3(x / s), to nearest even
-// e4m3 is a floating format, so a power of two costs it no precision, x / s is exact, and an earlier code brought to
-// a larger scale only steps down in exponent: exact again, except for what falls under its smallest normal. The tokens are read once, kept in
-// registers between the maximum and the encoding. Bound: HBM (2 bytes read and 1 written an element: 402 MB in 66 us, 6.1 TB/s); for one new
-// token a sequence, the latency of start, table entry, scale and token, one after another (5 us with the launch). Divisions by the vectors
-// of a token in the addresses had it at 94 us and bound by instructions; the next head's tokens loaded ahead took the registers of half the CTAs and gained nothing.
+// e4m3 is a floating format, so a power of two costs it no precision, x / s is exact, and an earlier code brought to a larger scale only steps
+// down in exponent: exact again, except for what falls under its smallest normal. The tokens are read once, kept in registers between the maximum
+// and the encoding. Bound: HBM (2 bytes read and 1 written an element: 402 MB in 66 us, 6.1 TB/s); for one new token a sequence, the latency of
+// start, table entry, scale and token, one after another (5 us with the launch). Divisions by the vectors of a token in the addresses had it at
+// 94 us and bound by instructions; the next head's tokens loaded ahead took the registers of half the CTAs and gained nothing.
 //
-// Copying. Source and target pages are given by the host, which is where a cache's pages are handed out; they travel to the kernel as
-// its argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 87 us, 6.3 TB/s). Small pages of several layers are
-// one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
+// Copying. Source and target pages are given by the host, which is where a cache's pages are handed out; they travel to the kernel as its
+// argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 87 us, 6.3 TB/s). Small pages of several
+// layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -470,9 +470,9 @@ extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const 
   p.tokens = static_cast<int>(tokens);
   p.head_dim = static_cast<int>(head_dim);
   p.touched = static_cast<int>((tokens + page_tokens - 2) / page_tokens + 1);
-  // A warp where it keeps a page's new tokens in registers, else a CTA; and each several heads where there would be more than four times as many teams as run at
-  // once (128 warps, 32 CTAs an SM). us, with as many as run at once, four times as many and one for every head: 32 x 8 heads of 2047 tokens of 128, pages of 64 68.4, 65.8,
-  // 65.7, pages of 16 77.7, 71.5, 71.6; 32 x 12 of 64, pages of 16 82.4, 74.8, 85.9.
+  // A warp where it keeps a page's new tokens in registers, else a CTA; and each several heads where there would be more than four times as many
+  // teams as run at once (128 warps, 32 CTAs an SM). us, with as many as run at once, four times as many and one for every head: 32 x 8 heads of
+  // 2047 tokens of 128, pages of 64 68.4, 65.8, 65.7, pages of 16 77.7, 71.5, 71.6; 32 x 12 of 64, pages of 16 82.4, 74.8, 85.9.
   const bool warps = (tokens < page_tokens ? tokens : page_tokens) * head_dim <= 8 * 32 * 8;
   const long long pairs = static_cast<long long>(p.batch) * p.touched, teams_at_once = static_cast<long long>(tq::sm_count(device)) * (warps ? 128 : 32);
   const long long runs = teams_at_once / pairs < 1 ? 1 : teams_at_once / pairs < 2 * kv_heads ? teams_at_once / pairs : 2 * kv_heads;

@@ -6,20 +6,35 @@
 //   8 bits: k_j = code_j * k_scale[page, head], v_j likewise (e4m3 codes, an f32 scale a page and head)
 //
 // Heads that share a key head are rows of one tile, so a key is read once for all of them. Bound: HBM (the visible keys' and
-// values' bytes); the multiply-adds of up to 16 rows would not fit the CUDA cores beside it, so both products are warp-level
-// matrix instructions over keys and values that go from memory to registers in the instructions' own layout, without
-// shared memory: the order of the summed-over axis of a product is free, so a lane's 16 contiguous bytes of a key are
-// whatever elements of the head the instruction takes from it, and the query is laid out to match. Transposed, S^T = K Q^T
-// and O^T = V^T P^T: keys (then head elements) are the instruction's 16 rows and query rows its 8 columns, so that a
-// head of its own wastes 7 columns of 8 and not 15 rows of 16.
+// values' bytes). The multiply-adds of up to 16 rows would not fit the CUDA cores beside it, so both products are warp-level
+// matrix instructions, transposed: S^T = K Q^T and O^T = V^T P^T, keys (then head elements) the instruction's 16 rows and query rows its 8
+// columns, so that a head of its own wastes 7 columns of 8 and not 15 rows of 16. The order of the summed-over axis of
+// a product is free, so a lane's 16 contiguous bytes of a key are whatever elements of the head the instruction takes
+// from it, and the query is laid out to match; a value's bytes are paired with the next key's by one byte permute.
+//
+// Memory: a warp has a ring of two stages of 8 KB (16 to 64 keys and their values) that TMA fills from a page or through the dense
+// strides; no warp waits for another. Keys straight into registers left too little under way (616 us for 16 x 8 key heads of 128 of 20001 to
+// 40000 keys with a CTA a head, 232 with the split below; rings 178).
+//
+// Split: the chunks of all (sequence, key head, 8 or 16 rows), each unit counted a little longer than it is, are one range in equal shares, a
+// warp each; whole units are written at once, and what a border between shares cuts is left in scratch as (maximum, sum, unscaled result) and
+// joined by a second kernel whose start passes under the first one's end. With a CTA for each share, units of a chunk or two (short sequences of
+// a ragged batch) queued up behind one another's latency: 64 x 12 heads of 64 of 1 to 2000 keys 94 us, with a warp 24. Few units have a CTA's
+// warps join theirs before (one head of 128000 keys 121 -> 23 us), and units of few chunks a CTA each (plan_shape). Tried beside the second
+// kernel: the last CTA to arrive at a ticket joins (48 us for 33 + 6: fences, and code that nobody has run yet, at the very end).
+//
+// Measured (kernels and join; us, and of HBM's 6456 GB/s): 16 x 64/8 heads of 128, 20001 to 40000 keys in 8 bits 160 (0.95); 32 x 32/8 heads,
+// 2052 keys in 16 bits 52 (0.80); 64 x 12 heads of 64, 1 to 2000 keys 28 (0.54); four queries of 48 x 32/8, 1028 keys 39 (0.39). A fixed 13 us
+// (launch, lengths, first pages and keys, join) is what the short ones pay, and 16 rows twice the products; the special functions, tensor pipe
+// and issue slots are below 50 %.
 //
 // Precision: scores, maxima, sums and results in f32. e4m3 to f16 is exact, and so is the query in f16: a row is scaled by a power of two to
 // a maximum of 2^14, so only elements 2^-38 of it or less lose digits. Probabilities against f16 values (cache codes too) are rounded to
-// f16 (half a step is 2^-12, under the result's 2^-9 in bf16); against bf16 values they take two bf16 operands, the
-// rounded value and what rounding took off (2^-17).
+// f16 (half a step is 2^-11, under the result's 2^-8 in bf16); against bf16 values they take two bf16 operands, the
+// rounded value and what rounding took off (2^-16).
 //
-// A masked key must not reach a result through 0 * NaN: its score is replaced, and where the rows of a tile see a chunk's keys
-// alike its value is replaced by zeros. Where they do not (several queries, at an end of the window) the chunk's product is
+// A masked key must not reach a result through 0 * NaN: its score is replaced, and a value that no row of the tile sees becomes zeros in the
+// stage. Where rows see different keys (several queries, at an end of the window) and a value they do see is no number, the chunk's product is
 // taken once a query with that query's keys alone, and each row keeps its own.
 #include <cuda.h>
 
@@ -37,8 +52,8 @@ namespace {
 constexpr int kKeyedWarps = 4;
 constexpr int kKeyedThreads = 32 * kKeyedWarps;
 
-// Chunks of a warp in flight or in use. Measured, 16 x 8 key heads of 128 of 20001 to 40000 keys: two stages and two CTAs an SM 165 us, three stages 164, two stages and three CTAs 181 (registers spill); four
-// queries under a window 45.2, 49.2, 44.8.
+// Chunks of a warp in flight or in use. Measured, 16 x 8 key heads of 128 of 20001 to 40000 keys: two stages and two CTAs an SM 165 us, three
+// stages 164, two stages and three CTAs 181 (registers spill); four queries under a window 45.2, 49.2, 44.8.
 constexpr int kKeyedStages = 2;
 constexpr uint32_t kStageBytes = 8192;
 constexpr uint32_t kWarpRing = kKeyedStages * kStageBytes;
@@ -208,8 +223,9 @@ __device__ __forceinline__ int counted(const KeyedParams& p, int sequence) {
   return max(sequence_chunks<BITS, CHUNK>(p, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
 }
 
-// What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another, and its masked ends. Measured with 2, 4 and 6 of them, us: heads of
-// 128, 48 x 8 of four queries under a window 41.2, 39.3, 40.4, 30 x 4 of 96 55.7, 51.4, 52.8; heads of 64 (chunks of twice the keys) 100 x 12 34.3, 36.9, 39.0.
+// What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another, and its masked ends. Measured with
+// 2, 4 and 6 of them, us: heads of 128, 48 x 8 of four queries under a window 41.2, 39.3, 40.4, 30 x 4 of 96 55.7, 51.4, 52.8; heads of 64
+// (chunks of twice the keys) 100 x 12 34.3, 36.9, 39.0.
 constexpr int unit_cost(int chunk) { return chunk > 32 ? 2 : 4; }
 constexpr int kLeastShare = 4;       // of the same
 
@@ -274,8 +290,9 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   return dealt;
 }
 
-// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal shares, one a warp (then
-// keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared memory. ONE: a chunk lies in one page (or in none: dense keys).
+// T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal
+// shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared
+// memory. ONE: a chunk lies in one page (or in none: dense keys).
 template <typename T, int BITS, int W, int NT, int JOINS, bool ONE>
 __global__ void __launch_bounds__(kKeyedThreads, 2)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
@@ -337,628 +354,630 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
   }
   while (at < until) {
-  // ---- one unit, or what of it is in the share: chunks [first_chunk, last_chunk) ----
-  int batch, kv_head, tile, first_chunk = 0, last_chunk;
-  bool whole = true, begins = true;
-  int counted_length;
-  ChunkList list;
-  if constexpr (SHARED) {
-    batch = place.sequence;
-    counted_length = length_of<BITS, S::kKeys>(p, batch);
-    list = sequence_chunks<BITS, S::kKeys>(p, counted_length);
-    const int cost = kUnitCost + max(list.count(), 1), units = p.kv_heads * p.row_tiles;
-    const int inside = at - place.before;
-    const int unit = inside / cost;
-    tile = unit % p.row_tiles;
-    kv_head = unit / p.row_tiles;
-    const int from = inside - unit * cost, to = min(cost, from + (until - at));
-    first_chunk = max(from - kUnitCost, 0);
-    last_chunk = max(to - kUnitCost, 0);
-    begins = first_chunk == 0;
-    whole = begins && to == cost;
-    const int unit_start = at - from;
-    at += to - from;
-    if (last_chunk > 0 && !whole && lane == 0) {         // which shares have parts of the unit
-      const int first = dealt.holder(unit_start + kUnitCost), last = dealt.holder(unit_start + cost - 1);
-      if constexpr (JOINS > 1) pieces[warp][begins ? 1 : 0] = {batch, unit, first, last, true, begins, to == cost};
-      else if (to < cost) p.borders[share] = make_int4(batch, unit, first, last);      // the border behind this share cuts it
-    }
-    if (at - place.before >= units * cost) place = {batch + 1, place.before + units * cost};
-    if (last_chunk == 0) continue;                     // a border just before its first chunk: it is the next share's
-    last_chunk = min(last_chunk, list.count());
-  } else {
-    const long long unit = blockIdx.x;
-    tile = static_cast<int>(unit % p.row_tiles);
-    const long long head_index = unit / p.row_tiles;
-    kv_head = static_cast<int>(head_index % p.kv_heads);
-    batch = static_cast<int>(head_index / p.kv_heads);
-    counted_length = length_of<BITS, S::kKeys>(p, batch);
-    at = until;
-  }
-  const int length = counted_length;
-  const int row0 = tile * kRows;
-  if constexpr (BITS == 8) {
-    if ((SHARED ? lane : threadIdx.x) == 0 && p.lengths[batch] > length) report(p.status, kKeyedLength, batch, p.lengths[batch]);      // the table does not go that far
-  }
-  const int first_token = row0 / p.group, last_token = (min(row0 + kRows, rows) - 1) / p.group;
-  const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
-  if constexpr (!SHARED) {
-    list = chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys);
-    last_chunk = list.count();
-  }
-
-  // ---- the warp's chunks ----
-  if constexpr (!SHARED) first_chunk = warp;
-  const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
-  auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
-  // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks.
-  const int boxes = ONE ? 1 : p.boxes, box_shift = ONE ? 31 : p.box_shift;
-  const int ahead = ONE ? 32 : 32 / boxes;
-  auto look_up = [&](int n) {
-    if constexpr (BITS == 8) {
-      n += ONE ? lane : lane / boxes;
-      if (n >= mine) return -1;
-      const int key = chunk_at(n) * S::kKeys + (ONE ? 0 : (lane % boxes) << box_shift);
-      if (key >= length) return -1;
-      const int at_block = key >> p.page_shift;
-      const int page = p.table[batch * p.table_stride + at_block];
-      if (page >= 0 && page < p.pages) return page;
-      report(p.status, kKeyedPage, batch, at_block);
-    }
-    return -1;
-  };
-  int page_now = look_up(0), page_next = look_up(ahead);
-  // The query: row `quad` of each eight, the elements that the lane's pieces of a key hold.
-  constexpr int kWords = S::kPieceWidth / 2;                     // of a piece's query elements: 8 or 4
-  uint32_t word[NT][S::kPieces][kWords];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = row0 + n * 8 + quad;
-    const int token = row / p.group, head = kv_head * p.group + row % p.group;
-    const T* from = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
-#pragma unroll
-    for (int j = 0; j < S::kPieces; ++j) {
-      const int column = (4 * j + corner) * S::kPieceWidth;
-#pragma unroll
-      for (int w = 0; w < kWords; w += 4) {
-        uint4 four = make_uint4(0, 0, 0, 0);
-        if (row < rows && column + 2 * w < p.head_dim) four = *reinterpret_cast<const uint4*>(from + column + 2 * w);
-        word[n][j][w] = four.x;
-        word[n][j][w + 1] = four.y;
-        word[n][j][w + 2] = four.z;
-        word[n][j][w + 3] = four.w;
+    // ---- one unit, or what of it is in the share: chunks [first_chunk, last_chunk) ----
+    int batch, kv_head, tile, first_chunk = 0, last_chunk;
+    bool whole = true, begins = true;
+    int counted_length;
+    ChunkList list;
+    if constexpr (SHARED) {
+      batch = place.sequence;
+      counted_length = length_of<BITS, S::kKeys>(p, batch);
+      list = sequence_chunks<BITS, S::kKeys>(p, counted_length);
+      const int cost = kUnitCost + max(list.count(), 1), units = p.kv_heads * p.row_tiles;
+      const int inside = at - place.before;
+      const int unit = inside / cost;
+      tile = unit % p.row_tiles;
+      kv_head = unit / p.row_tiles;
+      const int from = inside - unit * cost, to = min(cost, from + (until - at));
+      first_chunk = max(from - kUnitCost, 0);
+      last_chunk = max(to - kUnitCost, 0);
+      begins = first_chunk == 0;
+      whole = begins && to == cost;
+      const int unit_start = at - from;
+      at += to - from;
+      if (last_chunk > 0 && !whole && lane == 0) {         // which shares have parts of the unit
+        const int first = dealt.holder(unit_start + kUnitCost), last = dealt.holder(unit_start + cost - 1);
+        if constexpr (JOINS > 1) pieces[warp][begins ? 1 : 0] = {batch, unit, first, last, true, begins, to == cost};
+        else if (to < cost) p.borders[share] = make_int4(batch, unit, first, last);      // the border behind this share cuts it
       }
-    }
-  }
-  auto fill = [&](int n, int stage) {                  // chunk n of the warp into a stage that nobody reads any more
-    const int key0 = chunk_at(n) * S::kKeys;
-    const uint32_t to = ring + stage * kStageBytes, bar = barrier0 + 8 * stage;
-    if constexpr (BITS == 8) {
-      if (n > 0 && n % ahead == 0) {
-        page_now = page_next;
-        page_next = look_up(n + ahead);
-      }
-      const int inside = key0 & ((1 << p.page_shift) - 1);
-      if constexpr (ONE) {
-        const int page = __shfl_sync(0xffffffffu, page_now, n & 31);
-        if (lane == 0) {
-          staged_page[warp][stage][0] = page;
-          barrier_expect_tx(bar, page >= 0 ? kStageBytes : 0);
-          if (page >= 0) {
-            const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + inside;      // (below 2^31: keyed_maps)
-            tma_load_rows(to, &map_k, bar, 0, row);
-            tma_load_rows(to + kStageBytes / 2, &map_v, bar, 0, row);
-          }
-        }
-      } else {
-        const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
-        const bool loads = lane < boxes && page >= 0;
-        const uint32_t box_bytes = static_cast<uint32_t>(S::kLine) << box_shift;
-        const uint32_t bytes = 2u * box_bytes * __popc(__ballot_sync(0xffffffffu, loads));
-        if (lane < boxes) staged_page[warp][stage][lane] = page;
-        if (lane == 0) barrier_expect_tx(bar, bytes);
-        __syncwarp();
-        if (loads) {
-          const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + ((key0 + (lane << box_shift)) & ((1 << p.page_shift) - 1));
-          tma_load_rows(to + lane * box_bytes, &map_k, bar, 0, row);
-          tma_load_rows(to + kStageBytes / 2 + lane * box_bytes, &map_v, bar, 0, row);
-        }
-      }
+      if (at - place.before >= units * cost) place = {batch + 1, place.before + units * cost};
+      if (last_chunk == 0) continue;                     // a border just before its first chunk: it is the next share's
+      last_chunk = min(last_chunk, list.count());
     } else {
-      if (lane == 0) {
-        barrier_expect_tx(bar, kStageBytes);
-#pragma unroll
-        for (int l = 0; l < S::kLines; ++l) {
-          tma_load_tokens(to + l * S::kBoxBytes, &map_k, bar, l * 64, key0, kv_head, batch);
-          tma_load_tokens(to + kStageBytes / 2 + l * S::kBoxBytes, &map_v, bar, l * 64, key0, kv_head, batch);
-        }
-      }
+      const long long unit = blockIdx.x;
+      tile = static_cast<int>(unit % p.row_tiles);
+      const long long head_index = unit / p.row_tiles;
+      kv_head = static_cast<int>(head_index % p.kv_heads);
+      batch = static_cast<int>(head_index / p.kv_heads);
+      counted_length = length_of<BITS, S::kKeys>(p, batch);
+      at = until;
     }
-  };
-  // The scales of the next chunk's pages (of its tile t in lane t, unless they are one page's) are asked for a step before they are used; 0: no page.
-  float k_scale_next = 0.f, v_scale_next = 0.f;
-  auto ask_scales = [&](int stage) {
+    const int length = counted_length;
+    const int row0 = tile * kRows;
     if constexpr (BITS == 8) {
-      if (ONE || lane < kTiles) {
-        const int page = staged_page[warp][stage][ONE ? 0 : (lane * 16) >> box_shift];
-        k_scale_next = v_scale_next = 0.f;
-        if (page >= 0) {
-          const int block = page * p.kv_heads + kv_head;
-          k_scale_next = p.k_scales[block];
-          v_scale_next = p.v_scales[block];
-        }
-      }
+      if ((SHARED ? lane : threadIdx.x) == 0 && p.lengths[batch] > length) report(p.status, kKeyedLength, batch, p.lengths[batch]);      // the table does not go that far
     }
-  };
-  for (int first = 0; first < min(mine, kKeyedStages); ++first) fill(first, (turn + first) % kKeyedStages);
-  __syncwarp();
-  if (mine > 0) ask_scales(turn % kKeyedStages);
-
-  // ... as the matrix instructions take it: [piece][step of 16 elements][operand word]
-  uint32_t query[NT][S::kPieces][32 / BITS][2];
-  float row_scale[NT][2];                                        // of the lane's two columns: rows 2 corner and 2 corner + 1
-  int position[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float back = p.scale_log2;
-    if constexpr (BITS == 8) {
-      float largest = 0.f;
-#pragma unroll
-      for (int j = 0; j < S::kPieces; ++j) {
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-          const float2 pair = widen_pair<T>(word[n][j][w]);
-          largest = fmaxf(largest, fmaxf(fabsf(pair.x), fabsf(pair.y)));
-        }
-      }
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      // a power of two that brings the row's largest element to [2^14, 2^15); none for zeros and infinities
-      int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
-      if (exponent < -100 || exponent > 127) exponent = 14;
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
-      back *= __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
-#pragma unroll
-      for (int j = 0; j < S::kPieces; ++j) {
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-          const float2 pair = widen_pair<T>(word[n][j][w]);
-          word[n][j][w] = round_pair<__half>(pair.x * up, pair.y * up);
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < S::kPieces; ++j) {
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) query[n][j][w / 2][w % 2] = word[n][j][w];
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * corner + e) * 4);
-      const int here = row0 + n * 8 + 2 * corner + e;
-      position[n][e] = here < rows ? length - p.q_tokens + here / p.group : high;
-    }
-  }
-
-  float top[NT][2], sum[NT][2], result[NT][kSlices][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      top[n][e] = -INFINITY;
-      sum[n][e] = 0.f;
-    }
-#pragma unroll
-    for (int s = 0; s < kSlices; ++s) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) result[n][s][e] = 0.f;
-    }
-  }
-
-  for (int step = 0; step < mine; ++step, ++turn) {
-    const int key0 = chunk_at(step) * S::kKeys;
-    const int stage = turn % kKeyedStages;
-    if (!barrier_wait(barrier0 + 8 * stage, (turn / kKeyedStages) & 1, p.status, kWaitKeyed)) {
-      // the result is lost (the status says so); the copies that are under way still have to land before the stages are used otherwise
-      for (int m = step; m < min(step + kKeyedStages, mine); ++m, ++turn) {
-        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(barrier0 + 8 * (turn % kKeyedStages), (turn / kKeyedStages) & 1); ++spin) {
-        }
-      }
-      break;
-    }
-    const uint32_t k_at = ring + stage * kStageBytes, v_at = k_at + kStageBytes / 2;
-    int stop = length;                                 // keys from here on are not there
-    constexpr int kScales = BITS == 8 && !ONE ? kTiles : 1;
-    float k_scale[kScales], v_scale[kScales], v_scale_now = 0.f;
-    k_scale[0] = k_scale_next;
-    v_scale[0] = v_scale_next;
-    if constexpr (BITS == 8) {
-      if constexpr (ONE) {
-        if (staged_page[warp][stage][0] < 0) stop = key0;
-      } else {
-#pragma unroll
-        for (int t = kTiles - 1; t >= 0; --t) {
-          k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
-          v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
-          if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
-        }
-      }
-      v_scale_now = v_scale_next;
-      if (step + 1 < mine) ask_scales((turn + 1) % kKeyedStages);
+    const int first_token = row0 / p.group, last_token = (min(row0 + kRows, rows) - 1) / p.group;
+    const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
+    if constexpr (!SHARED) {
+      list = chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys);
+      last_chunk = list.count();
     }
 
-    // S^T: keys quad and quad + 8 of each tile by rows 2 corner and 2 corner + 1
-    float score[kTiles][NT][4];
-#pragma unroll
-    for (int j = 0; j < S::kPieces; ++j) {
-      uint4 near[kTiles], far[kTiles];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        near[t] = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
-        far[t] = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
+    // ---- the warp's chunks ----
+    if constexpr (!SHARED) first_chunk = warp;
+    const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
+    auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
+    // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks.
+    const int boxes = ONE ? 1 : p.boxes, box_shift = ONE ? 31 : p.box_shift;
+    const int ahead = ONE ? 32 : 32 / boxes;
+    auto look_up = [&](int n) {
+      if constexpr (BITS == 8) {
+        n += ONE ? lane : lane / boxes;
+        if (n >= mine) return -1;
+        const int key = chunk_at(n) * S::kKeys + (ONE ? 0 : (lane % boxes) << box_shift);
+        if (key >= length) return -1;
+        const int at_block = key >> p.page_shift;
+        const int page = p.table[batch * p.table_stride + at_block];
+        if (page >= 0 && page < p.pages) return page;
+        report(p.status, kKeyedPage, batch, at_block);
       }
-#pragma unroll
-      for (int w = 0; w < 32 / BITS; ++w) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const uint32_t x[4] = {near[t].x, near[t].y, near[t].z, near[t].w}, y[4] = {far[t].x, far[t].y, far[t].z, far[t].w};
-          uint32_t a[4];
-          if constexpr (BITS == 8) {
-            a[0] = decode_low(x[w]);
-            a[1] = decode_low(y[w]);
-            a[2] = decode_high(x[w]);
-            a[3] = decode_high(y[w]);
-          } else {
-            a[0] = x[2 * w];
-            a[1] = y[2 * w];
-            a[2] = x[2 * w + 1];
-            a[3] = y[2 * w + 1];
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) multiply<M>(score[t][n], a, query[n][j][w][0], query[n][j][w][1], j == 0 && w == 0);
-        }
-      }
-    }
-
-    // A chunk whose keys every row sees needs no mask.
-    const int last = key0 + S::kKeys - 1;
-    const bool open = last <= low && last < stop && (key0 > high - p.window || last < p.sinks);
-    auto sees = [&](int at, int key) { return key <= at && key < stop && (key > at - p.window || key < p.sinks); };
-    // Any reference point gives the same softmax: a row's moves only when a score lies more than 2^kSlack above it, which one vote tells.
-    float most[NT][2];
-    bool rises = false;
-#pragma unroll
+      return -1;
+    };
+    int page_now = look_up(0), page_next = look_up(ahead);
+    // The query: row `quad` of each eight, the elements that the lane's pieces of a key hold.
+    constexpr int kWords = S::kPieceWidth / 2;                     // of a piece's query elements: 8 or 4
+    uint32_t word[NT][S::kPieces][kWords];
+  #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      most[n][0] = most[n][1] = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        float2 by = make_float2(row_scale[n][0], row_scale[n][1]);
-        if constexpr (BITS == 8) by = __fmul2_rn(by, make_float2(k_scale[t % kScales], k_scale[t % kScales]));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 scaled = __fmul2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), by);
-          score[t][n][2 * h] = scaled.x;
-          score[t][n][2 * h + 1] = scaled.y;
-          if (!open) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (!sees(position[n][e], key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) most[n][e] = fmaxf(most[n][e], fmaxf(score[t][n][e], score[t][n][2 + e]));
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
-    }
-    if (__any_sync(0xffffffffu, rises)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float now = most[n][e];
-          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
-          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
-          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
-          now = fmaxf(now, top[n][e]);
-          const float factor = rescale(top[n][e], now);
-          top[n][e] = now;
-          sum[n][e] *= factor;
-#pragma unroll
-          for (int s = 0; s < kSlices; ++s) {
-            result[n][s][e] *= factor;
-            result[n][s][2 + e] *= factor;
-          }
+      const int row = row0 + n * 8 + quad;
+      const int token = row / p.group, head = kv_head * p.group + row % p.group;
+      const T* from = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
+  #pragma unroll
+      for (int j = 0; j < S::kPieces; ++j) {
+        const int column = (4 * j + corner) * S::kPieceWidth;
+  #pragma unroll
+        for (int w = 0; w < kWords; w += 4) {
+          uint4 four = make_uint4(0, 0, 0, 0);
+          if (row < rows && column + 2 * w < p.head_dim) four = *reinterpret_cast<const uint4*>(from + column + 2 * w);
+          word[n][j][w] = four.x;
+          word[n][j][w + 1] = four.y;
+          word[n][j][w + 2] = four.z;
+          word[n][j][w + 3] = four.w;
         }
       }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : -top[n][0], top[n][1] == -INFINITY ? 0.f : -top[n][1]);
-      float2 gained = make_float2(sum[n][0], sum[n][1]);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 moved = __fadd2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), shift);
-          score[t][n][2 * h] = exp2_ftz(moved.x);
-          score[t][n][2 * h + 1] = exp2_ftz(moved.y);
-          gained = __fadd2_rn(gained, make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]));
+    auto fill = [&](int n, int stage) {                  // chunk n of the warp into a stage that nobody reads any more
+      const int key0 = chunk_at(n) * S::kKeys;
+      const uint32_t to = ring + stage * kStageBytes, bar = barrier0 + 8 * stage;
+      if constexpr (BITS == 8) {
+        if (n > 0 && n % ahead == 0) {
+          page_now = page_next;
+          page_next = look_up(n + ahead);
         }
-      }
-      sum[n][0] = gained.x;
-      sum[n][1] = gained.y;
-    }
-
-    // P^T in the layout of the second product: keys 2 corner ... of row quad
-    uint32_t weight[kTiles][NT][2], rest[kTiles][kTwoOperands ? NT : 1][2];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x = score[t][n][2 * h], y = score[t][n][2 * h + 1];
-          const uint32_t rounded = round_pair<M>(x, y);
-          weight[t][n][h] = transpose_tile(rounded);
-          if constexpr (kTwoOperands) {
-            const float2 wide = widen_pair<M>(rounded);
-            rest[t][n][h] = transpose_tile(round_pair<M>(x - wide.x, y - wide.y));
-          }
-        }
-      }
-    }
-
-    bool apart = false;                                // the rows' products have to be taken one query at a time
-    if (!open) {
-      // Values of keys that no row sees become zeros; where several queries see different keys, a probability of zero is mask enough if
-      // all the values are numbers.
-      constexpr int kUnits = W * BITS / 128;           // 16-byte units of a value
-#pragma unroll 1
-      for (int i = lane; i < S::kKeys * kUnits; i += 32) {
-        const int inside = i / kUnits, key = key0 + inside;
-        const uint32_t unit_at = v_at + S::at(inside, i % kUnits * 16);
-        if (!(key <= high && key < stop && (key > low - p.window || key < p.sinks))) {
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(unit_at), "r"(0) : "memory");
-        } else if (low != high) {
-          const uint4 unit = load_shared_16(unit_at);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t four = c == 0 ? unit.x : c == 1 ? unit.y : c == 2 ? unit.z : unit.w;
-            if constexpr (BITS == 8) {
-              apart |= (((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
-            } else {
-              constexpr uint32_t kExponent = std::is_same_v<M, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
-              apart |= (four & kExponent) == kExponent || (four >> 16 & kExponent) == kExponent;
+        const int inside = key0 & ((1 << p.page_shift) - 1);
+        if constexpr (ONE) {
+          const int page = __shfl_sync(0xffffffffu, page_now, n & 31);
+          if (lane == 0) {
+            staged_page[warp][stage][0] = page;
+            barrier_expect_tx(bar, page >= 0 ? kStageBytes : 0);
+            if (page >= 0) {
+              const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + inside;      // (below 2^31: keyed_maps)
+              tma_load_rows(to, &map_k, bar, 0, row);
+              tma_load_rows(to + kStageBytes / 2, &map_v, bar, 0, row);
             }
           }
+        } else {
+          const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
+          const bool loads = lane < boxes && page >= 0;
+          const uint32_t box_bytes = static_cast<uint32_t>(S::kLine) << box_shift;
+          const uint32_t bytes = 2u * box_bytes * __popc(__ballot_sync(0xffffffffu, loads));
+          if (lane < boxes) staged_page[warp][stage][lane] = page;
+          if (lane == 0) barrier_expect_tx(bar, bytes);
+          __syncwarp();
+          if (loads) {
+            const int row = ((page * p.kv_heads + kv_head) << p.page_shift) + ((key0 + (lane << box_shift)) & ((1 << p.page_shift) - 1));
+            tma_load_rows(to + lane * box_bytes, &map_k, bar, 0, row);
+            tma_load_rows(to + kStageBytes / 2 + lane * box_bytes, &map_v, bar, 0, row);
+          }
         }
-      }
-      apart = __any_sync(0xffffffffu, apart);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA fills the stage again
-      __syncwarp();
-    }
-
-    // One slice of V^T (16 head elements) for one tile of keys, as the instruction takes it, from the words of the lane's four keys.
-    auto operand = [&](const uint32_t (&v)[4], int half, uint32_t (&a)[4]) {
-      if constexpr (BITS == 8) {
-        const uint32_t near = __byte_perm(v[0], v[1], half ? 0x7362 : 0x5140), far = __byte_perm(v[2], v[3], half ? 0x7362 : 0x5140);
-        a[0] = decode_low(near);
-        a[1] = decode_high(near);
-        a[2] = decode_low(far);
-        a[3] = decode_high(far);
       } else {
-        a[0] = __byte_perm(v[0], v[1], 0x5410);
-        a[1] = __byte_perm(v[0], v[1], 0x7632);
-        a[2] = __byte_perm(v[2], v[3], 0x5410);
-        a[3] = __byte_perm(v[2], v[3], 0x7632);
+        if (lane == 0) {
+          barrier_expect_tx(bar, kStageBytes);
+  #pragma unroll
+          for (int l = 0; l < S::kLines; ++l) {
+            tma_load_tokens(to + l * S::kBoxBytes, &map_k, bar, l * 64, key0, kv_head, batch);
+            tma_load_tokens(to + kStageBytes / 2 + l * S::kBoxBytes, &map_v, bar, l * 64, key0, kv_head, batch);
+          }
+        }
       }
     };
-    auto key_of = [&](int t, int r) { return t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1); };
-    constexpr int kHalves = BITS == 8 ? 2 : 1;
-    if (!apart) {
-      // O^T += V^T P^T
-      uint32_t value[kTiles][4][S::kValueWords];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (S::kValueWords == 2) {
-            const uint2 two = load_shared_8(v_at + S::at(key_of(t, r), quad * 8));
-            value[t][r][0] = two.x;
-            value[t][r][1] = two.y;
-          } else {
-#pragma unroll
-            for (int w = 0; w < S::kValueWords; w += 4) {
-              const uint4 four = load_shared_16(v_at + S::at(key_of(t, r), ((w / 4) * 8 + quad) * 16));
-              value[t][r][w] = four.x;
-              value[t][r][w + 1] = four.y;
-              value[t][r][w + 2] = four.z;
-              value[t][r][w + 3] = four.w;
-            }
+    // The scales of the next chunk's pages (of its tile t in lane t, unless they are one page's) are asked for a step before they are used; 0: no
+    // page.
+    float k_scale_next = 0.f, v_scale_next = 0.f;
+    auto ask_scales = [&](int stage) {
+      if constexpr (BITS == 8) {
+        if (ONE || lane < kTiles) {
+          const int page = staged_page[warp][stage][ONE ? 0 : (lane * 16) >> box_shift];
+          k_scale_next = v_scale_next = 0.f;
+          if (page >= 0) {
+            const int block = page * p.kv_heads + kv_head;
+            k_scale_next = p.k_scales[block];
+            v_scale_next = p.v_scales[block];
           }
         }
       }
-#pragma unroll
-      for (int w = 0; w < S::kValueWords; ++w) {
-#pragma unroll
-        for (int half = 0; half < kHalves; ++half) {
-          const int slice = kHalves * w + half;
-          float d[NT][4];
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            uint32_t a[4];
-            const uint32_t v[4] = {value[t][0][w], value[t][1][w], value[t][2][w], value[t][3][w]};
-            operand(v, half, a);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if constexpr (BITS == 16) {
-                multiply<M>(result[n][slice], a, weight[t][n][0], weight[t][n][1], false);
-                if constexpr (kTwoOperands) multiply<M>(result[n][slice], a, rest[t][n][0], rest[t][n][1], false);
-              } else {
-                multiply<M>(d[n], a, weight[t][n][0], weight[t][n][1], kScales > 1 || t == 0);
-              }
-              if constexpr (kScales > 1) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) result[n][slice][e] = fmaf(d[n][e], v_scale[t], result[n][slice][e]);
-              }
-            }
+    };
+    for (int first = 0; first < min(mine, kKeyedStages); ++first) fill(first, (turn + first) % kKeyedStages);
+    __syncwarp();
+    if (mine > 0) ask_scales(turn % kKeyedStages);
+
+    // ... as the matrix instructions take it: [piece][step of 16 elements][operand word]
+    uint32_t query[NT][S::kPieces][32 / BITS][2];
+    float row_scale[NT][2];                                        // of the lane's two columns: rows 2 corner and 2 corner + 1
+    int position[NT][2];
+  #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float back = p.scale_log2;
+      if constexpr (BITS == 8) {
+        float largest = 0.f;
+  #pragma unroll
+        for (int j = 0; j < S::kPieces; ++j) {
+  #pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            const float2 pair = widen_pair<T>(word[n][j][w]);
+            largest = fmaxf(largest, fmaxf(fabsf(pair.x), fabsf(pair.y)));
           }
-          if constexpr (BITS == 8 && kScales == 1) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                const float2 sum2 = __ffma2_rn(make_float2(d[n][e], d[n][e + 1]), make_float2(v_scale[0], v_scale[0]), make_float2(result[n][slice][e], result[n][slice][e + 1]));
-                result[n][slice][e] = sum2.x;
-                result[n][slice][e + 1] = sum2.y;
-              }
-            }
+        }
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        // a power of two that brings the row's largest element to [2^14, 2^15); none for zeros and infinities
+        int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
+        if (exponent < -100 || exponent > 127) exponent = 14;
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
+        back *= __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
+  #pragma unroll
+        for (int j = 0; j < S::kPieces; ++j) {
+  #pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            const float2 pair = widen_pair<T>(word[n][j][w]);
+            word[n][j][w] = round_pair<__half>(pair.x * up, pair.y * up);
           }
         }
       }
-    } else {
-      // (Rare, and written to be small.) The probabilities go where the chunk's keys were, and each query has a pass of its own over the tiles, with the
-      // values it does not see as zeros; each row keeps what its own query's pass gives.
-      uint32_t* const kept = reinterpret_cast<uint32_t*>(parts_at + warp * kWarpRing + stage * kStageBytes);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            kept[((t * NT + n) * 4 + h) * 32 + lane] = weight[t][n][h];
-            if constexpr (kTwoOperands) kept[((t * NT + n) * 4 + 2 + h) * 32 + lane] = rest[t][n][h];
+  #pragma unroll
+      for (int j = 0; j < S::kPieces; ++j) {
+  #pragma unroll
+        for (int w = 0; w < kWords; ++w) query[n][j][w / 2][w % 2] = word[n][j][w];
+      }
+  #pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * corner + e) * 4);
+        const int here = row0 + n * 8 + 2 * corner + e;
+        position[n][e] = here < rows ? length - p.q_tokens + here / p.group : high;
+      }
+    }
+
+    float top[NT][2], sum[NT][2], result[NT][kSlices][4];
+  #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = -INFINITY;
+        sum[n][e] = 0.f;
+      }
+  #pragma unroll
+      for (int s = 0; s < kSlices; ++s) {
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) result[n][s][e] = 0.f;
+      }
+    }
+
+    for (int step = 0; step < mine; ++step, ++turn) {
+      const int key0 = chunk_at(step) * S::kKeys;
+      const int stage = turn % kKeyedStages;
+      if (!barrier_wait(barrier0 + 8 * stage, (turn / kKeyedStages) & 1, p.status, kWaitKeyed)) {
+        // the result is lost (the status says so); the copies that are under way still have to land before the stages are used otherwise
+        for (int m = step; m < min(step + kKeyedStages, mine); ++m, ++turn) {
+          for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(barrier0 + 8 * (turn % kKeyedStages), (turn / kKeyedStages) & 1); ++spin) {
           }
         }
+        break;
       }
-#pragma unroll 1
-      for (int at = low; at <= high; ++at) {
-#pragma unroll 1
+      const uint32_t k_at = ring + stage * kStageBytes, v_at = k_at + kStageBytes / 2;
+      int stop = length;                                 // keys from here on are not there
+      constexpr int kScales = BITS == 8 && !ONE ? kTiles : 1;
+      float k_scale[kScales], v_scale[kScales], v_scale_now = 0.f;
+      k_scale[0] = k_scale_next;
+      v_scale[0] = v_scale_next;
+      if constexpr (BITS == 8) {
+        if constexpr (ONE) {
+          if (staged_page[warp][stage][0] < 0) stop = key0;
+        } else {
+  #pragma unroll
+          for (int t = kTiles - 1; t >= 0; --t) {
+            k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
+            v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
+            if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
+          }
+        }
+        v_scale_now = v_scale_next;
+        if (step + 1 < mine) ask_scales((turn + 1) % kKeyedStages);
+      }
+
+      // S^T: keys quad and quad + 8 of each tile by rows 2 corner and 2 corner + 1
+      float score[kTiles][NT][4];
+  #pragma unroll
+      for (int j = 0; j < S::kPieces; ++j) {
+        uint4 near[kTiles], far[kTiles];
+  #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          float scale = v_scale[0];
-          if constexpr (kScales > 1) scale = __shfl_sync(0xffffffffu, v_scale_now, t);
-#pragma unroll
-          for (int w = 0; w < S::kValueWords; ++w) {
-            uint32_t v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int column = S::kValueWords == 2 ? quad * 8 + w * 4 : ((w / 4) * 8 + quad) * 16 + w % 4 * 4;
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(v_at + S::at(key_of(t, r), column)));
-              if (!sees(at, key0 + key_of(t, r))) v[r] = 0;
+          near[t] = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
+          far[t] = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
+        }
+  #pragma unroll
+        for (int w = 0; w < 32 / BITS; ++w) {
+  #pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const uint32_t x[4] = {near[t].x, near[t].y, near[t].z, near[t].w}, y[4] = {far[t].x, far[t].y, far[t].z, far[t].w};
+            uint32_t a[4];
+            if constexpr (BITS == 8) {
+              a[0] = decode_low(x[w]);
+              a[1] = decode_low(y[w]);
+              a[2] = decode_high(x[w]);
+              a[3] = decode_high(y[w]);
+            } else {
+              a[0] = x[2 * w];
+              a[1] = y[2 * w];
+              a[2] = x[2 * w + 1];
+              a[3] = y[2 * w + 1];
             }
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
+  #pragma unroll
+            for (int n = 0; n < NT; ++n) multiply<M>(score[t][n], a, query[n][j][w][0], query[n][j][w][1], j == 0 && w == 0);
+          }
+        }
+      }
+
+      // A chunk whose keys every row sees needs no mask.
+      const int last = key0 + S::kKeys - 1;
+      const bool open = last <= low && last < stop && (key0 > high - p.window || last < p.sinks);
+      auto sees = [&](int at, int key) { return key <= at && key < stop && (key > at - p.window || key < p.sinks); };
+      // Any reference point gives the same softmax: a row's moves only when a score lies more than 2^kSlack above it, which one vote tells.
+      float most[NT][2];
+      bool rises = false;
+  #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        most[n][0] = most[n][1] = -INFINITY;
+  #pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          float2 by = make_float2(row_scale[n][0], row_scale[n][1]);
+          if constexpr (BITS == 8) by = __fmul2_rn(by, make_float2(k_scale[t % kScales], k_scale[t % kScales]));
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 scaled = __fmul2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), by);
+            score[t][n][2 * h] = scaled.x;
+            score[t][n][2 * h + 1] = scaled.y;
+            if (!open) {
+  #pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (!sees(position[n][e], key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
+            }
+          }
+  #pragma unroll
+          for (int e = 0; e < 2; ++e) most[n][e] = fmaxf(most[n][e], fmaxf(score[t][n][e], score[t][n][2 + e]));
+        }
+  #pragma unroll
+        for (int e = 0; e < 2; ++e) rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
+      }
+      if (__any_sync(0xffffffffu, rises)) {
+  #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float now = most[n][e];
+            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
+            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
+            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+            now = fmaxf(now, top[n][e]);
+            const float factor = rescale(top[n][e], now);
+            top[n][e] = now;
+            sum[n][e] *= factor;
+  #pragma unroll
+            for (int s = 0; s < kSlices; ++s) {
+              result[n][s][e] *= factor;
+              result[n][s][2 + e] *= factor;
+            }
+          }
+        }
+      }
+  #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : -top[n][0], top[n][1] == -INFINITY ? 0.f : -top[n][1]);
+        float2 gained = make_float2(sum[n][0], sum[n][1]);
+  #pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 moved = __fadd2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), shift);
+            score[t][n][2 * h] = exp2_ftz(moved.x);
+            score[t][n][2 * h + 1] = exp2_ftz(moved.y);
+            gained = __fadd2_rn(gained, make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]));
+          }
+        }
+        sum[n][0] = gained.x;
+        sum[n][1] = gained.y;
+      }
+
+      // P^T in the layout of the second product: keys 2 corner ... of row quad
+      uint32_t weight[kTiles][NT][2], rest[kTiles][kTwoOperands ? NT : 1][2];
+  #pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+  #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = score[t][n][2 * h], y = score[t][n][2 * h + 1];
+            const uint32_t rounded = round_pair<M>(x, y);
+            weight[t][n][h] = transpose_tile(rounded);
+            if constexpr (kTwoOperands) {
+              const float2 wide = widen_pair<M>(rounded);
+              rest[t][n][h] = transpose_tile(round_pair<M>(x - wide.x, y - wide.y));
+            }
+          }
+        }
+      }
+
+      bool apart = false;                                // the rows' products have to be taken one query at a time
+      if (!open) {
+        // Values of keys that no row sees become zeros; where several queries see different keys, a probability of zero is mask enough if
+        // all the values are numbers.
+        constexpr int kUnits = W * BITS / 128;           // 16-byte units of a value
+  #pragma unroll 1
+        for (int i = lane; i < S::kKeys * kUnits; i += 32) {
+          const int inside = i / kUnits, key = key0 + inside;
+          const uint32_t unit_at = v_at + S::at(inside, i % kUnits * 16);
+          if (!(key <= high && key < stop && (key > low - p.window || key < p.sinks))) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(unit_at), "r"(0) : "memory");
+          } else if (low != high) {
+            const uint4 unit = load_shared_16(unit_at);
+  #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t four = c == 0 ? unit.x : c == 1 ? unit.y : c == 2 ? unit.z : unit.w;
+              if constexpr (BITS == 8) {
+                apart |= (((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+              } else {
+                constexpr uint32_t kExponent = std::is_same_v<M, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+                apart |= (four & kExponent) == kExponent || (four >> 16 & kExponent) == kExponent;
+              }
+            }
+          }
+        }
+        apart = __any_sync(0xffffffffu, apart);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA fills the stage again
+        __syncwarp();
+      }
+
+      // One slice of V^T (16 head elements) for one tile of keys, as the instruction takes it, from the words of the lane's four keys.
+      auto operand = [&](const uint32_t (&v)[4], int half, uint32_t (&a)[4]) {
+        if constexpr (BITS == 8) {
+          const uint32_t near = __byte_perm(v[0], v[1], half ? 0x7362 : 0x5140), far = __byte_perm(v[2], v[3], half ? 0x7362 : 0x5140);
+          a[0] = decode_low(near);
+          a[1] = decode_high(near);
+          a[2] = decode_low(far);
+          a[3] = decode_high(far);
+        } else {
+          a[0] = __byte_perm(v[0], v[1], 0x5410);
+          a[1] = __byte_perm(v[0], v[1], 0x7632);
+          a[2] = __byte_perm(v[2], v[3], 0x5410);
+          a[3] = __byte_perm(v[2], v[3], 0x7632);
+        }
+      };
+      auto key_of = [&](int t, int r) { return t * 16 + 2 * corner + (r & 1) + 8 * (r >> 1); };
+      constexpr int kHalves = BITS == 8 ? 2 : 1;
+      if (!apart) {
+        // O^T += V^T P^T
+        uint32_t value[kTiles][4][S::kValueWords];
+  #pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+  #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (S::kValueWords == 2) {
+              const uint2 two = load_shared_8(v_at + S::at(key_of(t, r), quad * 8));
+              value[t][r][0] = two.x;
+              value[t][r][1] = two.y;
+            } else {
+  #pragma unroll
+              for (int w = 0; w < S::kValueWords; w += 4) {
+                const uint4 four = load_shared_16(v_at + S::at(key_of(t, r), ((w / 4) * 8 + quad) * 16));
+                value[t][r][w] = four.x;
+                value[t][r][w + 1] = four.y;
+                value[t][r][w + 2] = four.z;
+                value[t][r][w + 3] = four.w;
+              }
+            }
+          }
+        }
+  #pragma unroll
+        for (int w = 0; w < S::kValueWords; ++w) {
+  #pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+            const int slice = kHalves * w + half;
+            float d[NT][4];
+  #pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
               uint32_t a[4];
+              const uint32_t v[4] = {value[t][0][w], value[t][1][w], value[t][2][w], value[t][3][w]};
               operand(v, half, a);
-#pragma unroll
+  #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const uint32_t* b = kept + (t * NT + n) * 4 * 32 + lane;
-                float d[4];
-                multiply<M>(d, a, b[0], b[32], true);
-                if constexpr (kTwoOperands) multiply<M>(d, a, b[64], b[96], false);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if (position[n][e & 1] == at) {
-                    float& into = result[n][kHalves * w + half][e];
-                    into = BITS == 8 ? fmaf(d[e], scale, into) : into + d[e];
+                if constexpr (BITS == 16) {
+                  multiply<M>(result[n][slice], a, weight[t][n][0], weight[t][n][1], false);
+                  if constexpr (kTwoOperands) multiply<M>(result[n][slice], a, rest[t][n][0], rest[t][n][1], false);
+                } else {
+                  multiply<M>(d[n], a, weight[t][n][0], weight[t][n][1], kScales > 1 || t == 0);
+                }
+                if constexpr (kScales > 1) {
+  #pragma unroll
+                  for (int e = 0; e < 4; ++e) result[n][slice][e] = fmaf(d[n][e], v_scale[t], result[n][slice][e]);
+                }
+              }
+            }
+            if constexpr (BITS == 8 && kScales == 1) {
+  #pragma unroll
+              for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                  const float2 sum2 = __ffma2_rn(make_float2(d[n][e], d[n][e + 1]), make_float2(v_scale[0], v_scale[0]), make_float2(result[n][slice][e], result[n][slice][e + 1]));
+                  result[n][slice][e] = sum2.x;
+                  result[n][slice][e + 1] = sum2.y;
+                }
+              }
+            }
+          }
+        }
+      } else {
+        // (Rare, and written to be small.) The probabilities go where the chunk's keys were, and each query has a pass of its own over the tiles,
+        // with the values it does not see as zeros; each row keeps what its own query's pass gives.
+        uint32_t* const kept = reinterpret_cast<uint32_t*>(parts_at + warp * kWarpRing + stage * kStageBytes);
+  #pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+  #pragma unroll
+          for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              kept[((t * NT + n) * 4 + h) * 32 + lane] = weight[t][n][h];
+              if constexpr (kTwoOperands) kept[((t * NT + n) * 4 + 2 + h) * 32 + lane] = rest[t][n][h];
+            }
+          }
+        }
+  #pragma unroll 1
+        for (int at = low; at <= high; ++at) {
+  #pragma unroll 1
+          for (int t = 0; t < kTiles; ++t) {
+            float scale = v_scale[0];
+            if constexpr (kScales > 1) scale = __shfl_sync(0xffffffffu, v_scale_now, t);
+  #pragma unroll
+            for (int w = 0; w < S::kValueWords; ++w) {
+              uint32_t v[4];
+  #pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int column = S::kValueWords == 2 ? quad * 8 + w * 4 : ((w / 4) * 8 + quad) * 16 + w % 4 * 4;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(v_at + S::at(key_of(t, r), column)));
+                if (!sees(at, key0 + key_of(t, r))) v[r] = 0;
+              }
+  #pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                uint32_t a[4];
+                operand(v, half, a);
+  #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint32_t* b = kept + (t * NT + n) * 4 * 32 + lane;
+                  float d[4];
+                  multiply<M>(d, a, b[0], b[32], true);
+                  if constexpr (kTwoOperands) multiply<M>(d, a, b[64], b[96], false);
+  #pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    if (position[n][e & 1] == at) {
+                      float& into = result[n][kHalves * w + half][e];
+                      into = BITS == 8 ? fmaf(d[e], scale, into) : into + d[e];
+                    }
                   }
                 }
               }
             }
           }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();                                      // the stage has been read
+      if (step + kKeyedStages < mine) fill(step + kKeyedStages, stage);
     }
-    __syncwarp();                                      // the stage has been read
-    if (step + kKeyedStages < mine) fill(step + kKeyedStages, stage);
-  }
 
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int offset = 4; offset < 32; offset *= 2) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], offset);
-    }
-  }
-  // A lane has, of its rows, runs of eight neighbouring elements.
-  constexpr int kRuns = kSlices / 4;
-  auto column_of = [&](int run) { return BITS == 8 ? quad * (W / 8) + 8 * run : run * 64 + quad * 8; };
-  auto run_of = [&](int n, int e, int run, float (&value)[8]) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      value[2 * c] = result[n][4 * run + c][e];
-      value[2 * c + 1] = result[n][4 * run + c][2 + e];
-    }
-  };
-  if constexpr (SHARED) {
-    const long long slot0 = (2LL * share + (begins ? 1 : 0)) * kRows;
-#pragma unroll
+  #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
+  #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = n * 8 + 2 * corner + e;
-        if (row0 + row >= rows) continue;
-        if (!whole && quad == 0) *(JOINS > 1 ? &piece_stats[JOINS > 1 ? warp : 0][begins ? 1 : 0][JOINS > 1 ? row : 0] : p.part_stats + slot0 + row) = make_float2(top[n][e], sum[n][e]);
-#pragma unroll
-        for (int run = 0; run < kRuns; ++run) {
-          float value[8];
-          run_of(n, e, run, value);
-          const int column = column_of(run);
-          if (column >= p.head_dim) continue;
-          if (whole) {
-            write_result<T>(p, batch, kv_head, row0 + row, column, length, sum[n][e], value);
-          } else {
-            float4* to = reinterpret_cast<float4*>((JOINS > 1 ? piece_at(warp, begins ? 1 : 0) + row * W : p.parts + (slot0 + row) * W) + column);
+  #pragma unroll
+        for (int offset = 4; offset < 32; offset *= 2) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], offset);
+      }
+    }
+    // A lane has, of its rows, runs of eight neighbouring elements.
+    constexpr int kRuns = kSlices / 4;
+    auto column_of = [&](int run) { return BITS == 8 ? quad * (W / 8) + 8 * run : run * 64 + quad * 8; };
+    auto run_of = [&](int n, int e, int run, float (&value)[8]) {
+  #pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        value[2 * c] = result[n][4 * run + c][e];
+        value[2 * c + 1] = result[n][4 * run + c][2 + e];
+      }
+    };
+    if constexpr (SHARED) {
+      const long long slot0 = (2LL * share + (begins ? 1 : 0)) * kRows;
+  #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + 2 * corner + e;
+          if (row0 + row >= rows) continue;
+          if (!whole && quad == 0) *(JOINS > 1 ? &piece_stats[JOINS > 1 ? warp : 0][begins ? 1 : 0][JOINS > 1 ? row : 0] : p.part_stats + slot0 + row) = make_float2(top[n][e], sum[n][e]);
+  #pragma unroll
+          for (int run = 0; run < kRuns; ++run) {
+            float value[8];
+            run_of(n, e, run, value);
+            const int column = column_of(run);
+            if (column >= p.head_dim) continue;
+            if (whole) {
+              write_result<T>(p, batch, kv_head, row0 + row, column, length, sum[n][e], value);
+            } else {
+              float4* to = reinterpret_cast<float4*>((JOINS > 1 ? piece_at(warp, begins ? 1 : 0) + row * W : p.parts + (slot0 + row) * W) + column);
+              to[0] = make_float4(value[0], value[1], value[2], value[3]);
+              to[1] = make_float4(value[4], value[5], value[6], value[7]);
+            }
+          }
+        }
+      }
+    } else {
+  #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = n * 8 + 2 * corner + e;
+          if (quad == 0) {
+            part_top[warp][row] = top[n][e];
+            part_sum[warp][row] = sum[n][e];
+          }
+  #pragma unroll
+          for (int run = 0; run < kRuns; ++run) {
+            float value[8];
+            run_of(n, e, run, value);
+            float4* to = reinterpret_cast<float4*>(parts_at + warp * kWarpRing + (row * W + column_of(run)) * 4);
             to[0] = make_float4(value[0], value[1], value[2], value[3]);
             to[1] = make_float4(value[4], value[5], value[6], value[7]);
           }
         }
       }
-    }
-  } else {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = n * 8 + 2 * corner + e;
-        if (quad == 0) {
-          part_top[warp][row] = top[n][e];
-          part_sum[warp][row] = sum[n][e];
+      __syncthreads();
+      for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
+        const int row = item / (W / 8), column = item % (W / 8) * 8;
+        if (row0 + row >= rows || column >= p.head_dim) continue;
+        float most = part_top[0][row];
+  #pragma unroll
+        for (int w = 1; w < kKeyedWarps; ++w) most = fmaxf(most, part_top[w][row]);
+        float total = 0.f, value[8] = {};
+  #pragma unroll
+        for (int w = 0; w < kKeyedWarps; ++w) {
+          const float by = rescale(part_top[w][row], most);
+          total += part_sum[w][row] * by;
+  #pragma unroll
+          for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
         }
-#pragma unroll
-        for (int run = 0; run < kRuns; ++run) {
-          float value[8];
-          run_of(n, e, run, value);
-          float4* to = reinterpret_cast<float4*>(parts_at + warp * kWarpRing + (row * W + column_of(run)) * 4);
-          to[0] = make_float4(value[0], value[1], value[2], value[3]);
-          to[1] = make_float4(value[4], value[5], value[6], value[7]);
-        }
+        write_result<T>(p, batch, kv_head, row0 + row, column, length, total, value);
       }
     }
-    __syncthreads();
-    for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
-      const int row = item / (W / 8), column = item % (W / 8) * 8;
-      if (row0 + row >= rows || column >= p.head_dim) continue;
-      float most = part_top[0][row];
-#pragma unroll
-      for (int w = 1; w < kKeyedWarps; ++w) most = fmaxf(most, part_top[w][row]);
-      float total = 0.f, value[8] = {};
-#pragma unroll
-      for (int w = 0; w < kKeyedWarps; ++w) {
-        const float by = rescale(part_top[w][row], most);
-        total += part_sum[w][row] * by;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
-      }
-      write_result<T>(p, batch, kv_head, row0 + row, column, length, total, value);
-    }
-  }
   }
   if constexpr (JOINS > 1) {
-    // The pieces of a unit meet, in the order of the warps; what other CTAs have parts of too goes to memory, as the part of the first of its warps.
+    // The pieces of a unit meet, in the order of the warps; what other CTAs have parts of too goes to memory, as the part of the first of its
+    // warps.
     __syncthreads();
     for (int i = 0; i < 2 * kKeyedWarps;) {
       if (!pieces[i / 2][i % 2].there) {
@@ -1011,9 +1030,9 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
 }
 
-// SHARED: joins the parts of the units that a border between two shares (or two CTAs' shares: JOINS of them) cut. A CTA for each border; the CTAs of a
-// unit's borders split its result, 64 elements of a row at a time: eight lanes of eight elements, by as many groups as there are
-// parts, four groups in a warp or, of many parts, sixteen in the CTA.
+// SHARED: joins the parts of the units that a border between two shares (or two CTAs' shares: JOINS of them) cut. A CTA for each border; the CTAs
+// of a unit's borders split its result, 64 elements of a row at a time: eight lanes of eight elements, by as many groups as there are parts, four
+// groups in a warp or, of many parts, sixteen in the CTA.
 template <typename T, int W, int NT, int JOINS>
 __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_constant__ KeyedParams p) {
   constexpr int kRows = 8 * NT;
@@ -1141,9 +1160,10 @@ long long most_chunks(const KeyedParams& p, long long tokens, long long keys, in
   return all < seen ? all : seen;
 }
 
-// A unit of few chunks is a CTA's; of more, chunks are dealt out, which costs the finding of places at the start and the join at the end: from 14 us on, whatever there is to do.
-// A CTA a unit takes 6 and about 1 for each step of its warps, and where CTAs come in several waves about 5 more for each. In us, CTA a unit and dealt out, 16-bit queries: 12 heads of 64
-// 1000 tokens 9.3 / 14.5, 64 x 12 heads 25.1 / 29.0, 64 x 12 x 1500 32.9 / 37.4, 8 x 8 key heads of 128 1000 tokens 12.4 / 16.5, 128 x 8 x 300 30.8 / 26.8, x 600 40.8 / 39.0.
+// A unit of few chunks is a CTA's; of more, chunks are dealt out, which costs the finding of places at the start and the join at the end: from 14
+// us on, whatever there is to do. A CTA a unit takes 6 and about 1 for each step of its warps, and where CTAs come in several waves about 5 more
+// for each. In us, CTA a unit and dealt out, 16-bit queries: 12 heads of 64 1000 tokens 9.3 / 14.5, 64 x 12 heads 25.1 / 29.0, 64 x 12 x 1500
+// 32.9 / 37.4, 8 x 8 key heads of 128 1000 tokens 12.4 / 16.5, 128 x 8 x 300 30.8 / 26.8, x 600 40.8 / 39.0.
 constexpr int kFewChunks = 2 * kKeyedWarps, kSomeChunks = 8 * kKeyedWarps;
 
 // From as many parts a unit on, the warps of a CTA join theirs before they go to memory.
