@@ -81,7 +81,7 @@ struct KeyedShape {
   }
 };
 // The rings and, where a CTA's warps join their parts of a unit first, room for each warp's first part (its last one goes where its ring was).
-constexpr size_t keyed_smem(bool gather, int w, int nt) { return 1024 + kKeyedWarps * (kWarpRing + (gather ? 8 * nt * w * sizeof(float) : 0)); }
+constexpr size_t keyed_smem(bool gather, int w, int nt, int warps = kKeyedWarps) { return 1024 + warps * (kWarpRing + (gather ? 8 * nt * w * sizeof(float) : 0)); }
 
 __device__ __forceinline__ uint4 load_shared_16(uint32_t address) {
   uint4 word;
@@ -247,6 +247,17 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   __shared__ Place found[kKeyedWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int units = p.kv_heads * p.row_tiles;
+  if constexpr (BITS == 16) {      // all sequences are alike
+    const int each = (unit_cost(CHUNK) + counted<BITS, CHUNK>(p, 0)) * units;
+    Dealt dealt;
+    dealt.total = each * p.batch;
+    dealt.shares = min(p.shares, (dealt.total + kLeastShare - 1) / kLeastShare);
+    dealt.each = dealt.total / dealt.shares;
+    dealt.longer = dealt.total % dealt.shares;
+    const int sequence = dealt.start(min(first_share + warp, dealt.shares - 1)) / each;
+    place = {sequence, sequence * each};
+    return dealt;
+  }
   const int run = (p.batch + kKeyedThreads - 1) / kKeyedThreads;
   const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
   int mine = 0;
@@ -293,20 +304,21 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal
 // shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared
 // memory. ONE: a chunk lies in one page (or in none: dense keys).
-template <typename T, int BITS, int W, int NT, int JOINS, bool ONE>
-__global__ void __launch_bounds__(kKeyedThreads, 2)
+template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps>
+__global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
   using M = std::conditional_t<BITS == 8, __half, T>;      // what the matrix instructions take
   constexpr bool SHARED = JOINS > 0;
+  static_assert(!SHARED || WARPS == kKeyedWarps, "shares are dealt out to CTAs of four warps");
   constexpr int kUnitCost = unit_cost(S::kKeys);
   constexpr bool kTwoOperands = std::is_same_v<M, __nv_bfloat16>;
   constexpr int kRows = 8 * NT, kTiles = S::kTiles, kSlices = S::kSlices;
   static_assert(kRows * W * sizeof(float) <= kWarpRing, "a warp leaves its part where its stages were");
   extern __shared__ unsigned char raw_smem[];
-  __shared__ float part_top[SHARED ? 1 : kKeyedWarps][kRows], part_sum[SHARED ? 1 : kKeyedWarps][kRows];
-  __shared__ __align__(8) uint64_t full[kKeyedWarps][kKeyedStages];
-  __shared__ int staged_page[kKeyedWarps][kKeyedStages][4];      // of each box of a stage; -1: not there
+  __shared__ float part_top[SHARED ? 1 : WARPS][kRows], part_sum[SHARED ? 1 : WARPS][kRows];
+  __shared__ __align__(8) uint64_t full[WARPS][kKeyedStages];
+  __shared__ int staged_page[WARPS][kKeyedStages][4];      // of each box of a stage; -1: not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring_all = (smem_address(raw_smem) + 1023u) & ~1023u, ring = ring_all + warp * kWarpRing;
@@ -337,7 +349,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group
 
   // SHARED: this warp's share of the range, [at, until)
-  constexpr int kStep = SHARED ? 1 : kKeyedWarps;      // a warp takes every chunk of its share, or every fourth of the unit
+  constexpr int kStep = SHARED ? 1 : WARPS;            // a warp takes every chunk of its share, or every WARPS-th of the unit
   const int share = static_cast<int>(blockIdx.x) * kKeyedWarps + warp;
   Place place = {0, 0};
   int at = 0, until = 1;
@@ -428,15 +440,15 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // The query: row `quad` of each eight, the elements that the lane's pieces of a key hold.
     constexpr int kWords = S::kPieceWidth / 2;                     // of a piece's query elements: 8 or 4
     uint32_t word[NT][S::kPieces][kWords];
-  #pragma unroll
+#pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + n * 8 + quad;
       const int token = row / p.group, head = kv_head * p.group + row % p.group;
       const T* from = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
-  #pragma unroll
+#pragma unroll
       for (int j = 0; j < S::kPieces; ++j) {
         const int column = (4 * j + corner) * S::kPieceWidth;
-  #pragma unroll
+#pragma unroll
         for (int w = 0; w < kWords; w += 4) {
           uint4 four = make_uint4(0, 0, 0, 0);
           if (row < rows && column + 2 * w < p.head_dim) four = *reinterpret_cast<const uint4*>(from + column + 2 * w);
@@ -484,7 +496,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       } else {
         if (lane == 0) {
           barrier_expect_tx(bar, kStageBytes);
-  #pragma unroll
+#pragma unroll
           for (int l = 0; l < S::kLines; ++l) {
             tma_load_tokens(to + l * S::kBoxBytes, &map_k, bar, l * 64, key0, kv_head, batch);
             tma_load_tokens(to + kStageBytes / 2 + l * S::kBoxBytes, &map_v, bar, l * 64, key0, kv_head, batch);
@@ -516,14 +528,14 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint32_t query[NT][S::kPieces][32 / BITS][2];
     float row_scale[NT][2];                                        // of the lane's two columns: rows 2 corner and 2 corner + 1
     int position[NT][2];
-  #pragma unroll
+#pragma unroll
     for (int n = 0; n < NT; ++n) {
       float back = p.scale_log2;
       if constexpr (BITS == 8) {
         float largest = 0.f;
-  #pragma unroll
+#pragma unroll
         for (int j = 0; j < S::kPieces; ++j) {
-  #pragma unroll
+#pragma unroll
           for (int w = 0; w < kWords; ++w) {
             const float2 pair = widen_pair<T>(word[n][j][w]);
             largest = fmaxf(largest, fmaxf(fabsf(pair.x), fabsf(pair.y)));
@@ -536,21 +548,21 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (exponent < -100 || exponent > 127) exponent = 14;
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
         back *= __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
-  #pragma unroll
+#pragma unroll
         for (int j = 0; j < S::kPieces; ++j) {
-  #pragma unroll
+#pragma unroll
           for (int w = 0; w < kWords; ++w) {
             const float2 pair = widen_pair<T>(word[n][j][w]);
             word[n][j][w] = round_pair<__half>(pair.x * up, pair.y * up);
           }
         }
       }
-  #pragma unroll
+#pragma unroll
       for (int j = 0; j < S::kPieces; ++j) {
-  #pragma unroll
+#pragma unroll
         for (int w = 0; w < kWords; ++w) query[n][j][w / 2][w % 2] = word[n][j][w];
       }
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 2; ++e) {
         row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * corner + e) * 4);
         const int here = row0 + n * 8 + 2 * corner + e;
@@ -559,16 +571,16 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
 
     float top[NT][2], sum[NT][2], result[NT][kSlices][4];
-  #pragma unroll
+#pragma unroll
     for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[n][e] = -INFINITY;
         sum[n][e] = 0.f;
       }
-  #pragma unroll
+#pragma unroll
       for (int s = 0; s < kSlices; ++s) {
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 4; ++e) result[n][s][e] = 0.f;
       }
     }
@@ -594,7 +606,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if constexpr (ONE) {
           if (staged_page[warp][stage][0] < 0) stop = key0;
         } else {
-  #pragma unroll
+#pragma unroll
           for (int t = kTiles - 1; t >= 0; --t) {
             k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
             v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
@@ -607,17 +619,17 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
       // S^T: keys quad and quad + 8 of each tile by rows 2 corner and 2 corner + 1
       float score[kTiles][NT][4];
-  #pragma unroll
+#pragma unroll
       for (int j = 0; j < S::kPieces; ++j) {
         uint4 near[kTiles], far[kTiles];
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           near[t] = load_shared_16(k_at + S::at(t * 16 + quad, (4 * j + corner) * 16));
           far[t] = load_shared_16(k_at + S::at(t * 16 + quad + 8, (4 * j + corner) * 16));
         }
-  #pragma unroll
+#pragma unroll
         for (int w = 0; w < 32 / BITS; ++w) {
-  #pragma unroll
+#pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const uint32_t x[4] = {near[t].x, near[t].y, near[t].z, near[t].w}, y[4] = {far[t].x, far[t].y, far[t].z, far[t].w};
             uint32_t a[4];
@@ -632,7 +644,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
               a[2] = x[2 * w + 1];
               a[3] = y[2 * w + 1];
             }
-  #pragma unroll
+#pragma unroll
             for (int n = 0; n < NT; ++n) multiply<M>(score[t][n], a, query[n][j][w][0], query[n][j][w][1], j == 0 && w == 0);
           }
         }
@@ -645,34 +657,34 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       // Any reference point gives the same softmax: a row's moves only when a score lies more than 2^kSlack above it, which one vote tells.
       float most[NT][2];
       bool rises = false;
-  #pragma unroll
+#pragma unroll
       for (int n = 0; n < NT; ++n) {
         most[n][0] = most[n][1] = -INFINITY;
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           float2 by = make_float2(row_scale[n][0], row_scale[n][1]);
           if constexpr (BITS == 8) by = __fmul2_rn(by, make_float2(k_scale[t % kScales], k_scale[t % kScales]));
-  #pragma unroll
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float2 scaled = __fmul2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), by);
             score[t][n][2 * h] = scaled.x;
             score[t][n][2 * h + 1] = scaled.y;
             if (!open) {
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < 2; ++e)
                 if (!sees(position[n][e], key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
             }
           }
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 2; ++e) most[n][e] = fmaxf(most[n][e], fmaxf(score[t][n][e], score[t][n][2 + e]));
         }
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 2; ++e) rises |= most[n][e] > top[n][e] + kSlack;      // (-inf + kSlack is -inf)
       }
       if (__any_sync(0xffffffffu, rises)) {
-  #pragma unroll
+#pragma unroll
         for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 2; ++e) {
             float now = most[n][e];
             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
@@ -682,7 +694,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const float factor = rescale(top[n][e], now);
             top[n][e] = now;
             sum[n][e] *= factor;
-  #pragma unroll
+#pragma unroll
             for (int s = 0; s < kSlices; ++s) {
               result[n][s][e] *= factor;
               result[n][s][2 + e] *= factor;
@@ -690,13 +702,13 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
       }
-  #pragma unroll
+#pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : -top[n][0], top[n][1] == -INFINITY ? 0.f : -top[n][1]);
         float2 gained = make_float2(sum[n][0], sum[n][1]);
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-  #pragma unroll
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float2 moved = __fadd2_rn(make_float2(score[t][n][2 * h], score[t][n][2 * h + 1]), shift);
             score[t][n][2 * h] = exp2_ftz(moved.x);
@@ -710,11 +722,11 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
       // P^T in the layout of the second product: keys 2 corner ... of row quad
       uint32_t weight[kTiles][NT][2], rest[kTiles][kTwoOperands ? NT : 1][2];
-  #pragma unroll
+#pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-  #pragma unroll
+#pragma unroll
         for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float x = score[t][n][2 * h], y = score[t][n][2 * h + 1];
             const uint32_t rounded = round_pair<M>(x, y);
@@ -732,7 +744,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // Values of keys that no row sees become zeros; where several queries see different keys, a probability of zero is mask enough if
         // all the values are numbers.
         constexpr int kUnits = W * BITS / 128;           // 16-byte units of a value
-  #pragma unroll 1
+#pragma unroll 1
         for (int i = lane; i < S::kKeys * kUnits; i += 32) {
           const int inside = i / kUnits, key = key0 + inside;
           const uint32_t unit_at = v_at + S::at(inside, i % kUnits * 16);
@@ -740,7 +752,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(unit_at), "r"(0) : "memory");
           } else if (low != high) {
             const uint4 unit = load_shared_16(unit_at);
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < 4; ++c) {
               const uint32_t four = c == 0 ? unit.x : c == 1 ? unit.y : c == 2 ? unit.z : unit.w;
               if constexpr (BITS == 8) {
@@ -777,16 +789,16 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       if (!apart) {
         // O^T += V^T P^T
         uint32_t value[kTiles][4][S::kValueWords];
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-  #pragma unroll
+#pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (S::kValueWords == 2) {
               const uint2 two = load_shared_8(v_at + S::at(key_of(t, r), quad * 8));
               value[t][r][0] = two.x;
               value[t][r][1] = two.y;
             } else {
-  #pragma unroll
+#pragma unroll
               for (int w = 0; w < S::kValueWords; w += 4) {
                 const uint4 four = load_shared_16(v_at + S::at(key_of(t, r), ((w / 4) * 8 + quad) * 16));
                 value[t][r][w] = four.x;
@@ -797,18 +809,18 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
           }
         }
-  #pragma unroll
+#pragma unroll
         for (int w = 0; w < S::kValueWords; ++w) {
-  #pragma unroll
+#pragma unroll
           for (int half = 0; half < kHalves; ++half) {
             const int slice = kHalves * w + half;
             float d[NT][4];
-  #pragma unroll
+#pragma unroll
             for (int t = 0; t < kTiles; ++t) {
               uint32_t a[4];
               const uint32_t v[4] = {value[t][0][w], value[t][1][w], value[t][2][w], value[t][3][w]};
               operand(v, half, a);
-  #pragma unroll
+#pragma unroll
               for (int n = 0; n < NT; ++n) {
                 if constexpr (BITS == 16) {
                   multiply<M>(result[n][slice], a, weight[t][n][0], weight[t][n][1], false);
@@ -817,15 +829,15 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                   multiply<M>(d[n], a, weight[t][n][0], weight[t][n][1], kScales > 1 || t == 0);
                 }
                 if constexpr (kScales > 1) {
-  #pragma unroll
+#pragma unroll
                   for (int e = 0; e < 4; ++e) result[n][slice][e] = fmaf(d[n][e], v_scale[t], result[n][slice][e]);
                 }
               }
             }
             if constexpr (BITS == 8 && kScales == 1) {
-  #pragma unroll
+#pragma unroll
               for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 4; e += 2) {
                   const float2 sum2 = __ffma2_rn(make_float2(d[n][e], d[n][e + 1]), make_float2(v_scale[0], v_scale[0]), make_float2(result[n][slice][e], result[n][slice][e + 1]));
                   result[n][slice][e] = sum2.x;
@@ -839,43 +851,43 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // (Rare, and written to be small.) The probabilities go where the chunk's keys were, and each query has a pass of its own over the tiles,
         // with the values it does not see as zeros; each row keeps what its own query's pass gives.
         uint32_t* const kept = reinterpret_cast<uint32_t*>(parts_at + warp * kWarpRing + stage * kStageBytes);
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-  #pragma unroll
+#pragma unroll
           for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
               kept[((t * NT + n) * 4 + h) * 32 + lane] = weight[t][n][h];
               if constexpr (kTwoOperands) kept[((t * NT + n) * 4 + 2 + h) * 32 + lane] = rest[t][n][h];
             }
           }
         }
-  #pragma unroll 1
+#pragma unroll 1
         for (int at = low; at <= high; ++at) {
-  #pragma unroll 1
+#pragma unroll 1
           for (int t = 0; t < kTiles; ++t) {
             float scale = v_scale[0];
             if constexpr (kScales > 1) scale = __shfl_sync(0xffffffffu, v_scale_now, t);
-  #pragma unroll
+#pragma unroll
             for (int w = 0; w < S::kValueWords; ++w) {
               uint32_t v[4];
-  #pragma unroll
+#pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const int column = S::kValueWords == 2 ? quad * 8 + w * 4 : ((w / 4) * 8 + quad) * 16 + w % 4 * 4;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(v_at + S::at(key_of(t, r), column)));
                 if (!sees(at, key0 + key_of(t, r))) v[r] = 0;
               }
-  #pragma unroll
+#pragma unroll
               for (int half = 0; half < kHalves; ++half) {
                 uint32_t a[4];
                 operand(v, half, a);
-  #pragma unroll
+#pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   const uint32_t* b = kept + (t * NT + n) * 4 * 32 + lane;
                   float d[4];
                   multiply<M>(d, a, b[0], b[32], true);
                   if constexpr (kTwoOperands) multiply<M>(d, a, b[64], b[96], false);
-  #pragma unroll
+#pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     if (position[n][e & 1] == at) {
                       float& into = result[n][kHalves * w + half][e];
@@ -893,11 +905,11 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       if (step + kKeyedStages < mine) fill(step + kKeyedStages, stage);
     }
 
-  #pragma unroll
+#pragma unroll
     for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 2; ++e) {
-  #pragma unroll
+#pragma unroll
         for (int offset = 4; offset < 32; offset *= 2) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], offset);
       }
     }
@@ -905,7 +917,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     constexpr int kRuns = kSlices / 4;
     auto column_of = [&](int run) { return BITS == 8 ? quad * (W / 8) + 8 * run : run * 64 + quad * 8; };
     auto run_of = [&](int n, int e, int run, float (&value)[8]) {
-  #pragma unroll
+#pragma unroll
       for (int c = 0; c < 4; ++c) {
         value[2 * c] = result[n][4 * run + c][e];
         value[2 * c + 1] = result[n][4 * run + c][2 + e];
@@ -913,14 +925,14 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     };
     if constexpr (SHARED) {
       const long long slot0 = (2LL * share + (begins ? 1 : 0)) * kRows;
-  #pragma unroll
+#pragma unroll
       for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = n * 8 + 2 * corner + e;
           if (row0 + row >= rows) continue;
           if (!whole && quad == 0) *(JOINS > 1 ? &piece_stats[JOINS > 1 ? warp : 0][begins ? 1 : 0][JOINS > 1 ? row : 0] : p.part_stats + slot0 + row) = make_float2(top[n][e], sum[n][e]);
-  #pragma unroll
+#pragma unroll
           for (int run = 0; run < kRuns; ++run) {
             float value[8];
             run_of(n, e, run, value);
@@ -937,16 +949,16 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
       }
     } else {
-  #pragma unroll
+#pragma unroll
       for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = n * 8 + 2 * corner + e;
           if (quad == 0) {
             part_top[warp][row] = top[n][e];
             part_sum[warp][row] = sum[n][e];
           }
-  #pragma unroll
+#pragma unroll
           for (int run = 0; run < kRuns; ++run) {
             float value[8];
             run_of(n, e, run, value);
@@ -957,18 +969,18 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
       }
       __syncthreads();
-      for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
+      for (int item = threadIdx.x; item < kRows * (W / 8); item += 32 * WARPS) {
         const int row = item / (W / 8), column = item % (W / 8) * 8;
         if (row0 + row >= rows || column >= p.head_dim) continue;
         float most = part_top[0][row];
-  #pragma unroll
-        for (int w = 1; w < kKeyedWarps; ++w) most = fmaxf(most, part_top[w][row]);
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) most = fmaxf(most, part_top[w][row]);
         float total = 0.f, value[8] = {};
-  #pragma unroll
-        for (int w = 0; w < kKeyedWarps; ++w) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
           const float by = rescale(part_top[w][row], most);
           total += part_sum[w][row] * by;
-  #pragma unroll
+#pragma unroll
           for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
         }
         write_result<T>(p, batch, kv_head, row0 + row, column, length, total, value);
@@ -1133,20 +1145,20 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
 }
 
 // How many CTAs of a kernel run at once on `device`, asked once for each.
-template <auto kKernel>
+template <auto kKernel, int WARPS = kKeyedWarps>
 int resident(int32_t device, size_t smem) {
   static std::mutex mutex;
   static int known[64] = {};
-  if (device < 0 || device >= 64) return 2 * 148;
+  if (device < 0 || device >= 64) return 8 / WARPS * 148;
   std::lock_guard<std::mutex> lock(mutex);
   if (known[device] == 0) {
     int per_sm = 0;
     DeviceScope device_scope(device);
-    if (device_scope.status() != TQ_OK) return 2 * 148;      // (a plan without a GPU)
+    if (device_scope.status() != TQ_OK) return 8 / WARPS * 148;      // (a plan without a GPU)
     if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, kKeyedThreads, smem) != cudaSuccess || per_sm <= 0) {
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, 32 * WARPS, smem) != cudaSuccess || per_sm <= 0) {
       cudaGetLastError();
-      per_sm = 2;
+      per_sm = 8 / WARPS;
     }
     known[device] = per_sm * sm_count(device);
   }
@@ -1160,17 +1172,19 @@ long long most_chunks(const KeyedParams& p, long long tokens, long long keys, in
   return all < seen ? all : seen;
 }
 
-// A unit of few chunks is a CTA's; of more, chunks are dealt out, which costs the finding of places at the start and the join at the end: from 14
-// us on, whatever there is to do. A CTA a unit takes 6 and about 1 for each step of its warps, and where CTAs come in several waves about 5 more
-// for each. In us, CTA a unit and dealt out, 16-bit queries: 12 heads of 64 1000 tokens 9.3 / 14.5, 64 x 12 heads 25.1 / 29.0, 64 x 12 x 1500
-// 32.9 / 37.4, 8 x 8 key heads of 128 1000 tokens 12.4 / 16.5, 128 x 8 x 300 30.8 / 26.8, x 600 40.8 / 39.0.
-constexpr int kFewChunks = 2 * kKeyedWarps, kSomeChunks = 8 * kKeyedWarps;
+// Whether a unit is a CTA's, of 2, 4 or 8 warps, or the chunks of all units are dealt out, is decided by expected time (us, B200). Dealing out costs the finding of places at
+// the start and the join at the end, a CTA a unit the wait for the longest, and for the next wave. A step (a chunk a warp) takes kStep at least, and at
+// most what memory makes of the chunks under way.
+constexpr double kStepTime[2] = {0.9, 1.3};              // of 8 rows, of 16
+constexpr double kBytesPerMicrosecond[2] = {6.2e6, 4.4e6};
+constexpr double kWholeTime = 5.5, kWaveTime = 4.0, kDealtTime = 13.0;
+constexpr int kMostSteps = 20;                           // beyond, equal shares are worth more than what they cost
 
 // From as many parts a unit on, the warps of a CTA join theirs before they go to memory.
 constexpr int kManyParts = 8;
 
 struct KeyedPlan {
-  int nt, row_tiles, shares, joins;      // shares 0: a CTA a unit
+  int nt, row_tiles, shares, joins, warps;      // shares 0: a CTA of `warps` a unit
   size_t bytes;
 };
 
@@ -1185,10 +1199,28 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const long long own = most_chunks(p, tokens < p.q_tokens ? tokens : p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long chunks = most_chunks(p, p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
-  if (own > kFewChunks && chunks <= 2 * own && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
-    const int most = plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, 1, true>>(device, keyed_smem(false, W, 1))
-                                  : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, 1, true>>(device, keyed_smem(false, W, 2));
-    if (own <= kSomeChunks && units <= 2LL * most) return plan;
+  const int sixteen = plan.nt - 1;
+  auto most_of = [&](auto joins, auto warps) {
+    constexpr int kJoins = decltype(joins)::value, kWarps = decltype(warps)::value;
+    return plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, kJoins, true, kWarps>, kWarps>(device, keyed_smem(false, W, 1, kWarps))
+                        : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, kJoins, true, kWarps>, kWarps>(device, keyed_smem(false, W, 2, kWarps));
+  };
+  auto whole_time = [&](auto warps) {
+    constexpr int kWarps = decltype(warps)::value;
+    const double most = most_of(std::integral_constant<int, 0>{}, warps), waves = units <= most ? 1.0 : std::ceil(units / most);
+    const double memory = (units < most ? units : most) * kWarps * kStageBytes / kBytesPerMicrosecond[sixteen];
+    const double steps = static_cast<double>((own + kWarps - 1) / kWarps);
+    return kWholeTime + waves * steps * (memory > kStepTime[sixteen] ? memory : kStepTime[sixteen]) + (waves - 1) * kWaveTime;
+  };
+  const double times[3] = {whole_time(std::integral_constant<int, 2>{}), whole_time(std::integral_constant<int, 4>{}), whole_time(std::integral_constant<int, 8>{})};
+  int best = 0;
+  for (int i = 1; i < 3; ++i)
+    if (times[i] < times[best]) best = i;
+  plan.warps = 2 << best;
+  const double dealt = kDealtTime + static_cast<double>(chunks) * units * kStageBytes / kBytesPerMicrosecond[sixteen];
+  const bool whole = (own + plan.warps - 1) / plan.warps <= kMostSteps && times[best] <= dealt;
+  if (!whole && chunks <= 2 * own && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
+    const int most = most_of(std::integral_constant<int, 1>{}, std::integral_constant<int, kKeyedWarps>{});
     plan.shares = kKeyedWarps * static_cast<int>(chunks * units / kKeyedWarps < most ? (chunks * units + kKeyedWarps - 1) / kKeyedWarps : most);
     plan.joins = plan.shares >= kManyParts * units ? kKeyedWarps : 1;
     plan.bytes = plan.shares * (sizeof(int4) + 2ull * 8 * plan.nt * (W + 2) * sizeof(float));
@@ -1248,30 +1280,32 @@ tq_status keyed_maps(CUtensorMap* maps, KeyedParams& p) {
 }
 
 template <typename T, int BITS, int W, int NT>
-tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
+tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   CUtensorMap maps[2] = {};
   if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
-  auto start = [&](auto kernel, long long ctas) -> tq_status {
-    const size_t smem = keyed_smem(p.joins > 1, W, NT);
-    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(keyed_smem(true, W, NT))));
-    kernel<<<static_cast<unsigned>(ctas), kKeyedThreads, smem, stream>>>(maps[0], maps[1], p);
+  auto start = [&](auto kernel, int each, long long ctas) -> tq_status {
+    const size_t smem = keyed_smem(p.joins > 1, W, NT, each);
+    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    kernel<<<static_cast<unsigned>(ctas), 32 * each, smem, stream>>>(maps[0], maps[1], p);
     return check_launch("keyed_attention_kernel");
   };
-  auto start_boxes = [&](auto joins, long long ctas) {
-    constexpr int kJoins = decltype(joins)::value;
+  auto start_boxes = [&](auto joins, auto each, long long ctas) {
+    constexpr int kJoins = decltype(joins)::value, kWarps = decltype(each)::value;
     if constexpr (BITS == 8) {
-      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false>, ctas);
+      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false, kWarps>, kWarps, ctas);
     }
-    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true>, ctas);
+    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true, kWarps>, kWarps, ctas);
   };
+  constexpr std::integral_constant<int, 0> kWhole{};
+  constexpr std::integral_constant<int, kKeyedWarps> kFour{};
   if (p.shares == 0) {
     const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.row_tiles;
     TQ_REQUIRE(units < (1LL << 31), TQ_UNSUPPORTED, "too many heads and rows for one launch");
-    return start_boxes(std::integral_constant<int, 0>{}, units);
+    return warps == 2 ? start_boxes(kWhole, std::integral_constant<int, 2>{}, units) : warps == 4 ? start_boxes(kWhole, kFour, units)
+                                                                                              : start_boxes(kWhole, std::integral_constant<int, 8>{}, units);
   }
   const bool gathers = p.joins > 1;
-  if (tq_status s = gathers ? start_boxes(std::integral_constant<int, kKeyedWarps>{}, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, p.shares / kKeyedWarps))
-    return s;
+  if (tq_status s = gathers ? start_boxes(kFour, kFour, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, kFour, p.shares / kKeyedWarps)) return s;
   // The second kernel's start passes under the first one's end (it waits for all of it before it reads the parts).
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
@@ -1287,9 +1321,9 @@ tq_status launch_keyed(KeyedParams& p, cudaStream_t stream) {
 }
 
 template <typename T, int BITS>
-tq_status launch_keyed_width(KeyedParams& p, int nt, cudaStream_t stream) {
-  if (p.head_dim <= 64) return nt == 1 ? launch_keyed<T, BITS, 64, 1>(p, stream) : launch_keyed<T, BITS, 64, 2>(p, stream);
-  return nt == 1 ? launch_keyed<T, BITS, 128, 1>(p, stream) : launch_keyed<T, BITS, 128, 2>(p, stream);
+tq_status launch_keyed_width(KeyedParams& p, const KeyedPlan& plan, cudaStream_t stream) {
+  if (p.head_dim <= 64) return plan.nt == 1 ? launch_keyed<T, BITS, 64, 1>(p, plan.warps, stream) : launch_keyed<T, BITS, 64, 2>(p, plan.warps, stream);
+  return plan.nt == 1 ? launch_keyed<T, BITS, 128, 1>(p, plan.warps, stream) : launch_keyed<T, BITS, 128, 2>(p, plan.warps, stream);
 }
 
 }  // namespace
@@ -1308,8 +1342,8 @@ tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long 
   p.borders = static_cast<int4*>(workspace);
   p.part_stats = reinterpret_cast<float2*>(p.borders + plan.shares);
   p.parts = reinterpret_cast<float*>(p.part_stats + slots);
-  if (dtype == TQ_BF16) return paged ? launch_keyed_width<__nv_bfloat16, 8>(p, plan.nt, stream) : launch_keyed_width<__nv_bfloat16, 16>(p, plan.nt, stream);
-  return paged ? launch_keyed_width<__half, 8>(p, plan.nt, stream) : launch_keyed_width<__half, 16>(p, plan.nt, stream);
+  if (dtype == TQ_BF16) return paged ? launch_keyed_width<__nv_bfloat16, 8>(p, plan, stream) : launch_keyed_width<__nv_bfloat16, 16>(p, plan, stream);
+  return paged ? launch_keyed_width<__half, 8>(p, plan, stream) : launch_keyed_width<__half, 16>(p, plan, stream);
 }
 
 }  // namespace tq
