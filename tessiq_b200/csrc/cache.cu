@@ -111,6 +111,8 @@ template <typename T, int TEAM>
 __global__ void __launch_bounds__(kStoreThreads, 8) cache_store_kernel(const __grid_constant__ StoreParams p) {
   constexpr int kHeld = 8;                 // vectors of 8 elements a thread keeps: a page of 64 tokens of 128 for 128 threads
   __shared__ uint32_t warp_most[3][kStoreThreads / 32];
+  wait_for_earlier();
+  let_later_start();
   const int thread = threadIdx.x % TEAM;
   long long item = static_cast<long long>(blockIdx.x) * (kStoreThreads / TEAM) + threadIdx.x / TEAM;
   if (item >= static_cast<long long>(p.batch) * p.touched * p.runs) return;      // whole warps, and whole CTAs where a team is one
@@ -270,6 +272,8 @@ __device__ __forceinline__ void copy_piece(char* to, const char* from, int bytes
 
 // grid: (pieces of all tensors, pairs)
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+  wait_for_earlier();
+  let_later_start();
   int piece = static_cast<int>(blockIdx.x), t = 0;
   auto pieces_of = [&](const CopyTensor& tensor) { return (tensor.layers + tensor.piece_layers - 1) / tensor.piece_layers * tensor.layer_pieces; };
   while (t + 1 < p.count && piece >= pieces_of(p.tensors[t])) piece -= pieces_of(p.tensors[t++]);
@@ -312,7 +316,7 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
         p.targets[n] = static_cast<int>(targets[i + n]);
       }
       const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(p.pairs));
-      copy_pages_kernel<<<grid, kCopyThreads, 0, stream>>>(p);
+      TQ_CUDA(launch_overlapped(copy_pages_kernel, grid, kCopyThreads, 0, stream, p));
       if (tq_status s = check_launch("copy_pages_kernel")) return s;
     }
   }
@@ -481,8 +485,8 @@ extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const 
   const long long items = pairs * p.runs, ctas = warps ? (items + 3) / 4 : items;
   TQ_REQUIRE(ctas < (1LL << 31), TQ_UNSUPPORTED, "too many pages and heads for one launch");
   cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(ctas), tq::kStoreThreads, 0, cuda_stream>>>(p);
+  auto go = [&](auto kernel) -> tq_status {
+    TQ_CUDA(tq::launch_overlapped(kernel, dim3(static_cast<unsigned>(ctas)), tq::kStoreThreads, 0, cuda_stream, p));
     return tq::check_launch("cache_store_kernel");
   };
   if (dtype == TQ_BF16) return warps ? go(tq::cache_store_kernel<__nv_bfloat16, 32>) : go(tq::cache_store_kernel<__nv_bfloat16, tq::kStoreThreads>);

@@ -331,8 +331,10 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    if (blockIdx.x == 0 && warp == 0) p.status.begin();
   }
+  wait_for_earlier();
+  let_later_start();
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.status.begin();
   __syncwarp();
   // JOINS > 1: what a warp has of units that others have parts of too: of one that began before its share (0), of one that goes on behind it (1)
   struct Piece {
@@ -356,7 +358,6 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   Dealt dealt = {};
   if constexpr (SHARED) {
     dealt = deal<BITS, S::kKeys>(p, blockIdx.x * kKeyedWarps, place);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel may start: it waits for this one's end itself
     if (lane == 0) p.borders[share] = make_int4(0, 0, 0, 0);               // (the border behind this share; see below)
     if (share < dealt.shares) {
       at = dealt.start(share);
@@ -1050,7 +1051,8 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
   constexpr int kRows = 8 * NT;
   __shared__ float2 warp_stats[kKeyedWarps][8];
   __shared__ float4 warp_value[kKeyedWarps][8][2];
-  asm volatile("griddepcontrol.wait;" ::: "memory");      // by every CTA: whoever comes after this kernel comes after the one before it too
+  wait_for_earlier();
+  let_later_start();
   const int share = static_cast<int>(blockIdx.x) * JOINS + JOINS - 1;         // the border lies behind it
   const int4 border = p.borders[share];
   const int batch = border.x, unit = border.y, first = border.z, last = border.w;
@@ -1286,7 +1288,7 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   auto start = [&](auto kernel, int each, long long ctas) -> tq_status {
     const size_t smem = keyed_smem(p.joins > 1, W, NT, each);
     TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kernel<<<static_cast<unsigned>(ctas), 32 * each, smem, stream>>>(maps[0], maps[1], p);
+    TQ_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(ctas)), 32 * each, smem, stream, maps[0], maps[1], p));
     return check_launch("keyed_attention_kernel");
   };
   auto start_boxes = [&](auto joins, auto each, long long ctas) {
@@ -1306,17 +1308,9 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   }
   const bool gathers = p.joins > 1;
   if (tq_status s = gathers ? start_boxes(kFour, kFour, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, kFour, p.shares / kKeyedWarps)) return s;
-  // The second kernel's start passes under the first one's end (it waits for all of it before it reads the parts).
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
-  config.blockDim = dim3(kKeyedThreads);
-  config.stream = stream;
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = 1;
-  TQ_CUDA(gathers ? cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT, kKeyedWarps>, p) : cudaLaunchKernelEx(&config, keyed_join_kernel<T, W, NT, 1>, p));
+  const dim3 borders(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
+  TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps>, borders, kKeyedThreads, 0, stream, p)
+                  : launch_overlapped(keyed_join_kernel<T, W, NT, 1>, borders, kKeyedThreads, 0, stream, p));
   return check_launch("keyed_join_kernel");
 }
 

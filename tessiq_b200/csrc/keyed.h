@@ -55,6 +55,27 @@ tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long 
                           cudaStream_t stream);
 
 #ifdef __CUDACC__
+// Launches `kernel` so that its start (CTAs placed, barriers set up) passes under the end of the kernel before it in the stream. Each of its
+// threads calls wait_for_earlier() before it touches memory, and let_later_start() as soon as it likes. Every CTA waits, also one with nothing
+// to do: what comes after this kernel then comes after the one before it too. (One new token of 64 x 12 heads stored: 5.7 us without, 4.3 with;
+// four queries over a short cache 6.1 and 5.6; a kernel of the libraries before it ends first, as ever.)
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch_overlapped(void (*kernel)(Parameters...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const Arguments&... arguments) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, arguments...);
+}
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_later_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The first fault since the last poll is kept, with where it was.
 __device__ __forceinline__ void report(const WaitStatus& status, int code, int sequence, int what) {
   int* words = status.sticky();

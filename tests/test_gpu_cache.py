@@ -273,6 +273,14 @@ def test_chunks_dealt_out_over_the_gpu(tq, case):
     assert status() == 0
 
 
+@pytest.mark.parametrize("case", [(batch, heads, kv_heads, queries, width, 64, window, 3, 11 * 8192 // width // 2) for batch in (1, 20, 58)
+                                  for heads, kv_heads, queries, width, window in [(12, 12, 1, 64, None), (24, 12, 6, 128, 300)]],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_a_unit_of_two_four_and_eight_warps(tq, case):
+    """Eleven steps a key head, of 12, 240 and 696 of them: few units take eight warps each, more of them four, many two."""
+    test_chunks_dealt_out_over_the_gpu(tq, case)
+
+
 @pytest.mark.parametrize("spread", [2.0**-60, 2.0**-20, 2.0**20, 2.0**60])
 def test_queries_of_any_size(tq, spread):
     """bf16 queries far outside the range of f16, with scores that stay moderate."""
@@ -537,6 +545,65 @@ def test_a_step_replayed_from_a_graph(tq, blocks, long):
     torch.cuda.synchronize()
     for cache, got in zip(caches, results):
         held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [long + 20, 25], None, 0, 0.125))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("captured", [False, True], ids=["eager", "captured"])
+@pytest.mark.parametrize("blocks, long", [(40, 600), (300, 4500)], ids=["whole units", "shares"])
+def test_kernels_that_start_early_wait_for_what_they_read(tq, blocks, long, captured):
+    """Copies, fills, another stream's work, stores, page copies and attention in turn, each reading what the one before wrote: as with a wait after each."""
+    cache = Cache(2, 2, 64, 16, blocks, seed=3).fill([long, 5])
+    before = [t.view(torch.uint8).clone() for t in cache.tensors]
+    spare = [min(set(range(2 * blocks + 2)) - set(cache.table.flatten().tolist()))]
+    last = [int(cache.table[0, (long + 1) // 16])]
+    host = torch.randn(2, 1, 2, 64, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).pin_memory()
+    starts, lengths = (torch.tensor([long + more, 5 + more], dtype=torch.int32).cuda() for more in (0, 1))
+    k, q = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+
+    def chain(wait):
+        main, results = torch.cuda.current_stream(), []
+        for step in range(6):
+            k.copy_(host, non_blocking=True)
+            wait()
+            tq.cache_store(k.transpose(1, 2), k.transpose(1, 2), *cache.tensors, cache.table, starts)
+            wait()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                q.fill_(step / 4 - 1)
+                q[:, 1].zero_()
+            main.wait_stream(side)
+            wait()
+            results.append(tq.cache_attention(q, *cache.tensors, cache.table, lengths))
+            wait()
+            tq.copy_pages(cache.tensors, last, spare)
+            wait()
+            cache.codes[1].view(torch.uint8)[last[0]].zero_()
+            wait()
+            results.append(tq.cache_attention(q, *cache.tensors, cache.table, lengths))
+            wait()
+            tq.copy_pages(cache.tensors, spare, last)
+            wait()
+            results.append(tq.cache_attention(q, *cache.tensors, cache.table, lengths))
+            results.append(tq.window_attention(q, q, results[-1]))
+            k.zero_()
+            wait()
+        return results
+
+    expected = [t.clone() for t in chain(torch.cuda.synchronize)]
+    for tensor, was in zip(cache.tensors, before):
+        tensor.view(torch.uint8).copy_(was)
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            results = chain(lambda: None)
+        for _ in range(3):
+            graph.replay()
+    else:
+        results = chain(lambda: None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(results, expected)) and not torch.equal(expected[0], expected[1])
     assert status() == 0
 
 
