@@ -538,6 +538,19 @@ struct WindowAttnParams : AttnParams {
   int window, sinks;
   const void *q, *k, *v;
   long long q_strides[3], k_strides[3], v_strides[3];
+  bool out_vectors;                // every eight elements of the result lie on 16 bytes
+};
+
+// Heads above 64: a softmax warp's results on their way out, 32 rows of 32 elements. A thread has a row, and a store of 16 bytes to each of 32 rows
+// is as many halves of sectors; eight rows of 64 bytes are whole ones (4 x 37 heads of 128, 2048 tokens under a window of 257 91 us, without
+// 103; 2 x 32 x 2501 under 333 58.9 and 60.5). Heads of 64 have half the bytes a row and a third CTA's stores beside: 1 to 4 % slower with it.
+template <int D, int KEYS>
+struct WindowLayout : AttnLayout<D, KEYS, false> {
+  using Base = AttnLayout<D, KEYS, false>;
+  static constexpr bool kStaged = D > kHeadDim;
+  static constexpr uint32_t kStageBytes = 32 * 32 * 2, kOffsetStages = Base::kOffsetBarriers + 256;
+  static constexpr size_t kSmemBytes = Base::kSmemBytes + (kStaged ? kRows / 32 * kStageBytes : 0);
+  static_assert(Base::kCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "as many CTAs an SM");
 };
 
 // The first n of 32 bits; none for n <= 0, all for n >= 32.
@@ -626,7 +639,7 @@ template <typename T, int D, int KEYS>
 __global__ void __launch_bounds__(kAttnThreads, AttnLayout<D, KEYS, false>::kCtasPerSm)
 window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const WindowAttnParams p) {
-  using L = AttnLayout<D, KEYS, false>;
+  using L = WindowLayout<D, KEYS>;
   constexpr int kKeys = KEYS, kRing = L::kRing, kSubTiles = L::kSubTiles;
   constexpr uint32_t kSubTileBytes = L::kSubTileBytes, kTileBytes = L::kTileBytes, kOffsetK = L::kOffsetK, kOffsetV = L::kOffsetV;
   constexpr uint32_t kOffsetBarriers = L::kOffsetBarriers, kColumnO = L::kColumnO;
@@ -645,6 +658,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const uint32_t tmem_slot = barriers + 8u * kBarrierCount;
   volatile uint32_t* tmem_slot_pointer = reinterpret_cast<volatile uint32_t*>(aligned + kOffsetBarriers + 8 * kBarrierCount);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* const stage = aligned + L::kOffsetStages + (warp & 3) * L::kStageBytes;      // kStaged: of a softmax warp's results
   const int items = p.q_blocks * p.batch * p.heads;
 
   auto load_queries = [&](const WindowBlock& b) {
@@ -664,7 +678,6 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-    if (blockIdx.x == 0) p.status.begin();
     barrier_init(q_full, 1);
     for (int s = 0; s < kRing; ++s) {
       barrier_init(k_full(s), 1);
@@ -679,6 +692,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     barrier_init(q_empty, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     const WindowBlock b = window_block<KEYS>(p, blockIdx.x);
+    wait_for_earlier();
+    if (blockIdx.x == 0) p.status.begin();
     load_queries(b);
     for (int j = 0; j < early; ++j) load_tile(&map_k, kOffsetK, k_full(j), b, j, j);
     for (int j = 0; j < early; ++j) load_tile(&map_v, kOffsetV, v_full(j), b, j, j);
@@ -691,6 +706,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       tmem_alloc(tmem_slot, L::kTmemColumns);
     }
   }
+  wait_for_earlier();
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
@@ -724,6 +740,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         }
         g += b.steps;
       }
+      let_later_start();
       if (!alive) {      // what is under way has to land before the CTA leaves
         auto landed = [&](uint32_t bar, uint32_t parity) {
           for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(bar, parity); ++spin) {
@@ -900,8 +917,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       // the result row leaves tensor memory 32 columns at a time (every lane takes part; rows beyond the queries only skip the stores)
       const bool stores = query < p.q_tokens, sees_some = position >= 0;      // a query before the first key: zeros
       const float inverse = sees_some ? 1.0f / row_sum : 0.f;
-      T* out_row = static_cast<T*>(p.out) + b.batch * p.out_batch + b.head * p.out_head + static_cast<long long>(query) * p.out_token;
-      const bool vector_ok = (reinterpret_cast<uintptr_t>(out_row) & 15) == 0;
+      T* const out = static_cast<T*>(p.out) + b.batch * p.out_batch + b.head * p.out_head;
+      T* const out_row = out + static_cast<long long>(query) * p.out_token;
       bool odd = false;                                  // something in the row is no finite number
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -915,7 +932,22 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           value[i] = sees_some ? __uint_as_float(o[i]) * inverse : 0.f;
           odd |= !(fabsf(value[i]) < INFINITY);
         }
-        if (stores && vector_ok) {
+        if (L::kStaged && p.out_vectors) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + (v ^ (lane >> 1 & 3)) * 16) =
+                make_uint4(pack_pair<T>(value[v * 8], value[v * 8 + 1]), pack_pair<T>(value[v * 8 + 2], value[v * 8 + 3]),
+                           pack_pair<T>(value[v * 8 + 4], value[v * 8 + 5]), pack_pair<T>(value[v * 8 + 6], value[v * 8 + 7]));
+          __syncwarp();
+          const int column = c * 32 + lane % 4 * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + lane / 4;
+            const uint4 part = *reinterpret_cast<const uint4*>(stage + row * 64 + ((lane ^ (row >> 1)) & 3) * 16);
+            const int at = b.q0 + warp * 32 + row;
+            if (at < p.q_tokens && column < p.head_dim) *reinterpret_cast<uint4*>(out + static_cast<long long>(at) * p.out_token + column) = part;
+          }
+        } else if (stores && p.out_vectors) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             if (c * 32 + v * 8 < p.head_dim) {
@@ -1084,6 +1116,8 @@ tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, int sm
   p.out_batch = from.out_strides[0];
   p.out_head = from.out_strides[1];
   p.out_token = from.out_strides[2];
+  p.out_vectors = from.head_dim % 8 == 0 && aligned_to(from.out, 16) &&
+                  (((p.batch > 1 ? p.out_batch : 0) | (p.heads > 1 ? p.out_head : 0) | (p.q_tokens > 1 ? p.out_token : 0)) & 7) == 0;
   p.status = from.status;
   p.group = from.group;
   p.offset = from.k_tokens - from.q_tokens;
@@ -1101,11 +1135,11 @@ tq_status window_tiles(tq_dtype dtype, const KeyedParams& from, int keys, int sm
   TQ_REQUIRE(blocks < (1LL << 30), TQ_UNSUPPORTED, "too many query blocks for one launch");
   auto go = [&](auto width, auto step) -> tq_status {
     constexpr int kWidth = decltype(width)::value, kKeys = decltype(step)::value;
-    constexpr size_t smem = AttnLayout<kWidth, kKeys, false>::kSmemBytes;
+    constexpr size_t smem = WindowLayout<kWidth, kKeys>::kSmemBytes;
     auto start = [&](auto kernel) -> tq_status {
       TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
       const long long fit = static_cast<long long>(sms) * AttnLayout<kWidth, kKeys, false>::kCtasPerSm;
-      kernel<<<static_cast<unsigned>(blocks < fit ? blocks : fit), kAttnThreads, smem, stream>>>(map_q, map_k, map_v, p);
+      TQ_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks < fit ? blocks : fit)), kAttnThreads, smem, stream, map_q, map_k, map_v, p));
       return check_launch("window_attention_kernel");
     };
     if (dtype == TQ_BF16) return start(window_attention_kernel<__nv_bfloat16, kWidth, kKeys>);
