@@ -106,16 +106,18 @@ __device__ __forceinline__ uint32_t encode_again(uint32_t codes, float ratio) {
   return encode(scaled(pair[0].x, ratio), scaled(pair[0].y, ratio), scaled(pair[1].x, ratio), scaled(pair[1].y, ratio));
 }
 
-// TEAM threads (a warp, or all) take some heads of the keys and values of one page, one after another.
-template <typename T, int TEAM>
-__global__ void __launch_bounds__(kStoreThreads, 8) cache_store_kernel(const __grid_constant__ StoreParams p) {
-  constexpr int kHeld = 8;                 // vectors of 8 elements a thread keeps: a page of 64 tokens of 128 for 128 threads
+// TEAM threads (half a warp, a warp, or all) take some heads of the keys and values of one page, one after another.
+template <typename T, int TEAM, int HELD>
+__global__ void __launch_bounds__(kStoreThreads, TEAM == kStoreThreads ? (HELD == 8 ? 8 : 12) : HELD == 8 ? 7 : 10)
+cache_store_kernel(const __grid_constant__ StoreParams p) {
+  constexpr int kHeld = HELD;              // vectors of 8 elements a thread keeps: 8 are a page of 64 tokens of 128 for 128 threads
   __shared__ uint32_t warp_most[3][kStoreThreads / 32];
   wait_for_earlier();
   let_later_start();
   const int thread = threadIdx.x % TEAM;
+  const uint32_t team = TEAM == 16 ? 0xffffu << (threadIdx.x & 16) : 0xffffffffu;      // of this warp
   long long item = static_cast<long long>(blockIdx.x) * (kStoreThreads / TEAM) + threadIdx.x / TEAM;
-  if (item >= static_cast<long long>(p.batch) * p.touched * p.runs) return;      // whole warps, and whole CTAs where a team is one
+  if (item >= static_cast<long long>(p.batch) * p.touched * p.runs) return;      // whole teams
   const int run = static_cast<int>(item % p.runs);
   item /= p.runs;
   const int nth = static_cast<int>(item % p.touched), sequence = static_cast<int>(item / p.touched);
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kStoreThreads, 8) cache_store_kernel(const __g
       });
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) take(kept[h]);
-      uint32_t most = __reduce_max_sync(0xffffffffu, max(pair & 0xffffu, pair >> 16));      // (magnitudes order like integers)
+      uint32_t most = __reduce_max_sync(team, max(pair & 0xffffu, pair >> 16));      // (magnitudes order like integers)
       if constexpr (TEAM > 32) {           // (places in turn: the next maxima do not overtake these)
         if (threadIdx.x % 32 == 0) warp_most[turn][threadIdx.x / 32] = most;
         __syncthreads();
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kStoreThreads, 8) cache_store_kernel(const __g
         earlier[i] = make_uint2(encode_again(word.x, ratio), encode_again(word.y, ratio));
       }
     }
-    __syncwarp();
+    __syncwarp(team);
     if (thread == 0) *scale_at = scale;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
@@ -474,23 +476,33 @@ extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const 
   p.tokens = static_cast<int>(tokens);
   p.head_dim = static_cast<int>(head_dim);
   p.touched = static_cast<int>((tokens + page_tokens - 2) / page_tokens + 1);
-  // A warp where it keeps a page's new tokens in registers, else a CTA; and each several heads where there would be more than four times as many
-  // teams as run at once (128 warps, 32 CTAs an SM). us, with as many as run at once, four times as many and one for every head: 32 x 8 heads of
-  // 2047 tokens of 128, pages of 64 68.4, 65.8, 65.7, pages of 16 77.7, 71.5, 71.6; 32 x 12 of 64, pages of 16 82.4, 74.8, 85.9.
-  const bool warps = (tokens < page_tokens ? tokens : page_tokens) * head_dim <= 8 * 32 * 8;
-  const long long pairs = static_cast<long long>(p.batch) * p.touched, teams_at_once = static_cast<long long>(tq::sm_count(device)) * (warps ? 128 : 32);
+  // Half a warp where it keeps a page's new tokens in registers (eight vectors a thread), else a warp, else a CTA: a team waits for its loads a head
+  // at a time, and more and smaller teams have more of them under way (32 x 12 heads of 64, 2047 tokens in pages of 16 with a warp 73.2 us, with
+  // half a one 52.6; one token of 128 x 8 heads of 128 4.2 and 3.8). Registers for eight vectors where four or one do cost CTAs an SM and empty
+  // instructions (the same in pages of 64, a CTA each: 64.4 and 54.4). A team takes several heads where there would be more than four times as
+  // many teams as run at once; with as many as run at once, four times as many and one for every head: 32 x 8 heads of 2047 tokens of 128, pages
+  // of 64 68.4, 65.8, 65.7, pages of 16 (then a warp each) 77.7, 71.5, 71.6; 32 x 12 of 64, pages of 16 82.4, 74.8, 85.9.
+  const long long vectors = (tokens < page_tokens ? tokens : page_tokens) * head_dim / 8;
+  const int team = vectors <= 8 * 16 ? 16 : vectors <= 8 * 32 ? 32 : tq::kStoreThreads;
+  const long long pairs = static_cast<long long>(p.batch) * p.touched;
+  const long long teams_at_once = static_cast<long long>(tq::sm_count(device)) * (32 * tq::kStoreThreads / team);
   const long long runs = teams_at_once / pairs < 1 ? 1 : teams_at_once / pairs < 2 * kv_heads ? teams_at_once / pairs : 2 * kv_heads;
   p.each = static_cast<int>((2 * kv_heads + runs - 1) / runs);
   p.runs = (2 * p.kv_heads + p.each - 1) / p.each;
-  const long long items = pairs * p.runs, ctas = warps ? (items + 3) / 4 : items;
+  const long long items = pairs * p.runs, ctas = (items * team + tq::kStoreThreads - 1) / tq::kStoreThreads;
   TQ_REQUIRE(ctas < (1LL << 31), TQ_UNSUPPORTED, "too many pages and heads for one launch");
   cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel) -> tq_status {
     TQ_CUDA(tq::launch_overlapped(kernel, dim3(static_cast<unsigned>(ctas)), tq::kStoreThreads, 0, cuda_stream, p));
     return tq::check_launch("cache_store_kernel");
   };
-  if (dtype == TQ_BF16) return warps ? go(tq::cache_store_kernel<__nv_bfloat16, 32>) : go(tq::cache_store_kernel<__nv_bfloat16, tq::kStoreThreads>);
-  return warps ? go(tq::cache_store_kernel<__half, 32>) : go(tq::cache_store_kernel<__half, tq::kStoreThreads>);
+  auto with_held = [&](auto type) -> tq_status {
+    using T = decltype(type);
+    if (team == 16) return vectors <= 16 ? go(tq::cache_store_kernel<T, 16, 1>) : go(tq::cache_store_kernel<T, 16, 8>);
+    if (team == 32) return go(tq::cache_store_kernel<T, 32, 8>);
+    return vectors <= 512 ? go(tq::cache_store_kernel<T, tq::kStoreThreads, 4>) : go(tq::cache_store_kernel<T, tq::kStoreThreads, 8>);
+  };
+  return dtype == TQ_BF16 ? with_held(__nv_bfloat16{}) : with_held(__half{});
 }
 
 extern "C" tq_status tq_copy_pages_launch(const tq_paged_tensor* tensors, int32_t count, int64_t pages, const int64_t* sources, const int64_t* targets,

@@ -333,7 +333,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
   }
   wait_for_earlier();
-  let_later_start();
+  if constexpr (SHARED) let_later_start();      // (the joining kernel; see launch_overlapped)
   if (blockIdx.x == 0 && threadIdx.x == 0) p.status.begin();
   __syncwarp();
   // JOINS > 1: what a warp has of units that others have parts of too: of one that began before its share (0), of one that goes on behind it (1)
@@ -988,6 +988,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
   }
+  if constexpr (!SHARED) let_later_start();
   if constexpr (JOINS > 1) {
     // The pieces of a unit meet, in the order of the warps; what other CTAs have parts of too goes to memory, as the part of the first of its
     // warps.
@@ -1052,7 +1053,6 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
   __shared__ float2 warp_stats[kKeyedWarps][8];
   __shared__ float4 warp_value[kKeyedWarps][8][2];
   wait_for_earlier();
-  let_later_start();
   const int share = static_cast<int>(blockIdx.x) * JOINS + JOINS - 1;         // the border lies behind it
   const int4 border = p.borders[share];
   const int batch = border.x, unit = border.y, first = border.z, last = border.w;

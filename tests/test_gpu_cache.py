@@ -375,6 +375,8 @@ STORES = [  # kv_heads, tokens, width, page, starts, counts
     (1, 1, 64, 16, [0], None), (2, 1, 64, 16, [0, 1, 15, 16, 31, -1], None), (12, 1, 64, 64, [999, 0, 63], None), (3, 5, 16, 16, [14, 0, 16, 30], [5, 0, 3, 2]),
     (2, 100, 128, 64, [0, 1, 63, 64], [100, 99, 1, 64]), (1, 300, 128, 128, [0, 100], None), (2, 40, 80, 16, [7, -5, 0], [40, 40, 17]), (1, 1100, 96, 1024, [3], None),
     (8, 2, 128, 32, [31, 30], None), (1, 17, 128, 16, [15], None),
+    (5, 33, 64, 16, [0, 3, 16], [33, 20, 0]), (7, 3, 128, 64, [62, 5, 64], None), (3, 130, 64, 64, [0, 63, 10], [130, 1, 70]), (1, 90, 96, 32, [31, 0], None),
+    (2, 150, 112, 64, [1], None), (3, 1, 16, 16, [15, 16, 2, 0, 7], None), (1, 31, 112, 16, [9, 100], None), (3, 66, 48, 32, [5, 31], [66, 2]),
 ]
 
 
@@ -423,6 +425,23 @@ def test_what_is_not_finite_is_stored_as_nan_and_has_no_say_in_the_scale(tq):
     assert cache.scales[0][page, 0].item() == 2.0**-8
     codes = cache.codes[0][page, 0, :4].float()
     assert torch.equal(codes.isnan(), ~k[0, 0].isfinite()) and (codes[~codes.isnan()] == 256.0).all()
+
+
+@pytest.mark.parametrize("page, tokens, width", [(16, 1, 64), (16, 16, 64), (32, 30, 64), (64, 64, 64), (64, 64, 128), (128, 120, 128)])
+def test_what_is_not_finite_stays_with_its_head(tq, page, tokens, width):
+    """Every other head has a NaN or an infinity, its neighbours come out as without them."""
+    before, *caches = [Cache(2, 6, width, page, 3).fill([5, 0]) for _ in range(3)]
+    k, v = (by_token((2, 6, tokens, width), torch.bfloat16, s) for s in (5, 6))
+    starts = torch.tensor([5, 0], dtype=torch.int32).cuda()
+    tq.cache_store(k, v, *caches[0].tensors, caches[0].table, starts)
+    for n, x in enumerate((k, v)):
+        x[:, n::2, -1, 3], x[:, n::2, 0, -1] = math.nan, -math.inf
+    tq.cache_store(k, v, *caches[1].tensors, caches[1].table, starts)
+    for n in range(2):
+        clean, bad = (c.codes[n].view(torch.uint8) for c in caches)
+        assert torch.equal(clean[:, 1 - n :: 2], bad[:, 1 - n :: 2]) and same(caches[0].scales[n][:, 1 - n :: 2], caches[1].scales[n][:, 1 - n :: 2])
+        expected = stored(before.codes[n], before.scales[n], before.table, (k, v)[n], [5, 0], [tokens] * 2, page)
+        assert same(caches[1].scales[n].cpu().double(), expected[1]) and same(caches[1].codes[n].cpu().float().double(), expected[0])
 
 
 def test_token_by_token_is_the_prompt_at_once(tq):
