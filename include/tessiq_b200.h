@@ -565,6 +565,8 @@ tq_status tq_recipe_destroy(tq_recipe* recipe);
 tq_status tq_recipe_begin_recording(tq_recipe* recipe);
 tq_status tq_recipe_end_recording(tq_recipe* recipe);
 int64_t tq_recipe_steps(const tq_recipe* recipe);
+/* 1 while the calling thread records (so that a caller can give a recorded launch scratch that stays), else 0. */
+int32_t tq_is_recording(void);
 tq_status tq_recipe_run(const tq_recipe* recipe, int32_t device, void* stream);
 
 /* Reads and clears the device-side status word of `device`: 0 when every bounded wait inside

@@ -111,6 +111,7 @@ SIGNATURES = {
     "tq_recipe_begin_recording": (c_int32, [c_void_p]),
     "tq_recipe_end_recording": (c_int32, [c_void_p]),
     "tq_recipe_steps": (c_int64, [c_void_p]),
+    "tq_is_recording": (c_int32, []),
     "tq_recipe_run": (c_int32, [c_void_p, c_int32, c_void_p]),
     "tq_status_poll": (c_int32, [c_int32, c_void_p, POINTER(c_int32)]),
     "tq_status_detail": (c_int32, [c_int32, c_void_p, POINTER(c_int32), c_int32]),

@@ -1314,7 +1314,7 @@ extern "C" tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, c
              "window attention has a kernel for heads of 8, 16, ... %d elements, not %lld", 2 * tq::kHeadDim, (long long)head_dim);
   if (batch == 0 || heads == 0 || q_tokens == 0) return TQ_OK;
   TQ_REQUIRE(kv_heads > 0 && heads % kv_heads == 0, TQ_INVALID_ARGUMENT, "%lld heads do not share %lld key heads evenly", (long long)heads, (long long)kv_heads);
-  TQ_REQUIRE(std::isfinite(scale) && scale > 0.0, TQ_UNSUPPORTED, "the score scale must be positive and finite, not %g", scale);
+  TQ_REQUIRE(scale > 0.0 && scale <= tq::kKeyedMostScale, TQ_UNSUPPORTED, "the score scale must be positive and finite in f32, not %g", scale);
   TQ_REQUIRE(q != nullptr && out != nullptr && (k_tokens == 0 || (k != nullptr && v != nullptr)), TQ_INVALID_ARGUMENT, "null operand or result");
   TQ_REQUIRE(q_tokens < (1LL << 24) && k_tokens < (1LL << 30) && heads < 65536 && batch * heads < (1LL << 24) && heads / kv_heads * q_tokens < (1LL << 24),
              TQ_UNSUPPORTED, "extents beyond the kernel's index range");

@@ -384,7 +384,7 @@ extern "C" tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, co
              (long long)heads, (long long)q_tokens, (long long)window, (long long)sinks);
   if (batch == 0 || heads == 0 || q_tokens == 0) return TQ_OK;
   TQ_REQUIRE(kv_heads > 0 && heads % kv_heads == 0, TQ_INVALID_ARGUMENT, "%lld heads do not share %lld key heads evenly", (long long)heads, (long long)kv_heads);
-  TQ_REQUIRE(std::isfinite(scale) && scale > 0.0, TQ_UNSUPPORTED, "the score scale must be positive and finite, not %g", scale);
+  TQ_REQUIRE(scale > 0.0 && scale <= tq::kKeyedMostScale, TQ_UNSUPPORTED, "the score scale must be positive and finite in f32, not %g", scale);
   TQ_REQUIRE(q != nullptr && out != nullptr && lengths != nullptr, TQ_INVALID_ARGUMENT, "null operand or result");
   TQ_REQUIRE(blocks == 0 || table != nullptr, TQ_INVALID_ARGUMENT, "null table");
   TQ_REQUIRE(pages == 0 || (k_pages != nullptr && v_pages != nullptr && k_scales != nullptr && v_scales != nullptr), TQ_INVALID_ARGUMENT, "null cache");

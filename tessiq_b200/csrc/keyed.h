@@ -27,6 +27,8 @@ struct KeyedParams {
   WaitStatus status;
 };
 
+constexpr double kKeyedMostScale = 2e38;      // times log2(e) it still is an f32
+
 // What queries and results have to be: read 16 bytes at a time, written through any strides.
 inline bool keyed_query_fits(const void* q, const int64_t* q_strides, const void* out, const int64_t* out_strides, int64_t batch, int64_t heads,
                              int64_t q_tokens) {

@@ -54,6 +54,7 @@ struct Library {
   decltype(&tq_cache_attention_launch) cache_attention_launch = nullptr;
   decltype(&tq_cache_store_launch) cache_store_launch = nullptr;
   decltype(&tq_copy_pages_launch) copy_pages_launch = nullptr;
+  decltype(&tq_is_recording) is_recording = nullptr;
 } library;
 
 template <typename Function>
@@ -312,14 +313,15 @@ PyObject* run(PyObject* const* values, Py_ssize_t count, bool by_type) {
     scratch = t.mutable_data_ptr();
     scratch_bytes = static_cast<size_t>(t.numel());
   }
+  // scratch of the call's own, so that calls on other streams and captured graphs never share it; torch's allocator orders its reuse
+  const int64_t own = plan->family == kWindow ? plan->ints[21] : plan->family == kCacheAttention ? plan->ints[18] : 0;
+  if (own > 0 && library.is_recording()) Py_RETURN_NONE;      // (a recorded launch keeps the address: the long way has a block that stays)
   std::vector<at::Tensor> out;
   tq_status status;
   {
     pybind11::gil_scoped_release unlocked;
     const c10::Device device(c10::kCUDA, static_cast<c10::DeviceIndex>(call.device));
     out.reserve(plan->outputs.size());
-    // scratch of the call's own, so that calls on other streams and captured graphs never share it; torch's allocator orders its reuse
-    const int64_t own = plan->family == kWindow ? plan->ints[21] : plan->family == kCacheAttention ? plan->ints[18] : 0;
     at::Tensor own_scratch;
     if (own > 0) {
       own_scratch = at::detail::empty_cuda({own}, at::kByte, device, std::nullopt);
@@ -445,7 +447,7 @@ PyObject* setup(PyObject*, PyObject* args) {
         find_entry(handle, "tq_window_attention_launch", library.window_attention_launch) &&
         find_entry(handle, "tq_cache_attention_launch", library.cache_attention_launch) &&
         find_entry(handle, "tq_cache_store_launch", library.cache_store_launch) &&
-        find_entry(handle, "tq_copy_pages_launch", library.copy_pages_launch))) {
+        find_entry(handle, "tq_copy_pages_launch", library.copy_pages_launch) && find_entry(handle, "tq_is_recording", library.is_recording))) {
     PyErr_Format(PyExc_ImportError, "%s: %s", path, dlerror());
     return nullptr;
   }

@@ -398,6 +398,8 @@ tq_status tq_recipe_end_recording(tq_recipe* recipe) {
   return TQ_OK;
 }
 
+int32_t tq_is_recording(void) { return tq::g_recording != nullptr; }
+
 int64_t tq_recipe_steps(const tq_recipe* recipe) { return recipe ? static_cast<int64_t>(recipe->steps.size()) : 0; }
 
 tq_status tq_recipe_run(const tq_recipe* recipe, int32_t device, void* stream) {

@@ -46,7 +46,8 @@ _gemm_kernel, _attention_kernel = lru_cache(maxsize=64)(GemmKernel), lru_cache(m
 # plan for; the long way below it leaves one when a call was a single launch over the operands as they came.
 _launcher = load_launcher()
 _launcher.setup(torch.nn.Parameter, workspace, str(LIBRARY_PATH))
-_FUSED, _REDUCE, _PACK, _SOFTMAX, _LAYER_NORM, _TRANSPOSED, _BATCH_NORM, _GEMM, _ATTENTION, _WINDOW, _CACHE_ATTENTION, _CACHE_STORE = range(12)      # launcher.cpp: Family
+_FUSED, _REDUCE, _PACK, _SOFTMAX, _LAYER_NORM, _TRANSPOSED, _BATCH_NORM, _GEMM, _ATTENTION = range(9)      # launcher.cpp: Family
+_WINDOW, _CACHE_ATTENTION, _CACHE_STORE = range(9, 12)
 _call, _keep_plan = _launcher.call, _launcher.keep
 _CODES = {name: 1 + i for i, name in enumerate(("pack", "softmax", "layer_norm", "native_layer_norm", "batch_norm", "attention", "sum", "mean", "amax",
                                                 "amin", "argmax", "gemm none", "gemm gelu", "gemm gelu_erf", "gemm gelu_tanh", "window attention",
@@ -590,9 +591,12 @@ def _window(window, sinks) -> tuple[int, int]:
     return 0 if window is None else int(window), int(sinks)
 
 
-def _own_scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    """Scratch of one call: from torch's allocator, so that calls on different streams, and captured graphs, never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _own_scratch(nbytes: int, device: int) -> torch.Tensor | None:
+    """Scratch of one call: from torch's allocator, so that calls on different streams, and captured graphs, never share it. A recorded launch keeps
+    its address: it gets the block that stays."""
+    if lib.tq_is_recording():
+        return workspace(device, _stream(None, device), nbytes)
+    return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}") if nbytes else None
 
 
 def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True):
@@ -622,7 +626,7 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, token_major=True
     extents = (batch, heads, k.shape[1], q_tokens, k.shape[2], width)
     nbytes = ctypes.c_size_t()
     check(lib.tq_window_attention_workspace_bytes(*extents, window, sinks, device, ctypes.byref(nbytes)))
-    scratch = _own_scratch(nbytes.value, q.device)
+    scratch = _own_scratch(nbytes.value, device)
     strides = (_three_strides(q, "the queries"), _three_strides(k, "the keys"), _three_strides(v, "the values"), _three_strides(out, "the result"))
     check(lib.tq_window_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k), _pointer(v), _pointer(out), *extents, *strides, scale, window, sinks,
                                          _pointer(scratch), nbytes.value, device, _stream(None, device)))
@@ -680,7 +684,7 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, win
     out = _attention_result(q, token_major)
     nbytes = ctypes.c_size_t()
     check(lib.tq_cache_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page_tokens, blocks, window, sinks, device, ctypes.byref(nbytes)))
-    scratch = _own_scratch(nbytes.value, q.device)
+    scratch = _own_scratch(nbytes.value, device)
     strides = (_three_strides(q, "the queries"), _three_strides(out, "the result"))
     extents = (batch, heads, kv_heads, q_tokens, width, pages, page_tokens, blocks, table_stride)
     check(lib.tq_cache_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),

@@ -31,7 +31,7 @@ def window(lib, **changed):
 @pytest.mark.parametrize("changed, code", [
     ({"dtype": 0}, "TQ_UNSUPPORTED"), ({"width": 63}, "TQ_UNSUPPORTED"), ({"width": 136}, "TQ_UNSUPPORTED"), ({"heads": 3}, "TQ_INVALID_ARGUMENT"),
     ({"kv_heads": 0}, "TQ_INVALID_ARGUMENT"), ({"batch": -1}, "TQ_INVALID_ARGUMENT"), ({"window": -1}, "TQ_INVALID_ARGUMENT"), ({"sinks": -2}, "TQ_INVALID_ARGUMENT"),
-    ({"scale": 0.0}, "TQ_UNSUPPORTED"), ({"scale": float("nan")}, "TQ_UNSUPPORTED"), ({"q": None}, "TQ_INVALID_ARGUMENT"), ({"out": None}, "TQ_INVALID_ARGUMENT"),
+    ({"scale": 0.0}, "TQ_UNSUPPORTED"), ({"scale": float("nan")}, "TQ_UNSUPPORTED"), ({"scale": 3e38}, "TQ_UNSUPPORTED"), ({"q": None}, "TQ_INVALID_ARGUMENT"), ({"out": None}, "TQ_INVALID_ARGUMENT"),
     ({"v": None}, "TQ_INVALID_ARGUMENT"), ({"q": OFF}, "TQ_UNSUPPORTED"), ({"k": OFF}, "TQ_UNSUPPORTED"), ({"k_strides": THREE(6400, 3200, 60)}, "TQ_UNSUPPORTED"),
     ({"k_strides": THREE(6400, 0, 64)}, "TQ_UNSUPPORTED"), ({"q_strides": THREE(768, 196, 64)}, "TQ_UNSUPPORTED"), ({"out_strides": THREE(768, -192, 64)}, "TQ_INVALID_ARGUMENT"),
     ({"k_tokens": 1 << 31}, "TQ_UNSUPPORTED"), ({"q_tokens": 1 << 31}, "TQ_UNSUPPORTED"), ({"k_strides": None}, "TQ_INVALID_ARGUMENT"),
@@ -55,7 +55,7 @@ def attend(lib, **changed):
     ({"page": 2048}, "TQ_UNSUPPORTED"), ({"pages": -1}, "TQ_INVALID_ARGUMENT"), ({"heads": 5}, "TQ_INVALID_ARGUMENT"), ({"kv_heads": 0}, "TQ_INVALID_ARGUMENT"),
     ({"window": -4}, "TQ_INVALID_ARGUMENT"), ({"lengths": None}, "TQ_INVALID_ARGUMENT"), ({"table": None}, "TQ_INVALID_ARGUMENT"), ({"ks": None}, "TQ_INVALID_ARGUMENT"),
     ({"q": OFF}, "TQ_UNSUPPORTED"), ({"v": OFF}, "TQ_UNSUPPORTED"), ({"table": OFF}, "TQ_UNSUPPORTED"), ({"blocks": 1 << 27}, "TQ_UNSUPPORTED"),
-    ({"scale": -1.0}, "TQ_UNSUPPORTED"), ({"batch": 0}, "TQ_OK"), ({"q_tokens": 0}, "TQ_OK"),
+    ({"scale": -1.0}, "TQ_UNSUPPORTED"), ({"scale": float("inf")}, "TQ_UNSUPPORTED"), ({"scale": 1e39}, "TQ_UNSUPPORTED"), ({"batch": 0}, "TQ_OK"), ({"q_tokens": 0}, "TQ_OK"),
 ], ids=str)
 def test_cache_attention_refuses(lib, changed, code):
     assert attend(lib, **changed) == getattr(lib, code), lib.last_error()

@@ -626,6 +626,37 @@ def test_kernels_that_start_early_wait_for_what_they_read(tq, blocks, long, capt
     assert status() == 0
 
 
+@pytest.mark.parametrize("seen_before", [False, True])
+def test_a_recorded_step_keeps_its_scratch(tq, seen_before):
+    """A recipe replays launches with the addresses they were recorded with: scratch that went back to torch's allocator would be someone else's by then."""
+    from tessiq_b200 import _lib
+
+    cache = Cache(2, 2, 64, 16, 300).fill([4500, 5])
+    lengths = torch.tensor([4500, 5], dtype=torch.int32).cuda()
+    q, other = (by_token((2, 4, 1, 64), torch.bfloat16, s) for s in (1, 2))
+    dense_q, dense_k = by_token((1, 4, 2, 64), torch.bfloat16, 3), by_token((1, 2, 5000, 64), torch.bfloat16, 4)
+    expected, dense = tq.cache_attention(other, *cache.tensors, cache.table, lengths), tq.window_attention(dense_q, dense_k, dense_k)
+    if not seen_before:
+        q, dense_q = (t.clone() for t in (q.contiguous(), dense_q.contiguous()))      # (a signature of its own)
+    handle = ctypes.c_void_p()
+    _lib.check(_lib.lib.tq_recipe_create(ctypes.byref(handle)))
+    assert _lib.lib.tq_is_recording() == 0
+    _lib.check(_lib.lib.tq_recipe_begin_recording(handle))
+    assert _lib.lib.tq_is_recording() == 1
+    got, dense_got = tq.cache_attention(q, *cache.tensors, cache.table, lengths), tq.window_attention(dense_q, dense_k, dense_k)
+    _lib.check(_lib.lib.tq_recipe_end_recording(handle))
+    guards = [torch.full((1 << n,), 0x55, dtype=torch.uint8, device="cuda") for n in range(9, 23) for _ in range(4)]      # whatever was given back
+    q.copy_(other)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        _lib.check(_lib.lib.tq_recipe_run(handle, 0, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(got, expected) and torch.equal(dense_got, dense)
+    assert all((g == 0x55).all() for g in guards)
+    assert _lib.lib.tq_recipe_steps(handle) == 2
+    _lib.check(_lib.lib.tq_recipe_destroy(handle))
+
+
 def test_repeated_calls_give_the_same_bits_on_any_stream_and_from_threads(tq):
     import threading
 
