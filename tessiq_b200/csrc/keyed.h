@@ -21,7 +21,8 @@ struct KeyedParams {
   int window, sinks;
   int row_tiles, shares, joins;                                            // joins: shares whose parts of a unit are joined before they go to memory
   float* parts;                                                            // of units that a border between two shares cuts
-  int4* borders;                                                           // the border behind each share: {sequence, unit, first and last share with parts of it}, none where these are equal
+  int4* borders;                                                           // the border behind each share: {sequence, unit, first and last share
+                                                                           // with parts of it}, none where these are equal
   float2* part_stats;                                                      // ... their maximum and sum
   float scale_log2;
   WaitStatus status;
