@@ -5,12 +5,12 @@
 //   code = e4m3(x / s), to nearest even
 // e4m3 is a floating format, so a power of two costs it no precision, x / s is exact, and an earlier code brought to a larger scale only steps
 // down in exponent: exact again, except for what falls under its smallest normal. The tokens are read once, kept in registers between the maximum
-// and the encoding. Bound: HBM (2 bytes read and 1 written an element: 402 MB in 66 us, 6.1 TB/s); for one new token a sequence, the latency of
-// start, table entry, scale and token, one after another (5 us with the launch). Divisions by the vectors of a token in the addresses had it at
+// and the encoding. Bound: HBM (2 bytes read and 1 written an element: 402 MB in 64.5 us, 6.2 TB/s); for one new token a sequence, the host (4 us;
+// from a graph the latency of start, table entry, scale and token, one after another: 2.4). Divisions by the vectors of a token in the addresses had it at
 // 94 us and bound by instructions; the next head's tokens loaded ahead took the registers of half the CTAs and gained nothing.
 //
 // Copying. Source and target pages are given by the host, which is where a cache's pages are handed out; they travel to the kernel as its
-// argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 87 us, 6.3 TB/s). Small pages of several
+// argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 85 us, 6.5 TB/s). Small pages of several
 // layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 #include <cmath>
 #include <new>

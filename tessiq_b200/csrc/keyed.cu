@@ -19,14 +19,15 @@
 // Split: the chunks of all (sequence, key head, 8 or 16 rows), each unit counted a little longer than it is, are one range in equal shares, a
 // warp each; whole units are written at once, and what a border between shares cuts is left in scratch as (maximum, sum, unscaled result) and
 // joined by a second kernel whose start passes under the first one's end. With a CTA for each share, units of a chunk or two (short sequences of
-// a ragged batch) queued up behind one another's latency: 64 x 12 heads of 64 of 1 to 2000 keys 94 us, with a warp 24. Few units have a CTA's
-// warps join theirs before (one head of 128000 keys 121 -> 23 us), and units of few chunks a CTA each (plan_shape). Tried beside the second
-// kernel: the last CTA to arrive at a ticket joins (48 us for 33 + 6: fences, and code that nobody has run yet, at the very end).
+// a ragged batch) queued up behind one another's latency: 64 x 12 heads of 64 of 1 to 2000 keys 94 us, with a warp 24 (without the host). Few
+// units have a CTA's warps join theirs before (one head of 128000 keys 121 -> 23 us). Units of few chunks have a CTA of 2, 4 or 8 warps each
+// and no second kernel (plan_shape). Tried beside the second kernel: the last CTA to arrive at a ticket joins (48 us for 33 + 6: fences, and code that nobody
+// has run yet, at the very end).
 //
 // Measured (kernels and join; us, and of HBM's 6456 GB/s): 16 x 64/8 heads of 128, 20001 to 40000 keys in 8 bits 160 (0.95); 32 x 32/8 heads,
-// 2052 keys in 16 bits 52 (0.80); 64 x 12 heads of 64, 1 to 2000 keys 28 (0.54); four queries of 48 x 32/8, 1028 keys 39 (0.39). A fixed 13 us
-// (launch, lengths, first pages and keys, join) is what the short ones pay, and 16 rows twice the products; the special functions, tensor pipe
-// and issue slots are below 50 %.
+// 2052 keys in 16 bits 50 (0.84); 64 x 12 heads of 64, 1 to 2000 keys 27 (0.57), all 1000 21 (0.74); four queries of 48 x 32/8, 1028 keys 34
+// (0.45); 12 heads of 64, 1500 keys 7. A fixed 12 us (launch, lengths, first pages and keys, join) is what dealt-out short ones pay, 5 us what
+// units do, and 16 rows twice the products; the special functions, tensor pipe and issue slots are below 50 %.
 //
 // Precision: scores, maxima, sums and results in f32. e4m3 to f16 is exact, and so is the query in f16: a row is scaled by a power of two to
 // a maximum of 2^14, so only elements 2^-38 of it or less lose digits. Probabilities against f16 values (cache codes too) are rounded to
@@ -302,7 +303,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 }
 
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal
-// shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every fourth chunk each and meet in shared
+// shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every WARPS-th chunk each and meet in shared
 // memory. ONE: a chunk lies in one page (or in none: dense keys).
 template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps>
 __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
@@ -1174,9 +1175,11 @@ long long most_chunks(const KeyedParams& p, long long tokens, long long keys, in
   return all < seen ? all : seen;
 }
 
-// Whether a unit is a CTA's, of 2, 4 or 8 warps, or the chunks of all units are dealt out, is decided by expected time (us, B200). Dealing out costs the finding of places at
-// the start and the join at the end, a CTA a unit the wait for the longest, and for the next wave. A step (a chunk a warp) takes kStep at least, and at
-// most what memory makes of the chunks under way.
+// Whether a unit is a CTA's, of 2, 4 or 8 warps, or the chunks of all units are dealt out, is decided by expected time (us, B200). Dealing out costs
+// the finding of places at the start and the join at the end, a CTA a unit the wait for the longest, and for the next wave. A step (a chunk a
+// warp) takes kStepTime at least, and at most what memory makes of the chunks under way. Always four warps or dealt out, and by this rule: 12 heads
+// of 64, 1500 keys 14.5, 8.5; 64 x 12 heads, 1000 keys 29.0, 22.9; 48 x 32/8 heads of 128, 300 keys 16.5, 12.4, 1000 keys 28.8, 25.1, 1500 keys
+// 36.8, 36.8; four queries of the same under a window of 1024 39.4, 36.0. (Since launches overlap, each is 1 to 2 us less.)
 constexpr double kStepTime[2] = {0.9, 1.3};              // of 8 rows, of 16
 constexpr double kBytesPerMicrosecond[2] = {6.2e6, 4.4e6};
 constexpr double kWholeTime = 5.5, kWaveTime = 4.0, kDealtTime = 13.0;
