@@ -124,6 +124,30 @@ def test_every_form_of_window_attention(tq, case, keys):
     assert status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case, keys", FORMS[:1] + FORMS[2:], ids=str)
+def test_a_result_at_any_alignment(tq, case, keys, dtype):
+    """Through the C interface a result may begin at any element and have any strides; what lies between its rows stays."""
+    from tessiq_b200 import _lib
+
+    batch, heads, kv_heads, queries, k_tokens, width, window, sinks = case
+    q, k, v = by_token((batch, heads, queries, width), dtype, 1), by_token((batch, kv_heads, k_tokens, width), dtype, 2), by_token((batch, kv_heads, k_tokens, width), dtype, 3)
+    expected = tq.window_attention(q, k, v, window or None, sinks)
+    buffer = torch.full((1 + batch * heads * queries * (width + 3),), 7.0, dtype=dtype, device="cuda")
+    out = buffer[1:].view(batch, heads, queries, width + 3)
+    three = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v, out)]
+    scratch = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    need = ctypes.c_size_t()
+    _lib.check(_lib.lib.tq_window_attention_workspace_bytes(batch, heads, kv_heads, queries, k_tokens, width, window, sinks, 0, ctypes.byref(need)))
+    assert need.value <= scratch.numel()
+    _lib.check(_lib.lib.tq_window_attention_launch(_lib.BF16 if dtype == torch.bfloat16 else _lib.F16, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), batch, heads,
+                                                   kv_heads, queries, k_tokens, width, *three, 1 / math.sqrt(width), window, sinks, scratch.data_ptr(), need.value, 0,
+                                                   torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[..., :width], expected)
+    assert (out[..., width:] == 7).all() and buffer[0] == 7
+    assert status() == 0
+
+
 def test_without_a_window_it_is_causal_attention(tq):
     q, k, v = (drawn((2, 4, 200, 64), torch.bfloat16, s) for s in (1, 2, 3))
     expected = reference(q, k, v, [200, 200], None, 0, 0.2)
