@@ -481,6 +481,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
               tma_load_rows(to + kStageBytes / 2, &map_v, bar, 0, row);
             }
           }
+          __syncwarp();                                  // every lane reads staged_page for the chunk's scales
         } else {
           const int page = __shfl_sync(0xffffffffu, page_now, (n % ahead) * boxes + lane % boxes);
           const bool loads = lane < boxes && page >= 0;

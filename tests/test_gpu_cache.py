@@ -326,6 +326,34 @@ def test_scales_far_apart_between_pages(tq):
         held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [96], window, 0, 0.125))
 
 
+@pytest.mark.parametrize("case", [  # batch, kv_heads, queries, width, page (a chunk of keys or more), tokens: a unit a CTA, then shares
+    (2, 3, 1, 64, 64, 1500), (2, 3, 1, 128, 32, 900), (1, 2, 3, 128, 128, 1100), (1, 1, 1, 64, 64, 40000), (24, 8, 1, 128, 32, 6000), (6, 2, 4, 64, 256, 9000)],
+    ids=lambda c: "-".join(map(str, c)))
+def test_every_chunk_takes_the_scales_of_its_own_page(tq, case):
+    """Neighbouring pages' scales are 2^3 (keys) and 2^9 (values) apart or more: another page's scale would show at once."""
+    batch, kv_heads, queries, width, page, tokens = case
+    blocks = -(-tokens // page)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    pages = batch * blocks
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32).reshape(batch, blocks)
+    nth = torch.empty(pages, device="cuda")
+    nth[table.flatten().long()] = (torch.arange(blocks, device="cuda") % 4).float().repeat(batch)
+    # keys of one size whatever their page's scale, so that every page has weight; values of one code, so that a page's size is its scale
+    signs = torch.randint(0, 2, (pages, kv_heads, page, width), dtype=torch.int8, device="cuda", generator=g).float() * 2 - 1
+    codes = [(signs * torch.exp2(3 * nth - 3)[:, None, None, None]).to(E4M3), torch.full_like(signs, 7.0).to(E4M3)]
+    scales = [torch.exp2(power * nth)[:, None].expand(pages, kv_heads).contiguous() for power in (-3, -9)]
+    q = by_token((batch, 2 * kv_heads, queries, width), torch.bfloat16, 1)
+    lengths = torch.full((batch,), tokens, dtype=torch.int32, device="cuda")
+    first = tq.cache_attention(q, *codes, *scales, table, lengths)
+    for _ in range(20):
+        assert torch.equal(tq.cache_attention(q, *codes, *scales, table, lengths), first)
+    for b in {0, batch - 1}:
+        at = table[b].long()
+        k, v = ((c.view(torch.uint8)[at].view(E4M3).float() * s[at][..., None, None]).permute(1, 0, 2, 3).flatten(1, 2)[None, :, :tokens] for c, s in zip(codes, scales))
+        held(first[b : b + 1], reference(q[b : b + 1], k.double(), v.double(), [tokens], None, 0, width**-0.5))
+    assert status() == 0
+
+
 def test_pages_that_are_not_there_are_left_out_and_reported(tq):
     from tessiq_b200.kernel import DeviceWaitError, check_status
 
