@@ -346,7 +346,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   __shared__ float2 piece_stats[JOINS > 1 ? kKeyedWarps : 1][2][JOINS > 1 ? kRows : 1];
   unsigned char* const heads_at = parts_at + kKeyedWarps * kWarpRing;      // [warp][row][column] f32
   auto piece_at = [&](int of, int which) { return reinterpret_cast<float*>(which ? parts_at + of * kWarpRing : heads_at + of * (kRows * W * 4)); };
-  if (JOINS > 1 && lane < 2) pieces[JOINS > 1 ? warp : 0][lane].there = false;
+  if (JOINS > 1 && lane == 0) pieces[JOINS > 1 ? warp : 0][0].there = pieces[JOINS > 1 ? warp : 0][1].there = false;      // (by the lane that fills them in)
   uint32_t turn = 0;                                   // chunks this warp has waited for: the stage and the phase of the next
   const int quad = lane >> 2, corner = lane & 3;       // the instruction's row (or column) of eight, and the lane's place in it
   const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group

@@ -148,6 +148,19 @@ def test_a_result_at_any_alignment(tq, case, keys, dtype):
     assert status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", [(1, 2, 1, 1, 40000, 64, 0, 0), (1, 4, 2, 2, 9000, 128, 8000, 4), (2, 2, 1, 7, 20000, 80, 0, 0)], ids=lambda c: "-".join(map(str, c)))
+def test_dense_keys_of_few_heads_are_joined_by_warps_and_then_by_ctas(tq, case, dtype):
+    batch, heads, kv_heads, queries, keys, width, window, sinks = case
+    assert form(*case) == 0
+    q, k, v = by_token((batch, heads, queries, width), dtype, 1), by_token((batch, kv_heads, keys, width), dtype, 2), by_token((batch, kv_heads, keys, width), dtype, 3)
+    got = tq.window_attention(q, k, v, window or None, sinks)
+    held(got, reference(q, k, v, [keys] * batch, window or None, sinks, 1 / math.sqrt(width)))
+    for _ in range(20):
+        assert torch.equal(tq.window_attention(q, k, v, window or None, sinks), got)
+    assert status() == 0
+
+
 def test_without_a_window_it_is_causal_attention(tq):
     q, k, v = (drawn((2, 4, 200, 64), torch.bfloat16, s) for s in (1, 2, 3))
     expected = reference(q, k, v, [200, 200], None, 0, 0.2)
