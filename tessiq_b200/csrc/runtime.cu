@@ -43,7 +43,10 @@ tq_status use_device(int32_t device) {
   if (status != cudaSuccess) {
     return fail(TQ_EXTERNAL, "no usable CUDA device: %s", cudaGetErrorString(status));
   }
-  if (current != device) TQ_CUDA(cudaSetDevice(device));
+  // A thread that has made no CUDA call yet is told device 0 and has no context, which the driver's own calls (a tensor map's encoding) want.
+  thread_local bool has_context = false;
+  if (current != device || !has_context) TQ_CUDA(cudaSetDevice(device));
+  has_context = true;
   return TQ_OK;
 }
 

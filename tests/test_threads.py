@@ -99,3 +99,21 @@ def test_threads_with_tiles_of_different_widths():
                 assert torch.equal(ops.softmax(columns[i], -1), rows[i])
 
     run_threads(work, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["window_attention", "few queries", "attention", "linear"])
+def test_the_first_call_of_a_thread(name):
+    """A host thread whose first CUDA call is one of the library's: launches that describe operands to TMA want a context by then. The second call of a
+    signature, so that nothing on the way there binds one."""
+    from tessiq_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k = (torch.randn(2, 4, tokens, 64, device="cuda", generator=g).bfloat16() for tokens in (200, 256))
+    weight = torch.randn(256, 256, device="cuda", generator=g).bfloat16()
+    calls = {"window_attention": lambda: ops.window_attention(q, k, k, 50, 4), "few queries": lambda: ops.window_attention(q[:, :, :2], k, k, 50, 4),
+             "attention": lambda: ops.attention(q, k, k), "linear": lambda: ops.mm(weight, weight)}
+    expected = calls[name]()
+    calls[name]()
+    torch.cuda.synchronize()
+    run_threads(lambda i: torch.testing.assert_close(calls[name](), expected, rtol=0, atol=0), 3)
