@@ -491,7 +491,8 @@ tq_status tq_attention_launch(tq_dtype dtype,
  * j > p - window or j < sinks. window 0: no window (every j <= p). A query before the first key (p < 0) sees nothing and
  * its result is zeros; what lies in keys that a query does not see, NaN included, does not reach its result. Types, head_dim,
  * strides and scale as for tq_attention_launch; heads is a multiple of kv_heads; k_tokens may be 0. `workspace` must hold
- * tq_window_attention_workspace_bytes bytes that no other launch in flight uses; null where that is 0. */
+ * tq_window_attention_workspace_bytes bytes that no other launch in flight uses, unless on the same stream (host threads may share it there); null where
+ * that is 0. */
 /* Which kernel the launch runs: keys streamed to few rows (TQ_ATTENTION_STREAMED), or tensor-core tiles (TQ_ATTENTION_TILES) with 64 or 128 keys a
  * step; device -1: on a B200, without a GPU. */
 tq_status tq_window_attention_form(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim, int64_t window,

@@ -1311,6 +1311,7 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
                                                                                               : start_boxes(kWhole, std::integral_constant<int, 8>{}, units);
   }
   const bool gathers = p.joins > 1;
+  const auto held = hold_scratch(p.borders);      // both launches, one after the other: recorded ones may share their scratch on a stream
   if (tq_status s = gathers ? start_boxes(kFour, kFour, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, kFour, p.shares / kKeyedWarps)) return s;
   const dim3 borders(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
   TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps>, borders, kKeyedThreads, 0, stream, p)

@@ -722,6 +722,48 @@ def test_a_recorded_step_keeps_its_scratch(tq, seen_before):
     _lib.check(_lib.lib.tq_recipe_destroy(handle))
 
 
+def test_recorded_steps_of_threads_on_one_stream(tq):
+    """Recordings of one stream share its scratch: what one thread's attention leaves there for its join must not be another's by then."""
+    import threading
+
+    from test_threads import run_threads
+
+    from tessiq_b200 import _lib
+
+    count, recipes = 4, []
+    caches = [Cache(1 + i, 2, 64, 16, 300, seed=i).fill([4500 - 700 * i, 60, 1, 900][: 1 + i]) for i in range(count)]
+    lengths = [torch.tensor([4500 - 700 * i, 60, 1, 900][: 1 + i], dtype=torch.int32).cuda() for i in range(count)]
+    queries = [by_token((1 + i, 4, 1 + i, 64), torch.bfloat16, i) for i in range(count)]
+    expected = [tq.cache_attention(q, *c.tensors, c.table, n) for q, c, n in zip(queries, caches, lengths)]
+    for q, c, n in zip(queries, caches, lengths):
+        handle = ctypes.c_void_p()
+        _lib.check(_lib.lib.tq_recipe_create(ctypes.byref(handle)))
+        _lib.check(_lib.lib.tq_recipe_begin_recording(handle))
+        recipes.append((handle, tq.cache_attention(q, *c.tensors, c.table, n)))
+        _lib.check(_lib.lib.tq_recipe_end_recording(handle))
+    stream = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    turn = threading.Barrier(count)
+
+    def work(i):
+        for _ in range(20):
+            turn.wait()
+            for _ in range(20):
+                _lib.check(_lib.lib.tq_recipe_run(recipes[i][0], 0, stream))
+            turn.wait()
+            if i == 0:
+                torch.cuda.synchronize()
+                for (_, got), right in zip(recipes, expected):
+                    assert torch.equal(got, right)
+                    got.zero_()
+                torch.cuda.synchronize()
+
+    run_threads(work, count)
+    for handle, _ in recipes:
+        _lib.check(_lib.lib.tq_recipe_destroy(handle))
+    assert status() == 0
+
+
 def test_repeated_calls_give_the_same_bits_on_any_stream_and_from_threads(tq):
     import threading
 
