@@ -508,8 +508,9 @@ tq_status tq_window_attention_launch(tq_dtype dtype, const void* q, const void* 
  * for the keys and as many for the values, and a packed [pages, kv_heads] f32 scale for each; an element is code times scale.
  * page_tokens is a power of two from 16 to 1024, head_dim a multiple of 16 up to 128. `table` is int32 [batch, blocks] with
  * `table_stride` elements between rows: the page that holds tokens page_tokens * n to page_tokens * (n + 1) - 1 of sequence b is
- * table[b][n]. Entries behind a sequence's end are not read. A page outside the pool, or a position behind the table's end, is left out
- * and reported through tq_status_poll (0x50414745 "PAGE", 0x4c454e47 "LENG").
+ * table[b][n]. Entries behind a sequence's end, and entries of pages that no query sees (behind the sinks and before the window of the first query), may
+ * be anything. A page outside the pool is left out, and a sequence longer than its table ends with it; both are reported through
+ * tq_status_poll (0x50414745 "PAGE", 0x4c454e47 "LENG").
  *
  * tq_cache_attention_launch: as tq_window_attention_launch over the first lengths[b] (int32, device memory) tokens of each sequence:
  * query i of q_tokens stands at position lengths[b] - q_tokens + i. bf16 or f16 q and out; k_tokens is lengths[b]; 0 is a

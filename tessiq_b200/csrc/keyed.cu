@@ -422,15 +422,16 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if constexpr (!SHARED) first_chunk = warp;
     const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
     auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
-    // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks.
+    // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks. Pages that no row sees are
+    // not looked at: a window may have left them behind, and the table may name anything there.
     const int boxes = ONE ? 1 : p.boxes, box_shift = ONE ? 31 : p.box_shift;
-    const int ahead = ONE ? 32 : 32 / boxes;
+    const int ahead = ONE ? 32 : 32 / boxes, box_keys = ONE ? S::kKeys : 1 << box_shift;
     auto look_up = [&](int n) {
       if constexpr (BITS == 8) {
         n += ONE ? lane : lane / boxes;
         if (n >= mine) return -1;
         const int key = chunk_at(n) * S::kKeys + (ONE ? 0 : (lane % boxes) << box_shift);
-        if (key >= length) return -1;
+        if (key > high || (key + box_keys - 1 <= low - p.window && key >= p.sinks)) return -1;
         const int at_block = key >> p.page_shift;
         const int page = p.table[batch * p.table_stride + at_block];
         if (page >= 0 && page < p.pages) return page;
@@ -600,20 +601,21 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         break;
       }
       const uint32_t k_at = ring + stage * kStageBytes, v_at = k_at + kStageBytes / 2;
-      int stop = length;                                 // keys from here on are not there
+      constexpr uint32_t kAllTiles = (1u << kTiles) - 1;
+      uint32_t there = kAllTiles;                        // bit t: the page of the chunk's 16 keys from 16 t on is there
       constexpr int kScales = BITS == 8 && !ONE ? kTiles : 1;
       float k_scale[kScales], v_scale[kScales], v_scale_now = 0.f;
       k_scale[0] = k_scale_next;
       v_scale[0] = v_scale_next;
       if constexpr (BITS == 8) {
         if constexpr (ONE) {
-          if (staged_page[warp][stage][0] < 0) stop = key0;
+          if (staged_page[warp][stage][0] < 0) there = 0;
         } else {
 #pragma unroll
           for (int t = kTiles - 1; t >= 0; --t) {
             k_scale[t] = __shfl_sync(0xffffffffu, k_scale_next, t);
             v_scale[t] = __shfl_sync(0xffffffffu, v_scale_next, t);
-            if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) stop = min(stop, key0 + t * 16);
+            if (staged_page[warp][stage][(t * 16) >> box_shift] < 0) there &= ~(1u << t);
           }
         }
         v_scale_now = v_scale_next;
@@ -655,8 +657,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
       // A chunk whose keys every row sees needs no mask.
       const int last = key0 + S::kKeys - 1;
-      const bool open = last <= low && last < stop && (key0 > high - p.window || last < p.sinks);
-      auto sees = [&](int at, int key) { return key <= at && key < stop && (key > at - p.window || key < p.sinks); };
+      const bool open = last <= low && there == kAllTiles && (key0 > high - p.window || last < p.sinks);
+      auto sees = [&](int at, int t, int key) { return key <= at && (there >> t & 1) && (key > at - p.window || key < p.sinks); };
       // Any reference point gives the same softmax: a row's moves only when a score lies more than 2^kSlack above it, which one vote tells.
       float most[NT][2];
       bool rises = false;
@@ -675,7 +677,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (!open) {
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                if (!sees(position[n][e], key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
+                if (!sees(position[n][e], t, key0 + t * 16 + quad + 8 * h)) score[t][n][2 * h + e] = -INFINITY;
             }
           }
 #pragma unroll
@@ -751,7 +753,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = lane; i < S::kKeys * kUnits; i += 32) {
           const int inside = i / kUnits, key = key0 + inside;
           const uint32_t unit_at = v_at + S::at(inside, i % kUnits * 16);
-          if (!(key <= high && key < stop && (key > low - p.window || key < p.sinks))) {
+          if (!(key <= high && (there >> (inside / 16) & 1) && (key > low - p.window || key < p.sinks))) {
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(unit_at), "r"(0) : "memory");
           } else if (low != high) {
             const uint4 unit = load_shared_16(unit_at);
@@ -878,7 +880,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
               for (int r = 0; r < 4; ++r) {
                 const int column = S::kValueWords == 2 ? quad * 8 + w * 4 : ((w / 4) * 8 + quad) * 16 + w % 4 * 4;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(v_at + S::at(key_of(t, r), column)));
-                if (!sees(at, key0 + key_of(t, r))) v[r] = 0;
+                if (!sees(at, t, key0 + key_of(t, r))) v[r] = 0;
               }
 #pragma unroll
               for (int half = 0; half < kHalves; ++half) {

@@ -399,6 +399,53 @@ def test_pages_that_are_not_there_are_left_out_and_reported(tq):
     assert status() == 0
 
 
+def kept_reference(q, k, v, kept, scale):
+    """`reference` where query i of every sequence sees the keys kept[i] and no others."""
+    parts = [reference(q[:, :, i : i + 1], k[:, :, kept[i]], v[:, :, kept[i]], [len(kept[i])] * q.shape[0], None, 0, scale) for i in range(q.shape[2])]
+    return torch.cat([r for r, _ in parts], 2), torch.cat([b for _, b in parts], 2)
+
+
+HOLES = [(page, width, queries, blocks, long) for page, width in ((16, 64), (32, 64), (16, 128), (64, 64)) for queries in (1, 3)
+         for blocks, long in ((800 // page, 700), (20000 // page, 19900))]      # a CTA a unit, and shares
+
+
+@pytest.mark.parametrize("case", HOLES, ids=lambda c: "-".join(map(str, c)))
+def test_a_page_that_is_not_there_takes_none_of_its_neighbours_along(tq, case):
+    from tessiq_b200.kernel import DeviceWaitError, check_status
+
+    page, width, queries, blocks, long = case
+    assert status() == 0
+    cache = Cache(1, 2, width, page, blocks).fill([long])
+    keys, values = cache.decoded(0).double(), cache.decoded(1).double()
+    table, gone = cache.table.clone(), [0, 5, 6, (long - queries) // page - 1]
+    table[0, gone] = torch.tensor([-1, 1 << 30, table.numel() + 2, -7], dtype=torch.int32, device="cuda")
+    q = by_token((1, 4, queries, width), torch.bfloat16, 1)
+    got = tq.cache_attention(q, *cache.tensors, table, torch.tensor([long], dtype=torch.int32).cuda())
+    with pytest.raises(DeviceWaitError, match="outside the pool"):
+        check_status()
+    kept = [[j for j in range(long - queries + i + 1) if j // page not in gone] for i in range(queries)]
+    held(got, kept_reference(q, keys, values, kept, width**-0.5))
+
+
+@pytest.mark.parametrize("case", HOLES, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("gone", ["no page", "a page whose scales are no numbers"])
+def test_pages_that_no_query_sees_are_not_looked_at(tq, case, gone):
+    """What a window has left behind, but for the sinks: the window begins inside a chunk of keys, and so do the pages behind the sinks end there."""
+    page, width, queries, blocks, long = case
+    sinks, window = 5, 300 if blocks * page < 1000 else 19000
+    while (long - queries - window + 1) % 64 < 33:      # from a chunk's last pages on
+        window -= 1
+    cache = Cache(1, 2, width, page, blocks).fill([long])
+    keys, values = cache.decoded(0).double(), cache.decoded(1).double()
+    unseen = list(range(-(-sinks // page), (long - queries - window + 1) // page))
+    assert len(unseen) >= 2
+    cache.table[0, unseen] = -1 if gone == "no page" else next(n for n in range(blocks + 2) if n not in cache.table[0].tolist())
+    q = by_token((1, 4, queries, width), torch.bfloat16, 1)
+    got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor([long], dtype=torch.int32).cuda(), window, sinks)
+    held(got, reference(q, keys, values, [long], window, sinks, width**-0.5))
+    assert status() == 0
+
+
 # ---- writing -------------------------------------------------------------------------------------
 
 
