@@ -35,8 +35,8 @@
 // rounded value and what rounding took off (2^-16).
 //
 // A masked key must not reach a result through 0 * NaN: its score is replaced, and a value that no row of the tile sees becomes zeros in the
-// stage. Where rows see different keys (several queries, at an end of the window) and a value they do see is no number, the chunk's product is
-// taken once a query with that query's keys alone, and each row keeps its own.
+// stage. Where rows see different keys (several queries, at an end of the window) and a value they do see is no number, or its page's scale, the
+// chunk's product is taken once a query with that query's keys alone, and each row keeps its own.
 #include <cuda.h>
 
 #include <cmath>
@@ -747,7 +747,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       bool apart = false;                                // the rows' products have to be taken one query at a time
       if (!open) {
         // Values of keys that no row sees become zeros; where several queries see different keys, a probability of zero is mask enough if
-        // all the values are numbers.
+        // all the values are numbers, and their scales.
+        if constexpr (BITS == 8) apart = low != high && (kScales == 1 || lane < kTiles) && !(fabsf(v_scale_now) < INFINITY);
         constexpr int kUnits = W * BITS / 128;           // 16-byte units of a value
 #pragma unroll 1
         for (int i = lane; i < S::kKeys * kUnits; i += 32) {
@@ -873,6 +874,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           for (int t = 0; t < kTiles; ++t) {
             float scale = v_scale[0];
             if constexpr (kScales > 1) scale = __shfl_sync(0xffffffffu, v_scale_now, t);
+            const int tile0 = key0 + t * 16;
+            if (tile0 > at || (tile0 + 15 <= at - p.window && tile0 >= p.sinks)) continue;      // nothing of the tile, its scale neither
 #pragma unroll
             for (int w = 0; w < S::kValueWords; ++w) {
               uint32_t v[4];

@@ -446,6 +446,31 @@ def test_pages_that_no_query_sees_are_not_looked_at(tq, case, gone):
     assert status() == 0
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", [(16, 64), (32, 64), (16, 128), (32, 128), (64, 64), (64, 128)], ids=lambda c: "-".join(map(str, c)))
+def test_a_scale_that_is_no_number_reaches_the_queries_that_see_its_page(tq, case, bad):
+    """Four queries whose window passes the end of a page, and the page that the last of them alone sees."""
+    page, width = case
+    lengths = [6 * page + 66, 12 * page + 1]
+    windows = [lengths[0] - 4 - (4 * page - 2) + 1, 7 * page]      # the first query sees the last two keys of page 3 of the first sequence, the third none
+    for b, window, block in ((0, windows[0], 3), (1, windows[1], 12)):
+        cache = Cache(2, 2, width, page, 13 + 66 // page).fill(lengths)
+        keys, values = cache.decoded(0).double(), cache.decoded(1).double()
+        where = int(cache.table[b, block])
+        cache.scales[1][where, 1] = bad
+        q = by_token((2, 4, 4, width), torch.float16, 1)
+        got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor(lengths, dtype=torch.int32).cuda(), window, 3)
+        exact, bound = reference(q, keys, values, lengths, window, 3, width**-0.5)
+        hit = torch.zeros(2, 4, 4, dtype=torch.bool)
+        for i in range(4):
+            at = lengths[b] - 4 + i
+            hit[b, 2:, i] = any(j > at - window and j <= at for j in range(block * page, (block + 1) * page))
+        assert hit.any() and not hit[b, 2:].all()
+        assert not got.cpu()[hit].isfinite().any()
+        held(torch.where(hit[..., None], 0, got.cpu()), (torch.where(hit[..., None], 0, exact), bound))
+        assert status() == 0
+
+
 # ---- writing -------------------------------------------------------------------------------------
 
 
