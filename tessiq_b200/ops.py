@@ -762,14 +762,21 @@ _library = None
 
 
 def _window_attention_by_aten(q, k, v, window, sinks, scale):
-    """`window_attention` in ATen, for what the kernels decline (f32, heads over 128 elements)."""
+    """`window_attention` in ATen, for what the kernels decline (f32, f64, heads over 128 elements): in f32, or in f64 for f64, rounded once."""
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     group, difference = q.shape[1] // max(k.shape[1], 1), k.shape[2] - q.shape[2]
-    k, v = (t.repeat_interleave(group, 1) for t in (k, v))
-    scores = (q @ k.transpose(-1, -2)) * (q.shape[-1] ** -0.5 if scale is None else scale)
+    k, v = (t.to(wide).repeat_interleave(group, 1) for t in (k, v))
+    scores = (q.to(wide) @ k.transpose(-1, -2)) * (q.shape[-1] ** -0.5 if scale is None else scale)
     at, key = torch.arange(q.shape[2], device=q.device)[:, None] + difference, torch.arange(k.shape[2], device=q.device)
     sees = (key <= at) & ((key > at - (k.shape[2] + 1 if window is None else window)) | (key < sinks))
-    weights = torch.softmax(scores.float().masked_fill(~sees, -math.inf), -1).masked_fill(~sees, 0.0)
-    return (weights.to(q.dtype) @ v).contiguous()
+    weights = torch.softmax(scores.masked_fill(~sees, -math.inf), -1).masked_fill(~sees, 0.0)
+    # A weight of zero does not keep out a value that is no finite number, so those come in apart: NaN where a query sees one (or an infinity of weight
+    # zero), an infinity where it sees that.
+    finite, up, down = (weights @ part for part in (v.masked_fill(~v.isfinite(), 0.0), (v == math.inf).to(wide), (v == -math.inf).to(wide)))
+    nan = torch.cat([sees.expand_as(weights), sees & (weights == 0)], -1).to(wide) @ torch.cat([v.isnan(), v.isinf()], -2).to(wide)
+    out = torch.where(up > 0, math.inf, torch.where(down > 0, -math.inf, finite))
+    out = out.masked_fill((nan > 0) | ((up > 0) & (down > 0)), math.nan)
+    return out.to(q.dtype).contiguous()
 
 
 def register_custom_ops() -> None:

@@ -274,3 +274,72 @@ def test_a_step_names_pages_starts_and_lengths():
     for bad in (dict(page_tokens=48), dict(width=24), dict(layers=0), dict(pages=0)):
         with pytest.raises(ValueError):
             PagedCache(**{**dict(layers=1, kv_heads=2, width=64, pages=4, device="cpu"), **bad})
+
+
+# ---- window attention in ATen, for what the kernels decline ----------------------------------------
+
+
+def by_rows(q, k, v, window, sinks, scale):
+    """The definition, a query and head at a time, in 64 bits, over the keys that it sees and nothing else."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(q.shape[0]):
+        for h in range(q.shape[1]):
+            for i in range(q.shape[2]):
+                at, head = k.shape[2] - q.shape[2] + i, h // (q.shape[1] // k.shape[1])
+                seen = [j for j in range(at + 1) if window is None or j > at - window or j < sinks]
+                if seen:
+                    weights = torch.softmax(k[b, head, seen].double() @ q[b, h, i].double() * scale, 0)
+                    out[b, h, i] = (weights[:, None] * v[b, head, seen].double()).sum(0)
+    return out
+
+
+def roundings(q, k, v, scale):
+    """How many half steps of the type that is computed in a result may be off, times the largest value: a score's width + 4 roundings of its products' sizes
+    count twice in a probability; the exponential, the sums over the keys and the quotient have the rest."""
+    q, k, v = (t.double().nan_to_num(0.0, 0.0, 0.0).abs() for t in (q, k, v))
+    if k.shape[2] == 0:
+        return 0.0
+    sizes = (q @ k.repeat_interleave(q.shape[1] // k.shape[1], 1).transpose(-1, -2)).max().item() * scale
+    return (2 * (q.shape[3] + 4) * sizes + 2 * k.shape[2] + 20) * v.max().item()
+
+
+@pytest.mark.parametrize("window, sinks", [(None, 0), (3, 0), (4, 2), (1, 1)], ids=str)
+@pytest.mark.parametrize("queries, keys", [(6, 6), (3, 11), (9, 4), (2, 0)], ids=str)
+def test_the_aten_form_in_64_bits(window, sinks, queries, keys):
+    from tessiq_b200.ops import _window_attention_by_aten
+
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(2, n, t, 7, generator=g, dtype=torch.float64) for n, t in ((4, queries), (2, keys), (2, keys)))
+    got = _window_attention_by_aten(q, k, v, window, sinks, None)
+    assert got.dtype == torch.float64 and got.is_contiguous()
+    torch.testing.assert_close(got, by_rows(q, k, v, window, sinks, 7**-0.5), rtol=0, atol=2.0**-53 * roundings(q, k, v, 7**-0.5))
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16], ids=str)
+def test_the_aten_form_lets_nobody_see_what_is_hidden(dtype):
+    """Key 7 is the last query's alone, key 2 lies between the sinks and the first query's window: NaN and infinities there, and in a value that two queries see."""
+    from tessiq_b200.ops import _window_attention_by_aten
+
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(1, 2, t, 4, generator=g).to(dtype) for t in (3, 8, 8))
+    k[0, 0, 2], v[0, 0, 2] = float("nan"), float("nan")
+    v[0, 0, 7, 1], v[0, 0, 7, 2], v[0, 0, 7, 3], v[0, 1, 6, 0] = float("nan"), float("inf"), float("-inf"), float("inf")
+    k[0, 1, 7] = float("inf")                    # scores of infinity, or NaN: the last query's row of head 1
+    got, exact = _window_attention_by_aten(q, k, v, 3, 2, 0.5).double(), by_rows(q, k, v, 3, 2, 0.5)
+    assert got[:, 0, :2].isfinite().all() and got[0, 1, 0].isfinite().all()
+    assert torch.equal(got.isnan(), exact.isnan()) and torch.equal(got.isinf(), exact.isinf())
+    assert torch.equal(got[got.isinf()], exact[exact.isinf()])
+    fine = exact.isfinite()
+    inside = torch.finfo(torch.float64 if dtype == torch.float64 else torch.float32).eps / 2
+    assert ((got - exact).abs()[fine] <= torch.finfo(dtype).eps / 2 * exact.abs()[fine] + inside * roundings(q, k, v, 0.5)).all()
+
+
+def test_the_aten_form_keeps_scores_in_32_bits():
+    """f16 operands whose scores pass 65504 before they are scaled, and lie a step of f16 apart after it."""
+    from tessiq_b200.ops import _window_attention_by_aten
+
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(1, 1, t, 256, generator=g).mul(size).half() for t, size in ((2, 60.0), (5, 60.0), (5, 1.0)))
+    scale = 2.0**-12
+    got, exact = _window_attention_by_aten(q, k, v, None, 0, scale).double(), by_rows(q, k, v, None, 0, scale)
+    assert ((got - exact).abs() <= 2.0**-11 * exact.abs() + 2.0**-24 * roundings(q, k, v, scale)).all()

@@ -95,3 +95,17 @@ def test_window_attention_and_the_cache_are_operations_too(tessiq):
     assert torch.equal(got, ops.cache_attention(q, *pages, *scales, table, lengths, 16, 2)) and got.isfinite().all()
     tessiq.copy_pages([*(p.view(torch.uint8) for p in pages), *scales], [0], [5], 0)
     assert torch.equal(scales[0][5], scales[0][0]) and torch.equal(pages[1].view(torch.uint8)[5], pages[1].view(torch.uint8)[0])
+
+
+def test_window_attention_that_has_no_kernel_is_in_f32_or_f64_and_keeps_hidden_keys_out(tessiq):
+    from test_cache import by_rows, roundings
+
+    g = torch.Generator().manual_seed(3)
+    for dtype, width in ((torch.float64, 64), (torch.float32, 64), (torch.bfloat16, 256)):
+        q, k, v = (torch.randn(1, n, t, width, generator=g).to(dtype) for n, t in ((4, 3), (2, 40), (2, 40)))
+        k[:, :, 10:20], v[:, :, 10:20] = float("nan"), float("inf")      # between the sinks and the first query's window
+        got = tessiq.window_attention(q.cuda(), k.cuda(), v.cuda(), 16, 4, None)
+        exact = by_rows(q, k, v, 16, 4, width**-0.5)
+        assert got.dtype == dtype and got.isfinite().all()
+        inside = torch.finfo(torch.float64 if dtype == torch.float64 else torch.float32).eps / 2
+        assert ((got.cpu().double() - exact).abs() <= torch.finfo(dtype).eps / 2 * exact.abs() + inside * roundings(q, k, v, width**-0.5)).all()
