@@ -21,7 +21,7 @@ Not for several host threads at once.
 from __future__ import annotations
 
 import heapq
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Sequence
 
 import torch
@@ -41,6 +41,8 @@ class Pages:
         self._free = list(range(pages))      # a heap: the lowest is handed out first
         self._sequences: dict[int, tuple[list[int], int]] = {}
         self._next = 0
+        self.changes = 0                     # of all sequences together
+        self._changes: dict[int, list[int]] = {}      # sequence -> [how often what was named as its own is not any more, ... was copied]
 
     @property
     def free_pages(self) -> int:
@@ -65,7 +67,19 @@ class Pages:
     def _add(self, pages: list[int], length: int) -> int:
         sequence, self._next = self._next, self._next + 1
         self._sequences[sequence] = (pages, length)
+        self._changes[sequence] = [0, 0]
         return sequence
+
+    def _changed(self, sequence: int, which: int) -> None:
+        self._changes[sequence][which] += 1
+        self.changes += 1
+
+    def changes_of(self, sequence: int) -> tuple[int, int]:
+        """How often pages or tokens that were the sequence's stopped being its own (truncated, moved, its last page exchanged for a copy), and how often a
+        copy was taken of a page it has."""
+        self._of(sequence)
+        moved, copied = self._changes[sequence]
+        return moved, copied
 
     def _take(self) -> int:
         page = heapq.heappop(self._free)
@@ -89,7 +103,8 @@ class Pages:
 
     def free(self, sequence: int) -> None:
         pages, _ = self._of(sequence)
-        del self._sequences[sequence]
+        del self._sequences[sequence], self._changes[sequence]
+        self.changes += 1
         for page in pages:
             self._drop(page)
 
@@ -102,6 +117,8 @@ class Pages:
         for page in pages[keep:]:
             self._drop(page)
         self._sequences[sequence] = (pages[:keep], length)
+        if length < now:
+            self._changed(sequence, 0)
 
     def extend(self, sequences: Sequence[int], counts: Sequence[int]) -> tuple[list[int], list[int]]:
         """Room for `counts` tokens more in each of `sequences`. Returns the pages to copy, (from, to): last pages that are shared and will be
@@ -127,6 +144,10 @@ class Pages:
         for sequence, count, copies in zip(sequences, counts, copied):
             pages, length = self._of(sequence)
             if copies:
+                block = len(pages) - 1           # (forks have a page they share at the same place)
+                for other, (theirs, _) in self._sequences.items():
+                    if len(theirs) > block and theirs[block] == pages[block]:
+                        self._changed(other, 0 if other == sequence else 1)
                 sources.append(pages[-1])
                 self._drop(pages[-1])
                 pages[-1] = self._take()
@@ -146,21 +167,27 @@ class Pages:
         for source, target in moved.items():
             self.references[target], self.references[source] = self.references[source], 0
         for sequence, (pages, length) in self._sequences.items():
-            self._sequences[sequence] = ([moved.get(page, page) for page in pages], length)
+            if any(page in moved for page in pages):
+                self._sequences[sequence] = ([moved.get(page, page) for page in pages], length)
+                self._changed(sequence, 0)
         self._free = list(range(used, len(self.references)))
         return list(moved), list(moved.values())
 
 
 @dataclass
 class Step:
-    """Where the new tokens of some sequences go, on the device: what `ops.cache_store` and `ops.cache_attention` take. Good until pages move (`compact`)
-    or one of its sequences is truncated or freed."""
+    """Where the new tokens of some sequences go, on the device: what `ops.cache_store` and `ops.cache_attention` take. Good until pages move (`compact`),
+    one of its sequences is truncated or freed, or its last page, shared with a fork, is exchanged for a copy as it is extended again; to store also until a
+    fork takes such a copy, which would miss what is stored then. `PagedCache` refuses a step beyond that. Steps of a sequence are stored in the
+    order they were made: tokens in a page behind those that are stored are not encoded again."""
 
     table: torch.Tensor      # int32 [batch, blocks]
     starts: torch.Tensor     # int32 [batch]
     counts: torch.Tensor
     lengths: torch.Tensor    # starts + counts
     tokens: int              # the largest count
+    changes: int = 0         # the books' counts as the step was made (Pages.changes, Pages.changes_of each sequence)
+    sequences: dict[int, tuple[int, int]] = field(default_factory=dict)
 
 
 class PagedCache:
@@ -217,16 +244,31 @@ class PagedCache:
             host = host.pin_memory()
         there = host.to(self.k_scales.device, non_blocking=True)
         table, starts, counts_there, lengths = there.split([batch * blocks, batch, batch, batch])
-        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0))
+        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), self.books.changes,
+                    {sequence: self.books.changes_of(sequence) for sequence in sequences})
+
+    def _good(self, step: Step, stores: bool) -> None:
+        if step.changes == self.books.changes:
+            return
+        for sequence, (moved, copied) in step.sequences.items():
+            if sequence not in self.books._sequences:
+                raise ValueError(f"sequence {sequence} of the step has been freed")
+            moved_now, copied_now = self.books.changes_of(sequence)
+            if moved != moved_now:
+                raise ValueError(f"the step is from before pages of sequence {sequence} were moved, truncated or exchanged for a copy")
+            if stores and copied != copied_now:
+                raise ValueError(f"a fork of sequence {sequence} has copied the page the step writes: what is stored now would be missing there")
 
     def store(self, step: Step, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes [batch, kv_heads, tokens, width] new keys and values of one layer; of a sequence that got fewer than `tokens`, the first ones."""
+        self._good(step, True)
         if k.dim() == 4 and k.shape[2] < step.tokens:
             raise ValueError(f"the step has room for {step.tokens} tokens and was given {k.shape[2]}: attention would read what nobody wrote")
         ops.cache_store(k, v, *self.layer(layer), step.table, step.starts, step.counts)
 
     def attention(self, step: Step, layer: int, q: torch.Tensor, window=None, sinks=0, scale=None, token_major=True) -> torch.Tensor:
         """q [batch, heads, q_tokens, width] are the last `q_tokens` tokens of each sequence (a query before its first token gives zeros)."""
+        self._good(step, False)
         return ops.cache_attention(q, *self.layer(layer), step.table, step.lengths, window, sinks, scale, token_major)
 
     def compact(self) -> int:

@@ -276,6 +276,65 @@ def test_a_step_names_pages_starts_and_lengths():
             PagedCache(**{**dict(layers=1, kv_heads=2, width=64, pages=4, device="cpu"), **bad})
 
 
+def test_a_step_that_has_ended_is_refused(monkeypatch):
+    """Each way in which pages or tokens that a step names stop being its sequences' own; steps of other sequences go on."""
+    from tessiq_b200 import cache as module
+
+    launched = []
+    monkeypatch.setattr(module.ops, "copy_pages", lambda *a, **k: launched.append("copy"))
+    monkeypatch.setattr(module.ops, "cache_store", lambda *a: launched.append("store"))
+    monkeypatch.setattr(module.ops, "cache_attention", lambda *a: launched.append("attend"))
+    k = torch.zeros(1, 1, 9, 16).half()
+
+    def made():
+        cache = module.PagedCache(1, 1, 16, pages=20, page_tokens=16, device="cpu")
+        a, other = cache.start(), cache.start()
+        return cache, a, cache.extend([a], 9), cache.extend([other], 2)
+
+    def ended(cache, step, other, stores=True, reads=True):
+        for refused, call in ((stores, lambda s: cache.store(s, 0, k, k)), (reads, lambda s: cache.attention(s, 0, k))):
+            launched.clear()
+            if refused:
+                with pytest.raises(ValueError, match="sequence"):
+                    call(step)
+                assert not launched
+            else:
+                call(step)
+            call(other)
+            assert len(launched) == 2 - refused
+
+    cache, a, step, other = made()
+    ended(cache, step, other, False, False)
+    b = cache.fork(a)                        # writing what both of them have is what both of them see
+    ended(cache, step, other, False, False)
+    cache.truncate(a, 9)                     # nothing forgotten
+    ended(cache, step, other, False, False)
+    cache.extend([b], 0)
+    ended(cache, step, other, False, False)
+    cache.extend([b], 1)                     # b has a copy from before what is stored now
+    ended(cache, step, other, True, False)
+    later = cache.extend([a], 1)             # (alone on its page again)
+    ended(cache, step, other, True, False)
+    ended(cache, later, other, False, False)
+    for end in ("truncate", "free", "exchange", "compact"):
+        cache, a, step, other = made()
+        if end == "truncate":
+            cache.truncate(a, 8)
+        elif end == "free":
+            cache.free(a)
+        elif end == "exchange":              # a moves to a copy, the page it wrote is its fork's
+            cache.fork(a)
+            later = cache.extend([a], 1)
+            ended(cache, later, other, False, False)
+        else:
+            low = cache.start()
+            third = cache.extend([low], 20)
+            cache.free(a)
+            a, step, other = low, third, other
+            assert cache.compact() == 1
+        ended(cache, step, other)
+
+
 # ---- window attention in ATen, for what the kernels decline ----------------------------------------
 
 
