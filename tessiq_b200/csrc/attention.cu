@@ -871,7 +871,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           reference = tile_max;
         }
         const bool rescale = j != 0 && __any_sync(0xffffffffu, moves);
-        const float shift = reference == -INFINITY ? 0.f : -reference * p.scale_log2;
+        // (f16: probabilities 2^7 times as large, up to 2^(8 + 7), so that those under 2^-21 of the largest and not of 2^-14 on lose digits)
+        constexpr float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;
+        const float shift = reference == -INFINITY ? 0.f : fmaf(-reference, p.scale_log2, kLift);
         float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
         uint32_t packed[kKeys / 2];
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);

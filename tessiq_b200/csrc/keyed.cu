@@ -31,8 +31,8 @@
 //
 // Precision: scores, maxima, sums and results in f32. e4m3 to f16 is exact, and so is the query in f16: a row is scaled by a power of two to
 // a maximum of 2^14, so only elements 2^-38 of it or less lose digits. Probabilities against f16 values (cache codes too) are rounded to
-// f16 (half a step is 2^-11, under the result's 2^-8 in bf16); against bf16 values they take two bf16 operands, the
-// rounded value and what rounding took off (2^-16).
+// f16 (half a step is 2^-11, under the result's 2^-8 in bf16; below 2^-21 of the largest it is 2^-32 of that, see kLift);
+// against bf16 values they take two bf16 operands, the rounded value and what rounding took off (2^-16).
 //
 // A masked key must not reach a result through 0 * NaN: its score is replaced, and a value that no row of the tile sees becomes zeros in the
 // stage. Where rows see different keys (several queries, at an end of the window) and a value they do see is no number, or its page's scale, the
@@ -60,6 +60,10 @@ constexpr uint32_t kStageBytes = 8192;
 constexpr uint32_t kWarpRing = kKeyedStages * kStageBytes;
 constexpr int kWaitKeyed = 0x4b455931;      // "KEY1"
 constexpr float kSlack = 8.f;
+// Probabilities that are rounded to f16 are taken 2^kLift times as large, which cancels in the quotient: 2^(kSlack + kLift) is the largest then, inside
+// f16's 2^16, and those that fall under its normal range, 2^-14, are under 2^-21 of the row's largest.
+template <typename M>
+constexpr float kLift = std::is_same_v<M, __half> ? 7.f : 0.f;
 
 // BITS of a key element, W: the head's elements, rounded up to 64 or 128.
 template <int BITS, int W>
@@ -709,7 +713,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : -top[n][0], top[n][1] == -INFINITY ? 0.f : -top[n][1]);
+        const float2 shift = make_float2(top[n][0] == -INFINITY ? 0.f : kLift<M> - top[n][0], top[n][1] == -INFINITY ? 0.f : kLift<M> - top[n][1]);
         float2 gained = make_float2(sum[n][0], sum[n][1]);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {

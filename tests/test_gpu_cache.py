@@ -329,6 +329,46 @@ def test_queries_of_any_size(tq, spread):
     held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [50], None, 0, scale))
 
 
+def behind_a_strong_key(q, k, v, keys, scale):
+    """`reference` without what f16 loses below its normal range: weights are kept 2^7 times as large, so half a step there is 2^-32 of the largest."""
+    exact, bound = reference(q, k, v, [keys], None, 0, scale)
+    group = q.shape[1] // k.shape[1]
+    return exact, bound - (2.0**-25 - 2.0**-32) * v.double().cpu().abs().sum(2).repeat_interleave(group, 1)[:, :, None]
+
+
+WEAK = math.log(2.0**24 / 1.4)      # a weight of 1.4 times f16's smallest number
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("keys, width, queries", [(700, 64, 1), (40000, 64, 1), (9000, 128, 3)], ids=str)
+def test_many_weak_keys_behind_a_strong_one_in_the_cache(tq, keys, width, queries, dtype):
+    cache = Cache(1, 2, width, 64, -(-keys // 64)).fill([keys])
+    for codes, scales in zip(cache.codes, cache.scales):
+        scales.fill_(1.0)
+    first = int(cache.table[0, 0])
+    cache.codes[0].view(torch.uint8).zero_()
+    cache.codes[0][first, :, 0] = torch.ones(width, device="cuda").to(E4M3)
+    cache.codes[1].view(torch.uint8).copy_((torch.rand(cache.codes[1].shape, generator=cache.generator) + 0.5).to(E4M3).view(torch.uint8))
+    cache.codes[1].view(torch.uint8)[first, :, 0] = 0
+    q = torch.ones(1, 4, queries, width, dtype=dtype, device="cuda")
+    got = tq.cache_attention(q, *cache.tensors, cache.table, torch.tensor([keys], dtype=torch.int32).cuda(), scale=WEAK / width)
+    held(got, behind_a_strong_key(q, cache.decoded(0)[:, :, :keys], cache.decoded(1)[:, :, :keys], keys, WEAK / width))
+
+
+@pytest.mark.parametrize("batch, heads, kv_heads, queries, keys, width, tiles", [(1, 2, 1, 1, 700, 64, 0), (1, 2, 1, 2, 20000, 128, 0), (40, 12, 6, 150, 1500, 64, 64),
+                                                                                 (1, 8, 8, 300, 2000, 128, 128)], ids=str)
+def test_many_weak_keys_behind_a_strong_one_in_f16(tq, batch, heads, kv_heads, queries, keys, width, tiles):
+    assert form(batch, heads, kv_heads, queries, keys, width, 0, 0) == tiles
+    k = torch.zeros(1, kv_heads, keys, width, dtype=torch.float16, device="cuda")
+    k[:, :, 0] = 1.0
+    v = drawn((1, kv_heads, keys, width), torch.float32, 1).abs().clamp(0.5, 1.5).half()
+    v[:, :, 0] = 0.0
+    q = torch.ones(1, heads, queries, width, dtype=torch.float16, device="cuda")
+    got = tq.window_attention(*(t.repeat(batch, 1, 1, 1) for t in (q, k, v)), scale=WEAK / width)
+    assert torch.equal(got[0], got[-1])
+    held(got[:1, :, -2:], behind_a_strong_key(q[:, :, -2:], k, v, keys, WEAK / width))
+
+
 def test_scales_far_apart_between_pages(tq):
     cache = Cache(1, 1, 64, 16, 6).fill([96])
     cache.scales[1][cache.table[0].long(), 0] = torch.tensor([1e-12, 1e12, 3.0, 1e-30, 1e20, 0.7]).cuda()
