@@ -30,7 +30,8 @@
 // units do, and 16 rows twice the products; the special functions, tensor pipe and issue slots are below 50 %.
 //
 // Precision: scores, maxima, sums and results in f32. e4m3 to f16 is exact, and so is the query in f16: a row is scaled by a power of two to
-// a maximum of 2^14, so only elements 2^-38 of it or less lose digits. Probabilities against f16 values (cache codes too) are rounded to
+// a maximum of 2^14, so only elements 2^-38 of it or less lose digits (2^126 at most, which
+// brings every bf16 into f16's range). Probabilities against f16 values (cache codes too) are rounded to
 // f16 (half a step is 2^-11, under the result's 2^-8 in bf16; below 2^-21 of the largest it is 2^-32 of that, see kLift);
 // against bf16 values they take two bf16 operands, the rounded value and what rounding took off (2^-16).
 //
@@ -551,9 +552,9 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        // a power of two that brings the row's largest element to [2^14, 2^15); none for zeros and infinities
-        int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
-        if (exponent < -100 || exponent > 127) exponent = 14;
+        // a power of two that brings the row's largest element to [2^14, 2^15), 2^126 at most (from 2^-126 to 1); none for infinities
+        int exponent = max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -112);
+        if (exponent > 127) exponent = 14;
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
         back *= __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
 #pragma unroll

@@ -329,6 +329,12 @@ def test_queries_of_any_size(tq, spread):
     held(got, reference(q, cache.decoded(0).double(), cache.decoded(1).double(), [50], None, 0, scale))
 
 
+@pytest.mark.parametrize("spread", [2.0**-102, 2.0**-115, 2.0**-125, 2.0**90, 2.0**125])
+def test_queries_at_the_ends_of_bf16(tq, spread):
+    """The largest element under 2^-100, or near the largest number; 2^-133 is the smallest."""
+    test_queries_of_any_size(tq, spread)
+
+
 def behind_a_strong_key(q, k, v, keys, scale):
     """`reference` without what f16 loses below its normal range: weights are kept 2^7 times as large, so half a step there is 2^-32 of the largest."""
     exact, bound = reference(q, k, v, [keys], None, 0, scale)
