@@ -527,8 +527,9 @@ tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, const void* k
  * with element strides {batch, head, token}, multiples of 8, 16-byte aligned) goes to position starts[b] + i. `starts` and `counts` are
  * int32 [batch] in device memory; counts null: all tokens; starts[b] < 0: the sequence is left as it is. The scale of each page and head
  * that is written becomes the smallest power of two s, at least 2^-126, with every new |x| <= 448 s, and at least the scale that
- * was there if the page held tokens before starts[b]; codes are x / s rounded to nearest even; where s has grown, the page's earlier
- * tokens are encoded again. NaN and infinities become NaN and do not count for the scale. What lies behind the new tokens in a page stays as codes,
+ * was there if the page held tokens before starts[b] (2^127 at most); codes are x / s rounded to nearest even; where s has grown, the page's
+ * earlier tokens are encoded again. NaN and infinities become NaN and do not count for the scale; nor does a scale that was there and is no finite number,
+ * whose tokens become NaN. What lies behind the new tokens in a page stays as codes,
  * of a scale that may be another now: a sequence's tokens are written in their order. A page
  * that is written must belong to one sequence alone. */
 tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const void* v, void* k_pages, void* v_pages, float* k_scales, float* v_scales,

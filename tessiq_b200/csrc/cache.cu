@@ -209,12 +209,13 @@ cache_store_kernel(const __grid_constant__ StoreParams p) {
     const uint32_t bits = __float_as_uint(largest);
     int exponent = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     const uint32_t old_bits = __float_as_uint(old) & 0x7fffffffu;
-    if (old_bits < 0x7f000000u) exponent = max(exponent, static_cast<int>(old_bits >> 23) + ((old_bits & 0x7fffffu) != 0 ? 1 : 0));
+    const bool old_finite = old_bits < 0x7f800000u;
+    if (old_finite) exponent = max(exponent, min(static_cast<int>(old_bits >> 23) + ((old_bits & 0x7fffffu) != 0 ? 1 : 0), 254));
     exponent = max(exponent, 1);
     const float scale = __uint_as_float(static_cast<uint32_t>(exponent) << 23);
-    const float inverse = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
+    const float inverse = __uint_as_float(exponent == 254 ? 0x400000u : static_cast<uint32_t>(254 - exponent) << 23);      // (2^-127 is subnormal)
     if (held_tokens > 0 && scale != old) {
-      const float ratio = old * inverse;
+      const float ratio = old_finite ? old * inverse : NAN;
       uint2* const earlier = reinterpret_cast<uint2*>(page_at);
       for (int i = thread; i < held_tokens * vectors; i += TEAM) {
         const uint2 word = earlier[i];

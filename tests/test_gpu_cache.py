@@ -610,6 +610,43 @@ def test_what_is_not_finite_is_stored_as_nan_and_has_no_say_in_the_scale(tq):
     assert torch.equal(codes.isnan(), ~k[0, 0].isfinite()) and (codes[~codes.isnan()] == 256.0).all()
 
 
+@pytest.mark.parametrize("old", [2.0**126, 1.5 * 2.0**126, 2.0**127, 1.5 * 2.0**127, 2.0**-140, 0.0, -0.25], ids=str)
+def test_a_store_behind_tokens_of_any_finite_scale(tq, old):
+    """A pool may come with scales that `cache_store` does not make: the page's earlier tokens keep what they stood for, as far as e4m3 at the new scale has it, and
+    a value beyond 448 times the largest power of two, which is beyond f32, becomes that."""
+    cache = Cache(2, 2, 64, 16, 1).fill([7, 0])
+    page = int(cache.table[0, 0])
+    for scales in cache.scales:
+        scales[page, 0] = old
+    was = [c[page, 0, :7].cpu().float().double() * old for c in cache.codes]
+    k, v = (by_token((2, 2, 2, 64), torch.bfloat16, s) for s in (5, 6))
+    tq.cache_store(k, v, *cache.tensors, cache.table, torch.tensor([7, 0], dtype=torch.int32).cuda())
+    for i, x in enumerate((k, v)):
+        scale = cache.scales[i][page, 0].item()
+        largest = x[0, 0].abs().max().item()
+        s = 2.0**-126
+        while largest > 448 * s or (s < abs(old) and s < 2.0**127):
+            s *= 2
+        assert scale == s
+        codes = cache.codes[i][page, 0, :9].cpu().float().double()
+        assert torch.equal(codes[7:], nearest_code(x[0, 0].cpu().double() / s))
+        assert torch.equal(codes[:7], nearest_code((was[i] / s).clamp(-448, 448)))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("old", [math.nan, math.inf, -math.inf], ids=str)
+def test_a_store_behind_tokens_whose_scale_is_no_number(tq, old):
+    """They are no numbers either, and have no say in the new scale."""
+    cache = Cache(1, 1, 64, 16, 1).fill([7])
+    page = int(cache.table[0, 0])
+    for scales in cache.scales:
+        scales[page] = old
+    k = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    tq.cache_store(k, k, *cache.tensors, cache.table, torch.tensor([7], dtype=torch.int32).cuda())
+    for codes, scales in zip(cache.codes, cache.scales):
+        assert scales[page, 0].item() == 2.0**-8 and (codes[page, 0, 7:9].float() == 256.0).all() and codes[page, 0, :7].float().isnan().all()
+
+
 @pytest.mark.parametrize("page, tokens, width", [(16, 1, 64), (16, 16, 64), (32, 30, 64), (64, 64, 64), (64, 64, 128), (128, 120, 128)])
 def test_what_is_not_finite_stays_with_its_head(tq, page, tokens, width):
     """Every other head has a NaN or an infinity, its neighbours come out as without them."""
