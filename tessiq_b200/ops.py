@@ -588,7 +588,8 @@ def _window(window, sinks) -> tuple[int, int]:
         raise ValueError(f"a window has at least one key, not {window}; None is no window")
     if int(sinks) < 0:
         raise ValueError(f"sinks are a number of first keys, not {sinks}")
-    return 0 if window is None else int(window), int(sinks)
+    most = 1 << 31      # (beyond every position; ctypes would take numbers over 64 bits modulo 2^64)
+    return 0 if window is None else min(int(window), most), min(int(sinks), most)
 
 
 def _own_scratch(nbytes: int, device: int) -> torch.Tensor | None:

@@ -155,6 +155,15 @@ def test_python_refuses_before_the_library():
     ops.copy_pages([], [0], [1])
 
 
+def test_windows_and_sinks_of_any_length():
+    from tessiq_b200 import ops
+
+    for n in (1 << 31, (1 << 63) - 1, 1 << 63, (1 << 64) + 3, 10**30):
+        window, sinks = ops._window(n, n)
+        assert 1 << 30 <= window < 1 << 63 and 1 << 30 <= sinks < 1 << 63
+    assert ops._window(None, 0) == (0, 0) and ops._window(7, 3) == (7, 3)
+
+
 # ---- the books -----------------------------------------------------------------------------------
 
 
