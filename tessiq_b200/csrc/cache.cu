@@ -521,7 +521,8 @@ extern "C" tq_status tq_copy_pages_launch(const tq_paged_tensor* tensors, int32_
       if (t.layers == 0 || t.page_bytes == 0) continue;
       TQ_REQUIRE(t.base != nullptr, TQ_INVALID_ARGUMENT, "tensor %d is null", i);
       TQ_REQUIRE(t.page_stride >= t.page_bytes, TQ_INVALID_ARGUMENT, "the pages of tensor %d overlap", i);
-      TQ_REQUIRE(t.layers <= 65535 && t.page_bytes < (1LL << 34), TQ_UNSUPPORTED, "extents beyond the kernel's index range");
+      TQ_REQUIRE(t.layers <= 65535 && t.page_bytes < (1LL << 34) && t.layers * ((t.page_bytes + tq::kCopyBytes - 1) / tq::kCopyBytes) < (1LL << 31),
+                 TQ_UNSUPPORTED, "extents beyond the kernel's index range");
       some.push_back(t);
     }
     // what is a source, what a target: a bit each

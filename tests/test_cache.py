@@ -93,6 +93,12 @@ def test_copy_pages_refuses(lib, sources, targets, changed):
     assert copy(lib, sources, targets, **changed) == lib.TQ_INVALID_ARGUMENT, lib.last_error()
 
 
+@pytest.mark.parametrize("changed", [{"layers": 65536}, {"page_bytes": 1 << 34}, {"layers": 65535, "page_bytes": 1 << 33}, {"layers": 4096, "page_bytes": 1 << 33}], ids=str)
+def test_copy_pages_beyond_a_launch(lib, changed):
+    """(A tensor's layers may lie anywhere, on one another too, so these are not beyond what memory can hold.)"""
+    assert copy(lib, [0], [1], **{**changed, "page_stride": 1 << 35}) == lib.TQ_UNSUPPORTED, lib.last_error()
+
+
 def test_copy_pages_with_nothing_to_do(lib):
     assert copy(lib, [], []) == lib.TQ_OK
     assert lib.lib.tq_copy_pages_launch(None, 0, 4, None, None, 3, 0, None) == lib.TQ_OK
