@@ -227,8 +227,13 @@ class PagedCache:
     def length(self, sequence: int) -> int:
         return self.books.length(sequence)
 
+    def _not_in_a_graph(self, what: str) -> None:
+        if self.k_scales.is_cuda and (torch.cuda.is_current_stream_capturing() or ops.lib.tq_is_recording()):
+            raise RuntimeError(f"{what} keeps its books on the host and cannot go into a graph or a recording; storing and attention of a step can")
+
     def extend(self, sequences: Sequence[int], tokens) -> Step:
         """Room for `tokens` (one number, or one for each) tokens more in each of `sequences`; last pages that forks share are copied first."""
+        self._not_in_a_graph("extend")
         sequences = list(sequences)
         counts = [int(tokens)] * len(sequences) if isinstance(tokens, int) else [int(count) for count in tokens]
         starts = [self.books.length(sequence) for sequence in sequences]
@@ -273,6 +278,7 @@ class PagedCache:
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers; how many moved. Steps from before must not be used again."""
+        self._not_in_a_graph("compact")
         sources, targets = self.books.compact()
         if sources:
             ops.copy_pages(self.tensors, sources, targets, page_axis=1)

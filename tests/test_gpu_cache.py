@@ -1028,3 +1028,47 @@ def test_a_paged_cache_through_forks_drafts_and_moves(tq):
     agrees(live, write(live, 1), 20, 3)
     used = {page for sequence in live for page in cache.books.pages_of(sequence)}
     assert len(used) + cache.books.free_pages == 24 and status() == 0
+
+
+@pytest.mark.parametrize("way", ["captured", "recorded"])
+def test_the_books_are_not_kept_in_a_graph(tq, way):
+    """A step's table is made on the host, as pages are handed out: in a graph it would be sent again from memory that is somebody else's by then, and the
+    copies that the books count on would not have been made. Storing and attention go into a graph, extend and compact are refused and change nothing."""
+    from tessiq_b200 import _lib
+    from tessiq_b200.cache import PagedCache
+
+    cache = PagedCache(1, 2, 32, pages=8, page_tokens=16)
+    gone, a = cache.start(), cache.start()
+    k, q = by_token((1, 2, 20, 32), torch.bfloat16, 1), by_token((1, 4, 1, 32), torch.bfloat16, 2)
+    cache.extend([gone], 3)
+    step = cache.extend([a], 20)
+    cache.free(gone)
+    cache.store(step, 0, k, k)
+    expected = cache.attention(step, 0, q)
+    torch.cuda.synchronize()
+    before = (cache.books.pages_of(a), cache.length(a), cache.books.free_pages)
+
+    def inside():
+        for call in (lambda: cache.extend([a], 1), cache.compact):
+            with pytest.raises(RuntimeError, match="graph"):
+                call()
+        cache.store(step, 0, k, k)
+        return cache.attention(step, 0, q)
+
+    if way == "captured":
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = inside()
+        graph.replay()
+    else:
+        handle = ctypes.c_void_p()
+        _lib.check(_lib.lib.tq_recipe_create(ctypes.byref(handle)))
+        _lib.check(_lib.lib.tq_recipe_begin_recording(handle))
+        got = inside()
+        _lib.check(_lib.lib.tq_recipe_end_recording(handle))
+        _lib.check(_lib.lib.tq_recipe_run(handle, 0, torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        _lib.check(_lib.lib.tq_recipe_destroy(handle))
+    torch.cuda.synchronize()
+    assert torch.equal(got, expected) and before == (cache.books.pages_of(a), cache.length(a), cache.books.free_pages)
+    assert cache.compact() == 1 and cache.extend([a], 1).lengths.tolist() == [21] and status() == 0
