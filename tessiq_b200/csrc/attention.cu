@@ -580,6 +580,61 @@ __device__ __forceinline__ WindowBlock window_block(const WindowAttnParams& p, i
   return b;
 }
 
+// Which columns of the values are a NaN (bit 0), an infinity (1), minus infinity (2) in some key that all rows from position `first` to `last` see, by a
+// warp: column 64 h + 2 lane + e in bits 3 (2 h + e) and up. Ends where every column is a NaN.
+template <typename T, int D>
+__device__ __forceinline__ uint32_t not_finite_for_all(const WindowAttnParams& p, int batch, int key_head, int first, int last) {
+  constexpr uint32_t kInfinity = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+  constexpr int kPairs = D / 64, kAtOnce = 8;
+  const int lane = threadIdx.x & 31;
+  const T* v = static_cast<const T*>(p.v) + batch * p.v_strides[0] + key_head * p.v_strides[1] + 2 * lane;
+  const int start = max(last - p.window + 1, 0), sinks = max(min(min(p.sinks, first + 1), start), 0), count = sinks + max(first + 1 - start, 0);
+  uint32_t found = 0, all = 0;
+#pragma unroll
+  for (int h = 0; h < kPairs; ++h) all |= 64 * h + 2 * lane < p.head_dim ? 9u << 6 * h : 0u;
+#pragma unroll 1
+  for (int nth0 = 0; nth0 < count && !__all_sync(0xffffffffu, (found & all) == all); nth0 += kAtOnce) {
+    uint32_t pair[kAtOnce][kPairs];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int nth = nth0 + i, key = nth < sinks ? nth : nth - sinks + start;
+#pragma unroll
+      for (int h = 0; h < kPairs; ++h) {
+        pair[i][h] = 0;
+        if (nth < count && 64 * h + 2 * lane < p.head_dim) pair[i][h] = *reinterpret_cast<const uint32_t*>(v + key * p.v_strides[2] + 64 * h);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+      for (int n = 0; n < 2 * kPairs; ++n) {
+        const uint32_t x = n % 2 ? pair[i][n / 2] >> 16 : pair[i][n / 2] & 0xffffu, size = x & 0x7fffu;
+        found |= (size > kInfinity ? 1u : size < kInfinity ? 0u : x >> 15 ? 4u : 2u) << 3 * n;
+      }
+    }
+  }
+  return found;
+}
+
+// Whether what is no finite number in a result row is what the row's own keys make it, by what not_finite_for_all has found: a NaN where a value is one or
+// values are infinities of both signs, an infinity (which a NaN of any other key would not have left) where a value is that.
+template <typename T, int D>
+__device__ __forceinline__ bool row_stands(const WindowAttnParams& p, int batch, int head, int row, uint32_t found) {
+  constexpr uint32_t kInfinity = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+  const T* out = static_cast<const T*>(p.out) + batch * p.out_batch + head * p.out_head + row * p.out_token;
+  bool stands = true;
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n) {
+    const int column = 64 * (n / 2) + 2 * (threadIdx.x & 31) + n % 2;
+    if (column < p.head_dim) {
+      const uint32_t x = reinterpret_cast<const unsigned short*>(out)[column], size = x & 0x7fffu, here = found >> 3 * n & 7u;
+      if (size > kInfinity) stands &= (here & 1u) != 0 || here == 6u;
+      else if (size == kInfinity) stands &= (here & (x >> 15 ? 4u : 2u)) != 0;
+    }
+  }
+  return __all_sync(0xffffffffu, stands);
+}
+
 // One result row from the keys it sees and nothing else, by a warp: 32 keys at a time, a key a lane for its score, D / 32 elements of the head a
 // lane for the result.
 template <typename T, int D>
@@ -968,12 +1023,18 @@ window_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       tcgen05_fence_before();
       // The products take every key of a tile, at a probability of zero where a row does not see it, and zero times an infinity or a NaN is a
-      // NaN. So a row that came out with one is taken again from its own keys alone, by the warp, in plain f32: slow, and rare on real data.
-      uint32_t again = __ballot_sync(0xffffffffu, odd && stores);
-      while (again != 0) {
-        const int row = b.q0 + warp * 32 + __ffs(again) - 1;
-        again &= again - 1;
-        take_row_again<T, D>(p, b.batch, b.head, b.key_head, row);
+      // NaN. So a row that came out with one is taken again from its own keys alone, by the warp, in plain f32, unless it must be one: its sum, which
+      // no other key is in, is no positive number (a NaN in the queries or in a key it sees), or values that all rows of the warp see make it one. Without
+      // these two a NaN that everybody sees was a thousand times the launch (2 x 12 x 4096 under a window of 1024 54 us, all NaN 43.5 ms).
+      uint32_t again = __ballot_sync(0xffffffffu, odd && stores && row_sum > 0.f);
+      if (again != 0) {
+        const int first = b.q0 + warp * 32 + p.offset, last = min(first + 31, p.q_tokens - 1 + p.offset);
+        const uint32_t found = not_finite_for_all<T, D>(p, b.batch, b.key_head, first, last);
+        do {
+          const int row = b.q0 + warp * 32 + __ffs(again) - 1;
+          again &= again - 1;
+          if (!row_stands<T, D>(p, b.batch, b.head, row, found)) take_row_again<T, D>(p, b.batch, b.head, b.key_head, row);
+        } while (again != 0);
       }
     }
   }

@@ -216,6 +216,72 @@ def test_a_value_that_is_not_a_number_reaches_the_queries_that_see_it(tq, batch,
     assert ((got - expected[0]).abs()[fine] <= expected[1][fine]).all()
 
 
+TILES = [(40, 12, 6, 150, 180, 64, 70, 3, 64), (1, 12, 12, 300, 1500, 64, 0, 0, 128), (12, 16, 8, 150, 200, 96, 90, 70, 64), (1, 8, 8, 300, 2000, 128, 0, 8, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", TILES, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("bad", ["a sink", "a channel", "signs", "scattered", "keys", "queries", "everything"])
+def test_what_is_no_number_on_the_tiles(tq, case, dtype, bad):
+    """Seen by all rows, by some, or by none of a tile: each row has what its own keys make of it."""
+    *extents, tiles = case
+    batch, heads, kv_heads, queries, keys, width, window, sinks = extents
+    assert form(*extents) == tiles
+    q, k, v = (by_token((1, n, t, width), dtype, s) for n, t, s in ((heads, queries, 1), (kv_heads, keys, 2), (kv_heads, keys, 3)))
+    at = torch.randint(0, keys, (9,), generator=torch.Generator().manual_seed(4)).tolist()
+    if bad == "a sink":
+        v[:, :, 0, 5], v[:, :, 1, 6] = math.nan, math.inf
+    elif bad == "a channel":
+        v[:, :, :, 7] = math.inf
+    elif bad == "signs":
+        v[:, :, keys // 2, 2], v[:, :, keys // 2 + 3, 2], v[:, :, keys // 2 + 9, 3] = math.inf, -math.inf, -math.inf
+    elif bad == "scattered":
+        for n, j in enumerate(at):
+            v[:, :, j, (7 * n) % width] = (math.nan, math.inf, -math.inf)[n % 3]
+    elif bad == "keys":
+        k[:, :, at, 1] = math.nan
+    elif bad == "queries":
+        q[:, :, ::7] = math.nan
+    else:
+        q, k, v = (torch.full_like(t, math.nan) for t in (q, k, v))
+    got = tq.window_attention(*(t.expand(batch, -1, -1, -1).clone(memory_format=torch.preserve_format) if batch > 1 else t for t in (q, k, v)), window or None, sinks)
+    rows = sorted({0, 1, 30, 31, 32, 33, 62, 63, 127, 128, 129, queries - 1, *(j - keys + queries + d for j in at for d in (-1, 0, 1) if 0 <= j - keys + queries + d < queries)})
+    some = max(1, 2 * kv_heads // heads)
+    exact, bound = (torch.cat(parts, 2) for parts in zip(*(reference(q[:, :2, i : i + 1], k[:, :some], v[:, :some], [keys - queries + i + 1], window or None, sinks, width**-0.5)
+                                                           for i in rows)))
+    got = got[-1:, :2, rows].cpu().double()
+    assert torch.equal(got.isnan(), exact.isnan()) and torch.equal(got[got.isinf()], exact[exact.isinf()]) and torch.equal(got.isinf(), exact.isinf())
+    fine = exact.isfinite()
+    assert ((got - exact).abs()[fine] <= bound[fine]).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("bad", ["everything", "a key", "a value"])
+def test_a_nan_that_everybody_sees_costs_no_second_reading(tq, bad):
+    """(It was 800 times the launch; a reading of the values by each warp is a few times it.)"""
+    q, k, v = (drawn((2, 12, 4096, 64), torch.bfloat16, s) for s in (1, 2, 3))
+
+    def time_of(q, k, v):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        for n in range(4):
+            if n == 1:
+                start.record()
+            got = tq.window_attention(q, k, v, 1024, 4)
+        end.record()
+        torch.cuda.synchronize()
+        return start.elapsed_time(end), got
+
+    fine, _ = time_of(q, k, v)
+    if bad == "everything":
+        q, k, v = (torch.full_like(t, math.nan) for t in (q, k, v))
+    elif bad == "a key":
+        k[:, :, 0] = math.nan
+    else:
+        v[:, :, 0] = math.nan
+    slow, got = time_of(q, k, v)
+    assert got.isnan().all() and slow < 50 * fine
+
+
 def test_scores_that_are_all_minus_infinity_are_not_a_number(tq):
     """As softmax over them is; a query that sees nothing is zeros instead."""
     q, k, v = (drawn((1, 1, 2, 64), torch.bfloat16, s).abs() + 0.5 for s in (1, 2, 3))
