@@ -656,8 +656,12 @@ __device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int ba
     if (nth < count) {
       const T* from = k + key * p.k_strides[2];
       score = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < p.head_dim; ++c) score = fmaf(to_compute(q[c]), to_compute(from[c]), score);
+#pragma unroll 2
+      for (int c = 0; c < p.head_dim; c += 8) {      // (rows of q and k are 16-byte aligned: TMA reads them too)
+        const uint4 a = *reinterpret_cast<const uint4*>(q + c), b = *reinterpret_cast<const uint4*>(from + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) score = fmaf(to_compute(reinterpret_cast<const T*>(&a)[e]), to_compute(reinterpret_cast<const T*>(&b)[e]), score);
+      }
       score *= p.scale_log2;
     }
     float top = score;
@@ -670,7 +674,7 @@ __device__ __forceinline__ void take_row_again(const WindowAttnParams& p, int ba
     total = total * factor + warp_sum(weight);
 #pragma unroll
     for (int c = 0; c < kMine; ++c) result[c] *= factor;
-#pragma unroll 1
+#pragma unroll 4
     for (int i = 0; i < min(32, count - first); ++i) {
       const float w = __shfl_sync(0xffffffffu, weight, i);
       const T* from = v + __shfl_sync(0xffffffffu, key, i) * p.v_strides[2];
