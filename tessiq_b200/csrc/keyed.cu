@@ -597,7 +597,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     for (int step = 0; step < mine; ++step, ++turn) {
       const int key0 = chunk_at(step) * S::kKeys;
       const int stage = turn % kKeyedStages;
-      if (!barrier_wait(barrier0 + 8 * stage, (turn / kKeyedStages) & 1, p.status, kWaitKeyed)) {
+      // (by a vote: lanes that gave up leave the loop, and its shuffles, with all the others)
+      if (!__all_sync(0xffffffffu, barrier_wait(barrier0 + 8 * stage, (turn / kKeyedStages) & 1, p.status, kWaitKeyed))) {
         // the result is lost (the status says so); the copies that are under way still have to land before the stages are used otherwise
         for (int m = step; m < min(step + kKeyedStages, mine); ++m, ++turn) {
           for (uint32_t spin = 0; spin < kSpinLimit && !barrier_try_wait(barrier0 + 8 * (turn % kKeyedStages), (turn / kKeyedStages) & 1); ++spin) {
