@@ -1138,3 +1138,27 @@ def test_the_books_are_not_kept_in_a_graph(tq, way):
     torch.cuda.synchronize()
     assert torch.equal(got, expected) and before == (cache.books.pages_of(a), cache.length(a), cache.books.free_pages)
     assert cache.compact() == 1 and cache.extend([a], 1).lengths.tolist() == [21] and status() == 0
+
+
+def test_steps_of_nothing(tq):
+    """No sequence, sequences without tokens, and no new tokens for those that have some."""
+    from tessiq_b200.cache import PagedCache
+
+    cache = PagedCache(1, 2, 32, pages=8, page_tokens=16)
+    a, b = cache.start(), cache.start()
+    k, q = by_token((2, 2, 5, 32), torch.bfloat16, 1), by_token((2, 4, 3, 32), torch.bfloat16, 2)
+    nobody = cache.extend([], 1)
+    cache.store(nobody, 0, k[:0], k[:0])
+    assert cache.attention(nobody, 0, q[:0]).shape == (0, 4, 3, 32)
+    empty = cache.extend([a, b], 0)
+    cache.store(empty, 0, k[:, :, :0], k[:, :, :0])
+    assert cache.attention(empty, 0, q).count_nonzero().item() == 0
+    first = cache.extend([a, b], [5, 0])
+    cache.store(first, 0, k, k)
+    got = cache.attention(first, 0, q)
+    assert got[1].count_nonzero().item() == 0 and got[0].count_nonzero().item() > 0
+    again = cache.extend([a, b], 0)
+    before = [t.view(torch.uint8).clone() for t in cache.tensors]
+    cache.store(again, 0, k, k)
+    assert torch.equal(cache.attention(again, 0, q), got) and all(torch.equal(t.view(torch.uint8), was) for t, was in zip(cache.tensors, before))
+    assert status() == 0
