@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import math
 from functools import lru_cache
+from operator import index
 from typing import Sequence
 
 import torch
@@ -750,9 +751,13 @@ def copy_pages(tensors, sources, targets, page_axis=0) -> None:
         one.layer_stride = t.stride(0) * size if page_axis else 0
         one.page_bytes = math.prod(t.shape[page_axis + 1 :]) * size
         one.page_stride = max(t.stride(page_axis) * size, one.page_bytes if pages == 1 else 0)
+    sources, targets = [index(page) for page in sources], [index(page) for page in targets]
+    for page in (*sources, *targets):
+        if not 0 <= page < pages:      # (ctypes would take it modulo 2^64)
+            raise ValueError(f"there is no page {page} among {pages}")
     device = _device_of(tensors)
     numbers = ctypes.c_int64 * len(sources)
-    check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*map(int, sources)), numbers(*map(int, targets)), len(sources), device,
+    check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*sources), numbers(*targets), len(sources), device,
                                    _stream(None, device)))
 
 

@@ -161,6 +161,18 @@ def test_python_refuses_before_the_library():
     ops.copy_pages([], [0], [1])
 
 
+@pytest.mark.parametrize("page", [7, -1, 1 << 64, (1 << 64) + 2, -(1 << 63) - 1])
+def test_pages_are_numbers_of_pages(page):
+    from tessiq_b200 import ops
+
+    scales = torch.ones(7, 2)
+    for pair in (([page], [1]), ([1], [page]), ([0, page], [2, 3])):
+        with pytest.raises(ValueError, match=f"no page {page}"):
+            ops.copy_pages([scales], *pair)
+    with pytest.raises(TypeError):
+        ops.copy_pages([scales], [0.5], [1])
+
+
 def test_windows_and_sinks_of_any_length():
     from tessiq_b200 import ops
 
