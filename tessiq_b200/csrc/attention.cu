@@ -1137,12 +1137,14 @@ AttentionForm choose_attention_form(long long heads, long long q_tokens, long lo
 }
 
 // Keys a step of the tensor-core tiles for window attention, or 0: the keys are streamed (keyed.cu), which shares a head's keys among all SMs but
-// takes 16 rows of a key head at a time where a tile has 128 and walks its keys in one CTA. The smaller of two expected times (us; B200, bf16;
-// measured: tiles / streamed). 12 heads of 64, 8000 keys, 8 queries 80 / 14.5, 128 queries 80 / 36, 300 queries 82 / 70; 8 x 12 heads 40 queries
-// 84 / 88, 100 queries 85 / 190; 8 key heads of 128 for 32, 100 queries, 300 keys 10.3 / 12.4, 2000 keys 24.7 / 41, 8000 keys 83 / 107, 5 queries
-// 82 / 29. Tiles: 128 keys a step where few CTAs leave the steps' latency bare (up to two an SM, one of heads above 64), and for heads up to 64
-// where there are many steps: 8 x 12 x 4096 tokens under a window of 64 110.9 with 128 and 86.6 with 64, of 1024 196.4 and 195.9, of 4096 334 and
-// 356; 2 x 32 x 2501 of 128 under 333 104 and 76.
+// takes 16 rows of a key head at a time where a tile has 128 and walks its keys in one CTA. The smaller of two expected times, each coarser than
+// what runs: the streamed one counts CTAs of four warps (keyed.cu has two, four or eight, by an estimate of its own), the tiles' 128 keys a step. Both
+// sides measured (us, bf16; tiles / streamed): 12 heads of 64, 8000 keys, 8 queries 79 / 14.6, 128 queries 80 / 36, 300 queries 80 / 70; 8 x 12
+// heads 40 queries 82 / 79 (the rule takes the tiles), 100 queries 83 / 183; 2000 keys, 17 queries 24.2 / 21.5 (tiles: the farthest from the
+// better one of 20 shapes); 8 key heads of 128 for 32, 100 queries, 300 keys 8.7 / 10.2, 2000 keys 23.4 / 39, 8000 keys 80 / 105, 5 queries 79 /
+// 20.5. Tiles: 128 keys a step where few CTAs leave the steps' latency bare (up to two an SM, one of heads above 64), and for heads up to 64
+// where there are many steps: 8 x 12 x 4096 tokens under a window of 64 83.0 with 128 and 63.4 with 64, of 1024 179.5 and 177.8, of 4096 311.9 and
+// 326.4; 2 x 32/8 x 2501 of 128 under 333 78.7 and 60.9.
 int window_tile_keys(const KeyedParams& p, long long sms) {
   const bool wide = p.head_dim > kHeadDim;
   const long long rows = static_cast<long long>(p.group) * p.q_tokens;
@@ -1156,7 +1158,7 @@ int window_tile_keys(const KeyedParams& p, long long sms) {
   const double tiles = 5.5 + 1.2 * steps_of(p.q_tokens < kRows ? p.q_tokens : kRows, 128) * (ctas > at_once ? static_cast<double>(ctas) / at_once : 1.0);
   const long long tile_rows = rows <= 8 ? 8 : 16, units = (rows + tile_rows - 1) / tile_rows * p.kv_heads * p.batch;
   const long long chunks = steps_of((tile_rows + p.group - 1) / p.group, wide ? 16 : 32);
-  const bool whole = chunks <= 8 || (chunks <= 32 && units <= 4 * sms);      // keyed.cu: a CTA a unit
+  const bool whole = chunks <= 8 || (chunks <= 32 && units <= 4 * sms);      // a CTA a unit
   const double steps = static_cast<double>((chunks + 3) / 4), waves = units > 2 * sms ? units / (2.0 * sms) : 1.0;
   const double streamed = whole ? 1.0 + waves * (5.0 + steps) : 13.0 + units * chunks * 1.2 / (8.0 * sms);
   if (streamed <= tiles) return 0;

@@ -24,16 +24,15 @@
 // and no second kernel (plan_shape). Tried beside the second kernel: the last CTA to arrive at a ticket joins (48 us for 33 + 6: fences, and code that nobody
 // has run yet, at the very end).
 //
-// Measured (kernels and join; us, and of HBM's 6456 GB/s): 16 x 64/8 heads of 128, 20001 to 40000 keys in 8 bits 160 (0.95); 32 x 32/8 heads,
-// 2052 keys in 16 bits 50 (0.84); 64 x 12 heads of 64, 1 to 2000 keys 27 (0.57), all 1000 21 (0.74); four queries of 48 x 32/8, 1028 keys 34
-// (0.45); 12 heads of 64, 1500 keys 7. A fixed 12 us (launch, lengths, first pages and keys, join) is what dealt-out short ones pay, 5 us what
+// Measured (kernels and join; us, and of HBM's 6456 GB/s): 16 x 64/8 heads of 128, 20001 to 40000 keys in 8 bits 163 (0.93); 32 x 32/8 heads,
+// 2052 keys in 16 bits 50 (0.83); 64 x 12 heads of 64, 1 to 2000 keys 27 (0.57), all 1000 21 (0.74); four queries of 48 x 32/8, 1028 keys 34.5
+// (0.44); 12 heads of 64, 1500 keys 7. How chunks are split goes by the table's width, not by lengths, which are on the device. A fixed 12 us (launch, lengths, first pages and keys, join) is what dealt-out short ones pay, 5 us what
 // units do, and 16 rows twice the products; the special functions, tensor pipe and issue slots are below 50 %.
 //
 // Precision: scores, maxima, sums and results in f32. e4m3 to f16 is exact, and so is the query in f16: a row is scaled by a power of two to
-// a maximum of 2^14, so only elements 2^-38 of it or less lose digits (2^126 at most, which
-// brings every bf16 into f16's range). Probabilities against f16 values (cache codes too) are rounded to
-// f16 (half a step is 2^-11, under the result's 2^-8 in bf16; below 2^-21 of the largest it is 2^-32 of that, see kLift);
-// against bf16 values they take two bf16 operands, the rounded value and what rounding took off (2^-16).
+// a maximum of 2^14 (by 2^126 at most, which brings every bf16 into f16's range), so only elements 2^-38 of it or less lose digits. Probabilities
+// against f16 values (cache codes too) are rounded to f16: half a step is 2^-11, under the result's 2^-8 in bf16, and below 2^-21 of the row's largest
+// 2^-32 of that (kLift). Against bf16 values they take two bf16 operands, the rounded value and what rounding took off (2^-16).
 //
 // A masked key must not reach a result through 0 * NaN: its score is replaced, and a value that no row of the tile sees becomes zeros in the
 // stage. Where rows see different keys (several queries, at an end of the window) and a value they do see is no number, or its page's scale, the
