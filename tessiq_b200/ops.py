@@ -779,7 +779,7 @@ def _window_attention_by_aten(q, k, v, window, sinks, scale):
     # A weight of zero does not keep out a value that is no finite number, so those come in apart: NaN where a query sees one (or an infinity of weight
     # zero), an infinity where it sees that.
     finite, up, down = (weights @ part for part in (v.masked_fill(~v.isfinite(), 0.0), (v == math.inf).to(wide), (v == -math.inf).to(wide)))
-    nan = torch.cat([sees.expand_as(weights), sees & (weights == 0)], -1).to(wide) @ torch.cat([v.isnan(), v.isinf()], -2).to(wide)
+    nan = sees.to(wide) @ v.isnan().to(wide) + (sees & (weights == 0)).to(wide) @ v.isinf().to(wide)
     out = torch.where(up > 0, math.inf, torch.where(down > 0, -math.inf, finite))
     out = out.masked_fill((nan > 0) | ((up > 0) & (down > 0)), math.nan)
     return out.to(q.dtype).contiguous()
