@@ -666,8 +666,8 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, win
     a power of two from 16 to 1024, width a multiple of 16 up to 128), the scales float32 [pages, kv_heads]; an element is
     code * scale. Row b of `table` (int32 [batch, blocks]) names the pages of sequence b in order, lengths[b] (int32, on the
     device) says how many tokens it has, the queries' own among them: query i of q [batch, heads, q_tokens, width] stands at
-    position lengths[b] - q_tokens + i. Page numbers and lengths stay on the device; one that leads out of the pool or the table is left
-    out, and `kernel.check_status` then raises."""
+    position lengths[b] - q_tokens + i. Page numbers and lengths stay on the device: a page outside the pool is left out, a sequence longer
+    than its table ends with it, and `kernel.check_status` then raises. Pages that no query sees are not looked at: the table may name anything there."""
     given = (q, k_pages, v_pages, k_scales, v_scales, table, lengths, window, sinks, scale, token_major)
     out = _call(_CODES["cache attention"], *given)
     if out is not None:
