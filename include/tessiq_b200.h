@@ -523,6 +523,19 @@ tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, const void* k
                                     const int64_t* q_strides, const int64_t* out_strides, double scale, int64_t window, int64_t sinks, void* workspace,
                                     size_t workspace_bytes, int32_t device, void* stream);
 
+/* tq_prefix_attention_launch: tq_cache_attention_launch without a window, for a batch of `runs` equal runs of neighbouring sequences whose first
+ * shared[r] (int32 [runs], device memory) tokens are the same: the caller says so, and may name the same pages in their tables or others of the same
+ * content. Whole tiles of 128 of these are read once for all sequences of the run that are at least so long (every query stands behind them), through
+ * the table row of the first of those; what is left of them, and the shared tokens of shorter sequences (a padded row of length 0 among them), each
+ * sequence reads itself. shared[r] <= 0: nothing is shared. `workspace` as there, tq_prefix_attention_workspace_bytes of it. */
+tq_status tq_prefix_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens,
+                                              int64_t blocks, int64_t runs, int32_t device, size_t* bytes);
+tq_status tq_prefix_attention_launch(tq_dtype dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
+                                     const float* v_scales, const int32_t* table, const int32_t* lengths, const int32_t* shared, void* out, int64_t batch,
+                                     int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t pages, int64_t page_tokens, int64_t blocks,
+                                     int64_t table_stride, int64_t runs, const int64_t* q_strides, const int64_t* out_strides, double scale,
+                                     void* workspace, size_t workspace_bytes, int32_t device, void* stream);
+
 /* Writes new tokens into the cache: token i < counts[b] of sequence b (k and v are [batch, kv_heads, tokens, head_dim], bf16 or f16,
  * with element strides {batch, head, token}, multiples of 8, 16-byte aligned) goes to position starts[b] + i. `starts` and `counts` are
  * int32 [batch] in device memory; counts null: all tokens; starts[b] < 0: the sequence is left as it is. The scale of each page and head
@@ -547,6 +560,33 @@ typedef struct tq_paged_tensor {
  * numbers below `pages`; the targets are distinct and none of them is a source (TQ_INVALID_ARGUMENT otherwise), so the order of the copies does not show. */
 tq_status tq_copy_pages_launch(const tq_paged_tensor* tensors, int32_t count, int64_t pages, const int64_t* sources, const int64_t* targets,
                                int64_t pairs, int32_t device, void* stream);
+
+/* One step of the books of beams, on the device. Row b of the table (int32 [batch, blocks], `table_stride` elements apart) has the pages of lengths[b]
+ * tokens; references[p] says how many rows, or others, have page p, and 0 that it is free. Row b of the new table goes on from row parents[b] (parents
+ * null: from b; negative: an empty row) and gets room for counts[b] tokens:
+ *   starts[b] = lengths[parents[b]], new_lengths[b] = starts[b] + counts[b];
+ *   where counts[b] > 0 and starts[b] lies inside a page that others have too, the row gets a copy of it: all rows that write into such a page, but for the
+ *   last of them where nobody else has it;
+ *   pages that are copied to, and new ones behind, are the lowest free ones, row by row, a row's copy first. Entries behind a row's end stay.
+ * The contents of copied pages are copied in every layer of up to four tensors. All arrays are device memory; new_table, new_lengths and new_references
+ * may be the operands themselves, and overlap them in no other way. If the free pages do not suffice, a row would not fit the table or is longer than it, a parent is not below
+ * `batch` or a page not in the pool, nothing changes, every starts[b] is -1 (which tq_cache_store_launch passes over), and tq_status_poll reports
+ * 0x46554c4c "FULL", 0x4c454e47 "LENG", 0x50415245 "PARE" or 0x50414745 "PAGE". `workspace` as for the attention calls. */
+tq_status tq_cache_advance_workspace_bytes(int64_t batch, int64_t blocks, int64_t pages, int64_t page_tokens, size_t* bytes);
+tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int32_t count, const int32_t* table, const int32_t* lengths, const int32_t* references,
+                                  const int32_t* counts, const int32_t* parents, int32_t* new_table, int32_t* new_lengths, int32_t* new_references,
+                                  int32_t* starts, int64_t batch, int64_t blocks, int64_t pages, int64_t page_tokens, int64_t table_stride,
+                                  int64_t new_stride, void* workspace, size_t workspace_bytes, int32_t device, void* stream);
+
+/* Beam search's selection: of all beams and tokens of each request the `keep` largest of scores[r, b] + log_softmax(logits[r, b, :])[t], in falling order,
+ * ties to the lower beam and then the lower token: out_scores, out_parents (r * beams + b) and out_tokens, [requests, keep]. logits are f32, f16 or bf16
+ * with element strides `request_stride` and `beam_stride` and packed tokens, scores packed f32, finished packed bytes or null: a finished beam has one
+ * candidate, `end`, at its score as it is, and -inf for every other token. A beam whose score is -inf, or whose logits all are, has -inf for all its
+ * candidates; one with a NaN or +inf among them, NaN, which counts as the largest. At most 128 beams a request, 65535 in all, 128 kept, 2^24 - 1 tokens. */
+tq_status tq_beam_select_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab, int64_t keep, size_t* bytes);
+tq_status tq_beam_select_launch(tq_dtype dtype, const void* logits, const float* scores, const uint8_t* finished, float* out_scores, int32_t* out_parents,
+                                int32_t* out_tokens, int64_t requests, int64_t beams, int64_t vocab, int64_t keep, int64_t end, int64_t request_stride,
+                                int64_t beam_stride, void* workspace, size_t workspace_bytes, int32_t device, void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Recipes: a compiled graph's launches, replayed by native code                                */

@@ -12,6 +12,11 @@
 // Copying. Source and target pages are given by the host, which is where a cache's pages are handed out; they travel to the kernel as its
 // argument, so nothing is uploaded before it. Bound: HBM (each byte read and written once: 551 MB in 85 us, 6.5 TB/s). Small pages of several
 // layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
+//
+// Advancing. A step of beam search as the books see it, without the host: rows of the table go on from other rows, pages count how many rows have them,
+// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of eight, makes the new table
+// and counts (what its CTAs tell each other goes through memory between cluster barriers); a second kernel copies the pages that it names. Bound: the
+// latency of those barriers and of dependent reads, and the copied pages' bytes.
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -293,6 +298,13 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
   else copy_piece<uint8_t>(to, from, bytes, layers, tensor.layer_stride);
 }
 
+CopyTensor copy_tensor(const tq_paged_tensor& from) {
+  const bool sixteen = aligned_to(from.base, 16) && from.layer_stride % 16 == 0 && from.page_stride % 16 == 0 && from.page_bytes % 16 == 0;
+  const bool four = aligned_to(from.base, 4) && from.layer_stride % 4 == 0 && from.page_stride % 4 == 0 && from.page_bytes % 4 == 0;
+  return {static_cast<char*>(from.base), from.layer_stride, from.page_stride, from.page_bytes, static_cast<int>(from.layers), sixteen ? 16 : four ? 4 : 1,
+          static_cast<int>((from.page_bytes + kCopyBytes - 1) / kCopyBytes), static_cast<int>(from.page_bytes < kCopyBytes ? kCopyBytes / from.page_bytes : 1)};
+}
+
 tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vector<int64_t>& sources, const std::vector<int64_t>& targets, int32_t device,
                      cudaStream_t stream) {
   DeviceScope device_scope(device);
@@ -302,11 +314,8 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
     long long pieces = 0;
     for (; t0 < tensors.size() && p.count < kCopyTensors; ++t0) {
       const tq_paged_tensor& from = tensors[t0];
-      const bool sixteen = aligned_to(from.base, 16) && from.layer_stride % 16 == 0 && from.page_stride % 16 == 0 && from.page_bytes % 16 == 0;
-      const bool four = aligned_to(from.base, 4) && from.layer_stride % 4 == 0 && from.page_stride % 4 == 0 && from.page_bytes % 4 == 0;
       CopyTensor& to = p.tensors[p.count];
-      to = {static_cast<char*>(from.base), from.layer_stride, from.page_stride, from.page_bytes, static_cast<int>(from.layers), sixteen ? 16 : four ? 4 : 1,
-            static_cast<int>((from.page_bytes + kCopyBytes - 1) / kCopyBytes), static_cast<int>(from.page_bytes < kCopyBytes ? kCopyBytes / from.page_bytes : 1)};
+      to = copy_tensor(from);
       const long long more = (from.layers + to.piece_layers - 1) / to.piece_layers * to.layer_pieces;
       if (p.count > 0 && pieces + more >= (1LL << 31)) break;
       pieces += more;
@@ -326,26 +335,316 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
   return TQ_OK;
 }
 
-// log2 of a page's tokens, or -1.
-int page_shift_of(int64_t page_tokens) {
-  for (int shift = 4; shift <= 10; ++shift)
-    if (page_tokens == (1LL << shift)) return shift;
-  return -1;
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kAdvanceThreads = 1024, kAdvanceWarps = kAdvanceThreads / 32, kAdvanceCtas = 8;
+constexpr int kAdvanceSmall = 1 << 14;     // entries and pages that one CTA takes by itself
+
+// Codes of the status word for a step that could not be made: nothing has changed then, and each row starts at -1.
+enum AdvanceFault { kAdvanceFull = 0x46554c4c, kAdvanceParent = 0x50415245 };      // "FULL", "PARE"
+
+struct AdvanceParams {
+  const int32_t *table, *lengths, *references, *counts, *parents;      // parents null: each row goes on
+  long long table_stride, new_stride;
+  int32_t *new_table, *new_lengths, *new_references, *starts;          // results; may be the operands
+  bool same_table, same_lengths, same_references;
+  int batch, blocks, pages, page_shift;
+  // scratch
+  int32_t* rows;                       // same_table: the new rows, packed
+  int32_t* counted;                    // same_references: the new counts
+  int32_t *writers, *final_writer;     // [pages], of the last pages alone
+  int32_t *needs_before, *copies_before;      // [batch]: pages needed, and copies made, by the rows before
+  int32_t* free_pages;                 // the lowest free ones
+  int32_t *sources, *targets;          // of the copies
+  int32_t* totals;                     // {needed, copies, faults, where} and from kAdvanceCtas on the free pages of each CTA's stretch
+};
+constexpr int kTotals = 8 + kAdvanceCtas;
+
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Exclusive sums over the CTA of two numbers a thread; `totals` of all.
+__device__ __forceinline__ int2 sums_before(int2 mine, int2* warp_totals, int2& total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int2 upto = mine;
+#pragma unroll
+  for (int offset = 1; offset < 32; offset *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, upto.x, offset), y = __shfl_up_sync(0xffffffffu, upto.y, offset);
+    if (lane >= offset) {
+      upto.x += x;
+      upto.y += y;
+    }
+  }
+  if (lane == 31) warp_totals[warp] = upto;
+  __syncthreads();
+  if (warp == 0) {
+    int2 all = warp_totals[lane];
+#pragma unroll
+    for (int offset = 1; offset < 32; offset *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, all.x, offset), y = __shfl_up_sync(0xffffffffu, all.y, offset);
+      if (lane >= offset) {
+        all.x += x;
+        all.y += y;
+      }
+    }
+    warp_totals[lane] = all;
+  }
+  __syncthreads();
+  const int2 before = warp == 0 ? make_int2(0, 0) : warp_totals[warp - 1];
+  total = warp_totals[kAdvanceWarps - 1];
+  __syncthreads();
+  return make_int2(upto.x - mine.x + before.x, upto.y - mine.y + before.y);
+}
+
+__global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __grid_constant__ AdvanceParams p, const WaitStatus status) {
+  __shared__ int2 warp_totals[kAdvanceWarps];
+  __shared__ int stretch_free[kAdvanceWarps];
+  wait_for_earlier();
+  const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+  const int thread = cta * kAdvanceThreads + static_cast<int>(threadIdx.x), threads = ctas * kAdvanceThreads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = ctas * kAdvanceWarps, nth_warp = cta * kAdvanceWarps + warp;
+  const int page_tokens = 1 << p.page_shift;
+  int32_t* const rows = p.same_table ? p.rows : p.new_table;
+  const long long row_stride = p.same_table ? p.blocks : p.new_stride;
+  int32_t* const counted = p.same_references ? p.counted : p.new_references;
+  const long long capacity = static_cast<long long>(p.blocks) << p.page_shift;
+  auto fault = [&](int code, int row, int what) {
+    if (atomicCAS(p.totals + 2, 0, code) == 0) p.totals[3] = row;
+    report(status, code, row, what);
+  };
+  auto blocks_of = [&](long long tokens) { return static_cast<int>((tokens + page_tokens - 1) >> p.page_shift); };
+  auto parent_of = [&](int row) { return p.parents == nullptr ? row : p.parents[row]; };
+  auto held = [&](int row) { return row < 0 || row >= p.batch ? 0 : p.lengths[row]; };      // tokens
+  auto in_table = [&](int tokens) { return static_cast<int>(min(static_cast<long long>(max(tokens, 0)), capacity)); };
+
+  if (thread < kTotals) p.totals[thread] = 0;
+  for (int i = thread; i < p.pages; i += threads) counted[i] = p.references[i];
+  for (int row = thread; row < p.batch; row += threads) {
+    const int parent = parent_of(row), start = in_table(held(parent));
+    if (p.counts[row] > 0 && (start & (page_tokens - 1)) != 0) {
+      const int last = p.table[parent * p.table_stride + (start >> p.page_shift)];
+      if (last >= 0 && last < p.pages) {
+        p.writers[last] = 0;
+        p.final_writer[last] = -1;
+      }
+    }
+  }
+  cluster_meet();
+
+  // Rows: the parents' pages, and how many rows have each; a warp a row.
+  for (int row = nth_warp; row < p.batch; row += warps) {
+    const int parent = parent_of(row), own_tokens = held(row), tokens = held(parent), count = p.counts[row];
+    if (lane == 0) {
+      if (parent >= p.batch) fault(kAdvanceParent, row, parent);
+      else if (own_tokens > capacity || tokens > capacity || static_cast<long long>(max(tokens, 0)) + max(count, 0) > capacity) fault(kKeyedLength, row, max(tokens, own_tokens));
+    }
+    const int had = blocks_of(in_table(own_tokens)), has = blocks_of(in_table(tokens));
+    const int32_t* const own = p.table + row * p.table_stride;
+    const int32_t* const from = parent < 0 || parent >= p.batch ? own : p.table + parent * p.table_stride;
+    for (int i = lane; i < p.blocks; i += 32) {
+      const int before = own[i], now = i < has ? from[i] : before;
+      rows[row * row_stride + i] = now;
+      const bool drops = i < had, takes = i < has;
+      if ((drops && (before < 0 || before >= p.pages)) || (takes && (now < 0 || now >= p.pages))) {
+        fault(kKeyedPage, row, i);
+      } else if (drops != takes || before != now) {
+        if (takes) atomicAdd(counted + now, 1);
+        if (drops) atomicAdd(counted + before, -1);
+      }
+    }
+    const int start = in_table(tokens);
+    if (lane == 0 && count > 0 && (start & (page_tokens - 1)) != 0) {
+      const int last = from[start >> p.page_shift];
+      if (last >= 0 && last < p.pages) {
+        atomicAdd(p.writers + last, 1);
+        atomicMax(p.final_writer + last, row);
+      }
+    }
+  }
+  cluster_meet();
+
+  // What each row needs (the first CTA), and where the free pages are (all; a warp has a stretch of pages).
+  auto copies = [&](int row, int start, int count) {      // the row's last page is others' too, and it is not the one that keeps it
+    if (count <= 0 || (start & (page_tokens - 1)) == 0) return -1;
+    const int last = __ldcg(rows + row * row_stride + (start >> p.page_shift));
+    if (last < 0 || last >= p.pages) return -1;
+    return __ldcg(counted + last) > __ldcg(p.writers + last) || __ldcg(p.final_writer + last) != row ? last : -1;
+  };
+  if (cta == 0) {
+    const int run = (p.batch + kAdvanceThreads - 1) / kAdvanceThreads;
+    const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
+    int2 mine = make_int2(0, 0);
+    for (int row = first; row < last; ++row) {
+      const int start = in_table(held(parent_of(row))), count = max(p.counts[row], 0);
+      const int copied = copies(row, start, count) >= 0 ? 1 : 0;
+      p.needs_before[row] = mine.x;      // (within the run so far)
+      p.copies_before[row] = mine.y;
+      mine.x += copied + static_cast<int>(min(static_cast<long long>(blocks_of(static_cast<long long>(start) + count)) - blocks_of(start), 0x3fffffffLL));
+      mine.y += copied;
+    }
+    int2 total;
+    const int2 before = sums_before(mine, warp_totals, total);
+    for (int row = first; row < last; ++row) {
+      p.needs_before[row] += before.x;
+      p.copies_before[row] += before.y;
+    }
+    if (threadIdx.x == 0) {
+      p.totals[0] = total.x;
+      p.totals[1] = total.y;
+    }
+  }
+  const int stretch = ((p.pages + warps - 1) / warps + 31) / 32 * 32;
+  const int page0 = static_cast<int>(min(static_cast<long long>(nth_warp) * stretch, static_cast<long long>(p.pages)));
+  const int page1 = static_cast<int>(min(static_cast<long long>(page0) + stretch, static_cast<long long>(p.pages)));
+  int free_here = 0;
+  for (int page = page0; page < page1; page += 32) {
+    const bool is_free = page + lane < page1 && __ldcg(counted + page + lane) == 0;
+    free_here += __popc(__ballot_sync(0xffffffffu, is_free));
+  }
+  if (lane == 0) stretch_free[warp] = free_here;
+  __syncthreads();
+  int free_before = 0, free_cta = 0;
+  for (int w = 0; w < kAdvanceWarps; ++w) {
+    if (w < warp) free_before += stretch_free[w];
+    free_cta += stretch_free[w];
+  }
+  if (threadIdx.x == 0) p.totals[8 + cta] = free_cta;
+  cluster_meet();
+
+  const int needed = __ldcg(p.totals);
+  int free_all = 0;
+  for (int c = 0; c < ctas; ++c) {
+    const int there = __ldcg(p.totals + 8 + c);
+    if (c < cta) free_before += there;
+    free_all += there;
+  }
+  const int fault_before = __ldcg(p.totals + 2);
+  const bool good = fault_before == 0 && needed <= free_all;
+  if (good) {
+    for (int page = page0; page < page1 && free_before < needed; page += 32) {
+      const bool is_free = page + lane < page1 && __ldcg(counted + page + lane) == 0;
+      const uint32_t free_lanes = __ballot_sync(0xffffffffu, is_free);
+      const int place = free_before + __popc(free_lanes & ((1u << lane) - 1));
+      if (is_free && place < needed) p.free_pages[place] = page + lane;
+      free_before += __popc(free_lanes);
+    }
+  } else if (thread == 0 && fault_before == 0) {
+    report(status, kAdvanceFull, needed, free_all);
+  }
+  cluster_meet();
+
+  // The rows take their pages; a warp a row.
+  for (int row = nth_warp; row < p.batch; row += warps) {
+    const int parent = parent_of(row), start = in_table(held(parent)), count = max(p.counts[row], 0);
+    if (good) {
+      const int has = blocks_of(start), will = blocks_of(static_cast<long long>(start) + count);
+      int at = __ldcg(p.needs_before + row);
+      const int last = copies(row, start, count);
+      __syncwarp();
+      if (last >= 0) {
+        const int page = __ldcg(p.free_pages + at++);
+        if (lane == 0) {
+          const int pair = __ldcg(p.copies_before + row);
+          p.sources[pair] = last;
+          p.targets[pair] = page;
+          rows[row * row_stride + has - 1] = page;
+        }
+      }
+      for (int i = has + lane; i < will; i += 32) rows[row * row_stride + i] = __ldcg(p.free_pages + at + i - has);
+    }
+  }
+  cluster_meet();      // (`counted` and `rows` of last pages are read until here, and lengths of parents)
+  for (int row = nth_warp; row < p.batch; row += warps) {
+    const int parent = parent_of(row), start = in_table(held(parent));
+    if (lane == 0) p.starts[row] = good ? start : -1;
+  }
+  if (good) {
+    for (int i = thread; i < __ldcg(p.totals + 1); i += threads) atomicAdd(counted + __ldcg(p.sources + i), -1);
+    for (int i = thread; i < needed; i += threads) atomicExch(counted + __ldcg(p.free_pages + i), 1);
+  } else if (thread == 0) {
+    p.totals[1] = 0;                      // nothing is copied
+  }
+  cluster_meet();
+  for (int row = thread; row < p.batch; row += threads) {
+    const int start = __ldcg(p.starts + row);
+    if (good) p.new_lengths[row] = start + max(p.counts[row], 0);
+    else if (!p.same_lengths) p.new_lengths[row] = p.lengths[row];
+  }
+  if (good ? p.same_references : !p.same_references)
+    for (int i = thread; i < p.pages; i += threads) p.new_references[i] = good ? __ldcg(counted + i) : p.references[i];
+  if (good ? p.same_table : !p.same_table) {
+    for (int row = nth_warp; row < p.batch; row += warps)
+      for (int i = lane; i < p.blocks; i += 32)
+        p.new_table[row * p.new_stride + i] = good ? __ldcg(rows + row * row_stride + i) : p.table[row * p.table_stride + i];
+  }
+}
+
+struct NamedCopies {
+  CopyTensor tensors[4];
+  int count;
+  const int32_t *sources, *targets, *pairs;      // device memory
+};
+
+// grid: (pieces of all tensors, pairs at once)
+__global__ void __launch_bounds__(kCopyThreads) copy_named_pages_kernel(const __grid_constant__ NamedCopies p) {
+  wait_for_earlier();
+  let_later_start();
+  const int pairs = *p.pairs;
+  if (static_cast<int>(blockIdx.y) >= pairs) return;
+  int piece = static_cast<int>(blockIdx.x), t = 0;
+  auto pieces_of = [&](const CopyTensor& tensor) { return (tensor.layers + tensor.piece_layers - 1) / tensor.piece_layers * tensor.layer_pieces; };
+  while (t + 1 < p.count && piece >= pieces_of(p.tensors[t])) piece -= pieces_of(p.tensors[t++]);
+  const CopyTensor& tensor = p.tensors[t];
+  const int layer = piece / tensor.layer_pieces * tensor.piece_layers;
+  const long long first = static_cast<long long>(piece % tensor.layer_pieces) * kCopyBytes;
+  const int bytes = static_cast<int>(min(tensor.page_bytes - first, static_cast<long long>(kCopyBytes)));
+  const int layers = min(tensor.piece_layers, tensor.layers - layer);
+  char* const base = tensor.base + layer * tensor.layer_stride + first;
+  for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
+    const char* from = base + p.sources[pair] * tensor.page_stride;
+    char* to = base + p.targets[pair] * tensor.page_stride;
+    if (tensor.width == 16) copy_piece<uint4>(to, from, bytes, layers, tensor.layer_stride);
+    else if (tensor.width == 4) copy_piece<uint32_t>(to, from, bytes, layers, tensor.layer_stride);
+    else copy_piece<uint8_t>(to, from, bytes, layers, tensor.layer_stride);
+  }
+}
+
+// Scratch of an advance: where each array begins, in int32.
+struct AdvanceScratch {
+  int64_t rows, counted, writers, final_writer, needs, copies, free_pages, sources, targets, totals, all;
+};
+AdvanceScratch advance_scratch(int64_t batch, int64_t blocks, int64_t pages) {
+  AdvanceScratch at = {};
+  int64_t end = 0;
+  auto take = [&](int64_t count) {
+    const int64_t begin = end;
+    end += (count + 3) / 4 * 4;
+    return begin;
+  };
+  at.rows = take(batch * blocks);
+  at.counted = take(pages);
+  at.writers = take(pages);
+  at.final_writer = take(pages);
+  at.needs = take(batch);
+  at.copies = take(batch);
+  at.free_pages = take(pages);
+  at.sources = take(batch);
+  at.targets = take(batch);
+  at.totals = take(kTotals);
+  at.all = end;
+  return at;
+}
+
+bool advance_takes(int64_t batch, int64_t blocks, int64_t pages, int64_t page_tokens) {
+  const int page_shift = page_shift_of(page_tokens);
+  return batch > 0 && blocks >= 0 && pages >= 0 && page_shift >= 0 && pages < (1LL << 30) && batch < (1LL << 20) && blocks < (1LL << 30) >> page_shift &&
+         batch * blocks < (1LL << 30);
 }
 
 }  // namespace
 }  // namespace tq
-
-#define TQ_CACHE_CHECKS()                                                                                                                          \
-  TQ_REQUIRE(dtype == TQ_BF16 || dtype == TQ_F16, TQ_UNSUPPORTED, "the cache takes and gives bf16 or f16, not %s", tq::dtype_name(dtype));         \
-  TQ_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0, TQ_UNSUPPORTED, "the cache holds heads of 16, 32, ... 128 elements, not %lld", \
-             (long long)head_dim);                                                                                                                 \
-  const int page_shift = tq::page_shift_of(page_tokens);                                                                                           \
-  TQ_REQUIRE(page_shift >= 0, TQ_UNSUPPORTED, "a page holds 16, 32, 64, ... 1024 tokens, not %lld", (long long)page_tokens);                       \
-  TQ_REQUIRE(pages >= 0 && blocks >= 0 && kv_heads >= 0 && batch >= 0, TQ_INVALID_ARGUMENT,                                                        \
-             "negative extent in batch=%lld kv_heads=%lld pages=%lld blocks=%lld", (long long)batch, (long long)kv_heads, (long long)pages, (long long)blocks); \
-  TQ_REQUIRE(pages < (1LL << 31) && kv_heads < 65536 && batch < (1LL << 24) && blocks < (1LL << 30) >> page_shift, TQ_UNSUPPORTED,                    \
-             "extents beyond the kernel's index range")
 
 extern "C" tq_status tq_cache_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim,
                                                         int64_t page_tokens, int64_t blocks, int64_t window, int64_t sinks, int32_t device,
@@ -380,7 +679,8 @@ extern "C" tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, co
                                        page_tokens, blocks, table_stride, kept.q, kept.out, scale, window, sinks, workspace, workspace_bytes, d, s);
     });
   }
-  TQ_CACHE_CHECKS();
+  if (tq_status s = tq::cache_checks(dtype, batch, kv_heads, head_dim, pages, page_tokens, blocks)) return s;
+  const int page_shift = tq::page_shift_of(page_tokens);
   TQ_REQUIRE(heads >= 0 && q_tokens >= 0 && window >= 0 && sinks >= 0, TQ_INVALID_ARGUMENT, "negative heads=%lld, q_tokens=%lld, window=%lld or sinks=%lld",
              (long long)heads, (long long)q_tokens, (long long)window, (long long)sinks);
   if (batch == 0 || heads == 0 || q_tokens == 0) return TQ_OK;
@@ -436,7 +736,8 @@ extern "C" tq_status tq_cache_store_launch(tq_dtype dtype, const void* k, const 
                                    page_tokens, blocks, table_stride, kept.k, kept.v, d, s);
     });
   }
-  TQ_CACHE_CHECKS();
+  if (tq_status s = tq::cache_checks(dtype, batch, kv_heads, head_dim, pages, page_tokens, blocks)) return s;
+  const int page_shift = tq::page_shift_of(page_tokens);
   TQ_REQUIRE(tokens >= 0, TQ_INVALID_ARGUMENT, "negative extent in tokens=%lld", (long long)tokens);
   TQ_REQUIRE(tokens < (1LL << 30), TQ_UNSUPPORTED, "extents beyond the kernel's index range");
   if (batch == 0 || kv_heads == 0 || tokens == 0) return TQ_OK;
@@ -544,4 +845,120 @@ extern "C" tq_status tq_copy_pages_launch(const tq_paged_tensor* tensors, int32_
   } catch (const std::bad_alloc&) {
     return tq::fail(TQ_RESOURCE_EXHAUSTED, "no host memory for %lld pages and %lld pairs", (long long)pages, (long long)pairs);
   }
+}
+
+extern "C" tq_status tq_cache_advance_workspace_bytes(int64_t batch, int64_t blocks, int64_t pages, int64_t page_tokens, size_t* bytes) {
+  TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
+  *bytes = tq::advance_takes(batch, blocks, pages, page_tokens) ? static_cast<size_t>(tq::advance_scratch(batch, blocks, pages).all) * sizeof(int32_t) : 0;
+  return TQ_OK;
+}
+
+extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int32_t count, const int32_t* table, const int32_t* lengths,
+                                             const int32_t* references, const int32_t* counts, const int32_t* parents, int32_t* new_table,
+                                             int32_t* new_lengths, int32_t* new_references, int32_t* starts, int64_t batch, int64_t blocks, int64_t pages,
+                                             int64_t page_tokens, int64_t table_stride, int64_t new_stride, void* workspace, size_t workspace_bytes,
+                                             int32_t device, void* stream) {
+  TQ_REQUIRE(count >= 0 && count <= 4 && (count == 0 || tensors != nullptr), TQ_INVALID_ARGUMENT, "%d tensors of pages, not up to 4", count);
+  if (tq::recording()) {
+    struct Kept { tq_paged_tensor tensors[4]; } kept = {};
+    for (int i = 0; i < count; ++i) kept.tensors[i] = tensors[i];
+    return tq::record([=](int32_t d, void* s) {
+      return tq_cache_advance_launch(kept.tensors, count, table, lengths, references, counts, parents, new_table, new_lengths, new_references, starts, batch,
+                                     blocks, pages, page_tokens, table_stride, new_stride, workspace, workspace_bytes, d, s);
+    });
+  }
+  TQ_REQUIRE(batch >= 0 && blocks >= 0 && pages >= 0, TQ_INVALID_ARGUMENT, "negative extent in batch=%lld blocks=%lld pages=%lld", (long long)batch,
+             (long long)blocks, (long long)pages);
+  TQ_REQUIRE(tq::page_shift_of(page_tokens) >= 0, TQ_UNSUPPORTED, "a page holds 16, 32, 64, ... 1024 tokens, not %lld", (long long)page_tokens);
+  if (batch == 0) {
+    TQ_REQUIRE(pages == 0 || references == new_references, TQ_UNSUPPORTED, "a table of no rows advances in place alone");
+    return TQ_OK;
+  }
+  TQ_REQUIRE(tq::advance_takes(batch, blocks, pages, page_tokens), TQ_UNSUPPORTED, "extents beyond the kernel's index range");
+  TQ_REQUIRE(lengths != nullptr && counts != nullptr && new_lengths != nullptr && starts != nullptr && (blocks == 0 || (table != nullptr && new_table != nullptr)) &&
+                 (pages == 0 || (references != nullptr && new_references != nullptr)),
+             TQ_INVALID_ARGUMENT, "null operand or result");
+  TQ_REQUIRE(table_stride >= blocks || batch == 1, TQ_INVALID_ARGUMENT, "the table's rows overlap");
+  TQ_REQUIRE(new_stride >= blocks || batch == 1, TQ_INVALID_ARGUMENT, "the new table's rows overlap");
+  TQ_REQUIRE(new_table != table || new_stride == table_stride || batch == 1, TQ_INVALID_ARGUMENT, "a table in place has one stride");
+  for (const void* each : {static_cast<const void*>(table), static_cast<const void*>(lengths), static_cast<const void*>(references),
+                           static_cast<const void*>(counts), static_cast<const void*>(parents), static_cast<const void*>(new_table),
+                           static_cast<const void*>(new_lengths), static_cast<const void*>(new_references), static_cast<const void*>(starts)})
+    TQ_REQUIRE(tq::aligned_to(each, 4), TQ_UNSUPPORTED, "the books' tensors must be 4-byte aligned");
+  const tq::AdvanceScratch at = tq::advance_scratch(batch, blocks, pages);
+  TQ_REQUIRE(workspace != nullptr && workspace_bytes >= static_cast<size_t>(at.all) * sizeof(int32_t) && tq::aligned_to(workspace, 16), TQ_INVALID_ARGUMENT,
+             "this advance needs %zu bytes of workspace, 16-byte aligned, and was given %zu", static_cast<size_t>(at.all) * sizeof(int32_t), workspace_bytes);
+  tq::NamedCopies copies = {};
+  long long pieces = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    const tq_paged_tensor& t = tensors[i];
+    TQ_REQUIRE(t.layers >= 0 && t.page_bytes >= 0 && t.layer_stride >= 0 && t.page_stride >= 0, TQ_INVALID_ARGUMENT, "negative extent of tensor %d", i);
+    if (t.layers == 0 || t.page_bytes == 0) continue;
+    TQ_REQUIRE(t.base != nullptr, TQ_INVALID_ARGUMENT, "tensor %d is null", i);
+    TQ_REQUIRE(t.page_stride >= t.page_bytes, TQ_INVALID_ARGUMENT, "the pages of tensor %d overlap", i);
+    TQ_REQUIRE(t.layers <= 65535 && t.page_bytes < (1LL << 34) && t.layers * ((t.page_bytes + tq::kCopyBytes - 1) / tq::kCopyBytes) < (1LL << 29),
+               TQ_UNSUPPORTED, "extents beyond the kernel's index range");
+    tq::CopyTensor& to = copies.tensors[copies.count++];
+    to = tq::copy_tensor(t);
+    pieces += (to.layers + to.piece_layers - 1) / to.piece_layers * static_cast<long long>(to.layer_pieces);
+  }
+  tq::DeviceScope device_scope(device);
+  if (tq_status s = device_scope.status()) return s;
+  const tq::WaitStatus status = tq::wait_status_for(device);
+  TQ_REQUIRE(status.abort != nullptr, TQ_RESOURCE_EXHAUSTED, "no device memory for the status word");
+  int32_t* const scratch = static_cast<int32_t*>(workspace);
+  tq::AdvanceParams p = {};
+  p.table = table;
+  p.lengths = lengths;
+  p.references = references;
+  p.counts = counts;
+  p.parents = parents;
+  p.table_stride = table_stride;
+  p.new_stride = new_stride;
+  p.new_table = new_table;
+  p.new_lengths = new_lengths;
+  p.new_references = new_references;
+  p.starts = starts;
+  p.same_table = new_table == table;
+  p.same_lengths = new_lengths == lengths;
+  p.same_references = new_references == references;
+  p.batch = static_cast<int>(batch);
+  p.blocks = static_cast<int>(blocks);
+  p.pages = static_cast<int>(pages);
+  p.page_shift = tq::page_shift_of(page_tokens);
+  p.rows = scratch + at.rows;
+  p.counted = scratch + at.counted;
+  p.writers = scratch + at.writers;
+  p.final_writer = scratch + at.final_writer;
+  p.needs_before = scratch + at.needs;
+  p.copies_before = scratch + at.copies;
+  p.free_pages = scratch + at.free_pages;
+  p.sources = scratch + at.sources;
+  p.targets = scratch + at.targets;
+  p.totals = scratch + at.totals;
+  cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
+  const auto held = tq::hold_scratch(workspace);
+  const unsigned ctas = batch * blocks + pages <= tq::kAdvanceSmall ? 1 : tq::kAdvanceCtas;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(tq::kAdvanceThreads);
+  config.stream = cuda_stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = ctas;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  TQ_CUDA(cudaLaunchKernelEx(&config, tq::cache_advance_kernel, p, status));
+  if (tq_status s = tq::check_launch("cache_advance_kernel")) return s;
+  if (copies.count == 0) return TQ_OK;
+  copies.sources = p.sources;
+  copies.targets = p.targets;
+  copies.pairs = p.totals + 1;
+  const long long at_once = tq::sm_count(device) * 8LL / pieces;
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(at_once < 1 ? 1 : at_once < batch ? at_once : batch));
+  TQ_CUDA(tq::launch_overlapped(tq::copy_named_pages_kernel, grid, tq::kCopyThreads, 0, cuda_stream, copies));
+  return tq::check_launch("copy_named_pages_kernel");
 }

@@ -60,10 +60,8 @@ constexpr uint32_t kStageBytes = 8192;
 constexpr uint32_t kWarpRing = kKeyedStages * kStageBytes;
 constexpr int kWaitKeyed = 0x4b455931;      // "KEY1"
 constexpr float kSlack = 8.f;
-// Probabilities that are rounded to f16 are taken 2^kLift times as large, which cancels in the quotient: 2^(kSlack + kLift) is the largest then, inside
-// f16's 2^16, and those that fall under its normal range, 2^-14, are under 2^-21 of the row's largest.
 template <typename M>
-constexpr float kLift = std::is_same_v<M, __half> ? 7.f : 0.f;
+constexpr float kLift = std::is_same_v<M, __half> ? kHalfLift : 0.f;
 
 // BITS of a key element, W: the head's elements, rounded up to 64 or 128.
 template <int BITS, int W>
@@ -189,7 +187,7 @@ __device__ __forceinline__ ChunkList chunks_of(int low, int high, int window, in
 
 // Eight elements of a result row: the gathered values over their sum, zeros for a query before the first key.
 template <typename T>
-__device__ __forceinline__ void write_result(const KeyedParams& p, int batch, int kv_head, int row, int column, int length, float total, const float (&value)[8]) {
+__device__ __forceinline__ void write_values(const KeyedParams& p, int batch, int kv_head, int row, int column, int length, float total, const float (&value)[8]) {
   const int token = row / p.group, head = kv_head * p.group + row % p.group;
   const bool sees_some = length - p.q_tokens + token >= 0;
   T* to = static_cast<T*>(p.out) + batch * p.out_strides[0] + head * p.out_strides[1] + token * p.out_strides[2] + column;
@@ -205,15 +203,58 @@ __device__ __forceinline__ void write_result(const KeyedParams& p, int batch, in
   }
 }
 
+// PREFIX: joined with the parts of the keys that the sequence shares with its run.
+template <typename T, int W, bool PREFIX>
+__device__ __forceinline__ void write_result(const KeyedParams& p, int batch, int kv_head, int row, int column, int length, float most, float total,
+                                             const float (&value)[8]) {
+  if constexpr (!PREFIX) {
+    write_values<T>(p, batch, kv_head, row, column, length, total, value);
+  } else {
+    const int run = batch / p.each, shared = shared_keys(p, run);
+    float joined[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) joined[c] = value[c];
+    if (shared > 0 && takes_part(p, shared, length)) {
+      const int inside = (batch - run * p.each) * p.group * p.q_tokens + row, block = inside / p.prefix_rows;
+      const long long slot0 = static_cast<long long>((run * p.kv_heads + kv_head) * p.row_blocks + block) * p.splits;
+#pragma unroll 2
+      for (int part = 0; part < p.splits; ++part) {
+        const long long slot = (slot0 + part) * p.prefix_rows + (inside - block * p.prefix_rows);
+        const float2 stats = p.prefix_stats[slot];
+        if (stats.x == -INFINITY) continue;      // no keys (what lies there is nothing then)
+        const float4* from = reinterpret_cast<const float4*>(p.prefix_parts + slot * W + column);
+        const float4 near = from[0], far = from[1];
+        const float both = fmaxf(most, stats.x), mine = rescale(most, both), theirs = rescale(stats.x, both);
+        const float x[8] = {near.x, near.y, near.z, near.w, far.x, far.y, far.z, far.w};
+        most = both;
+        total = total * mine + stats.y * theirs;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) joined[c] = joined[c] * mine + x[c] * theirs;
+      }
+    }
+    write_values<T>(p, batch, kv_head, row, column, length, total, joined);
+  }
+}
+
 // A sequence's chunks, by every query of it.
 template <int BITS, int CHUNK>
 __device__ __forceinline__ int length_of(const KeyedParams& p, int sequence) {
   if constexpr (BITS == 16) return p.k_tokens;
   return min(max(p.lengths[sequence], 0), p.blocks << p.page_shift);
 }
-template <int BITS, int CHUNK>
-__device__ __forceinline__ ChunkList sequence_chunks(const KeyedParams& p, int length) {
-  return chunks_of(length - p.q_tokens, max(length - 1, -1), p.window, p.sinks, CHUNK);
+// PREFIX: a list without the keys that the sequence shares with its run.
+template <int CHUNK, bool PREFIX>
+__device__ __forceinline__ ChunkList behind_prefix(const KeyedParams& p, int sequence, int length, ChunkList list) {
+  if constexpr (PREFIX) {
+    static_assert(kPrefixTile % CHUNK == 0, "the keys behind the shared ones begin with a chunk");
+    const int shared = shared_keys(p, sequence / p.each);
+    if (takes_part(p, shared, length)) list.start = min(max(list.start, shared / CHUNK), list.stop);
+  }
+  return list;
+}
+template <int BITS, int CHUNK, bool PREFIX>
+__device__ __forceinline__ ChunkList sequence_chunks(const KeyedParams& p, int sequence, int length) {
+  return behind_prefix<CHUNK, PREFIX>(p, sequence, length, chunks_of(length - p.q_tokens, max(length - 1, -1), p.window, p.sinks, CHUNK));
 }
 
 // Where the chunks of all units (sequence, key head, tile of rows) are dealt out as one range of equal shares, a CTA each: a place in that range.
@@ -223,9 +264,9 @@ struct Place {
 };
 
 // The chunks that a head of sequence `sequence` counts for: one at least, so that each has somebody to write its result.
-template <int BITS, int CHUNK>
+template <int BITS, int CHUNK, bool PREFIX>
 __device__ __forceinline__ int counted(const KeyedParams& p, int sequence) {
-  return max(sequence_chunks<BITS, CHUNK>(p, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
+  return max(sequence_chunks<BITS, CHUNK, PREFIX>(p, sequence, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
 }
 
 // What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another, and its masked ends. Measured with
@@ -246,14 +287,14 @@ struct Dealt {
 };
 
 // All threads: the range, and where in it the share of each warp, first_share + warp, starts. Each thread adds up a run of sequences.
-template <int BITS, int CHUNK>
+template <int BITS, int CHUNK, bool PREFIX>
 __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Place& place) {
   __shared__ int warp_sum_of[kKeyedWarps];
   __shared__ Place found[kKeyedWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int units = p.kv_heads * p.row_tiles;
   if constexpr (BITS == 16) {      // all sequences are alike
-    const int each = (unit_cost(CHUNK) + counted<BITS, CHUNK>(p, 0)) * units;
+    const int each = (unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, 0)) * units;
     Dealt dealt;
     dealt.total = each * p.batch;
     dealt.shares = min(p.shares, (dealt.total + kLeastShare - 1) / kLeastShare);
@@ -266,7 +307,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   const int run = (p.batch + kKeyedThreads - 1) / kKeyedThreads;
   const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
   int mine = 0;
-  for (int b = first; b < last; ++b) mine += unit_cost(CHUNK) + counted<BITS, CHUNK>(p, b);
+  for (int b = first; b < last; ++b) mine += unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, b);
   mine *= units;
   int upto = mine;
 #pragma unroll
@@ -294,7 +335,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
     if (before <= at && at < upto) {
       int b = first;
       for (; b < last; ++b) {
-        const int here = (unit_cost(CHUNK) + counted<BITS, CHUNK>(p, b)) * units;
+        const int here = (unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, b)) * units;
         if (at < before + here) break;
         before += here;
       }
@@ -309,7 +350,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal
 // shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every WARPS-th chunk each and meet in shared
 // memory. ONE: a chunk lies in one page (or in none: dense keys).
-template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps>
+template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps, bool PREFIX = false>
 __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
@@ -362,7 +403,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   int at = 0, until = 1;
   Dealt dealt = {};
   if constexpr (SHARED) {
-    dealt = deal<BITS, S::kKeys>(p, blockIdx.x * kKeyedWarps, place);
+    dealt = deal<BITS, S::kKeys, PREFIX>(p, blockIdx.x * kKeyedWarps, place);
     if (lane == 0) p.borders[share] = make_int4(0, 0, 0, 0);               // (the border behind this share; see below)
     if (share < dealt.shares) {
       at = dealt.start(share);
@@ -380,7 +421,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if constexpr (SHARED) {
       batch = place.sequence;
       counted_length = length_of<BITS, S::kKeys>(p, batch);
-      list = sequence_chunks<BITS, S::kKeys>(p, counted_length);
+      list = sequence_chunks<BITS, S::kKeys, PREFIX>(p, batch, counted_length);
       const int cost = kUnitCost + max(list.count(), 1), units = p.kv_heads * p.row_tiles;
       const int inside = at - place.before;
       const int unit = inside / cost;
@@ -418,7 +459,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int first_token = row0 / p.group, last_token = (min(row0 + kRows, rows) - 1) / p.group;
     const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
     if constexpr (!SHARED) {
-      list = chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys);
+      list = behind_prefix<S::kKeys, PREFIX>(p, batch, length, chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys));
       last_chunk = list.count();
     }
 
@@ -956,7 +997,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const int column = column_of(run);
             if (column >= p.head_dim) continue;
             if (whole) {
-              write_result<T>(p, batch, kv_head, row0 + row, column, length, sum[n][e], value);
+              write_result<T, W, PREFIX>(p, batch, kv_head, row0 + row, column, length, top[n][e], sum[n][e], value);
             } else {
               float4* to = reinterpret_cast<float4*>((JOINS > 1 ? piece_at(warp, begins ? 1 : 0) + row * W : p.parts + (slot0 + row) * W) + column);
               to[0] = make_float4(value[0], value[1], value[2], value[3]);
@@ -1000,7 +1041,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
           for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
         }
-        write_result<T>(p, batch, kv_head, row0 + row, column, length, total, value);
+        write_result<T, W, PREFIX>(p, batch, kv_head, row0 + row, column, length, most, total, value);
       }
     }
   }
@@ -1047,7 +1088,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           for (int c = 0; c < 8; ++c) value[c] = value[c] * mine + x[c] * theirs;
         }
         if (whole) {
-          write_result<T>(p, head.sequence, kv_head, tile * kRows + row, column, length_of<BITS, S::kKeys>(p, head.sequence), total, value);
+          write_result<T, W, PREFIX>(p, head.sequence, kv_head, tile * kRows + row, column, length_of<BITS, S::kKeys>(p, head.sequence), most, total, value);
         } else {
           float4* to = reinterpret_cast<float4*>(p.parts + (slot0 + row) * W + column);
           to[0] = make_float4(value[0], value[1], value[2], value[3]);
@@ -1063,7 +1104,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 // SHARED: joins the parts of the units that a border between two shares (or two CTAs' shares: JOINS of them) cut. A CTA for each border; the CTAs
 // of a unit's borders split its result, 64 elements of a row at a time: eight lanes of eight elements, by as many groups as there are parts, four
 // groups in a warp or, of many parts, sixteen in the CTA.
-template <typename T, int W, int NT, int JOINS>
+template <typename T, int W, int NT, int JOINS, bool PREFIX = false>
 __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_constant__ KeyedParams p) {
   constexpr int kRows = 8 * NT;
   __shared__ float2 warp_stats[kKeyedWarps][8];
@@ -1157,7 +1198,7 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
         }
       }
       if (item < items && lane < 8 && (!many || warp == 0) && column < p.head_dim)
-        write_result<T>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, total[i], value[i]);
+        write_result<T, W, PREFIX>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, most[i], total[i], value[i]);
     }
   }
 }
@@ -1299,7 +1340,7 @@ tq_status keyed_maps(CUtensorMap* maps, KeyedParams& p) {
   return TQ_OK;
 }
 
-template <typename T, int BITS, int W, int NT>
+template <typename T, int BITS, int W, int NT, bool PREFIX>
 tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   CUtensorMap maps[2] = {};
   if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
@@ -1312,9 +1353,9 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   auto start_boxes = [&](auto joins, auto each, long long ctas) {
     constexpr int kJoins = decltype(joins)::value, kWarps = decltype(each)::value;
     if constexpr (BITS == 8) {
-      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false, kWarps>, kWarps, ctas);
+      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false, kWarps, PREFIX>, kWarps, ctas);
     }
-    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true, kWarps>, kWarps, ctas);
+    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true, kWarps, PREFIX>, kWarps, ctas);
   };
   constexpr std::integral_constant<int, 0> kWhole{};
   constexpr std::integral_constant<int, kKeyedWarps> kFour{};
@@ -1325,18 +1366,20 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
                                                                                               : start_boxes(kWhole, std::integral_constant<int, 8>{}, units);
   }
   const bool gathers = p.joins > 1;
-  const auto held = hold_scratch(p.borders);      // both launches, one after the other: recorded ones may share their scratch on a stream
+  // both launches, one after the other: recorded ones may share their scratch on a stream (behind prefix.cu's kernel its caller holds it)
+  const auto held = hold_scratch(PREFIX ? nullptr : p.borders);
   if (tq_status s = gathers ? start_boxes(kFour, kFour, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, kFour, p.shares / kKeyedWarps)) return s;
   const dim3 borders(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
-  TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps>, borders, kKeyedThreads, 0, stream, p)
-                  : launch_overlapped(keyed_join_kernel<T, W, NT, 1>, borders, kKeyedThreads, 0, stream, p));
+  TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps, PREFIX>, borders, kKeyedThreads, 0, stream, p)
+                  : launch_overlapped(keyed_join_kernel<T, W, NT, 1, PREFIX>, borders, kKeyedThreads, 0, stream, p));
   return check_launch("keyed_join_kernel");
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool PREFIX = false>
 tq_status launch_keyed_width(KeyedParams& p, const KeyedPlan& plan, cudaStream_t stream) {
-  if (p.head_dim <= 64) return plan.nt == 1 ? launch_keyed<T, BITS, 64, 1>(p, plan.warps, stream) : launch_keyed<T, BITS, 64, 2>(p, plan.warps, stream);
-  return plan.nt == 1 ? launch_keyed<T, BITS, 128, 1>(p, plan.warps, stream) : launch_keyed<T, BITS, 128, 2>(p, plan.warps, stream);
+  if (p.head_dim <= 64)
+    return plan.nt == 1 ? launch_keyed<T, BITS, 64, 1, PREFIX>(p, plan.warps, stream) : launch_keyed<T, BITS, 64, 2, PREFIX>(p, plan.warps, stream);
+  return plan.nt == 1 ? launch_keyed<T, BITS, 128, 1, PREFIX>(p, plan.warps, stream) : launch_keyed<T, BITS, 128, 2, PREFIX>(p, plan.warps, stream);
 }
 
 }  // namespace
@@ -1355,6 +1398,7 @@ tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long 
   p.borders = static_cast<int4*>(workspace);
   p.part_stats = reinterpret_cast<float2*>(p.borders + plan.shares);
   p.parts = reinterpret_cast<float*>(p.part_stats + slots);
+  if (p.shared != nullptr) return dtype == TQ_BF16 ? launch_keyed_width<__nv_bfloat16, 8, true>(p, plan, stream) : launch_keyed_width<__half, 8, true>(p, plan, stream);
   if (dtype == TQ_BF16) return paged ? launch_keyed_width<__nv_bfloat16, 8>(p, plan, stream) : launch_keyed_width<__nv_bfloat16, 16>(p, plan, stream);
   return paged ? launch_keyed_width<__half, 8>(p, plan, stream) : launch_keyed_width<__half, 16>(p, plan, stream);
 }

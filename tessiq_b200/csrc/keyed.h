@@ -26,9 +26,38 @@ struct KeyedParams {
   float2* part_stats;                                                      // ... their maximum and sum
   float scale_log2;
   WaitStatus status;
+  // Sequences in runs of `each` that share their first keys, whose part of the result prefix.cu leaves (null: none do).
+  const int32_t* shared;                                                   // of each run: how many first keys its sequences have in common
+  int each, prefix_rows, row_blocks, splits;                               // rows of a block, blocks of a run and key head, parts of each
+  float* prefix_parts;                                                     // [run][key head][block][part][row][64 or 128]
+  float2* prefix_stats;                                                    // ... their maximum and sum
 };
 
+// The keys of a run's beginning are taken together in tiles of so many; what is left of it each sequence reads itself.
+constexpr int kPrefixTile = 128;
+
 constexpr double kKeyedMostScale = 2e38;      // times log2(e) it still is an f32
+
+// log2 of a page's tokens, or -1.
+inline int page_shift_of(int64_t page_tokens) {
+  for (int shift = 4; shift <= 10; ++shift)
+    if (page_tokens == (1LL << shift)) return shift;
+  return -1;
+}
+
+// What every call over the cache checks of it first.
+inline tq_status cache_checks(tq_dtype dtype, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_tokens, int64_t blocks) {
+  TQ_REQUIRE(dtype == TQ_BF16 || dtype == TQ_F16, TQ_UNSUPPORTED, "the cache takes and gives bf16 or f16, not %s", dtype_name(dtype));
+  TQ_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0, TQ_UNSUPPORTED, "the cache holds heads of 16, 32, ... 128 elements, not %lld",
+             (long long)head_dim);
+  const int page_shift = page_shift_of(page_tokens);
+  TQ_REQUIRE(page_shift >= 0, TQ_UNSUPPORTED, "a page holds 16, 32, 64, ... 1024 tokens, not %lld", (long long)page_tokens);
+  TQ_REQUIRE(pages >= 0 && blocks >= 0 && kv_heads >= 0 && batch >= 0, TQ_INVALID_ARGUMENT,
+             "negative extent in batch=%lld kv_heads=%lld pages=%lld blocks=%lld", (long long)batch, (long long)kv_heads, (long long)pages, (long long)blocks);
+  TQ_REQUIRE(pages < (1LL << 31) && kv_heads < 65536 && batch < (1LL << 24) && blocks < (1LL << 30) >> page_shift, TQ_UNSUPPORTED,
+             "extents beyond the kernel's index range");
+  return TQ_OK;
+}
 
 // What queries and results have to be: read 16 bytes at a time, written through any strides.
 inline bool keyed_query_fits(const void* q, const int64_t* q_strides, const void* out, const int64_t* out_strides, int64_t batch, int64_t heads,
@@ -52,7 +81,12 @@ inline void keyed_extents(KeyedParams& p, int64_t batch, int64_t heads, int64_t 
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
 }
 
-// Few rows a key head against many keys: `p` is complete but for what follows from the plan; no sequence has more than `keys` keys.
+// Probabilities that are rounded to f16 are taken 2^kHalfLift times as large, which cancels in the quotient: 2^(kSlack + kHalfLift) is the largest then,
+// inside f16's 2^16, and those that fall under its normal range, 2^-14, are under 2^-21 of the row's largest.
+constexpr float kHalfLift = 7.f;
+
+// Few rows a key head against many keys: `p` is complete but for what follows from the plan; no sequence has more than `keys` keys. With `p.shared`
+// (paged keys, no window): the keys behind the shared ones, joined with what prefix.cu has left in p.prefix_parts.
 size_t keyed_workspace(bool paged, const KeyedParams& p, long long keys, int32_t device);
 tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long keys, void* workspace, size_t workspace_bytes, int32_t device,
                           cudaStream_t stream);
@@ -80,6 +114,12 @@ cudaError_t launch_overlapped(void (*kernel)(Parameters...), dim3 grid, unsigned
 }
 __device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_later_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// How many of a sequence's first keys are taken together with those of its run: whole tiles, and only if all of its queries see them all.
+__device__ __forceinline__ int shared_keys(const KeyedParams& p, int run) {
+  return min(max(p.shared[run], 0), p.blocks << p.page_shift) / kPrefixTile * kPrefixTile;
+}
+__device__ __forceinline__ bool takes_part(const KeyedParams& p, int shared, int length) { return length - p.q_tokens + 1 >= shared; }
 
 // The first fault since the last poll is kept, with where it was.
 __device__ __forceinline__ void report(const WaitStatus& status, int code, int sequence, int what) {

@@ -36,7 +36,8 @@
 
 namespace {
 
-enum Family { kFused, kReduce, kPack, kSoftmax, kLayerNorm, kTransposed, kBatchNorm, kGemm, kAttention, kWindow, kCacheAttention, kCacheStore, kFamilies };
+enum Family { kFused, kReduce, kPack, kSoftmax, kLayerNorm, kTransposed, kBatchNorm, kGemm, kAttention, kWindow, kCacheAttention, kCacheStore,
+              kPrefixAttention, kBeamSelect, kCacheAdvance, kFamilies };
 
 // The library's entry points.
 struct Library {
@@ -54,6 +55,9 @@ struct Library {
   decltype(&tq_cache_attention_launch) cache_attention_launch = nullptr;
   decltype(&tq_cache_store_launch) cache_store_launch = nullptr;
   decltype(&tq_copy_pages_launch) copy_pages_launch = nullptr;
+  decltype(&tq_prefix_attention_launch) prefix_attention_launch = nullptr;
+  decltype(&tq_beam_select_launch) beam_select_launch = nullptr;
+  decltype(&tq_cache_advance_launch) cache_advance_launch = nullptr;
   decltype(&tq_is_recording) is_recording = nullptr;
 } library;
 
@@ -238,6 +242,7 @@ tq_status launch(const Plan& p, const Call& call, const std::vector<at::Tensor>&
   const int64_t* n = p.ints.data();
   const int32_t device = call.device;
   auto small = [&](int i) { return static_cast<int32_t>(n[i]); };
+  auto written = [&](int i) -> void* { return i < call.tensor_count && call.tensors[i] != nullptr ? call.tensors[i]->mutable_data_ptr() : nullptr; };
   switch (p.family) {
     case kFused: {
       const void* inputs[kMostOperands];
@@ -277,10 +282,28 @@ tq_status launch(const Plan& p, const Call& call, const std::vector<at::Tensor>&
                                        result(0), n[1], n[2], n[3], n[4], n[5], n[6], n[7], n[8], n[9], n + 10, n + 13, p.doubles[0], n[16], n[17], scratch,
                                        scratch_bytes, device, stream);
     case kCacheStore: {
-      auto written = [&](int i) -> void* { return i < call.tensor_count && call.tensors[i] != nullptr ? call.tensors[i]->mutable_data_ptr() : nullptr; };
       return library.cache_store_launch(small(0), pointer(0), pointer(1), written(2), written(3), static_cast<float*>(written(4)), static_cast<float*>(written(5)),
                                    static_cast<const int32_t*>(pointer(6)), static_cast<const int32_t*>(pointer(7)), static_cast<const int32_t*>(pointer(8)), n[1],
                                    n[2], n[3], n[4], n[5], n[6], n[7], n[8], n + 9, n + 12, device, stream);
+    }
+    case kPrefixAttention:
+      return library.prefix_attention_launch(small(0), pointer(0), pointer(1), pointer(2), static_cast<const float*>(pointer(3)),
+                                        static_cast<const float*>(pointer(4)), static_cast<const int32_t*>(pointer(5)), static_cast<const int32_t*>(pointer(6)),
+                                        static_cast<const int32_t*>(pointer(7)), result(0), n[1], n[2], n[3], n[4], n[5], n[6], n[7], n[8], n[9], n[10], n + 11,
+                                        n + 14, p.doubles[0], scratch, scratch_bytes, device, stream);
+    case kBeamSelect:
+      return library.beam_select_launch(small(0), pointer(0), static_cast<const float*>(pointer(1)), static_cast<const uint8_t*>(pointer(2)),
+                                   static_cast<float*>(result(0)), static_cast<int32_t*>(result(1)), static_cast<int32_t*>(result(2)), n[1], n[2], n[3], n[4],
+                                   n[5], n[6], n[7], scratch, scratch_bytes, device, stream);
+    case kCacheAdvance: {
+      tq_paged_tensor tensors[4];
+      for (int i = 0; i < 4; ++i) tensors[i] = {written(i), n[4 * i], n[4 * i + 1], n[4 * i + 2], n[4 * i + 3]};
+      const bool in_place = n[22] != 0;
+      auto changed = [&](int operand, size_t output) { return static_cast<int32_t*>(in_place ? written(operand) : result(output)); };
+      return library.cache_advance_launch(tensors, 4, static_cast<const int32_t*>(pointer(4)), static_cast<const int32_t*>(pointer(5)),
+                                     static_cast<const int32_t*>(pointer(6)), static_cast<const int32_t*>(pointer(7)), static_cast<const int32_t*>(pointer(8)),
+                                     changed(4, 1), changed(5, 2), changed(6, 3), static_cast<int32_t*>(result(0)), n[16], n[17], n[18], n[19], n[20], n[21],
+                                     scratch, scratch_bytes, device, stream);
     }
     case kFamilies:
       break;
@@ -314,7 +337,8 @@ PyObject* run(PyObject* const* values, Py_ssize_t count, bool by_type) {
     scratch_bytes = static_cast<size_t>(t.numel());
   }
   // scratch of the call's own, so that calls on other streams and captured graphs never share it; torch's allocator orders its reuse
-  const int64_t own = plan->family == kWindow ? plan->ints[21] : plan->family == kCacheAttention ? plan->ints[18] : 0;
+  const int64_t own = plan->family == kWindow ? plan->ints[21] : plan->family == kCacheAttention ? plan->ints[18] : plan->family == kPrefixAttention ? plan->ints[17]
+                      : plan->family == kBeamSelect ? plan->ints[8] : plan->family == kCacheAdvance ? plan->ints[23] : 0;
   if (own > 0 && library.is_recording()) Py_RETURN_NONE;      // (a recorded launch keeps the address: the long way has a block that stays)
   std::vector<at::Tensor> out;
   tq_status status;
@@ -393,13 +417,13 @@ PyObject* keep(PyObject*, PyObject* args) {
   if (PyErr_Occurred()) return nullptr;
   // Behind the operands that `launch` reads come numbers, whose values the key holds, unless a number came as a tensor: the long way
   // read its value, of which the key has nothing.
-  const Py_ssize_t operands_of[] = {kMostOperands, 1, 1, 1, 3, plan->ints.size() > 0 && plan->ints[0] == 0 ? 1 : 3, 5, 4, 3, 3, 7, 9};
+  const Py_ssize_t operands_of[] = {kMostOperands, 1, 1, 1, 3, plan->ints.size() > 0 && plan->ints[0] == 0 ? 1 : 3, 5, 4, 3, 3, 7, 9, 8, 4, 9};
   for (Py_ssize_t i = operands_of[family]; i < PyTuple_GET_SIZE(operands); ++i)
     if (THPVariable_Check(PyTuple_GET_ITEM(operands, i))) Py_RETURN_FALSE;
   // what `launch` reads of each family
-  const size_t least[] = {2, 6, 2, 5, 4, 6, 5, 12, 19, 22, 19, 15};
+  const size_t least[] = {2, 6, 2, 5, 4, 6, 5, 12, 19, 22, 19, 15, 18, 9, 24};
   const bool has_double = family == kLayerNorm || family == kTransposed || family == kBatchNorm || family == kAttention || family == kWindow ||
-                          family == kCacheAttention;
+                          family == kCacheAttention || family == kPrefixAttention;
   if (plan->ints.size() < least[family] || (has_double && plan->doubles.empty()) ||
       (family == kPack && plan->ints.size() < 2 + 2 * static_cast<size_t>(plan->ints[1])))
     Py_RETURN_FALSE;
@@ -447,7 +471,10 @@ PyObject* setup(PyObject*, PyObject* args) {
         find_entry(handle, "tq_window_attention_launch", library.window_attention_launch) &&
         find_entry(handle, "tq_cache_attention_launch", library.cache_attention_launch) &&
         find_entry(handle, "tq_cache_store_launch", library.cache_store_launch) &&
-        find_entry(handle, "tq_copy_pages_launch", library.copy_pages_launch) && find_entry(handle, "tq_is_recording", library.is_recording))) {
+        find_entry(handle, "tq_copy_pages_launch", library.copy_pages_launch) &&
+        find_entry(handle, "tq_prefix_attention_launch", library.prefix_attention_launch) &&
+        find_entry(handle, "tq_beam_select_launch", library.beam_select_launch) &&
+        find_entry(handle, "tq_cache_advance_launch", library.cache_advance_launch) && find_entry(handle, "tq_is_recording", library.is_recording))) {
     PyErr_Format(PyExc_ImportError, "%s: %s", path, dlerror());
     return nullptr;
   }

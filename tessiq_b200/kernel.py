@@ -369,6 +369,7 @@ _WAIT_CODES = {0x53454c46: "the bounded-wait self test", 0x504e4c31: "panel norm
                0x504e4c36: "panel normalisation: a statistics buffer was never handed back", 0x504e4c37: "panel normalisation: statistics never reached shared memory",
                0x504e4c38: "panel normalisation: the second visit never caught up", 0x504e4c39: "panel normalisation: a stage arrived out of order",
                0x50414745: "a cache's table names a page outside the pool", 0x4c454e47: "a cache's sequence is longer than its table",
+               0x46554c4c: "a cache's free pages do not suffice for a step", 0x50415245: "a row of a cache's table goes on from one that is not there",
                0x53544d31: "streaming column reduction: a tile's data never arrived", 0x53544d32: "streaming column reduction: a stage was never handed back"}
 
 
@@ -382,6 +383,9 @@ def check_status(device: int = 0, stream: int | None = None) -> None:
     check(lib.tq_status_poll(device, ctypes.c_void_p(stream or 0), ctypes.byref(code)))
     if code.value != 0:
         what = _WAIT_CODES.get(code.value, "a tensor-core kernel's pipeline wait")
+        if code.value in (0x46554c4c, 0x50415245):
+            raise DeviceWaitError(f"a cache's step on device {device} was not made: {what}; "
+                                  + (f"{words[3]} needed, {words[4]} free" if code.value == 0x46554c4c else f"row {words[3]}, parent {words[4]}"))
         if code.value in (0x50414745, 0x4c454e47):
             raise DeviceWaitError(f"a cache launch on device {device} left out what it could not follow: {what}; sequence {words[3]}, "
                                   f"{'block' if code.value == 0x50414745 else 'length or start'} {words[4]}")

@@ -48,11 +48,11 @@ _gemm_kernel, _attention_kernel = lru_cache(maxsize=64)(GemmKernel), lru_cache(m
 _launcher = load_launcher()
 _launcher.setup(torch.nn.Parameter, workspace, str(LIBRARY_PATH))
 _FUSED, _REDUCE, _PACK, _SOFTMAX, _LAYER_NORM, _TRANSPOSED, _BATCH_NORM, _GEMM, _ATTENTION = range(9)      # launcher.cpp: Family
-_WINDOW, _CACHE_ATTENTION, _CACHE_STORE = range(9, 12)
+_WINDOW, _CACHE_ATTENTION, _CACHE_STORE, _PREFIX_ATTENTION, _BEAM_SELECT, _CACHE_ADVANCE = range(9, 15)
 _call, _keep_plan = _launcher.call, _launcher.keep
 _CODES = {name: 1 + i for i, name in enumerate(("pack", "softmax", "layer_norm", "native_layer_norm", "batch_norm", "attention", "sum", "mean", "amax",
                                                 "amin", "argmax", "gemm none", "gemm gelu", "gemm gelu_erf", "gemm gelu_tanh", "window attention",
-                                                "cache attention", "cache store"))}
+                                                "cache attention", "cache store", "prefix attention", "beam select", "cache advance"))}
 
 
 def _fused_ints(kernel: FusedKernel, elements: int, divisors) -> tuple:
@@ -698,6 +698,44 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, win
     return out
 
 
+def prefix_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, shared, scale=None, token_major=True):
+    """`cache_attention` of a batch whose sequences share their beginnings, which are read once: beams of a request, samples of a prompt, requests behind
+    one instruction text. `shared` (int32 [runs], on the device) makes the batch as many equal runs of neighbouring sequences, and says of each how
+    many first tokens its sequences have in common: the pages that hold these have the same content, mostly the same numbers, in all of its table rows.
+    Everything else is as there, without a window. Whole tiles of 128 shared tokens are taken together by all sequences that are at least so
+    long, through the table row of the first of these; the rest of them, and the shared tokens of a shorter sequence, each sequence reads by itself."""
+    given = (q, k_pages, v_pages, k_scales, v_scales, table, lengths, shared, scale, token_major)
+    out = _call(_CODES["prefix attention"], *given)
+    if out is not None:
+        return out
+    if q.dim() != 4:
+        raise Declined("the queries must be [batch, heads, tokens, width]")
+    batch, heads, q_tokens, width = q.shape
+    kv_heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    pages, page_tokens, blocks, table_stride = _cache_extents(k_pages, v_pages, k_scales, v_scales, table, batch, kv_heads, width)
+    if (kv_heads == 0) != (heads == 0) or (heads and heads % kv_heads):
+        raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
+    _per_sequence(lengths, batch, "lengths")
+    if shared.dtype != torch.int32 or shared.dim() != 1 or not shared.is_contiguous() or (batch and (shared.numel() == 0 or batch % shared.numel())):
+        raise ValueError(f"shared is packed int32 [runs] with a number of runs that divides {batch} sequences, not {shared.dtype} {tuple(shared.shape)}")
+    runs = shared.numel()
+    scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
+    device = _device_of((q, k_pages, v_pages, k_scales, v_scales, table, lengths, shared))
+    out = _attention_result(q, token_major)
+    nbytes = ctypes.c_size_t()
+    check(lib.tq_prefix_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page_tokens, blocks, runs, device, ctypes.byref(nbytes)))
+    scratch = _own_scratch(nbytes.value, device)
+    strides = (_three_strides(q, "the queries"), _three_strides(out, "the result"))
+    extents = (batch, heads, kv_heads, q_tokens, width, pages, page_tokens, blocks, table_stride, runs)
+    check(lib.tq_prefix_attention_launch(dtype_code(q.dtype), _pointer(q), _pointer(k_pages), _pointer(v_pages), _pointer(k_scales), _pointer(v_scales),
+                                         _pointer(table), _pointer(lengths), _pointer(shared), _pointer(out), *extents, *strides, scale, _pointer(scratch),
+                                         nbytes.value, device, _stream(None, device)))
+    if out.numel():
+        _keep_plan(False, _CODES["prefix attention"], given, _PREFIX_ATTENTION, (out,),
+                   (dtype_code(q.dtype), *extents, *[n for three in strides for n in three], nbytes.value), (scale,), b"", None)
+    return out
+
+
 def cache_store(k, v, k_pages, v_pages, k_scales, v_scales, table, starts, counts=None) -> None:
     """Writes new keys and values [batch, kv_heads, tokens, width] (bf16 or f16) into the cache that `cache_attention` reads: token i
     of sequence b goes to position starts[b] + i, for i < counts[b] (None: all of them); starts[b] < 0 leaves a sequence as it is.
@@ -759,6 +797,100 @@ def copy_pages(tensors, sources, targets, page_axis=0) -> None:
     numbers = ctypes.c_int64 * len(sources)
     check(lib.tq_copy_pages_launch(described, len(tensors), pages, numbers(*sources), numbers(*targets), len(sources), device,
                                    _stream(None, device)))
+
+
+def cache_advance(k_pages, v_pages, k_scales, v_scales, table, lengths, references, counts, parents=None, in_place=False):
+    """A step of a batch's books on the device: rows go on from other rows, as beams do, and get room for new tokens. Nothing of it is known to the host,
+    so it can be captured with the step it prepares. The cache is one layer's ([pages, kv_heads, page_tokens, width], scales [pages, kv_heads]) or, with
+    an axis in front, that of all layers. Row b of `table` (int32 [batch, blocks]) has the pages of lengths[b] tokens (int32 [batch]); references[p]
+    (int32 [pages]) counts the rows, and any others, that have page p: 0 is a free page. Row b goes on from row parents[b] (int32 [batch]; None: from
+    itself; negative: empty) and gets room for counts[b] (int32 [batch]) tokens. A last page that the row will write into and that others have
+    too is copied, except for the last of the rows that write into it where nobody else has it; pages are handed out lowest first, row by row, as
+    `cache.Pages.extend` does. Returns (table, lengths, references, starts): new tensors, or with `in_place` the operands; starts[b] is where row b's new
+    tokens go, as `cache_store` takes it. Where the free pages or the table do not suffice, or a parent or page is none, nothing changes, starts are
+    -1 and `kernel.check_status` raises."""
+    given = (k_pages, v_pages, k_scales, v_scales, table, lengths, references, counts, parents, bool(in_place))
+    found = _call(_CODES["cache advance"], *given)
+    if found is not None:
+        return (table, lengths, references, found) if in_place else (*found[1:], found[0])
+    one_layer = k_pages.dim() == 4
+    if k_pages.dim() not in (4, 5) or any(t.dim() != d for t, d in ((v_pages, k_pages.dim()), (k_scales, k_pages.dim() - 2), (v_scales, k_pages.dim() - 2))):
+        raise ValueError("the cache's pages are [pages, kv_heads, page_tokens, width], its scales [pages, kv_heads], or both with an axis of layers in front")
+    if table.dim() != 2:
+        raise ValueError(f"the table is int32 [batch, blocks], not {table.dtype} {tuple(table.shape)}")
+    batch, blocks = table.shape
+    pools = [t.unsqueeze(0) if one_layer else t for t in (k_pages, v_pages, k_scales, v_scales)]
+    layers, pages, kv_heads, page_tokens, width = pools[0].shape
+    if any(t.shape[0] != layers for t in pools):
+        raise ValueError("the cache's tensors have the same layers")
+    for layer in range(min(layers, 1)):
+        _cache_extents(*[t[layer] for t in pools], table, batch, kv_heads, width)
+    _per_sequence(lengths, batch, "lengths")
+    _per_sequence(counts, batch, "counts")
+    _per_sequence(parents, batch, "parents")
+    if references.dtype != torch.int32 or tuple(references.shape) != (pages,) or not references.is_contiguous():
+        raise ValueError(f"references are packed int32 [pages], not {references.dtype} {tuple(references.shape)}")
+    device = _device_of([t for t in given[:9] if t is not None])
+    described = (_lib.tq_paged_tensor * 4)()
+    for one, t in zip(described, pools):
+        size = t.element_size()
+        one.base, one.layers, one.layer_stride = t.data_ptr(), layers, t.stride(0) * size
+        one.page_bytes = math.prod(t.shape[2:]) * size
+        one.page_stride = max(t.stride(1) * size, one.page_bytes)
+    new = (table, lengths, references) if in_place else (torch.empty(batch, blocks, dtype=torch.int32, device=table.device), torch.empty_like(lengths), torch.empty_like(references))
+    starts = torch.empty_like(lengths)
+    if batch == 0:
+        return (*(new if in_place else (new[0], new[1], references.clone())), starts)
+    nbytes = ctypes.c_size_t()
+    check(lib.tq_cache_advance_workspace_bytes(batch, blocks, pages, page_tokens, ctypes.byref(nbytes)))
+    scratch = _own_scratch(nbytes.value, device)
+    strides = (table.stride(0), new[0].stride(0))
+    check(lib.tq_cache_advance_launch(described, 4, _pointer(table), _pointer(lengths), _pointer(references), _pointer(counts), _pointer(parents),
+                                      *[_pointer(t) for t in new], _pointer(starts), batch, blocks, pages, page_tokens, *strides, _pointer(scratch),
+                                      nbytes.value, device, _stream(None, device)))
+    _keep_plan(False, _CODES["cache advance"], given, _CACHE_ADVANCE, (starts,) if in_place else (starts, *new),
+               (*[n for one in described for n in (one.layers, one.layer_stride, one.page_stride, one.page_bytes)], batch, blocks, pages, page_tokens, *strides,
+                int(bool(in_place)), nbytes.value), (), b"", None)
+    return (*new, starts)
+
+
+def beam_select(logits, scores, keep, finished=None, end=0):
+    """Beam search's selection: of all beams and tokens of each request the `keep` best of scores[r, b] + log_softmax(logits[r, b])[t]. logits are
+    [requests, beams, vocab] (f32, f16, bf16; packed tokens), scores float32 [requests, beams]. Returns (scores, parents, tokens), [requests, keep] in falling
+    order, ties to the lower beam and then the lower token: float32; int32 rows r * beams + b of the batch, as `cache_advance` takes its parents; int32.
+    A beam that is `finished` (bool [requests, beams]) has one candidate, the token `end` at its score as it is. A beam at -inf is not there, nor
+    is one whose logits are all -inf; NaN or +inf among a beam's logits, or in its score, makes its values NaN, which count as the largest. Candidates are
+    compared by values of 64 bits."""
+    given = (logits, scores, keep, finished, end)
+    found = _call(_CODES["beam select"], *given)
+    if found is not None:
+        return found
+    if logits.dim() != 3:
+        raise ValueError(f"logits are [requests, beams, vocab], not {tuple(logits.shape)}")
+    requests, beams, vocab = logits.shape
+    for t, dtype, what in ((scores, torch.float32, "scores"), (finished, torch.bool, "finished")):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (requests, beams) or not t.is_contiguous()):
+            raise ValueError(f"{what} are packed {dtype} [requests, beams], not {t.dtype} {tuple(t.shape)}")
+    if logits.numel() and vocab > 1 and logits.stride(2) != 1:
+        raise Declined("the logits of a beam must be contiguous")
+    plain = type(keep) is int and type(end) is int
+    keep, end = index(keep), index(end)
+    if not 0 <= keep <= beams * vocab:
+        raise ValueError(f"{keep} of {beams} beams by {vocab} tokens cannot be kept")
+    if finished is not None and not 0 <= end < max(vocab, 1):
+        raise ValueError(f"there is no token {end} among {vocab} to end with")
+    end = end if finished is not None else 0
+    device = _device_of([t for t in (logits, scores, finished) if t is not None])
+    out = tuple(torch.empty(requests, keep, dtype=dtype, device=logits.device) for dtype in (torch.float32, torch.int32, torch.int32))
+    nbytes = ctypes.c_size_t()
+    check(lib.tq_beam_select_workspace_bytes(requests, beams, vocab, keep, ctypes.byref(nbytes)))
+    scratch = _own_scratch(nbytes.value, device)
+    ints = (requests, beams, vocab, keep, end, logits.stride(0), logits.stride(1))
+    check(lib.tq_beam_select_launch(dtype_code(logits.dtype), _pointer(logits), _pointer(scores), _pointer(finished), *[_pointer(t) for t in out], *ints,
+                                    _pointer(scratch), nbytes.value, device, _stream(None, device)))
+    if plain and requests and keep:
+        _keep_plan(False, _CODES["beam select"], given, _BEAM_SELECT, out, (dtype_code(logits.dtype), *ints, nbytes.value), (), b"", None)
+    return out
 
 
 # ---------------------------------------------------------------------------------------------
@@ -831,6 +963,11 @@ def register_custom_ops() -> None:
         "cache_store(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor table, Tensor starts, "
         "Tensor? counts) -> ()": cache_store,
         "copy_pages(Tensor(a!)[] tensors, int[] sources, int[] targets, int page_axis) -> ()": copy_pages,
+        "prefix_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor table, Tensor lengths, Tensor shared, "
+        "float? scale) -> Tensor": prefix_attention,
+        "cache_advance(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor table, Tensor lengths, Tensor references, "
+        "Tensor counts, Tensor? parents) -> (Tensor, Tensor, Tensor, Tensor)": cache_advance,
+        "beam_select(Tensor logits, Tensor scores, int keep, Tensor? finished, int end) -> (Tensor, Tensor, Tensor)": beam_select,
     }
     for schema, implementation in schemas.items():
         library.define(schema)
