@@ -448,7 +448,7 @@ tq_status tq_gemm_bias_act_residual_launch(tq_dtype dtype,
 /* Which kernel the launch below runs for `heads` (batch times heads) of these extents: keys streamed by CUDA cores
  * (decoding), or the tensor-core kernel with 64 or 128 keys a step, in its form for many queries or for a few. It depends
  * on the number of SMs of `device`; device -1 stands for a B200 and needs no GPU. */
-enum { TQ_ATTENTION_STREAMED = 0, TQ_ATTENTION_TILES = 1, TQ_ATTENTION_TILES_FEW = 2 };
+enum { TQ_ATTENTION_STREAMED = 0, TQ_ATTENTION_TILES = 1, TQ_ATTENTION_TILES_FEW = 2, TQ_ATTENTION_APART = 3 };
 tq_status tq_attention_form(int64_t heads, int64_t q_tokens, int64_t k_tokens, int64_t head_dim, int32_t causal, int32_t device,
                             int32_t* form, int32_t* keys);
 /* out[b,h,i,:] = sum_j softmax_j(scale * q[b,h,i,:] . k[b,h,j,:]) * v[b,h,j,:], over j <= i when
@@ -528,6 +528,10 @@ tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, const void* k
  * content. Whole tiles of 128 of these are read once for all sequences of the run that are at least so long (every query stands behind them), through
  * the table row of the first of those; what is left of them, and the shared tokens of shorter sequences (a padded row of length 0 among them), each
  * sequence reads itself. shared[r] <= 0: nothing is shared. `workspace` as there, tq_prefix_attention_workspace_bytes of it. */
+/* Which way the launch takes: each sequence reads all its keys (TQ_ATTENTION_APART), or the shared ones are read for all rows of a run together, streamed
+ * (TQ_ATTENTION_STREAMED) or on tensor-core tiles (TQ_ATTENTION_TILES), in so many parts; device -1: on a B200, without a GPU. */
+tq_status tq_prefix_attention_form(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens, int64_t blocks,
+                                   int64_t runs, int32_t device, int32_t* form, int32_t* parts);
 tq_status tq_prefix_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens,
                                               int64_t blocks, int64_t runs, int32_t device, size_t* bytes);
 tq_status tq_prefix_attention_launch(tq_dtype dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scales,
@@ -583,7 +587,7 @@ tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int32_t count,
  * with element strides `request_stride` and `beam_stride` and packed tokens, scores packed f32, finished packed bytes or null: a finished beam has one
  * candidate, `end`, at its score as it is, and -inf for every other token. A beam whose score is -inf, or whose logits all are, has -inf for all its
  * candidates; one with a NaN or +inf among them, NaN, which counts as the largest. At most 128 beams a request, 65535 in all, 128 kept, 2^24 - 1 tokens. */
-tq_status tq_beam_select_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab, int64_t keep, size_t* bytes);
+tq_status tq_beam_select_workspace_bytes(tq_dtype dtype, int64_t requests, int64_t beams, int64_t vocab, int64_t keep, size_t* bytes);
 tq_status tq_beam_select_launch(tq_dtype dtype, const void* logits, const float* scores, const uint8_t* finished, float* out_scores, int32_t* out_parents,
                                 int32_t* out_tokens, int64_t requests, int64_t beams, int64_t vocab, int64_t keep, int64_t end, int64_t request_stride,
                                 int64_t beam_stride, void* workspace, size_t workspace_bytes, int32_t device, void* stream);

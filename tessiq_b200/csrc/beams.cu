@@ -5,13 +5,14 @@
 // Within a beam the order is that of the logits, so a beam's candidates are its `keep` largest logits, and the logarithm of its sum is needed to compare
 // beams alone. Bound: HBM (each logit is read once).
 //
-// First kernel: a CTA takes up to 8184 logits of a beam, into registers: their maximum and sum of exponentials, and their `keep` largest. Every warp's
-// r-th largest thread maximum, r = keep / warps, is a bound below which nothing is needed (warps * r threads have something at or above it); what is
-// at or above the lowest of these bounds goes to a list, a few times `keep` long, and its members' places are counted against each other. A list that
-// overflows (very many equal logits, a mask of -inf) is answered by `keep` rounds of the CTA's maximum over what is still in registers.
+// First kernel: a CTA takes a part of a beam's logits, chunks of 8192 in registers one after another, and the next one's loads are under way meanwhile:
+// their sum of exponentials, and their `keep` largest. In the first chunk every warp's r-th largest thread maximum, r = keep / warps, is a bound below
+// which nothing is needed (warps * r threads have something at or above it); what is at or above the lowest of these goes to a list, a few times
+// `keep` long. Its `keep`-th best is the bound for the chunks behind, of which 32 / n of the n-th reach it. Places in a list are counted by comparing
+// its members with each other. A list that overflows (very many equal logits, a mask of -inf) is answered by `keep` rounds of the CTA's maximum.
 // Second kernel: a CTA a request joins the parts: sums, values in f64, and the same two steps over all its candidates.
 //
-// Precision: sums of exponentials in f32 a thread (32 of them), then f64: a logarithm is off by 1e-7 or so. Values of neighbours are as close as that
+// Precision: sums of exponentials in f32 a thread (16 of them), then f64: a logarithm is off by 1e-7 or so. Values of neighbours are as close as that
 // now and then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout. Ties are then ties.
 #include <cmath>
 #include <type_traits>
@@ -24,11 +25,14 @@ namespace tq {
 namespace {
 
 constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
-constexpr int kEach = 32;                                   // logits of a thread
-constexpr int kChunk = kSelectThreads * kEach - 8;          // of a CTA: a row may begin inside a vector of 16 bytes
+constexpr int kVecs = 4;                                    // a thread's vectors of 16 bytes of a chunk
+constexpr int kChunkBytes = kSelectThreads * kVecs * 16;
+constexpr int kStages = 2;                                  // chunks on chip
 constexpr int kListed = 1024;                               // candidates on chip
 constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
+constexpr int kUppers = 6144;                               // candidates of which the joining kernel keeps half the order
 constexpr int kMostBeams = 128, kMostKept = 128;
+constexpr int kSelectCtas = 592;                            // at once on a B200, four an SM
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct SelectParams {
@@ -37,7 +41,7 @@ struct SelectParams {
   const float* scores;                                      // [requests, beams]
   const uint8_t* finished;                                  // the same, or null
   int beams, vocab, keep, parts, chunk, end;
-  float2* sums;                                             // [rows, parts]: the exponent the sum stands at, in log2, and the sum
+  double2* sums;                                            // [rows, parts]: the whole power of two the sum stands at, and the sum
   unsigned long long* keys;                                 // [rows, parts, keep]: candidates of a part, the best first; 0: none
   float* out_scores;                                        // [requests, keep]
   int32_t *out_parents, *out_tokens;
@@ -83,126 +87,144 @@ __device__ __forceinline__ void widen(const uint4& word, float* to) {
   }
 }
 
+// How many of a list on chip come before an item (the same list for all threads: its reads are under way together).
+template <typename Item, typename Before>
+__device__ __forceinline__ int place_in(const Item* list, int found, Before&& before_it) {
+  int place = 0;
+#pragma unroll 8
+  for (int j = 0; j < found; ++j) place += before_it(list[j]) ? 1 : 0;
+  return place;
+}
+
+__device__ __forceinline__ void copy_async_16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_address(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Whether an element of the vector is at or above the bound, which is one of T's numbers.
+template <typename T>
+__device__ __forceinline__ bool reaches(const uint4& word, float bound) {
+  const uint32_t w[4] = {word.x, word.y, word.z, word.w};
+  uint32_t any = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (std::is_same_v<T, float>) {
+      any |= __uint_as_float(w[c]) >= bound ? 1u : 0u;
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      any |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[c]), __float2bfloat162_rn(bound));
+    } else {
+      any |= __hge2_mask(*reinterpret_cast<const __half2*>(&w[c]), __float2half2_rn(bound));
+    }
+  }
+  return any != 0;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __grid_constant__ SelectParams p) {
-  constexpr int kVec = 16 / sizeof(T), kVecs = kEach / kVec;
+  constexpr int kVec = 16 / sizeof(T), kChunk = kChunkBytes / sizeof(T);
+  __shared__ uint4 ring[kStages][kVecs][kSelectThreads];    // a thread reads what it has copied itself
   __shared__ uint32_t warp_most[kSelectWarps], warp_bound[kSelectWarps];
   __shared__ double warp_sum[kSelectWarps];
-  __shared__ unsigned long long list[kListed], warp_key[kSelectWarps];
+  __shared__ unsigned long long lists[kListed + kMostKept], warp_key[kSelectWarps];      // the list, and room for the best of it
   __shared__ int listed;
   const int part = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.y;
   const int request = static_cast<int>(row / p.beams), beam = static_cast<int>(row % p.beams);
+  unsigned long long* const list = lists;
+  unsigned long long* const kept = lists + kListed;
   if (threadIdx.x == 0) listed = 0;
   wait_for_earlier();
   if (p.finished != nullptr && p.finished[row]) return;     // (its one candidate is made below)
   const int first = part * p.chunk, count = min(p.chunk, p.vocab - first);
   const T* const from = static_cast<const T*>(p.logits) + request * p.request_stride + beam * p.beam_stride + first;
   const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
-  const T* const whole = from - skew;
+  const int chunks = (count + skew + kChunk - 1) / kChunk;
 
-  // A thread's vectors; what lies before or behind the part is -inf.
-  uint4 word[kVecs];
+  // A thread's vectors of a chunk, whole vectors of 16 bytes from the one that the part begins in; what lies before or behind the part is -inf.
+  auto place_of = [&](int chunk, int i) { return ((chunk * kVecs + i) * kSelectThreads + static_cast<int>(threadIdx.x)) * kVec - skew; };      // in the part
+  auto ask = [&](int chunk) {
+    if (chunk < chunks) {
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int at = (i * kSelectThreads + static_cast<int>(threadIdx.x)) * kVec - skew;      // of its first element, in the part
-    if (at >= 0 && at + kVec <= count) {
-      const Vec<T, kVec> vector = load_stream<T, kVec>(whole + at + skew);
-      word[i] = *reinterpret_cast<const uint4*>(&vector);
-    } else {
-      Vec<T, kVec> vector;
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) vector.v[c] = at + c >= 0 && at + c < count ? from[at + c] : from_compute<T, float>(-INFINITY);
-      word[i] = *reinterpret_cast<const uint4*>(&vector);
-    }
-  }
-  float most = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    float x[kVec];
-    widen<T>(word[i], x);
-#pragma unroll
-    for (int c = 0; c < kVec; ++c) most = fmaxf(most, x[c]);
-  }
-  // Warps of which every thread has logits: of a part of 2048 or more all.
-  const int vectors = (count + skew + kVec - 1) / kVec, full = min(vectors / 32, kSelectWarps);
-  const int nth = full == 0 ? 33 : (p.keep + full - 1) / full;
-  const uint32_t mine = ordered(most);
-  const uint32_t in_warp = __reduce_max_sync(0xffffffffu, mine);
-  const uint32_t bound = nth > 32 ? 0 : nth == 1 ? in_warp : warp_nth(mine, nth);
-  if (lane == 0) {
-    warp_most[warp] = in_warp;
-    warp_bound[warp] = bound;
-  }
-  __syncthreads();
-  uint32_t top = 0, least = 0xffffffffu;
-#pragma unroll
-  for (int w = 0; w < kSelectWarps; ++w) {
-    top = max(top, warp_most[w]);
-    if (w < full) least = min(least, warp_bound[w]);
-  }
-  if (nth > 32) least = 0;
-  const float threshold = least <= 0x007fffffu ? -INFINITY : from_ordered(least);
-  most = from_ordered(top);
-  const float shift = most == -INFINITY ? 0.f : most * kLog2E;      // (rounded, and the sum stands at what it was rounded to)
-  float sum0 = 0.f, sum1 = 0.f;
-  auto key_of = [&](float x, int at) { return static_cast<unsigned long long>(ordered(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(first + at)); };
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    float x[kVec];
-    widen<T>(word[i], x);
-    const int at = (i * kSelectThreads + static_cast<int>(threadIdx.x)) * kVec - skew;
-    bool any = false;
-#pragma unroll
-    for (int c = 0; c < kVec; c += 2) {
-      sum0 += exp2_ftz(fmaf(x[c], kLog2E, -shift));
-      sum1 += exp2_ftz(fmaf(x[c + 1], kLog2E, -shift));
-      any |= x[c] >= threshold || x[c + 1] >= threshold;
-    }
-    if (any) {
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) {
-        if (x[c] >= threshold && at + c >= 0 && at + c < count) {
-          const int place = atomicAdd(&listed, 1);
-          if (place < kListed) list[place] = key_of(x[c], at + c);
+      for (int i = 0; i < kVecs; ++i) {
+        const int at = place_of(chunk, i);
+        uint4* const to = &ring[chunk % kStages][i][threadIdx.x];
+        if (at >= 0 && at + kVec <= count) {
+          copy_async_16(to, from + at);
+        } else {
+          for (int c = 0; c < kVec; ++c) reinterpret_cast<T*>(to)[c] = at + c >= 0 && at + c < count ? from[at + c] : from_compute<T, float>(-INFINITY);
         }
       }
     }
-  }
-  double sum = static_cast<double>(sum0) + static_cast<double>(sum1);
+    copy_async_commit();
+  };
+  auto words = [&](int chunk, int i, float (&x)[kVec]) { widen<T>(ring[chunk % kStages][i][threadIdx.x], x); };
+  auto key_of = [&](float x, int at) { return static_cast<unsigned long long>(ordered(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(first + at)); };
+  float threshold = -INFINITY, shift = 0.f;
+  double sum = 0.0;
+  // Adds a chunk to the sum, and what reaches the bound to the list: whether that has become long, for the CTA.
+  auto take = [&](int chunk) {
+    float sum0 = 0.f, sum1 = 0.f;
+    int last = 0;
 #pragma unroll
-  for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-  if (lane == 0) warp_sum[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0.0;
+    for (int i = 0; i < kVecs; ++i) {
+      const uint4 word = ring[chunk % kStages][i][threadIdx.x];
+      float x[kVec];
+      widen<T>(word, x);
 #pragma unroll
-    for (int w = 0; w < kSelectWarps; ++w) all += warp_sum[w];
-    p.sums[row * p.parts + part] = make_float2(shift, static_cast<float>(all));
-  }
-  unsigned long long* const to = p.keys + (row * p.parts + part) * p.keep;
-  const int found = listed;
-  if (found <= kListed) {
+      for (int c = 0; c < kVec; c += 2) {
+        sum0 += exp2_ftz(fmaf(x[c], kLog2E, -shift));
+        sum1 += exp2_ftz(fmaf(x[c + 1], kLog2E, -shift));
+      }
+      if (reaches<T>(word, threshold)) {                      // (few vectors do)
+        const int at = place_of(chunk, i);
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+          if (x[c] >= threshold && at + c >= 0 && at + c < count) {
+            last = atomicAdd(&listed, 1);
+            if (last < kListed) list[last] = key_of(x[c], at + c);
+          }
+        }
+      }
+    }
+    sum += static_cast<double>(sum0) + static_cast<double>(sum1);
+    return __syncthreads_or(last >= max(2 * p.keep, 32)) != 0;
+  };
+  // The list's best `keep` in their order, as the list; all threads.
+  auto prune = [&] {
+    const int found = listed;
+    for (int i = threadIdx.x; i < p.keep; i += kSelectThreads) kept[i] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < found; i += kSelectThreads) {
       const unsigned long long key = list[i];
-      int place = 0;
-      for (int j = 0; j < found; ++j) place += list[j] > key ? 1 : 0;
-      if (place < p.keep) to[place] = key;
+      const int place = place_in(list, found, [&](unsigned long long other) { return other > key; });
+      if (place < p.keep) kept[place] = key;
     }
-    for (int i = found + threadIdx.x; i < p.keep; i += kSelectThreads) to[i] = 0;
-  } else {
-    unsigned long long before = ~0ull;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.keep; i += kSelectThreads) list[i] = kept[i];
+    if (threadIdx.x == 0) listed = min(found, p.keep);
+    __syncthreads();                                          // (nobody adds before that)
+    if (found >= p.keep) threshold = from_ordered(static_cast<uint32_t>(list[p.keep - 1] >> 32));
+  };
+  // The same where the list has overflown (very many equal logits, a mask of -inf), by as many rounds: over what the list has, and the chunk.
+  auto prune_chunk = [&](int chunk) {
+    unsigned long long last = ~0ull;
     for (int n = 0; n < p.keep; ++n) {
       unsigned long long best = 0;
-#pragma unroll
+      for (int i = threadIdx.x; i < kListed; i += kSelectThreads)
+        if (list[i] < last && list[i] > best) best = list[i];
+#pragma unroll 1
       for (int i = 0; i < kVecs; ++i) {
         float x[kVec];
-        widen<T>(word[i], x);
-        const int at = (i * kSelectThreads + static_cast<int>(threadIdx.x)) * kVec - skew;
+        words(chunk, i, x);
+        const int at = place_of(chunk, i);
 #pragma unroll
         for (int c = 0; c < kVec; ++c) {
           const unsigned long long key = at + c >= 0 && at + c < count ? key_of(x[c], at + c) : 0;
-          if (key < before && key > best) best = key;
+          if (key < last && key > best) best = key;
         }
       }
 #pragma unroll
@@ -211,11 +233,99 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kSelectWarps; ++w) best = max(best, warp_key[w]);
-      if (threadIdx.x == 0) to[n] = best;
-      before = best;
+      if (threadIdx.x == 0) kept[n] = best;
+      last = best;
       __syncthreads();
     }
+    for (int i = threadIdx.x; i < p.keep; i += kSelectThreads) list[i] = kept[i];
+    if (threadIdx.x == 0) listed = p.keep;                    // (some may be 0, none)
+    __syncthreads();
+    if (list[p.keep - 1] != 0) threshold = from_ordered(static_cast<uint32_t>(list[p.keep - 1] >> 32));
+  };
+
+  for (int chunk = 0; chunk < kStages; ++chunk) ask(chunk);
+  copy_async_wait<kStages - 1>();
+  // The first chunk says what the sum stands at, a whole power of two (so that parts and beams join without exponentials; +inf and NaN make the sum
+  // NaN), and a bound.
+  {
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      float x[kVec];
+      words(0, i, x);
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) most = fmaxf(most, x[c]);
+    }
+    // Warps of which every thread has logits: of 2048 or more all.
+    const int vectors = (count + skew + kVec - 1) / kVec, full = min(vectors / 32, kSelectWarps);
+    const int nth = full == 0 ? 33 : (p.keep + full - 1) / full;
+    const uint32_t mine = ordered(most);
+    const uint32_t in_warp = __reduce_max_sync(0xffffffffu, mine);
+    const uint32_t bound = nth > 32 ? 0 : nth == 1 ? in_warp : warp_nth(mine, nth);
+    if (lane == 0) {
+      warp_most[warp] = in_warp;
+      warp_bound[warp] = bound;
+    }
+    __syncthreads();
+    uint32_t top = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) {
+      top = max(top, warp_most[w]);
+      if (w < full) least = min(least, warp_bound[w]);
+    }
+    if (nth > 32) least = 0;
+    threshold = least <= 0x007fffffu ? -INFINITY : from_ordered(least);
+    most = from_ordered(top);
+    shift = most == -INFINITY ? 0.f : rintf(most * kLog2E);
   }
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    copy_async_wait<kStages - 1>();
+    if (take(chunk)) {
+      if (listed > kListed) prune_chunk(chunk);
+      else prune();
+    } else if (chunk == 0 && chunks > 1) {
+      prune();                                                // (a tighter bound for the others)
+    }
+    ask(chunk + kStages);
+  }
+  copy_async_wait<0>();
+  // A sum that a later chunk has carried far from what it stands at is taken again, from the true maximum.
+  auto whole_sum = [&] {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) all += warp_sum[w];
+    __syncthreads();
+    return all;
+  };
+  double all = whole_sum();
+  if (chunks > 1 && !(all > 1e-30 && all < 1e30)) {
+    float most = -INFINITY;
+    for (int t = threadIdx.x; t < count; t += kSelectThreads) most = fmaxf(most, to_compute(from[t]));
+    const uint32_t in_warp = __reduce_max_sync(0xffffffffu, ordered(most));
+    if (lane == 0) warp_most[warp] = in_warp;
+    __syncthreads();
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) top = max(top, warp_most[w]);
+    most = from_ordered(top);
+    shift = most == -INFINITY ? 0.f : rintf(most * kLog2E);
+    sum = 0.0;
+    for (int t = threadIdx.x; t < count; t += kSelectThreads) sum += static_cast<double>(exp2_ftz(fmaf(to_compute(from[t]), kLog2E, -shift)));
+    all = whole_sum();
+  }
+  if (threadIdx.x == 0) p.sums[row * p.parts + part] = make_double2(shift, all);
+  unsigned long long* const to = p.keys + (row * p.parts + part) * p.keep;
+  const int found = listed;
+  for (int i = threadIdx.x; i < found; i += kSelectThreads) {
+    const unsigned long long key = list[i];
+    const int place = place_in(list, found, [&](unsigned long long other) { return other > key; });
+    if (place < p.keep) to[place] = key;
+  }
+  for (int i = found + threadIdx.x; i < p.keep; i += kSelectThreads) to[i] = 0;
 }
 
 enum BeamState { kGoesOn = 0, kFinished, kNothing, kNoNumber };      // kNothing: every logit, or the score, is -inf; kNoNumber: NaN, or +inf
@@ -231,17 +341,27 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   return a.order != b.order ? a.order > b.order : a.beam != b.beam ? a.beam < b.beam : a.token < b.token;
 }
 
+// A sum that stands at 2^from, at 2^to >= 2^from (whole numbers, or -inf for no sum, and what is +inf is NaN by now).
+__device__ __forceinline__ double brought(double sum, float from, float to) {
+  const float down = to - from;
+  if (!(down > 0.f)) return sum;
+  return down > 1000.f ? 0.0 : sum * __longlong_as_double(static_cast<long long>(1023 - static_cast<int>(down)) << 52);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ SelectParams p) {
   __shared__ double logarithm[kMostBeams], score_of[kMostBeams];
   __shared__ uint8_t state[kMostBeams], again[kMostBeams];
   __shared__ Candidate list[kListed], warp_best[kJoinWarps];
-  __shared__ uint32_t warp_bound[kJoinWarps];
+  __shared__ int bins[6][16];
+  __shared__ uint32_t uppers[kUppers];
   __shared__ double warp_sum[kJoinWarps];
   __shared__ float largest_shift;
   __shared__ int listed, near;
   const int request = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_earlier();
+  const int slots = p.parts * p.keep + 1, all = p.beams * slots;      // of a beam, and of the request
+  const long long keys0 = static_cast<long long>(request) * p.beams * (slots - 1);
   if (threadIdx.x == 0) {
     largest_shift = 0.f;
     near = 0;
@@ -255,20 +375,19 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     double sum = 0.0;
     if (!finished) {
       for (int part = lane; part < p.parts; part += 32) {
-        const float2 one = p.sums[row * p.parts + part];
+        const double2 one = p.sums[row * p.parts + part];
         // (a part of -inf alone has the sum 0 at 0; of a NaN its sum is one)
-        if (one.y == 0.f) continue;
-        const float both = fmaxf(at, one.x);
-        sum = sum * (at == both ? 1.0 : exp2(static_cast<double>(at) - both)) + one.y * (one.x == both ? 1.0 : exp2(static_cast<double>(one.x) - both));
+        if (one.y == 0.0) continue;
+        const float there = static_cast<float>(one.x), both = fmaxf(at, there);
+        sum = brought(sum, at, both) + brought(one.y, there, both);
         at = both;
       }
+      const float lane_at = at;
 #pragma unroll
-      for (int offset = 16; offset > 0; offset /= 2) {
-        const float other = __shfl_xor_sync(0xffffffffu, at, offset), both = fmaxf(at, other);
-        const double theirs = __shfl_xor_sync(0xffffffffu, sum, offset);
-        sum = sum * (at == both ? 1.0 : exp2(static_cast<double>(at) - both)) + theirs * (other == both ? 1.0 : exp2(static_cast<double>(other) - both));
-        at = both;
-      }
+      for (int offset = 16; offset > 0; offset /= 2) at = fmaxf(at, __shfl_xor_sync(0xffffffffu, at, offset));
+      sum = brought(sum, lane_at, at);
+#pragma unroll
+      for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
     }
     if (lane == 0) {
       score_of[beam] = score;
@@ -279,20 +398,18 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       else if (!(sum >= 0.0) || !(sum < INFINITY) || at == INFINITY) now = kNoNumber;
       else if (sum == 0.0 || score == -INFINITY) now = kNothing;
       state[beam] = static_cast<uint8_t>(now);
-      logarithm[beam] = now == kGoesOn ? (static_cast<double>(at) + log2(sum)) * 0.6931471805599453 : 0.0;
+      logarithm[beam] = now == kGoesOn ? at * 0.6931471805599453 + log(sum) : 0.0;
       if (now == kGoesOn) atomicMax(reinterpret_cast<int*>(&largest_shift), __float_as_int(fabsf(at)));
     }
   }
   __syncthreads();
   const int most_tokens = min(p.keep, p.vocab);
-  const int slots = p.parts * p.keep + 1, all = p.beams * slots;      // of a beam, and of the request
   const double close = kNear * (1.0 + static_cast<double>(largest_shift) / 16.0);
   auto candidate = [&](int i) {
-    const int beam = i / slots, c = i % slots;
+    const int beam = i / slots, c = i - beam * slots;
     Candidate one = {0, static_cast<uint32_t>(beam), static_cast<uint32_t>(c)};
     if (state[beam] == kGoesOn) {
-      if (c == slots - 1) return one;
-      const unsigned long long key = p.keys[(static_cast<long long>(request) * p.beams + beam) * p.parts * p.keep + c];
+      const unsigned long long key = c == slots - 1 ? 0ull : p.keys[keys0 + i - beam];
       if (key == 0) return one;
       one.token = 0xffffffffu - static_cast<uint32_t>(key);
       one.order = ordered(score_of[beam] + (static_cast<double>(from_ordered(static_cast<uint32_t>(key >> 32))) - logarithm[beam]));
@@ -310,31 +427,53 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     return order == ~0ull ? static_cast<double>(NAN) : __longlong_as_double(static_cast<long long>(order >> 63 ? order & ~(1ull << 63) : ~order));
   };
   for (int round = 0;; ++round) {
-    // A bound that `keep` candidates reach, from the order's upper half; lowered by what is close.
-    uint32_t mine = 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < all; i += kJoinThreads) mine = max(mine, static_cast<uint32_t>(candidate(i).order >> 32));
-    const int full = min(all / 32, kJoinWarps), nth = full == 0 ? 33 : (p.keep + full - 1) / full;
-    const uint32_t bound = nth > 32 ? 0 : warp_nth(mine, nth);
-    if (lane == 0) warp_bound[warp] = bound;
+    // The upper halves of the candidates' orders stay on chip (beyond kUppers they are made again and again). Loops as they are: what runs once waits for
+    // its instructions, and unrolled this took twice as long.
+    auto upper = [&](int i) { return i < kUppers ? uppers[i] : static_cast<uint32_t>(candidate(i).order >> 32); };
+#pragma unroll 1
+    for (int i = threadIdx.x; i < min(all, kUppers); i += kJoinThreads) uppers[i] = static_cast<uint32_t>(candidate(i).order >> 32);
+    // The largest bound that `keep` candidates reach, four of the order's upper 24 bits (12 of f64's fraction) at a time; lowered by what is close.
+    uint32_t least = 0;
+    for (int i = threadIdx.x; i < 6 * 16; i += kJoinThreads) bins[i / 16][i % 16] = 0;
+    __syncthreads();
+    int above = 0;                                            // candidates above the bits found so far
+#pragma unroll 1
+    for (int n = 0; n < 6; ++n) {
+      const int low = 28 - 4 * n;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+        const uint32_t order = upper(i);
+        if (order != 0 && (n == 0 || order >> (low + 4) == least >> (low + 4))) atomicAdd(&bins[n][order >> low & 15], 1);
+      }
+      __syncthreads();
+      // Lane d has how many reach digit d: the last lane that `keep` reach, or 0.
+      const int mine = lane < 16 ? bins[n][lane] : 0;
+      int reach = mine;
+#pragma unroll
+      for (int offset = 1; offset < 16; offset *= 2) {
+        const int more = __shfl_down_sync(0xffffffffu, reach, offset);
+        if (lane + offset < 16) reach += more;
+      }
+      const uint32_t enough = __ballot_sync(0xffffffffu, lane < 16 && above + reach >= p.keep);
+      const int digit = enough == 0 ? 0 : 31 - __clz(enough);
+      above += __shfl_sync(0xffffffffu, reach - mine, digit);
+      least |= static_cast<uint32_t>(digit) << low;
+    }
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    uint32_t least = 0xffffffffu;
-    for (int w = 0; w < full; ++w) least = min(least, warp_bound[w]);
-    if (nth > 32) least = 0;
     unsigned long long threshold = static_cast<unsigned long long>(least) << 32;
-    if (round == 0 && least != 0 && least != 0xffffffffu) {
+    if (round == 0 && least != 0 && least != 0xffffff00u) {
       const double lower = value_of(threshold) - 2.0 * close;
       if (lower == lower) threshold = ordered(lower);      // (of -inf: -inf)
     }
     if (threshold == 0) threshold = 1;
-#pragma unroll 4
+#pragma unroll 1
     for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+      if (upper(i) < static_cast<uint32_t>(threshold >> 32)) continue;
       const Candidate one = candidate(i);
-      if (one.order >= threshold) {
-        const int place = atomicAdd(&listed, 1);
-        if (place < kListed) list[place] = one;
-      }
+      if (one.order < threshold) continue;
+      const int place = atomicAdd(&listed, 1);
+      if (place < kListed) list[place] = one;
     }
     __syncthreads();
     const int found = listed;
@@ -347,13 +486,16 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     if (found <= kListed) {
       for (int i = threadIdx.x; i < found; i += kJoinThreads) {
         const Candidate one = list[i];
-        const double value = value_of(one.order);
         int place = 0;
+#pragma unroll 4
         for (int j = 0; j < found; ++j) place += before(list[j], one) ? 1 : 0;
         if (place >= p.keep) continue;
         write(place, one);
         if (round > 0) continue;
-        for (int j = 0; j < found; ++j) {      // (-inf and NaN are close to nothing; beams of one sum and one score compare as their logits do)
+        // (-inf and NaN are close to nothing; beams of one sum and one score compare as their logits do)
+        const double value = value_of(one.order);
+#pragma unroll 1
+        for (int j = 0; j < found; ++j) {
           const Candidate other = list[j];
           if (other.beam != one.beam && fabs(value_of(other.order) - value) < close &&
               !(logarithm[one.beam] == logarithm[other.beam] && score_of[one.beam] == score_of[other.beam]))
@@ -363,8 +505,10 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     } else {
       // (very many equal values, of which only the order of beams and tokens tells)
       Candidate last = {~0ull, 0, 0};
+#pragma unroll 1
       for (int n = 0; n < p.keep; ++n) {
         Candidate best = {0, 0, 0};
+#pragma unroll 1
         for (int i = threadIdx.x; i < all; i += kJoinThreads) {
           const Candidate one = candidate(i);
           if (one.order != 0 && (n == 0 || before(last, one)) && (best.order == 0 || before(one, best))) best = one;
@@ -377,6 +521,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
         }
         if (lane == 0) warp_best[warp] = best;
         __syncthreads();
+#pragma unroll 1
         for (int w = 0; w < kJoinWarps; ++w) {
           const Candidate other = warp_best[w];
           if (other.order != 0 && (best.order == 0 || before(other, best))) best = other;
@@ -394,6 +539,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       const T* const from = static_cast<const T*>(p.logits) + request * p.request_stride + beam * p.beam_stride;
       double sum = 0.0;
       const double shift = logarithm[beam];
+#pragma unroll 1
       for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) sum += exp(static_cast<double>(to_compute(from[t])) - shift);
 #pragma unroll
       for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
@@ -401,6 +547,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       __syncthreads();
       if (threadIdx.x == 0) {
         double whole = 0.0;
+#pragma unroll 1
         for (int w = 0; w < kJoinWarps; ++w) whole += warp_sum[w];
         logarithm[beam] = shift + log(whole);
       }
@@ -413,13 +560,15 @@ struct SelectPlan {
   int parts, chunk;
   size_t sums_bytes, keys_bytes;
 };
-SelectPlan plan_select(int64_t rows, int64_t vocab, int64_t keep) {
+// As many parts of a row as there are CTAs at once for it, and one at least. (512 rows of 128000 in one part 49 us, in two 80.)
+SelectPlan plan_select(int64_t rows, int64_t vocab, int64_t keep, int64_t bytes) {
   SelectPlan plan = {};
-  const int64_t parts = (vocab + kChunk - 1) / kChunk;
+  const int64_t chunk = kChunkBytes / bytes - 8, chunks = (vocab + chunk - 1) / chunk;      // (a row may begin inside a vector)
+  const int64_t parts = kSelectCtas / rows < 1 ? 1 : kSelectCtas / rows < chunks ? kSelectCtas / rows : chunks;
   plan.chunk = static_cast<int>(((vocab + parts - 1) / parts + 7) / 8 * 8);
   plan.parts = static_cast<int>((vocab + plan.chunk - 1) / plan.chunk);
   plan.keys_bytes = static_cast<size_t>(rows) * plan.parts * keep * sizeof(unsigned long long);
-  plan.sums_bytes = static_cast<size_t>(rows) * plan.parts * sizeof(float2);
+  plan.sums_bytes = static_cast<size_t>(rows) * plan.parts * sizeof(double2);
   return plan;
 }
 
@@ -430,11 +579,11 @@ bool select_takes(int64_t requests, int64_t beams, int64_t vocab, int64_t keep) 
 }  // namespace
 }  // namespace tq
 
-extern "C" tq_status tq_beam_select_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab, int64_t keep, size_t* bytes) {
+extern "C" tq_status tq_beam_select_workspace_bytes(tq_dtype dtype, int64_t requests, int64_t beams, int64_t vocab, int64_t keep, size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   *bytes = 0;
-  if (requests > (1LL << 31) || !tq::select_takes(requests, beams, vocab, keep)) return TQ_OK;
-  const tq::SelectPlan plan = tq::plan_select(requests * beams, vocab, keep);
+  if (tq::dtype_size(dtype) == 0 || requests > (1LL << 31) || !tq::select_takes(requests, beams, vocab, keep)) return TQ_OK;
+  const tq::SelectPlan plan = tq::plan_select(requests * beams, vocab, keep, tq::dtype_size(dtype));
   *bytes = plan.sums_bytes + plan.keys_bytes;
   return TQ_OK;
 }
@@ -462,9 +611,9 @@ extern "C" tq_status tq_beam_select_launch(tq_dtype dtype, const void* logits, c
   TQ_REQUIRE(finished == nullptr || (end >= 0 && end < vocab), TQ_INVALID_ARGUMENT, "there is no token %lld among %lld to end with", (long long)end, (long long)vocab);
   TQ_REQUIRE(request_stride >= 0 && beam_stride >= 0 && tq::aligned_to(logits, tq::dtype_size(dtype)) && tq::aligned_to(scores, 4), TQ_UNSUPPORTED,
              "logits have no negative strides and are aligned to their type");
-  const tq::SelectPlan plan = tq::plan_select(requests * beams, vocab, keep);
-  TQ_REQUIRE(workspace != nullptr && workspace_bytes >= plan.sums_bytes + plan.keys_bytes && tq::aligned_to(workspace, 8), TQ_INVALID_ARGUMENT,
-             "this selection needs %zu bytes of workspace, 8-byte aligned, and was given %zu", plan.sums_bytes + plan.keys_bytes, workspace_bytes);
+  const tq::SelectPlan plan = tq::plan_select(requests * beams, vocab, keep, tq::dtype_size(dtype));
+  TQ_REQUIRE(workspace != nullptr && workspace_bytes >= plan.sums_bytes + plan.keys_bytes && tq::aligned_to(workspace, 16), TQ_INVALID_ARGUMENT,
+             "this selection needs %zu bytes of workspace, 16-byte aligned, and was given %zu", plan.sums_bytes + plan.keys_bytes, workspace_bytes);
   tq::DeviceScope device_scope(device);
   if (tq_status s = device_scope.status()) return s;
   tq::SelectParams p = {};
@@ -479,8 +628,8 @@ extern "C" tq_status tq_beam_select_launch(tq_dtype dtype, const void* logits, c
   p.parts = plan.parts;
   p.chunk = plan.chunk;
   p.end = static_cast<int>(end);
-  p.keys = static_cast<unsigned long long*>(workspace);
-  p.sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + plan.keys_bytes);
+  p.sums = static_cast<double2*>(workspace);
+  p.keys = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + plan.sums_bytes);
   p.out_scores = out_scores;
   p.out_parents = out_parents;
   p.out_tokens = out_tokens;

@@ -203,58 +203,47 @@ __device__ __forceinline__ void write_values(const KeyedParams& p, int batch, in
   }
 }
 
-// PREFIX: joined with the parts of the keys that the sequence shares with its run.
-template <typename T, int W, bool PREFIX>
+// PARTS: left as a part of the row's result.
+template <typename T, int W, bool PARTS>
 __device__ __forceinline__ void write_result(const KeyedParams& p, int batch, int kv_head, int row, int column, int length, float most, float total,
                                              const float (&value)[8]) {
-  if constexpr (!PREFIX) {
+  if constexpr (!PARTS) {
     write_values<T>(p, batch, kv_head, row, column, length, total, value);
   } else {
-    const int run = batch / p.each, shared = shared_keys(p, run);
-    float joined[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) joined[c] = value[c];
-    if (shared > 0 && takes_part(p, shared, length)) {
-      const int inside = (batch - run * p.each) * p.group * p.q_tokens + row, block = inside / p.prefix_rows;
-      const long long slot0 = static_cast<long long>((run * p.kv_heads + kv_head) * p.row_blocks + block) * p.splits;
-#pragma unroll 2
-      for (int part = 0; part < p.splits; ++part) {
-        const long long slot = (slot0 + part) * p.prefix_rows + (inside - block * p.prefix_rows);
-        const float2 stats = p.prefix_stats[slot];
-        if (stats.x == -INFINITY) continue;      // no keys (what lies there is nothing then)
-        const float4* from = reinterpret_cast<const float4*>(p.prefix_parts + slot * W + column);
-        const float4 near = from[0], far = from[1];
-        const float both = fmaxf(most, stats.x), mine = rescale(most, both), theirs = rescale(stats.x, both);
-        const float x[8] = {near.x, near.y, near.z, near.w, far.x, far.y, far.z, far.w};
-        most = both;
-        total = total * mine + stats.y * theirs;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) joined[c] = joined[c] * mine + x[c] * theirs;
-      }
-    }
-    write_values<T>(p, batch, kv_head, row, column, length, total, joined);
+    const int own = batch - p.runs, run = own < 0 ? batch : own / p.each;
+    const long long slot = part_slot(p, run, kv_head, own < 0 ? 0 : p.part_count - 1, own < 0 ? row : (own - run * p.each) * p.group * p.q_tokens + row);
+    float4* const to = reinterpret_cast<float4*>(p.row_parts + slot * W + column);
+    to[0] = make_float4(value[0], value[1], value[2], value[3]);
+    to[1] = make_float4(value[4], value[5], value[6], value[7]);
+    if (column == 0) p.row_stats[slot] = make_float2(most, total);
   }
 }
 
 // A sequence's chunks, by every query of it.
-template <int BITS, int CHUNK>
+template <int BITS, int CHUNK, bool PARTS>
 __device__ __forceinline__ int length_of(const KeyedParams& p, int sequence) {
   if constexpr (BITS == 16) return p.k_tokens;
+  if constexpr (PARTS) {
+    if (sequence < p.runs) return shared_keys(p, sequence);
+    sequence -= p.runs;
+  }
   return min(max(p.lengths[sequence], 0), p.blocks << p.page_shift);
 }
-// PREFIX: a list without the keys that the sequence shares with its run.
-template <int CHUNK, bool PREFIX>
+// PARTS: a list without the keys that the sequence shares with its run.
+template <int CHUNK, bool PARTS>
 __device__ __forceinline__ ChunkList behind_prefix(const KeyedParams& p, int sequence, int length, ChunkList list) {
-  if constexpr (PREFIX) {
+  if constexpr (PARTS) {
     static_assert(kPrefixTile % CHUNK == 0, "the keys behind the shared ones begin with a chunk");
-    const int shared = shared_keys(p, sequence / p.each);
+    if (sequence < p.runs) return list;
+    const int shared = shared_keys(p, (sequence - p.runs) / p.each);
     if (takes_part(p, shared, length)) list.start = min(max(list.start, shared / CHUNK), list.stop);
   }
   return list;
 }
-template <int BITS, int CHUNK, bool PREFIX>
+template <int BITS, int CHUNK, bool PARTS>
 __device__ __forceinline__ ChunkList sequence_chunks(const KeyedParams& p, int sequence, int length) {
-  return behind_prefix<CHUNK, PREFIX>(p, sequence, length, chunks_of(length - p.q_tokens, max(length - 1, -1), p.window, p.sinks, CHUNK));
+  // (rows of a run see all the shared keys; there is no window then)
+  return behind_prefix<CHUNK, PARTS>(p, sequence, length, chunks_of(length - p.q_tokens, max(length - 1, -1), p.window, p.sinks, CHUNK));
 }
 
 // Where the chunks of all units (sequence, key head, tile of rows) are dealt out as one range of equal shares, a CTA each: a place in that range.
@@ -264,9 +253,9 @@ struct Place {
 };
 
 // The chunks that a head of sequence `sequence` counts for: one at least, so that each has somebody to write its result.
-template <int BITS, int CHUNK, bool PREFIX>
+template <int BITS, int CHUNK, bool PARTS>
 __device__ __forceinline__ int counted(const KeyedParams& p, int sequence) {
-  return max(sequence_chunks<BITS, CHUNK, PREFIX>(p, sequence, length_of<BITS, CHUNK>(p, sequence)).count(), 1);
+  return max(sequence_chunks<BITS, CHUNK, PARTS>(p, sequence, length_of<BITS, CHUNK, PARTS>(p, sequence)).count(), 1);
 }
 
 // What a unit costs beside its chunks, in chunks: to find it, its pages and its first keys, one after another, and its masked ends. Measured with
@@ -287,14 +276,14 @@ struct Dealt {
 };
 
 // All threads: the range, and where in it the share of each warp, first_share + warp, starts. Each thread adds up a run of sequences.
-template <int BITS, int CHUNK, bool PREFIX>
+template <int BITS, int CHUNK, bool PARTS>
 __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Place& place) {
   __shared__ int warp_sum_of[kKeyedWarps];
   __shared__ Place found[kKeyedWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int units = p.kv_heads * p.row_tiles;
   if constexpr (BITS == 16) {      // all sequences are alike
-    const int each = (unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, 0)) * units;
+    const int each = (unit_cost(CHUNK) + counted<BITS, CHUNK, PARTS>(p, 0)) * units;
     Dealt dealt;
     dealt.total = each * p.batch;
     dealt.shares = min(p.shares, (dealt.total + kLeastShare - 1) / kLeastShare);
@@ -307,7 +296,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
   const int run = (p.batch + kKeyedThreads - 1) / kKeyedThreads;
   const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
   int mine = 0;
-  for (int b = first; b < last; ++b) mine += unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, b);
+  for (int b = first; b < last; ++b) mine += unit_cost(CHUNK) + counted<BITS, CHUNK, PARTS>(p, b);
   mine *= units;
   int upto = mine;
 #pragma unroll
@@ -335,7 +324,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
     if (before <= at && at < upto) {
       int b = first;
       for (; b < last; ++b) {
-        const int here = (unit_cost(CHUNK) + counted<BITS, CHUNK, PREFIX>(p, b)) * units;
+        const int here = (unit_cost(CHUNK) + counted<BITS, CHUNK, PARTS>(p, b)) * units;
         if (at < before + here) break;
         before += here;
       }
@@ -350,7 +339,7 @@ __device__ __forceinline__ Dealt deal(const KeyedParams& p, int first_share, Pla
 // T: the type of q and out. BITS, W as above. NT: eights of rows of a tile. JOINS > 0 (SHARED): the chunks of all units are dealt out in equal
 // shares, one a warp (then keyed_join_kernel follows), or each unit has a CTA, whose warps take every WARPS-th chunk each and meet in shared
 // memory. ONE: a chunk lies in one page (or in none: dense keys).
-template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps, bool PREFIX = false>
+template <typename T, int BITS, int W, int NT, int JOINS, bool ONE, int WARPS = kKeyedWarps, bool PARTS = false>
 __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
 keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KeyedParams p) {
   using S = KeyedShape<BITS, W>;
@@ -378,8 +367,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
   }
-  wait_for_earlier();
-  if constexpr (SHARED) let_later_start();      // (the joining kernel; see launch_overlapped)
+  if (!PARTS || !p.late) wait_for_earlier();
+  if constexpr (SHARED || PARTS) let_later_start();      // (the joining kernel, or the next part's; see launch_overlapped)
   if (blockIdx.x == 0 && threadIdx.x == 0) p.status.begin();
   __syncwarp();
   // JOINS > 1: what a warp has of units that others have parts of too: of one that began before its share (0), of one that goes on behind it (1)
@@ -394,7 +383,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   if (JOINS > 1 && lane == 0) pieces[JOINS > 1 ? warp : 0][0].there = pieces[JOINS > 1 ? warp : 0][1].there = false;      // (by the lane that fills them in)
   uint32_t turn = 0;                                   // chunks this warp has waited for: the stage and the phase of the next
   const int quad = lane >> 2, corner = lane & 3;       // the instruction's row (or column) of eight, and the lane's place in it
-  const int rows = p.group * p.q_tokens;               // of a key head: row = token * group + head in the group
+  const int rows_each = p.group * p.q_tokens;          // of a sequence and key head: row = token * group + head in the group
 
   // SHARED: this warp's share of the range, [at, until)
   constexpr int kStep = SHARED ? 1 : WARPS;            // a warp takes every chunk of its share, or every WARPS-th of the unit
@@ -403,7 +392,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   int at = 0, until = 1;
   Dealt dealt = {};
   if constexpr (SHARED) {
-    dealt = deal<BITS, S::kKeys, PREFIX>(p, blockIdx.x * kKeyedWarps, place);
+    dealt = deal<BITS, S::kKeys, PARTS>(p, blockIdx.x * kKeyedWarps, place);
     if (lane == 0) p.borders[share] = make_int4(0, 0, 0, 0);               // (the border behind this share; see below)
     if (share < dealt.shares) {
       at = dealt.start(share);
@@ -420,8 +409,8 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     ChunkList list;
     if constexpr (SHARED) {
       batch = place.sequence;
-      counted_length = length_of<BITS, S::kKeys>(p, batch);
-      list = sequence_chunks<BITS, S::kKeys, PREFIX>(p, batch, counted_length);
+      counted_length = length_of<BITS, S::kKeys, PARTS>(p, batch);
+      list = sequence_chunks<BITS, S::kKeys, PARTS>(p, batch, counted_length);
       const int cost = kUnitCost + max(list.count(), 1), units = p.kv_heads * p.row_tiles;
       const int inside = at - place.before;
       const int unit = inside / cost;
@@ -448,24 +437,42 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       const long long head_index = unit / p.row_tiles;
       kv_head = static_cast<int>(head_index % p.kv_heads);
       batch = static_cast<int>(head_index / p.kv_heads);
-      counted_length = length_of<BITS, S::kKeys>(p, batch);
+      counted_length = length_of<BITS, S::kKeys, PARTS>(p, batch);
       at = until;
     }
     const int length = counted_length;
+    const bool all_see = PARTS && batch < p.runs;        // a run, whose every row sees every key
+    const int own = PARTS ? batch - p.runs : batch, rows = all_see ? p.each * rows_each : rows_each;
     const int row0 = tile * kRows;
     if constexpr (BITS == 8) {
-      if ((SHARED ? lane : threadIdx.x) == 0 && p.lengths[batch] > length) report(p.status, kKeyedLength, batch, p.lengths[batch]);      // the table does not go that far
+      if ((SHARED ? lane : threadIdx.x) == 0 && !all_see && p.lengths[own] > length) report(p.status, kKeyedLength, own, p.lengths[own]);      // the table does not go that far
     }
     const int first_token = row0 / p.group, last_token = (min(row0 + kRows, rows) - 1) / p.group;
-    const int low = length - p.q_tokens + first_token, high = length - p.q_tokens + last_token;
+    const int low = all_see ? length - 1 : length - p.q_tokens + first_token, high = all_see ? length - 1 : length - p.q_tokens + last_token;
     if constexpr (!SHARED) {
-      list = behind_prefix<S::kKeys, PREFIX>(p, batch, length, chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys));
+      list = behind_prefix<S::kKeys, PARTS>(p, batch, length, chunks_of(low, max(high, -1), p.window, p.sinks, S::kKeys));
       last_chunk = list.count();
     }
 
     // ---- the warp's chunks ----
     if constexpr (!SHARED) first_chunk = warp;
-    const int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
+    int mine = max(last_chunk - first_chunk + kStep - 1, 0) / kStep;
+    long long table_row = own;
+    if constexpr (PARTS) {
+      if (all_see) {                                     // through the table row of the first sequence that is long enough; none is: nobody wants it
+        int taker = 0x7fffffff;
+        for (int i = lane; i < p.each; i += 32) {
+          const int theirs = min(max(p.lengths[batch * p.each + i], 0), p.blocks << p.page_shift);
+          if (takes_part(p, length, theirs)) {
+            taker = i;
+            break;
+          }
+        }
+        taker = __reduce_min_sync(0xffffffffu, taker);
+        if (taker == 0x7fffffff) mine = 0;
+        else table_row = static_cast<long long>(batch) * p.each + taker;
+      }
+    }
     auto chunk_at = [&](int n) { return list.at(first_chunk + n * kStep); };
     // Lane l looks up the page of box l % boxes of chunk n + l / boxes, so one look-up serves the next 32 / boxes chunks. Pages that no row sees are
     // not looked at: a window may have left them behind, and the table may name anything there.
@@ -478,9 +485,9 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const int key = chunk_at(n) * S::kKeys + (ONE ? 0 : (lane % boxes) << box_shift);
         if (key > high || (key + box_keys - 1 <= low - p.window && key >= p.sinks)) return -1;
         const int at_block = key >> p.page_shift;
-        const int page = p.table[batch * p.table_stride + at_block];
+        const int page = p.table[table_row * p.table_stride + at_block];
         if (page >= 0 && page < p.pages) return page;
-        report(p.status, kKeyedPage, batch, at_block);
+        report(p.status, kKeyedPage, static_cast<int>(table_row), at_block);
       }
       return -1;
     };
@@ -491,8 +498,9 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + n * 8 + quad;
-      const int token = row / p.group, head = kv_head * p.group + row % p.group;
-      const T* from = static_cast<const T*>(p.q) + batch * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
+      const int inside = all_see ? row % rows_each : row, token = inside / p.group, head = kv_head * p.group + inside % p.group;
+      const long long sequence = all_see ? static_cast<long long>(batch) * p.each + row / rows_each : own;
+      const T* from = static_cast<const T*>(p.q) + sequence * p.q_strides[0] + head * p.q_strides[1] + token * p.q_strides[2];
 #pragma unroll
       for (int j = 0; j < S::kPieces; ++j) {
         const int column = (4 * j + corner) * S::kPieceWidth;
@@ -615,7 +623,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       for (int e = 0; e < 2; ++e) {
         row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * corner + e) * 4);
         const int here = row0 + n * 8 + 2 * corner + e;
-        position[n][e] = here < rows ? length - p.q_tokens + here / p.group : high;
+        position[n][e] = here < rows && !all_see ? length - p.q_tokens + here / p.group : high;
       }
     }
 
@@ -997,7 +1005,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const int column = column_of(run);
             if (column >= p.head_dim) continue;
             if (whole) {
-              write_result<T, W, PREFIX>(p, batch, kv_head, row0 + row, column, length, top[n][e], sum[n][e], value);
+              write_result<T, W, PARTS>(p, batch, kv_head, row0 + row, column, length, top[n][e], sum[n][e], value);
             } else {
               float4* to = reinterpret_cast<float4*>((JOINS > 1 ? piece_at(warp, begins ? 1 : 0) + row * W : p.parts + (slot0 + row) * W) + column);
               to[0] = make_float4(value[0], value[1], value[2], value[3]);
@@ -1041,11 +1049,11 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
           for (int c = 0; c < 8; ++c) value[c] += reinterpret_cast<const float*>(parts_at + w * kWarpRing)[row * W + column + c] * by;
         }
-        write_result<T, W, PREFIX>(p, batch, kv_head, row0 + row, column, length, most, total, value);
+        write_result<T, W, PARTS>(p, batch, kv_head, row0 + row, column, length, most, total, value);
       }
     }
   }
-  if constexpr (!SHARED) let_later_start();
+  if constexpr (!SHARED && !PARTS) let_later_start();
   if constexpr (JOINS > 1) {
     // The pieces of a unit meet, in the order of the warps; what other CTAs have parts of too goes to memory, as the part of the first of its
     // warps.
@@ -1072,7 +1080,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll 1
       for (int item = threadIdx.x; item < kRows * (W / 8); item += kKeyedThreads) {
         const int row = item / (W / 8), column = item % (W / 8) * 8;
-        if (tile * kRows + row >= rows || column >= p.head_dim) continue;
+        if (tile * kRows + row >= (PARTS && head.sequence < p.runs ? p.each : 1) * rows_each || column >= p.head_dim) continue;
         float most = -INFINITY, total = 0.f, value[8] = {};
 #pragma unroll 1
         for (int j = i; j <= last; ++j) {
@@ -1088,7 +1096,7 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           for (int c = 0; c < 8; ++c) value[c] = value[c] * mine + x[c] * theirs;
         }
         if (whole) {
-          write_result<T, W, PREFIX>(p, head.sequence, kv_head, tile * kRows + row, column, length_of<BITS, S::kKeys>(p, head.sequence), most, total, value);
+          write_result<T, W, PARTS>(p, head.sequence, kv_head, tile * kRows + row, column, length_of<BITS, S::kKeys, PARTS>(p, head.sequence), most, total, value);
         } else {
           float4* to = reinterpret_cast<float4*>(p.parts + (slot0 + row) * W + column);
           to[0] = make_float4(value[0], value[1], value[2], value[3]);
@@ -1099,12 +1107,13 @@ keyed_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       i = last + 1;
     }
   }
+  if (PARTS && p.late) wait_for_earlier();      // (what comes after this kernel comes after the one before it)
 }
 
 // SHARED: joins the parts of the units that a border between two shares (or two CTAs' shares: JOINS of them) cut. A CTA for each border; the CTAs
 // of a unit's borders split its result, 64 elements of a row at a time: eight lanes of eight elements, by as many groups as there are parts, four
 // groups in a warp or, of many parts, sixteen in the CTA.
-template <typename T, int W, int NT, int JOINS, bool PREFIX = false>
+template <typename T, int W, int NT, int JOINS, bool PARTS = false>
 __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_constant__ KeyedParams p) {
   constexpr int kRows = 8 * NT;
   __shared__ float2 warp_stats[kKeyedWarps][8];
@@ -1116,8 +1125,8 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
   const int borders = last / JOINS - first / JOINS, nth = share / JOINS - first / JOINS, parts = borders + 1;
   if (first == last || borders == 0) return;              // it lies between two units
   const int tile = unit % p.row_tiles, kv_head = unit / p.row_tiles;
-  const int rows = min(kRows, p.group * p.q_tokens - tile * kRows);
-  const int length = p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
+  const int rows = min(kRows, (PARTS && batch < p.runs ? p.each : 1) * p.group * p.q_tokens - tile * kRows);
+  const int length = PARTS ? 0 : p.lengths == nullptr ? p.k_tokens : min(max(p.lengths[batch], 0), p.blocks << p.page_shift);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool many = JOINS > 1 && parts > 16;              // (uniform in the CTA)
   constexpr int kAtOnce = NT == 1 ? 2 : 4;                // rows whose loads are under way together
@@ -1198,7 +1207,7 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
         }
       }
       if (item < items && lane < 8 && (!many || warp == 0) && column < p.head_dim)
-        write_result<T, W, PREFIX>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, most[i], total[i], value[i]);
+        write_result<T, W, PARTS>(p, batch, kv_head, tile * kRows + item / (W / 64), column, length, most[i], total[i], value[i]);
     }
   }
 }
@@ -1247,12 +1256,13 @@ constexpr int kManyParts = 8;
 struct KeyedPlan {
   int nt, row_tiles, shares, joins, warps;      // shares 0: a CTA of `warps` a unit
   size_t bytes;
+  double time;                                  // expected, us
 };
 
 template <int BITS, int W>
 KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   KeyedPlan plan = {};
-  const int rows = p.group * p.q_tokens;
+  const int rows = (p.runs > 0 ? p.each : 1) * p.group * p.q_tokens;
   plan.nt = rows <= 8 ? 1 : 2;
   plan.row_tiles = (rows + 8 * plan.nt - 1) / (8 * plan.nt);
   // a tile's own, and of all the sequence's queries together, which is what every tile walks where chunks are dealt out
@@ -1260,6 +1270,7 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const long long own = most_chunks(p, tokens < p.q_tokens ? tokens : p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long chunks = most_chunks(p, p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
+  const long long average = p.typical > 0 && p.typical < keys ? most_chunks(p, p.q_tokens, p.typical, KeyedShape<BITS, W>::kKeys) : chunks;
   const int sixteen = plan.nt - 1;
   auto most_of = [&](auto joins, auto warps) {
     constexpr int kJoins = decltype(joins)::value, kWarps = decltype(warps)::value;
@@ -1270,15 +1281,17 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
     constexpr int kWarps = decltype(warps)::value;
     const double most = most_of(std::integral_constant<int, 0>{}, warps), waves = units <= most ? 1.0 : std::ceil(units / most);
     const double memory = (units < most ? units : most) * kWarps * kStageBytes / kBytesPerMicrosecond[sixteen];
-    const double steps = static_cast<double>((own + kWarps - 1) / kWarps);
-    return kWholeTime + waves * steps * (memory > kStepTime[sixteen] ? memory : kStepTime[sixteen]) + (waves - 1) * kWaveTime;
+    const double steps = static_cast<double>((own + kWarps - 1) / kWarps), step = memory > kStepTime[sixteen] ? memory : kStepTime[sixteen];
+    if (average < own) return kWholeTime + steps * step + (waves - 1) * (std::ceil(static_cast<double>(average) / kWarps) * step + kWaveTime);
+    return kWholeTime + waves * steps * step + (waves - 1) * kWaveTime;
   };
   const double times[3] = {whole_time(std::integral_constant<int, 2>{}), whole_time(std::integral_constant<int, 4>{}), whole_time(std::integral_constant<int, 8>{})};
   int best = 0;
   for (int i = 1; i < 3; ++i)
     if (times[i] < times[best]) best = i;
   plan.warps = 2 << best;
-  const double dealt = kDealtTime + static_cast<double>(chunks) * units * kStageBytes / kBytesPerMicrosecond[sixteen];
+  const double dealt = kDealtTime + static_cast<double>(average) * units * kStageBytes / kBytesPerMicrosecond[sixteen];
+  plan.time = times[best] < dealt ? times[best] : dealt;
   const bool whole = (own + plan.warps - 1) / plan.warps <= kMostSteps && times[best] <= dealt;
   if (!whole && chunks <= 2 * own && (chunks + unit_cost(KeyedShape<BITS, W>::kKeys)) * units < (1LL << 31)) {
     const int most = most_of(std::integral_constant<int, 1>{}, std::integral_constant<int, kKeyedWarps>{});
@@ -1340,7 +1353,7 @@ tq_status keyed_maps(CUtensorMap* maps, KeyedParams& p) {
   return TQ_OK;
 }
 
-template <typename T, int BITS, int W, int NT, bool PREFIX>
+template <typename T, int BITS, int W, int NT, bool PARTS>
 tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   CUtensorMap maps[2] = {};
   if (tq_status s = keyed_maps<T, BITS, W>(maps, p)) return s;
@@ -1353,9 +1366,9 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
   auto start_boxes = [&](auto joins, auto each, long long ctas) {
     constexpr int kJoins = decltype(joins)::value, kWarps = decltype(each)::value;
     if constexpr (BITS == 8) {
-      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false, kWarps, PREFIX>, kWarps, ctas);
+      if (p.boxes > 1) return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, false, kWarps, PARTS>, kWarps, ctas);
     }
-    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true, kWarps, PREFIX>, kWarps, ctas);
+    return start(keyed_attention_kernel<T, BITS, W, NT, kJoins, true, kWarps, PARTS>, kWarps, ctas);
   };
   constexpr std::integral_constant<int, 0> kWhole{};
   constexpr std::integral_constant<int, kKeyedWarps> kFour{};
@@ -1366,25 +1379,27 @@ tq_status launch_keyed(KeyedParams& p, int warps, cudaStream_t stream) {
                                                                                               : start_boxes(kWhole, std::integral_constant<int, 8>{}, units);
   }
   const bool gathers = p.joins > 1;
-  // both launches, one after the other: recorded ones may share their scratch on a stream (behind prefix.cu's kernel its caller holds it)
-  const auto held = hold_scratch(PREFIX ? nullptr : p.borders);
+  // both launches, one after the other: recorded ones may share their scratch on a stream (of parts, prefix.cu holds it)
+  const auto held = hold_scratch(PARTS ? nullptr : p.borders);
   if (tq_status s = gathers ? start_boxes(kFour, kFour, p.shares / kKeyedWarps) : start_boxes(std::integral_constant<int, 1>{}, kFour, p.shares / kKeyedWarps)) return s;
   const dim3 borders(static_cast<unsigned>((p.shares - 1) / p.joins + (p.joins == 1 ? 0 : 1)));
-  TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps, PREFIX>, borders, kKeyedThreads, 0, stream, p)
-                  : launch_overlapped(keyed_join_kernel<T, W, NT, 1, PREFIX>, borders, kKeyedThreads, 0, stream, p));
+  TQ_CUDA(gathers ? launch_overlapped(keyed_join_kernel<T, W, NT, kKeyedWarps, PARTS>, borders, kKeyedThreads, 0, stream, p)
+                  : launch_overlapped(keyed_join_kernel<T, W, NT, 1, PARTS>, borders, kKeyedThreads, 0, stream, p));
   return check_launch("keyed_join_kernel");
 }
 
-template <typename T, int BITS, bool PREFIX = false>
+template <typename T, int BITS, bool PARTS = false>
 tq_status launch_keyed_width(KeyedParams& p, const KeyedPlan& plan, cudaStream_t stream) {
   if (p.head_dim <= 64)
-    return plan.nt == 1 ? launch_keyed<T, BITS, 64, 1, PREFIX>(p, plan.warps, stream) : launch_keyed<T, BITS, 64, 2, PREFIX>(p, plan.warps, stream);
-  return plan.nt == 1 ? launch_keyed<T, BITS, 128, 1, PREFIX>(p, plan.warps, stream) : launch_keyed<T, BITS, 128, 2, PREFIX>(p, plan.warps, stream);
+    return plan.nt == 1 ? launch_keyed<T, BITS, 64, 1, PARTS>(p, plan.warps, stream) : launch_keyed<T, BITS, 64, 2, PARTS>(p, plan.warps, stream);
+  return plan.nt == 1 ? launch_keyed<T, BITS, 128, 1, PARTS>(p, plan.warps, stream) : launch_keyed<T, BITS, 128, 2, PARTS>(p, plan.warps, stream);
 }
 
 }  // namespace
 
 size_t keyed_workspace(bool paged, const KeyedParams& p, long long keys, int32_t device) { return plan_keyed(paged, p, keys, device).bytes; }
+
+double keyed_time(bool paged, const KeyedParams& p, long long keys, int32_t device) { return plan_keyed(paged, p, keys, device).time; }
 
 tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long keys, void* workspace, size_t workspace_bytes, int32_t device,
                           cudaStream_t stream) {

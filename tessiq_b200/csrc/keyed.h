@@ -26,11 +26,17 @@ struct KeyedParams {
   float2* part_stats;                                                      // ... their maximum and sum
   float scale_log2;
   WaitStatus status;
-  // Sequences in runs of `each` that share their first keys, whose part of the result prefix.cu leaves (null: none do).
+  // Sequences in runs of `each` that share their first keys (null: none do). Parts of a row's result are left, not the result: prefix.cu joins them.
   const int32_t* shared;                                                   // of each run: how many first keys its sequences have in common
-  int each, prefix_rows, row_blocks, splits;                               // rows of a block, blocks of a run and key head, parts of each
-  float* prefix_parts;                                                     // [run][key head][block][part][row][64 or 128]
-  float2* prefix_stats;                                                    // ... their maximum and sum
+  int each;
+  int runs;                                                                // so many of the first "sequences" are runs: the shared keys, for the rows of
+                                                                           // a run together; the others are sequences, and what each has behind them
+  bool late;                                                               // the kernel before in the stream leaves other parts and need not have ended
+  int typical;                                                             // for the plan: the keys a unit has on average, where that is known to be less
+                                                                           // than the most; else 0
+  int part_rows, part_count;                                               // rows of a run and key head, rounded up; parts of each, the sequences' own last
+  float* row_parts;                                                        // [run][key head][part][row][64 or 128]
+  float2* row_stats;                                                       // ... their maximum and sum
 };
 
 // The keys of a run's beginning are taken together in tiles of so many; what is left of it each sequence reads itself.
@@ -86,8 +92,10 @@ inline void keyed_extents(KeyedParams& p, int64_t batch, int64_t heads, int64_t 
 constexpr float kHalfLift = 7.f;
 
 // Few rows a key head against many keys: `p` is complete but for what follows from the plan; no sequence has more than `keys` keys. With `p.shared`
-// (paged keys, no window): the keys behind the shared ones, joined with what prefix.cu has left in p.prefix_parts.
+// (paged keys, no window): parts of the rows' results.
 size_t keyed_workspace(bool paged, const KeyedParams& p, long long keys, int32_t device);
+// The time it is expected to take, us.
+double keyed_time(bool paged, const KeyedParams& p, long long keys, int32_t device);
 tq_status keyed_attention(tq_dtype dtype, bool paged, KeyedParams& p, long long keys, void* workspace, size_t workspace_bytes, int32_t device,
                           cudaStream_t stream);
 
@@ -120,6 +128,10 @@ __device__ __forceinline__ int shared_keys(const KeyedParams& p, int run) {
   return min(max(p.shared[run], 0), p.blocks << p.page_shift) / kPrefixTile * kPrefixTile;
 }
 __device__ __forceinline__ bool takes_part(const KeyedParams& p, int shared, int length) { return length - p.q_tokens + 1 >= shared; }
+// Where part `part` of a row (of the run's rows of a key head) lies.
+__device__ __forceinline__ long long part_slot(const KeyedParams& p, int run, int kv_head, int part, int row) {
+  return ((static_cast<long long>(run) * p.kv_heads + kv_head) * p.part_count + part) * p.part_rows + row;
+}
 
 // The first fault since the last poll is kept, with where it was.
 __device__ __forceinline__ void report(const WaitStatus& status, int code, int sequence, int what) {

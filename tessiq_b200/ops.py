@@ -883,7 +883,7 @@ def beam_select(logits, scores, keep, finished=None, end=0):
     device = _device_of([t for t in (logits, scores, finished) if t is not None])
     out = tuple(torch.empty(requests, keep, dtype=dtype, device=logits.device) for dtype in (torch.float32, torch.int32, torch.int32))
     nbytes = ctypes.c_size_t()
-    check(lib.tq_beam_select_workspace_bytes(requests, beams, vocab, keep, ctypes.byref(nbytes)))
+    check(lib.tq_beam_select_workspace_bytes(dtype_code(logits.dtype), requests, beams, vocab, keep, ctypes.byref(nbytes)))
     scratch = _own_scratch(nbytes.value, device)
     ints = (requests, beams, vocab, keep, end, logits.stride(0), logits.stride(1))
     check(lib.tq_beam_select_launch(dtype_code(logits.dtype), _pointer(logits), _pointer(scores), _pointer(finished), *[_pointer(t) for t in out], *ints,
