@@ -529,9 +529,10 @@ tq_status tq_cache_attention_launch(tq_dtype dtype, const void* q, const void* k
  * the table row of the first of those; what is left of them, and the shared tokens of shorter sequences (a padded row of length 0 among them), each
  * sequence reads itself. shared[r] <= 0: nothing is shared. `workspace` as there, tq_prefix_attention_workspace_bytes of it. */
 /* Which way the launch takes: each sequence reads all its keys (TQ_ATTENTION_APART), or the shared ones are read for all rows of a run together, streamed
- * (TQ_ATTENTION_STREAMED) or on tensor-core tiles (TQ_ATTENTION_TILES), in so many parts; device -1: on a B200, without a GPU. */
+ * (TQ_ATTENTION_STREAMED) or on tensor-core tiles (TQ_ATTENTION_TILES), in so many parts, of so many rows (128 or 256 on tiles); device -1: on a
+ * B200, without a GPU. */
 tq_status tq_prefix_attention_form(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens, int64_t blocks,
-                                   int64_t runs, int32_t device, int32_t* form, int32_t* parts);
+                                   int64_t runs, int32_t device, int32_t* form, int32_t* parts, int32_t* block_rows);
 tq_status tq_prefix_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens,
                                               int64_t blocks, int64_t runs, int32_t device, size_t* bytes);
 tq_status tq_prefix_attention_launch(tq_dtype dtype, const void* q, const void* k_pages, const void* v_pages, const float* k_scales,

@@ -106,7 +106,7 @@ SIGNATURES = {
                                   + [c_double, c_int64, c_int64, c_void_p, c_size_t, c_int32, c_void_p]),
     "tq_cache_store_launch": (c_int32, [c_int32] + [c_void_p] * 9 + [c_int64] * 8 + [POINTER(c_int64)] * 2 + [c_int32, c_void_p]),
     "tq_copy_pages_launch": (c_int32, [POINTER(tq_paged_tensor), c_int32, c_int64, POINTER(c_int64), POINTER(c_int64), c_int64, c_int32, c_void_p]),
-    "tq_prefix_attention_form": (c_int32, [c_int64] * 8 + [c_int32, POINTER(c_int32), POINTER(c_int32)]),
+    "tq_prefix_attention_form": (c_int32, [c_int64] * 8 + [c_int32] + [POINTER(c_int32)] * 3),
     "tq_prefix_attention_workspace_bytes": (c_int32, [c_int64] * 8 + [c_int32, POINTER(c_size_t)]),
     "tq_prefix_attention_launch": (c_int32, [c_int32] + [c_void_p] * 9 + [c_int64] * 10 + [POINTER(c_int64)] * 2
                                    + [c_double, c_void_p, c_size_t, c_int32, c_void_p]),

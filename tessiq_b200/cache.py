@@ -2,7 +2,8 @@
 
 `Pages` keeps the books on the host (no GPU): pages are handed out, shared by forked sequences, copied when one of
 them writes, taken back and moved together. `PagedCache` has the memory of all layers and makes the launches: `ops.cache_store`,
-`ops.cache_attention` and `ops.copy_pages`, on torch's current stream. The reference has no cache; its models run whole
+`ops.cache_attention` or `ops.prefix_attention`, and `ops.copy_pages`, on torch's current stream. `Beams` are rows whose books are on the device
+(`ops.cache_advance`), for a search that goes on without the host. The reference has no cache; its models run whole
 sequences (tests/python/test_models.py:64-67).
 
     cache = PagedCache(layers=12, kv_heads=12, width=64, pages=4096)
@@ -14,6 +15,12 @@ sequences (tests/python/test_models.py:64-67).
     cache.store(step, layer, k, v)
     out = cache.attention(step, layer, q, window=1024, sinks=4)
     cache.truncate(b, 30); cache.free(a); cache.compact()
+
+    search = cache.beams([a], 4, 64)                    # four rows that go on from a, up to 64 tokens each
+    step = search.step(parents)                         # row r goes on from row parents[r] (None: each from itself), with one token more
+    cache.store(step, layer, k, v); out = cache.attention(step, layer, q)       # all of it can be captured into a graph
+    scores, parents, tokens = ops.beam_select(logits, scores, 4)
+    best = search.keep(0); search.free()                # row 0 becomes a sequence like others
 
 Not for several host threads at once.
 """
@@ -158,6 +165,32 @@ class Pages:
             self._sequences[sequence] = (pages, length)
         return sources, targets
 
+    def reserve(self, count: int) -> list[int]:
+        """`count` pages that belong to no sequence yet; `drop` gives them back."""
+        if count > len(self._free):
+            raise MemoryError(f"{count} pages are needed and {len(self._free)} are free")
+        return [self._take() for _ in range(count)]
+
+    def drop(self, pages: Sequence[int]) -> None:
+        for page in pages:
+            self._drop(page)
+
+    def adopt(self, pages: Sequence[int], length: int) -> int:
+        """A sequence of `length` tokens on pages that others have (`reserve`, sequences), who keep their hold on them."""
+        for page in pages:
+            self.references[page] += 1
+        return self._add(list(pages), length)
+
+    def shared_tokens(self, sequences: Sequence[int]) -> int:
+        """How many first tokens of all of `sequences` lie on the same pages."""
+        rows = [self._of(sequence) for sequence in sequences]
+        common = 0
+        for pages in zip(*[pages for pages, _ in rows]):
+            if len(set(pages)) > 1:
+                break
+            common += 1
+        return min([common * self.page_tokens, *[length for _, length in rows]])
+
     def compact(self) -> tuple[list[int], list[int]]:
         """Gives the pages in use the lowest numbers. Returns the pages to copy, (from, to)."""
         used = len(self.references) - len(self._free)
@@ -186,8 +219,11 @@ class Step:
     counts: torch.Tensor
     lengths: torch.Tensor    # starts + counts
     tokens: int              # the largest count
+    shared: torch.Tensor | None = None      # int32 [runs]: how many first tokens the sequences of each of as many equal runs have in common
     changes: int = 0         # the books' counts as the step was made (Pages.changes, Pages.changes_of each sequence)
     sequences: dict[int, tuple[int, int]] = field(default_factory=dict)
+    search: Beams | None = None      # whose step it is, and its number
+    number: int = 0
 
 
 class PagedCache:
@@ -202,6 +238,7 @@ class PagedCache:
         self.k_scales, self.v_scales = (torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
         self.layers = layers
         self.books = Pages(pages, page_tokens)
+        self._searches = 0       # `Beams` that have not been freed
 
     @property
     def tensors(self) -> list[torch.Tensor]:
@@ -231,10 +268,14 @@ class PagedCache:
         if self.k_scales.is_cuda and (torch.cuda.is_current_stream_capturing() or ops.lib.tq_is_recording()):
             raise RuntimeError(f"{what} keeps its books on the host and cannot go into a graph or a recording; storing and attention of a step can")
 
-    def extend(self, sequences: Sequence[int], tokens) -> Step:
-        """Room for `tokens` (one number, or one for each) tokens more in each of `sequences`; last pages that forks share are copied first."""
+    def extend(self, sequences: Sequence[int], tokens, runs: int | None = None) -> Step:
+        """Room for `tokens` (one number, or one for each) tokens more in each of `sequences`; last pages that forks share are copied first. `runs`:
+        the sequences are as many equal runs of neighbours that go back to a common beginning (forks of one prompt), whose attention reads
+        what is still common to all of a run once; None: each reads its own."""
         self._not_in_a_graph("extend")
         sequences = list(sequences)
+        if runs is not None and (runs < 1 or len(sequences) % runs):
+            raise ValueError(f"{len(sequences)} sequences are not {runs} equal runs")
         counts = [int(tokens)] * len(sequences) if isinstance(tokens, int) else [int(count) for count in tokens]
         starts = [self.books.length(sequence) for sequence in sequences]
         sources, targets = self.books.extend(sequences, counts)
@@ -244,15 +285,19 @@ class PagedCache:
         blocks = max([len(row) for row in rows], default=0)
         numbers = [page for row in rows for page in row + [0] * (blocks - len(row))]
         batch = len(sequences)
-        host = torch.tensor([*numbers, *starts, *counts, *[s + c for s, c in zip(starts, counts)]], dtype=torch.int32)
+        each = len(sequences) // runs if runs else 0
+        shared = [self.books.shared_tokens(sequences[r * each : (r + 1) * each]) for r in range(runs or 0)] if each else []
+        host = torch.tensor([*numbers, *starts, *counts, *[s + c for s, c in zip(starts, counts)], *shared], dtype=torch.int32)
         if self.k_scales.is_cuda:
             host = host.pin_memory()
         there = host.to(self.k_scales.device, non_blocking=True)
-        table, starts, counts_there, lengths = there.split([batch * blocks, batch, batch, batch])
-        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), self.books.changes,
+        table, starts, counts_there, lengths, shared = there.split([batch * blocks, batch, batch, batch, len(shared)])
+        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), shared if each else None, self.books.changes,
                     {sequence: self.books.changes_of(sequence) for sequence in sequences})
 
     def _good(self, step: Step, stores: bool) -> None:
+        if step.search is not None and (step.search.cache is not self or step.search.steps != step.number):
+            raise ValueError("the step of the beams is over: another one has been made since, or they have been freed")
         if step.changes == self.books.changes:
             return
         for sequence, (moved, copied) in step.sequences.items():
@@ -274,12 +319,99 @@ class PagedCache:
     def attention(self, step: Step, layer: int, q: torch.Tensor, window=None, sinks=0, scale=None, token_major=True) -> torch.Tensor:
         """q [batch, heads, q_tokens, width] are the last `q_tokens` tokens of each sequence (a query before its first token gives zeros)."""
         self._good(step, False)
+        if step.shared is not None and window is None:
+            return ops.prefix_attention(q, *self.layer(layer), step.table, step.lengths, step.shared, scale, token_major)
         return ops.cache_attention(q, *self.layer(layer), step.table, step.lengths, window, sinks, scale, token_major)
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers; how many moved. Steps from before must not be used again."""
         self._not_in_a_graph("compact")
+        if self._searches:
+            raise RuntimeError("beams have pages that only the device's books know: free them before compact")
         sources, targets = self.books.compact()
         if sources:
             ops.copy_pages(self.tensors, sources, targets, page_axis=1)
         return len(sources)
+
+    def beams(self, sequences: Sequence[int], beams: int, tokens: int) -> Beams:
+        """`beams` rows for each of `sequences`, which go on from it; see `Beams`."""
+        return Beams(self, sequences, beams, tokens)
+
+
+class Beams:
+    """Rows that go on from some sequences, `beams` of them each, by up to `tokens` tokens, as a search's beams do: which pages each has is known to the device
+    alone, and a step needs nothing of the host. A sequence's whole pages are all its rows' together; behind them the rows have pages that are set aside for
+    them here, as many as they can ever need at once. The sequences may be extended, truncated or freed meanwhile; `compact` has to wait for `free`.
+
+    `rows` of the batch: sequence s's beams are rows s * beams to (s + 1) * beams - 1. A step is good until the next one is made: its tensors are the
+    search's own."""
+
+    def __init__(self, cache: PagedCache, sequences: Sequence[int], beams: int, tokens: int):
+        cache._not_in_a_graph("beams")
+        sequences = list(sequences)
+        if beams < 1 or tokens < 0 or not sequences:
+            raise ValueError(f"no search of {beams} beams of {tokens} tokens for {len(sequences)} sequences")
+        books, page = cache.books, cache.books.page_tokens
+        lengths = [books.length(sequence) for sequence in sequences]
+        blocks = max(1, *[-(-(length + tokens) // page) for length in lengths])
+        self.reserved = books.reserve(sum(beams * (-(-(length + tokens) // page) - length // page) for length in lengths))
+        self.held = [books.fork(sequence) for sequence in sequences]      # (the rows' hold on the sequences' pages)
+        self.cache, self.beams, self.rows, self.tokens = cache, beams, beams * len(sequences), tokens
+        references = [1] * len(books.references)                          # whatever is others' is never free, nor a row's alone
+        for reserved in self.reserved:
+            references[reserved] = 0
+        table = []
+        for sequence in self.held:
+            pages = books.pages_of(sequence)
+            for number in pages:
+                references[number] += beams
+            table += (pages + [0] * (blocks - len(pages))) * beams
+        shared = [length // page * page for length in lengths]
+        host = torch.tensor([*table, *[length for length in lengths for _ in range(beams)], *shared, *references], dtype=torch.int32)
+        there = host.to(cache.k_scales.device)
+        sizes = [self.rows * blocks, self.rows, len(sequences), len(references)]
+        self.table, self.lengths, self.shared, self.references = (part.clone() for part in there.split(sizes))
+        self.table = self.table.reshape(self.rows, blocks)
+        self._counts: dict[int, torch.Tensor] = {}
+        self.steps = 0
+        cache._searches += 1
+
+    def _alive(self) -> None:
+        if self.cache is None:
+            raise ValueError("the beams have been freed")
+
+    def step(self, parents: torch.Tensor | None = None, count: int = 1) -> Step:
+        """Row r goes on from row parents[r] (int32, any shape of `rows` elements, as `ops.beam_select` gives them; None: from itself) and gets room for `count`
+        tokens more. Beyond `tokens` of them the step is not made (`kernel.check_status` raises) and its stores write nothing."""
+        self._alive()
+        if count < 0:
+            raise ValueError(f"a step of {count} tokens")
+        if count not in self._counts:
+            self.cache._not_in_a_graph("a count that no step before had")
+            self._counts[count] = torch.full((self.rows,), count, dtype=torch.int32, device=self.lengths.device)
+        if parents is not None:
+            parents = parents.reshape(-1)
+        cache = self.cache
+        _, _, _, starts = ops.cache_advance(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, self.table, self.lengths, self.references,
+                                            self._counts[count], parents, in_place=True)
+        self.steps += 1
+        return Step(self.table, starts, self._counts[count], self.lengths, count, self.shared, cache.books.changes, {}, self, self.steps)
+
+    def keep(self, row: int) -> int:
+        """Row `row` as a sequence of the cache, which `free` leaves. Waits for the device."""
+        self._alive()
+        self.cache._not_in_a_graph("keep")
+        if not 0 <= row < self.rows:
+            raise ValueError(f"there is no row {row} among {self.rows}")
+        length = int(self.lengths[row])
+        pages = self.table[row, : -(-length // self.cache.books.page_tokens)].tolist()
+        return self.cache.books.adopt(pages, length)
+
+    def free(self) -> None:
+        """Gives back what no kept sequence has."""
+        self._alive()
+        for sequence in self.held:
+            self.cache.books.free(sequence)
+        self.cache.books.drop(self.reserved)
+        self.cache._searches -= 1
+        self.cache = None

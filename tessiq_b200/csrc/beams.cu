@@ -13,7 +13,7 @@
 // Second kernel: a CTA a request joins the parts: sums, values in f64, and the same two steps over all its candidates.
 //
 // Precision: sums of exponentials in f32 a thread (16 of them), then f64: a logarithm is off by 1e-7 or so. Values of neighbours are as close as that
-// now and then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout. Ties are then ties.
+// now and then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout.
 #include <cmath>
 #include <type_traits>
 
@@ -41,7 +41,7 @@ struct SelectParams {
   const float* scores;                                      // [requests, beams]
   const uint8_t* finished;                                  // the same, or null
   int beams, vocab, keep, parts, chunk, end;
-  double2* sums;                                            // [rows, parts]: the whole power of two the sum stands at, and the sum
+  double2* sums;                                            // [rows, parts]: the logit the sum stands at, and the sum of exponentials over it
   unsigned long long* keys;                                 // [rows, parts, keep]: candidates of a part, the best first; 0: none
   float* out_scores;                                        // [requests, keep]
   int32_t *out_parents, *out_tokens;
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
   unsigned long long* const kept = lists + kListed;
   if (threadIdx.x == 0) listed = 0;
   wait_for_earlier();
-  if (p.finished != nullptr && p.finished[row]) return;     // (its one candidate is made below)
+  if (p.finished != nullptr && p.finished[row]) return;     // (its one candidate is made in the joining kernel)
   const int first = part * p.chunk, count = min(p.chunk, p.vocab - first);
   const T* const from = static_cast<const T*>(p.logits) + request * p.request_stride + beam * p.beam_stride + first;
   const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
       widen<T>(word, x);
 #pragma unroll
       for (int c = 0; c < kVec; c += 2) {
-        sum0 += exp2_ftz(fmaf(x[c], kLog2E, -shift));
-        sum1 += exp2_ftz(fmaf(x[c + 1], kLog2E, -shift));
+        sum0 += exp2_ftz((x[c] - shift) * kLog2E);
+        sum1 += exp2_ftz((x[c + 1] - shift) * kLog2E);
       }
       if (reaches<T>(word, threshold)) {                      // (few vectors do)
         const int at = place_of(chunk, i);
@@ -245,8 +245,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
 
   for (int chunk = 0; chunk < kStages; ++chunk) ask(chunk);
   copy_async_wait<kStages - 1>();
-  // The first chunk says what the sum stands at, a whole power of two (so that parts and beams join without exponentials; +inf and NaN make the sum
-  // NaN), and a bound.
+  // The first chunk says what the sum stands at, its maximum (+inf and NaN make the sum NaN), and a bound.
   {
     float most = -INFINITY;
 #pragma unroll
@@ -276,7 +275,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
     if (nth > 32) least = 0;
     threshold = least <= 0x007fffffu ? -INFINITY : from_ordered(least);
     most = from_ordered(top);
-    shift = most == -INFINITY ? 0.f : rintf(most * kLog2E);
+    shift = most == -INFINITY ? 0.f : most;
   }
   for (int chunk = 0; chunk < chunks; ++chunk) {
     copy_async_wait<kStages - 1>();
@@ -289,6 +288,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
     ask(chunk + kStages);
   }
   copy_async_wait<0>();
+  let_later_start();
   // A sum that a later chunk has carried far from what it stands at is taken again, from the true maximum.
   auto whole_sum = [&] {
 #pragma unroll
@@ -312,9 +312,9 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
 #pragma unroll
     for (int w = 0; w < kSelectWarps; ++w) top = max(top, warp_most[w]);
     most = from_ordered(top);
-    shift = most == -INFINITY ? 0.f : rintf(most * kLog2E);
+    shift = most == -INFINITY ? 0.f : most;
     sum = 0.0;
-    for (int t = threadIdx.x; t < count; t += kSelectThreads) sum += static_cast<double>(exp2_ftz(fmaf(to_compute(from[t]), kLog2E, -shift)));
+    for (int t = threadIdx.x; t < count; t += kSelectThreads) sum += static_cast<double>(exp2_ftz((to_compute(from[t]) - shift) * kLog2E));
     all = whole_sum();
   }
   if (threadIdx.x == 0) p.sums[row * p.parts + part] = make_double2(shift, all);
@@ -330,8 +330,8 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
 
 enum BeamState { kGoesOn = 0, kFinished, kNothing, kNoNumber };      // kNothing: every logit, or the score, is -inf; kNoNumber: NaN, or +inf
 
-// Candidates whose values lie closer than this, times 1 + the larger magnitude of a logit's log2 / 16: sums of two beams may be off by as much.
-constexpr double kNear = 1e-6;
+// Candidates whose values lie closer than this: the logarithms of two beams' sums may be off by as much.
+constexpr double kNear = 2e-6;
 
 struct Candidate {
   unsigned long long order;      // of the value; 0: none
@@ -341,12 +341,8 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   return a.order != b.order ? a.order > b.order : a.beam != b.beam ? a.beam < b.beam : a.token < b.token;
 }
 
-// A sum that stands at 2^from, at 2^to >= 2^from (whole numbers, or -inf for no sum, and what is +inf is NaN by now).
-__device__ __forceinline__ double brought(double sum, float from, float to) {
-  const float down = to - from;
-  if (!(down > 0.f)) return sum;
-  return down > 1000.f ? 0.0 : sum * __longlong_as_double(static_cast<long long>(1023 - static_cast<int>(down)) << 52);
-}
+// A sum that stands at `from`, at `to` >= `from` (-inf: no sum; what is +inf is NaN by now).
+__device__ __forceinline__ double brought(double sum, float from, float to) { return from == to || from == -INFINITY ? sum : sum * exp(static_cast<double>(from) - to); }
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ SelectParams p) {
@@ -356,16 +352,12 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   __shared__ int bins[6][16];
   __shared__ uint32_t uppers[kUppers];
   __shared__ double warp_sum[kJoinWarps];
-  __shared__ float largest_shift;
   __shared__ int listed, near;
   const int request = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   wait_for_earlier();
   const int slots = p.parts * p.keep + 1, all = p.beams * slots;      // of a beam, and of the request
   const long long keys0 = static_cast<long long>(request) * p.beams * (slots - 1);
-  if (threadIdx.x == 0) {
-    largest_shift = 0.f;
-    near = 0;
-  }
+  if (threadIdx.x == 0) near = 0;
   __syncthreads();
   for (int beam = warp; beam < p.beams; beam += kJoinWarps) {
     const long long row = static_cast<long long>(request) * p.beams + beam;
@@ -398,13 +390,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       else if (!(sum >= 0.0) || !(sum < INFINITY) || at == INFINITY) now = kNoNumber;
       else if (sum == 0.0 || score == -INFINITY) now = kNothing;
       state[beam] = static_cast<uint8_t>(now);
-      logarithm[beam] = now == kGoesOn ? at * 0.6931471805599453 + log(sum) : 0.0;
-      if (now == kGoesOn) atomicMax(reinterpret_cast<int*>(&largest_shift), __float_as_int(fabsf(at)));
+      logarithm[beam] = now == kGoesOn ? at + log(sum) : 0.0;
     }
   }
   __syncthreads();
   const int most_tokens = min(p.keep, p.vocab);
-  const double close = kNear * (1.0 + static_cast<double>(largest_shift) / 16.0);
   auto candidate = [&](int i) {
     const int beam = i / slots, c = i - beam * slots;
     Candidate one = {0, static_cast<uint32_t>(beam), static_cast<uint32_t>(c)};
@@ -463,7 +453,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     __syncthreads();
     unsigned long long threshold = static_cast<unsigned long long>(least) << 32;
     if (round == 0 && least != 0 && least != 0xffffff00u) {
-      const double lower = value_of(threshold) - 2.0 * close;
+      const double lower = value_of(threshold) - 2.0 * kNear;
       if (lower == lower) threshold = ordered(lower);      // (of -inf: -inf)
     }
     if (threshold == 0) threshold = 1;
@@ -497,7 +487,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
 #pragma unroll 1
         for (int j = 0; j < found; ++j) {
           const Candidate other = list[j];
-          if (other.beam != one.beam && fabs(value_of(other.order) - value) < close &&
+          if (other.beam != one.beam && fabs(value_of(other.order) - value) < kNear &&
               !(logarithm[one.beam] == logarithm[other.beam] && score_of[one.beam] == score_of[other.beam]))
             near = again[one.beam] = again[other.beam] = 1;
         }
@@ -537,8 +527,17 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     for (int beam = 0; beam < p.beams; ++beam) {
       if (!again[beam] || state[beam] != kGoesOn) continue;
       const T* const from = static_cast<const T*>(p.logits) + request * p.request_stride + beam * p.beam_stride;
+      float most = -INFINITY;
+#pragma unroll 1
+      for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) most = fmaxf(most, to_compute(from[t]));
+      const uint32_t in_warp = __reduce_max_sync(0xffffffffu, ordered(most));
+      if (lane == 0) uppers[warp] = in_warp;      // (they are made again)
+      __syncthreads();
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int w = 0; w < kJoinWarps; ++w) top = max(top, uppers[w]);
+      const double shift = from_ordered(top);
       double sum = 0.0;
-      const double shift = logarithm[beam];
 #pragma unroll 1
       for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) sum += exp(static_cast<double>(to_compute(from[t])) - shift);
 #pragma unroll

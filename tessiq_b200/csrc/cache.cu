@@ -339,6 +339,7 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
 
 constexpr int kAdvanceThreads = 1024, kAdvanceWarps = kAdvanceThreads / 32, kAdvanceCtas = 8;
 constexpr int kAdvanceSmall = 1 << 14;     // entries and pages that one CTA takes by itself
+constexpr int kAdvanceRows = 4096;         // of a cluster, whose books each CTA has in shared memory
 
 // Codes of the status word for a step that could not be made: nothing has changed then, and each row starts at -1.
 enum AdvanceFault { kAdvanceFull = 0x46554c4c, kAdvanceParent = 0x50415245 };      // "FULL", "PARE"
@@ -347,16 +348,17 @@ struct AdvanceParams {
   const int32_t *table, *lengths, *references, *counts, *parents;      // parents null: each row goes on
   long long table_stride, new_stride;
   int32_t *new_table, *new_lengths, *new_references, *starts;          // results; may be the operands
-  bool same_table, same_lengths, same_references;
+  bool same_table, same_lengths, same_references, counts_apart;        // counts_apart: not counted in new_references
   int batch, blocks, pages, page_shift;
   // scratch
   int32_t* rows;                       // same_table: the new rows, packed
-  int32_t* counted;                    // same_references: the new counts
-  int32_t *writers, *final_writer;     // [pages], of the last pages alone
-  int32_t *needs_before, *copies_before;      // [batch]: pages needed, and copies made, by the rows before
+  int32_t* counted;                    // counts_apart; what follows is in shared memory where one CTA does it all: rows that have a page,
+  int32_t* writer;                     // [pages], of last pages alone: the last row that writes into it
+  int32_t *row_parent, *row_start, *row_last;      // [batch]: parent, its tokens, the page they end inside (-1: they do not, or nothing is written there)
+  int32_t *needs_before, *copies_before;           // [batch]: pages needed, and copies made, by the rows before
   int32_t* free_pages;                 // the lowest free ones
   int32_t *sources, *targets;          // of the copies
-  int32_t* totals;                     // {needed, copies, faults, where} and from kAdvanceCtas on the free pages of each CTA's stretch
+  int32_t* totals;                     // {needed, copies, faults} and from 8 on the free pages of each CTA's stretch
 };
 constexpr int kTotals = 8 + kAdvanceCtas;
 
@@ -365,11 +367,11 @@ __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive sums over the CTA of two numbers a thread; `totals` of all.
+// Exclusive sums over the CTA of two numbers a thread; `total` of all.
 __device__ __forceinline__ int2 sums_before(int2 mine, int2* warp_totals, int2& total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int2 upto = mine;
-#pragma unroll
+#pragma unroll 1
   for (int offset = 1; offset < 32; offset *= 2) {
     const int x = __shfl_up_sync(0xffffffffu, upto.x, offset), y = __shfl_up_sync(0xffffffffu, upto.y, offset);
     if (lane >= offset) {
@@ -379,205 +381,300 @@ __device__ __forceinline__ int2 sums_before(int2 mine, int2* warp_totals, int2& 
   }
   if (lane == 31) warp_totals[warp] = upto;
   __syncthreads();
-  if (warp == 0) {
-    int2 all = warp_totals[lane];
-#pragma unroll
-    for (int offset = 1; offset < 32; offset *= 2) {
-      const int x = __shfl_up_sync(0xffffffffu, all.x, offset), y = __shfl_up_sync(0xffffffffu, all.y, offset);
-      if (lane >= offset) {
-        all.x += x;
-        all.y += y;
-      }
+  int2 before = make_int2(0, 0);
+  total = before;
+#pragma unroll 4
+  for (int w = 0; w < kAdvanceWarps; ++w) {
+    const int2 one = warp_totals[w];
+    total.x += one.x;
+    total.y += one.y;
+    if (w < warp) {
+      before.x += one.x;
+      before.y += one.y;
     }
-    warp_totals[lane] = all;
   }
-  __syncthreads();
-  const int2 before = warp == 0 ? make_int2(0, 0) : warp_totals[warp - 1];
-  total = warp_totals[kAdvanceWarps - 1];
-  __syncthreads();
   return make_int2(upto.x - mine.x + before.x, upto.y - mine.y + before.y);
 }
 
+// SMALL: one CTA with all books in shared memory; else a cluster with them in scratch. Each step is few instructions and few loads after one another: a
+// kernel of a few microseconds waits for both (a warp a row, page counts in memory and their writers counted apart: 4 rows 17 us, 256 rows 35).
+template <bool SMALL>
 __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __grid_constant__ AdvanceParams p, const WaitStatus status) {
+  extern __shared__ int32_t books[];
   __shared__ int2 warp_totals[kAdvanceWarps];
-  __shared__ int stretch_free[kAdvanceWarps];
-  wait_for_earlier();
-  const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+  __shared__ int stretch_free[kAdvanceWarps], totals_here[kTotals];
+  const int ctas = SMALL ? 1 : static_cast<int>(gridDim.x), cta = SMALL ? 0 : static_cast<int>(blockIdx.x);
   const int thread = cta * kAdvanceThreads + static_cast<int>(threadIdx.x), threads = ctas * kAdvanceThreads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = ctas * kAdvanceWarps, nth_warp = cta * kAdvanceWarps + warp;
   const int page_tokens = 1 << p.page_shift;
+  int32_t* const counted = SMALL ? books : p.counts_apart ? p.counted : p.new_references;
+  int32_t* const writer = SMALL ? counted + p.pages : p.writer;
+  int32_t* const row_parent = SMALL ? writer + p.pages : p.row_parent;
+  int32_t* const row_start = SMALL ? row_parent + p.batch : p.row_start;
+  int32_t* const row_last = SMALL ? row_start + p.batch : p.row_last;
+  int32_t* const needs_before = SMALL ? row_last + p.batch : p.needs_before;
+  int32_t* const copies_before = SMALL ? needs_before + p.batch : p.copies_before;
+  int32_t* const free_pages = SMALL ? copies_before + p.batch : p.free_pages;
+  int32_t* const totals = SMALL ? totals_here : p.totals;
   int32_t* const rows = p.same_table ? p.rows : p.new_table;
   const long long row_stride = p.same_table ? p.blocks : p.new_stride;
-  int32_t* const counted = p.same_references ? p.counted : p.new_references;
   const long long capacity = static_cast<long long>(p.blocks) << p.page_shift;
+  auto meet = [&] {
+    if constexpr (SMALL) __syncthreads();
+    else cluster_meet();
+  };
+  auto peek = [&](const int32_t* at) {      // what another thread has written
+    if constexpr (SMALL) return *at;
+    else return __ldcg(at);
+  };
   auto fault = [&](int code, int row, int what) {
-    if (atomicCAS(p.totals + 2, 0, code) == 0) p.totals[3] = row;
+    atomicCAS(totals + 2, 0, code);
     report(status, code, row, what);
   };
   auto blocks_of = [&](long long tokens) { return static_cast<int>((tokens + page_tokens - 1) >> p.page_shift); };
-  auto parent_of = [&](int row) { return p.parents == nullptr ? row : p.parents[row]; };
-  auto held = [&](int row) { return row < 0 || row >= p.batch ? 0 : p.lengths[row]; };      // tokens
   auto in_table = [&](int tokens) { return static_cast<int>(min(static_cast<long long>(max(tokens, 0)), capacity)); };
+  wait_for_earlier();
+  let_later_start();                   // (the copying kernel)
 
-  if (thread < kTotals) p.totals[thread] = 0;
-  for (int i = thread; i < p.pages; i += threads) counted[i] = p.references[i];
+  // Rows, and what there is of each page.
+  if (thread < kTotals) totals[thread] = 0;
+#pragma unroll 4
+  for (int i = thread; i < p.pages; i += threads) {
+    counted[i] = p.references[i];
+    writer[i] = -1;
+  }
+  meet();
+#pragma unroll 1
   for (int row = thread; row < p.batch; row += threads) {
-    const int parent = parent_of(row), start = in_table(held(parent));
-    if (p.counts[row] > 0 && (start & (page_tokens - 1)) != 0) {
-      const int last = p.table[parent * p.table_stride + (start >> p.page_shift)];
-      if (last >= 0 && last < p.pages) {
-        p.writers[last] = 0;
-        p.final_writer[last] = -1;
+    const int parent = p.parents == nullptr ? row : p.parents[row], own = p.lengths[row], count = p.counts[row];
+    const int tokens = parent < 0 || parent >= p.batch ? 0 : p.lengths[parent];
+    row_parent[row] = parent < 0 || parent >= p.batch ? -1 : parent;
+    row_start[row] = in_table(tokens);
+    row_last[row] = -1;
+    if (parent >= p.batch) fault(kAdvanceParent, row, parent);
+    else if (own > capacity || tokens > capacity || static_cast<long long>(max(tokens, 0)) + max(count, 0) > capacity) fault(kKeyedLength, row, max(tokens, own));
+  }
+  meet();
+
+  // Entries: the parents' pages, and how many rows have each; a row that will write into its last page gives that up, for now.
+  const bool near = !SMALL && p.batch <= kAdvanceRows;      // each CTA has all rows' books at hand
+  if (near) {
+#pragma unroll 1
+    for (int row = threadIdx.x; row < p.batch; row += kAdvanceThreads) {
+      books[row] = peek(row_parent + row);
+      books[kAdvanceRows + row] = peek(row_start + row);
+      books[2 * kAdvanceRows + row] = p.lengths[row];
+    }
+    __syncthreads();
+  }
+  // A thread has several entries at a time, so that their loads are under way together: of one row by a warp, or, of up to 32 entries, of several rows by
+  // as many lanes as hold a row. (Of 1024 rows of 138 this takes 13 us of 36, with eight at a time too: the counts' atomics.)
+  constexpr int kAtOnce = 4;
+  auto take = [&](const int (&row)[kAtOnce], const int (&i)[kAtOnce]) {
+    int before[kAtOnce], now[kAtOnce], start[kAtOnce], had[kAtOnce];
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (row[n] >= p.batch || i[n] >= p.blocks) continue;
+      const int parent = near ? books[row[n]] : peek(row_parent + row[n]);
+      start[n] = near ? books[kAdvanceRows + row[n]] : peek(row_start + row[n]);
+      had[n] = blocks_of(in_table(near ? books[2 * kAdvanceRows + row[n]] : p.lengths[row[n]]));
+      before[n] = p.table[row[n] * p.table_stride + i[n]];
+      now[n] = i[n] < blocks_of(start[n]) ? p.table[parent * p.table_stride + i[n]] : before[n];
+    }
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (row[n] >= p.batch || i[n] >= p.blocks) continue;
+      rows[row[n] * row_stride + i[n]] = now[n];
+      const bool drops = i[n] < had[n], takes = i[n] < blocks_of(start[n]);
+      if ((drops && (before[n] < 0 || before[n] >= p.pages)) || (takes && (now[n] < 0 || now[n] >= p.pages))) {
+        fault(kKeyedPage, row[n], i[n]);
+        continue;
       }
+      const bool writes = takes && i[n] == start[n] >> p.page_shift && p.counts[row[n]] > 0;      // (the tokens end inside this page)
+      if (drops != takes || before[n] != now[n]) {
+        if (drops) atomicAdd(counted + before[n], -1);
+        if (takes && !writes) atomicAdd(counted + now[n], 1);
+      } else if (writes) {
+        atomicAdd(counted + now[n], -1);
+      }
+      if (writes) {
+        atomicMax(writer + now[n], row[n]);
+        row_last[row[n]] = now[n];
+      }
+    }
+  };
+  if (p.blocks > 32) {
+#pragma unroll 1
+    for (int row = nth_warp; row < p.batch; row += warps) {
+#pragma unroll 1
+      for (int i = lane; i < p.blocks; i += 32 * kAtOnce) {
+        int of[kAtOnce], at[kAtOnce];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          of[n] = row;
+          at[n] = i + 32 * n;
+        }
+        take(of, at);
+      }
+    }
+  } else {
+    const int shift = p.blocks <= 1 ? 0 : 32 - __clz(p.blocks - 1), step = threads >> shift;      // lanes of a row: 2^shift
+#pragma unroll 1
+    for (int row = thread >> shift; row < p.batch; row += kAtOnce * step) {
+      int of[kAtOnce], at[kAtOnce];
+#pragma unroll
+      for (int n = 0; n < kAtOnce; ++n) {
+        of[n] = row + n * step;
+        at[n] = thread & ((1 << shift) - 1);
+      }
+      take(of, at);
     }
   }
-  cluster_meet();
+  meet();
 
-  // Rows: the parents' pages, and how many rows have each; a warp a row.
-  for (int row = nth_warp; row < p.batch; row += warps) {
-    const int parent = parent_of(row), own_tokens = held(row), tokens = held(parent), count = p.counts[row];
-    if (lane == 0) {
-      if (parent >= p.batch) fault(kAdvanceParent, row, parent);
-      else if (own_tokens > capacity || tokens > capacity || static_cast<long long>(max(tokens, 0)) + max(count, 0) > capacity) fault(kKeyedLength, row, max(tokens, own_tokens));
-    }
-    const int had = blocks_of(in_table(own_tokens)), has = blocks_of(in_table(tokens));
-    const int32_t* const own = p.table + row * p.table_stride;
-    const int32_t* const from = parent < 0 || parent >= p.batch ? own : p.table + parent * p.table_stride;
-    for (int i = lane; i < p.blocks; i += 32) {
-      const int before = own[i], now = i < has ? from[i] : before;
-      rows[row * row_stride + i] = now;
-      const bool drops = i < had, takes = i < has;
-      if ((drops && (before < 0 || before >= p.pages)) || (takes && (now < 0 || now >= p.pages))) {
-        fault(kKeyedPage, row, i);
-      } else if (drops != takes || before != now) {
-        if (takes) atomicAdd(counted + now, 1);
-        if (drops) atomicAdd(counted + before, -1);
-      }
-    }
-    const int start = in_table(tokens);
-    if (lane == 0 && count > 0 && (start & (page_tokens - 1)) != 0) {
-      const int last = from[start >> p.page_shift];
-      if (last >= 0 && last < p.pages) {
-        atomicAdd(p.writers + last, 1);
-        atomicMax(p.final_writer + last, row);
-      }
-    }
-  }
-  cluster_meet();
-
-  // What each row needs (the first CTA), and where the free pages are (all; a warp has a stretch of pages).
-  auto copies = [&](int row, int start, int count) {      // the row's last page is others' too, and it is not the one that keeps it
-    if (count <= 0 || (start & (page_tokens - 1)) == 0) return -1;
-    const int last = __ldcg(rows + row * row_stride + (start >> p.page_shift));
-    if (last < 0 || last >= p.pages) return -1;
-    return __ldcg(counted + last) > __ldcg(p.writers + last) || __ldcg(p.final_writer + last) != row ? last : -1;
+  // The last of the rows that write into a page keeps it where nobody else has it; the others copy it. What each row needs (the first CTA).
+  auto copied = [&](int row) {      // the page that the row copies, or -1
+    const int last = peek(row_last + row);
+    return last >= 0 && (peek(counted + last) > 0 || peek(writer + last) != row) ? last : -1;
   };
   if (cta == 0) {
     const int run = (p.batch + kAdvanceThreads - 1) / kAdvanceThreads;
     const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
     int2 mine = make_int2(0, 0);
+#pragma unroll 1
     for (int row = first; row < last; ++row) {
-      const int start = in_table(held(parent_of(row))), count = max(p.counts[row], 0);
-      const int copied = copies(row, start, count) >= 0 ? 1 : 0;
-      p.needs_before[row] = mine.x;      // (within the run so far)
-      p.copies_before[row] = mine.y;
-      mine.x += copied + static_cast<int>(min(static_cast<long long>(blocks_of(static_cast<long long>(start) + count)) - blocks_of(start), 0x3fffffffLL));
-      mine.y += copied;
+      const int start = peek(row_start + row), count = max(p.counts[row], 0), copies = copied(row) >= 0 ? 1 : 0;
+      needs_before[row] = mine.x;      // (within the run so far)
+      copies_before[row] = mine.y;
+      mine.x += copies + blocks_of(static_cast<long long>(start) + count) - blocks_of(start);
+      mine.y += copies;
     }
     int2 total;
-    const int2 before = sums_before(mine, warp_totals, total);
+    const int2 before = sums_before(mine, warp_totals, total);      // (the CTA meets in there, after which pages that are kept count again)
+#pragma unroll 1
     for (int row = first; row < last; ++row) {
-      p.needs_before[row] += before.x;
-      p.copies_before[row] += before.y;
+      const int page = peek(row_last + row);
+      needs_before[row] += before.x;
+      copies_before[row] += before.y;
+      if (page >= 0 && copied(row) < 0) row_last[row] = -2 - page;
     }
     if (threadIdx.x == 0) {
-      p.totals[0] = total.x;
-      p.totals[1] = total.y;
+      totals[0] = total.x;
+      totals[1] = total.y;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int row = first; row < last; ++row) {
+      const int page = row_last[row];
+      if (page <= -2) atomicExch(counted + (-2 - page), 1);
     }
   }
-  const int stretch = ((p.pages + warps - 1) / warps + 31) / 32 * 32;
+  meet();
+
+  // Where the free pages are; a warp has a stretch of pages, a lane four neighbouring ones at a time (`counted` is 16-byte aligned).
+  const int stretch = ((p.pages + warps - 1) / warps + 127) / 128 * 128;
   const int page0 = static_cast<int>(min(static_cast<long long>(nth_warp) * stretch, static_cast<long long>(p.pages)));
   const int page1 = static_cast<int>(min(static_cast<long long>(page0) + stretch, static_cast<long long>(p.pages)));
+  auto free_of_four = [&](int page) {      // bits
+    page += 4 * lane;
+    if (page + 3 < page1) {
+      const int4 four = SMALL ? *reinterpret_cast<const int4*>(counted + page) : __ldcg(reinterpret_cast<const int4*>(counted + page));
+      return (four.x == 0 ? 1 : 0) | (four.y == 0 ? 2 : 0) | (four.z == 0 ? 4 : 0) | (four.w == 0 ? 8 : 0);
+    }
+    int bits = 0;
+    for (int n = 0; n < 4; ++n)
+      if (page + n < page1 && peek(counted + page + n) == 0) bits |= 1 << n;
+    return bits;
+  };
   int free_here = 0;
-  for (int page = page0; page < page1; page += 32) {
-    const bool is_free = page + lane < page1 && __ldcg(counted + page + lane) == 0;
-    free_here += __popc(__ballot_sync(0xffffffffu, is_free));
-  }
+#pragma unroll 4
+  for (int page = page0; page < page1; page += 128) free_here += __popc(free_of_four(page));
+  free_here = __reduce_add_sync(0xffffffffu, free_here);
   if (lane == 0) stretch_free[warp] = free_here;
   __syncthreads();
-  int free_before = 0, free_cta = 0;
+  int free_before = 0, free_all = 0;
+#pragma unroll 4
   for (int w = 0; w < kAdvanceWarps; ++w) {
-    if (w < warp) free_before += stretch_free[w];
-    free_cta += stretch_free[w];
-  }
-  if (threadIdx.x == 0) p.totals[8 + cta] = free_cta;
-  cluster_meet();
-
-  const int needed = __ldcg(p.totals);
-  int free_all = 0;
-  for (int c = 0; c < ctas; ++c) {
-    const int there = __ldcg(p.totals + 8 + c);
-    if (c < cta) free_before += there;
+    const int there = stretch_free[w];
+    if (w < warp) free_before += there;
     free_all += there;
   }
-  const int fault_before = __ldcg(p.totals + 2);
+  if constexpr (!SMALL) {
+    if (threadIdx.x == 0) totals[8 + cta] = free_all;
+    meet();
+    free_all = 0;
+#pragma unroll 1
+    for (int c = 0; c < ctas; ++c) {
+      const int there = peek(totals + 8 + c);
+      if (c < cta) free_before += there;
+      free_all += there;
+    }
+  }
+  const int needed = peek(totals), copies = peek(totals + 1), fault_before = peek(totals + 2);
   const bool good = fault_before == 0 && needed <= free_all;
   if (good) {
-    for (int page = page0; page < page1 && free_before < needed; page += 32) {
-      const bool is_free = page + lane < page1 && __ldcg(counted + page + lane) == 0;
-      const uint32_t free_lanes = __ballot_sync(0xffffffffu, is_free);
-      const int place = free_before + __popc(free_lanes & ((1u << lane) - 1));
-      if (is_free && place < needed) p.free_pages[place] = page + lane;
-      free_before += __popc(free_lanes);
+#pragma unroll 1
+    for (int page = page0; page < page1 && free_before < needed; page += 128) {
+      const int bits = free_of_four(page), mine = __popc(bits);
+      int upto = mine;
+#pragma unroll
+      for (int offset = 1; offset < 32; offset *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, offset);
+        if (lane >= offset) upto += other;
+      }
+      int place = free_before + upto - mine;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if ((bits >> n & 1) == 0) continue;
+        if (place < needed) free_pages[place] = page + 4 * lane + n;
+        ++place;
+      }
+      free_before += __shfl_sync(0xffffffffu, upto, 31);
     }
   } else if (thread == 0 && fault_before == 0) {
     report(status, kAdvanceFull, needed, free_all);
   }
-  cluster_meet();
+  meet();
 
-  // The rows take their pages; a warp a row.
-  for (int row = nth_warp; row < p.batch; row += warps) {
-    const int parent = parent_of(row), start = in_table(held(parent)), count = max(p.counts[row], 0);
-    if (good) {
-      const int has = blocks_of(start), will = blocks_of(static_cast<long long>(start) + count);
-      int at = __ldcg(p.needs_before + row);
-      const int last = copies(row, start, count);
-      __syncwarp();
-      if (last >= 0) {
-        const int page = __ldcg(p.free_pages + at++);
-        if (lane == 0) {
-          const int pair = __ldcg(p.copies_before + row);
-          p.sources[pair] = last;
-          p.targets[pair] = page;
-          rows[row * row_stride + has - 1] = page;
-        }
-      }
-      for (int i = has + lane; i < will; i += 32) rows[row * row_stride + i] = __ldcg(p.free_pages + at + i - has);
+  // The rows take their pages, which then have one row each.
+#pragma unroll 1
+  for (int row = thread; good && row < p.batch; row += threads) {
+    const int start = peek(row_start + row), has = blocks_of(start), will = blocks_of(static_cast<long long>(start) + max(p.counts[row], 0));
+    int at = peek(needs_before + row);
+    const int last = peek(row_last + row);
+    if (last >= 0) {
+      const int pair = peek(copies_before + row), page = peek(free_pages + at++);
+      p.sources[pair] = last;
+      p.targets[pair] = page;
+      rows[row * row_stride + has - 1] = page;
     }
+#pragma unroll 1
+    for (int i = has; i < will; ++i) rows[row * row_stride + i] = peek(free_pages + at++);
   }
-  cluster_meet();      // (`counted` and `rows` of last pages are read until here, and lengths of parents)
-  for (int row = nth_warp; row < p.batch; row += warps) {
-    const int parent = parent_of(row), start = in_table(held(parent));
-    if (lane == 0) p.starts[row] = good ? start : -1;
-  }
-  if (good) {
-    for (int i = thread; i < __ldcg(p.totals + 1); i += threads) atomicAdd(counted + __ldcg(p.sources + i), -1);
-    for (int i = thread; i < needed; i += threads) atomicExch(counted + __ldcg(p.free_pages + i), 1);
-  } else if (thread == 0) {
-    p.totals[1] = 0;                      // nothing is copied
-  }
-  cluster_meet();
+#pragma unroll 1
+  for (int i = thread; good && i < needed; i += threads) atomicExch(counted + peek(free_pages + i), 1);
+  if (thread == 0) *p.totals = good ? copies : 0;      // how many the next kernel copies
+  // (lengths and counts are read until here, results that may be these written from here on)
+#pragma unroll 1
+  for (int row = thread; row < p.batch; row += threads) p.starts[row] = good ? peek(row_start + row) : -1;
+  if (p.same_lengths || p.same_table || p.same_references || !SMALL) meet();
+  else __syncthreads();
+#pragma unroll 1
   for (int row = thread; row < p.batch; row += threads) {
-    const int start = __ldcg(p.starts + row);
-    if (good) p.new_lengths[row] = start + max(p.counts[row], 0);
+    if (good) p.new_lengths[row] = peek(row_start + row) + max(p.counts[row], 0);
     else if (!p.same_lengths) p.new_lengths[row] = p.lengths[row];
   }
-  if (good ? p.same_references : !p.same_references)
-    for (int i = thread; i < p.pages; i += threads) p.new_references[i] = good ? __ldcg(counted + i) : p.references[i];
+  if (good ? SMALL || p.counts_apart : !p.same_references) {
+#pragma unroll 4
+    for (int i = thread; i < p.pages; i += threads) p.new_references[i] = good ? peek(counted + i) : p.references[i];
+  }
   if (good ? p.same_table : !p.same_table) {
-    for (int row = nth_warp; row < p.batch; row += warps)
+#pragma unroll 1
+    for (int row = nth_warp; row < p.batch; row += warps) {
+#pragma unroll 4
       for (int i = lane; i < p.blocks; i += 32)
         p.new_table[row * p.new_stride + i] = good ? __ldcg(rows + row * row_stride + i) : p.table[row * p.table_stride + i];
+    }
   }
 }
 
@@ -611,12 +708,17 @@ __global__ void __launch_bounds__(kCopyThreads) copy_named_pages_kernel(const __
   }
 }
 
-// Scratch of an advance: where each array begins, in int32.
+// Scratch of an advance: where each array begins, in int32. `small`: what one CTA keeps in shared memory, and how much of that there is.
+constexpr size_t kAdvanceShared = 200 * 1024;
 struct AdvanceScratch {
-  int64_t rows, counted, writers, final_writer, needs, copies, free_pages, sources, targets, totals, all;
+  bool small;
+  size_t shared_bytes;
+  int64_t rows, counted, writer, parent, start, last, needs, copies, free_pages, sources, targets, totals, all;
 };
 AdvanceScratch advance_scratch(int64_t batch, int64_t blocks, int64_t pages) {
   AdvanceScratch at = {};
+  at.shared_bytes = static_cast<size_t>(3 * pages + 5 * batch) * sizeof(int32_t);
+  at.small = batch * blocks + pages <= kAdvanceSmall && at.shared_bytes <= kAdvanceShared;
   int64_t end = 0;
   auto take = [&](int64_t count) {
     const int64_t begin = end;
@@ -624,15 +726,19 @@ AdvanceScratch advance_scratch(int64_t batch, int64_t blocks, int64_t pages) {
     return begin;
   };
   at.rows = take(batch * blocks);
-  at.counted = take(pages);
-  at.writers = take(pages);
-  at.final_writer = take(pages);
-  at.needs = take(batch);
-  at.copies = take(batch);
-  at.free_pages = take(pages);
   at.sources = take(batch);
   at.targets = take(batch);
   at.totals = take(kTotals);
+  if (!at.small) {
+    at.counted = take(pages);
+    at.writer = take(pages);
+    at.parent = take(batch);
+    at.start = take(batch);
+    at.last = take(batch);
+    at.needs = take(batch);
+    at.copies = take(batch);
+    at.free_pages = take(pages);
+  }
   at.all = end;
   return at;
 }
@@ -880,7 +986,7 @@ extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int
              TQ_INVALID_ARGUMENT, "null operand or result");
   TQ_REQUIRE(table_stride >= blocks || batch == 1, TQ_INVALID_ARGUMENT, "the table's rows overlap");
   TQ_REQUIRE(new_stride >= blocks || batch == 1, TQ_INVALID_ARGUMENT, "the new table's rows overlap");
-  TQ_REQUIRE(new_table != table || new_stride == table_stride || batch == 1, TQ_INVALID_ARGUMENT, "a table in place has one stride");
+  TQ_REQUIRE(new_table != table || new_stride == table_stride || batch == 1 || blocks == 0, TQ_INVALID_ARGUMENT, "a table in place has one stride");
   for (const void* each : {static_cast<const void*>(table), static_cast<const void*>(lengths), static_cast<const void*>(references),
                            static_cast<const void*>(counts), static_cast<const void*>(parents), static_cast<const void*>(new_table),
                            static_cast<const void*>(new_lengths), static_cast<const void*>(new_references), static_cast<const void*>(starts)})
@@ -922,14 +1028,17 @@ extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int
   p.same_table = new_table == table;
   p.same_lengths = new_lengths == lengths;
   p.same_references = new_references == references;
+  p.counts_apart = p.same_references || !tq::aligned_to(new_references, 16);
   p.batch = static_cast<int>(batch);
   p.blocks = static_cast<int>(blocks);
   p.pages = static_cast<int>(pages);
   p.page_shift = tq::page_shift_of(page_tokens);
   p.rows = scratch + at.rows;
   p.counted = scratch + at.counted;
-  p.writers = scratch + at.writers;
-  p.final_writer = scratch + at.final_writer;
+  p.writer = scratch + at.writer;
+  p.row_parent = scratch + at.parent;
+  p.row_start = scratch + at.start;
+  p.row_last = scratch + at.last;
   p.needs_before = scratch + at.needs;
   p.copies_before = scratch + at.copies;
   p.free_pages = scratch + at.free_pages;
@@ -938,25 +1047,31 @@ extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int
   p.totals = scratch + at.totals;
   cudaStream_t cuda_stream = static_cast<cudaStream_t>(stream);
   const auto held = tq::hold_scratch(workspace);
-  const unsigned ctas = batch * blocks + pages <= tq::kAdvanceSmall ? 1 : tq::kAdvanceCtas;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(ctas);
-  config.blockDim = dim3(tq::kAdvanceThreads);
-  config.stream = cuda_stream;
-  cudaLaunchAttribute attributes[2];
-  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[0].val.programmaticStreamSerializationAllowed = 1;
-  attributes[1].id = cudaLaunchAttributeClusterDimension;
-  attributes[1].val.clusterDim.x = ctas;
-  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
-  config.attrs = attributes;
-  config.numAttrs = 2;
-  TQ_CUDA(cudaLaunchKernelEx(&config, tq::cache_advance_kernel, p, status));
+  if (at.small) {
+    TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tq::kAdvanceShared)));
+    TQ_CUDA(tq::launch_overlapped(tq::cache_advance_kernel<true>, dim3(1), tq::kAdvanceThreads, at.shared_bytes, cuda_stream, p, status));
+  } else {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(tq::kAdvanceCtas);
+    config.blockDim = dim3(tq::kAdvanceThreads);
+    config.dynamicSmemBytes = 3 * tq::kAdvanceRows * sizeof(int32_t);
+    config.stream = cuda_stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = tq::kAdvanceCtas;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes)));
+    TQ_CUDA(cudaLaunchKernelEx(&config, tq::cache_advance_kernel<false>, p, status));
+  }
   if (tq_status s = tq::check_launch("cache_advance_kernel")) return s;
   if (copies.count == 0) return TQ_OK;
   copies.sources = p.sources;
   copies.targets = p.targets;
-  copies.pairs = p.totals + 1;
+  copies.pairs = p.totals;
   const long long at_once = tq::sm_count(device) * 8LL / pieces;
   const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(at_once < 1 ? 1 : at_once < batch ? at_once : batch));
   TQ_CUDA(tq::launch_overlapped(tq::copy_named_pages_kernel, grid, tq::kCopyThreads, 0, cuda_stream, copies));

@@ -827,13 +827,14 @@ PrefixPlan plan_call(KeyedParams& p, int64_t batch, int64_t heads, int64_t kv_he
 }  // namespace tq
 
 extern "C" tq_status tq_prefix_attention_form(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_tokens, int64_t head_dim, int64_t page_tokens,
-                                              int64_t blocks, int64_t runs, int32_t device, int32_t* form, int32_t* parts) {
-  TQ_REQUIRE(form != nullptr && parts != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
+                                              int64_t blocks, int64_t runs, int32_t device, int32_t* form, int32_t* parts, int32_t* block_rows) {
+  TQ_REQUIRE(form != nullptr && parts != nullptr && block_rows != nullptr, TQ_INVALID_ARGUMENT, "null out-pointer");
   TQ_REQUIRE(tq::prefix_takes(batch, heads, kv_heads, q_tokens, head_dim, page_tokens, blocks, runs), TQ_INVALID_ARGUMENT, "no attention of these extents");
   tq::KeyedParams p = {};
   const tq::PrefixPlan plan = tq::plan_call(p, batch, heads, kv_heads, q_tokens, head_dim, page_tokens, blocks, runs, 1.0, device);
   *form = plan.form == tq::kApart ? TQ_ATTENTION_APART : plan.form == tq::kStreamed ? TQ_ATTENTION_STREAMED : TQ_ATTENTION_TILES;
   *parts = plan.form == tq::kApart ? 0 : plan.part_count - 1;
+  *block_rows = plan.form == tq::kApart ? 0 : plan.form == tq::kStreamed ? plan.part_rows : plan.tiles * tq::kTileRows;
   return TQ_OK;
 }
 
