@@ -1267,10 +1267,11 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   plan.row_tiles = (rows + 8 * plan.nt - 1) / (8 * plan.nt);
   // a tile's own, and of all the sequence's queries together, which is what every tile walks where chunks are dealt out
   const long long tokens = (8 * plan.nt + p.group - 2) / p.group + 1;
-  const long long own = most_chunks(p, tokens < p.q_tokens ? tokens : p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
+  long long own = most_chunks(p, tokens < p.q_tokens ? tokens : p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long chunks = most_chunks(p, p.q_tokens, keys, KeyedShape<BITS, W>::kKeys);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * plan.row_tiles;
   const long long average = p.typical > 0 && p.typical < keys ? most_chunks(p, p.q_tokens, p.typical, KeyedShape<BITS, W>::kKeys) : chunks;
+  if (p.runs == 0 && average < own) own = average;      // sequences without the keys of their runs: none of them is taken to be long
   const int sixteen = plan.nt - 1;
   auto most_of = [&](auto joins, auto warps) {
     constexpr int kJoins = decltype(joins)::value, kWarps = decltype(warps)::value;

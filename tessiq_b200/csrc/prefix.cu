@@ -753,9 +753,9 @@ struct PrefixPlan {
   size_t parts_bytes, stats_bytes, keyed_bytes;
   size_t bytes() const { return parts_bytes + stats_bytes + keyed_bytes; }
 };
-constexpr double kStartTime = 8.0;                     // a CTA's, to its first scores and behind its last ones
-constexpr double kTileTimes[2][2] = {{1.7, 2.4}, {2.1, 2.75}};      // 128 keys: heads up to 64, 128; one tile of rows, two
-constexpr double kPartBytesPerMicrosecond = 5e6;
+constexpr double kStartTime = 10.0;                    // a CTA's, to its first scores and behind its last ones
+constexpr double kTileTimes[2][2] = {{1.55, 2.3}, {1.75, 2.5}};     // 128 keys: heads up to 64, 128; one tile of rows, two
+constexpr double kPartBytesPerMicrosecond = 2.2e6;
 constexpr double kOwnTime = 9.0, kJoinTime = 3.0;      // what each sequence has behind the shared keys; the join
 constexpr int kMostStreamed = 16;                      // rows of a run: a warp's
 constexpr long long kOwnKeys = 128;                    // what a sequence is taken to have behind the shared keys
@@ -801,10 +801,12 @@ PrefixPlan plan_prefix(KeyedParams p, int runs, long long keys, int32_t device) 
   const size_t slots = static_cast<size_t>(runs) * p.kv_heads * plan.part_count * plan.part_rows;
   plan.parts_bytes = slots * (wide ? 128 : 64) * sizeof(float);
   plan.stats_bytes = (slots * sizeof(float2) + 15) / 16 * 16;
-  if (plan.form == kStreamed) {
-    plan.typical = both.typical;
-    plan.keyed_bytes = keyed_workspace(true, both, keys, device);
+  plan.typical = both.typical;
+  if (plan.form == kTiles) {
+    both = p;
+    both.typical = plan.typical = static_cast<int>(keys < kOwnKeys ? keys : kOwnKeys);
   }
+  plan.keyed_bytes = keyed_workspace(true, both, keys, device);
   return plan;
 }
 
@@ -920,10 +922,10 @@ extern "C" tq_status tq_prefix_attention_launch(tq_dtype dtype, const void* q, c
   const bool bf16 = dtype == TQ_BF16, wide = head_dim > 64;
   const auto held = tq::hold_scratch(workspace);      // all kernels, one after the other
   tq::KeyedParams keyed = p;
+  keyed.typical = plan.typical;
   if (plan.form == tq::kStreamed) {
     keyed.runs = static_cast<int>(runs);
     keyed.batch = static_cast<int>(runs + batch);
-    keyed.typical = plan.typical;
   } else {
     const tq_status s = wide ? (plan.tiles == 2 ? tq::launch_prefix<128, 2>(p, bf16, plan.ctas, cuda_stream) : tq::launch_prefix<128, 1>(p, bf16, plan.ctas, cuda_stream))
                              : (plan.tiles == 2 ? tq::launch_prefix<64, 2>(p, bf16, plan.ctas, cuda_stream) : tq::launch_prefix<64, 1>(p, bf16, plan.ctas, cuda_stream));

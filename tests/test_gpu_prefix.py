@@ -119,8 +119,8 @@ SHAPES = [  # runs, each, heads, kv_heads, q_tokens, prompt, tail, width, page, 
     (16, 2, 40, 8, 1, 4096, 100, 128, 1024, "streamed"), (12, 8, 16, 16, 1, 2048, 100, 32, 256, "streamed"),
     (1, 128, 2, 1, 1, 9000, 33, 64, 16, "tiles 128"), (1, 80, 32, 8, 1, 4000, 33, 64, 32, "tiles 128"), (1, 24, 20, 4, 1, 9000, 33, 128, 64, "tiles 128"),
     (1, 200, 8, 2, 1, 4000, 40, 128, 64, "tiles 128"), (2, 100, 9, 3, 1, 3333, 50, 96, 128, "tiles 128"), (1, 300, 8, 8, 1, 2600, 8, 48, 256, "tiles 128"),
-    (1, 256, 8, 4, 1, 6000, 33, 64, 16, "tiles 256"), (1, 100, 64, 8, 1, 3000, 40, 128, 64, "tiles 256"), (1, 150, 16, 4, 2, 1800, 40, 128, 32, "tiles 256"),
-    (3, 70, 14, 2, 4, 1300, 11, 112, 16, "tiles 256"), (1, 200, 32, 4, 1, 5000, 30, 64, 1024, "tiles 256"),
+    (1, 256, 8, 4, 1, 6000, 33, 64, 16, "tiles 128"), (1, 100, 64, 8, 1, 3000, 40, 128, 64, "tiles 128"), (1, 150, 16, 4, 2, 1800, 40, 128, 32, "tiles 128"),
+    (3, 70, 14, 2, 4, 1300, 11, 112, 16, "tiles 128"), (1, 200, 32, 4, 1, 5000, 30, 64, 1024, "tiles 256"),
 ]
 
 
@@ -137,8 +137,8 @@ def test_prefix_attention(tq, shape, dtype):
 
 
 KINDS = [  # a case of each way
-    (12, 4, 12, 12, 1, 2048, 40, 64, 64), (1, 128, 2, 1, 1, 9000, 33, 64, 16, torch.float16), (1, 24, 20, 4, 1, 9000, 60, 128, 64), (1, 150, 16, 4, 2, 1800, 40, 128, 32),
-    (1, 256, 8, 4, 1, 6000, 33, 64, 16),
+    (12, 4, 12, 12, 1, 2048, 40, 64, 64), (1, 128, 2, 1, 1, 9000, 33, 64, 16, torch.float16), (1, 24, 20, 4, 1, 9000, 60, 128, 64), (1, 160, 16, 4, 4, 2500, 40, 128, 32),
+    (1, 200, 32, 4, 1, 4000, 33, 64, 16),
 ]
 
 
