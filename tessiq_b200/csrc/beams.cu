@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
   // Adds a chunk to the sum, and what reaches the bound to the list: whether that has become long, for the CTA.
   auto take = [&](int chunk) {
     float sum0 = 0.f, sum1 = 0.f;
-    int last = 0;
+    uint32_t reaching = 0;                                    // vectors; few do
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const uint4 word = ring[chunk % kStages][i][threadIdx.x];
@@ -179,15 +179,27 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
         sum0 += exp2_ftz((x[c] - shift) * kLog2E);
         sum1 += exp2_ftz((x[c + 1] - shift) * kLog2E);
       }
-      if (reaches<T>(word, threshold)) {                      // (few vectors do)
-        const int at = place_of(chunk, i);
+      reaching |= reaches<T>(word, threshold) ? 1u << i : 0u;
+    }
+    int last = 0;
+    if (reaching != 0) {                                      // (behind the loop, so that a warp's threads go through this together)
+      static_assert(kVecs * kVec <= 32, "a bit for each of a thread's logits of a chunk");
+      uint32_t taken = 0;
+#pragma unroll 1
+      for (uint32_t left = reaching; left != 0; left &= left - 1) {
+        const int i = __ffs(left) - 1, at = place_of(chunk, i);
+        float x[kVec];
+        words(chunk, i, x);
+        uint32_t some = 0;
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-          if (x[c] >= threshold && at + c >= 0 && at + c < count) {
-            last = atomicAdd(&listed, 1);
-            if (last < kListed) list[last] = key_of(x[c], at + c);
-          }
-        }
+        for (int c = 0; c < kVec; ++c) some |= x[c] >= threshold && at + c >= 0 && at + c < count ? 1u << c : 0u;
+        taken |= some << (i * kVec);
+      }
+      last = atomicAdd(&listed, __popc(taken));
+#pragma unroll 1
+      for (; taken != 0; taken &= taken - 1, ++last) {
+        const int bit = __ffs(taken) - 1, i = bit / kVec, c = bit % kVec;
+        if (last < kListed) list[last] = key_of(to_compute(reinterpret_cast<const T*>(&ring[chunk % kStages][i][threadIdx.x])[c]), place_of(chunk, i) + c);
       }
     }
     sum += static_cast<double>(sum0) + static_cast<double>(sum1);

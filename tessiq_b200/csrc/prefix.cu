@@ -757,6 +757,7 @@ constexpr double kStartTime = 10.0;                    // a CTA's, to its first 
 constexpr double kTileTimes[2][2] = {{1.55, 2.3}, {1.75, 2.5}};     // 128 keys: heads up to 64, 128; one tile of rows, two
 constexpr double kPartBytesPerMicrosecond = 2.2e6;
 constexpr double kOwnTime = 9.0, kJoinTime = 3.0;      // what each sequence has behind the shared keys; the join
+constexpr double kStreamedTime = 6.0;                  // the join, and runs that end later than sequences
 constexpr int kMostStreamed = 16;                      // rows of a run: a warp's
 constexpr long long kOwnKeys = 128;                    // what a sequence is taken to have behind the shared keys
 
@@ -773,7 +774,7 @@ PrefixPlan plan_prefix(KeyedParams p, int runs, long long keys, int32_t device) 
   both.runs = runs;
   both.batch = runs + p.batch;
   both.typical = static_cast<int>((runs * keys + p.batch * (keys < kOwnKeys ? keys : kOwnKeys)) / (runs + p.batch));
-  const double streamed = rows <= kMostStreamed ? kJoinTime + keyed_time(true, both, keys, device) : INFINITY;
+  const double streamed = rows <= kMostStreamed ? kStreamedTime + keyed_time(true, both, keys, device) : INFINITY;
   double on_tiles = INFINITY;
   long long blocks = 0, units = 0, splits = 0;
   for (int t = 1; t <= (rows <= kTileRows ? 1 : 2); ++t) {
