@@ -105,24 +105,6 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
-// Whether an element of the vector is at or above the bound, which is one of T's numbers.
-template <typename T>
-__device__ __forceinline__ bool reaches(const uint4& word, float bound) {
-  const uint32_t w[4] = {word.x, word.y, word.z, word.w};
-  uint32_t any = 0;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    if constexpr (std::is_same_v<T, float>) {
-      any |= __uint_as_float(w[c]) >= bound ? 1u : 0u;
-    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-      any |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[c]), __float2bfloat162_rn(bound));
-    } else {
-      any |= __hge2_mask(*reinterpret_cast<const __half2*>(&w[c]), __float2half2_rn(bound));
-    }
-  }
-  return any != 0;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kVec = 16 / sizeof(T), kChunk = kChunkBytes / sizeof(T);
@@ -167,20 +149,25 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
   double sum = 0.0;
   // Adds a chunk to the sum, and what reaches the bound to the list: whether that has become long, for the CTA.
   auto take = [&](int chunk) {
-    float sum0 = 0.f, sum1 = 0.f;
+    float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
     uint32_t reaching = 0;                                    // vectors; few do
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const uint4 word = ring[chunk % kStages][i][threadIdx.x];
       float x[kVec];
-      widen<T>(word, x);
+      words(chunk, i, x);
+      float most = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kVec; c += 2) {
-        sum0 += exp2_ftz((x[c] - shift) * kLog2E);
-        sum1 += exp2_ftz((x[c + 1] - shift) * kLog2E);
+        const float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[c], x[c + 1]), make_float2(-shift, -shift)), make_float2(kLog2E, kLog2E));
+        const float2 e = make_float2(exp2_ftz(t.x), exp2_ftz(t.y));
+        if (c % 4 == 0) sum0 = __fadd2_rn(sum0, e);
+        else sum1 = __fadd2_rn(sum1, e);
+        most = fmaxf(most, fmaxf(x[c], x[c + 1]));
       }
-      reaching |= reaches<T>(word, threshold) ? 1u << i : 0u;
+      reaching |= most >= threshold ? 1u << i : 0u;
     }
+    const float2 both = __fadd2_rn(sum0, sum1);
+    sum += static_cast<double>(both.x) + static_cast<double>(both.y);
     int last = 0;
     if (reaching != 0) {                                      // (behind the loop, so that a warp's threads go through this together)
       static_assert(kVecs * kVec <= 32, "a bit for each of a thread's logits of a chunk");
@@ -202,7 +189,6 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
         if (last < kListed) list[last] = key_of(to_compute(reinterpret_cast<const T*>(&ring[chunk % kStages][i][threadIdx.x])[c]), place_of(chunk, i) + c);
       }
     }
-    sum += static_cast<double>(sum0) + static_cast<double>(sum1);
     return __syncthreads_or(last >= max(2 * p.keep, 32)) != 0;
   };
   // The list's best `keep` in their order, as the list; all threads.
