@@ -7,7 +7,12 @@
 //   keyed.cu then takes each sequence's own keys and joins: any number of (m, l, o) of one row add up after 2^(m - max m).
 //
 // The products are the tensor cores' (tcgen05, f16 operands, f32 sums in tensor memory): a CTA owns one or two tiles of 128 rows and walks its part of
-// the keys 128 at a time.
+// the keys 128 at a time, in steps of 64: of each tile two steps' scores lie in tensor memory, so that one is in its softmax while the products of the
+// other run (128 keys at once over single scores: 256 x 64/8 heads of 128 behind 30000 tokens 479 us, so 343).
+//
+// Bound: no unit is above 40 % (tensor pipe 32, issue slots 38, special functions 33, shared memory 25 % with two tiles): 128 keys take 2.5 us for two
+// tiles and 1.75 for one (heads of 128; of 64 2.3 and 1.55). Without the exponentials they would take 2.2, without the conversion, or 7 in 8 of the first
+// products, 2.35: what is left is the chain of a step (scores, maximum, exponentials, probabilities, product), of which a CTA holds two or four.
 //
 //   warps of a tile (4)   a row a thread: tcgen05.ld of its 128 scores, the keys' scales, ex2, sum; probabilities times the values' scales go
 //                         back into tensor memory as f16 pairs, the A operand of the second product
@@ -743,7 +748,10 @@ tq_status launch_join(const KeyedParams& p, cudaStream_t stream) {
 
 // What becomes of a call, by expected time (us, B200): each sequence reads all its keys (kApart), or the shared ones are taken for all rows of a run
 // together, streamed through warps of 8 or 16 rows as a sequence's are (kStreamed), or on the tensor cores' tiles (kTiles). How many keys are shared is
-// known on the device only: the table's width stands for it.
+// known on the device only: the table's width stands for it. Measured (us, from a graph, cold caches), apart, streamed, on tiles: 16 x 4 sequences of 12
+// heads of 64 behind 1024 tokens 24.6, 30.7, 53.2; 12 x 4 of them behind 2048 30.7, 28.7, 49.2; 64 x 4 of 32/8 heads of 128 behind 2000 172, 96, 186; 16 x 16 of 12
+// heads of 64 behind 4000 189, 62, 125; 16 of 32/8 heads of 128 behind 4000 30.5, -, 34.8; 64 behind 8001 143, -, 57; 32 of 12 heads of 64 behind 4000 38.9, -, 26.7.
+// Tiles of 256 rows halve what is converted, and double what parts cost: 64 x 32/8 behind 8001 57 with 128 rows, 65 with 256; 256 x 64/8 behind 30000 494, 350.
 enum PrefixForm { kApart, kStreamed, kTiles };
 struct PrefixPlan {
   PrefixForm form;
