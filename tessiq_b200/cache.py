@@ -382,7 +382,8 @@ class Beams:
 
     def step(self, parents: torch.Tensor | None = None, count: int = 1) -> Step:
         """Row r goes on from row parents[r] (int32, any shape of `rows` elements, as `ops.beam_select` gives them; None: from itself) and gets room for `count`
-        tokens more. Beyond `tokens` of them the step is not made (`kernel.check_status` raises) and its stores write nothing."""
+        tokens more. parents[r] is one of the rows of r's own sequence: `attention` reads what these have in common once. Beyond `tokens` tokens, or where kept
+        sequences have taken the pages, the step is not made (`kernel.check_status` raises) and its stores write nothing."""
         self._alive()
         if count < 0:
             raise ValueError(f"a step of {count} tokens")
@@ -398,14 +399,16 @@ class Beams:
         return Step(self.table, starts, self._counts[count], self.lengths, count, self.shared, cache.books.changes, {}, self, self.steps)
 
     def keep(self, row: int) -> int:
-        """Row `row` as a sequence of the cache, which `free` leaves. Waits for the device."""
+        """Row `row` as a sequence of the cache, which `free` leaves. Waits for the device. The rows may go on: the sequence's pages are its own then, and
+        not among those set aside for them any more."""
         self._alive()
         self.cache._not_in_a_graph("keep")
         if not 0 <= row < self.rows:
             raise ValueError(f"there is no row {row} among {self.rows}")
         length = int(self.lengths[row])
-        pages = self.table[row, : -(-length // self.cache.books.page_tokens)].tolist()
-        return self.cache.books.adopt(pages, length)
+        pages = self.table[row, : -(-length // self.cache.books.page_tokens)].long()
+        self.references[pages] += 1                                       # (rows that go on neither write into them nor hand them out again)
+        return self.cache.books.adopt(pages.tolist(), length)
 
     def free(self) -> None:
         """Gives back what no kept sequence has."""

@@ -161,6 +161,21 @@ def test_values_that_are_close(tq):
     check(tq, same, torch.zeros_like(scores), 6)      # (beams of one sum: ties, to the lower beam)
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 2**24 - 1, 128), (65535, 1, 3, 2), (511, 128, 2, 128), (2, 128, 1, 128)], ids=str)
+def test_selection_at_its_limits(tq, shape):
+    requests, beams, vocab, keep = shape
+    check(tq, *drawn((requests, beams, vocab), torch.float16, spread=4.0), keep)
+    assert status() == 0
+
+
+def test_beams_that_are_alike(tq):
+    """All values of a request's beams are equal in pairs or more, so that every sum is taken again."""
+    logits, _ = drawn((3, 1, 5000), torch.bfloat16)
+    for scores in (torch.zeros(3, 48, device="cuda"), torch.arange(48, device="cuda").div(7, rounding_mode="floor").float().expand(3, 48).contiguous()):
+        check(tq, logits.expand(3, 48, 5000), scores, 96)
+        check(tq, logits.expand(3, 48, 5000).contiguous(), scores, 96)
+
+
 def test_selection_in_graphs_and_on_streams(tq):
     logits, scores = drawn((8, 4, 30000), torch.bfloat16)
     expected = check(tq, logits, scores, 8)
@@ -354,6 +369,34 @@ def test_one_layer_and_small_pools(tq):
     assert torch.equal(got[2], expected[2]) and got[2] is odd and status() == 0
 
 
+def test_advances_on_two_streams(tq):
+    """Steps of two caches at once, of a CTA and of a cluster each, give what they give one after another."""
+    sides = []
+    for _ in range(2):
+        sides.append([Books(rows, 6, 9 * rows, 16, seed=rows) for rows in (40, 3001, 41, 3002)])
+        for books in sides[-1]:
+            books.step(tq, [5 + i % 60 for i in range(books.rows)], None, True)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for turn in range(5):
+        given = []
+        for n, (apart, alone) in enumerate(zip(*sides)):
+            g = torch.Generator().manual_seed(10 * turn + n)
+            parents = torch.randint(0, apart.rows, (apart.rows,), generator=g).int().cuda()
+            counts = torch.randint(0, 3, (apart.rows,), generator=g).int().cuda()
+            torch.cuda.synchronize()
+            tq.cache_advance(*alone.pools, alone.table, alone.lengths, alone.references, counts, parents, True)
+            given.append((counts, parents))
+        torch.cuda.synchronize()
+        for stream, apart, numbers in zip(streams, sides[0], given):
+            with torch.cuda.stream(stream):
+                tq.cache_advance(*apart.pools, apart.table, apart.lengths, apart.references, *numbers, True)
+        torch.cuda.synchronize()
+        assert status() == 0
+    for apart, alone in zip(*sides):
+        assert all(torch.equal(x, y) for x, y in zip((apart.table, apart.lengths, apart.references), (alone.table, alone.lengths, alone.references)))
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(apart.pools, alone.pools))
+
+
 def test_no_rows_and_no_blocks(tq):
     books = filled(tq)
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
@@ -542,3 +585,39 @@ def test_forks_of_a_prompt_read_it_once(tq):
     assert (got.double() - alone.double()).abs().max() <= 2 * (2.0**-8 * alone.double().abs().max() + 2.0**-11 * 6)
     assert torch.equal(cache.attention(step, 0, q, window=100), tq.cache_attention(q, *cache.layer(0), step.table, step.lengths, 100))
     assert status() == 0
+
+
+def test_a_row_that_is_kept_while_the_others_go_on(tq):
+    """What a kept sequence has stays as it is while the rows write, part and leave pages behind, and while it is extended itself."""
+    from tessiq_b200.cache import PagedCache
+
+    g = torch.Generator().manual_seed(5)
+    cache = PagedCache(1, 2, 32, 60, 16)
+    a = cache.start()
+    step = cache.extend([a], 37)
+    x = torch.randn(1, 2, 37, 32, generator=g).bfloat16().cuda()
+    cache.store(step, 0, x, -x)
+    search = cache.beams([a], 4, 60)
+
+    def go_on(parents):
+        new = torch.randn(4, 2, 1, 32, generator=g).bfloat16().cuda()
+        cache.store(search.step(torch.tensor(parents, dtype=torch.int32, device="cuda")), 0, new * 4, -new)
+
+    for turn in range(9):
+        go_on([0, 0, 1, 3] if turn % 3 == 0 else [0, 1, 2, 3])
+    kept = search.keep(2)
+    row = torch.tensor(cache.books.pages_of(kept), device="cuda")
+    had = decoded(cache, 0, row, 46)
+    for turn in range(20):      # (row 2 goes its own way first, then nobody has it)
+        go_on([0, 1, 2, 3] if turn < 3 else [0, 0, 0, 0])
+        assert torch.equal(decoded(cache, 0, row, 46), had)
+    step = cache.extend([kept], 1)
+    assert torch.equal(decoded(cache, 0, step.table[0], 46), had)
+    rows = [decoded(cache, 0, search.table[r], 66) for r in range(4)]
+    cache.store(step, 0, x[:, :, :1], x[:, :, :1])
+    assert all(torch.equal(decoded(cache, 0, search.table[r], 66), rows[r]) for r in range(4))
+    search.free()
+    assert torch.equal(decoded(cache, 0, step.table[0], 32), had[:, :, :32]) and status() == 0      # (the store may have raised the last page's scale)
+    cache.free(kept)
+    cache.free(a)
+    assert cache.books.free_pages == 60
