@@ -767,7 +767,10 @@ constexpr double kPartBytesPerMicrosecond = 2.2e6;
 constexpr double kOwnTime = 9.0, kJoinTime = 3.0;      // what each sequence has behind the shared keys; the join
 constexpr double kStreamedTime = 6.0;                  // the join, and runs that end later than sequences
 constexpr int kMostStreamed = 16;                      // rows of a run: a warp's
-constexpr long long kOwnKeys = 128;                    // what a sequence is taken to have behind the shared keys
+constexpr long long kOwnKeys = 128;                    // what a sequence is taken to have behind the shared keys, beside streamed ones
+// And behind those on tiles, which says how many warps its CTA has. (24 of 20/4 heads of 128 behind 9000 tokens, with up to 3000 of their own: 63 us by
+// kOwnKeys, so 53; with up to 60 39 both.)
+constexpr long long kTailKeys = 512;
 
 PrefixPlan plan_prefix(KeyedParams p, int runs, long long keys, int32_t device) {
   PrefixPlan plan = {};
@@ -813,7 +816,7 @@ PrefixPlan plan_prefix(KeyedParams p, int runs, long long keys, int32_t device) 
   plan.typical = both.typical;
   if (plan.form == kTiles) {
     both = p;
-    both.typical = plan.typical = static_cast<int>(keys < kOwnKeys ? keys : kOwnKeys);
+    both.typical = plan.typical = static_cast<int>(keys < kTailKeys ? keys : kTailKeys);
   }
   plan.keyed_bytes = keyed_workspace(true, both, keys, device);
   return plan;
