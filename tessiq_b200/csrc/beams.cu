@@ -498,10 +498,23 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
         }
       }
     } else {
-      // (very many equal values, of which only the order of beams and tokens tells)
+      // Very many values that are equal or close. Where they are several beams', whose sums or scores are not the same, these beams' sums are taken again first.
+      if (round == 0) {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+          const Candidate one = candidate(i);
+          if (one.order >= threshold && state[one.beam] == kGoesOn) again[one.beam] = 1;
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < p.beams && again[threadIdx.x]) {
+          for (int beam = 0; beam < static_cast<int>(threadIdx.x); ++beam)
+            if (again[beam] && (logarithm[beam] != logarithm[threadIdx.x] || score_of[beam] != score_of[threadIdx.x])) near = 1;
+        }
+        __syncthreads();
+      }
       Candidate last = {~0ull, 0, 0};
 #pragma unroll 1
-      for (int n = 0; n < p.keep; ++n) {
+      for (int n = 0; n < p.keep && (round > 0 || near == 0); ++n) {
         Candidate best = {0, 0, 0};
 #pragma unroll 1
         for (int i = threadIdx.x; i < all; i += kJoinThreads) {

@@ -176,6 +176,20 @@ def test_beams_that_are_alike(tq):
         check(tq, logits.expand(3, 48, 5000).contiguous(), scores, 96)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+def test_more_equal_values_than_a_list_has(tq, dtype):
+    """Beams that are alike at addresses that are not: thousands of equal values, of which the lowest beam's first tokens are the best."""
+    g = torch.Generator().manual_seed(3)
+    for vocab, beams, keep in ((3001, 64, 64), (50257, 128, 30), (777, 128, 128)):
+        high = torch.rand(vocab, generator=g) < 0.5
+        logits = torch.where(high, 1.1, 0.3).to(dtype).cuda().expand(2, beams, vocab).contiguous()
+        scores = torch.full((2, beams), -1.25, device="cuda")
+        scores[1, 0] = -1.3125                                # (its first beam is worse, the second the best)
+        got = tq.beam_select(logits, scores, keep)
+        assert got[1].tolist() == [[0] * keep, [beams + 1] * keep]
+        assert got[2].tolist() == [high.nonzero()[:keep, 0].tolist()] * 2 and status() == 0
+
+
 def test_selection_in_graphs_and_on_streams(tq):
     logits, scores = drawn((8, 4, 30000), torch.bfloat16)
     expected = check(tq, logits, scores, 8)
