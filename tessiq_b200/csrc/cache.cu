@@ -337,7 +337,7 @@ tq_status copy_pages(const std::vector<tq_paged_tensor>& tensors, const std::vec
 
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kAdvanceThreads = 1024, kAdvanceWarps = kAdvanceThreads / 32, kAdvanceCtas = 8;
+constexpr int kAdvanceThreads = 1024, kAdvanceWarps = kAdvanceThreads / 32, kAdvanceCtas = 16;
 constexpr int kAdvanceSmall = 1 << 14;     // entries and pages that one CTA takes by itself
 constexpr int kAdvanceRows = 4096;         // of a cluster, whose books each CTA has in shared memory
 
@@ -532,18 +532,16 @@ __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __
   }
   meet();
 
-  // The last of the rows that write into a page keeps it where nobody else has it; the others copy it. What each row needs (the first CTA).
-  auto copied = [&](int row) {      // the page that the row copies, or -1
-    const int last = peek(row_last + row);
-    return last >= 0 && (peek(counted + last) > 0 || peek(writer + last) != row) ? last : -1;
-  };
+  // The last of the rows that write into a page keeps it where nobody else has it (-2 - page from here on); the others copy it. What each row needs (the first CTA).
   if (cta == 0) {
     const int run = (p.batch + kAdvanceThreads - 1) / kAdvanceThreads;
     const int first = min(static_cast<int>(threadIdx.x) * run, p.batch), last = min(first + run, p.batch);
     int2 mine = make_int2(0, 0);
 #pragma unroll 1
     for (int row = first; row < last; ++row) {
-      const int start = peek(row_start + row), count = max(p.counts[row], 0), copies = copied(row) >= 0 ? 1 : 0;
+      const int start = peek(row_start + row), count = max(p.counts[row], 0), page = peek(row_last + row);
+      const int copies = page >= 0 && (peek(counted + page) > 0 || peek(writer + page) != row) ? 1 : 0;
+      if (page >= 0 && copies == 0) row_last[row] = -2 - page;
       needs_before[row] = mine.x;      // (within the run so far)
       copies_before[row] = mine.y;
       mine.x += copies + blocks_of(static_cast<long long>(start) + count) - blocks_of(start);
@@ -553,20 +551,14 @@ __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __
     const int2 before = sums_before(mine, warp_totals, total);      // (the CTA meets in there, after which pages that are kept count again)
 #pragma unroll 1
     for (int row = first; row < last; ++row) {
-      const int page = peek(row_last + row);
+      const int page = row_last[row];
       needs_before[row] += before.x;
       copies_before[row] += before.y;
-      if (page >= 0 && copied(row) < 0) row_last[row] = -2 - page;
+      if (page <= -2) atomicExch(counted + (-2 - page), 1);
     }
     if (threadIdx.x == 0) {
       totals[0] = total.x;
       totals[1] = total.y;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int row = first; row < last; ++row) {
-      const int page = row_last[row];
-      if (page <= -2) atomicExch(counted + (-2 - page), 1);
     }
   }
   meet();
@@ -602,13 +594,9 @@ __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __
   if constexpr (!SMALL) {
     if (threadIdx.x == 0) totals[8 + cta] = free_all;
     meet();
-    free_all = 0;
-#pragma unroll 1
-    for (int c = 0; c < ctas; ++c) {
-      const int there = peek(totals + 8 + c);
-      if (c < cta) free_before += there;
-      free_all += there;
-    }
+    const int there = lane < ctas ? peek(totals + 8 + lane) : 0;
+    free_before += __reduce_add_sync(0xffffffffu, lane < cta ? there : 0);
+    free_all = __reduce_add_sync(0xffffffffu, there);
   }
   const int needed = peek(totals), copies = peek(totals + 1), fault_before = peek(totals + 2);
   const bool good = fault_before == 0 && needed <= free_all;
@@ -1065,6 +1053,7 @@ extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int
     config.attrs = attributes;
     config.numAttrs = 2;
     TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes)));
+    TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     TQ_CUDA(cudaLaunchKernelEx(&config, tq::cache_advance_kernel<false>, p, status));
   }
   if (tq_status s = tq::check_launch("cache_advance_kernel")) return s;
