@@ -14,7 +14,7 @@
 // layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 //
 // Advancing. A step of beam search as the books see it, without the host: rows of the table go on from other rows, pages count how many rows have them,
-// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of eight, makes the new table
+// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of sixteen, makes the new table
 // and counts (what its CTAs tell each other goes through memory between cluster barriers); a second kernel copies the pages that it names. Bound: the
 // latency of those barriers and of dependent reads, and the copied pages' bytes.
 #include <cmath>
@@ -396,8 +396,9 @@ __device__ __forceinline__ int2 sums_before(int2 mine, int2* warp_totals, int2& 
   return make_int2(upto.x - mine.x + before.x, upto.y - mine.y + before.y);
 }
 
-// SMALL: one CTA with all books in shared memory; else a cluster with them in scratch (of sixteen: 1024 rows of 138 in a pool of 92000 pages 32 us, of eight 42). Each step is few instructions and few loads after one another: a
-// kernel of a few microseconds waits for both (a warp a row, page counts in memory and their writers counted apart: 4 rows 17 us, 256 rows 35).
+// SMALL: one CTA with all books in shared memory; else a cluster with them in scratch (of sixteen: 1024 rows of 138 in a pool of 92000 pages 32 us, of
+// eight 42). Each step is few instructions and few loads after one another: a kernel of a few microseconds waits for both (a warp a row, page counts in
+// memory and their writers counted apart: 4 rows 17 us, so 10; 256 rows 35).
 template <bool SMALL>
 __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __grid_constant__ AdvanceParams p, const WaitStatus status) {
   extern __shared__ int32_t books[];

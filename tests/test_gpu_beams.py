@@ -383,6 +383,25 @@ def test_one_layer_and_small_pools(tq):
     assert torch.equal(got[2], expected[2]) and got[2] is odd and status() == 0
 
 
+def test_a_cluster_s_advance_in_a_graph(tq):
+    a, b = (Books(3001, 6, 27009, 16, seed=4) for _ in range(2))
+    for books in (a, b):
+        books.step(tq, [5 + i % 60 for i in range(books.rows)], None, True)
+    counts, parents = torch.ones(3001, dtype=torch.int32, device="cuda"), torch.arange(3001, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        starts = tq.cache_advance(*a.pools, a.table, a.lengths, a.references, counts, parents, True)[3]
+    for turn in range(3):
+        parents.copy_(torch.randint(0, 3001, (3001,), generator=torch.Generator().manual_seed(turn)))
+        graph.replay()
+        expected = tq.cache_advance(*b.pools, b.table, b.lengths, b.references, counts, parents, True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip((a.table, a.lengths, a.references, starts), expected))
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a.pools, b.pools))
+    assert status() == 0
+
+
 def test_advances_on_two_streams(tq):
     """Steps of two caches at once, of a CTA and of a cluster each, give what they give one after another."""
     sides = []
