@@ -121,6 +121,9 @@ SHAPES = [  # runs, each, heads, kv_heads, q_tokens, prompt, tail, width, page, 
     (1, 200, 8, 2, 1, 4000, 40, 128, 64, "tiles 128"), (2, 100, 9, 3, 1, 3333, 50, 96, 128, "tiles 128"), (1, 300, 8, 8, 1, 2600, 8, 48, 256, "tiles 128"),
     (1, 256, 8, 4, 1, 6000, 33, 64, 16, "tiles 128"), (1, 100, 64, 8, 1, 3000, 40, 128, 64, "tiles 128"), (1, 150, 16, 4, 2, 1800, 40, 128, 32, "tiles 128"),
     (3, 70, 14, 2, 4, 1300, 11, 112, 16, "tiles 128"), (1, 200, 32, 4, 1, 5000, 30, 64, 1024, "tiles 256"),
+    (1, 200, 32, 4, 1, 4000, 33, 64, 16, "tiles 256"), (1, 128, 64, 8, 1, 6000, 40, 128, 64, "tiles 256"), (1, 160, 16, 4, 4, 2500, 40, 128, 32, "tiles 256"),
+    (3, 110, 14, 2, 4, 1300, 11, 112, 16, "tiles 256"), (2, 400, 16, 8, 1, 1500, 33, 48, 32, "tiles 256"), (1, 256, 64, 8, 1, 2000, 10, 80, 16, "tiles 128"),
+    (1, 3, 4, 2, 130, 700, 150, 64, 16, None), (2, 2, 6, 1, 77, 1000, 90, 128, 32, None), (1, 5, 16, 4, 300, 2100, 310, 128, 64, None),
 ]
 
 
