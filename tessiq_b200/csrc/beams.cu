@@ -18,9 +18,10 @@
 // special-function unit 46 %, warps that wait for the list's pruning), 64 x 4 beams of 50257 in f32 31 us (51 MB), one request of 4 beams 16 us, nearly all of
 // it launches and waits for what came before (the parts 6.4, the join 8).
 //
-// Precision: a thread sums 4 or 8 exponentials of a chunk in f32 at a time, four times, and adds these in f64: a logarithm is off by 1e-7 or so. Sums stand
-// at a logit (the first chunk's largest), so that a lone token's logarithm is exact. Values of neighbours are as close as 1e-7
-// now and then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout.
+// Precision: a thread adds up to 9 exponentials of a chunk in f32 at a time, and these sums in f64. An exponent's rounding grows with the logit's distance
+// from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk has one that is kStand above it;
+// the sum is brought to that one then, and the chunk's taken again. A lone token's logarithm is exact. Values of neighbours are as close as 1e-7 now and
+// then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout.
 #include <cmath>
 #include <type_traits>
 
@@ -40,6 +41,9 @@ constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
 constexpr int kUppers = 6144;                               // candidates of which the joining kernel keeps half the order
 constexpr int kMostBeams = 128, kMostKept = 128;
 constexpr int kSelectCtas = 592;                            // at once on a B200, four an SM
+// How far above what a sum stands at a logit may lie: no farther than most of a vocabulary lies below it. (Each move takes a chunk's sum again: 32 x 16 x
+// 128000 bf16 with tokens that stand out 57.2 us, by 4 58.2, without any moves 56.4.)
+constexpr float kStand = 8.f;
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct SelectParams {
@@ -152,9 +156,9 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
   };
   auto words = [&](int chunk, int i, float (&x)[kVec]) { widen<T>(ring[chunk % kStages][i][threadIdx.x], x); };
   auto key_of = [&](float x, int at) { return static_cast<unsigned long long>(ordered(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(first + at)); };
-  float threshold = -INFINITY, shift = 0.f;
-  double sum = 0.0;
-  // Adds a chunk to the sum, and what reaches the bound to the list: whether that has become long, for the CTA.
+  float threshold = -INFINITY, shift = 0.f, bar = -INFINITY;      // the sum stands at `shift` (at no logit yet: bar is -inf); logits above `bar` move it
+  double sum = 0.0, here = 0.0;                                   // here: of the chunk
+  // Sums a chunk up, and adds what reaches the bound to the list: whether that has become long, or a logit is above the bar, for the CTA.
   auto take = [&](int chunk) {
     float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
     uint32_t reaching = 0;                                    // vectors; few do
@@ -174,8 +178,9 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
       reaching |= most >= threshold ? 1u << i : 0u;
     }
     const float2 both = __fadd2_rn(sum0, sum1);
-    sum += static_cast<double>(both.x) + static_cast<double>(both.y);
+    here = static_cast<double>(both.x) + static_cast<double>(both.y);
     int last = 0;
+    bool above = false;
     if (reaching != 0) {                                      // (behind the loop, so that a warp's threads go through this together)
       static_assert(kVecs * kVec <= 32, "a bit for each of a thread's logits of a chunk");
       uint32_t taken = 0;
@@ -193,10 +198,28 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
 #pragma unroll 1
       for (; taken != 0; taken &= taken - 1, ++last) {
         const int bit = __ffs(taken) - 1, i = bit / kVec, c = bit % kVec;
-        if (last < kListed) list[last] = key_of(to_compute(reinterpret_cast<const T*>(&ring[chunk % kStages][i][threadIdx.x])[c]), place_of(chunk, i) + c);
+        const float x = to_compute(reinterpret_cast<const T*>(&ring[chunk % kStages][i][threadIdx.x])[c]);
+        above |= x > bar;                                     // (above the bar is above all before, and so among the best)
+        if (last < kListed) list[last] = key_of(x, place_of(chunk, i) + c);
       }
     }
-    return __syncthreads_or(last >= max(2 * p.keep, 32)) != 0;
+    return __syncthreads_or(above || last >= max(2 * p.keep, 32)) != 0;
+  };
+  // Brings the sum to a logit above the bar, the best of the list now, and takes the chunk's again.
+  auto stand = [&](int chunk) {
+    const float top = from_ordered(static_cast<uint32_t>(list[0] >> 32));
+    if (!(top > bar)) return;
+    sum *= exp(static_cast<double>(bar == -INFINITY ? bar : shift) - top);      // (no logits before: 0, or NaN)
+    shift = top;
+    bar = top + kStand;
+    here = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < kVecs; ++i) {
+      float x[kVec];
+      words(chunk, i, x);
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) here += static_cast<double>(exp2_ftz((x[c] - shift) * kLog2E));
+    }
   };
   // The list's best `keep` in their order, as the list; all threads.
   auto prune = [&] {
@@ -280,49 +303,35 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
     if (nth > 32) least = 0;
     threshold = least <= 0x007fffffu ? -INFINITY : from_ordered(least);
     most = from_ordered(top);
-    shift = most == -INFINITY ? 0.f : most;
+    if (most > -INFINITY) {
+      shift = most;
+      bar = most + kStand;
+    }
   }
   for (int chunk = 0; chunk < chunks; ++chunk) {
     copy_async_wait<kStages - 1>();
     if (take(chunk)) {
       if (listed > kListed) prune_chunk(chunk);
       else prune();
+      stand(chunk);
     } else if (chunk == 0 && chunks > 1) {
       prune();                                                // (a tighter bound for the others)
     }
+    sum += here;
     ask(chunk + kStages);
   }
   copy_async_wait<0>();
   let_later_start();
-  // A sum that a later chunk has carried far from what it stands at is taken again, from the true maximum.
-  auto whole_sum = [&] {
 #pragma unroll
-    for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    if (lane == 0) warp_sum[warp] = sum;
-    __syncthreads();
+  for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+  if (lane == 0) warp_sum[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
     double all = 0.0;
 #pragma unroll
     for (int w = 0; w < kSelectWarps; ++w) all += warp_sum[w];
-    __syncthreads();
-    return all;
-  };
-  double all = whole_sum();
-  if (chunks > 1 && !(all > 1e-30 && all < 1e30)) {
-    float most = -INFINITY;
-    for (int t = threadIdx.x; t < count; t += kSelectThreads) most = fmaxf(most, to_compute(from[t]));
-    const uint32_t in_warp = __reduce_max_sync(0xffffffffu, ordered(most));
-    if (lane == 0) warp_most[warp] = in_warp;
-    __syncthreads();
-    uint32_t top = 0;
-#pragma unroll
-    for (int w = 0; w < kSelectWarps; ++w) top = max(top, warp_most[w]);
-    most = from_ordered(top);
-    shift = most == -INFINITY ? 0.f : most;
-    sum = 0.0;
-    for (int t = threadIdx.x; t < count; t += kSelectThreads) sum += static_cast<double>(exp2_ftz((to_compute(from[t]) - shift) * kLog2E));
-    all = whole_sum();
+    p.sums[row * p.parts + part] = make_double2(shift, all);
   }
-  if (threadIdx.x == 0) p.sums[row * p.parts + part] = make_double2(shift, all);
   unsigned long long* const to = p.keys + (row * p.parts + part) * p.keep;
   const int found = listed;
   for (int i = threadIdx.x; i < found; i += kSelectThreads) {

@@ -136,6 +136,93 @@ def test_numbers_that_are_none(tq):
     check(tq, logits.bfloat16(), scores, 1)
 
 
+# Parts of several chunks: 160 rows of 60000 are three parts each, of three chunks of two-byte logits or five of f32; 600 rows are one part each.
+
+
+def in_other_orders(row, beams, g, place=None):
+    """[beams, vocab]: `row` in as many orders, its largest where place() says."""
+    rows = torch.stack([row[torch.randperm(len(row), generator=g)] for _ in range(beams)])
+    for beam in range(beams if place else 0):
+        at, to = int(rows[beam].argmax()), place()
+        rows[beam, at], rows[beam, to] = rows[beam, to].clone(), rows[beam, at].clone()
+    return rows
+
+
+def behind_a_first_chunk(g):
+    return lambda: int(torch.randint(0, 3, (1,), generator=g)) * 20000 + int(torch.randint(10000, 20000, (1,), generator=g))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("above", [3, 10, 20, 25, 40, 65])
+def test_a_token_far_above_its_parts_first_chunk(tq, above, dtype):
+    """Two beams of the same logits in two orders, scores 1e-8 to 3e-6 apart, either way: which is better is their scores' alone."""
+    g = torch.Generator().manual_seed(above)
+    rows = torch.randn(80, 60000, generator=g)
+    rows[:, 0] = 4 + above + 4 * torch.rand(80, generator=g)
+    logits = torch.stack([in_other_orders(row, 2, g, behind_a_first_chunk(g)) for row in rows]).to(dtype).cuda()
+    apart = 10.0 ** (torch.rand(80, generator=g) * 2.5 - 8) * torch.where(torch.rand(80, generator=g) < 0.5, -1, 1)
+    check(tq, logits, torch.stack([torch.zeros(80), apart], 1).cuda(), 4)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("allowed", [1, 2, 5, 40])
+def test_few_tokens_allowed_behind_a_first_chunk(tq, allowed, dtype):
+    """Masks that leave few tokens, none of a part's first chunk among them. A lone token's value is its beam's score as it is, so that ties go to the lower beam."""
+    g = torch.Generator().manual_seed(allowed)
+    for level in (-70.0, -1.0, 45.0):
+        logits = torch.full((40, 4, 60000), -math.inf)
+        for r in range(40):
+            place, kept = behind_a_first_chunk(g), level + 15 * torch.rand(allowed, generator=g)
+            for beam in range(4):
+                places = {place() for _ in range(3 * allowed + 9)}
+                logits[r, beam, torch.tensor(sorted(places))[torch.randperm(len(places), generator=g)[:allowed]]] = kept
+        logits = logits.to(dtype).cuda()
+        if allowed == 1:
+            got = check(tq, logits, torch.full((40, 4), -1.25, device="cuda"), 4)
+            assert (got[0] == -1.25).all()
+        scores = -torch.rand(40, 4, generator=g).cuda()
+        check(tq, logits, scores, 3)
+        check(tq, logits, scores, 30)      # (more than are allowed, or some that are not)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_parts_of_several_chunks(tq, dtype):
+    """Rising and falling rows, steps, equal logits and masks, where chunks come one after another."""
+    vocab = 33333
+    rising = torch.linspace(-30, 30, vocab, device="cuda")
+    step = torch.full((vocab,), -300.0, device="cuda")
+    step[vocab // 2 :] = 300.0 + torch.randn(vocab - vocab // 2, generator=torch.Generator().manual_seed(1)).cuda()
+    hidden = torch.randn(vocab, generator=torch.Generator().manual_seed(2)).cuda()
+    hidden[: vocab // 2] = -math.inf
+    huge = torch.randn(vocab, generator=torch.Generator().manual_seed(3)).cuda() * 1e30
+    for row in (rising, rising.flip(0), rising * 20, rising * -20, step, step.flip(0), hidden, hidden.flip(0), huge, torch.full_like(rising, 0.25)):
+        logits = torch.stack([row, torch.randn(vocab, generator=torch.Generator().manual_seed(4)).cuda()]).to(dtype)[None].expand(300, 2, vocab).contiguous()
+        scores = -torch.arange(600, device="cuda").reshape(300, 2) / 64.0
+        got = [t.cpu() for t in tq.beam_select(logits, scores, 9)]
+        values, parents, tokens = [t.cpu() for t in selected(logits[:1], scores[:1], 9)]
+        for r in range(300):      # (a request's scores are the first one's, less 2 r / 64)
+            assert torch.equal(got[1][r] - 2 * r, parents[0].int()) and torch.equal(got[2][r], tokens[0].int())
+            expected = values[0] - 2 * r / 64.0
+            assert ((got[0][r].double() - expected).abs() <= expected.abs() * 2.0**-24 + 1e-6).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_numbers_that_are_none_in_a_later_chunk(tq, dtype):
+    logits, scores = drawn((80, 2, 60000), dtype, 11)
+    place = behind_a_first_chunk(torch.Generator().manual_seed(12))
+    for r in range(0, 80, 2):
+        logits[r, r // 2 % 2, place()] = (math.nan, math.inf)[r // 4 % 2]
+        if r % 3 == 0:
+            logits[r, r // 2 % 2, :9000] = -math.inf
+            logits[r, r // 2 % 2, 20000:29000] = -math.inf
+            logits[r, r // 2 % 2, 40000:49000] = -math.inf
+    check(tq, logits, scores, 7)
+    assert status() == 0
+
+
 def test_finished_beams(tq):
     logits, scores = drawn((4, 4, 5000), torch.bfloat16)
     finished = torch.tensor([[True, False, False, True], [True, True, True, True], [False, False, False, False], [False, True, True, True]], device="cuda")
