@@ -21,7 +21,7 @@
 // Precision: a thread adds up to 9 exponentials of a chunk in f32 at a time, and these sums in f64. An exponent's rounding grows with the logit's distance
 // from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk has one that is kStand above it;
 // the sum is brought to that one then, and the chunk's taken again. A lone token's logarithm is exact. Values of neighbours are as close as 1e-7 now and
-// then, so candidates of two beams within kNear of each other have their beams' sums taken again, in f64 throughout.
+// then, so candidates of two beams that their sums cannot tell apart (near_values: 4e-6) have these taken again, in f64 throughout.
 #include <cmath>
 #include <type_traits>
 
@@ -52,6 +52,7 @@ struct SelectParams {
   const float* scores;                                      // [requests, beams]
   const uint8_t* finished;                                  // the same, or null
   int beams, vocab, keep, parts, chunk, end;
+  double near;                                              // near_values
   double2* sums;                                            // [rows, parts]: the logit the sum stands at, and the sum of exponentials over it
   unsigned long long* keys;                                 // [rows, parts, keep]: candidates of a part, the best first; 0: none
   float* out_scores;                                        // [requests, keep]
@@ -344,9 +345,6 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_parts_kernel(const __g
 
 enum BeamState { kGoesOn = 0, kFinished, kNothing, kNoNumber };      // kNothing: every logit, or the score, is -inf; kNoNumber: NaN, or +inf
 
-// Candidates whose values lie closer than this: the logarithms of two beams' sums may be off by as much.
-constexpr double kNear = 2e-6;
-
 struct Candidate {
   unsigned long long order;      // of the value; 0: none
   uint32_t beam, token;
@@ -467,7 +465,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     __syncthreads();
     unsigned long long threshold = static_cast<unsigned long long>(least) << 32;
     if (round == 0 && least != 0 && least != 0xffffff00u) {
-      const double lower = value_of(threshold) - 2.0 * kNear;
+      const double lower = value_of(threshold) - p.near;
       if (lower == lower) threshold = ordered(lower);      // (of -inf: -inf)
     }
     if (threshold == 0) threshold = 1;
@@ -501,7 +499,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
 #pragma unroll 1
         for (int j = 0; j < found; ++j) {
           const Candidate other = list[j];
-          if (other.beam != one.beam && fabs(value_of(other.order) - value) < kNear &&
+          if (other.beam != one.beam && fabs(value_of(other.order) - value) < p.near &&
               !(logarithm[one.beam] == logarithm[other.beam] && score_of[one.beam] == score_of[other.beam]))
             near = again[one.beam] = again[other.beam] = 1;
         }
@@ -550,20 +548,15 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     }
     __syncthreads();
     if (round > 0 || near == 0) break;
-    // Sums of the beams that are close, in f64.
+    // Sums of the beams that are close, in f64, over the largest logit (alike beams have the same sum then), which the parts know.
     for (int beam = 0; beam < p.beams; ++beam) {
       if (!again[beam] || state[beam] != kGoesOn) continue;
       const T* const from = static_cast<const T*>(p.logits) + request * p.request_stride + beam * p.beam_stride;
-      float most = -INFINITY;
-#pragma unroll 1
-      for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) most = fmaxf(most, to_compute(from[t]));
-      const uint32_t in_warp = __reduce_max_sync(0xffffffffu, ordered(most));
-      if (lane == 0) uppers[warp] = in_warp;      // (they are made again)
-      __syncthreads();
+      const unsigned long long* const best = p.keys + keys0 + static_cast<long long>(beam) * (slots - 1);
       uint32_t top = 0;
 #pragma unroll 1
-      for (int w = 0; w < kJoinWarps; ++w) top = max(top, uppers[w]);
-      const double shift = from_ordered(top);
+      for (int part = lane; part < p.parts; part += 32) top = max(top, static_cast<uint32_t>(best[part * p.keep] >> 32));
+      const double shift = from_ordered(__reduce_max_sync(0xffffffffu, top));
       double sum = 0.0;
 #pragma unroll 1
       for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) sum += exp(static_cast<double>(to_compute(from[t])) - shift);
@@ -586,6 +579,12 @@ struct SelectPlan {
   int parts, chunk;
   size_t sums_bytes, keys_bytes;
 };
+// Candidates of two beams whose values are closer than this may be in either order: both beams' logarithms are off by half of it at most. A logit at a
+// distance d from what the sum stands at has its exponent off by 1.33e-7 d (subtraction and product by 2^-24 each, log2 e by 2^-26), its exponential by 2^-22 and
+// the sums in f32 by 8 * 2^-24, 7.2e-7 together. With their exponentials as weights, distances average at ln N - 1 at most: N logits at d below the largest
+// weigh N e^-d / (1 + N e^-d), which times d is W(N / e) <= ln(N / e) at its largest (W: Lambert's function). Above, none is farther than kStand.
+double near_values(int64_t vocab) { return 2.0 * (1.33e-7 * std::fmax(std::log(static_cast<double>(vocab)) - 1.0, kStand + 0.5) + 7.2e-7); }
+
 // As many parts of a row as there are CTAs at once for it, and one at least. (512 rows of 128000 in one part 49 us, in two 80.)
 SelectPlan plan_select(int64_t rows, int64_t vocab, int64_t keep, int64_t bytes) {
   SelectPlan plan = {};
@@ -654,6 +653,7 @@ extern "C" tq_status tq_beam_select_launch(tq_dtype dtype, const void* logits, c
   p.parts = plan.parts;
   p.chunk = plan.chunk;
   p.end = static_cast<int>(end);
+  p.near = tq::near_values(vocab);
   p.sums = static_cast<double2*>(workspace);
   p.keys = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + plan.sums_bytes);
   p.out_scores = out_scores;

@@ -248,6 +248,25 @@ def test_values_that_are_close(tq):
     check(tq, same, torch.zeros_like(scores), 6)      # (beams of one sum: ties, to the lower beam)
 
 
+def test_roundings_that_add_up(tq):
+    """One token over a background of equal logits, whose exponents are all rounded the same way: two beams of other distances whose values are within 1e-7 or
+    less of each other, either way."""
+    g = torch.Generator().manual_seed(6)
+    top = (8 + 1.5 * torch.rand(300, 2, generator=g)).cuda()
+    low = torch.exp2(-1 - 12 * torch.rand(300, 2, generator=g)).cuda()
+    logits = low[:, :, None].expand(300, 2, 50257).contiguous()
+    logits[:, :, 30000] = top
+    value = -torch.log1p(50256 * torch.exp(low.double() - top.double()))
+    scores = torch.zeros(300, 2, device="cuda")
+    scores[:, 1] = value[:, 0] - value[:, 1] + (torch.rand(300, generator=g).cuda() - 0.5) * 2e-7
+    values = scores.double() + value
+    got = tq.beam_select(logits, scores, 2)
+    best = (values[:, 1] > values[:, 0]).int()
+    rows = torch.arange(300, device="cuda", dtype=torch.int32) * 2
+    assert torch.equal(got[1], torch.stack([rows + best, rows + 1 - best], 1)) and (got[2] == 30000).all()
+    assert ((got[0].double() - values.sort(dim=1, descending=True).values).abs() <= 2.0**-24 + 2e-12 + 1e-6).all() and status() == 0
+
+
 @pytest.mark.parametrize("shape", [(1, 1, 2**24 - 1, 128), (65535, 1, 3, 2), (511, 128, 2, 128), (2, 128, 1, 128)], ids=str)
 def test_selection_at_its_limits(tq, shape):
     requests, beams, vocab, keep = shape
