@@ -494,28 +494,27 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
         if (place >= p.keep) continue;
         write(place, one);
         if (round > 0) continue;
-        // (-inf and NaN are close to nothing; beams of one sum and one score compare as their logits do)
+        // (-inf and NaN are close to nothing. Beams whose sums are equal may yet differ: roundings make one number of several.)
         const double value = value_of(one.order);
 #pragma unroll 1
         for (int j = 0; j < found; ++j) {
           const Candidate other = list[j];
-          if (other.beam != one.beam && fabs(value_of(other.order) - value) < p.near &&
-              !(logarithm[one.beam] == logarithm[other.beam] && score_of[one.beam] == score_of[other.beam]))
+          if (other.beam != one.beam && fabs(value_of(other.order) - value) < p.near && (state[one.beam] == kGoesOn || state[other.beam] == kGoesOn))
             near = again[one.beam] = again[other.beam] = 1;
         }
       }
     } else {
-      // Very many values that are equal or close. Where they are several beams', whose sums or scores are not the same, these beams' sums are taken again first.
+      // Very many values that are equal or close. Where they are several beams', these beams' sums are taken again first.
       if (round == 0) {
 #pragma unroll 1
         for (int i = threadIdx.x; i < all; i += kJoinThreads) {
           const Candidate one = candidate(i);
-          if (one.order >= threshold && state[one.beam] == kGoesOn) again[one.beam] = 1;
+          if (one.order >= threshold && fabs(value_of(one.order)) < static_cast<double>(INFINITY)) again[one.beam] = 1;
         }
         __syncthreads();
-        if (static_cast<int>(threadIdx.x) < p.beams && again[threadIdx.x]) {
-          for (int beam = 0; beam < static_cast<int>(threadIdx.x); ++beam)
-            if (again[beam] && (logarithm[beam] != logarithm[threadIdx.x] || score_of[beam] != score_of[threadIdx.x])) near = 1;
+        if (static_cast<int>(threadIdx.x) < p.beams && again[threadIdx.x] && state[threadIdx.x] == kGoesOn) {
+          for (int beam = 0; beam < p.beams; ++beam)
+            if (again[beam] && beam != static_cast<int>(threadIdx.x)) near = 1;
         }
         __syncthreads();
       }

@@ -267,6 +267,38 @@ def test_roundings_that_add_up(tq):
     assert ((got[0].double() - values.sort(dim=1, descending=True).values).abs() <= 2.0**-24 + 2e-12 + 1e-6).all() and status() == 0
 
 
+def test_beams_whose_sums_round_to_the_same(tq):
+    """Backgrounds that are neighbours in f32, and whose exponents, times log2 e, are the same number: the sums are equal to the last bit and the values are not."""
+    log2_e, low = torch.tensor(math.log2(math.e)), torch.tensor(-1.5)
+    pairs = []
+    while len(pairs) < 40:
+        lower = torch.nextafter(low, torch.tensor(-2.0))
+        if torch.equal(low * log2_e, lower * log2_e):
+            pairs.append((low.item(), lower.item()))
+        low = lower
+    for vocab in (100, 3000, 20000):
+        logits = torch.tensor(pairs, device="cuda")[:, :, None].repeat(1, 1, vocab)
+        logits[:, :, vocab // 3] = 0.0
+        for first, second in ((logits[:, 0], logits[:, 1]), (logits[:, 1], logits[:, 0])):
+            check(tq, torch.stack([first, second], 1), torch.full((40, 2), -2.0, device="cuda"), 3)
+    # more such values than a list has: 1500 zeros of each of 64 beams over one background, and over its neighbour in the last beam, the best
+    high = torch.rand(3001, generator=torch.Generator().manual_seed(3)) < 0.5
+    logits = torch.where(high, 0.0, pairs[0][0]).expand(2, 64, 3001).clone()
+    logits[:, 63] = torch.where(high, 0.0, pairs[0][1])
+    got = tq.beam_select(logits.cuda(), torch.full((2, 64), -1.25, device="cuda"), 64)
+    assert got[1].tolist() == [[63] * 64, [127] * 64] and got[2].tolist() == [high.nonzero()[:64, 0].tolist()] * 2
+    # ... and of a beam beside a finished one, whose score is that beam's value or a little off
+    logits = torch.where(torch.rand(60000, generator=torch.Generator().manual_seed(4)) < 0.5, 0.0, pairs[0][0]).expand(40, 2, 60000).contiguous()
+    total = torch.logsumexp(logits[0, 0].double(), 0)
+    value = total.float().double() - total
+    scores = torch.stack([total.float().expand(40), (value + torch.linspace(-4e-7, 4e-7, 40, dtype=torch.float64)).float()], 1)
+    got = tq.beam_select(logits.cuda(), scores.cuda(), 128, torch.tensor([[False, True]] * 40, device="cuda"), 5)
+    for r in range(40):
+        first = scores[r, 1].double() > value
+        assert got[1][r].tolist() == [2 * r + 1] * first + [2 * r] * (128 - int(first))
+    assert status() == 0
+
+
 @pytest.mark.parametrize("shape", [(1, 1, 2**24 - 1, 128), (65535, 1, 3, 2), (511, 128, 2, 128), (2, 128, 1, 128)], ids=str)
 def test_selection_at_its_limits(tq, shape):
     requests, beams, vocab, keep = shape
