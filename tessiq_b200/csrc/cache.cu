@@ -401,7 +401,7 @@ __device__ __forceinline__ int2 sums_before(int2 mine, int2* warp_totals, int2& 
 // memory and their writers counted apart: 4 rows 17 us, so 10; 256 rows 35).
 template <bool SMALL>
 __global__ void __launch_bounds__(kAdvanceThreads) cache_advance_kernel(const __grid_constant__ AdvanceParams p, const WaitStatus status) {
-  extern __shared__ int32_t books[];
+  extern __shared__ __align__(16) int32_t books[];      // (read four at a time)
   __shared__ int2 warp_totals[kAdvanceWarps];
   __shared__ int stretch_free[kAdvanceWarps], totals_here[kTotals];
   const int ctas = SMALL ? 1 : static_cast<int>(gridDim.x), cta = SMALL ? 0 : static_cast<int>(blockIdx.x);
