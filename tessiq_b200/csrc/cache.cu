@@ -14,10 +14,11 @@
 // layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 //
 // Advancing. A step of beam search as the books see it, without the host: rows of the table go on from other rows, pages count how many rows have them,
-// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of sixteen, makes the new table
+// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of sixteen (eight where there is no room for it), makes the new table
 // and counts (what its CTAs tell each other goes through memory between cluster barriers); a second kernel copies the pages that it names. Bound: the
 // latency of those barriers and of dependent reads, and the copied pages' bytes.
 #include <cmath>
+#include <mutex>
 #include <new>
 #include <type_traits>
 #include <vector>
@@ -733,6 +734,40 @@ AdvanceScratch advance_scratch(int64_t batch, int64_t blocks, int64_t pages) {
   return at;
 }
 
+cudaLaunchConfig_t advance_cluster(int ctas, cudaLaunchAttribute* attribute) {
+  attribute->id = cudaLaunchAttributeClusterDimension;
+  attribute->val.clusterDim.x = static_cast<unsigned>(ctas);
+  attribute->val.clusterDim.y = attribute->val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(ctas));
+  config.blockDim = dim3(kAdvanceThreads);
+  config.dynamicSmemBytes = 3 * kAdvanceRows * sizeof(int32_t);
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  return config;
+}
+
+// CTAs of the cluster: sixteen where `device` has room for them in one (not every part of a GPU has), or the eight that always have. Asked once for each.
+tq_status advance_ctas(int32_t device, int* ctas) {
+  static std::mutex mutex;
+  static int known[64] = {};
+  std::lock_guard<std::mutex> lock(mutex);
+  int asked = 0;
+  int& of = device >= 0 && device < 64 ? known[device] : asked;
+  if (of == 0) {
+    cudaLaunchAttribute attribute;
+    const cudaLaunchConfig_t config = advance_cluster(kAdvanceCtas, &attribute);
+    TQ_CUDA(cudaFuncSetAttribute(cache_advance_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes)));
+    int clusters = 0;
+    const bool fits = cudaFuncSetAttribute(cache_advance_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                      cudaOccupancyMaxActiveClusters(&clusters, cache_advance_kernel<false>, &config) == cudaSuccess && clusters > 0;
+    if (!fits) cudaGetLastError();
+    of = fits ? kAdvanceCtas : 8;
+  }
+  *ctas = of;
+  return TQ_OK;
+}
+
 bool advance_takes(int64_t batch, int64_t blocks, int64_t pages, int64_t page_tokens) {
   const int page_shift = page_shift_of(page_tokens);
   return batch > 0 && blocks >= 0 && pages >= 0 && page_shift >= 0 && pages < (1LL << 30) && batch < (1LL << 20) && blocks < (1LL << 30) >> page_shift &&
@@ -1041,21 +1076,15 @@ extern "C" tq_status tq_cache_advance_launch(const tq_paged_tensor* tensors, int
     TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tq::kAdvanceShared)));
     TQ_CUDA(tq::launch_overlapped(tq::cache_advance_kernel<true>, dim3(1), tq::kAdvanceThreads, at.shared_bytes, cuda_stream, p, status));
   } else {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(tq::kAdvanceCtas);
-    config.blockDim = dim3(tq::kAdvanceThreads);
-    config.dynamicSmemBytes = 3 * tq::kAdvanceRows * sizeof(int32_t);
-    config.stream = cuda_stream;
+    int ctas = 0;
+    if (tq_status s = tq::advance_ctas(device, &ctas)) return s;
     cudaLaunchAttribute attributes[2];
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
-    attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = tq::kAdvanceCtas;
-    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = tq::advance_cluster(ctas, attributes + 1);
+    config.stream = cuda_stream;
     config.attrs = attributes;
     config.numAttrs = 2;
-    TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes)));
-    TQ_CUDA(cudaFuncSetAttribute(tq::cache_advance_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     TQ_CUDA(cudaLaunchKernelEx(&config, tq::cache_advance_kernel<false>, p, status));
   }
   if (tq_status s = tq::check_launch("cache_advance_kernel")) return s;

@@ -16,3 +16,11 @@ def test_dynamic_shared_memory_is_aligned_by_what_declares_it(source):
     text = source.read_text()
     for aligned, element, name in DECLARED.findall(text):
         assert aligned or element == "uint4" or re.search(rf"smem_address\({name}\) \+ \d+u\) & ~\d+u", text), f"{source.name}: {element} {name}[]"
+
+
+@pytest.mark.parametrize("source", SOURCES, ids=lambda path: path.name)
+def test_clusters_that_not_every_gpu_has_room_for_are_asked_about(source):
+    """Clusters over eight are not portable: a part of a GPU, or one whose processing clusters have fewer multiprocessors, runs none of them."""
+    text = source.read_text()
+    if "cudaFuncAttributeNonPortableClusterSizeAllowed" in text:
+        assert "cudaOccupancyMaxActiveClusters" in text
