@@ -219,9 +219,9 @@ class Step:
     counts: torch.Tensor
     lengths: torch.Tensor    # starts + counts
     tokens: int              # the largest count
-    shared: torch.Tensor | None = None      # int32 [runs]: how many first tokens the sequences of each of as many equal runs have in common
     changes: int = 0         # the books' counts as the step was made (Pages.changes, Pages.changes_of each sequence)
     sequences: dict[int, tuple[int, int]] = field(default_factory=dict)
+    shared: torch.Tensor | None = None      # int32 [runs]: how many first tokens the sequences of each of as many equal runs have in common
     search: Beams | None = None      # whose step it is, and its number
     number: int = 0
 
@@ -292,8 +292,8 @@ class PagedCache:
             host = host.pin_memory()
         there = host.to(self.k_scales.device, non_blocking=True)
         table, starts, counts_there, lengths, shared = there.split([batch * blocks, batch, batch, batch, len(shared)])
-        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), shared if each else None, self.books.changes,
-                    {sequence: self.books.changes_of(sequence) for sequence in sequences})
+        return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), self.books.changes,
+                    {sequence: self.books.changes_of(sequence) for sequence in sequences}, shared if each else None)
 
     def _good(self, step: Step, stores: bool) -> None:
         if step.search is not None and (step.search.cache is not self or step.search.steps != step.number):
@@ -396,7 +396,7 @@ class Beams:
         _, _, _, starts = ops.cache_advance(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, self.table, self.lengths, self.references,
                                             self._counts[count], parents, in_place=True)
         self.steps += 1
-        return Step(self.table, starts, self._counts[count], self.lengths, count, self.shared, cache.books.changes, {}, self, self.steps)
+        return Step(self.table, starts, self._counts[count], self.lengths, count, cache.books.changes, {}, self.shared, self, self.steps)
 
     def keep(self, row: int) -> int:
         """Row `row` as a sequence of the cache, which `free` leaves. Waits for the device. The rows may go on: the sequence's pages are its own then, and

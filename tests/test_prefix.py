@@ -169,3 +169,12 @@ def test_runs_of_an_extended_step():
         cache.extend(rows, 0, runs=3)
     with pytest.raises(ValueError, match="equal runs"):
         cache.extend(rows, 0, runs=0)
+
+
+def test_a_step_made_by_position():
+    """Books' counts are its sixth and seventh, as before steps knew of shared tokens."""
+    from tessiq_b200.cache import Step
+
+    numbers = torch.zeros(1, dtype=torch.int32)
+    step = Step(numbers[None], numbers, numbers, numbers, 3, 5, {1: (2, 0)})
+    assert step.changes == 5 and step.sequences == {1: (2, 0)} and step.shared is None and step.search is None
