@@ -355,8 +355,20 @@ class Beams:
         lengths = [books.length(sequence) for sequence in sequences]
         blocks = max(1, *[-(-(length + tokens) // page) for length in lengths])
         self.reserved = books.reserve(sum(beams * (-(-(length + tokens) // page) - length // page) for length in lengths))
-        self.held = [books.fork(sequence) for sequence in sequences]      # (the rows' hold on the sequences' pages)
+        self.held: list[int] = []                                         # (the rows' hold on the sequences' pages)
+        try:
+            self._begin(cache, sequences, beams, blocks, lengths)
+        except BaseException:
+            self._give_back(books)
+            raise
         self.cache, self.beams, self.rows, self.tokens = cache, beams, beams * len(sequences), tokens
+        self.steps = 0
+        cache._searches += 1
+
+    def _begin(self, cache: PagedCache, sequences: list[int], beams: int, blocks: int, lengths: list[int]) -> None:
+        books, page = cache.books, cache.books.page_tokens
+        for sequence in sequences:
+            self.held.append(books.fork(sequence))
         references = [1] * len(books.references)                          # whatever is others' is never free, nor a row's alone
         for reserved in self.reserved:
             references[reserved] = 0
@@ -369,12 +381,16 @@ class Beams:
         shared = [length // page * page for length in lengths]
         host = torch.tensor([*table, *[length for length in lengths for _ in range(beams)], *shared, *references], dtype=torch.int32)
         there = host.to(cache.k_scales.device)
-        sizes = [self.rows * blocks, self.rows, len(sequences), len(references)]
+        rows = beams * len(sequences)
+        sizes = [rows * blocks, rows, len(sequences), len(references)]
         self.table, self.lengths, self.shared, self.references = (part.clone() for part in there.split(sizes))
-        self.table = self.table.reshape(self.rows, blocks)
+        self.table = self.table.reshape(rows, blocks)
         self._counts: dict[int, torch.Tensor] = {}
-        self.steps = 0
-        cache._searches += 1
+
+    def _give_back(self, books: Pages) -> None:
+        for sequence in self.held:
+            books.free(sequence)
+        books.drop(self.reserved)
 
     def _alive(self) -> None:
         if self.cache is None:
@@ -413,8 +429,6 @@ class Beams:
     def free(self) -> None:
         """Gives back what no kept sequence has."""
         self._alive()
-        for sequence in self.held:
-            self.cache.books.free(sequence)
-        self.cache.books.drop(self.reserved)
+        self._give_back(self.cache.books)
         self.cache._searches -= 1
         self.cache = None

@@ -178,3 +178,32 @@ def test_a_step_made_by_position():
     numbers = torch.zeros(1, dtype=torch.int32)
     step = Step(numbers[None], numbers, numbers, numbers, 3, 5, {1: (2, 0)})
     assert step.changes == 5 and step.sequences == {1: (2, 0)} and step.shared is None and step.search is None
+
+
+@pytest.mark.parametrize("fails", ["tensor", "fork"])
+def test_beams_that_cannot_be_made_leave_the_books_as_they_were(monkeypatch, fails):
+    from tessiq_b200.cache import PagedCache
+
+    cache = PagedCache(1, 1, 16, 64, 16, device="cpu")
+    a, b = cache.start(), cache.start()
+    cache.books.extend([a, b], [40, 7])
+    before = (list(cache.books.references), sorted(cache.books._free), cache.books.sequences, cache._searches)
+    real, calls = cache.books.fork, []
+
+    def fork(sequence):
+        calls.append(sequence)
+        if len(calls) == 2:
+            raise MemoryError("no room")
+        return real(sequence)
+
+    def tensor(*_, **__):
+        raise torch.OutOfMemoryError("no room")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(cache.books, "fork", fork) if fails == "fork" else patch.setattr(torch, "tensor", tensor)
+        with pytest.raises((MemoryError, torch.OutOfMemoryError)):
+            cache.beams([a, b], 4, 30)
+    assert (list(cache.books.references), sorted(cache.books._free), cache.books.sequences, cache._searches) == before
+    cache.beams([a, b], 4, 30).free()
+    assert (list(cache.books.references), sorted(cache.books._free), cache.books.sequences, cache._searches) == before
+    cache.compact()
