@@ -222,8 +222,18 @@ class Step:
     changes: int = 0         # the books' counts as the step was made (Pages.changes, Pages.changes_of each sequence)
     sequences: dict[int, tuple[int, int]] = field(default_factory=dict)
     shared: torch.Tensor | None = None      # int32 [runs]: how many first tokens the sequences of each of as many equal runs have in common
+    together: bool = False   # whether these are enough to be worth reading once (see `worth_reading_once`)
     search: Beams | None = None      # whose step it is, and its number
     number: int = 0
+
+
+def worth_reading_once(shared: Sequence[int], longest: int) -> bool:
+    """Whether attention reads what runs of sequences share (tokens, of each run) once for all of a run, or with each sequence: it takes a launch or two more,
+    and how the work is split is decided by the table's width, so that sequences with much of their own behind little that they share are slower. Measured
+    (us, each alone / once, from cold caches, one run of 64 x 32/8 heads of 128, of 32 x 12 of 64, sixteen of 4 x 12 of 64): 512 tokens shared and 2048
+    of their own 57 / 72, 33 / 33, 45 / 51; 2048 and 8192 176 / 182, 76 / 121, 131 / 119; 2048 and 2048 82 / 74, 39 / 47, 62 / 55; 8192 and 2048 176 / 84, 72 /
+    55, 131 / 72."""
+    return bool(shared) and max(shared) >= 128 and 3 * sum(shared) >= longest * len(shared)
 
 
 class PagedCache:
@@ -271,7 +281,7 @@ class PagedCache:
     def extend(self, sequences: Sequence[int], tokens, runs: int | None = None) -> Step:
         """Room for `tokens` (one number, or one for each) tokens more in each of `sequences`; last pages that forks share are copied first. `runs`:
         the sequences are as many equal runs of neighbours that go back to a common beginning (forks of one prompt), whose attention reads
-        what is still common to all of a run once; None: each reads its own."""
+        what is still common to all of a run once, where that is a third of the sequences or more; None: each reads its own."""
         self._not_in_a_graph("extend")
         sequences = list(sequences)
         if runs is not None and (runs < 1 or len(sequences) % runs):
@@ -287,13 +297,14 @@ class PagedCache:
         batch = len(sequences)
         each = len(sequences) // runs if runs else 0
         shared = [self.books.shared_tokens(sequences[r * each : (r + 1) * each]) for r in range(runs or 0)] if each else []
+        together = worth_reading_once(shared, max([s + c for s, c in zip(starts, counts)], default=0))
         host = torch.tensor([*numbers, *starts, *counts, *[s + c for s, c in zip(starts, counts)], *shared], dtype=torch.int32)
         if self.k_scales.is_cuda:
             host = host.pin_memory()
         there = host.to(self.k_scales.device, non_blocking=True)
         table, starts, counts_there, lengths, shared = there.split([batch * blocks, batch, batch, batch, len(shared)])
         return Step(table.reshape(batch, blocks), starts, counts_there, lengths, max(counts, default=0), self.books.changes,
-                    {sequence: self.books.changes_of(sequence) for sequence in sequences}, shared if each else None)
+                    {sequence: self.books.changes_of(sequence) for sequence in sequences}, shared if each else None, together)
 
     def _good(self, step: Step, stores: bool) -> None:
         if step.search is not None and (step.search.cache is not self or step.search.steps != step.number):
@@ -319,7 +330,7 @@ class PagedCache:
     def attention(self, step: Step, layer: int, q: torch.Tensor, window=None, sinks=0, scale=None, token_major=True) -> torch.Tensor:
         """q [batch, heads, q_tokens, width] are the last `q_tokens` tokens of each sequence (a query before its first token gives zeros)."""
         self._good(step, False)
-        if step.shared is not None and window is None:
+        if step.shared is not None and step.together and window is None:
             return ops.prefix_attention(q, *self.layer(layer), step.table, step.lengths, step.shared, scale, token_major)
         return ops.cache_attention(q, *self.layer(layer), step.table, step.lengths, window, sinks, scale, token_major)
 
@@ -385,6 +396,7 @@ class Beams:
         sizes = [rows * blocks, rows, len(sequences), len(references)]
         self.table, self.lengths, self.shared, self.references = (part.clone() for part in there.split(sizes))
         self.table = self.table.reshape(rows, blocks)
+        self.together = worth_reading_once(shared, blocks * page)         # (the rows' own tokens as they may come to be)
         self._counts: dict[int, torch.Tensor] = {}
 
     def _give_back(self, books: Pages) -> None:
@@ -412,7 +424,7 @@ class Beams:
         _, _, _, starts = ops.cache_advance(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, self.table, self.lengths, self.references,
                                             self._counts[count], parents, in_place=True)
         self.steps += 1
-        return Step(self.table, starts, self._counts[count], self.lengths, count, cache.books.changes, {}, self.shared, self, self.steps)
+        return Step(self.table, starts, self._counts[count], self.lengths, count, cache.books.changes, {}, self.shared, self.together, self, self.steps)
 
     def keep(self, row: int) -> int:
         """Row `row` as a sequence of the cache, which `free` leaves. Waits for the device. The rows may go on: the sequence's pages are its own then, and

@@ -207,3 +207,41 @@ def test_beams_that_cannot_be_made_leave_the_books_as_they_were(monkeypatch, fai
     cache.beams([a, b], 4, 30).free()
     assert (list(cache.books.references), sorted(cache.books._free), cache.books.sequences, cache._searches) == before
     cache.compact()
+
+
+def test_which_attention_a_step_takes(monkeypatch):
+    """What runs share is read once where it is a whole tile and a third of the longest sequence; a window, or little in common, leaves each sequence its own."""
+    from tessiq_b200 import cache as module
+    from tessiq_b200.cache import PagedCache
+
+    taken = []
+    monkeypatch.setattr(module.ops, "prefix_attention", lambda *given: taken.append("together"))
+    monkeypatch.setattr(module.ops, "cache_attention", lambda *given: taken.append("each"))
+    monkeypatch.setattr(module.ops, "copy_pages", lambda *given, **how: None)
+    cache = PagedCache(1, 1, 16, 2000, 16, device="cpu")
+
+    def route(prompts, own, **how):
+        sequences = []
+        for prompt in prompts:
+            first = cache.start()
+            cache.books.extend([first], [prompt])
+            sequences += [first, cache.books.fork(first)]
+        step = cache.extend(sequences, own, runs=len(prompts))
+        assert step.shared.tolist() == [prompt // 16 * 16 if own else prompt for prompt in prompts]
+        cache.attention(step, 0, None, **how)
+        for sequence in sequences:
+            cache.books.free(sequence)
+        return taken.pop()
+
+    assert route([300], 1) == "together" and route([300], 1, window=64) == "each"
+    assert route([30], 1) == "each" and route([127], 0) == "each" and route([128], 0) == "together"      # (no whole tile)
+    assert route([320], 600) == "together" and route([320], 700) == "each"
+    assert route([320, 20], 200) == "each" and route([320, 320], 200) == "together"
+    for prompt, tokens, way in ((300, 64, "together"), (100, 64, "each"), (300, 2000, "each")):
+        first = cache.start()
+        cache.books.extend([first], [prompt])
+        search = cache.beams([first], 2, tokens)
+        step = module.Step(search.table, search.lengths, search.lengths, search.lengths, 1, cache.books.changes, {}, search.shared, search.together, search, search.steps)
+        cache.attention(step, 0, None)
+        assert taken.pop() == way
+        search.free(), cache.books.free(first)
