@@ -1212,21 +1212,27 @@ __global__ void __launch_bounds__(kKeyedThreads) keyed_join_kernel(const __grid_
   }
 }
 
-// How many CTAs of a kernel run at once on `device`, asked once for each.
-template <auto kKernel, int WARPS = kKeyedWarps>
+// Warps for which an SM of a B200 has registers: of the kernels below, those of 168 a thread or fewer as compiled leave room for three in each quarter of it, of
+// up to 255 for two.
+constexpr int register_warps(int bits, int w, int nt, int joins) { return w == 64 && (nt == 1 || (bits == 16 && joins == 0)) ? 12 : 8; }
+
+// How many CTAs of a kernel run at once on `device`, asked once for each; without a GPU, on a B200, whose SMs have shared memory of 228 KB and registers for
+// SM_WARPS of its warps.
+template <auto kKernel, int WARPS, int SM_WARPS>
 int resident(int32_t device, size_t smem) {
   static std::mutex mutex;
   static int known[64] = {};
-  if (device < 0 || device >= 64) return 8 / WARPS * 148;
+  const int by_registers = SM_WARPS / WARPS, by_memory = static_cast<int>(228 * 1024 / (smem + 1024)), assumed = by_registers < by_memory ? by_registers : by_memory;
+  if (device < 0 || device >= 64) return assumed * 148;
   std::lock_guard<std::mutex> lock(mutex);
   if (known[device] == 0) {
     int per_sm = 0;
     DeviceScope device_scope(device);
-    if (device_scope.status() != TQ_OK) return 8 / WARPS * 148;      // (a plan without a GPU)
+    if (device_scope.status() != TQ_OK) return assumed * 148;      // (a plan without a GPU)
     if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, 32 * WARPS, smem) != cudaSuccess || per_sm <= 0) {
       cudaGetLastError();
-      per_sm = 8 / WARPS;
+      per_sm = assumed;
     }
     known[device] = per_sm * sm_count(device);
   }
@@ -1275,8 +1281,10 @@ KeyedPlan plan_shape(const KeyedParams& p, long long keys, int32_t device) {
   const int sixteen = plan.nt - 1;
   auto most_of = [&](auto joins, auto warps) {
     constexpr int kJoins = decltype(joins)::value, kWarps = decltype(warps)::value;
-    return plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, kJoins, true, kWarps>, kWarps>(device, keyed_smem(false, W, 1, kWarps))
-                        : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, kJoins, true, kWarps>, kWarps>(device, keyed_smem(false, W, 2, kWarps));
+    return plan.nt == 1 ? resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 1, kJoins, true, kWarps>, kWarps, register_warps(BITS, W, 1, kJoins)>(
+                              device, keyed_smem(false, W, 1, kWarps))
+                        : resident<keyed_attention_kernel<__nv_bfloat16, BITS, W, 2, kJoins, true, kWarps>, kWarps, register_warps(BITS, W, 2, kJoins)>(
+                              device, keyed_smem(false, W, 2, kWarps));
   };
   auto whole_time = [&](auto warps) {
     constexpr int kWarps = decltype(warps)::value;

@@ -415,3 +415,28 @@ def test_the_custom_operation(tq):
     case = Case(*KINDS[2])
     got = torch.ops.tessiq.prefix_attention(case.q, *case.tensors, case.table, case.lengths, case.shared, None)
     assert torch.equal(got, case.run(tq)) and status() == 0
+
+
+def test_a_plan_without_a_gpu_is_that_of_one(tq):
+    """Device -1 stands for a B200: the way a call takes and the scratch it asks for, of paged and of dense keys, by extents drawn at random."""
+    import random
+
+    from tessiq_b200 import _lib
+
+    rng = random.Random(3)
+
+    def plan(device, extents, group, window):
+        batch, heads, kv_heads, q_tokens, width, page, blocks, runs = extents
+        way, size, sizes = [ctypes.c_int32() for _ in range(3)], ctypes.c_size_t(), []
+        _lib.check(_lib.lib.tq_prefix_attention_form(*extents, device, *[ctypes.byref(n) for n in way]))
+        for function, given in ((_lib.lib.tq_prefix_attention_workspace_bytes, extents), (_lib.lib.tq_cache_attention_workspace_bytes, (*extents[:7], window, 0)),
+                                (_lib.lib.tq_window_attention_workspace_bytes, (batch, heads, kv_heads, q_tokens, page * blocks, width, window, 0))):
+            _lib.check(function(*given, device, ctypes.byref(size)))
+            sizes.append(size.value)
+        return [n.value for n in way], sizes
+
+    for _ in range(4000):
+        runs, each, kv_heads, group = rng.choice([1, 1, 2, 3, 8, 16]), rng.choice([1, 2, 4, 7, 16, 64]), rng.choice([1, 2, 8, 12]), rng.choice([1, 2, 4, 8])
+        extents = (runs * each, kv_heads * group, kv_heads, rng.choice([1, 1, 1, 2, 4]), rng.choice([64, 128, 32, 96]), rng.choice([16, 64, 128]), rng.randint(1, 400), runs)
+        window = rng.choice([0, 0, 1000])
+        assert plan(-1, extents, group, window) == plan(0, extents, group, window), extents
