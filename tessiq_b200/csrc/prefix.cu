@@ -759,7 +759,11 @@ struct PrefixPlan {
   int part_rows, part_count, typical;
   long long ctas;
   size_t parts_bytes, stats_bytes, keyed_bytes;
-  size_t bytes() const { return parts_bytes + stats_bytes + keyed_bytes; }
+  size_t apart_bytes;              // (over a pool of no pages each sequence is its own)
+  size_t bytes() const {
+    const size_t together = parts_bytes + stats_bytes + keyed_bytes;
+    return together > apart_bytes ? together : apart_bytes;
+  }
 };
 constexpr double kStartTime = 10.0;                    // a CTA's, to its first scores and behind its last ones
 constexpr double kTileTimes[2][2] = {{1.55, 2.3}, {1.75, 2.5}};     // 128 keys: heads up to 64, 128; one tile of rows, two
@@ -777,7 +781,7 @@ PrefixPlan plan_prefix(KeyedParams p, int runs, long long keys, int32_t device) 
   const long long rows = static_cast<long long>(p.each) * p.group * p.q_tokens, tiles = keys / kKeys, sms = sm_count(device);
   const int wide = p.head_dim > 64;
   const double apart = keyed_time(true, p, keys, device);
-  plan.keyed_bytes = keyed_workspace(true, p, keys, device);
+  plan.apart_bytes = keyed_workspace(true, p, keys, device);
   plan.form = kApart;
   if (p.each == 1 || tiles < 2) return plan;
   // (streamed, runs and sequences are one launch's units, of one tile of rows each)

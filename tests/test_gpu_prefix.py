@@ -440,3 +440,15 @@ def test_a_plan_without_a_gpu_is_that_of_one(tq):
         extents = (runs * each, kv_heads * group, kv_heads, rng.choice([1, 1, 1, 2, 4]), rng.choice([64, 128, 32, 96]), rng.choice([16, 64, 128]), rng.randint(1, 400), runs)
         window = rng.choice([0, 0, 1000])
         assert plan(-1, extents, group, window) == plan(0, extents, group, window), extents
+
+
+@pytest.mark.parametrize("extents", [(7, 8, 2, 4, 32, 128, 1961, 1), (56, 16, 2, 2, 128, 16, 333, 8), (64, 12, 12, 1, 64, 64, 64, 16)], ids=str)
+def test_a_pool_of_no_pages(tq, extents):
+    """Sequences of no tokens: zeros, as from cache_attention."""
+    batch, heads, kv_heads, q_tokens, width, page, blocks, runs = extents
+    codes, scales = torch.empty(0, kv_heads, page, width, dtype=E4M3, device="cuda"), torch.empty(0, kv_heads, device="cuda")
+    table, lengths = torch.zeros(batch, blocks, dtype=torch.int32, device="cuda"), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, heads, q_tokens, width, device="cuda").bfloat16()
+    for shared in (0, 4096):
+        out = tq.prefix_attention(q, codes, codes, scales, scales, table, lengths, torch.full((runs,), shared, dtype=torch.int32, device="cuda"))
+        assert out.shape == q.shape and not out.any() and status() == 0

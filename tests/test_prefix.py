@@ -245,3 +245,13 @@ def test_which_attention_a_step_takes(monkeypatch):
         cache.attention(step, 0, None)
         assert taken.pop() == way
         search.free(), cache.books.free(first)
+
+
+def test_scratch_is_enough_for_a_pool_of_no_pages(lib):
+    """Such a call is cache_attention's, with what it takes: whichever way the extents choose otherwise."""
+    size = [ctypes.c_size_t() for _ in range(2)]
+    for batch, heads, kv_heads, q_tokens, width, page, blocks, runs in ((7, 8, 2, 4, 32, 128, 1961, 1), (2, 2, 2, 64, 96, 1024, 635, 1), (56, 16, 2, 2, 128, 16, 333, 8),
+                                                                       (64, 12, 12, 1, 64, 64, 64, 16), (256, 64, 8, 1, 128, 64, 474, 1)):
+        lib.check(lib.lib.tq_prefix_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page, blocks, runs, -1, ctypes.byref(size[0])))
+        lib.check(lib.lib.tq_cache_attention_workspace_bytes(batch, heads, kv_heads, q_tokens, width, page, blocks, 0, 0, -1, ctypes.byref(size[1])))
+        assert form(lib, batch, heads, kv_heads, q_tokens, width, page, blocks, runs) != "apart" and size[0].value >= size[1].value
