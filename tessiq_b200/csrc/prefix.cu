@@ -699,7 +699,8 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
       }
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        if (stats[u].x == -INFINITY) continue;      // no keys; what lies there is nothing then
+        // no keys: what lies there is nothing then (of keys of which some are none, and others' scores NaN, the sum is)
+        if (stats[u].x == -INFINITY && stats[u].y == stats[u].y) continue;
         const float both = fmaxf(most, stats[u].x), mine = rescale(most, both), theirs = rescale(stats[u].x, both);
         const float x[8] = {near[u].x, near[u].y, near[u].z, near[u].w, far[u].x, far[u].y, far[u].z, far[u].w};
         most = both;

@@ -452,3 +452,18 @@ def test_a_pool_of_no_pages(tq, extents):
     for shared in (0, 4096):
         out = tq.prefix_attention(q, codes, codes, scales, scales, table, lengths, torch.full((runs,), shared, dtype=torch.int32, device="cuda"))
         assert out.shape == q.shape and not out.any() and status() == 0
+
+
+@pytest.mark.parametrize("which", range(len(KINDS)))
+def test_a_scale_that_is_no_number_behind_pages_that_are_not_there(tq, which):
+    """Of the shared keys one page is left, whose keys' scale is NaN in one head: that head's queries see it, whatever is missing before and behind it."""
+    case = Case(*KINDS[which])
+    shared = int(case.shared[0]) // case.page
+    at = max(1, 64 // case.page)
+    left = case.table[:, at].clone()
+    case.table[:, :shared] = -1
+    case.table[:, at] = left
+    case.scales[0][left.long(), 0] = math.nan
+    got, group = case.run(tq), case.heads // case.kv_heads
+    assert status() == 0x50414745
+    assert got[:, :group].isnan().all() and not got[:, group:].isnan().any()
