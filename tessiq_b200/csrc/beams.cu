@@ -556,8 +556,15 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       for (int part = lane; part < p.parts; part += 32) top = max(top, static_cast<uint32_t>(best[part * p.keep] >> 32));
       const double shift = from_ordered(__reduce_max_sync(0xffffffffu, top));
       double sum = 0.0;
+      constexpr int kLoads = 16;                                // of a thread, under way together
 #pragma unroll 1
-      for (int t = threadIdx.x; t < p.vocab; t += kJoinThreads) sum += exp(static_cast<double>(to_compute(from[t])) - shift);
+      for (int t0 = threadIdx.x; t0 < p.vocab; t0 += kLoads * kJoinThreads) {
+        float x[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) x[u] = t0 + u * kJoinThreads < p.vocab ? to_compute(from[t0 + u * kJoinThreads]) : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) sum += exp(static_cast<double>(x[u]) - shift);
+      }
 #pragma unroll
       for (int offset = 16; offset > 0; offset /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
       if (lane == 0) warp_sum[warp] = sum;
