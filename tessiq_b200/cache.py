@@ -166,7 +166,7 @@ class Pages:
         return sources, targets
 
     def reserve(self, count: int) -> list[int]:
-        """`count` pages that belong to no sequence yet; `drop` gives them back."""
+        """`count` pages that belong to no sequence yet; `drop` gives them back, and `compact` has to wait for that."""
         if count > len(self._free):
             raise MemoryError(f"{count} pages are needed and {len(self._free)} are free")
         return [self._take() for _ in range(count)]
@@ -410,8 +410,9 @@ class Beams:
 
     def step(self, parents: torch.Tensor | None = None, count: int = 1) -> Step:
         """Row r goes on from row parents[r] (int32, any shape of `rows` elements, as `ops.beam_select` gives them; None: from itself) and gets room for `count`
-        tokens more. parents[r] is one of the rows of r's own sequence: `attention` reads what these have in common once. Beyond `tokens` tokens, or where kept
-        sequences have taken the pages, the step is not made (`kernel.check_status` raises) and its stores write nothing."""
+        tokens more. parents[r] is one of the rows of r's own sequence: `attention` reads what these have in common once. Beyond `tokens` tokens (and what
+        their last page has room for), or where kept sequences have taken the pages, the step is not made (`kernel.check_status` raises) and its stores
+        write nothing."""
         self._alive()
         if count < 0:
             raise ValueError(f"a step of {count} tokens")

@@ -11,12 +11,14 @@
 // sum of exponentials, and their `keep` largest. In the first chunk every warp's r-th largest thread maximum, r = keep / warps, is a bound below
 // which nothing is needed (warps * r threads have something at or above it); what is at or above the lowest of these goes to a list, a few times
 // `keep` long. Its `keep`-th best is the bound for the chunks behind, of which 32 / n of the n-th reach it. Places in a list are counted by comparing
-// its members with each other. A list that overflows (very many equal logits, a mask of -inf) is answered by `keep` rounds of the CTA's maximum.
+// its members with each other. A list that overflows (very many equal logits, a mask of -inf) is answered by `keep` rounds of the CTA's maximum, a chunk
+// after the other for as long as the bound lets that many logits through: a mask that leaves few tokens is dear, see below.
 // Second kernel: a CTA a request joins the parts: sums, values in f64, a bound by the digits of their order, and places by comparison.
 //
 // Measured (B200, from a graph, cold caches): 32 x 16 beams of 128000 bf16 logits, 32 kept, 61 us (131 MB; the first kernel 48: issue slots 58 % taken, the
 // special-function unit 46 %, warps that wait for the list's pruning), 64 x 4 beams of 50257 in f32 31 us (51 MB), one request of 4 beams 16 us, nearly all of
-// it launches and waits for what came before (the parts 6.4, the join 8).
+// it launches and waits for what came before (the parts 6.4, the join 8). 32 x 16 x 128000 of which all but 16 tokens are hidden: 8 kept 0.47 ms, 32 kept 2.6 ms.
+// A second look (8 of 100 such calls without masks) 40 us for each of its beams; 64 x 4 x 50257 where a request's beams are alike 103 us.
 //
 // Precision: a thread adds up to 9 exponentials of a chunk in f32 at a time, and these sums in f64. An exponent's rounding grows with the logit's distance
 // from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk has one that is kStand above it;

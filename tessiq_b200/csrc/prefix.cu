@@ -14,7 +14,7 @@
 // tiles and 1.75 for one (heads of 128; of 64 2.3 and 1.55). Without the exponentials they would take 2.2, without the conversion, or 7 in 8 of the first
 // products, 2.35: what is left is the chain of a step (scores, maximum, exponentials, probabilities, product), of which a CTA holds two or four.
 //
-//   warps of a tile (4)   a row a thread: tcgen05.ld of its 128 scores, the keys' scales, ex2, sum; probabilities times the values' scales go
+//   warps of a tile (4)   a row a thread: tcgen05.ld of a step's 64 scores, the keys' scales, ex2, sum; probabilities times the values' scales go
 //                         back into tensor memory as f16 pairs, the A operand of the second product
 //   converters (4 warps)  e4m3 codes, as TMA brought them from the pages, to f16 (exact) in the layout of the products' operands
 //   producer (1 warp)     looks pages up, loads their codes (TMA) and scales
@@ -44,7 +44,7 @@ namespace {
 constexpr int kKeys = kPrefixTile;          // of a tile, which is loaded and converted at a time
 constexpr int kStep = kKeys / 2;            // a step
 constexpr int kTileRows = 128;              // rows of an instruction's tile
-constexpr float kSlack = 8.f;               // a row's reference point moves when a tile's maximum is more than 2^kSlack above it
+constexpr float kSlack = 8.f;               // a row's reference point moves when a step's maximum is more than kSlack (in units of log2) above it
 constexpr int kSpan = 12;                   // powers of two of the values' scales that a walk takes
 constexpr int kInfos = 8;                   // tiles whose scales are on chip
 constexpr int kSixteens = kKeys / 16;       // of a tile: the smallest page

@@ -860,7 +860,7 @@ def beam_select(logits, scores, keep, finished=None, end=0):
     order, ties to the lower beam and then the lower token: float32; int32 rows r * beams + b of the batch, as `cache_advance` takes its parents; int32.
     A beam that is `finished` (bool [requests, beams]) has one candidate, the token `end` at its score as it is. A beam at -inf is not there, nor
     is one whose logits are all -inf; NaN or +inf among a beam's logits, or in its score, makes its values NaN, which count as the largest. Candidates are
-    compared by values of 64 bits."""
+    compared by values of 64 bits. Masks of -inf that leave fewer than `keep` tokens of a beam are right, and many times as slow as none."""
     given = (logits, scores, keep, finished, end)
     found = _call(_CODES["beam select"], *given)
     if found is not None:
