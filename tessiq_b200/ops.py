@@ -703,7 +703,9 @@ def prefix_attention(q, k_pages, v_pages, k_scales, v_scales, table, lengths, sh
     one instruction text. `shared` (int32 [runs], on the device) makes the batch as many equal runs of neighbouring sequences, and says of each how
     many first tokens its sequences have in common: the pages that hold these have the same content, mostly the same numbers, in all of its table rows.
     Everything else is as there, without a window. Whole tiles of 128 shared tokens are taken together by all sequences that are at least so
-    long, through the table row of the first of these; the rest of them, and the shared tokens of a shorter sequence, each sequence reads by itself."""
+    long, through the table row of the first of these; the rest of them, and the shared tokens of a shorter sequence, each sequence reads by itself.
+    How the work is split follows from the table's width: where less than a third of the sequences is shared, `cache_attention` is quicker as a rule
+    (`cache.worth_reading_once`)."""
     given = (q, k_pages, v_pages, k_scales, v_scales, table, lengths, shared, scale, token_major)
     out = _call(_CODES["prefix attention"], *given)
     if out is not None:
