@@ -20,7 +20,7 @@
 // it launches and waits for what came before (the parts 6.4, the join 8). 32 x 16 x 128000 of which all but 16 tokens are hidden: 8 kept 0.47 ms, 32 kept 2.6 ms.
 // A second look (8 of 100 such calls without masks) 40 us for each of its beams; 64 x 4 x 50257 where a request's beams are alike 103 us.
 //
-// Precision: a thread adds up to 9 exponentials of a chunk in f32 at a time, and these sums in f64. An exponent's rounding grows with the logit's distance
+// Precision: a thread adds up to 16 exponentials of a chunk in f32 at a time (8 roundings after one another), and these sums in f64. An exponent's rounding grows with the logit's distance
 // from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk has one that is kStand above it;
 // the sum is brought to that one then, and the chunk's taken again. A lone token's logarithm is exact. Values of neighbours are as close as 1e-7 now and
 // then, so candidates of two beams that their sums cannot tell apart (near_values: 4e-6) have these taken again, in f64 throughout.
