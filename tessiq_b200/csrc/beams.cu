@@ -17,13 +17,14 @@
 //
 // Measured (B200, from a graph, cold caches): 32 x 16 beams of 128000 bf16 logits, 32 kept, 61 us (131 MB; the first kernel 48: issue slots 58 % taken, the
 // special-function unit 46 %, warps that wait for the list's pruning), 64 x 4 beams of 50257 in f32 31 us (51 MB), one request of 4 beams 16 us, nearly all of
-// it launches and waits for what came before (the parts 6.4, the join 8). 32 x 16 x 128000 of which all but 16 tokens are hidden: 8 kept 0.47 ms, 32 kept 2.6 ms.
-// A second look (8 of 100 such calls without masks) 40 us for each of its beams; 64 x 4 x 50257 where a request's beams are alike 103 us.
+// it launches and waits for what came before (the parts 6.4, the join 8). 32 x 16 x 128000 of which all but 16 tokens are hidden: 8 kept 0.47 ms, 32 kept
+// 2.6 ms. A second look (8 of 100 such calls without masks) 40 us for each of its beams; 64 x 4 x 50257 where a request's beams are alike 103 us.
 //
-// Precision: a thread adds up to 16 exponentials of a chunk in f32 at a time (8 roundings after one another), and these sums in f64. An exponent's rounding grows with the logit's distance
-// from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk has one that is kStand above it;
-// the sum is brought to that one then, and the chunk's taken again. A lone token's logarithm is exact. Values of neighbours are as close as 1e-7 now and
-// then, so candidates of two beams that their sums cannot tell apart (near_values: 4e-6) have these taken again, in f64 throughout.
+// Precision: a thread adds up to 16 exponentials of a chunk in f32 at a time (8 roundings after one another), and these sums in f64. An exponent's rounding
+// grows with the logit's distance from what the sum stands at, so that is a logit, and not far from the largest: the first chunk's, until a later chunk
+// has one that is kStand above it; the sum is brought to that one then, and the chunk's taken again. A lone token's logarithm is exact. Values of
+// neighbours are as close as 1e-7 now and then, so candidates of two beams that their sums cannot tell apart (near_values: 4e-6) have these taken again,
+// in f64 throughout.
 #include <cmath>
 #include <type_traits>
 

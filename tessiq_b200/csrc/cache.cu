@@ -14,9 +14,9 @@
 // layers are one CTA's: scales with a CTA for each layer, and two launches of 384 pairs, made that 96.
 //
 // Advancing. A step of beam search as the books see it, without the host: rows of the table go on from other rows, pages count how many rows have them,
-// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of sixteen (eight where there is no room for it), makes the new table
-// and counts (what its CTAs tell each other goes through memory between cluster barriers); a second kernel copies the pages that it names. Bound: the
-// latency of those barriers and of dependent reads, and the copied pages' bytes.
+// last pages that several rows would write into are copied, new pages are the lowest free ones. One CTA, or a cluster of sixteen (eight where there is no
+// room for it), makes the new table and counts (what its CTAs tell each other goes through memory between cluster barriers); a second kernel copies the
+// pages that it names. Bound: the latency of those barriers and of dependent reads, and the copied pages' bytes.
 #include <cmath>
 #include <mutex>
 #include <new>
